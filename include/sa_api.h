@@ -39,6 +39,17 @@ extern "C" {
 #define SA_ERR_UNSUPPORTED (-2) /* valid but not implemented (e.g. head_dim != 64) */
 #define SA_ERR_HIP (-3)         /* a HIP runtime call failed (launch, device query) */
 
+/* Element types of the entry points that take one. */
+#define SA_DTYPE_BF16 0
+#define SA_DTYPE_F16 1
+#define SA_DTYPE_F32 2
+
+/* Types of the positions of sa_rotary_table. */
+#define SA_POSITION_I32 0
+#define SA_POSITION_I64 1
+#define SA_POSITION_F32 2
+#define SA_POSITION_F64 3
+
 #define SA_ABI_VERSION 3
 
 /* Version of this ABI (SA_ABI_VERSION). */
@@ -214,6 +225,90 @@ int sa_block_sparse_fwd_f32_terms(const float* q, const int64_t q_strides[3], co
                                   const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, float sm_scale,
                                   const int32_t* work_order, int64_t n_slots, void* workspace,
                                   int64_t workspace_bytes, void* stream);
+
+/*
+ * Training. The reference kernel has no backward pass (its autograd function raises
+ * NotImplementedError, utils/block_sparse_attn_kernel.py:278-281); these three calls are one.
+ *
+ * sa_block_sparse_fwd_lse: sa_block_sparse_fwd (dtype SA_DTYPE_BF16), sa_block_sparse_fwd_f16
+ * (SA_DTYPE_F16) or the fp32 attention (SA_DTYPE_F32), same arguments and output bits, that also
+ * stores each row's log2-sum-exp2 of its scores times log2(e): lse fp32 [B*H][64*ceil(Lq/64)],
+ * +inf for rows without a key (empty lists, keys all biased to -inf) and past Lq.
+ *   parts, workspace  16-bit: as sa_block_sparse_fwd_split (1: none; > 1 plain lists only, work_order
+ *             is not read). fp32: parts = 1, workspace NULL (sa_block_sparse_fwd_f32) or as for
+ *             sa_block_sparse_fwd_f32_terms; key_bias must be NULL.
+ */
+int sa_block_sparse_fwd_lse(int dtype, const void* q, const int64_t q_strides[3], const void* k,
+                            const int64_t k_strides[3], const void* v, const int64_t v_strides[3], void* out,
+                            const int64_t out_strides[3], int B, int H, int Lq, int Lk, int D,
+                            const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, const float* key_bias,
+                            const int64_t bias_strides[2], float sm_scale, const int32_t* work_order,
+                            int64_t n_slots, int parts, void* workspace, int64_t workspace_bytes, float* lse,
+                            void* stream);
+
+/*
+ * Transposed kv lists: for each head the query blocks that list each key block, ascending.
+ *   kv_idx, kv_cnt  lists of BH * nqb rows (counts clamped to [0, max_cnt], entries outside [0, nkb)
+ *             skipped); max_cnt at most 65535.
+ *   q_beg     int32 [BH][nkb + 1]: key block j's entries are q_idx[bh][q_beg[j] .. q_beg[j + 1]).
+ *   q_idx     int32 [BH][nqb * max_cnt]. A key block listed twice by a row has it twice.
+ */
+int sa_kv_list_transpose(const int32_t* kv_idx, const int32_t* kv_cnt, int BH, int nqb, int nkb, int max_cnt,
+                         int32_t* q_beg, int32_t* q_idx, void* stream);
+
+/*
+ * Gradients of sa_block_sparse_fwd_lse: dq, dk, dv for the gradient dout of out, the probabilities
+ * recomputed from lse (P = exp2(score - lse), dS = P * (dout v^T - rowsum(dout * out)), dq =
+ * sm_scale dS k, dk = sm_scale dS^T q, dv = P^T dout). Rows and keys in no list get zeros. Sums are
+ * fp32 in a fixed order: results repeat bit for bit. 16-bit types round P and dS to the type.
+ *   dq, dk, dv  each nullable (not computed); NULL dk and dv need no transposed lists.
+ *   strides   8 triples {b, h, l}: q, k, v, out, dout, dq, dk, dv.
+ *   q_beg, q_idx  the transposed lists.
+ *   q_order, k_order  nullable dispatch orders of the query blocks and the key blocks
+ *             (sa_attn_work_order for B, H and their number).
+ *   workspace sa_block_sparse_bwd_workspace bytes, 256-byte aligned: the query rows' statistics.
+ * Rows of one head of q, k, v and dout span less than 2 GiB. No key_bias with fp32.
+ */
+int sa_block_sparse_bwd_workspace(int B, int H, int Lq, int64_t* bytes);
+int sa_block_sparse_bwd(int dtype, const void* q, const void* k, const void* v, const void* out,
+                        const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                        const int64_t strides[24], int B, int H, int Lq, int Lk, int D, const int32_t* kv_idx,
+                        const int32_t* kv_cnt, int max_cnt, const int32_t* q_beg, const int32_t* q_idx,
+                        const float* key_bias, const int64_t bias_strides[2], float sm_scale,
+                        const int32_t* q_order, int64_t n_q_slots, const int32_t* k_order, int64_t n_k_slots,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions (the host model's part of the attention call: its processors receive q and k that
+ * it has turned, SildingTileAttention.py:100-105 give the token order).
+ *
+ * sa_rotary_table: table [L][pairs][2] fp32 = {cos, sin} * factors[axis] of position * frequency.
+ *   positions device [n_axes][L] of position_type, element strides {axis, token}.
+ *   axis_pairs  host int32 [n_axes] (1 to 4 axes): consecutive pairs that each axis has, at most
+ *             128 in all.  frequencies: host [pairs], radians per position.  factors: host [n_axes].
+ * Angles are formed and reduced in 64 bits.
+ */
+int sa_rotary_table(const void* positions, int position_type, const int64_t strides[2], int64_t L, int n_axes,
+                    const int32_t* axis_pairs, const double* frequencies, const double* factors, float* table,
+                    void* stream);
+
+/*
+ * out = x with each pair (a, b) of a token's first 2 * pairs values turned: (a cos - b sin, b cos +
+ * a sin), computed in fp32 and rounded once; the other values are copied. For q [B,H,L,D] and, unless
+ * NULL, k [B,Hk,L,D] in one launch. out may be x itself; otherwise they must not overlap.
+ *   strides   4 triples {b, h, l} in elements: q, q_out, k, k_out; the D axis is contiguous. D up to
+ *             256; 16-byte aligned rows and multiples of 8 pairs (4 interleaved) take wide accesses.
+ *   table     [n_rows][pairs][2].
+ *   rows      nullable int32 [B or 1][L]: table row of token t of sequence b at rows[b *
+ *             rows_batch_stride + t]; a token whose entry lies outside [0, n_rows) is copied.
+ *             NULL: token t has row t - skip, and the first `skip` tokens are copied.
+ *   halves    0: pair i is values 2 i and 2 i + 1; 1: values i and i + pairs.
+ *   inverse   1: the sines negated, which is the transpose (gradients).
+ */
+int sa_rotary_apply(int dtype, const void* q, void* q_out, const void* k, void* k_out, const int64_t strides[12],
+                    int B, int H, int Hk, int L, int D, const float* table, int n_rows, int pairs,
+                    const int32_t* rows, int64_t rows_batch_stride, int skip, int halves, int inverse,
+                    void* stream);
 
 /*
  * Block-sparse attention with token-level masks inside cut blocks: as sa_block_sparse_fwd

@@ -63,6 +63,23 @@ _PROTOTYPES = {
         [_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, ctypes.c_int64, _P,
          ctypes.c_int64, _P],
     ),
+    "sa_block_sparse_fwd_lse": (
+        _I,
+        [_I, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I64P, _F, _P,
+         ctypes.c_int64, _I, _P, ctypes.c_int64, _P, _P],
+    ),
+    "sa_kv_list_transpose": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
+    "sa_block_sparse_bwd_workspace": (_I, [_I, _I, _I, _I64P]),
+    "sa_block_sparse_bwd": (
+        _I,
+        [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _P, _I64P, _F, _P,
+         ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_int64, _P],
+    ),
+    "sa_rotary_table": (_I, [_P, _I, _I64P, ctypes.c_int64, _I, _P, _P, _P, _P, _P]),
+    "sa_rotary_apply": (
+        _I,
+        [_I, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _P, _I, _I, _P, ctypes.c_int64, _I, _I, _I, _P],
+    ),
     "sa_block_sparse_fwd_tilemask": (
         _I,
         [_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _P, _F, _P,
@@ -199,7 +216,11 @@ def check(rc: int, what: str) -> None:
     raise SAError(msg)
 
 
-_I64_ARRAYS = {n: ctypes.c_int64 * n for n in range(1, 10)}
+# Element types of the entry points that take one (SA_DTYPE_* of include/sa_api.h).
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+_I64_ARRAYS = {n: ctypes.c_int64 * n for n in (*range(1, 10), 12, 24)}
 
 
 def i64(*vals: int):

@@ -1,0 +1,712 @@
+// Gradients of block-sparse attention (the reference's backward raises NotImplementedError,
+// special_attentions/utils/block_sparse_attn_kernel.py:278-281), recomputing the probabilities.
+//
+// With S = q k^T, lse the rows' log2-sum-exp2 that the forward pass stored, do the gradient of out
+// and everything restricted to the listed 64 x 64 blocks:
+//   P     = exp2(S * sm_scale * log2(e) [+ bias * log2(e)] - lse)
+//   delta = rowsum(do * out),  dP = do v^T,  dS = P * (dP - delta)
+//   dq = sm_scale dS k,  dk = sm_scale dS^T q,  dv = P^T do
+// Two passes, each over the lists of one side: one per query block for dq (and delta), one per key
+// block, over the transposed lists (kv_list.hip), for dk and dv. S and dP are computed in both: seven
+// products instead of five, but no score leaves the chip (writing dS would move 16 KB per tile, as
+// long as two tiles' products) and no sum is shared by workgroups, so that results do not depend on
+// the order in which they run.
+//
+// Both passes are one kernel: the "own" side is the block whose gradients a workgroup computes, the
+// "streamed" side the listed blocks. kKeys: own = (k, v), streamed = (q, do), results (dk, dv); else
+// own = (q, do), streamed = (k, v), result dq. A pair of waves shares the streamed rows, 32 at a time
+// (a step), in two LDS stages: rows of step i + 1 are copied while step i computes; one barrier per
+// step. Each wave owns 32 rows of the block. Its operands stay in registers, the own row is the
+// MFMA column, and P and dS come out of the first products in the layout of the second ones' B operand
+// (attn_fwd.hip's P^T):
+//   S^T-like [streamed][own] = st_a own_a^T,  [streamed][own] dP = st_b own_b^T
+//   grad_a^T [d][own] += st_a^T dS,  kKeys: grad_b^T [d][own] += st_b^T P
+// with row reads for the first and transposed reads for the second from the same LDS rows. For dk and
+// dv the streamed rows' -lse / scale and -delta start the accumulators of S and dP, so that an element
+// costs two products, an exp2 and its share of two roundings.
+#include <math.h>
+
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "attn_tile.h"
+#include "sa_common.h"
+
+namespace {
+
+constexpr int kBlk = 64;   // rows per block of either side
+constexpr int kStep = 32;  // streamed rows per step, own rows per wave
+
+struct BwdArgs {
+  const void* own_a;  // k or q
+  const void* own_b;  // v or do
+  const void* st_a;   // q or k
+  const void* st_b;   // do or v
+  const void* out;    // for delta (query pass)
+  void* grad_a;       // dk or dq; may be null
+  void* grad_b;       // dv; may be null
+  int64_t oa_sb, oa_sh, oa_sl;
+  int64_t ob_sb, ob_sh, ob_sl;
+  int64_t sa_sb, sa_sh, sa_sl;
+  int64_t sb_sb, sb_sh, sb_sl;
+  int64_t o_sb, o_sh, o_sl;
+  int64_t ga_sb, ga_sh, ga_sl;
+  int64_t gb_sb, gb_sh, gb_sl;
+  int H, L_own, L_st, n_own, n_st;  // rows and 64-row blocks of the two sides
+  int n_items;                      // B * H * n_own
+  const int32_t* order;             // dispatch slot -> item, -1 = idle; may be null
+  int n_slots;
+  // Query pass: item's entries idx[item * max_cnt ..], cnt[item] of them (clamped). Key pass: entries
+  // idx[bh * n_st * max_cnt + beg[bh * (n_own + 1) + block] ..] up to the next block's.
+  const int32_t* idx;
+  const int32_t* cnt;
+  int max_cnt;
+  const float* bias;  // [b * bias_sb + h * bias_sh + key]
+  int64_t bias_sb, bias_sh;
+  float sm_scale;
+  float scale_log2;     // sm_scale * log2(e)
+  float inv_scale_log2;
+  const float* lse;     // query pass: [bh][64 * query blocks]
+  // [bh][2 * query blocks][2][32]: per 32 query rows their -lse / scale_log2, then their -delta. Written
+  // by the query pass, read by the key pass.
+  float* stats;
+};
+
+// The first eight row operands of a step (16 bytes per lane each): four of each streamed matrix at the
+// lane's addresses a[s], kMat bytes apart.
+template <int kOff, int kMat>
+__device__ __forceinline__ void read_rows(const uint32_t (&a)[4], sa_u32x4v (&x)[4], sa_u32x4v (&y)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %8 offset:%12\n\tds_read_b128 %4, %8 offset:%13\n\t"
+      "ds_read_b128 %1, %9 offset:%12\n\tds_read_b128 %5, %9 offset:%13\n\t"
+      "ds_read_b128 %2, %10 offset:%12\n\tds_read_b128 %6, %10 offset:%13\n\t"
+      "ds_read_b128 %3, %11 offset:%12\n\tds_read_b128 %7, %11 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(kOff), "i"(kOff + kMat)
+      : "memory");
+}
+
+// 32 floats of a step's statistics: elements e of x and y are rows 8 (e / 4) + 4 hh + e % 4 of the
+// first and the second 32 floats (a: the stage's address + 16 hh).
+__device__ __forceinline__ void read_stats(uint32_t a, sa_u32x4v (&x)[4], sa_u32x4v (&y)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:32\n\t"
+      "ds_read_b128 %2, %8 offset:64\n\tds_read_b128 %3, %8 offset:96\n\t"
+      "ds_read_b128 %4, %8 offset:128\n\tds_read_b128 %5, %8 offset:160\n\t"
+      "ds_read_b128 %6, %8 offset:192\n\tds_read_b128 %7, %8 offset:224\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+      : "v"(a)
+      : "memory");
+}
+
+// Transposed operands of 64 columns of a step's 32 rows: r[dc][u] = the A operand of d chunk dc and
+// 16-row step u (two transposed reads each, at a[dc][0] and a[dc][1]).
+template <int kOff>
+__device__ __forceinline__ void read_transposed(const uint32_t (&a)[2][2], sa_u32x2v (&r)[2][2][2]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %6, %10 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0][0][0]), "=&v"(r[0][0][1]), "=&v"(r[1][0][0]), "=&v"(r[1][0][1]), "=&v"(r[0][1][0]),
+        "=&v"(r[0][1][1]), "=&v"(r[1][1][0]), "=&v"(r[1][1][1])
+      : "v"(a[0][0]), "v"(a[0][1]), "v"(a[1][0]), "v"(a[1][1]), "i"(kOff), "i"(kOff + 2048)
+      : "memory");
+}
+
+__device__ inline sa_f32x16 as_f32x16(const sa_u32x4v (&x)[4]) {
+  sa_f32x16 r;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) r[e] = __uint_as_float(x[e >> 2][e & 3]);
+  return r;
+}
+
+// The two 16-bit values of a pair as floats.
+template <typename T>
+__device__ inline float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __bf16>::value)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  const sa_f16x2 h = __builtin_bit_cast(sa_f16x2, w);
+  return make_float2((float)h[0], (float)h[1]);
+}
+
+// Item of a workgroup: the four slots of dispatch group w (placed on XCD w % 8 by the work order) go to
+// the workgroups 32 (w / 8) + 8 i + w % 8, i = 0 .. 3, which the dispatcher places on the same XCD.
+__device__ inline int bwd_item(const BwdArgs& a, int x) {
+  const int slot = 4 * (8 * (x >> 5) + (x & 7)) + ((x >> 3) & 3);
+  if (slot >= a.n_slots) return -1;
+  return a.order ? order_item(a.order, slot) : slot;
+}
+
+// The item's list: entries list[0 .. n).
+template <bool kKeys>
+__device__ inline const __attribute__((address_space(4))) int32_t* bwd_list(const BwdArgs& a, int item, int bh,
+                                                                              int blk, int& n) {
+  const int32_t* p;
+  if (kKeys) {
+    const int32_t* beg = a.cnt + (int64_t)bh * (a.n_own + 1) + blk;
+    p = a.idx + (int64_t)bh * a.n_st * a.max_cnt + beg[0];
+    n = beg[1] - beg[0];
+  } else {
+    p = a.idx + (int64_t)item * a.max_cnt;
+    n = min(max(a.cnt[item], 0), a.max_cnt);
+  }
+  return (const __attribute__((address_space(4))) int32_t*)p;
+}
+
+// kParts: pairs per workgroup, each on its share of the item's list; their sums are added in LDS, in
+// order, at the end.
+template <bool kKeys, bool kBias, typename T, int kD, int kParts>
+__global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
+  typedef Elem<T> E;
+  typedef typename E::v8 v8;
+  constexpr int kDS = kD / 16;      // 16-wide d steps of the first products
+  constexpr int kDC = kD / 32;      // 32-row d chunks of the results
+  constexpr int kHalves = kD / 64;  // 128-byte half rows per row
+  constexpr int kRowTile = kStep * 128;          // one half of a step's rows
+  constexpr int kMat = kHalves * kRowTile;       // a step's rows of one matrix
+  constexpr bool kStats = kKeys || kBias;
+  constexpr int kAcc = kKeys ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) uint8_t tile_lds[kParts * 2 * 2 * kMat];
+  __shared__ __attribute__((aligned(256))) float stat_lds[kParts * 2 * 64];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = wave >> 1, w = wave & 1;
+  const int col = lane & 31, hh = lane >> 5;
+  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x));
+  if (item < 0 || item >= a.n_items) return;  // (the whole workgroup)
+  const int bh = item / a.n_own;
+  const int blk = item - bh * a.n_own;
+  const int b = bh / a.H;
+  const int h = bh - b * a.H;
+  int cnt;
+  const auto list = bwd_list<kKeys>(a, item, bh, blk, cnt);
+
+  const uint16_t* oa = static_cast<const uint16_t*>(a.own_a) + b * a.oa_sb + h * a.oa_sh;
+  const uint16_t* ob = static_cast<const uint16_t*>(a.own_b) + b * a.ob_sb + h * a.ob_sh;
+  const int own_row = blk * kBlk + kStep * w + col;
+  const int own_clamped = min(own_row, a.L_own - 1);  // rows past L_own are never stored
+  v8 fa[kDS], fb[kDS];
+#pragma unroll
+  for (int s = 0; s < kDS; ++s) {
+    fa[s] = __builtin_bit_cast(v8, *reinterpret_cast<const uint4*>(oa + (int64_t)own_clamped * a.oa_sl + 16 * s + 8 * hh));
+    fb[s] = __builtin_bit_cast(v8, *reinterpret_cast<const uint4*>(ob + (int64_t)own_clamped * a.ob_sl + 16 * s + 8 * hh));
+  }
+
+  float lse = 0.f, delta = 0.f;
+  if constexpr (!kKeys) {
+    const uint16_t* op = static_cast<const uint16_t*>(a.out) + b * a.o_sb + h * a.o_sh + (int64_t)own_clamped * a.o_sl;
+#pragma unroll
+    for (int s = 0; s < kDS; ++s) {
+      const sa_u32x4v x = __builtin_bit_cast(sa_u32x4v, *reinterpret_cast<const uint4*>(op + 16 * s + 8 * hh));
+      const sa_u32x4v y = __builtin_bit_cast(sa_u32x4v, fb[s]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 o = unpack2<T>(x[i]), d = unpack2<T>(y[i]);
+        delta = fmaf(o.x, d.x, fmaf(o.y, d.y, delta));
+      }
+    }
+    delta = xhalf_sum(delta);
+    lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col];
+    if (part == 0) {
+      const bool row_ok = own_row < a.L_own;
+      const float v = hh == 0 ? -lse * a.inv_scale_log2 : -delta;
+      a.stats[(((int64_t)bh * a.n_own + blk) * 2 + w) * 64 + lane] = row_ok ? v : hh == 0 ? -INFINITY : 0.f;
+    }
+    if (!a.grad_a) return;  // only the statistics are wanted
+  }
+  float own_bias = 0.f;
+  const float* bias = kBias ? a.bias + b * a.bias_sb + h * a.bias_sh : nullptr;
+  if (kKeys && kBias) own_bias = bias[own_clamped] * kLog2e;
+
+  // Streamed rows: wave 0 of the pair copies st_a's (and the statistics or biases), wave 1 st_b's.
+  const uint16_t* st = w == 0 ? static_cast<const uint16_t*>(a.st_a) + b * a.sa_sb + h * a.sa_sh
+                              : static_cast<const uint16_t*>(a.st_b) + b * a.sb_sb + h * a.sb_sh;
+  const uint32_t row_bytes = (uint32_t)(w == 0 ? a.sa_sl : a.sb_sl) * 2;
+  const uint32_t st_bytes = (uint32_t)(a.L_st - 1) * row_bytes + 128;
+  uint32_t goff[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+    goff[p] = (lane >> 3) * row_bytes + 16 * ((lane & 7) ^ swz(8 * p + (lane >> 3)));
+  const float* stat_src = kKeys ? a.stats + (int64_t)bh * a.n_st * 128 : bias;
+  const uint32_t stat_bytes = kKeys ? (uint32_t)a.n_st * 512 : (uint32_t)a.L_st * 4;
+  lds_u8* tile = (lds_u8*)tile_lds + part * 4 * kMat;
+  lds_u8* stat = (lds_u8*)stat_lds + part * 512;
+
+  const int n_steps = 2 * cnt;
+  const int per_part = (n_steps + kParts - 1) / kParts;
+  const int beg = part * per_part;
+  auto block_of = [&](int i) -> int {  // the streamed block of the part's i-th step, -1: none
+    const int s = beg + i;
+    return i < per_part && s < n_steps ? list[s >> 1] : -1;
+  };
+  auto issue = [&](int rb, int i) {
+    if ((unsigned)rb >= (unsigned)a.n_st) return;
+    const uint32_t row0 = __builtin_amdgcn_readfirstlane(rb * kBlk + kStep * ((beg + i) & 1));
+    lds_u8* dst = tile + (i & 1) * 2 * kMat + w * kMat;
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf) {
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(st + 64 * hf),
+                                                                            (short)0, (int)st_bytes, 0x00020000);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_u8*)(dst + hf * kRowTile + 1024 * j), 16,
+                                                 (row0 + 8 * j) * row_bytes + goff[j & 1], 0, 0, 0);
+    }
+    if (kStats && w == 0) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(stat_src), (short)0,
+                                                                          (int)stat_bytes, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u8*)(stat + (i & 1) * 256), 4,
+                                               (kKeys ? row0 * 8 : row0 * 4) + 4 * lane, 0, 0, 0);
+    }
+  };
+
+  // Lane constants: row operand reads of chunk s and transposed reads (attn_fwd.hip's kro and vro).
+  const uint32_t tile_at = (uint32_t)(uintptr_t)tile, stat_at = (uint32_t)(uintptr_t)stat + 16 * hh;
+  uint32_t ro[4], to[2][2];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) ro[s] = tile_at + 128 * col + 16 * ((2 * s + hh) ^ swz(col));
+  {
+    const int i = lane & 15, hq = lane >> 5, dg = (lane >> 4) & 1;
+#pragma unroll
+    for (int dc = 0; dc < 2; ++dc)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = 8 * t + 4 * hq + (i >> 2);
+        const int chunk = 4 * dc + 2 * dg + ((i & 3) >> 1);
+        to[dc][t] = tile_at + 128 * r + 16 * (chunk ^ swz(r)) + 8 * (i & 1);
+      }
+  }
+
+  sa_f32x16 acc[kAcc][kDC];
+#pragma unroll
+  for (int x = 0; x < kAcc; ++x)
+#pragma unroll
+    for (int dc = 0; dc < kDC; ++dc) acc[x][dc] = sa_f32x16{};
+
+  int rb = block_of(0);
+  issue(rb, 0);
+  int rb_next = block_of(1);
+  for (int i = 0; i < per_part; ++i) {
+    // This wave's copies of step i have landed, then everyone's; every wave is done with step i - 1,
+    // whose stage the copies of step i + 1 overwrite.
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    wg_barrier();
+    issue(rb_next, i + 1);
+    const int cur = rb;
+    rb = rb_next;
+    rb_next = block_of(i + 2);
+    if ((unsigned)cur >= (unsigned)a.n_st) continue;
+    const uint32_t stage = (i & 1) * 2 * kMat;
+    sa_f32x16 S = {}, dP = {};
+    if constexpr (kStats) {
+      sa_u32x4v x[4], y[4];
+      read_stats(stat_at + (i & 1) * 256, x, y);
+      S = as_f32x16(x);
+      if constexpr (kKeys) dP = as_f32x16(y);
+    }
+    sa_f32x16 kb2 = {};
+    if constexpr (!kKeys && kBias) {
+      kb2 = S;
+      S = sa_f32x16{};
+    }
+#pragma unroll
+    for (int hf = 0; hf < kHalves; ++hf) {
+      sa_u32x4v x[4], y[4];
+      const uint32_t at[4] = {ro[0] + stage, ro[1] + stage, ro[2] + stage, ro[3] + stage};
+      if (hf == 0) read_rows<0, kMat>(at, x, y);
+      else read_rows<kRowTile, kMat>(at, x, y);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        S = E::mfma(E::as8(x[s]), fa[4 * hf + s], S);
+        dP = E::mfma(E::as8(y[s]), fb[4 * hf + s], dP);
+      }
+    }
+    // Elements e: streamed row 8 (e / 4) + 4 hh + e % 4 of the step, own row col.
+    uint32_t Pp[8], Sp[8];
+    if constexpr (kKeys) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = fast_exp2(kBias ? fmaf(S[e], a.scale_log2, own_bias) : S[e] * a.scale_log2);
+        const float p1 = fast_exp2(kBias ? fmaf(S[e + 1], a.scale_log2, own_bias) : S[e + 1] * a.scale_log2);
+        Pp[e >> 1] = E::pack(p0, p1);
+        Sp[e >> 1] = E::pack(p0 * dP[e], p1 * dP[e + 1]);
+      }
+    } else {
+      const int row0 = cur * kBlk + kStep * ((beg + i) & 1);
+      float p[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        p[e] = fast_exp2(fmaf(S[e], a.scale_log2, kBias ? fmaf(kb2[e], kLog2e, -lse) : -lse));
+      if (row0 + kStep > a.L_st) {  // keys past the last one
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (row0 + 8 * (e >> 2) + 4 * hh + (e & 3) >= a.L_st) p[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) Sp[e >> 1] = E::pack(p[e] * (dP[e] - delta), p[e + 1] * (dP[e + 1] - delta));
+    }
+#pragma unroll
+    for (int x = kAcc - 1; x >= 0; --x)  // st_b^T P first: P is ready first
+#pragma unroll
+      for (int hf = 0; hf < kHalves; ++hf) {
+        const uint32_t at[2][2] = {{to[0][0] + stage, to[0][1] + stage}, {to[1][0] + stage, to[1][1] + stage}};
+        sa_u32x2v r[2][2][2];
+        if (x == 0) {
+          if (hf == 0) read_transposed<0>(at, r);
+          else read_transposed<kRowTile>(at, r);
+        } else {
+          if (hf == 0) read_transposed<kMat>(at, r);
+          else read_transposed<kMat + kRowTile>(at, r);
+        }
+        const uint32_t(&P)[8] = x == 0 ? Sp : Pp;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int dc = 0; dc < 2; ++dc)
+            acc[x][2 * hf + dc] = E::mfma(
+                E::as8(sa_u32x4v{r[dc][u][0].x, r[dc][u][0].y, r[dc][u][1].x, r[dc][u][1].y}),
+                E::as8(sa_u32x4v{P[4 * u], P[4 * u + 1], P[4 * u + 2], P[4 * u + 3]}), acc[x][2 * hf + dc]);
+      }
+  }
+
+  // ---- Results: element 4 q4 + j of acc[x][dc] is d = 32 dc + 8 q4 + 4 hh + j of own row col.
+#pragma unroll
+  for (int x = 0; x < kAcc; ++x) {
+    uint16_t* g = static_cast<uint16_t*>(x == 0 ? a.grad_a : a.grad_b);
+    const int64_t sb = x == 0 ? a.ga_sb : a.gb_sb, sh = x == 0 ? a.ga_sh : a.gb_sh, sl = x == 0 ? a.ga_sl : a.gb_sl;
+    const float f = x == 0 ? a.sm_scale : 1.f;
+    if constexpr (kParts == 1) {
+      if (g && own_row < a.L_own) {
+        uint16_t* p = g + b * sb + h * sh + (int64_t)own_row * sl + 4 * hh;
+#pragma unroll
+        for (int dc = 0; dc < kDC; ++dc)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const sa_f32x16& A = acc[x][dc];
+            *reinterpret_cast<uint2*>(p + 32 * dc + 8 * q4) =
+                make_uint2(E::pack(A[4 * q4] * f, A[4 * q4 + 1] * f), E::pack(A[4 * q4 + 2] * f, A[4 * q4 + 3] * f));
+          }
+      }
+    } else {
+      constexpr int kCh = kD / 4;  // 16-byte chunks of a row of sums
+      float* sums = reinterpret_cast<float*>(tile_lds);  // [part][64 rows][kD], chunks swizzled by the row
+      __syncthreads();  // every wave is done with the stages (x = 0) or with the last sums
+      float* mine = sums + (part * kBlk + kStep * w + col) * kD;
+#pragma unroll
+      for (int dc = 0; dc < kDC; ++dc)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const sa_f32x16& A = acc[x][dc];
+          *reinterpret_cast<float4*>(mine + 4 * ((8 * dc + 2 * q4 + hh) ^ (col & (kCh - 1)))) =
+              make_float4(A[4 * q4], A[4 * q4 + 1], A[4 * q4 + 2], A[4 * q4 + 3]);
+        }
+      __syncthreads();
+      for (int t = threadIdx.x; t < kBlk * kCh; t += 128 * kParts) {
+        const int r = t / kCh, ch = t % kCh;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+          const float4 y = *reinterpret_cast<const float4*>(sums + (p * kBlk + r) * kD + 4 * (ch ^ (r & 31 & (kCh - 1))));
+          s.x += y.x;
+          s.y += y.y;
+          s.z += y.z;
+          s.w += y.w;
+        }
+        if (g && blk * kBlk + r < a.L_own)
+          *reinterpret_cast<uint2*>(g + b * sb + h * sh + (int64_t)(blk * kBlk + r) * sl + 4 * ch) =
+              make_uint2(E::pack(s.x * f, s.y * f), E::pack(s.z * f, s.w * f));
+      }
+    }
+  }
+}
+
+// ---- fp32: the same passes on v_mfma_f32_32x32x2_f32, operands straight from memory (the caches hold
+// a step's rows: its 32 x 32 x kD products take 16 times as long as in 16 bits).
+
+__device__ inline sa_f32x16 mfma32x2(float x, float y, sa_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x2f32(x, y, c, 0, 0, 0);
+}
+
+// A workgroup computes 32 own rows (half `blockIdx.x & 1` of an item): its four waves take a share of
+// the steps each and add their sums in LDS, in order. The contraction over d gives k slot hh of step s
+// the value d = hh * kD / 2 + s, so that a lane reads half a row; that over the streamed rows takes row
+// 8 (e / 4) + 4 hh + e % 4 at step e, where P and dS lie.
+template <bool kKeys, int kD>
+__global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdArgs a) {
+  constexpr int kHD = kD / 2;
+  constexpr int kDC = kD / 32;
+  constexpr int kAcc = kKeys ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float sums[4 * kStep * kD];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, hh = lane >> 5;
+  const int half = blockIdx.x & 1;
+  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x >> 1));
+  if (item < 0 || item >= a.n_items) return;  // (the whole workgroup)
+  const int bh = item / a.n_own;
+  const int blk = item - bh * a.n_own;
+  const int b = bh / a.H;
+  const int h = bh - b * a.H;
+  int cnt;
+  const auto list = bwd_list<kKeys>(a, item, bh, blk, cnt);
+  const int own_row = blk * kBlk + kStep * half + col;
+  const int own_clamped = min(own_row, a.L_own - 1);  // rows past L_own are never stored
+  const float* oa = static_cast<const float*>(a.own_a) + b * a.oa_sb + h * a.oa_sh + (int64_t)own_clamped * a.oa_sl;
+  const float* ob = static_cast<const float*>(a.own_b) + b * a.ob_sb + h * a.ob_sh + (int64_t)own_clamped * a.ob_sl;
+  float fa[kHD], fb[kHD];
+#pragma unroll
+  for (int s = 0; s < kHD; s += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(oa + hh * kHD + s);
+    const float4 y = *reinterpret_cast<const float4*>(ob + hh * kHD + s);
+    fa[s] = x.x; fa[s + 1] = x.y; fa[s + 2] = x.z; fa[s + 3] = x.w;
+    fb[s] = y.x; fb[s + 1] = y.y; fb[s + 2] = y.z; fb[s + 3] = y.w;
+  }
+  float lse = 0.f, delta = 0.f;
+  if constexpr (!kKeys) {
+    const float* op = static_cast<const float*>(a.out) + b * a.o_sb + h * a.o_sh + (int64_t)own_clamped * a.o_sl;
+#pragma unroll
+    for (int s = 0; s < kHD; s += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(op + hh * kHD + s);
+      delta = fmaf(x.x, fb[s], fmaf(x.y, fb[s + 1], fmaf(x.z, fb[s + 2], fmaf(x.w, fb[s + 3], delta))));
+    }
+    delta = xhalf_sum(delta);
+    lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * half + col];
+    if (wave == 0) {
+      const bool row_ok = own_row < a.L_own;
+      // (the key pass takes lse as it is here: its element costs a fused multiply-add either way)
+      const float v = hh == 0 ? -lse : -delta;
+      a.stats[(((int64_t)bh * a.n_own + blk) * 2 + half) * 64 + lane] = row_ok ? v : hh == 0 ? -INFINITY : 0.f;
+    }
+    if (!a.grad_a) return;
+  }
+  const float* sa = static_cast<const float*>(a.st_a) + b * a.sa_sb + h * a.sa_sh;
+  const float* sb = static_cast<const float*>(a.st_b) + b * a.sb_sb + h * a.sb_sh;
+
+  sa_f32x16 acc[kAcc][kDC];
+#pragma unroll
+  for (int x = 0; x < kAcc; ++x)
+#pragma unroll
+    for (int dc = 0; dc < kDC; ++dc) acc[x][dc] = sa_f32x16{};
+  for (int i = wave; i < 2 * cnt; i += 4) {
+    const int rb = list[i >> 1];
+    if ((unsigned)rb >= (unsigned)a.n_st) continue;
+    const int row0 = rb * kBlk + kStep * (i & 1);
+    if (row0 >= a.L_st) continue;
+    const int64_t row = min(row0 + col, a.L_st - 1);  // clamped rows get P = 0
+    sa_f32x16 S = {}, dP = {};
+    float nl[16];
+    if constexpr (kKeys) {
+      const float* sp = a.stats + (((int64_t)bh * a.n_st + rb) * 2 + (i & 1)) * 64 + 4 * hh;
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 x = *reinterpret_cast<const float4*>(sp + 8 * q4);
+        const float4 y = *reinterpret_cast<const float4*>(sp + 32 + 8 * q4);
+        nl[4 * q4] = x.x; nl[4 * q4 + 1] = x.y; nl[4 * q4 + 2] = x.z; nl[4 * q4 + 3] = x.w;
+        dP[4 * q4] = y.x; dP[4 * q4 + 1] = y.y; dP[4 * q4 + 2] = y.z; dP[4 * q4 + 3] = y.w;
+      }
+    }
+    {
+      const float* pa = sa + row * a.sa_sl + hh * kHD;
+      const float* pb = sb + row * a.sb_sl + hh * kHD;
+#pragma unroll
+      for (int s = 0; s < kHD; s += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(pa + s);
+        const float4 y = *reinterpret_cast<const float4*>(pb + s);
+        S = mfma32x2(x.x, fa[s], S);
+        dP = mfma32x2(y.x, fb[s], dP);
+        S = mfma32x2(x.y, fa[s + 1], S);
+        dP = mfma32x2(y.y, fb[s + 1], dP);
+        S = mfma32x2(x.z, fa[s + 2], S);
+        dP = mfma32x2(y.z, fb[s + 2], dP);
+        S = mfma32x2(x.w, fa[s + 3], S);
+        dP = mfma32x2(y.w, fb[s + 3], dP);
+      }
+    }
+    float p[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const bool ok = row0 + 8 * (e >> 2) + 4 * hh + (e & 3) < a.L_st;
+      p[e] = ok ? exp2f(fmaf(S[e], a.scale_log2, kKeys ? nl[e] : -lse)) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int64_t r = min(row0 + 8 * (e >> 2) + 4 * hh + (e & 3), a.L_st - 1);
+      const float ds = kKeys ? p[e] * dP[e] : p[e] * (dP[e] - delta);
+#pragma unroll
+      for (int dc = 0; dc < kDC; ++dc) {
+        acc[0][dc] = mfma32x2(sa[r * a.sa_sl + 32 * dc + col], ds, acc[0][dc]);
+        if constexpr (kKeys) acc[kAcc - 1][dc] = mfma32x2(sb[r * a.sb_sl + 32 * dc + col], p[e], acc[kAcc - 1][dc]);
+      }
+    }
+  }
+  constexpr int kCh = kD / 4;
+#pragma unroll
+  for (int x = 0; x < kAcc; ++x) {
+    float* g = static_cast<float*>(x == 0 ? a.grad_a : a.grad_b);
+    const int64_t gsb = x == 0 ? a.ga_sb : a.gb_sb, gsh = x == 0 ? a.ga_sh : a.gb_sh, gsl = x == 0 ? a.ga_sl : a.gb_sl;
+    const float f = x == 0 ? a.sm_scale : 1.f;
+    __syncthreads();
+    float* mine = sums + (wave * kStep + col) * kD;
+#pragma unroll
+    for (int dc = 0; dc < kDC; ++dc)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const sa_f32x16& A = acc[x][dc];
+        *reinterpret_cast<float4*>(mine + 4 * ((8 * dc + 2 * q4 + hh) ^ (col & (kCh - 1)))) =
+            make_float4(A[4 * q4], A[4 * q4 + 1], A[4 * q4 + 2], A[4 * q4 + 3]);
+      }
+    __syncthreads();
+    for (int t = threadIdx.x; t < kStep * kCh; t += 256) {
+      const int r = t / kCh, ch = t % kCh;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float4 y = *reinterpret_cast<const float4*>(sums + (p * kStep + r) * kD + 4 * (ch ^ (r & (kCh - 1))));
+        s.x += y.x;
+        s.y += y.y;
+        s.z += y.z;
+        s.w += y.w;
+      }
+      const int row = blk * kBlk + kStep * half + r;
+      if (g && row < a.L_own)
+        *reinterpret_cast<float4*>(g + b * gsb + h * gsh + (int64_t)row * gsl + 4 * ch) =
+            make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+    }
+  }
+}
+
+template <bool kKeys, typename T, int kD>
+void launch_pass(const BwdArgs& a, hipStream_t s) {
+  const int64_t groups = (a.n_slots + 3) / 4;
+  const unsigned wgs = (unsigned)((groups + 7) / 8 * 32);
+  const bool bias = a.bias != nullptr;
+  const bool parts = a.n_items <= 512;
+  if (parts) {
+    if (bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, 4>), dim3(wgs), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, 4>), dim3(wgs), dim3(512), 0, s, a);
+  } else {
+    if (bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, 1>), dim3(wgs), dim3(128), 0, s, a);
+    else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, 1>), dim3(wgs), dim3(128), 0, s, a);
+  }
+}
+
+template <bool kKeys>
+void launch_pass_f32(const BwdArgs& a, int D, hipStream_t s) {
+  const int64_t groups = (a.n_slots + 3) / 4;
+  const dim3 grid((unsigned)((groups + 7) / 8 * 64)), blk(256);
+  if (D == 64) hipLaunchKernelGGL((bsa_bwd_f32_kernel<kKeys, 64>), grid, blk, 0, s, a);
+  else hipLaunchKernelGGL((bsa_bwd_f32_kernel<kKeys, 128>), grid, blk, 0, s, a);
+}
+
+template <bool kKeys>
+void launch_pass_any(const BwdArgs& a, int dtype, int D, hipStream_t s) {
+  if (dtype == SA_DTYPE_F32) return launch_pass_f32<kKeys>(a, D, s);
+  if (dtype == SA_DTYPE_F16) return D == 64 ? launch_pass<kKeys, _Float16, 64>(a, s) : launch_pass<kKeys, _Float16, 128>(a, s);
+  return D == 64 ? launch_pass<kKeys, __bf16, 64>(a, s) : launch_pass<kKeys, __bf16, 128>(a, s);
+}
+
+int64_t stats_bytes(int B, int H, int Lq) { return (int64_t)B * H * sa::cdiv(Lq, kBlk) * 128 * sizeof(float); }
+
+}  // namespace
+
+extern "C" int sa_block_sparse_bwd_workspace(int B, int H, int Lq, int64_t* bytes) {
+  SA_REQUIRE(bytes, "sa_block_sparse_bwd_workspace: null bytes");
+  SA_REQUIRE(B > 0 && H > 0 && Lq > 0, "sa_block_sparse_bwd_workspace: bad shape B=%d H=%d Lq=%d", B, H, Lq);
+  *bytes = stats_bytes(B, H, Lq);
+  return sa::ok();
+}
+
+extern "C" int sa_block_sparse_bwd(int dtype, const void* q, const void* k, const void* v, const void* out,
+                                   const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                                   const int64_t strides[24], int B, int H, int Lq, int Lk, int D,
+                                   const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, const int32_t* q_beg,
+                                   const int32_t* q_idx, const float* key_bias, const int64_t bias_strides[2],
+                                   float sm_scale, const int32_t* q_order, int64_t n_q_slots, const int32_t* k_order,
+                                   int64_t n_k_slots, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* fn = "sa_block_sparse_bwd";
+  SA_REQUIRE(dtype == SA_DTYPE_BF16 || dtype == SA_DTYPE_F16 || dtype == SA_DTYPE_F32, "%s: dtype %d", fn, dtype);
+  SA_REQUIRE(q && k && v && out && dout && lse && strides && kv_idx && kv_cnt, "%s: null pointer", fn);
+  SA_REQUIRE(!(dk || dv) || (q_beg && q_idx), "%s: dk and dv need the transposed lists", fn);
+  SA_REQUIRE(B > 0 && H > 0 && Lq > 0 && Lk > 0, "%s: bad shape B=%d H=%d Lq=%d Lk=%d", fn, B, H, Lq, Lk);
+  if (D != 64 && D != 128) return sa::fail(SA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", fn, D);
+  SA_REQUIRE(max_cnt > 0, "%s: max_cnt must be > 0", fn);
+  SA_REQUIRE(std::isfinite(sm_scale) && sm_scale > 0.f, "%s: sm_scale must be finite and > 0", fn);
+  SA_REQUIRE(!key_bias || bias_strides, "%s: key_bias without bias_strides", fn);
+  const bool f32 = dtype == SA_DTYPE_F32;
+  if (f32 && key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
+  const int nqb = sa::cdiv(Lq, kBlk), nkb = sa::cdiv(Lk, kBlk);
+  const int64_t q_items = (int64_t)B * H * nqb, k_items = (int64_t)B * H * nkb;
+  SA_REQUIRE(q_items < (1LL << 28) && k_items < (1LL << 28), "%s: too many blocks", fn);
+  SA_REQUIRE((int64_t)nqb * max_cnt < (1LL << 31), "%s: lists of one head too long", fn);
+  const int per16 = f32 ? 4 : 8, size = f32 ? 4 : 2;
+  const void* ptrs[8] = {q, k, v, out, dout, dq, dk, dv};
+  for (int i = 0; i < 8; ++i) {
+    if (reinterpret_cast<uintptr_t>(ptrs[i]) % 16 != 0)
+      return sa::fail(SA_ERR_UNSUPPORTED, "%s: tensor base not 16-byte aligned", fn);
+    for (int j = 0; j < 3; ++j)
+      if (ptrs[i] && strides[3 * i + j] % per16 != 0)
+        return sa::fail(SA_ERR_UNSUPPORTED, "%s: strides must be multiples of %d elements", fn, per16);
+  }
+  // Streamed rows are copied through 32-bit buffer offsets relative to each head's first row.
+  const int64_t rows[4] = {Lq, Lk, Lk, Lq};
+  const int at[4] = {0, 1, 2, 4};
+  for (int i = 0; i < 4; ++i)
+    if (strides[3 * at[i] + 2] < 0 || (rows[i] + kBlk) * strides[3 * at[i] + 2] * size + 2 * D > INT_MAX)
+      return sa::fail(SA_ERR_UNSUPPORTED, "%s: rows of one head span more than 2 GiB", fn);
+  SA_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "%s: workspace null or not 256-byte aligned",
+             fn);
+  SA_REQUIRE(workspace_bytes >= stats_bytes(B, H, Lq), "%s: workspace of %lld bytes < %lld", fn,
+             (long long)workspace_bytes, (long long)stats_bytes(B, H, Lq));
+  SA_REQUIRE((!q_order || (n_q_slots > 0 && n_q_slots % 4 == 0 && n_q_slots < (1LL << 30))) &&
+                 (!k_order || (n_k_slots > 0 && n_k_slots % 4 == 0 && n_k_slots < (1LL << 30))),
+             "%s: slots must be a positive multiple of 4", fn);
+  hipStream_t s = sa::as_stream(stream);
+  BwdArgs a;
+  a.H = H;
+  a.max_cnt = max_cnt;
+  a.bias = key_bias;
+  a.bias_sb = key_bias ? bias_strides[0] : 0;
+  a.bias_sh = key_bias ? bias_strides[1] : 0;
+  a.sm_scale = sm_scale;
+  a.scale_log2 = sm_scale * kLog2e;
+  a.inv_scale_log2 = 1.f / a.scale_log2;
+  a.lse = lse;
+  a.stats = static_cast<float*>(workspace);
+  a.out = out;
+  a.o_sb = strides[9]; a.o_sh = strides[10]; a.o_sl = strides[11];
+
+  a.own_a = q; a.oa_sb = strides[0]; a.oa_sh = strides[1]; a.oa_sl = strides[2];
+  a.own_b = dout; a.ob_sb = strides[12]; a.ob_sh = strides[13]; a.ob_sl = strides[14];
+  a.st_a = k; a.sa_sb = strides[3]; a.sa_sh = strides[4]; a.sa_sl = strides[5];
+  a.st_b = v; a.sb_sb = strides[6]; a.sb_sh = strides[7]; a.sb_sl = strides[8];
+  a.grad_a = dq; a.ga_sb = strides[15]; a.ga_sh = strides[16]; a.ga_sl = strides[17];
+  a.grad_b = nullptr; a.gb_sb = a.gb_sh = a.gb_sl = 0;
+  a.L_own = Lq; a.L_st = Lk; a.n_own = nqb; a.n_st = nkb;
+  a.n_items = (int)q_items;
+  a.order = q_order;
+  a.n_slots = (int)(q_order ? n_q_slots : (q_items + 3) / 4 * 4);
+  a.idx = kv_idx; a.cnt = kv_cnt;
+  launch_pass_any<false>(a, dtype, D, s);
+  if (int rc = sa::check_launch(fn)) return rc;
+  if (!dk && !dv) return sa::ok();
+
+  a.own_a = k; a.oa_sb = strides[3]; a.oa_sh = strides[4]; a.oa_sl = strides[5];
+  a.own_b = v; a.ob_sb = strides[6]; a.ob_sh = strides[7]; a.ob_sl = strides[8];
+  a.st_a = q; a.sa_sb = strides[0]; a.sa_sh = strides[1]; a.sa_sl = strides[2];
+  a.st_b = dout; a.sb_sb = strides[12]; a.sb_sh = strides[13]; a.sb_sl = strides[14];
+  a.grad_a = dk; a.ga_sb = strides[18]; a.ga_sh = strides[19]; a.ga_sl = strides[20];
+  a.grad_b = dv; a.gb_sb = strides[21]; a.gb_sh = strides[22]; a.gb_sl = strides[23];
+  a.L_own = Lk; a.L_st = Lq; a.n_own = nkb; a.n_st = nqb;
+  a.n_items = (int)k_items;
+  a.order = k_order;
+  a.n_slots = (int)(k_order ? n_k_slots : (k_items + 3) / 4 * 4);
+  a.idx = q_idx; a.cnt = q_beg;
+  launch_pass_any<true>(a, dtype, D, s);
+  return sa::check_launch(fn);
+}

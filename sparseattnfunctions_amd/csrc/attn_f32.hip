@@ -64,13 +64,18 @@ struct F32Args {
   // log2-sum-exp2 to pool_lse[bh * pool_lpad + row].
   float* pool_r;
   int pool_ncol;
-  float* pool_lse;
+  float* pool_lse;  // (without pooling nullable, stored as the backward pass wants it: train_lse)
   int pool_lpad;
   // bsa_fwd_f32_terms_kernel: the split operands and the per-key-block flags (f32_terms_kernel).
   const uint8_t* planes;
   const uint4* flags;
   int plain_after;  // bsa_fwd_f32_kernel follows for the heads flagged kTermSkip
 };
+
+// log2-sum-exp2 of a row for the backward pass: +inf for a row without a key, as past Lq.
+__device__ inline float train_lse(float m, float l, bool row_ok) {
+  return row_ok && l != 0.f ? (m == -INFINITY ? 0.f : m) + log2f(l) : INFINITY;
+}
 
 __device__ inline sa_f32x4 mfma16x4(float a, float b, sa_f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -260,6 +265,8 @@ __device__ __forceinline__ void f32_store(const F32Args& a, int bh, int qb, int 
     const int row = qb * kBlk + row0 + 16 * j + r;
     if constexpr (kPool != 0) {
       if (g == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = (m[j] == -INFINITY ? 0.f : m[j]) + log2f(l_tot);
+    } else if (a.pool_lse && g == 0) {
+      a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(m[j], l_tot, row < a.Lq);
     }
     if (row < a.Lq) {
       float* orow = obase + (int64_t)row * a.o_sl;
@@ -789,6 +796,8 @@ __global__ __launch_bounds__(256, 2) void bsa_fwd_f32_terms_kernel(F32Args a) {
         const int row = qb * kBlk + row0 + lrow;
         if constexpr (kPool != 0) {
           if (hh == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = (m[g] == -INFINITY ? 0.f : m[g]) + log2f(l_tot);
+        } else if (a.pool_lse && hh == 0) {
+          a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(m[g], l_tot, row < a.Lq);
         }
         if (row < a.Lq) {
           float* orow = a.o + b * a.o_sb + h * a.o_sh + (int64_t)row * a.o_sl;
@@ -841,6 +850,8 @@ __global__ __launch_bounds__(256, 2) void bsa_fwd_f32_terms_kernel(F32Args a) {
       const int row = qb * kBlk + row0 + lrow;
       if constexpr (kPool != 0) {
         if (ch == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = (M == -INFINITY ? 0.f : M) + log2f(L);
+      } else if (a.pool_lse && ch == 0) {
+        a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(M, L, row < a.Lq);
       }
       if (row < a.Lq) {
         float* orow = a.o + b * a.o_sb + h * a.o_sh + (int64_t)row * a.o_sl;
@@ -1009,6 +1020,21 @@ int launch_f32(const float* q, const int64_t q_strides[3], const float* k, const
 
 namespace sa {
 int64_t attn_f32_terms_bytes(int B, int Hk, int Lk, int D) { return terms_blocks(B, Hk, Lk) * (768LL * D + 16); }
+
+// fp32 attention that stores the rows' log2-sum-exp2 (with a workspace on split operands).
+int attn_f32_lse(const float* q, const int64_t q_strides[3], const float* k, const int64_t k_strides[3],
+                 const float* v, const int64_t v_strides[3], float* out, const int64_t out_strides[3], int B, int H,
+                 int Lq, int Lk, int D, const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, float sm_scale,
+                 const int32_t* work_order, int64_t n_slots, void* workspace, int64_t workspace_bytes, float* lse,
+                 void* stream, const char* fn) {
+  if (workspace) {
+    SA_REQUIRE(B > 0 && H > 0 && Lk > 0, "%s: bad shape B=%d H=%d Lk=%d", fn, B, H, Lk);
+    if (D != 64 && D != 128) return sa::fail(SA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", fn, D);
+    if (int rc = check_terms(B, H, Lk, D, workspace, workspace_bytes, fn)) return rc;
+  }
+  return launch_f32(q, q_strides, k, k_strides, v, v_strides, out, out_strides, B, H, Lq, Lk, D, kv_idx, kv_cnt,
+                    max_cnt, false, sm_scale, work_order, n_slots, 1, false, 0, nullptr, lse, workspace, stream, fn);
+}
 
 // fp32 attention in pooling mode for the pooled-map entry point (attn_fwd.hip).
 int attn_f32_pooling(const float* q, const int64_t q_strides[3], const float* k, const int64_t k_strides[3],

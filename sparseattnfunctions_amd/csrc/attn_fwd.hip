@@ -46,6 +46,7 @@
 #include <type_traits>
 #include <vector>
 
+#include "attn_tile.h"
 #include "sa_common.h"
 
 namespace {
@@ -57,16 +58,11 @@ constexpr int kWaves = 4;        // independent waves per workgroup
 template <int kD>
 constexpr int kSplitFloats = kBlock * kD + 2 * kBlock;
 constexpr int kTileBytes = kBlock * kHeadDim * 2;  // one K or V tile: 64 rows x 128 B
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.0f;
 // fp16 scores: largest |S * scale_log2| bound (Cauchy-Schwarz of the row norms) for which an
 // item uses them, and the squared-norm limit below 65504^2 (the largest fp16 value).
 constexpr float kK16Bound = 32.0f;
 constexpr float kK16NormMax = 4.0e9f;
-
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
-typedef short sa_i16x4v __attribute__((ext_vector_type(4)));
-typedef unsigned sa_u32x4v __attribute__((ext_vector_type(4)));
 
 struct FwdArgs {
   const uint16_t* q;
@@ -112,7 +108,7 @@ struct FwdArgs {
   float* pool_r;
   int pool_ncol;
   int pool_lpad;
-  float* pool_lse;  // null: not stored
+  float* pool_lse;  // null: not stored. Without pooling: stored as the backward pass wants it (train_lse)
   // Fused pooled map (pool_po non-null; pooled block size = kPool): after its item the wave
   // forms the Po rows of its own query rows, Po[i][c] = max over the rows r of query block i
   // of exp2(R[c][r] - lse[r]), each Po row then divided by its sum. Po rows and columns are
@@ -139,156 +135,11 @@ __device__ inline int range_item(const FwdArgs& a, int slot) {
   return kDown ? hi - 1 - i : lo + i;
 }
 
-__device__ inline sa_bf16x8 as_bf16x8(uint4 x) { return __builtin_bit_cast(sa_bf16x8, x); }
-__device__ inline sa_bf16x8 as_bf16x8(sa_u32x4v x) { return __builtin_bit_cast(sa_bf16x8, x); }
-
-__device__ inline sa_f32x16 mfma32(sa_bf16x8 a, sa_bf16x8 b, sa_f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+// log2-sum-exp2 of a row for the backward pass: +inf for a row without a key (its recomputed
+// probabilities are then 0), as for rows past Lq, which the padded array has.
+__device__ inline float train_lse(float m, float l, bool row_ok) {
+  return row_ok && l != 0.f ? (m == -INFINITY ? 0.f : m) + log2f(l) : INFINITY;
 }
-
-__device__ inline float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-typedef __bf16 sa_bf16x2 __attribute__((ext_vector_type(2)));
-
-// Two fp32 -> packed bf16 pair (round to nearest even, v_cvt_pk_bf16_f32).
-__device__ inline uint32_t cvt_pk_bf16(float a, float b) {
-  sa_bf16x2 r = {(__bf16)a, (__bf16)b};
-  return __builtin_bit_cast(uint32_t, r);
-}
-
-__device__ inline float dot2_bf16_ones(uint32_t pair, float acc) {
-  const sa_bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
-  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(sa_bf16x2, pair), ones, acc, false);
-}
-
-typedef _Float16 sa_f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 sa_f16x8 __attribute__((ext_vector_type(8)));
-
-// Operand element type of a launch: the MFMA, the rounding of P (and of the output) to the
-// element type (round to nearest even), and the row-sum dot of a packed pair with ones.
-template <typename T>
-struct Elem;
-template <>
-struct Elem<__bf16> {
-  typedef sa_bf16x8 v8;
-  __device__ static inline v8 as8(sa_u32x4v x) { return as_bf16x8(x); }
-  __device__ static inline sa_f32x16 mfma(v8 a, v8 b, sa_f32x16 c) { return mfma32(a, b, c); }
-  __device__ static inline uint32_t pack(float a, float b) { return cvt_pk_bf16(a, b); }
-  __device__ static inline float dot2_ones(uint32_t pair, float acc) { return dot2_bf16_ones(pair, acc); }
-};
-template <>
-struct Elem<_Float16> {
-  typedef sa_f16x8 v8;
-  __device__ static inline v8 as8(sa_u32x4v x) { return __builtin_bit_cast(sa_f16x8, x); }
-  __device__ static inline sa_f32x16 mfma(v8 a, v8 b, sa_f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-  }
-  __device__ static inline uint32_t pack(float a, float b) {  // v_cvt_pk_f16_f32
-    const sa_f16x2 r = {(_Float16)a, (_Float16)b};
-    return __builtin_bit_cast(uint32_t, r);
-  }
-  __device__ static inline float dot2_ones(uint32_t pair, float acc) {
-    const sa_f16x2 ones = {(_Float16)1.0f, (_Float16)1.0f};
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(sa_f16x2, pair), ones, acc, false);
-  }
-};
-
-// max / sum of x over lanes l and l ^ 32 (v_permlane32_swap: no LDS traffic).
-__device__ inline float xhalf_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ inline float xhalf_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// 16-byte chunk swizzle of LDS tile row r (depends on r mod 16). Chunk c of row r is stored
-// at chunk c ^ swz(r). With 64 or 32 LDS banks it makes conflict-free (a) the K operand
-// reads, 16 lanes reading 16 consecutive rows at one chunk, and (b) the transposed V reads,
-// 32 lanes reading 4 consecutive rows x 4 chunks.
-__device__ inline int swz(int r) {
-  const int j = (r >> 1) & 7;
-  return (((j & 1) << 2) | (j >> 1)) ^ ((r & 1) << 1);
-}
-
-__device__ inline sa_u32x4v lds_read_b128(const lds_u8* p) {
-  return *reinterpret_cast<const __attribute__((address_space(3))) sa_u32x4v*>(p);
-}
-// ds_read_b64_tr_b16: within each 16-lane group, lane i points at 4 consecutive bf16 (row
-// i/4, columns 4(i%4)..+3 of a 4 x 16 block); lane j receives column j of that block.
-__device__ inline uint2 lds_read_tr16(const lds_u8* p) {
-  const sa_i16x4v v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sa_i16x4v*)(p));
-  return __builtin_bit_cast(uint2, v);
-}
-typedef unsigned sa_u32x2v __attribute__((ext_vector_type(2)));
-// The same read issued as inline assembly: the compiler's wait analysis cannot tell these
-// reads from the copies still landing in the other LDS buffers and would otherwise wait for
-// all of them; the caller waits for the reads explicitly (lgkm_wait_pair).
-template <int kOff>
-__device__ inline sa_u32x2v lds_read_tr16_asm(uint32_t addr) {
-  sa_u32x2v r;
-  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(kOff));
-  return r;
-}
-
-// Copy one 64-row tile into LDS: instruction i, lane l -> row 8i + l/8 (tile-relative),
-// 16-byte slot l of the i-th KB of `dst`. goff[p] = lane offset for rows with (row/8) odd
-// (p = 1) or even (p = 0); it holds the swizzle. Offsets at or past `bytes` read as zero.
-__device__ inline void dma_tile(const void* base, uint32_t bytes, uint32_t tile_off, uint32_t row_bytes,
-                                const uint32_t (&goff)[2], lds_u8* dst) {
-  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0,
-                                                                        (int)bytes, 0x00020000);
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_u8*)(dst + 1024 * i), 16,
-                                             tile_off + 8 * i * row_bytes + goff[i & 1], 0, 0, 0);
-}
-
-// dma_tile for a tile of contiguous 128-byte rows (head dim 64, row stride 64 elements): the
-// same copies, with the descriptors based at the tile's rows 0 and 32, so that the lane
-// offsets stay loop invariant and the instruction offset (added to both the global and the
-// LDS address) steps the 8-row groups; no per-tile vector address arithmetic. Each
-// descriptor's size ends at the same byte as dma_tile's (0 when row 32 lies past it): a lane
-// reads offset goff + 1024 j of the descriptor at off iff off + goff + 1024 j < bytes, so rows
-// past Lk read as zero as before.
-__device__ inline void dma_tile_c128(const uint16_t* base, uint32_t bytes, uint32_t tile_off,
-                                     const uint32_t (&goff)[2], lds_u8* dst) {
-#pragma unroll
-  for (int hq = 0; hq < 2; ++hq) {
-    // Wave-uniform by construction; readfirstlane lets the compiler build the descriptor
-    // in scalar registers.
-    const uint32_t off = __builtin_amdgcn_readfirstlane(tile_off + 4096u * hq);
-    const uint32_t end = __builtin_amdgcn_readfirstlane(bytes);
-    const int size = __builtin_amdgcn_readfirstlane(end - min(off, end));
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(base) + off), (short)0, size, 0x00020000);
-    lds_u8* d = dst + 4096 * hq;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, d, 16, goff[0], 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, d, 16, goff[1], 0, 1024, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, d, 16, goff[0], 0, 2048, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, d, 16, goff[1], 0, 3072, 0);
-  }
-}
-
-// Waits until at most n LDS reads are outstanding (n in 0..14, even), tying the wait to
-// the two registers it makes valid so that nothing reads them earlier.
-__device__ __forceinline__ void lgkm_wait_pair(int n, sa_u32x2v& a, sa_u32x2v& b) {
-  switch (n) {
-    case 14: asm volatile("s_waitcnt lgkmcnt(14)" : "+v"(a), "+v"(b)); break;
-    case 12: asm volatile("s_waitcnt lgkmcnt(12)" : "+v"(a), "+v"(b)); break;
-    case 10: asm volatile("s_waitcnt lgkmcnt(10)" : "+v"(a), "+v"(b)); break;
-    case 8: asm volatile("s_waitcnt lgkmcnt(8)" : "+v"(a), "+v"(b)); break;
-    case 6: asm volatile("s_waitcnt lgkmcnt(6)" : "+v"(a), "+v"(b)); break;
-    case 4: asm volatile("s_waitcnt lgkmcnt(4)" : "+v"(a), "+v"(b)); break;
-    case 2: asm volatile("s_waitcnt lgkmcnt(2)" : "+v"(a), "+v"(b)); break;
-    default: asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a), "+v"(b) : : "memory"); break;
-  }
-}
-
-// s_waitcnt encodings (gfx9): vmcnt in bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8.
-constexpr int waitcnt_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
-constexpr int kWaitLgkm0 = 0xC07F;
 
 // T: bf16 or fp16 operands (and output). kD: head dim 64 or 128. A 128-dim row is staged as
 // two 128-byte half rows in two half tiles with the 64-dim layout, so every read pattern of
@@ -979,6 +830,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs 
       const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
       int row = qb * kBlock + r;
       bool store = row < a.Lq;
+      if (kPool == 0 && a.pool_lse && ch == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(M, lsum, store);
       if (store && a.o_rows) {
         row = a.o_rows[row];
         store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -1035,6 +887,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs 
     }
     int row = qb * kBlock + 32 * g + col;
     bool store = row < a.Lq;
+    if (kPool == 0 && a.pool_lse && g == hh) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(m[g], l_tot, store);
     if (store && a.o_rows) {  // remapped layout: query i goes to out row o_rows[i]
       row = a.o_rows[row];
       store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -1119,10 +972,6 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs 
 }
 
 
-// Workgroup barrier with no memory fence: the waits before it are explicit (a fence would
-// also wait for the copies in flight). The clobber keeps the compiler from moving LDS
-// accesses across it.
-__device__ __forceinline__ void wg_barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // Head dim 128, plain lists: one query block per workgroup of two waves (a wave pair). Wave g
 // holds query rows 32g .. 32g + 31 of the block: its Q^T operands, O^T accumulators and S^T
@@ -1471,6 +1320,7 @@ __global__ __launch_bounds__(128, 2) void bsa_fwd_pair_kernel(FwdArgs a) {
   const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
   int row = qb * kBlock + 32 * g + col;
   bool store = row < a.Lq;
+  if (a.pool_lse && hh == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(m, l_tot, store);
   if (store && a.o_rows) {  // remapped layout: query i goes to out row o_rows[i]
     row = a.o_rows[row];
     store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -1606,6 +1456,7 @@ __global__ __launch_bounds__(256) void split_merge_kernel(FwdArgs a) {
   }
   const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
   int row = qb * kBlock + r;
+  if (a.pool_lse && d0 == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(mx, lsum, row < a.Lq);
   if (row >= a.Lq) return;
   if (a.o_rows) {
     row = a.o_rows[row];
@@ -1988,6 +1839,31 @@ extern "C" int sa_block_sparse_fwd(const uint16_t* q, const int64_t q_strides[3]
   return launch_fwd(q, q_strides, k, k_strides, v, v_strides, out, out_strides, B, H, Lq, Lk, D, kv_idx, kv_cnt,
                     max_cnt, false, nullptr, nullptr, key_bias, bias_strides, sm_scale, work_order, n_slots, nullptr,
                     0, nullptr, 0, stream, "sa_block_sparse_fwd");
+}
+
+extern "C" int sa_block_sparse_fwd_lse(int dtype, const void* q, const int64_t q_strides[3], const void* k,
+                                       const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                                       void* out, const int64_t out_strides[3], int B, int H, int Lq, int Lk, int D,
+                                       const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt,
+                                       const float* key_bias, const int64_t bias_strides[2], float sm_scale,
+                                       const int32_t* work_order, int64_t n_slots, int parts, void* workspace,
+                                       int64_t workspace_bytes, float* lse, void* stream) {
+  const char* fn = "sa_block_sparse_fwd_lse";
+  SA_REQUIRE(dtype == SA_DTYPE_BF16 || dtype == SA_DTYPE_F16 || dtype == SA_DTYPE_F32, "%s: dtype %d", fn, dtype);
+  SA_REQUIRE(lse, "%s: null lse", fn);
+  SA_REQUIRE(parts >= 1, "%s: parts=%d must be >= 1", fn, parts);
+  if (dtype == SA_DTYPE_F32) {
+    if (key_bias || parts != 1) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias or key-range parts", fn);
+    return sa::attn_f32_lse(static_cast<const float*>(q), q_strides, static_cast<const float*>(k), k_strides,
+                            static_cast<const float*>(v), v_strides, static_cast<float*>(out), out_strides, B, H, Lq,
+                            Lk, D, kv_idx, kv_cnt, max_cnt, sm_scale, work_order, n_slots, workspace, workspace_bytes,
+                            lse, stream, fn);
+  }
+  return launch_fwd(static_cast<const uint16_t*>(q), q_strides, static_cast<const uint16_t*>(k), k_strides,
+                    static_cast<const uint16_t*>(v), v_strides, static_cast<uint16_t*>(out), out_strides, B, H, Lq, Lk,
+                    D, kv_idx, kv_cnt, max_cnt, false, nullptr, nullptr, key_bias, bias_strides, sm_scale, work_order,
+                    n_slots, nullptr, 0, nullptr, 0, stream, fn, 1, 0, nullptr, lse, nullptr, dtype == SA_DTYPE_F16,
+                    false, parts, workspace, workspace_bytes);
 }
 
 namespace {

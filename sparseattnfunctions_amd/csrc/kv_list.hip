@@ -93,6 +93,84 @@ __global__ __launch_bounds__(256) void mask_cells_to_list_kernel(CellArgs a) {
   if (lane == 0) a.kv_cnt[row] = total;
 }
 
+// Transposed lists. One workgroup per (head, 64 key blocks): a first walk over the head's lists counts
+// the entries below its key blocks and of each of them, which gives where their lists begin; a second
+// walk, 128 query blocks at a time, counts each pair in LDS and writes the key blocks' entries in
+// ascending order of the query block, an entry as often as it is listed.
+constexpr int kWin = 64;        // key blocks per workgroup
+constexpr int kRowChunk = 128;  // query blocks per pass: 64 words of two 16-bit counts
+__global__ __launch_bounds__(256) void transpose_lists_kernel(const int32_t* __restrict__ kv_idx,
+                                                              const int32_t* __restrict__ kv_cnt, int nqb, int nkb,
+                                                              int max_cnt, int n_win, int32_t* __restrict__ q_beg,
+                                                              int32_t* __restrict__ q_idx) {
+  __shared__ int hist[kWin], pos[kWin], below;
+  __shared__ uint32_t seen[kWin][kRowChunk / 2 + 1];
+  const int64_t bh = blockIdx.x / n_win;
+  const int kb0 = (int)(blockIdx.x - bh * n_win) * kWin;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int32_t* idx = kv_idx + bh * nqb * max_cnt;
+  const int32_t* cnt = kv_cnt + bh * nqb;
+  int32_t* out = q_idx + bh * nqb * max_cnt;
+  if (threadIdx.x < kWin) hist[threadIdx.x] = 0;
+  if (threadIdx.x == 0) below = 0;
+  __syncthreads();
+  int before = 0;
+  for (int r = wave; r < nqb; r += 4) {
+    const int n = min(max(cnt[r], 0), max_cnt);
+    const int32_t* list = idx + (int64_t)r * max_cnt;
+    for (int j = lane; j < n; j += 64) {
+      const int kb = list[j];
+      if ((unsigned)kb >= (unsigned)nkb) continue;
+      if (kb < kb0) ++before;
+      else if (kb < kb0 + kWin) atomicAdd(&hist[kb - kb0], 1);
+    }
+  }
+  if (before) atomicAdd(&below, before);
+  __syncthreads();
+  if (wave == 0) {
+    int sum = hist[lane];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(sum, o);
+      if (lane >= o) sum += y;
+    }
+    const int first = below + sum - hist[lane];
+    pos[lane] = first;
+    int32_t* beg = q_beg + bh * (nkb + 1);
+    if (kb0 + lane < nkb) beg[kb0 + lane] = first;
+    if (kb0 + lane == nkb - 1) beg[nkb] = below + sum;
+  }
+  for (int r0 = 0; r0 < nqb; r0 += kRowChunk) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kWin * (kRowChunk / 2); i += 256) seen[i >> 6][i & 63] = 0;
+    __syncthreads();
+    for (int r = r0 + wave; r < min(nqb, r0 + kRowChunk); r += 4) {
+      const int n = min(max(cnt[r], 0), max_cnt);
+      const int32_t* list = idx + (int64_t)r * max_cnt;
+      for (int j = lane; j < n; j += 64) {
+        const int kb = list[j];
+        if (kb >= kb0 && kb < min(kb0 + kWin, nkb)) atomicAdd(&seen[kb - kb0][(r - r0) >> 1], (r & 1) ? 0x10000u : 1u);
+      }
+    }
+    __syncthreads();
+    for (int k = wave; k < min(kWin, nkb - kb0); k += 4) {
+      const uint32_t word = seen[k][lane];
+      const int n0 = word & 0xffff, n1 = word >> 16;
+      int sum = n0 + n1;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(sum, o);
+        if (lane >= o) sum += y;
+      }
+      const int first = pos[k];
+      int at = first + sum - n0 - n1;
+      for (int i = 0; i < n0; ++i) out[at++] = r0 + 2 * lane;
+      for (int i = 0; i < n1; ++i) out[at++] = r0 + 2 * lane + 1;
+      if (lane == 63) pos[k] = first + sum;
+    }
+  }
+}
+
 bool pow2_block(int x) { return x >= 16 && x <= 1024 && (x & (x - 1)) == 0; }
 
 }  // namespace
@@ -151,4 +229,20 @@ extern "C" int sa_mask_to_kv_list(const uint8_t* mask, const int64_t mask_stride
                      mask_strides[0], mask_strides[1], mask_strides[2], mask_strides[3], H, nqb, nkb, rows,
                      kv_idx, max_cnt, kv_cnt);
   return sa::check_launch("sa_mask_to_kv_list");
+}
+
+extern "C" int sa_kv_list_transpose(const int32_t* kv_idx, const int32_t* kv_cnt, int BH, int nqb, int nkb, int max_cnt,
+                                    int32_t* q_beg, int32_t* q_idx, void* stream) {
+  const char* fn = "sa_kv_list_transpose";
+  SA_REQUIRE(kv_idx && kv_cnt && q_beg && q_idx, "%s: null pointer", fn);
+  SA_REQUIRE(BH > 0 && nqb > 0 && nkb > 0 && max_cnt > 0, "%s: bad shape BH=%d nqb=%d nkb=%d max_cnt=%d", fn, BH, nqb,
+             nkb, max_cnt);
+  if (max_cnt > 65535 || (int64_t)nqb * max_cnt >= (1LL << 31))
+    return sa::fail(SA_ERR_UNSUPPORTED, "%s: lists of %d entries for %d query blocks", fn, max_cnt, nqb);
+  const int n_win = (nkb + kWin - 1) / kWin;
+  const int64_t blocks = (int64_t)BH * n_win;
+  SA_REQUIRE(blocks < (1LL << 31), "%s: too many lists", fn);
+  hipLaunchKernelGGL(transpose_lists_kernel, dim3((unsigned)blocks), dim3(256), 0, sa::as_stream(stream), kv_idx, kv_cnt,
+                     nqb, nkb, max_cnt, n_win, q_beg, q_idx);
+  return sa::check_launch(fn);
 }

@@ -1,0 +1,321 @@
+// Rotary positions of queries and keys: pairs of a head's values turned by an angle per token.
+//
+//   angle[token][pair] = position[axis of pair][token] * frequency[pair]
+//   (a, b) -> (a cos - b sin, b cos + a sin), and with -sin for the gradient (the transpose)
+//
+// The table kernel forms the angles in 64 bits, as turns, so that far positions keep their fraction,
+// and takes the quarter turn off before the 32-bit sine and cosine. The rotation is bound by memory:
+// each value is read and written once, and a thread keeps its pairs' cosines and sines while it goes
+// through the heads.
+#include <math.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "sa_common.h"
+
+namespace {
+
+constexpr int kMaxAxes = 4;
+constexpr int kMaxPairs = 128;
+
+struct TableArgs {
+  const void* positions;
+  int64_t stride_axis, stride_token;
+  int64_t n;  // tokens * pairs
+  int pairs, n_axes;
+  int axis_end[kMaxAxes];  // pairs of the axes up to this one
+  float factor[kMaxAxes];  // of the axis's cosines and sines
+  double turns[kMaxPairs];  // turns per position
+  float2* table;
+};
+
+template <typename P>
+__global__ __launch_bounds__(256) void rotary_table_kernel(TableArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.n) return;
+  const int64_t token = i / a.pairs;
+  const int pair = (int)(i - token * a.pairs);
+  int axis = 0;
+  while (pair >= a.axis_end[axis]) ++axis;  // (axis_end of the last axis is the number of pairs)
+  const double pos = (double)static_cast<const P*>(a.positions)[axis * a.stride_axis + token * a.stride_token];
+  const double t = pos * a.turns[pair];
+  const double quarter = rint(4.0 * t);
+  const float f = (float)(t - 0.25 * quarter);  // |f| <= 1/8 turn
+  float s, c;
+  sincospif(2.f * f, &s, &c);
+  // quarter mod 4 (an infinite or NaN position gives NaN either way)
+  const int q = (int)(quarter - 4.0 * floor(0.25 * quarter));
+  const float sn = (q & 1) ? c : s, cs = (q & 1) ? s : c;
+  const float m = a.factor[axis];
+  a.table[i] = make_float2((q == 1 || q == 2) ? -cs * m : cs * m, (q & 2) ? -sn * m : sn * m);
+}
+
+// ---- rotation -----------------------------------------------------------------------------------
+
+struct RotArgs {
+  const void* x[2];  // q, k
+  void* y[2];
+  int64_t xs[2][3], ys[2][3];  // strides of b, h, l
+  int heads[2];
+  int B, L, D;
+  const float2* table;
+  int n_rows, pairs;
+  const int32_t* rows;  // nullable: table row of token (b, t) at rows[b * rows_sb + t]
+  int64_t rows_sb;
+  int skip;             // without rows: token t has row t - skip
+  float sign;           // of the sines
+  int copy;             // values that do not turn are copied (0: in place, they are left)
+  int units, tokens, slots;  // threads: unit + units * (token + tokens * head slot)
+  int group;            // heads per workgroup (of q's and k's together)
+};
+
+template <typename T>
+struct Vec8;  // eight values of a head as floats
+template <>
+struct Vec8<float> {
+  static __device__ inline void load(const void* p, float (&v)[8]) {
+    const float4 a = static_cast<const float4*>(p)[0], b = static_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  static __device__ inline void store(void* p, const float (&v)[8]) {
+    static_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    static_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+};
+template <typename T>
+struct Vec8 {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  static __device__ inline void load(const void* p, float (&v)[8]) {
+    const t8 a = *static_cast<const t8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+  }
+  static __device__ inline void store(void* p, const float (&v)[8]) {
+    t8 a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (T)v[i];  // round to nearest even
+    *static_cast<t8*>(p) = a;
+  }
+};
+
+// A thread turns one unit of one token in every head of its group: interleaved, eight consecutive
+// values (four pairs); halves, eight values of each half (eight pairs). Units past the turned part
+// copy eight values. Loads of kUnroll heads are in flight together.
+template <typename T, bool kHalf>
+__global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
+  constexpr int kUnroll = 4;
+  constexpr int kPairs = kHalf ? 8 : 4;
+  const int unit = threadIdx.x % a.units;
+  const int rest = threadIdx.x / a.units;
+  const int slot = rest / a.tokens;
+  const int token_groups = (a.L + a.tokens - 1) / a.tokens;
+  const int b = blockIdx.x / token_groups;
+  const int t = (blockIdx.x - b * token_groups) * a.tokens + (rest - slot * a.tokens);
+  if (slot >= a.slots || t >= a.L) return;
+  const int row = a.rows ? a.rows[b * a.rows_sb + t] : t - a.skip;
+  const int turned = kHalf ? a.pairs / 8 : a.pairs / 4;  // units that turn
+  const bool turn = unit < turned && (unsigned)row < (unsigned)a.n_rows;
+  if (!turn && !a.copy) return;
+  float c[kPairs], s[kPairs];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) c[i] = 1.f, s[i] = 0.f;
+  if (turn) {
+    const float4* p = reinterpret_cast<const float4*>(a.table + (int64_t)row * a.pairs + kPairs * unit);
+#pragma unroll
+    for (int i = 0; i < kPairs; i += 2) {
+      const float4 x = p[i >> 1];
+      c[i] = x.x; s[i] = x.y * a.sign;
+      c[i + 1] = x.z; s[i + 1] = x.w * a.sign;
+    }
+  }
+  // Halves: a unit has two chunks where it lies in the turned part, else one.
+  const bool two = kHalf && unit < turned;
+  const int at0 = kHalf ? (unit < turned ? 8 * unit : 2 * a.pairs + 8 * (unit - turned)) : 8 * unit;
+  const int at1 = a.pairs + 8 * unit;
+  const int n_heads = a.heads[0] + a.heads[1];
+  const int end = min(n_heads, (int)(blockIdx.y + 1) * a.group);
+  for (int h0 = blockIdx.y * a.group + slot; h0 < end; h0 += kUnroll * a.slots) {
+    float x[kUnroll][8], y[kHalf ? kUnroll : 1][8];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int h = h0 + u * a.slots;
+      if (h < end) {
+        const int w = h >= a.heads[0];
+        const T* p = static_cast<const T*>(w ? a.x[1] : a.x[0]) + b * (w ? a.xs[1][0] : a.xs[0][0]) +
+                     (h - (w ? a.heads[0] : 0)) * (w ? a.xs[1][1] : a.xs[0][1]) + t * (w ? a.xs[1][2] : a.xs[0][2]);
+        Vec8<T>::load(p + at0, x[u]);
+        if (two) Vec8<T>::load(p + at1, y[kHalf ? u : 0]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int h = h0 + u * a.slots;
+      if (h < end) {
+        const int w = h >= a.heads[0];
+        T* p = static_cast<T*>(w ? a.y[1] : a.y[0]) + b * (w ? a.ys[1][0] : a.ys[0][0]) +
+               (h - (w ? a.heads[0] : 0)) * (w ? a.ys[1][1] : a.ys[0][1]) + t * (w ? a.ys[1][2] : a.ys[0][2]);
+        if (turn) {  // (a token without a position keeps its values, infinities among them)
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) {
+            float& xa = kHalf ? x[u][i] : x[u][2 * (i & 3)];
+            float& xb = kHalf ? y[kHalf ? u : 0][i] : x[u][2 * (i & 3) + 1];
+            const float va = xa, vb = xb;
+            xa = fmaf(va, c[i], -(vb * s[i]));
+            xb = fmaf(vb, c[i], va * s[i]);
+          }
+        }
+        Vec8<T>::store(p + at0, x[u]);
+        if (two) Vec8<T>::store(p + at1, y[kHalf ? u : 0]);
+      }
+    }
+  }
+}
+
+// Any head dim, number of pairs, strides and alignment: a unit is one pair, then one value each.
+template <typename T, bool kHalf>
+__global__ __launch_bounds__(256) void rotary_any_kernel(RotArgs a) {
+  const int unit = threadIdx.x % a.units;
+  const int rest = threadIdx.x / a.units;
+  const int slot = rest / a.tokens;
+  const int token_groups = (a.L + a.tokens - 1) / a.tokens;
+  const int b = blockIdx.x / token_groups;
+  const int t = (blockIdx.x - b * token_groups) * a.tokens + (rest - slot * a.tokens);
+  if (slot >= a.slots || t >= a.L) return;
+  const int row = a.rows ? a.rows[b * a.rows_sb + t] : t - a.skip;
+  const bool pair = unit < a.pairs;
+  const bool turn = pair && (unsigned)row < (unsigned)a.n_rows;
+  if (!turn && !a.copy) return;
+  float2 cs = make_float2(1.f, 0.f);
+  if (turn) cs = a.table[(int64_t)row * a.pairs + unit];
+  cs.y *= a.sign;
+  const int at0 = !pair ? unit + a.pairs : kHalf ? unit : 2 * unit;
+  const int at1 = !pair ? at0 : kHalf ? unit + a.pairs : 2 * unit + 1;
+  const int n_heads = a.heads[0] + a.heads[1];
+  const int end = min(n_heads, (int)(blockIdx.y + 1) * a.group);
+  for (int h = blockIdx.y * a.group + slot; h < end; h += a.slots) {
+    const int w = h >= a.heads[0], hw = h - (w ? a.heads[0] : 0);
+    const T* p = static_cast<const T*>(a.x[w]) + b * a.xs[w][0] + hw * a.xs[w][1] + t * a.xs[w][2];
+    T* o = static_cast<T*>(a.y[w]) + b * a.ys[w][0] + hw * a.ys[w][1] + t * a.ys[w][2];
+    const T va = p[at0], vb = p[at1];
+    o[at0] = turn ? (T)fmaf((float)va, cs.x, -((float)vb * cs.y)) : va;
+    if (pair) o[at1] = turn ? (T)fmaf((float)vb, cs.x, (float)va * cs.y) : vb;
+  }
+}
+
+template <typename T>
+int launch_rotary(RotArgs a, bool half, bool wide, hipStream_t s, const char* fn) {
+  // units per token, then as many tokens (a power of two up to the length) and head slots as fit 256 threads
+  a.units = !wide ? a.D - a.pairs : half ? a.pairs / 8 + (a.D - 2 * a.pairs) / 8 : a.D / 8;
+  const int room = 256 / a.units;
+  a.tokens = 1;
+  while (2 * a.tokens <= room && a.tokens < a.L) a.tokens *= 2;
+  a.slots = room / a.tokens;
+  const int n_heads = a.heads[0] + a.heads[1];
+  const int64_t wgs = (int64_t)a.B * ((a.L + a.tokens - 1) / a.tokens);
+  SA_REQUIRE(wgs < (1LL << 31), "%s: grid too large", fn);
+  // A group of heads shares the table's values; groups as large as leave some 4 096 workgroups.
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(n_heads, 4096 / wgs));
+  a.group = std::max((int)((n_heads + want - 1) / want), std::min(n_heads, a.slots));
+  const dim3 grid((unsigned)wgs, (unsigned)((n_heads + a.group - 1) / a.group)), blk(256);
+  if (wide) {
+    if (half) hipLaunchKernelGGL((rotary_kernel<T, true>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, false>), grid, blk, 0, s, a);
+  } else {
+    if (half) hipLaunchKernelGGL((rotary_any_kernel<T, true>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((rotary_any_kernel<T, false>), grid, blk, 0, s, a);
+  }
+  return sa::check_launch(fn);
+}
+
+}  // namespace
+
+extern "C" int sa_rotary_table(const void* positions, int position_type, const int64_t strides[2], int64_t L, int n_axes,
+                               const int32_t* axis_pairs, const double* frequencies, const double* factors,
+                               float* table, void* stream) {
+  const char* fn = "sa_rotary_table";
+  SA_REQUIRE(positions && strides && axis_pairs && frequencies && factors && table, "%s: null pointer", fn);
+  SA_REQUIRE(L > 0 && L < (1LL << 31), "%s: L=%lld", fn, (long long)L);
+  SA_REQUIRE(n_axes >= 1 && n_axes <= kMaxAxes, "%s: %d axes (1 to %d)", fn, n_axes, kMaxAxes);
+  SA_REQUIRE(reinterpret_cast<uintptr_t>(table) % 8 == 0, "%s: table not 8-byte aligned", fn);
+  TableArgs a;
+  a.positions = positions;
+  a.stride_axis = strides[0];
+  a.stride_token = strides[1];
+  a.pairs = 0;
+  a.n_axes = n_axes;
+  for (int i = 0; i < n_axes; ++i) {
+    SA_REQUIRE(axis_pairs[i] > 0 && axis_pairs[i] <= kMaxPairs - a.pairs, "%s: axes of more than %d pairs", fn, kMaxPairs);
+    a.pairs += axis_pairs[i];
+    a.axis_end[i] = a.pairs;
+    SA_REQUIRE(std::isfinite(factors[i]), "%s: factor %d is not finite", fn, i);
+    a.factor[i] = (float)factors[i];
+  }
+  for (int i = 0; i < a.pairs; ++i) {
+    SA_REQUIRE(std::isfinite(frequencies[i]), "%s: frequency %d is not finite", fn, i);
+    a.turns[i] = frequencies[i] / 6.283185307179586476925287;
+  }
+  a.n = L * a.pairs;
+  a.table = reinterpret_cast<float2*>(table);
+  const int64_t wgs = (a.n + 255) / 256;
+  SA_REQUIRE(wgs < (1LL << 31), "%s: grid too large", fn);
+  const dim3 grid((unsigned)wgs), blk(256);
+  hipStream_t s = sa::as_stream(stream);
+  if (position_type == SA_POSITION_I32) hipLaunchKernelGGL(rotary_table_kernel<int32_t>, grid, blk, 0, s, a);
+  else if (position_type == SA_POSITION_I64) hipLaunchKernelGGL(rotary_table_kernel<int64_t>, grid, blk, 0, s, a);
+  else if (position_type == SA_POSITION_F32) hipLaunchKernelGGL(rotary_table_kernel<float>, grid, blk, 0, s, a);
+  else if (position_type == SA_POSITION_F64) hipLaunchKernelGGL(rotary_table_kernel<double>, grid, blk, 0, s, a);
+  else return sa::fail(SA_ERR_INVALID, "%s: position type %d", fn, position_type);
+  return sa::check_launch(fn);
+}
+
+extern "C" int sa_rotary_apply(int dtype, const void* q, void* q_out, const void* k, void* k_out,
+                               const int64_t strides[12], int B, int H, int Hk, int L, int D, const float* table,
+                               int n_rows, int pairs, const int32_t* rows, int64_t rows_batch_stride, int skip,
+                               int halves, int inverse, void* stream) {
+  const char* fn = "sa_rotary_apply";
+  SA_REQUIRE(dtype == SA_DTYPE_BF16 || dtype == SA_DTYPE_F16 || dtype == SA_DTYPE_F32, "%s: dtype %d", fn, dtype);
+  SA_REQUIRE(q && q_out && strides && table, "%s: null pointer", fn);
+  SA_REQUIRE(!k == !k_out, "%s: k without its output", fn);
+  SA_REQUIRE(B > 0 && H > 0 && (!k || Hk > 0) && L > 0 && D > 0, "%s: bad shape B=%d H=%d Hk=%d L=%d D=%d", fn, B, H, Hk,
+             L, D);
+  SA_REQUIRE(D <= 2 * kMaxPairs, "%s: head dim %d (at most %d)", fn, D, 2 * kMaxPairs);
+  SA_REQUIRE(n_rows > 0 && pairs > 0 && 2 * pairs <= D, "%s: a table of %d rows of %d pairs for head dim %d", fn, n_rows,
+             pairs, D);
+  SA_REQUIRE(skip >= 0 && skip <= L, "%s: skip=%d of %d tokens", fn, skip, L);
+  SA_REQUIRE(rows ? skip == 0 : L - skip <= n_rows, "%s: %d tokens after %d for %d table rows", fn, L - skip, skip, n_rows);
+  SA_REQUIRE(H + (int64_t)(k ? Hk : 0) < 65536, "%s: too many heads", fn);
+  SA_REQUIRE(reinterpret_cast<uintptr_t>(table) % 8 == 0, "%s: table not 8-byte aligned", fn);
+  RotArgs a;
+  a.x[0] = q; a.y[0] = q_out;
+  a.x[1] = k; a.y[1] = k_out;
+  a.heads[0] = H;
+  a.heads[1] = k ? Hk : 0;
+  const int size = dtype == SA_DTYPE_F32 ? 4 : 2;
+  bool wide = D % 8 == 0 && pairs % (halves ? 8 : 4) == 0 && reinterpret_cast<uintptr_t>(table) % 16 == 0;
+  for (int w = 0; w < (k ? 2 : 1); ++w)
+    for (int i = 0; i < 3; ++i) {
+      a.xs[w][i] = strides[6 * w + i];
+      a.ys[w][i] = strides[6 * w + 3 + i];
+      wide = wide && a.xs[w][i] * size % 16 == 0 && a.ys[w][i] * size % 16 == 0;
+    }
+  if (!k)
+    for (int i = 0; i < 3; ++i) a.xs[1][i] = a.ys[1][i] = 0;
+  for (const void* p : {q, (const void*)q_out, k, (const void*)k_out}) wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  a.B = B; a.L = L; a.D = D;
+  a.table = reinterpret_cast<const float2*>(table);
+  a.n_rows = n_rows;
+  a.pairs = pairs;
+  a.rows = rows;
+  a.rows_sb = rows_batch_stride;
+  a.skip = skip;
+  a.sign = inverse ? -1.f : 1.f;
+  // Each thread reads its values before it writes them, so that out may be the input itself.
+  a.copy = !(q == q_out && (!k || k == k_out));
+  hipStream_t s = sa::as_stream(stream);
+  if (dtype == SA_DTYPE_F32) return launch_rotary<float>(a, halves != 0, wide, s, fn);
+  if (dtype == SA_DTYPE_F16) return launch_rotary<_Float16>(a, halves != 0, wide, s, fn);
+  return launch_rotary<__bf16>(a, halves != 0, wide, s, fn);
+}

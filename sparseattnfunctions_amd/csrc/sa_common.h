@@ -61,6 +61,12 @@ int attn_f32_pooling(const float* q, const int64_t q_strides[3], const float* k,
                      int H, int L, int D, const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, int kv_rep,
                      bool causal, float sm_scale, int pool_cols, float* pool_r, float* pool_lse, void* terms_ws,
                      void* stream, const char* fn);
+// fp32 attention with the rows' log2-sum-exp2 (attn_f32.hip); workspace null or of attn_f32_terms_bytes.
+int attn_f32_lse(const float* q, const int64_t q_strides[3], const float* k, const int64_t k_strides[3],
+                 const float* v, const int64_t v_strides[3], float* out, const int64_t out_strides[3], int B, int H,
+                 int Lq, int Lk, int D, const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, float sm_scale,
+                 const int32_t* work_order, int64_t n_slots, void* workspace, int64_t workspace_bytes, float* lse,
+                 void* stream, const char* fn);
 // Bytes of the split-operand workspace of the fp32 attention (attn_f32.hip).
 int64_t attn_f32_terms_bytes(int B, int Hk, int Lk, int D);
 
