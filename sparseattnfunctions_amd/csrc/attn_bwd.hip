@@ -73,58 +73,6 @@ struct BwdArgs {
   float* stats;
 };
 
-// The first eight row operands of a step (16 bytes per lane each): four of each streamed matrix at the
-// lane's addresses a[s], kMat bytes apart.
-template <int kOff, int kMat>
-__device__ __forceinline__ void read_rows(const uint32_t (&a)[4], sa_u32x4v (&x)[4], sa_u32x4v (&y)[4]) {
-  asm volatile(
-      "ds_read_b128 %0, %8 offset:%12\n\tds_read_b128 %4, %8 offset:%13\n\t"
-      "ds_read_b128 %1, %9 offset:%12\n\tds_read_b128 %5, %9 offset:%13\n\t"
-      "ds_read_b128 %2, %10 offset:%12\n\tds_read_b128 %6, %10 offset:%13\n\t"
-      "ds_read_b128 %3, %11 offset:%12\n\tds_read_b128 %7, %11 offset:%13\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
-      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(kOff), "i"(kOff + kMat)
-      : "memory");
-}
-
-// 32 floats of a step's statistics: elements e of x and y are rows 8 (e / 4) + 4 hh + e % 4 of the
-// first and the second 32 floats (a: the stage's address + 16 hh).
-__device__ __forceinline__ void read_stats(uint32_t a, sa_u32x4v (&x)[4], sa_u32x4v (&y)[4]) {
-  asm volatile(
-      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:32\n\t"
-      "ds_read_b128 %2, %8 offset:64\n\tds_read_b128 %3, %8 offset:96\n\t"
-      "ds_read_b128 %4, %8 offset:128\n\tds_read_b128 %5, %8 offset:160\n\t"
-      "ds_read_b128 %6, %8 offset:192\n\tds_read_b128 %7, %8 offset:224\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
-      : "v"(a)
-      : "memory");
-}
-
-// Transposed operands of 64 columns of a step's 32 rows: r[dc][u] = the A operand of d chunk dc and
-// 16-row step u (two transposed reads each, at a[dc][0] and a[dc][1]).
-template <int kOff>
-__device__ __forceinline__ void read_transposed(const uint32_t (&a)[2][2], sa_u32x2v (&r)[2][2][2]) {
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %6, %10 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0][0][0]), "=&v"(r[0][0][1]), "=&v"(r[1][0][0]), "=&v"(r[1][0][1]), "=&v"(r[0][1][0]),
-        "=&v"(r[0][1][1]), "=&v"(r[1][1][0]), "=&v"(r[1][1][1])
-      : "v"(a[0][0]), "v"(a[0][1]), "v"(a[1][0]), "v"(a[1][1]), "i"(kOff), "i"(kOff + 2048)
-      : "memory");
-}
-
-__device__ inline sa_f32x16 as_f32x16(const sa_u32x4v (&x)[4]) {
-  sa_f32x16 r;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) r[e] = __uint_as_float(x[e >> 2][e & 3]);
-  return r;
-}
-
 // The two 16-bit values of a pair as floats.
 template <typename T>
 __device__ inline float2 unpack2(uint32_t w) {
@@ -161,7 +109,7 @@ __device__ inline const __attribute__((address_space(4))) int32_t* bwd_list(cons
 // kParts: pairs per workgroup, each on its share of the item's list; their sums are added in LDS, in
 // order, at the end.
 template <bool kKeys, bool kBias, typename T, int kD, int kParts>
-__global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
+__global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel(BwdArgs a) {
   typedef Elem<T> E;
   typedef typename E::v8 v8;
   constexpr int kDS = kD / 16;      // 16-wide d steps of the first products
@@ -171,8 +119,12 @@ __global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
   constexpr int kMat = kHalves * kRowTile;       // a step's rows of one matrix
   constexpr bool kStats = kKeys || kBias;
   constexpr int kAcc = kKeys ? 2 : 1;
-  __shared__ __attribute__((aligned(1024))) uint8_t tile_lds[kParts * 2 * 2 * kMat];
-  __shared__ __attribute__((aligned(256))) float stat_lds[kParts * 2 * 64];
+  constexpr int kRead = !kKeys && !kBias ? 4 : kKeys && kD == 128 ? 1 : 2;
+  constexpr bool kEarly = !kKeys || kD == 64;  // registers for the first transposed reads before the exponentials
+  // The two stages are separate objects, so that the compiler's waits tell reads of one from the
+  // copies into the other.
+  __shared__ __attribute__((aligned(1024))) uint8_t tile0[kParts * 2 * kMat], tile1[kParts * 2 * kMat];
+  __shared__ __attribute__((aligned(256))) float stat0[kParts * 64], stat1[kParts * 64];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -229,14 +181,12 @@ __global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
                               : static_cast<const uint16_t*>(a.st_b) + b * a.sb_sb + h * a.sb_sh;
   const uint32_t row_bytes = (uint32_t)(w == 0 ? a.sa_sl : a.sb_sl) * 2;
   const uint32_t st_bytes = (uint32_t)(a.L_st - 1) * row_bytes + 128;
-  uint32_t goff[2];
+  uint32_t goff[2];  // lane offsets of the copies of rows 0 .. 7 and 8 .. 15 (and of 16 .. 31 from row 16)
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
-    goff[p] = (lane >> 3) * row_bytes + 16 * ((lane & 7) ^ swz(8 * p + (lane >> 3)));
+  for (int j = 0; j < 2; ++j)
+    goff[j] = (8 * j + (lane >> 3)) * row_bytes + 16 * ((lane & 7) ^ swz(8 * j + (lane >> 3)));
   const float* stat_src = kKeys ? a.stats + (int64_t)bh * a.n_st * 128 : bias;
   const uint32_t stat_bytes = kKeys ? (uint32_t)a.n_st * 512 : (uint32_t)a.L_st * 4;
-  lds_u8* tile = (lds_u8*)tile_lds + part * 4 * kMat;
-  lds_u8* stat = (lds_u8*)stat_lds + part * 512;
 
   const int n_steps = 2 * cnt;
   const int per_part = (n_steps + kParts - 1) / kParts;
@@ -245,32 +195,39 @@ __global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
     const int s = beg + i;
     return i < per_part && s < n_steps ? list[s >> 1] : -1;
   };
-  auto issue = [&](int rb, int i) {
+  // Copies of the part's i-th step. The descriptors begin at the step's rows and end with the head's, so
+  // that rows past the last one read as zero and the lane offsets never change.
+  auto issue = [&](int rb, int i, lds_u8* tile, lds_u8* stat) __attribute__((always_inline)) {
     if ((unsigned)rb >= (unsigned)a.n_st) return;
     const uint32_t row0 = __builtin_amdgcn_readfirstlane(rb * kBlk + kStep * ((beg + i) & 1));
-    lds_u8* dst = tile + (i & 1) * 2 * kMat + w * kMat;
+    lds_u8* dst = tile + (part * 2 + w) * kMat;
 #pragma unroll
-    for (int hf = 0; hf < kHalves; ++hf) {
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(st + 64 * hf),
-                                                                            (short)0, (int)st_bytes, 0x00020000);
+    for (int r16 = 0; r16 < 2; ++r16) {
+      const uint32_t off = min((row0 + 16 * r16) * row_bytes, st_bytes);
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(st) + off;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_u8*)(dst + hf * kRowTile + 1024 * j), 16,
-                                                 (row0 + 8 * j) * row_bytes + goff[j & 1], 0, 0, 0);
+      for (int hf = 0; hf < kHalves; ++hf) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(from + 128 * hf), (short)0, (int)(st_bytes - off), 0x00020000);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_u8*)(dst + hf * kRowTile + 2048 * r16 + 1024 * j), 16,
+                                                   goff[j], 0, 0, 0);
+      }
     }
     if (kStats && w == 0) {
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(stat_src), (short)0,
-                                                                          (int)stat_bytes, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u8*)(stat + (i & 1) * 256), 4,
-                                               (kKeys ? row0 * 8 : row0 * 4) + 4 * lane, 0, 0, 0);
+      const uint32_t soff = min(kKeys ? row0 * 8 : row0 * 4, stat_bytes);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(stat_src) + soff), (short)0, (int)(stat_bytes - soff),
+          0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u8*)(stat + part * 256), 4, 4 * lane, 0, 0, 0);
     }
   };
 
   // Lane constants: row operand reads of chunk s and transposed reads (attn_fwd.hip's kro and vro).
-  const uint32_t tile_at = (uint32_t)(uintptr_t)tile, stat_at = (uint32_t)(uintptr_t)stat + 16 * hh;
-  uint32_t ro[4], to[2][2];
+  int ro[4], to[2][2];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) ro[s] = tile_at + 128 * col + 16 * ((2 * s + hh) ^ swz(col));
+  for (int s = 0; s < 4; ++s) ro[s] = part * 2 * kMat + 128 * col + 16 * ((2 * s + hh) ^ swz(col));
   {
     const int i = lane & 15, hq = lane >> 5, dg = (lane >> 4) & 1;
 #pragma unroll
@@ -279,7 +236,7 @@ __global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
       for (int t = 0; t < 2; ++t) {
         const int r = 8 * t + 4 * hq + (i >> 2);
         const int chunk = 4 * dc + 2 * dg + ((i & 3) >> 1);
-        to[dc][t] = tile_at + 128 * r + 16 * (chunk ^ swz(r)) + 8 * (i & 1);
+        to[dc][t] = part * 2 * kMat + 128 * r + 16 * (chunk ^ swz(r)) + 8 * (i & 1);
       }
   }
 
@@ -288,44 +245,66 @@ __global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
   for (int x = 0; x < kAcc; ++x)
 #pragma unroll
     for (int dc = 0; dc < kDC; ++dc) acc[x][dc] = sa_f32x16{};
+  sa_f32x16 less_delta;  // query pass: dP's accumulators start at -delta
+#pragma unroll
+  for (int e = 0; e < 16; ++e) less_delta[e] = -delta;
 
-  int rb = block_of(0);
-  issue(rb, 0);
-  int rb_next = block_of(1);
-  for (int i = 0; i < per_part; ++i) {
-    // This wave's copies of step i have landed, then everyone's; every wave is done with step i - 1,
-    // whose stage the copies of step i + 1 overwrite.
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    wg_barrier();
-    issue(rb_next, i + 1);
-    const int cur = rb;
-    rb = rb_next;
-    rb_next = block_of(i + 2);
-    if ((unsigned)cur >= (unsigned)a.n_st) continue;
-    const uint32_t stage = (i & 1) * 2 * kMat;
-    sa_f32x16 S = {}, dP = {};
-    if constexpr (kStats) {
-      sa_u32x4v x[4], y[4];
-      read_stats(stat_at + (i & 1) * 256, x, y);
-      S = as_f32x16(x);
-      if constexpr (kKeys) dP = as_f32x16(y);
-    }
-    sa_f32x16 kb2 = {};
-    if constexpr (!kKeys && kBias) {
-      kb2 = S;
-      S = sa_f32x16{};
-    }
+  auto compute = [&](int cur, int i, const lds_u8* tile, const float* stat) __attribute__((always_inline)) {
+    if ((unsigned)cur >= (unsigned)a.n_st) return;
+    const float* st_ = stat + part * 64 + 4 * hh;
+    auto stats = [&](int at) __attribute__((always_inline)) {  // 16 of the step's 32 statistics or biases
+      sa_f32x16 r;
 #pragma unroll
-    for (int hf = 0; hf < kHalves; ++hf) {
-      sa_u32x4v x[4], y[4];
-      const uint32_t at[4] = {ro[0] + stage, ro[1] + stage, ro[2] + stage, ro[3] + stage};
-      if (hf == 0) read_rows<0, kMat>(at, x, y);
-      else read_rows<kRowTile, kMat>(at, x, y);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        S = E::mfma(E::as8(x[s]), fa[4 * hf + s], S);
-        dP = E::mfma(E::as8(y[s]), fb[4 * hf + s], dP);
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 y = *reinterpret_cast<const float4*>(st_ + at + 8 * q4);
+        r[4 * q4] = y.x; r[4 * q4 + 1] = y.y; r[4 * q4 + 2] = y.z; r[4 * q4 + 3] = y.w;
       }
+      return r;
+    };
+    sa_f32x16 S = {}, dP = less_delta;
+    if constexpr (kKeys) {
+      S = stats(0);
+      dP = stats(32);
+    }
+    // Row operands in groups of kRead 16-column steps: a group's reads are issued while the products of
+    // the group before run, each of which waits for its own two.
+    sa_u32x4v x[kDS], y[kDS];
+    auto rows = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int s = s0; s < s0 + kRead; ++s) {
+        x[s] = lds_read_b128(tile + ro[s & 3] + (s >> 2) * kRowTile);
+        y[s] = lds_read_b128(tile + ro[s & 3] + (s >> 2) * kRowTile + kMat);
+      }
+    };
+    rows(0);
+#pragma unroll
+    for (int s0 = 0; s0 < kDS; s0 += kRead) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (s0 + kRead < kDS) rows(s0 + kRead);
+#pragma unroll
+      for (int s = s0; s < s0 + kRead; ++s) {
+        S = E::mfma(E::as8(x[s]), fa[s], S);
+        dP = E::mfma(E::as8(y[s]), fb[s], dP);
+      }
+    }
+    // Transposed operands of 64 columns: r[dc][u], requested before they are needed.
+    struct Trans {
+      uint2 r[2][2][2];
+    };
+    auto transposed = [&](int x, int hf) __attribute__((always_inline)) {
+      Trans t;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int dc = 0; dc < 2; ++dc)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) t.r[dc][u][j] = lds_read_tr16(tile + x * kMat + hf * kRowTile + 2048 * u + to[dc][j]);
+      return t;
+    };
+    Trans tr;
+    if constexpr (kEarly) {
+      tr = transposed(kAcc - 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
     // Elements e: streamed row 8 (e / 4) + 4 hh + e % 4 of the step, own row col.
     uint32_t Pp[8], Sp[8];
@@ -338,41 +317,58 @@ __global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
         Sp[e >> 1] = E::pack(p0 * dP[e], p1 * dP[e + 1]);
       }
     } else {
+      sa_f32x16 kb2 = {};
+      if constexpr (kBias) kb2 = stats(0);
       const int row0 = cur * kBlk + kStep * ((beg + i) & 1);
-      float p[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        p[e] = fast_exp2(fmaf(S[e], a.scale_log2, kBias ? fmaf(kb2[e], kLog2e, -lse) : -lse));
-      if (row0 + kStep > a.L_st) {  // keys past the last one
+      if (row0 + kStep > a.L_st) {  // keys past the last one: P = 0
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (row0 + 8 * (e >> 2) + 4 * hh + (e & 3) >= a.L_st) p[e] = 0.f;
+          if (row0 + 8 * (e >> 2) + 4 * hh + (e & 3) >= a.L_st) S[e] = -INFINITY;
       }
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) Sp[e >> 1] = E::pack(p[e] * (dP[e] - delta), p[e + 1] * (dP[e + 1] - delta));
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = fast_exp2(fmaf(S[e], a.scale_log2, kBias ? fmaf(kb2[e], kLog2e, -lse) : -lse));
+        const float p1 = fast_exp2(fmaf(S[e + 1], a.scale_log2, kBias ? fmaf(kb2[e + 1], kLog2e, -lse) : -lse));
+        Sp[e >> 1] = E::pack(p0 * dP[e], p1 * dP[e + 1]);
+      }
     }
+    if constexpr (!kEarly) tr = transposed(kAcc - 1, 0);
+    // st_b^T P first: P is ready first.
 #pragma unroll
-    for (int x = kAcc - 1; x >= 0; --x)  // st_b^T P first: P is ready first
+    for (int j = 0; j < kAcc * kHalves; ++j) {
+      const int x = kAcc - 1 - j / kHalves, hf = j % kHalves;
+      const Trans now = tr;
+      if (j + 1 < kAcc * kHalves) tr = transposed(kAcc - 1 - (j + 1) / kHalves, (j + 1) % kHalves);
+      const uint32_t(&P)[8] = x == 0 ? Sp : Pp;
 #pragma unroll
-      for (int hf = 0; hf < kHalves; ++hf) {
-        const uint32_t at[2][2] = {{to[0][0] + stage, to[0][1] + stage}, {to[1][0] + stage, to[1][1] + stage}};
-        sa_u32x2v r[2][2][2];
-        if (x == 0) {
-          if (hf == 0) read_transposed<0>(at, r);
-          else read_transposed<kRowTile>(at, r);
-        } else {
-          if (hf == 0) read_transposed<kMat>(at, r);
-          else read_transposed<kMat + kRowTile>(at, r);
-        }
-        const uint32_t(&P)[8] = x == 0 ? Sp : Pp;
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int dc = 0; dc < 2; ++dc)
-            acc[x][2 * hf + dc] = E::mfma(
-                E::as8(sa_u32x4v{r[dc][u][0].x, r[dc][u][0].y, r[dc][u][1].x, r[dc][u][1].y}),
-                E::as8(sa_u32x4v{P[4 * u], P[4 * u + 1], P[4 * u + 2], P[4 * u + 3]}), acc[x][2 * hf + dc]);
-      }
+        for (int dc = 0; dc < 2; ++dc)
+          acc[x][2 * hf + dc] = E::mfma(
+              E::as8(sa_u32x4v{now.r[dc][u][0].x, now.r[dc][u][0].y, now.r[dc][u][1].x, now.r[dc][u][1].y}),
+              E::as8(sa_u32x4v{P[4 * u], P[4 * u + 1], P[4 * u + 2], P[4 * u + 3]}), acc[x][2 * hf + dc]);
+    }
+  };
+
+  lds_u8* const t0 = (lds_u8*)tile0;
+  lds_u8* const t1 = (lds_u8*)tile1;
+  int rb = block_of(0);
+  issue(rb, 0, t0, (lds_u8*)stat0);
+  int rb_next = block_of(1);
+  for (int i = 0; i < per_part; i += 2) {
+    // This wave's copies of step i have landed, then everyone's; every wave is done with step i - 1,
+    // whose stage the copies of step i + 1 overwrite.
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    wg_barrier();
+    issue(rb_next, i + 1, t1, (lds_u8*)stat1);
+    compute(rb, i, t0, stat0);
+    if (i + 1 >= per_part) break;
+    rb = block_of(i + 2);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    wg_barrier();
+    issue(rb, i + 2, t0, (lds_u8*)stat0);
+    compute(rb_next, i + 1, t1, stat1);
+    rb_next = block_of(i + 3);
   }
 
   // ---- Results: element 4 q4 + j of acc[x][dc] is d = 32 dc + 8 q4 + 4 hh + j of own row col.
@@ -395,9 +391,14 @@ __global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
       }
     } else {
       constexpr int kCh = kD / 4;  // 16-byte chunks of a row of sums
-      float* sums = reinterpret_cast<float*>(tile_lds);  // [part][64 rows][kD], chunks swizzled by the row
+      // [part][64 rows][kD] sums, chunks swizzled by the row: the first half of the parts over one stage,
+      // the others over the other one.
+      auto sums = [&](int p) {
+        return reinterpret_cast<float*>(p < kParts / 2 ? tile0 : tile1) + (p % (kParts / 2)) * kBlk * kD;
+      };
+      static_assert(kParts == 1 || kParts / 2 * kBlk * kD * 4 <= kParts * 2 * kMat, "the sums fit a stage");
       __syncthreads();  // every wave is done with the stages (x = 0) or with the last sums
-      float* mine = sums + (part * kBlk + kStep * w + col) * kD;
+      float* mine = sums(part) + (kStep * w + col) * kD;
 #pragma unroll
       for (int dc = 0; dc < kDC; ++dc)
 #pragma unroll
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(128 * kParts, 2) void bsa_bwd_kernel(BwdArgs a) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int p = 0; p < kParts; ++p) {
-          const float4 y = *reinterpret_cast<const float4*>(sums + (p * kBlk + r) * kD + 4 * (ch ^ (r & 31 & (kCh - 1))));
+          const float4 y = *reinterpret_cast<const float4*>(sums(p) + r * kD + 4 * (ch ^ (r & 31 & (kCh - 1))));
           s.x += y.x;
           s.y += y.y;
           s.z += y.z;
