@@ -109,7 +109,7 @@ __device__ inline const __attribute__((address_space(4))) int32_t* bwd_list(cons
 // kParts: pairs per workgroup, each on its share of the item's list; their sums are added in LDS, in
 // order, at the end.
 template <bool kKeys, bool kBias, typename T, int kD, int kParts>
-__global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel(BwdArgs a) {
+__global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void bsa_bwd_kernel(BwdArgs a) {
   typedef Elem<T> E;
   typedef typename E::v8 v8;
   constexpr int kDS = kD / 16;      // 16-wide d steps of the first products
@@ -582,19 +582,38 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   }
 }
 
+template <bool kKeys, typename T, int kD, int kParts>
+void launch_parts(const BwdArgs& a, hipStream_t s) {
+  const int64_t groups = (a.n_slots + 3) / 4;
+  const dim3 grid((unsigned)((groups + 7) / 8 * 32)), blk(128 * kParts);
+  if (a.bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, kParts>), grid, blk, 0, s, a);
+  else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, kParts>), grid, blk, 0, s, a);
+}
+
+// Pairs per item, by the number of items and the lists' width (how many entries they hold the host does
+// not know). One, two or four pairs, us of the query pass (the key pass is alike):
+//   head dim 64, dense lists of 40: 40 items 41 / 23 / 19, 160 43 / 24 / 21, 320 47 / 32 / 40, 1 280
+//     93 / 86 / 107, 1 920 141 / 132 / 166; of 10: 40 items 13.8 / 10.3 / 10.6, 640 20 / 20 / 28, 1 500
+//     33 / 36 / 55; lists of 5 of 40: 640 items 19 / 17 / 24, 1 920 32 / 33 / 59, 3 200 45 / 51 / 93;
+//     28 of 278: 278 items 51 / 30 / 34, 2 224 120 / 115 / 154;
+//   head dim 128, dense lists of 40: 40 items 60 / 38 / 36, 160 62 / 41 / 37, 320 82 / 59 / 73, 640 98 / 100 /
+//     112, 1 280 178 / 165 / 203, 1 920 239 / 245 / 299; of 10: 320 27 / 24 / 33, 640 34 / 37 / 50; 28 of
+//     278: 1 112 139 / 125 / 149, 2 224 225 / 232 / 275.
+// (Lists much longer than the others, of text blocks say, gain further by a second pair: [1, 15, 17776,
+// 64] with 4 of 278 blocks dense 449 / 431 us.)
+int pairs_per_item(int n_items, int max_cnt, int D) {
+  if (n_items <= 160 && max_cnt >= 32) return 4;
+  if (D == 64) return n_items > 768 && max_cnt <= 16 ? 1 : 2;
+  return n_items <= 512 || (n_items <= 1536 && max_cnt >= 32) ? 2 : 1;
+}
+
 template <bool kKeys, typename T, int kD>
 void launch_pass(const BwdArgs& a, hipStream_t s) {
-  const int64_t groups = (a.n_slots + 3) / 4;
-  const unsigned wgs = (unsigned)((groups + 7) / 8 * 32);
-  const bool bias = a.bias != nullptr;
-  const bool parts = a.n_items <= 512;
-  if (parts) {
-    if (bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, 4>), dim3(wgs), dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, 4>), dim3(wgs), dim3(512), 0, s, a);
-  } else {
-    if (bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, 1>), dim3(wgs), dim3(128), 0, s, a);
-    else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, 1>), dim3(wgs), dim3(128), 0, s, a);
-  }
+  // (a key block's list is as long as there are query blocks, at most)
+  const int parts = pairs_per_item(a.n_items, kKeys ? a.n_st : a.max_cnt, kD);
+  if (parts == 4) launch_parts<kKeys, T, kD, 4>(a, s);
+  else if (parts == 2) launch_parts<kKeys, T, kD, 2>(a, s);
+  else launch_parts<kKeys, T, kD, 1>(a, s);
 }
 
 template <bool kKeys>

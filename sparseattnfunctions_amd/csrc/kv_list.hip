@@ -93,16 +93,20 @@ __global__ __launch_bounds__(256) void mask_cells_to_list_kernel(CellArgs a) {
   if (lane == 0) a.kv_cnt[row] = total;
 }
 
-// Transposed lists. One workgroup per (head, 64 key blocks): a first walk over the head's lists counts
-// the entries below its key blocks and of each of them, which gives where their lists begin; a second
-// walk, 128 query blocks at a time, counts each pair in LDS and writes the key blocks' entries in
-// ascending order of the query block, an entry as often as it is listed.
+// Transposed lists. One workgroup per (head, 64 key blocks): a walk over the head's lists counts the
+// entries below its key blocks and of each of them, which gives where their lists begin; each pair's
+// count is kept in LDS, for 512 query blocks at a time (the first 512 in that same walk), and from
+// there the key blocks' entries are written in ascending order of the query block, an entry as often as
+// it is listed. Bound by the latency of the walk: sixteen waves, four rows' loads in flight in each
+// ([1, 15, 17776], 59 of 278 blocks: 102 us with four waves, one row each and two walks).
 constexpr int kWin = 64;        // key blocks per workgroup
-constexpr int kRowChunk = 128;  // query blocks per pass: 64 words of two 16-bit counts
-__global__ __launch_bounds__(256) void transpose_lists_kernel(const int32_t* __restrict__ kv_idx,
-                                                              const int32_t* __restrict__ kv_cnt, int nqb, int nkb,
-                                                              int max_cnt, int n_win, int32_t* __restrict__ q_beg,
-                                                              int32_t* __restrict__ q_idx) {
+constexpr int kRowChunk = 512;  // query blocks per pass: words of two 16-bit counts
+constexpr int kTransWaves = 16;
+__global__ __launch_bounds__(64 * kTransWaves) void transpose_lists_kernel(const int32_t* __restrict__ kv_idx,
+                                                                           const int32_t* __restrict__ kv_cnt, int nqb,
+                                                                           int nkb, int max_cnt, int n_win,
+                                                                           int32_t* __restrict__ q_beg,
+                                                                           int32_t* __restrict__ q_idx) {
   __shared__ int hist[kWin], pos[kWin], below;
   __shared__ uint32_t seen[kWin][kRowChunk / 2 + 1];
   const int64_t bh = blockIdx.x / n_win;
@@ -111,20 +115,41 @@ __global__ __launch_bounds__(256) void transpose_lists_kernel(const int32_t* __r
   const int32_t* idx = kv_idx + bh * nqb * max_cnt;
   const int32_t* cnt = kv_cnt + bh * nqb;
   int32_t* out = q_idx + bh * nqb * max_cnt;
+  auto clear = [&]() {
+    for (int i = threadIdx.x; i < kWin * (kRowChunk / 2 + 1); i += 64 * kTransWaves) (&seen[0][0])[i] = 0;
+  };
+  // take(row, key block) for every entry of rows [r0, r1).
+  auto walk = [&](int r0, int r1, auto take) __attribute__((always_inline)) {
+    for (int r = r0 + 4 * wave; r < r1; r += 4 * kTransWaves) {
+      int n[4], most = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        n[u] = r + u < r1 ? min(max(cnt[r + u], 0), max_cnt) : 0;
+        most = max(most, n[u]);
+      }
+      for (int j = lane; j - lane < most; j += 64) {
+        int kb[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) kb[u] = j < n[u] ? idx[(int64_t)(r + u) * max_cnt + j] : -1;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if ((unsigned)kb[u] < (unsigned)nkb) take(r + u, kb[u]);
+      }
+    }
+  };
+  auto mark = [&](int row, int kb) {
+    if (kb >= kb0 && kb < kb0 + kWin) atomicAdd(&seen[kb - kb0][row >> 1], (row & 1) ? 0x10000u : 1u);
+  };
   if (threadIdx.x < kWin) hist[threadIdx.x] = 0;
   if (threadIdx.x == 0) below = 0;
+  clear();
   __syncthreads();
   int before = 0;
-  for (int r = wave; r < nqb; r += 4) {
-    const int n = min(max(cnt[r], 0), max_cnt);
-    const int32_t* list = idx + (int64_t)r * max_cnt;
-    for (int j = lane; j < n; j += 64) {
-      const int kb = list[j];
-      if ((unsigned)kb >= (unsigned)nkb) continue;
-      if (kb < kb0) ++before;
-      else if (kb < kb0 + kWin) atomicAdd(&hist[kb - kb0], 1);
-    }
-  }
+  walk(0, nqb, [&](int row, int kb) {
+    if (kb < kb0) ++before;
+    else if (kb < kb0 + kWin) atomicAdd(&hist[kb - kb0], 1);
+    if (row < kRowChunk) mark(row, kb);
+  });
   if (before) atomicAdd(&below, before);
   __syncthreads();
   if (wave == 0) {
@@ -141,32 +166,32 @@ __global__ __launch_bounds__(256) void transpose_lists_kernel(const int32_t* __r
     if (kb0 + lane == nkb - 1) beg[nkb] = below + sum;
   }
   for (int r0 = 0; r0 < nqb; r0 += kRowChunk) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kWin * (kRowChunk / 2); i += 256) seen[i >> 6][i & 63] = 0;
-    __syncthreads();
-    for (int r = r0 + wave; r < min(nqb, r0 + kRowChunk); r += 4) {
-      const int n = min(max(cnt[r], 0), max_cnt);
-      const int32_t* list = idx + (int64_t)r * max_cnt;
-      for (int j = lane; j < n; j += 64) {
-        const int kb = list[j];
-        if (kb >= kb0 && kb < min(kb0 + kWin, nkb)) atomicAdd(&seen[kb - kb0][(r - r0) >> 1], (r & 1) ? 0x10000u : 1u);
-      }
+    if (r0 > 0) {
+      __syncthreads();
+      clear();
+      __syncthreads();
+      walk(r0, min(nqb, r0 + kRowChunk), [&](int row, int kb) { mark(row - r0, kb); });
     }
     __syncthreads();
-    for (int k = wave; k < min(kWin, nkb - kb0); k += 4) {
-      const uint32_t word = seen[k][lane];
-      const int n0 = word & 0xffff, n1 = word >> 16;
-      int sum = n0 + n1;
+    for (int k = wave; k < min(kWin, nkb - kb0); k += kTransWaves) {
+      // lane l: rows r0 + 2 (l + 64 i), + 1 of word l + 64 i, in order of i
+      int at = pos[k];
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(sum, o);
-        if (lane >= o) sum += y;
+      for (int i = 0; i < kRowChunk / 128; ++i) {
+        const uint32_t word = seen[k][64 * i + lane];
+        const int n0 = word & 0xffff, n1 = word >> 16;
+        int sum = n0 + n1;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int y = __shfl_up(sum, o);
+          if (lane >= o) sum += y;
+        }
+        int p = at + sum - n0 - n1;
+        for (int j = 0; j < n0; ++j) out[p++] = r0 + 2 * (64 * i + lane);
+        for (int j = 0; j < n1; ++j) out[p++] = r0 + 2 * (64 * i + lane) + 1;
+        at += __shfl(sum, 63);
       }
-      const int first = pos[k];
-      int at = first + sum - n0 - n1;
-      for (int i = 0; i < n0; ++i) out[at++] = r0 + 2 * lane;
-      for (int i = 0; i < n1; ++i) out[at++] = r0 + 2 * lane + 1;
-      if (lane == 63) pos[k] = first + sum;
+      if (lane == 0) pos[k] = at;
     }
   }
 }
@@ -242,7 +267,7 @@ extern "C" int sa_kv_list_transpose(const int32_t* kv_idx, const int32_t* kv_cnt
   const int n_win = (nkb + kWin - 1) / kWin;
   const int64_t blocks = (int64_t)BH * n_win;
   SA_REQUIRE(blocks < (1LL << 31), "%s: too many lists", fn);
-  hipLaunchKernelGGL(transpose_lists_kernel, dim3((unsigned)blocks), dim3(256), 0, sa::as_stream(stream), kv_idx, kv_cnt,
+  hipLaunchKernelGGL(transpose_lists_kernel, dim3((unsigned)blocks), dim3(64 * kTransWaves), 0, sa::as_stream(stream), kv_idx, kv_cnt,
                      nqb, nkb, max_cnt, n_win, q_beg, q_idx);
   return sa::check_launch(fn);
 }

@@ -100,7 +100,9 @@ def _forward(q, k, v, kv: KVList, sm_scale: float, key_bias, n_text_blocks: int)
         if parts > 1:
             ws = torch.empty(split_workspace_bytes(B * H * nqb, D, parts), dtype=torch.uint8, device=q.device)
     if parts == 1:
-        share_text = q.dtype != torch.float32 and shares_text_rows(B * H * nqb, kv.nkb, n_text_blocks, kv.row_blocks, D)
+        # (lists of unknown length count as short beside the text rows')
+        row_blocks = kv.row_blocks if kv.row_blocks is not None else 0.0
+        share_text = q.dtype != torch.float32 and shares_text_rows(B * H * nqb, kv.nkb, n_text_blocks, row_blocks, D)
         order = work_order(B, H, nqb, n_text_blocks, q.device, share_text)
     bias_ptr, bias_strides = _bias_args(key_bias)
     with _lib.on(q.device):
