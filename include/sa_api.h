@@ -228,26 +228,59 @@ int sa_block_sparse_fwd_f32_terms(const float* q, const int64_t q_strides[3], co
 
 /*
  * Training. The reference kernel has no backward pass (its autograd function raises
- * NotImplementedError, utils/block_sparse_attn_kernel.py:278-281); these three calls are one.
- *
- * sa_block_sparse_fwd_lse: sa_block_sparse_fwd (dtype SA_DTYPE_BF16), sa_block_sparse_fwd_f16
- * (SA_DTYPE_F16) or the fp32 attention (SA_DTYPE_F32), same arguments and output bits, that also
- * stores each row's log2-sum-exp2 of its scores times log2(e): lse fp32 [B*H][64*ceil(Lq/64)],
- * +inf for rows without a key (empty lists, keys all biased to -inf) and past Lq.
- *   parts, workspace  16-bit: as sa_block_sparse_fwd_split (1: none; > 1 plain lists only, work_order
- *             is not read). fp32: parts = 1, workspace NULL (sa_block_sparse_fwd_f32) or as for
- *             sa_block_sparse_fwd_f32_terms; key_bias must be NULL.
+ * NotImplementedError, utils/block_sparse_attn_kernel.py:278-281); sa_block_sparse_fwd_lse and
+ * sa_block_sparse_bwd are a differentiable call of it. Both read one description of the call (pointers on
+ * the device but for the struct itself, which is read before they return):
  */
-int sa_block_sparse_fwd_lse(int dtype, const void* q, const int64_t q_strides[3], const void* k,
-                            const int64_t k_strides[3], const void* v, const int64_t v_strides[3], void* out,
-                            const int64_t out_strides[3], int B, int H, int Lq, int Lk, int D,
-                            const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, const float* key_bias,
-                            const int64_t bias_strides[2], float sm_scale, const int32_t* work_order,
-                            int64_t n_slots, int parts, void* workspace, int64_t workspace_bytes, float* lse,
-                            void* stream);
+typedef struct sa_attn_train {
+  int32_t dtype;       /* SA_DTYPE_*: of q .. dv */
+  int32_t B, H, Lq, Lk, D;
+  int32_t max_cnt;     /* width of the kv lists */
+  int32_t parts;       /* forward, 16-bit: key-range parts as sa_block_sparse_fwd_split has them, 1: none */
+  const void *q, *k, *v;
+  void* out;           /* forward: written; backward: read */
+  const void* dout;    /* gradient of out */
+  void *dq, *dk, *dv;  /* each nullable: not computed */
+  int64_t strides[24]; /* {b, h, l} in elements of q, k, v, out, dout, dq, dk, dv */
+  float* lse;          /* [B*H][64*ceil(Lq/64)]; forward: written; backward: read */
+  const int32_t *kv_idx, *kv_cnt;
+  const float* key_bias; /* nullable; not with fp32 */
+  int64_t bias_strides[2];
+  const int32_t* fwd_order; /* nullable dispatch order of the forward pass (not read with parts > 1), */
+  int64_t n_fwd_slots;      /* as sa_block_sparse_fwd's work_order */
+  const int32_t* q_order;   /* nullable dispatch orders of the backward pass: sa_attn_work_order of */
+  int64_t n_q_slots;        /* ceil(Lq/64) query blocks */
+  const int32_t* k_order;   /* and of ceil(Lk/64) key blocks per head */
+  int64_t n_k_slots;
+  void* workspace;          /* of the call that is made, 256-byte aligned */
+  int64_t workspace_bytes;
+  float sm_scale;
+} sa_attn_train;
 
 /*
- * Transposed kv lists: for each head the query blocks that list each key block, ascending.
+ * sa_block_sparse_fwd (bf16), sa_block_sparse_fwd_f16 or the fp32 attention, same contract and output
+ * bits, that also stores each row's log2-sum-exp2 of its scores times log2(e): +inf for rows without a
+ * key (empty lists, keys all biased to -inf) and past Lq. Reads neither dout nor the gradients.
+ *   workspace 16-bit: sa_attn_split_workspace bytes with parts > 1, else unused. fp32: NULL
+ *             (sa_block_sparse_fwd_f32) or as for sa_block_sparse_fwd_f32_terms.
+ */
+int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
+
+/*
+ * dq, dk, dv for the gradient dout of out, the probabilities recomputed from lse: P = exp2(score -
+ * lse), dS = P * (dout v^T - rowsum(dout * out)), dq = sm_scale dS k, dk = sm_scale dS^T q, dv = P^T
+ * dout. Rows and keys in no list get zeros; a block that a row lists twice counts twice. Sums are fp32 in a
+ * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type.
+ *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype and max_cnt): the query
+ *             rows' statistics, the transposed lists, sums of lists split over workgroups.
+ * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv.
+ */
+int sa_block_sparse_bwd_workspace(const sa_attn_train* call, int64_t* bytes);
+int sa_block_sparse_bwd(const sa_attn_train* call, void* stream);
+
+/*
+ * Transposed kv lists, as sa_block_sparse_bwd uses them: for each head the query blocks that list each
+ * key block, ascending.
  *   kv_idx, kv_cnt  lists of BH * nqb rows (counts clamped to [0, max_cnt], entries outside [0, nkb)
  *             skipped); max_cnt at most 65535.
  *   q_beg     int32 [BH][nkb + 1]: key block j's entries are q_idx[bh][q_beg[j] .. q_beg[j + 1]).
@@ -255,28 +288,6 @@ int sa_block_sparse_fwd_lse(int dtype, const void* q, const int64_t q_strides[3]
  */
 int sa_kv_list_transpose(const int32_t* kv_idx, const int32_t* kv_cnt, int BH, int nqb, int nkb, int max_cnt,
                          int32_t* q_beg, int32_t* q_idx, void* stream);
-
-/*
- * Gradients of sa_block_sparse_fwd_lse: dq, dk, dv for the gradient dout of out, the probabilities
- * recomputed from lse (P = exp2(score - lse), dS = P * (dout v^T - rowsum(dout * out)), dq =
- * sm_scale dS k, dk = sm_scale dS^T q, dv = P^T dout). Rows and keys in no list get zeros. Sums are
- * fp32 in a fixed order: results repeat bit for bit. 16-bit types round P and dS to the type.
- *   dq, dk, dv  each nullable (not computed); NULL dk and dv need no transposed lists.
- *   strides   8 triples {b, h, l}: q, k, v, out, dout, dq, dk, dv.
- *   q_beg, q_idx  the transposed lists.
- *   q_order, k_order  nullable dispatch orders of the query blocks and the key blocks
- *             (sa_attn_work_order for B, H and their number).
- *   workspace sa_block_sparse_bwd_workspace bytes, 256-byte aligned: the query rows' statistics.
- * Rows of one head of q, k, v and dout span less than 2 GiB. No key_bias with fp32.
- */
-int sa_block_sparse_bwd_workspace(int B, int H, int Lq, int64_t* bytes);
-int sa_block_sparse_bwd(int dtype, const void* q, const void* k, const void* v, const void* out,
-                        const void* dout, const float* lse, void* dq, void* dk, void* dv,
-                        const int64_t strides[24], int B, int H, int Lq, int Lk, int D, const int32_t* kv_idx,
-                        const int32_t* kv_cnt, int max_cnt, const int32_t* q_beg, const int32_t* q_idx,
-                        const float* key_bias, const int64_t bias_strides[2], float sm_scale,
-                        const int32_t* q_order, int64_t n_q_slots, const int32_t* k_order, int64_t n_k_slots,
-                        void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Rotary positions (the host model's part of the attention call: its processors receive q and k that

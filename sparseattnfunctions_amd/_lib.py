@@ -27,6 +27,17 @@ _I = ctypes.c_int
 _I64P = ctypes.POINTER(ctypes.c_int64)
 _F = ctypes.c_float
 
+
+class AttnTrain(ctypes.Structure):
+    """sa_attn_train of include/sa_api.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "B", "H", "Lq", "Lk", "D", "max_cnt", "parts")]
+                + [(n, _P) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")]
+                + [("strides", ctypes.c_int64 * 24)] + [(n, _P) for n in ("lse", "kv_idx", "kv_cnt", "key_bias")]
+                + [("bias_strides", ctypes.c_int64 * 2), ("fwd_order", _P), ("n_fwd_slots", ctypes.c_int64),
+                   ("q_order", _P), ("n_q_slots", ctypes.c_int64), ("k_order", _P), ("n_k_slots", ctypes.c_int64),
+                   ("workspace", _P), ("workspace_bytes", ctypes.c_int64), ("sm_scale", _F)])
+
+
 # name -> (restype, argtypes); must match include/sa_api.h.
 _PROTOTYPES = {
     "sa_abi_version": (_I, []),
@@ -63,18 +74,10 @@ _PROTOTYPES = {
         [_P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, ctypes.c_int64, _P,
          ctypes.c_int64, _P],
     ),
-    "sa_block_sparse_fwd_lse": (
-        _I,
-        [_I, _P, _I64P, _P, _I64P, _P, _I64P, _P, _I64P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I64P, _F, _P,
-         ctypes.c_int64, _I, _P, ctypes.c_int64, _P, _P],
-    ),
+    "sa_block_sparse_fwd_lse": (_I, [ctypes.POINTER(AttnTrain), _P]),
     "sa_kv_list_transpose": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
-    "sa_block_sparse_bwd_workspace": (_I, [_I, _I, _I, _I64P]),
-    "sa_block_sparse_bwd": (
-        _I,
-        [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _P, _I64P, _F, _P,
-         ctypes.c_int64, _P, ctypes.c_int64, _P, ctypes.c_int64, _P],
-    ),
+    "sa_block_sparse_bwd_workspace": (_I, [ctypes.POINTER(AttnTrain), _I64P]),
+    "sa_block_sparse_bwd": (_I, [ctypes.POINTER(AttnTrain), _P]),
     "sa_rotary_table": (_I, [_P, _I, _I64P, ctypes.c_int64, _I, _P, _P, _P, _P, _P]),
     "sa_rotary_apply": (
         _I,

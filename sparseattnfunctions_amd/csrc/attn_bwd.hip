@@ -26,6 +26,7 @@
 // costs two products, an exp2 and its share of two roundings.
 #include <math.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -71,6 +72,10 @@ struct BwdArgs {
   // [bh][2 * query blocks][2][32]: per 32 query rows their -lse / scale_log2, then their -delta. Written
   // by the query pass, read by the key pass.
   float* stats;
+  // More than one split: workgroup (item, blockIdx.y) computes the split's share of the item's steps and
+  // stores its sums to partial[item][split][result][64][kD]; bwd_merge_kernel adds them in order.
+  int splits;
+  float* partial;
 };
 
 // The two 16-bit values of a pair as floats.
@@ -165,7 +170,7 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void 
     }
     delta = xhalf_sum(delta);
     lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col];
-    if (part == 0) {
+    if (part == 0 && blockIdx.y == 0) {
       const bool row_ok = own_row < a.L_own;
       const float v = hh == 0 ? -lse * a.inv_scale_log2 : -delta;
       a.stats[(((int64_t)bh * a.n_own + blk) * 2 + w) * 64 + lane] = row_ok ? v : hh == 0 ? -INFINITY : 0.f;
@@ -188,9 +193,11 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void 
   const float* stat_src = kKeys ? a.stats + (int64_t)bh * a.n_st * 128 : bias;
   const uint32_t stat_bytes = kKeys ? (uint32_t)a.n_st * 512 : (uint32_t)a.L_st * 4;
 
-  const int n_steps = 2 * cnt;
-  const int per_part = (n_steps + kParts - 1) / kParts;
-  const int beg = part * per_part;
+  // The split's share of the 2 cnt steps, of it the part's.
+  const int per_split = (2 * cnt + a.splits - 1) / a.splits;
+  const int n_steps = min(2 * cnt, per_split * ((int)blockIdx.y + 1));
+  const int per_part = (per_split + kParts - 1) / kParts;
+  const int beg = (int)blockIdx.y * per_split + part * per_part;
   auto block_of = [&](int i) -> int {  // the streamed block of the part's i-th step, -1: none
     const int s = beg + i;
     return i < per_part && s < n_steps ? list[s >> 1] : -1;
@@ -419,7 +426,10 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void 
           s.z += y.z;
           s.w += y.w;
         }
-        if (g && blk * kBlk + r < a.L_own)
+        if (a.splits > 1)
+          *reinterpret_cast<float4*>(a.partial + ((((int64_t)item * a.splits + blockIdx.y) * kAcc + x) * kBlk + r) * kD +
+                                     4 * ch) = s;
+        else if (g && blk * kBlk + r < a.L_own)
           *reinterpret_cast<uint2*>(g + b * sb + h * sh + (int64_t)(blk * kBlk + r) * sl + 4 * ch) =
               make_uint2(E::pack(s.x * f, s.y * f), E::pack(s.z * f, s.w * f));
       }
@@ -478,7 +488,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
     }
     delta = xhalf_sum(delta);
     lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * half + col];
-    if (wave == 0) {
+    if (wave == 0 && blockIdx.y == 0) {
       const bool row_ok = own_row < a.L_own;
       // (the key pass takes lse as it is here: its element costs a fused multiply-add either way)
       const float v = hh == 0 ? -lse : -delta;
@@ -494,7 +504,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   for (int x = 0; x < kAcc; ++x)
 #pragma unroll
     for (int dc = 0; dc < kDC; ++dc) acc[x][dc] = sa_f32x16{};
-  for (int i = wave; i < 2 * cnt; i += 4) {
+  for (int i = wave + 4 * blockIdx.y; i < 2 * cnt; i += 4 * a.splits) {
     const int rb = list[i >> 1];
     if ((unsigned)rb >= (unsigned)a.n_st) continue;
     const int row0 = rb * kBlk + kStep * (i & 1);
@@ -575,17 +585,61 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
         s.w += y.w;
       }
       const int row = blk * kBlk + kStep * half + r;
-      if (g && row < a.L_own)
+      if (a.splits > 1)
+        *reinterpret_cast<float4*>(a.partial + ((((int64_t)item * a.splits + blockIdx.y) * kAcc + x) * kBlk + kStep * half + r) * kD +
+                                   4 * ch) = s;
+      else if (g && row < a.L_own)
         *reinterpret_cast<float4*>(g + b * gsb + h * gsh + (int64_t)row * gsl + 4 * ch) =
             make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
     }
   }
 }
 
+// Gradients from the splits' sums, in order: one workgroup per item and result.
+template <bool kKeys, typename T>
+__global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
+  constexpr int kAcc = kKeys ? 2 : 1;
+  const int item = blockIdx.x, x = blockIdx.y;
+  const int bh = item / a.n_own;
+  const int blk = item - bh * a.n_own;
+  const int b = bh / a.H;
+  const int h = bh - b * a.H;
+  T* g = static_cast<T*>(x == 0 ? a.grad_a : a.grad_b);
+  if (!g) return;
+  g += b * (x == 0 ? a.ga_sb : a.gb_sb) + h * (x == 0 ? a.ga_sh : a.gb_sh);
+  const int64_t sl = x == 0 ? a.ga_sl : a.gb_sl;
+  const float f = x == 0 ? a.sm_scale : 1.f;
+  const int64_t n = (int64_t)kBlk * D;
+  const float* from = a.partial + ((int64_t)item * a.splits * kAcc + x) * n;
+  for (int t = threadIdx.x; t < kBlk * D / 4; t += 256) {
+    const int r = t / (D / 4), d = 4 * (t % (D / 4));
+    if (blk * kBlk + r >= a.L_own) break;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < a.splits; ++p) {
+      const float4 y = *reinterpret_cast<const float4*>(from + (int64_t)p * kAcc * n + 4 * t);
+      s.x += y.x;
+      s.y += y.y;
+      s.z += y.z;
+      s.w += y.w;
+    }
+    T* o = g + (int64_t)(blk * kBlk + r) * sl + d;
+    if constexpr (std::is_same<T, float>::value)
+      *reinterpret_cast<float4*>(o) = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+    else
+      *reinterpret_cast<uint2*>(o) = make_uint2(Elem<T>::pack(s.x * f, s.y * f), Elem<T>::pack(s.z * f, s.w * f));
+  }
+}
+
+template <bool kKeys, typename T>
+void launch_merge(const BwdArgs& a, int D, hipStream_t s) {
+  if (a.splits > 1)
+    hipLaunchKernelGGL((bwd_merge_kernel<kKeys, T>), dim3((unsigned)a.n_items, kKeys ? 2 : 1), dim3(256), 0, s, a, D);
+}
+
 template <bool kKeys, typename T, int kD, int kParts>
 void launch_parts(const BwdArgs& a, hipStream_t s) {
   const int64_t groups = (a.n_slots + 3) / 4;
-  const dim3 grid((unsigned)((groups + 7) / 8 * 32)), blk(128 * kParts);
+  const dim3 grid((unsigned)((groups + 7) / 8 * 32), (unsigned)a.splits), blk(128 * kParts);
   if (a.bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, kParts>), grid, blk, 0, s, a);
   else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, kParts>), grid, blk, 0, s, a);
 }
@@ -607,65 +661,101 @@ int pairs_per_item(int n_items, int max_cnt, int D) {
   return n_items <= 512 || (n_items <= 1536 && max_cnt >= 32) ? 2 : 1;
 }
 
+// Splits of each item's list over workgroups, where the items leave most of the card idle and their
+// lists (of up to `width` entries) are long.
+int splits_of(int64_t n_items, int width, int D, bool f32) {
+  if (width < 32) return 1;
+  // workgroups of two pairs (fp32: two of four waves) per item that the card holds at once
+  const int64_t slots = f32 ? (D == 64 ? 256 : 128) : (D == 64 ? 768 : 512);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({slots / n_items, width / 8, 32}));
+}
+
 template <bool kKeys, typename T, int kD>
-void launch_pass(const BwdArgs& a, hipStream_t s) {
-  // (a key block's list is as long as there are query blocks, at most)
-  const int parts = pairs_per_item(a.n_items, kKeys ? a.n_st : a.max_cnt, kD);
+void launch_pass(const BwdArgs& a, int width, hipStream_t s) {
+  const int parts = a.splits > 1 ? 2 : pairs_per_item(a.n_items, width, kD);
   if (parts == 4) launch_parts<kKeys, T, kD, 4>(a, s);
   else if (parts == 2) launch_parts<kKeys, T, kD, 2>(a, s);
   else launch_parts<kKeys, T, kD, 1>(a, s);
+  launch_merge<kKeys, T>(a, kD, s);
 }
 
 template <bool kKeys>
 void launch_pass_f32(const BwdArgs& a, int D, hipStream_t s) {
   const int64_t groups = (a.n_slots + 3) / 4;
-  const dim3 grid((unsigned)((groups + 7) / 8 * 64)), blk(256);
+  const dim3 grid((unsigned)((groups + 7) / 8 * 64), (unsigned)a.splits), blk(256);
   if (D == 64) hipLaunchKernelGGL((bsa_bwd_f32_kernel<kKeys, 64>), grid, blk, 0, s, a);
   else hipLaunchKernelGGL((bsa_bwd_f32_kernel<kKeys, 128>), grid, blk, 0, s, a);
+  launch_merge<kKeys, float>(a, D, s);
 }
 
 template <bool kKeys>
-void launch_pass_any(const BwdArgs& a, int dtype, int D, hipStream_t s) {
+void launch_pass_any(const BwdArgs& a, int dtype, int D, int width, hipStream_t s) {
   if (dtype == SA_DTYPE_F32) return launch_pass_f32<kKeys>(a, D, s);
-  if (dtype == SA_DTYPE_F16) return D == 64 ? launch_pass<kKeys, _Float16, 64>(a, s) : launch_pass<kKeys, _Float16, 128>(a, s);
-  return D == 64 ? launch_pass<kKeys, __bf16, 64>(a, s) : launch_pass<kKeys, __bf16, 128>(a, s);
+  if (dtype == SA_DTYPE_F16)
+    return D == 64 ? launch_pass<kKeys, _Float16, 64>(a, width, s) : launch_pass<kKeys, _Float16, 128>(a, width, s);
+  return D == 64 ? launch_pass<kKeys, __bf16, 64>(a, width, s) : launch_pass<kKeys, __bf16, 128>(a, width, s);
 }
 
-int64_t stats_bytes(int B, int H, int Lq) { return (int64_t)B * H * sa::cdiv(Lq, kBlk) * 128 * sizeof(float); }
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// Workspace of a backward pass: the query rows' statistics, the transposed lists, the splits' sums (of one
+// pass at a time).
+struct Layout {
+  int64_t q_beg, q_idx, partial, bytes;
+  int q_splits, k_splits;
+};
+
+Layout layout(const sa_attn_train& t) {
+  const int64_t BH = (int64_t)t.B * t.H, nqb = sa::cdiv(t.Lq, kBlk), nkb = sa::cdiv(t.Lk, kBlk);
+  const bool f32 = t.dtype == SA_DTYPE_F32;
+  Layout l;
+  l.q_beg = align256(BH * nqb * 128 * (int64_t)sizeof(float));
+  l.q_idx = l.q_beg + align256(BH * (nkb + 1) * (int64_t)sizeof(int32_t));
+  l.partial = l.q_idx + align256(BH * nqb * t.max_cnt * (int64_t)sizeof(int32_t));
+  // (a list is no longer than the other side has blocks, but for repeated entries)
+  l.q_splits = splits_of(BH * nqb, std::min<int64_t>(t.max_cnt, nkb), t.D, f32);
+  l.k_splits = splits_of(BH * nkb, (int)nqb, t.D, f32);
+  const int64_t tile = (int64_t)kBlk * t.D * sizeof(float);
+  const int64_t q = l.q_splits > 1 ? BH * nqb * l.q_splits * tile : 0, k = l.k_splits > 1 ? BH * nkb * l.k_splits * 2 * tile : 0;
+  l.bytes = l.partial + std::max(q, k);
+  return l;
+}
+
+int check_train(const sa_attn_train* t, const char* fn) {
+  SA_REQUIRE(t, "%s: null pointer", fn);
+  SA_REQUIRE(t->dtype == SA_DTYPE_BF16 || t->dtype == SA_DTYPE_F16 || t->dtype == SA_DTYPE_F32, "%s: dtype %d", fn,
+             t->dtype);
+  SA_REQUIRE(t->B > 0 && t->H > 0 && t->Lq > 0 && t->Lk > 0, "%s: bad shape B=%d H=%d Lq=%d Lk=%d", fn, t->B, t->H,
+             t->Lq, t->Lk);
+  if (t->D != 64 && t->D != 128) return sa::fail(SA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", fn, t->D);
+  SA_REQUIRE(t->max_cnt > 0, "%s: max_cnt must be > 0", fn);
+  const int64_t nqb = sa::cdiv(t->Lq, kBlk), nkb = sa::cdiv(t->Lk, kBlk), BH = (int64_t)t->B * t->H;
+  SA_REQUIRE(BH * nqb < (1LL << 28) && BH * nkb < (1LL << 28), "%s: too many blocks", fn);
+  return SA_OK;
+}
 
 }  // namespace
 
-extern "C" int sa_block_sparse_bwd_workspace(int B, int H, int Lq, int64_t* bytes) {
-  SA_REQUIRE(bytes, "sa_block_sparse_bwd_workspace: null bytes");
-  SA_REQUIRE(B > 0 && H > 0 && Lq > 0, "sa_block_sparse_bwd_workspace: bad shape B=%d H=%d Lq=%d", B, H, Lq);
-  *bytes = stats_bytes(B, H, Lq);
+extern "C" int sa_block_sparse_bwd_workspace(const sa_attn_train* t, int64_t* bytes) {
+  const char* fn = "sa_block_sparse_bwd_workspace";
+  SA_REQUIRE(bytes, "%s: null bytes", fn);
+  if (int rc = check_train(t, fn)) return rc;
+  *bytes = layout(*t).bytes;
   return sa::ok();
 }
 
-extern "C" int sa_block_sparse_bwd(int dtype, const void* q, const void* k, const void* v, const void* out,
-                                   const void* dout, const float* lse, void* dq, void* dk, void* dv,
-                                   const int64_t strides[24], int B, int H, int Lq, int Lk, int D,
-                                   const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, const int32_t* q_beg,
-                                   const int32_t* q_idx, const float* key_bias, const int64_t bias_strides[2],
-                                   float sm_scale, const int32_t* q_order, int64_t n_q_slots, const int32_t* k_order,
-                                   int64_t n_k_slots, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   const char* fn = "sa_block_sparse_bwd";
-  SA_REQUIRE(dtype == SA_DTYPE_BF16 || dtype == SA_DTYPE_F16 || dtype == SA_DTYPE_F32, "%s: dtype %d", fn, dtype);
-  SA_REQUIRE(q && k && v && out && dout && lse && strides && kv_idx && kv_cnt, "%s: null pointer", fn);
-  SA_REQUIRE(!(dk || dv) || (q_beg && q_idx), "%s: dk and dv need the transposed lists", fn);
-  SA_REQUIRE(B > 0 && H > 0 && Lq > 0 && Lk > 0, "%s: bad shape B=%d H=%d Lq=%d Lk=%d", fn, B, H, Lq, Lk);
-  if (D != 64 && D != 128) return sa::fail(SA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", fn, D);
-  SA_REQUIRE(max_cnt > 0, "%s: max_cnt must be > 0", fn);
-  SA_REQUIRE(std::isfinite(sm_scale) && sm_scale > 0.f, "%s: sm_scale must be finite and > 0", fn);
-  SA_REQUIRE(!key_bias || bias_strides, "%s: key_bias without bias_strides", fn);
-  const bool f32 = dtype == SA_DTYPE_F32;
-  if (f32 && key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
+  if (int rc = check_train(t, fn)) return rc;
+  const int B = t->B, H = t->H, Lq = t->Lq, Lk = t->Lk, D = t->D;
+  SA_REQUIRE(t->q && t->k && t->v && t->out && t->dout && t->lse && t->kv_idx && t->kv_cnt, "%s: null pointer", fn);
+  SA_REQUIRE(std::isfinite(t->sm_scale) && t->sm_scale > 0.f, "%s: sm_scale must be finite and > 0", fn);
+  const bool f32 = t->dtype == SA_DTYPE_F32;
+  if (f32 && t->key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
   const int nqb = sa::cdiv(Lq, kBlk), nkb = sa::cdiv(Lk, kBlk);
-  const int64_t q_items = (int64_t)B * H * nqb, k_items = (int64_t)B * H * nkb;
-  SA_REQUIRE(q_items < (1LL << 28) && k_items < (1LL << 28), "%s: too many blocks", fn);
-  SA_REQUIRE((int64_t)nqb * max_cnt < (1LL << 31), "%s: lists of one head too long", fn);
   const int per16 = f32 ? 4 : 8, size = f32 ? 4 : 2;
-  const void* ptrs[8] = {q, k, v, out, dout, dq, dk, dv};
+  const void* ptrs[8] = {t->q, t->k, t->v, t->out, t->dout, t->dq, t->dk, t->dv};
+  const int64_t* strides = t->strides;
   for (int i = 0; i < 8; ++i) {
     if (reinterpret_cast<uintptr_t>(ptrs[i]) % 16 != 0)
       return sa::fail(SA_ERR_UNSUPPORTED, "%s: tensor base not 16-byte aligned", fn);
@@ -679,54 +769,64 @@ extern "C" int sa_block_sparse_bwd(int dtype, const void* q, const void* k, cons
   for (int i = 0; i < 4; ++i)
     if (strides[3 * at[i] + 2] < 0 || (rows[i] + kBlk) * strides[3 * at[i] + 2] * size + 2 * D > INT_MAX)
       return sa::fail(SA_ERR_UNSUPPORTED, "%s: rows of one head span more than 2 GiB", fn);
-  SA_REQUIRE(workspace && reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "%s: workspace null or not 256-byte aligned",
-             fn);
-  SA_REQUIRE(workspace_bytes >= stats_bytes(B, H, Lq), "%s: workspace of %lld bytes < %lld", fn,
-             (long long)workspace_bytes, (long long)stats_bytes(B, H, Lq));
-  SA_REQUIRE((!q_order || (n_q_slots > 0 && n_q_slots % 4 == 0 && n_q_slots < (1LL << 30))) &&
-                 (!k_order || (n_k_slots > 0 && n_k_slots % 4 == 0 && n_k_slots < (1LL << 30))),
+  const Layout l = layout(*t);
+  SA_REQUIRE(t->workspace && reinterpret_cast<uintptr_t>(t->workspace) % 256 == 0,
+             "%s: workspace null or not 256-byte aligned", fn);
+  SA_REQUIRE(t->workspace_bytes >= l.bytes, "%s: workspace of %lld bytes < %lld", fn, (long long)t->workspace_bytes,
+             (long long)l.bytes);
+  SA_REQUIRE((!t->q_order || (t->n_q_slots > 0 && t->n_q_slots % 4 == 0 && t->n_q_slots < (1LL << 30))) &&
+                 (!t->k_order || (t->n_k_slots > 0 && t->n_k_slots % 4 == 0 && t->n_k_slots < (1LL << 30))),
              "%s: slots must be a positive multiple of 4", fn);
+  uint8_t* ws = static_cast<uint8_t*>(t->workspace);
+  int32_t* q_beg = reinterpret_cast<int32_t*>(ws + l.q_beg);
+  int32_t* q_idx = reinterpret_cast<int32_t*>(ws + l.q_idx);
   hipStream_t s = sa::as_stream(stream);
+  if (t->dk || t->dv) {
+    if (int rc = sa_kv_list_transpose(t->kv_idx, t->kv_cnt, B * H, nqb, nkb, t->max_cnt, q_beg, q_idx, stream)) return rc;
+  }
   BwdArgs a;
   a.H = H;
-  a.max_cnt = max_cnt;
-  a.bias = key_bias;
-  a.bias_sb = key_bias ? bias_strides[0] : 0;
-  a.bias_sh = key_bias ? bias_strides[1] : 0;
-  a.sm_scale = sm_scale;
-  a.scale_log2 = sm_scale * kLog2e;
+  a.max_cnt = t->max_cnt;
+  a.bias = t->key_bias;
+  a.bias_sb = t->key_bias ? t->bias_strides[0] : 0;
+  a.bias_sh = t->key_bias ? t->bias_strides[1] : 0;
+  a.sm_scale = t->sm_scale;
+  a.scale_log2 = t->sm_scale * kLog2e;
   a.inv_scale_log2 = 1.f / a.scale_log2;
-  a.lse = lse;
-  a.stats = static_cast<float*>(workspace);
-  a.out = out;
+  a.lse = t->lse;
+  a.stats = reinterpret_cast<float*>(ws);
+  a.partial = reinterpret_cast<float*>(ws + l.partial);
+  a.out = t->out;
   a.o_sb = strides[9]; a.o_sh = strides[10]; a.o_sl = strides[11];
 
-  a.own_a = q; a.oa_sb = strides[0]; a.oa_sh = strides[1]; a.oa_sl = strides[2];
-  a.own_b = dout; a.ob_sb = strides[12]; a.ob_sh = strides[13]; a.ob_sl = strides[14];
-  a.st_a = k; a.sa_sb = strides[3]; a.sa_sh = strides[4]; a.sa_sl = strides[5];
-  a.st_b = v; a.sb_sb = strides[6]; a.sb_sh = strides[7]; a.sb_sl = strides[8];
-  a.grad_a = dq; a.ga_sb = strides[15]; a.ga_sh = strides[16]; a.ga_sl = strides[17];
+  a.own_a = t->q; a.oa_sb = strides[0]; a.oa_sh = strides[1]; a.oa_sl = strides[2];
+  a.own_b = t->dout; a.ob_sb = strides[12]; a.ob_sh = strides[13]; a.ob_sl = strides[14];
+  a.st_a = t->k; a.sa_sb = strides[3]; a.sa_sh = strides[4]; a.sa_sl = strides[5];
+  a.st_b = t->v; a.sb_sb = strides[6]; a.sb_sh = strides[7]; a.sb_sl = strides[8];
+  a.grad_a = t->dq; a.ga_sb = strides[15]; a.ga_sh = strides[16]; a.ga_sl = strides[17];
   a.grad_b = nullptr; a.gb_sb = a.gb_sh = a.gb_sl = 0;
   a.L_own = Lq; a.L_st = Lk; a.n_own = nqb; a.n_st = nkb;
-  a.n_items = (int)q_items;
-  a.order = q_order;
-  a.n_slots = (int)(q_order ? n_q_slots : (q_items + 3) / 4 * 4);
-  a.idx = kv_idx; a.cnt = kv_cnt;
-  launch_pass_any<false>(a, dtype, D, s);
+  a.n_items = B * H * nqb;
+  a.order = t->q_order;
+  a.n_slots = (int)(t->q_order ? t->n_q_slots : (a.n_items + 3) / 4 * 4);
+  a.idx = t->kv_idx; a.cnt = t->kv_cnt;
+  a.splits = t->dq ? l.q_splits : 1;
+  launch_pass_any<false>(a, t->dtype, D, std::min(t->max_cnt, nkb), s);
   if (int rc = sa::check_launch(fn)) return rc;
-  if (!dk && !dv) return sa::ok();
+  if (!t->dk && !t->dv) return sa::ok();
 
-  a.own_a = k; a.oa_sb = strides[3]; a.oa_sh = strides[4]; a.oa_sl = strides[5];
-  a.own_b = v; a.ob_sb = strides[6]; a.ob_sh = strides[7]; a.ob_sl = strides[8];
-  a.st_a = q; a.sa_sb = strides[0]; a.sa_sh = strides[1]; a.sa_sl = strides[2];
-  a.st_b = dout; a.sb_sb = strides[12]; a.sb_sh = strides[13]; a.sb_sl = strides[14];
-  a.grad_a = dk; a.ga_sb = strides[18]; a.ga_sh = strides[19]; a.ga_sl = strides[20];
-  a.grad_b = dv; a.gb_sb = strides[21]; a.gb_sh = strides[22]; a.gb_sl = strides[23];
+  a.own_a = t->k; a.oa_sb = strides[3]; a.oa_sh = strides[4]; a.oa_sl = strides[5];
+  a.own_b = t->v; a.ob_sb = strides[6]; a.ob_sh = strides[7]; a.ob_sl = strides[8];
+  a.st_a = t->q; a.sa_sb = strides[0]; a.sa_sh = strides[1]; a.sa_sl = strides[2];
+  a.st_b = t->dout; a.sb_sb = strides[12]; a.sb_sh = strides[13]; a.sb_sl = strides[14];
+  a.grad_a = t->dk; a.ga_sb = strides[18]; a.ga_sh = strides[19]; a.ga_sl = strides[20];
+  a.grad_b = t->dv; a.gb_sb = strides[21]; a.gb_sh = strides[22]; a.gb_sl = strides[23];
   a.L_own = Lk; a.L_st = Lq; a.n_own = nkb; a.n_st = nqb;
-  a.n_items = (int)k_items;
-  a.order = k_order;
-  a.n_slots = (int)(k_order ? n_k_slots : (k_items + 3) / 4 * 4);
+  a.n_items = B * H * nkb;
+  a.order = t->k_order;
+  a.n_slots = (int)(t->k_order ? t->n_k_slots : (a.n_items + 3) / 4 * 4);
   a.idx = q_idx; a.cnt = q_beg;
-  launch_pass_any<true>(a, dtype, D, s);
+  a.splits = l.k_splits;
+  launch_pass_any<true>(a, t->dtype, D, nqb, s);
   return sa::check_launch(fn);
 }

@@ -1841,29 +1841,27 @@ extern "C" int sa_block_sparse_fwd(const uint16_t* q, const int64_t q_strides[3]
                     0, nullptr, 0, stream, "sa_block_sparse_fwd");
 }
 
-extern "C" int sa_block_sparse_fwd_lse(int dtype, const void* q, const int64_t q_strides[3], const void* k,
-                                       const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
-                                       void* out, const int64_t out_strides[3], int B, int H, int Lq, int Lk, int D,
-                                       const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt,
-                                       const float* key_bias, const int64_t bias_strides[2], float sm_scale,
-                                       const int32_t* work_order, int64_t n_slots, int parts, void* workspace,
-                                       int64_t workspace_bytes, float* lse, void* stream) {
+extern "C" int sa_block_sparse_fwd_lse(const sa_attn_train* t, void* stream) {
   const char* fn = "sa_block_sparse_fwd_lse";
-  SA_REQUIRE(dtype == SA_DTYPE_BF16 || dtype == SA_DTYPE_F16 || dtype == SA_DTYPE_F32, "%s: dtype %d", fn, dtype);
-  SA_REQUIRE(lse, "%s: null lse", fn);
-  SA_REQUIRE(parts >= 1, "%s: parts=%d must be >= 1", fn, parts);
-  if (dtype == SA_DTYPE_F32) {
-    if (key_bias || parts != 1) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias or key-range parts", fn);
-    return sa::attn_f32_lse(static_cast<const float*>(q), q_strides, static_cast<const float*>(k), k_strides,
-                            static_cast<const float*>(v), v_strides, static_cast<float*>(out), out_strides, B, H, Lq,
-                            Lk, D, kv_idx, kv_cnt, max_cnt, sm_scale, work_order, n_slots, workspace, workspace_bytes,
-                            lse, stream, fn);
+  SA_REQUIRE(t, "%s: null pointer", fn);
+  SA_REQUIRE(t->dtype == SA_DTYPE_BF16 || t->dtype == SA_DTYPE_F16 || t->dtype == SA_DTYPE_F32, "%s: dtype %d", fn,
+             t->dtype);
+  SA_REQUIRE(t->lse, "%s: null lse", fn);
+  SA_REQUIRE(t->parts >= 1, "%s: parts=%d must be >= 1", fn, t->parts);
+  const int64_t* st = t->strides;
+  if (t->dtype == SA_DTYPE_F32) {
+    if (t->key_bias || t->parts != 1) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias or key-range parts", fn);
+    return sa::attn_f32_lse(static_cast<const float*>(t->q), st, static_cast<const float*>(t->k), st + 3,
+                            static_cast<const float*>(t->v), st + 6, static_cast<float*>(t->out), st + 9, t->B, t->H,
+                            t->Lq, t->Lk, t->D, t->kv_idx, t->kv_cnt, t->max_cnt, t->sm_scale, t->fwd_order,
+                            t->n_fwd_slots, t->workspace, t->workspace_bytes, t->lse, stream, fn);
   }
-  return launch_fwd(static_cast<const uint16_t*>(q), q_strides, static_cast<const uint16_t*>(k), k_strides,
-                    static_cast<const uint16_t*>(v), v_strides, static_cast<uint16_t*>(out), out_strides, B, H, Lq, Lk,
-                    D, kv_idx, kv_cnt, max_cnt, false, nullptr, nullptr, key_bias, bias_strides, sm_scale, work_order,
-                    n_slots, nullptr, 0, nullptr, 0, stream, fn, 1, 0, nullptr, lse, nullptr, dtype == SA_DTYPE_F16,
-                    false, parts, workspace, workspace_bytes);
+  return launch_fwd(static_cast<const uint16_t*>(t->q), st, static_cast<const uint16_t*>(t->k), st + 3,
+                    static_cast<const uint16_t*>(t->v), st + 6, static_cast<uint16_t*>(t->out), st + 9, t->B, t->H,
+                    t->Lq, t->Lk, t->D, t->kv_idx, t->kv_cnt, t->max_cnt, false, nullptr, nullptr, t->key_bias,
+                    t->bias_strides, t->sm_scale, t->fwd_order, t->n_fwd_slots, nullptr, 0, nullptr, 0, stream, fn, 1, 0,
+                    nullptr, t->lse, nullptr, t->dtype == SA_DTYPE_F16, false, t->parts, t->workspace,
+                    t->workspace_bytes);
 }
 
 namespace {

@@ -76,50 +76,99 @@ def _check_inputs(q, k, v, kv: KVList, key_bias):
     return key_bias
 
 
-def _bias_args(key_bias):
-    if key_bias is None:
-        return None, None
-    return key_bias.data_ptr(), _lib.i64(key_bias.stride(0), key_bias.stride(1))
+_OPERANDS = ("q", "k", "v", "out", "dout", "dq", "dk", "dv")  # in the order of AttnTrain.strides
 
 
-def _forward(q, k, v, kv: KVList, sm_scale: float, key_bias, n_text_blocks: int):
-    """(out, lse) of checked, aligned inputs; key_bias expanded."""
+def _set(call, **tensors):
+    for name, t in tensors.items():
+        setattr(call, name, t.data_ptr())
+        i = 3 * _OPERANDS.index(name)
+        call.strides[i:i + 3] = t.stride()[:3]
+
+
+def _call(q, k, v, kv: KVList, sm_scale: float, key_bias) -> "_lib.AttnTrain":
+    """The description of a call on checked, aligned inputs; key_bias expanded."""
     B, H, Lq, D = q.shape
-    Lk = k.shape[2]
-    nqb = kv.nqb
+    call = _lib.AttnTrain(dtype=_lib.DTYPES[q.dtype], B=B, H=H, Lq=Lq, Lk=k.shape[2], D=D, max_cnt=kv.max_cnt, parts=1,
+                          kv_idx=kv.idx.data_ptr(), kv_cnt=kv.cnt.data_ptr(), sm_scale=sm_scale)
+    _set(call, q=q, k=k, v=v)
+    if key_bias is not None:
+        call.key_bias = key_bias.data_ptr()
+        call.bias_strides[:] = key_bias.stride()[:2]
+    return call
+
+
+def _forward(call, q, k, v, kv: KVList, n_text_blocks: int):
+    """(out, lse) of a call."""
+    B, H, Lq, D = q.shape
+    n_items = B * H * kv.nqb
     out = torch.empty(B, H, Lq, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, nqb * BLOCK, dtype=torch.float32, device=q.device)
+    lse = torch.empty(B, H, kv.nqb * BLOCK, dtype=torch.float32, device=q.device)
     # The launch variants of block_sparse_attention: key-range parts for few blocks over long lists,
     # else a work order; fp32 on split operands where it takes them.
-    parts, ws, order = 1, None, None
+    ws = None
     if q.dtype == torch.float32:
-        if nqb >= F32_TERMS_BLOCKS:
-            ws = f32_terms_workspace(B, H, Lk, D, q.device)
-    elif key_bias is None:
-        parts = split_parts(B * H * nqb, kv.max_cnt, D)
-        if parts > 1:
-            ws = torch.empty(split_workspace_bytes(B * H * nqb, D, parts), dtype=torch.uint8, device=q.device)
-    if parts == 1:
-        # (lists of unknown length count as short beside the text rows')
-        row_blocks = kv.row_blocks if kv.row_blocks is not None else 0.0
-        share_text = q.dtype != torch.float32 and shares_text_rows(B * H * nqb, kv.nkb, n_text_blocks, row_blocks, D)
-        order = work_order(B, H, nqb, n_text_blocks, q.device, share_text)
-    bias_ptr, bias_strides = _bias_args(key_bias)
+        if kv.nqb >= F32_TERMS_BLOCKS:
+            ws = f32_terms_workspace(B, H, k.shape[2], D, q.device)
+    elif not call.key_bias:
+        call.parts = split_parts(n_items, kv.max_cnt, D)
+        if call.parts > 1:
+            ws = torch.empty(split_workspace_bytes(n_items, D, call.parts), dtype=torch.uint8, device=q.device)
+    if call.parts == 1:
+        # Lists of unknown length count as short ones beside the text rows': [1, 15, 17776, 64] with a
+        # fifth of the blocks 376 / 338 us without / with shared text rows, [1, 30, 4546, 64] 91 / 73 (were
+        # they all long after all: [1, 15, 17776, 64] dense 1 185 / 1 364).
+        row_blocks = kv.row_blocks if kv.row_blocks is not None or kv.dense else 0.0
+        share_text = q.dtype != torch.float32 and shares_text_rows(n_items, kv.nkb, n_text_blocks, row_blocks, D)
+        order = work_order(B, H, kv.nqb, n_text_blocks, q.device, share_text)
+        call.fwd_order, call.n_fwd_slots = order.data_ptr(), order.numel()
+    call.workspace, call.workspace_bytes = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
+    _set(call, out=out)
+    call.lse = lse.data_ptr()
     with _lib.on(q.device):
-        rc = _lib.load().sa_block_sparse_fwd_lse(
-            _lib.DTYPES[q.dtype], q.data_ptr(), _lib.i64(*q.stride()[:3]), k.data_ptr(), _lib.i64(*k.stride()[:3]),
-            v.data_ptr(), _lib.i64(*v.stride()[:3]), out.data_ptr(), _lib.i64(*out.stride()[:3]), B, H, Lq, Lk, D,
-            kv.idx.data_ptr(), kv.cnt.data_ptr(), kv.max_cnt, bias_ptr, bias_strides, float(sm_scale),
-            _lib.ptr(order), order.numel() if order is not None else 0, parts, _lib.ptr(ws),
-            ws.numel() if ws is not None else 0, lse.data_ptr(), _lib.stream_of(q))
+        rc = _lib.load().sa_block_sparse_fwd_lse(call, _lib.stream_of(q))
     _lib.check(rc, "sa_block_sparse_fwd_lse")
     return out, lse
+
+
+_WORKSPACE_BYTES = {}
+
+
+def _backward(call, dout, q, kv_nqb: int, kv_nkb: int, n_text_blocks: int, needs):
+    """(dq, dk, dv), None where not needed, of a call whose operands, out and lse are set."""
+    dout = _rows16(dout)
+    _set(call, dout=dout)
+    B, H, Lk, D = call.B, call.H, call.Lk, call.D
+    grads = [torch.empty(B, H, L, D, dtype=q.dtype, device=q.device) if n else None
+             for n, L in zip(needs, (call.Lq, Lk, Lk))]
+    for name, t in zip(("dq", "dk", "dv"), grads):
+        if t is None:
+            setattr(call, name, None)
+        else:
+            _set(call, **{name: t})
+    key = (call.dtype, B, H, call.Lq, Lk, D, call.max_cnt)
+    n = _WORKSPACE_BYTES.get(key)
+    if n is None:
+        b = ctypes.c_int64(0)
+        _lib.check(_lib.load().sa_block_sparse_bwd_workspace(call, ctypes.byref(b)), "sa_block_sparse_bwd_workspace")
+        n = _WORKSPACE_BYTES[key] = b.value
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    call.workspace, call.workspace_bytes = ws.data_ptr(), n
+    order = work_order(B, H, kv_nqb, n_text_blocks, q.device)
+    call.q_order, call.n_q_slots = order.data_ptr(), order.numel()
+    if kv_nkb != kv_nqb:
+        order = work_order(B, H, kv_nkb, n_text_blocks, q.device)
+    call.k_order, call.n_k_slots = order.data_ptr(), order.numel()
+    with _lib.on(q.device):
+        rc = _lib.load().sa_block_sparse_bwd(call, _lib.stream_of(q))
+    _lib.check(rc, "sa_block_sparse_bwd")
+    return grads
 
 
 def transpose_kv_list(kv: KVList) -> Tuple[torch.Tensor, torch.Tensor]:
     """(q_beg int32 [B*H, nkb + 1], q_idx int32 [B*H, nqb * max_cnt]): the query blocks that list each
     key block, ascending (`sa_kv_list_transpose`); key block j of a head has entries
-    q_idx[q_beg[j]:q_beg[j + 1]] of the head's row."""
+    q_idx[q_beg[j]:q_beg[j + 1]] of the head's row. The backward pass makes its own."""
     _lib.require_gpu(kv.idx, kv.cnt)
     BH = kv.B * kv.H
     beg = torch.empty(BH, kv.nkb + 1, dtype=torch.int32, device=kv.idx.device)
@@ -131,33 +180,6 @@ def transpose_kv_list(kv: KVList) -> Tuple[torch.Tensor, torch.Tensor]:
     return beg, idx
 
 
-def _backward(dout, q, k, v, out, lse, kv: KVList, sm_scale: float, key_bias, n_text_blocks: int, needs):
-    """(dq, dk, dv), None where not needed; q, k, v checked and aligned, key_bias expanded."""
-    B, H, Lq, D = q.shape
-    Lk = k.shape[2]
-    dout = _rows16(dout)
-    dq = torch.empty(B, H, Lq, D, dtype=q.dtype, device=q.device) if needs[0] else None
-    dk, dv = (torch.empty(B, H, Lk, D, dtype=q.dtype, device=q.device) if n else None for n in needs[1:])
-    strides = [s for t in (q, k, v, out, dout, dq, dk, dv) for s in (t.stride()[:3] if t is not None else (0, 0, 0))]
-    lib = _lib.load()
-    n = ctypes.c_int64(0)
-    _lib.check(lib.sa_block_sparse_bwd_workspace(B, H, Lq, ctypes.byref(n)), "sa_block_sparse_bwd_workspace")
-    ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-    q_beg, q_idx = transpose_kv_list(kv) if needs[1] or needs[2] else (None, None)
-    q_order = work_order(B, H, kv.nqb, n_text_blocks, q.device)
-    k_order = work_order(B, H, kv.nkb, n_text_blocks, q.device)
-    bias_ptr, bias_strides = _bias_args(key_bias)
-    with _lib.on(q.device):
-        rc = lib.sa_block_sparse_bwd(
-            _lib.DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(),
-            lse.data_ptr(), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.i64(*strides), B, H, Lq, Lk, D,
-            kv.idx.data_ptr(), kv.cnt.data_ptr(), kv.max_cnt, _lib.ptr(q_beg), _lib.ptr(q_idx), bias_ptr, bias_strides,
-            float(sm_scale), q_order.data_ptr(), q_order.numel(), k_order.data_ptr(), k_order.numel(), ws.data_ptr(),
-            ws.numel(), _lib.stream_of(q))
-    _lib.check(rc, "sa_block_sparse_bwd")
-    return dq, dk, dv
-
-
 def block_sparse_attention_lse(q, k, v, kv: KVList, sm_scale: float, key_bias: Optional[torch.Tensor] = None,
                                n_text_blocks: int = 0):
     """(out, lse): `block_sparse_attention` (q [B,H,Lq,D], k/v [B,H,Lk,D], bf16, fp16 or fp32, D 64 or
@@ -166,7 +188,8 @@ def block_sparse_attention_lse(q, k, v, kv: KVList, sm_scale: float, key_bias: O
     `n_text_blocks` only affects scheduling, as there."""
     key_bias = _check_inputs(q, k, v, kv, key_bias)
     with torch.no_grad():
-        return _forward(_rows16(q), _rows16(k), _rows16(v), kv, sm_scale, key_bias, n_text_blocks)
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        return _forward(_call(q, k, v, kv, float(sm_scale), key_bias), q, k, v, kv, n_text_blocks)
 
 
 def block_sparse_attention_backward(dout, q, k, v, out, lse, kv: KVList, sm_scale: float,
@@ -183,28 +206,37 @@ def block_sparse_attention_backward(dout, q, k, v, out, lse, kv: KVList, sm_scal
             or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError("lse must be block_sparse_attention_lse's")
     with torch.no_grad():
-        return _backward(dout, _rows16(q), _rows16(k), _rows16(v), _rows16(out), lse, kv, sm_scale, key_bias,
-                         n_text_blocks, tuple(needs))
+        q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
+        call = _call(q, k, v, kv, float(sm_scale), key_bias)
+        _set(call, out=out)
+        call.lse = lse.data_ptr()
+        return tuple(_backward(call, dout, q, kv.nqb, kv.nkb, n_text_blocks, needs))
 
 
 class _TrainAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, kv_idx, kv_cnt, key_bias, shape, sm_scale, n_text_blocks):
-        kv = KVList(kv_idx, kv_cnt, *shape[:4], row_blocks=shape[4])
+    def forward(ctx, q, k, v, kv, sm_scale, key_bias, n_text_blocks):
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        out, lse = _forward(q, k, v, kv, sm_scale, key_bias, n_text_blocks)
-        ctx.save_for_backward(q, k, v, out, lse, kv_idx, kv_cnt, key_bias)
-        ctx.args = shape, sm_scale, n_text_blocks
+        call = _call(q, k, v, kv, sm_scale, key_bias)
+        out, lse = _forward(call, q, k, v, kv, n_text_blocks)
+        ctx.save_for_backward(q, k, v, out, lse, kv.idx, kv.cnt, key_bias)
+        ctx.call, ctx.blocks = call, (kv.nqb, kv.nkb, n_text_blocks)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        if torch.is_grad_enabled():
+            raise RuntimeError("block-sparse attention is differentiable once (create_graph=True is not supported)")
         q, k, v, out, lse, kv_idx, kv_cnt, key_bias = ctx.saved_tensors
-        shape, sm_scale, n_text_blocks = ctx.args
-        kv = KVList(kv_idx, kv_cnt, *shape[:4])
-        grads = _backward(dout, q, k, v, out, lse, kv, sm_scale, key_bias, n_text_blocks, ctx.needs_input_grad[:3])
-        return (*grads, None, None, None, None, None, None)
+        # A copy of the forward pass's description: this may run twice, or in two threads, and hooks on
+        # saved tensors may have moved them.
+        call = _lib.AttnTrain.from_buffer_copy(ctx.call)
+        _set(call, q=q, k=k, v=v, out=out)
+        call.lse, call.kv_idx, call.kv_cnt = lse.data_ptr(), kv_idx.data_ptr(), kv_cnt.data_ptr()
+        if key_bias is not None:
+            call.key_bias = key_bias.data_ptr()
+            call.bias_strides[:] = key_bias.stride()[:2]
+        return (*_backward(call, dout, q, *ctx.blocks, ctx.needs_input_grad[:3]), None, None, None, None)
 
 
 class _NoKeys(torch.autograd.Function):
@@ -228,11 +260,10 @@ def block_sparse_attention_train(q, k, v, kv: KVList, sm_scale: float, key_bias:
     q [B,H,Lq,D], k/v [B,H,Lk,D] on the GPU, bf16, fp16 or fp32 (one type), D = 64 or 128, any strides
     (tensors whose rows are not 16-byte aligned are copied); key_bias fp32 [B,H,Lk] or None, not
     differentiated, not with fp32. `n_text_blocks` only affects scheduling: so many first block rows
-    and columns are listed by every other block. The lists (and key_bias) must stay as they are until
+    and columns are listed by every other block, beside shorter lists. The lists (and key_bias) must stay as they are until
     the backward pass has run."""
     key_bias = _check_inputs(q, k, v, kv, key_bias)
-    return _TrainAttention.apply(q, k, v, kv.idx, kv.cnt, key_bias, (kv.B, kv.H, kv.nqb, kv.nkb, kv.row_blocks),
-                                 float(sm_scale), int(n_text_blocks))
+    return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
 
 
 def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Optional[torch.Tensor] = None,

@@ -209,6 +209,8 @@ class _ApplyRotary(torch.autograd.Function):
         if dq is None and dk is None:
             return (None,) * 7
         # The transpose turns back; linear, so it is differentiable itself.
+        if not torch.is_grad_enabled():
+            return (*_turned(dq, dk, table, layout, skip, rows, not inverse), None, None, None, None, None)
         return (*_ApplyRotary.apply(dq, dk, table, layout, skip, rows, not inverse), None, None, None, None, None)
 
 

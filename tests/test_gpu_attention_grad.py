@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from conftest import case
 from grad_reference import check, reference, unit
@@ -51,7 +52,11 @@ SHAPES = [
     (1, 2, 300, 1, 1.0, 0.3),
     (2, 2, 400, 210, 0.4, 0.4),
     (1, 2, 700, 700, 0.3, 0.2),
-    (2, 30, 640, 600, 0.3, 0.1),  # more blocks than share workgroups
+    (2, 30, 640, 600, 0.3, 0.1),  # one pair of waves per block at head dim 128
+    (2, 45, 580, 640, 0.4, 0.0),  # and at 64
+    (1, 3, 70, 4500, 0.4, 0.0),  # few query blocks over long lists: split over workgroups
+    (1, 3, 4500, 70, 0.6, 0.1),  # few key blocks
+    (1, 2, 2300, 2200, 1.0, 0.0),
 ]
 
 
@@ -86,6 +91,36 @@ def test_forward_keeps_the_bits_of_block_sparse_triton_fn(dev, dtype):
         q, k, v = q.to(dev), k.to(dev), v.to(dev)
         want = block_sparse_triton_fn(q, k, v, mask, 0.1)
         assert torch.equal(block_sparse_train_fn(q, k, v, mask, 0.1), want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_text_blocks(dev, D):
+    # The hint of long first rows changes the schedule (shared rows in the forward pass) and no value.
+    case(f"text blocks D={D}")
+    (q, k, v, do), g = _inputs(16, BF16, 2, 75, 320, 300, D)
+    mask = _mask(g, 2, 75, 320, 300, 0.3)
+    mask[:, :, :2] = True
+    mask[..., :2] = True
+    got = _grads(lambda *x: block_sparse_train_fn(*x, mask.to(dev), 0.125, n_text_blocks=2), *(t.to(dev) for t in (q, k, v, do)))
+    check(got, reference(q, k, v, do, mask, 0.125), norm=1.5 * unit(BF16))
+
+
+def test_saved_tensor_hooks_and_two_backward_passes(dev):
+    case("saved tensor hooks")
+    (q, k, v, do), g = _inputs(17, BF16, 1, 2, 200, 200, 64)
+    mask = _mask(g, 1, 2, 200, 200, 0.6).to(dev)
+    x = [t.to(dev) for t in (q, k, v, do)]
+    want = _grads(lambda *y: block_sparse_train_fn(*y, mask, 0.125), *x)
+    with torch.autograd.graph.save_on_cpu():
+        got = _grads(lambda *y: block_sparse_train_fn(*y, mask, 0.125), *x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    leaves = [t.requires_grad_() for t in x[:3]]
+    out = block_sparse_train_fn(*leaves, mask, 0.125)
+    first = torch.autograd.grad(out, leaves, x[3], retain_graph=True)
+    again = torch.autograd.grad(out, leaves, x[3])
+    assert all(torch.equal(a, b) for a, b in zip(first, again)) and torch.equal(first[0], want[1])
+    ck = torch.utils.checkpoint.checkpoint(lambda *y: block_sparse_train_fn(*y, mask, 0.125), *leaves, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(ck, leaves, x[3]), first))
 
 
 def test_lse(dev):
@@ -400,9 +435,8 @@ def test_refusals(dev):
     with pytest.raises(ValueError):
         block_sparse_attention_backward(out, q, q, q, out, lse[..., :64], kv, 0.125)
     y = block_sparse_train_fn(q, q, q, mask, 0.125)
-    (first,) = torch.autograd.grad(y.float().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):  # differentiable once
-        torch.autograd.grad(first.float().sum(), q)
+        torch.autograd.grad(y.float().sum(), q, create_graph=True)
     # a change of a saved tensor in place is noticed
     x = q.detach().clone().requires_grad_()
     z = x * 1

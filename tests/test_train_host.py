@@ -80,31 +80,48 @@ def test_c_argument_checks():
         assert turn(**bad) == _lib.SA_ERR_INVALID, bad
 
     n = ctypes.c_int64(0)
-    assert lib.sa_block_sparse_bwd_workspace(2, 3, 65, ctypes.byref(n)) == 0 and n.value == 2 * 3 * 2 * 128 * 4
-    assert lib.sa_block_sparse_bwd_workspace(0, 3, 65, ctypes.byref(n)) == _lib.SA_ERR_INVALID
-    strides = [0, 0, 64] * 8
 
-    def bwd(dtype=0, q=p, k=p, dk=p, dv=p, lse=p, stride=strides, L=128, D=64, cnt=2, beg=p, bias=None, scale=0.125, ws=p,
-            nbytes=1 << 20, order=None, slots=0):
-        return lib.sa_block_sparse_bwd(dtype, q, k, p, p, p, lse, p, dk, dv, _lib.i64(*stride), 1, 1, L, L, D, p, p, cnt,
-                                       beg, p, bias, _lib.i64(0, 0), scale, order, slots, order, slots, ws, nbytes, None)
+    def call(**changed):
+        strides = changed.pop("stride", [0, 0, 64] * 8)
+        a = dict(dtype=0, B=1, H=1, Lq=128, Lk=128, D=64, max_cnt=2, parts=1, sm_scale=0.125, workspace=256,
+                 workspace_bytes=1 << 20)
+        a.update((x, 256) for x in ("q", "k", "v", "out", "dout", "dq", "dk", "dv", "lse", "kv_idx", "kv_cnt"))
+        t = _lib.AttnTrain(**{**a, **changed})
+        t.strides[:] = strides
+        return t
 
-    for bad in (dict(dtype=-1), dict(q=None), dict(lse=None), dict(beg=None), dict(L=0), dict(cnt=0), dict(scale=0.0),
-                dict(scale=math.nan), dict(ws=None), dict(ws=ctypes.c_void_p(16)), dict(nbytes=100), dict(order=p, slots=3)):
+    def need(**changed):
+        return lib.sa_block_sparse_bwd_workspace(call(**changed), ctypes.byref(n))
+
+    assert need(B=2, H=30, Lq=640, Lk=650, max_cnt=11) == 0  # statistics, list beginnings and entries
+    assert n.value == 60 * 10 * 128 * 4 + (60 * 12 * 4 + 255) // 256 * 256 + (60 * 10 * 11 * 4 + 255) // 256 * 256
+    for bad in (dict(B=0), dict(H=0), dict(Lq=0), dict(Lk=0), dict(max_cnt=0), dict(dtype=5), dict(H=1 << 27)):
+        assert need(**bad) == _lib.SA_ERR_INVALID, bad
+    assert need(D=32) == _lib.SA_ERR_UNSUPPORTED
+    assert lib.sa_block_sparse_bwd_workspace(None, ctypes.byref(n)) == _lib.SA_ERR_INVALID
+    assert lib.sa_block_sparse_bwd_workspace(call(), None) == _lib.SA_ERR_INVALID
+
+    def bwd(**changed):
+        return lib.sa_block_sparse_bwd(call(**changed), None)
+
+    assert lib.sa_block_sparse_bwd(None, None) == _lib.SA_ERR_INVALID
+    for bad in (dict(dtype=-1), *(dict([(x, None)]) for x in ("q", "k", "v", "out", "dout", "lse", "kv_idx", "kv_cnt")),
+                dict(Lq=0), dict(max_cnt=0), dict(sm_scale=0.0), dict(sm_scale=math.nan), dict(workspace=None),
+                dict(workspace=16), dict(workspace_bytes=100), dict(q_order=256, n_q_slots=3), dict(k_order=256)):
         assert bwd(**bad) == _lib.SA_ERR_INVALID, bad
-    for bad in (dict(D=96), dict(q=ctypes.c_void_p(8)), dict(stride=[0, 0, 65] * 8), dict(stride=[0, 0, 1 << 30] * 8),
-                dict(stride=[0, 0, -64] * 8), dict(dtype=2, bias=p)):
+    for bad in (dict(D=96), dict(q=8), dict(dv=8), dict(stride=[0, 0, 65] * 8), dict(stride=[0, 0, 1 << 30] * 8),
+                dict(stride=[0, 0, -64] * 8), dict(dtype=2, key_bias=256), dict(max_cnt=65536, workspace_bytes=1 << 40)):
         assert bwd(**bad) == _lib.SA_ERR_UNSUPPORTED, bad
 
-    def lse(dtype=0, out=p, bias=None, parts=1, ws=None, nbytes=0, buf=p):
-        s = _lib.i64(0, 0, 64)
-        return lib.sa_block_sparse_fwd_lse(dtype, p, s, p, s, p, s, out, s, 1, 1, 64, 64, 64, p, p, 1, bias,
-                                           _lib.i64(0, 0), 0.125, None, 0, parts, ws, nbytes, buf, None)
+    def lse(**changed):
+        return lib.sa_block_sparse_fwd_lse(call(**changed), None)
 
-    for bad in (dict(dtype=7), dict(buf=None), dict(parts=0), dict(parts=2), dict(out=None),
-                dict(dtype=2, ws=p, nbytes=10)):
+    assert lib.sa_block_sparse_fwd_lse(None, None) == _lib.SA_ERR_INVALID
+    for bad in (dict(dtype=7), dict(lse=None), dict(parts=0), dict(parts=2, workspace=None), dict(out=None), dict(sm_scale=-1.0),
+                dict(dtype=2, workspace_bytes=10), dict(Lk=0)):
         assert lse(**bad) == _lib.SA_ERR_INVALID, bad
-    for bad in (dict(dtype=2, bias=p), dict(dtype=2, parts=2), dict(bias=p, parts=2, ws=p, nbytes=1 << 30)):
+    for bad in (dict(dtype=2, key_bias=256), dict(dtype=2, parts=2), dict(key_bias=256, parts=2), dict(D=80),
+                dict(stride=[0, 0, 66] * 8)):
         assert lse(**bad) == _lib.SA_ERR_UNSUPPORTED, bad
 
     def transpose(idx=p, BH=1, nqb=2, nkb=2, cnt=2):
