@@ -72,7 +72,7 @@ struct BwdArgs {
   // [bh][2 * query blocks][2][32]: per 32 query rows their -lse / scale_log2, then their -delta. Written
   // by the query pass, read by the key pass.
   float* stats;
-  // More than one split: workgroup (item, blockIdx.y) computes the split's share of the item's steps and
+  // More than one split: a workgroup computes its split's share of the item's steps and
   // stores its sums to partial[item][split][result][64][kD]; bwd_merge_kernel adds them in order.
   int splits;
   float* partial;
@@ -89,7 +89,14 @@ __device__ inline float2 unpack2(uint32_t w) {
 
 // Item of a workgroup: the four slots of dispatch group w (placed on XCD w % 8 by the work order) go to
 // the workgroups 32 (w / 8) + 8 i + w % 8, i = 0 .. 3, which the dispatcher places on the same XCD.
-__device__ inline int bwd_item(const BwdArgs& a, int x) {
+// With splits there are no idle workgroups, which would leave CUs out of turn ([1, 1, 64 x 17776, 64] in
+// fp32 ran on a quarter of 32 CUs): item and split count up.
+__device__ inline int bwd_item(const BwdArgs& a, int x, int& split) {
+  split = 0;
+  if (a.splits > 1) {
+    split = x % a.splits;
+    return x / a.splits;
+  }
   const int slot = 4 * (8 * (x >> 5) + (x & 7)) + ((x >> 3) & 3);
   if (slot >= a.n_slots) return -1;
   return a.order ? order_item(a.order, slot) : slot;
@@ -135,7 +142,8 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = wave >> 1, w = wave & 1;
   const int col = lane & 31, hh = lane >> 5;
-  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x));
+  int split;
+  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x, split));
   if (item < 0 || item >= a.n_items) return;  // (the whole workgroup)
   const int bh = item / a.n_own;
   const int blk = item - bh * a.n_own;
@@ -170,7 +178,7 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void 
     }
     delta = xhalf_sum(delta);
     lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col];
-    if (part == 0 && blockIdx.y == 0) {
+    if (part == 0 && split == 0) {
       const bool row_ok = own_row < a.L_own;
       const float v = hh == 0 ? -lse * a.inv_scale_log2 : -delta;
       a.stats[(((int64_t)bh * a.n_own + blk) * 2 + w) * 64 + lane] = row_ok ? v : hh == 0 ? -INFINITY : 0.f;
@@ -195,9 +203,9 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void 
 
   // The split's share of the 2 cnt steps, of it the part's.
   const int per_split = (2 * cnt + a.splits - 1) / a.splits;
-  const int n_steps = min(2 * cnt, per_split * ((int)blockIdx.y + 1));
+  const int n_steps = min(2 * cnt, per_split * (split + 1));
   const int per_part = (per_split + kParts - 1) / kParts;
-  const int beg = (int)blockIdx.y * per_split + part * per_part;
+  const int beg = split * per_split + part * per_part;
   auto block_of = [&](int i) -> int {  // the streamed block of the part's i-th step, -1: none
     const int s = beg + i;
     return i < per_part && s < n_steps ? list[s >> 1] : -1;
@@ -427,7 +435,7 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void 
           s.w += y.w;
         }
         if (a.splits > 1)
-          *reinterpret_cast<float4*>(a.partial + ((((int64_t)item * a.splits + blockIdx.y) * kAcc + x) * kBlk + r) * kD +
+          *reinterpret_cast<float4*>(a.partial + ((((int64_t)item * a.splits + split) * kAcc + x) * kBlk + r) * kD +
                                      4 * ch) = s;
         else if (g && blk * kBlk + r < a.L_own)
           *reinterpret_cast<uint2*>(g + b * sb + h * sh + (int64_t)(blk * kBlk + r) * sl + 4 * ch) =
@@ -437,28 +445,39 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void 
   }
 }
 
-// ---- fp32: the same passes on v_mfma_f32_32x32x2_f32, operands straight from memory (the caches hold
-// a step's rows: its 32 x 32 x kD products take 16 times as long as in 16 bits).
+// ---- fp32: the same passes on v_mfma_f32_32x32x2_f32, which takes 16 times as long as the 16-bit
+// products. Steps, stages and parts are those of bsa_bwd_kernel. The contraction over d gives k slot hh of
+// step s the value d = hh * kD / 2 + s, so that a lane reads half a row in 16-byte chunks; that over the
+// streamed rows takes row 8 (e / 4) + 4 hh + e % 4 at step e, where P and dS lie, and reads 32
+// consecutive values of it per lane half.
 
 __device__ inline sa_f32x16 mfma32x2(float x, float y, sa_f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x2f32(x, y, c, 0, 0, 0);
 }
 
-// A workgroup computes 32 own rows (half `blockIdx.x & 1` of an item): its four waves take a share of
-// the steps each and add their sums in LDS, in order. The contraction over d gives k slot hh of step s
-// the value d = hh * kD / 2 + s, so that a lane reads half a row; that over the streamed rows takes row
-// 8 (e / 4) + 4 hh + e % 4 at step e, where P and dS lie.
+// Chunk c (16 bytes) of LDS row r lies at chunk c ^ swz_f32(r) of its 256 bytes. Sixteen rows at one
+// chunk take every bank once (row reads), as do 32 values of a row and of the row four below it
+// (column reads).
+__device__ inline int swz_f32(int r) { return (r & 3) | ((r >> 1) & 4) | ((r << 1) & 8); }
+
 template <bool kKeys, int kD>
 __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdArgs a) {
+  constexpr int kParts = 2;
   constexpr int kHD = kD / 2;
   constexpr int kDC = kD / 32;
   constexpr int kAcc = kKeys ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) float sums[4 * kStep * kD];
+  constexpr int kRow = kD * 4;             // bytes of a row
+  constexpr int kMat = kStep * kRow;       // a step's rows of one matrix
+  constexpr int kCopies = kMat / 1024;     // 1 KB each
+  constexpr int kLanes = kRow / 16;        // lanes per row of a copy
+  __shared__ __attribute__((aligned(1024))) uint8_t tile0[kParts * 2 * kMat], tile1[kParts * 2 * kMat];
+  __shared__ __attribute__((aligned(256))) float stat0[kParts * 64], stat1[kParts * 64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = wave >> 1, w = wave & 1;
   const int col = lane & 31, hh = lane >> 5;
-  const int half = blockIdx.x & 1;
-  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x >> 1));
+  int split;
+  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x, split));
   if (item < 0 || item >= a.n_items) return;  // (the whole workgroup)
   const int bh = item / a.n_own;
   const int blk = item - bh * a.n_own;
@@ -466,7 +485,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   const int h = bh - b * a.H;
   int cnt;
   const auto list = bwd_list<kKeys>(a, item, bh, blk, cnt);
-  const int own_row = blk * kBlk + kStep * half + col;
+  const int own_row = blk * kBlk + kStep * w + col;
   const int own_clamped = min(own_row, a.L_own - 1);  // rows past L_own are never stored
   const float* oa = static_cast<const float*>(a.own_a) + b * a.oa_sb + h * a.oa_sh + (int64_t)own_clamped * a.oa_sl;
   const float* ob = static_cast<const float*>(a.own_b) + b * a.ob_sb + h * a.ob_sh + (int64_t)own_clamped * a.ob_sl;
@@ -487,83 +506,153 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
       delta = fmaf(x.x, fb[s], fmaf(x.y, fb[s + 1], fmaf(x.z, fb[s + 2], fmaf(x.w, fb[s + 3], delta))));
     }
     delta = xhalf_sum(delta);
-    lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * half + col];
-    if (wave == 0 && blockIdx.y == 0) {
+    lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col];
+    if (part == 0 && split == 0) {
       const bool row_ok = own_row < a.L_own;
       // (the key pass takes lse as it is here: its element costs a fused multiply-add either way)
       const float v = hh == 0 ? -lse : -delta;
-      a.stats[(((int64_t)bh * a.n_own + blk) * 2 + half) * 64 + lane] = row_ok ? v : hh == 0 ? -INFINITY : 0.f;
+      a.stats[(((int64_t)bh * a.n_own + blk) * 2 + w) * 64 + lane] = row_ok ? v : hh == 0 ? -INFINITY : 0.f;
     }
     if (!a.grad_a) return;
   }
-  const float* sa = static_cast<const float*>(a.st_a) + b * a.sa_sb + h * a.sa_sh;
-  const float* sb = static_cast<const float*>(a.st_b) + b * a.sb_sb + h * a.sb_sh;
+
+  const float* st = w == 0 ? static_cast<const float*>(a.st_a) + b * a.sa_sb + h * a.sa_sh
+                           : static_cast<const float*>(a.st_b) + b * a.sb_sb + h * a.sb_sh;
+  const uint32_t row_bytes = (uint32_t)(w == 0 ? a.sa_sl : a.sb_sl) * 4;
+  const uint32_t st_bytes = (uint32_t)(a.L_st - 1) * row_bytes + kRow;
+  const float* stat_src = a.stats + (int64_t)bh * a.n_st * 128;
+  const uint32_t stat_bytes = (uint32_t)a.n_st * 512;
+
+  const int per_split = (2 * cnt + a.splits - 1) / a.splits;
+  const int n_steps = min(2 * cnt, per_split * (split + 1));
+  const int per_part = (per_split + kParts - 1) / kParts;
+  const int beg = split * per_split + part * per_part;
+  auto block_of = [&](int i) -> int {  // the streamed block of the part's i-th step, -1: none
+    const int s = beg + i;
+    return i < per_part && s < n_steps ? list[s >> 1] : -1;
+  };
+  auto issue = [&](int rb, int i, lds_u8* tile, lds_u8* stat) __attribute__((always_inline)) {
+    if ((unsigned)rb >= (unsigned)a.n_st) return;
+    const uint32_t row0 = __builtin_amdgcn_readfirstlane(rb * kBlk + kStep * ((beg + i) & 1));
+    const uint32_t off = min(row0 * row_bytes, st_bytes);
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(st) + off), (short)0, (int)(st_bytes - off), 0x00020000);
+    lds_u8* dst = tile + (part * 2 + w) * kMat;
+#pragma unroll
+    for (int j = 0; j < kCopies; ++j) {
+      const int r = j * (64 / kLanes) + lane / kLanes, c = lane % kLanes;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_u8*)(dst + 1024 * j), 16, r * row_bytes + 16 * (c ^ swz_f32(r)),
+                                               0, 0, 0);
+    }
+    if (kKeys && w == 0) {
+      const uint32_t soff = min(row0 * 8, stat_bytes);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(stat_src) + soff), (short)0, (int)(stat_bytes - soff),
+          0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u8*)(stat + part * 256), 4, 4 * lane, 0, 0, 0);
+    }
+  };
 
   sa_f32x16 acc[kAcc][kDC];
 #pragma unroll
   for (int x = 0; x < kAcc; ++x)
 #pragma unroll
     for (int dc = 0; dc < kDC; ++dc) acc[x][dc] = sa_f32x16{};
-  for (int i = wave + 4 * blockIdx.y; i < 2 * cnt; i += 4 * a.splits) {
-    const int rb = list[i >> 1];
-    if ((unsigned)rb >= (unsigned)a.n_st) continue;
-    const int row0 = rb * kBlk + kStep * (i & 1);
-    if (row0 >= a.L_st) continue;
-    const int64_t row = min(row0 + col, a.L_st - 1);  // clamped rows get P = 0
+  const int at_row = part * 2 * kMat + col * kRow, row_swz = swz_f32(col);
+  const int at_col = part * 2 * kMat + 4 * hh * kRow + 4 * (col & 3);
+
+  auto compute = [&](int cur, int i, const lds_u8* tile, const float* stat) __attribute__((always_inline)) {
+    const int row0 = cur * kBlk + kStep * ((beg + i) & 1);
+    if ((unsigned)cur >= (unsigned)a.n_st || row0 >= a.L_st) return;
+    typedef __attribute__((address_space(3))) const float lds_f;
     sa_f32x16 S = {}, dP = {};
     float nl[16];
     if constexpr (kKeys) {
-      const float* sp = a.stats + (((int64_t)bh * a.n_st + rb) * 2 + (i & 1)) * 64 + 4 * hh;
+      const float* x = stat + part * 64 + 4 * hh;
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const float4 x = *reinterpret_cast<const float4*>(sp + 8 * q4);
-        const float4 y = *reinterpret_cast<const float4*>(sp + 32 + 8 * q4);
-        nl[4 * q4] = x.x; nl[4 * q4 + 1] = x.y; nl[4 * q4 + 2] = x.z; nl[4 * q4 + 3] = x.w;
-        dP[4 * q4] = y.x; dP[4 * q4 + 1] = y.y; dP[4 * q4 + 2] = y.z; dP[4 * q4 + 3] = y.w;
+      for (int e = 0; e < 16; ++e) {
+        nl[e] = x[8 * (e >> 2) + (e & 3)];
+        dP[e] = x[32 + 8 * (e >> 2) + (e & 3)];
       }
     }
-    {
-      const float* pa = sa + row * a.sa_sl + hh * kHD;
-      const float* pb = sb + row * a.sb_sl + hh * kHD;
+    // (each group of reads is issued before the products of the group before it)
+    sa_u32x4v x[2], y[2];
+    auto rows = [&](int s) __attribute__((always_inline)) {
+      const lds_u8* q = tile + at_row + 16 * ((hh * (kHD / 4) + s / 4) ^ row_swz);
+      x[(s >> 2) & 1] = lds_read_b128(q);
+      y[(s >> 2) & 1] = lds_read_b128(q + kMat);
+    };
+    rows(0);
 #pragma unroll
-      for (int s = 0; s < kHD; s += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(pa + s);
-        const float4 y = *reinterpret_cast<const float4*>(pb + s);
-        S = mfma32x2(x.x, fa[s], S);
-        dP = mfma32x2(y.x, fb[s], dP);
-        S = mfma32x2(x.y, fa[s + 1], S);
-        dP = mfma32x2(y.y, fb[s + 1], dP);
-        S = mfma32x2(x.z, fa[s + 2], S);
-        dP = mfma32x2(y.z, fb[s + 2], dP);
-        S = mfma32x2(x.w, fa[s + 3], S);
-        dP = mfma32x2(y.w, fb[s + 3], dP);
+    for (int s = 0; s < kHD; s += 4) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (s + 4 < kHD) rows(s + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        S = mfma32x2(__uint_as_float(x[(s >> 2) & 1][j]), fa[s + j], S);
+        dP = mfma32x2(__uint_as_float(y[(s >> 2) & 1][j]), fb[s + j], dP);
       }
     }
-    float p[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const bool ok = row0 + 8 * (e >> 2) + 4 * hh + (e & 3) < a.L_st;
-      p[e] = ok ? exp2f(fmaf(S[e], a.scale_log2, kKeys ? nl[e] : -lse)) : 0.f;
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int64_t r = min(row0 + 8 * (e >> 2) + 4 * hh + (e & 3), a.L_st - 1);
-      const float ds = kKeys ? p[e] * dP[e] : p[e] * (dP[e] - delta);
+    float cols[2][kAcc][kDC];
+    auto columns = [&](int e) __attribute__((always_inline)) {
+      const int r = 8 * (e >> 2) + (e & 3);  // + 4 hh
 #pragma unroll
       for (int dc = 0; dc < kDC; ++dc) {
-        acc[0][dc] = mfma32x2(sa[r * a.sa_sl + 32 * dc + col], ds, acc[0][dc]);
-        if constexpr (kKeys) acc[kAcc - 1][dc] = mfma32x2(sb[r * a.sb_sl + 32 * dc + col], p[e], acc[kAcc - 1][dc]);
+        const lds_u8* q = tile + at_col + r * kRow + 16 * ((8 * dc + (col >> 2)) ^ (swz_f32(r) | (hh << 3)));
+#pragma unroll
+        for (int z = 0; z < kAcc; ++z) cols[e & 1][z][dc] = *reinterpret_cast<lds_f*>(q + z * kMat);
       }
+    };
+    columns(0);
+    float p[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) p[e] = exp2f(fmaf(S[e], a.scale_log2, kKeys ? nl[e] : -lse));
+    if (!kKeys && row0 + kStep > a.L_st) {  // keys past the last one (the statistics see to queries)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (row0 + 8 * (e >> 2) + 4 * hh + (e & 3) >= a.L_st) p[e] = 0.f;
     }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (e < 15) columns(e + 1);
+      const float ds = kKeys ? p[e] * dP[e] : p[e] * (dP[e] - delta);
+#pragma unroll
+      for (int dc = 0; dc < kDC; ++dc)
+#pragma unroll
+        for (int z = 0; z < kAcc; ++z) acc[z][dc] = mfma32x2(cols[e & 1][z][dc], z == 0 ? ds : p[e], acc[z][dc]);
+    }
+  };
+
+  lds_u8* const t0 = (lds_u8*)tile0;
+  lds_u8* const t1 = (lds_u8*)tile1;
+  int rb = block_of(0);
+  issue(rb, 0, t0, (lds_u8*)stat0);
+  int rb_next = block_of(1);
+  for (int i = 0; i < per_part; i += 2) {  // (as in bsa_bwd_kernel)
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    wg_barrier();
+    issue(rb_next, i + 1, t1, (lds_u8*)stat1);
+    compute(rb, i, t0, stat0);
+    if (i + 1 >= per_part) break;
+    rb = block_of(i + 2);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    wg_barrier();
+    issue(rb, i + 2, t0, (lds_u8*)stat0);
+    compute(rb_next, i + 1, t1, stat1);
+    rb_next = block_of(i + 3);
   }
+
+  // ---- Results: the parts' sums are added in LDS, in order.
   constexpr int kCh = kD / 4;
 #pragma unroll
   for (int x = 0; x < kAcc; ++x) {
     float* g = static_cast<float*>(x == 0 ? a.grad_a : a.grad_b);
-    const int64_t gsb = x == 0 ? a.ga_sb : a.gb_sb, gsh = x == 0 ? a.ga_sh : a.gb_sh, gsl = x == 0 ? a.ga_sl : a.gb_sl;
+    const int64_t sb = x == 0 ? a.ga_sb : a.gb_sb, sh = x == 0 ? a.ga_sh : a.gb_sh, sl = x == 0 ? a.ga_sl : a.gb_sl;
     const float f = x == 0 ? a.sm_scale : 1.f;
+    static_assert(kBlk * kD * 4 <= kParts * 2 * kMat, "the sums of a part fit a stage");
     __syncthreads();
-    float* mine = sums + (wave * kStep + col) * kD;
+    float* mine = reinterpret_cast<float*>(part ? tile1 : tile0) + (kStep * w + col) * kD;
 #pragma unroll
     for (int dc = 0; dc < kDC; ++dc)
 #pragma unroll
@@ -573,23 +662,18 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
             make_float4(A[4 * q4], A[4 * q4 + 1], A[4 * q4 + 2], A[4 * q4 + 3]);
       }
     __syncthreads();
-    for (int t = threadIdx.x; t < kStep * kCh; t += 256) {
+    for (int t = threadIdx.x; t < kBlk * kCh; t += 256) {
       const int r = t / kCh, ch = t % kCh;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float4 y = *reinterpret_cast<const float4*>(sums + (p * kStep + r) * kD + 4 * (ch ^ (r & (kCh - 1))));
-        s.x += y.x;
-        s.y += y.y;
-        s.z += y.z;
-        s.w += y.w;
-      }
-      const int row = blk * kBlk + kStep * half + r;
+      const int at = r * kD + 4 * (ch ^ (r & 31 & (kCh - 1)));
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tile0) + at);
+      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tile1) + at);
+      const float4 s = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+      const int row = blk * kBlk + r;
       if (a.splits > 1)
-        *reinterpret_cast<float4*>(a.partial + ((((int64_t)item * a.splits + blockIdx.y) * kAcc + x) * kBlk + kStep * half + r) * kD +
+        *reinterpret_cast<float4*>(a.partial + ((((int64_t)item * a.splits + split) * kAcc + x) * kBlk + r) * kD +
                                    4 * ch) = s;
       else if (g && row < a.L_own)
-        *reinterpret_cast<float4*>(g + b * gsb + h * gsh + (int64_t)row * gsl + 4 * ch) =
+        *reinterpret_cast<float4*>(g + b * sb + h * sh + (int64_t)row * sl + 4 * ch) =
             make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
     }
   }
@@ -636,10 +720,13 @@ void launch_merge(const BwdArgs& a, int D, hipStream_t s) {
     hipLaunchKernelGGL((bwd_merge_kernel<kKeys, T>), dim3((unsigned)a.n_items, kKeys ? 2 : 1), dim3(256), 0, s, a, D);
 }
 
+unsigned workgroups(const BwdArgs& a) {
+  return a.splits > 1 ? (unsigned)a.n_items * a.splits : (unsigned)(((a.n_slots + 3) / 4 + 7) / 8 * 32);
+}
+
 template <bool kKeys, typename T, int kD, int kParts>
 void launch_parts(const BwdArgs& a, hipStream_t s) {
-  const int64_t groups = (a.n_slots + 3) / 4;
-  const dim3 grid((unsigned)((groups + 7) / 8 * 32), (unsigned)a.splits), blk(128 * kParts);
+  const dim3 grid(workgroups(a)), blk(128 * kParts);
   if (a.bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, kParts>), grid, blk, 0, s, a);
   else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, kParts>), grid, blk, 0, s, a);
 }
@@ -662,12 +749,15 @@ int pairs_per_item(int n_items, int max_cnt, int D) {
 }
 
 // Splits of each item's list over workgroups, where the items leave most of the card idle and their
-// lists (of up to `width` entries) are long.
+// lists (of up to `width` entries) are long: at least 8 entries each, 2 in fp32, whose entries take 16 times
+// as long. Without / with, us of the query pass of 64 queries and the key pass of 64 keys against 17 776
+// of the other: one head 93 / 9 and 114 / 10, 30 heads 112 / 27 and 120 / 29; fp32, one head 594 / 36 and 1
+// 076 / 48; [1, 1, 2048, 64], 8 of 32 blocks, 10.3 / 7.0 and 10.9 / 8.0.
 int splits_of(int64_t n_items, int width, int D, bool f32) {
-  if (width < 32) return 1;
-  // workgroups of two pairs (fp32: two of four waves) per item that the card holds at once
-  const int64_t slots = f32 ? (D == 64 ? 256 : 128) : (D == 64 ? 768 : 512);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({slots / n_items, width / 8, 32}));
+  if (width < (f32 ? 8 : 32)) return 1;
+  // workgroups of two pairs that the card holds at once
+  const int64_t slots = f32 ? (D == 64 ? 512 : 256) : (D == 64 ? 768 : 512);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({slots / n_items, width / (f32 ? 2 : 8), 32}));
 }
 
 template <bool kKeys, typename T, int kD>
@@ -681,8 +771,7 @@ void launch_pass(const BwdArgs& a, int width, hipStream_t s) {
 
 template <bool kKeys>
 void launch_pass_f32(const BwdArgs& a, int D, hipStream_t s) {
-  const int64_t groups = (a.n_slots + 3) / 4;
-  const dim3 grid((unsigned)((groups + 7) / 8 * 64), (unsigned)a.splits), blk(256);
+  const dim3 grid(workgroups(a)), blk(256);
   if (D == 64) hipLaunchKernelGGL((bsa_bwd_f32_kernel<kKeys, 64>), grid, blk, 0, s, a);
   else hipLaunchKernelGGL((bsa_bwd_f32_kernel<kKeys, 128>), grid, blk, 0, s, a);
   launch_merge<kKeys, float>(a, D, s);

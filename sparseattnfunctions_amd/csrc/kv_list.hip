@@ -176,8 +176,8 @@ __global__ __launch_bounds__(64 * kTransWaves) void transpose_lists_kernel(const
     for (int k = wave; k < min(kWin, nkb - kb0); k += kTransWaves) {
       // lane l: rows r0 + 2 (l + 64 i), + 1 of word l + 64 i, in order of i
       int at = pos[k];
-#pragma unroll
-      for (int i = 0; i < kRowChunk / 128; ++i) {
+      const int words = (min(nqb - r0, kRowChunk) + 1) / 2;
+      for (int i = 0; 64 * i < words; ++i) {
         const uint32_t word = seen[k][64 * i + lane];
         const int n0 = word & 0xffff, n1 = word >> 16;
         int sum = n0 + n1;

@@ -86,19 +86,42 @@ def _set(call, **tensors):
         call.strides[i:i + 3] = t.stride()[:3]
 
 
-def _call(q, k, v, kv: KVList, sm_scale: float, key_bias) -> "_lib.AttnTrain":
-    """The description of a call on checked, aligned inputs; key_bias expanded."""
-    B, H, Lq, D = q.shape
-    call = _lib.AttnTrain(dtype=_lib.DTYPES[q.dtype], B=B, H=H, Lq=Lq, Lk=k.shape[2], D=D, max_cnt=kv.max_cnt, parts=1,
-                          kv_idx=kv.idx.data_ptr(), kv_cnt=kv.cnt.data_ptr(), sm_scale=sm_scale)
-    _set(call, q=q, k=k, v=v)
+def _set_bias(call, key_bias):
     if key_bias is not None:
         call.key_bias = key_bias.data_ptr()
         call.bias_strides[:] = key_bias.stride()[:2]
-    return call
 
 
-def _forward(call, q, k, v, kv: KVList, n_text_blocks: int):
+_WORKSPACE_BYTES = {}
+
+
+class _Call:
+    """What the backward pass needs of a call beside its tensors: the description of the call on checked,
+    aligned inputs (key_bias expanded), its dispatch orders and the size of its workspace."""
+
+    def __init__(self, q, k, v, kv: KVList, sm_scale: float, key_bias, n_text_blocks: int):
+        B, H, Lq, D = q.shape
+        Lk = k.shape[2]
+        self.args = _lib.AttnTrain(dtype=_lib.DTYPES[q.dtype], B=B, H=H, Lq=Lq, Lk=Lk, D=D, max_cnt=kv.max_cnt, parts=1,
+                                   kv_idx=kv.idx.data_ptr(), kv_cnt=kv.cnt.data_ptr(), sm_scale=sm_scale)
+        _set(self.args, q=q, k=k, v=v)
+        _set_bias(self.args, key_bias)
+        self.shapes = (B, H, Lq, D), (B, H, Lk, D), (B, H, Lk, D)  # of the gradients, contiguous
+        sq, sk = (H * Lq * D, Lq * D, D), (H * Lk * D, Lk * D, D)
+        self.args.strides[15:24] = (*sq, *sk, *sk)
+        self.orders = [work_order(B, H, n, n_text_blocks, q.device) for n in (kv.nqb, kv.nkb)]
+        (self.args.q_order, self.args.n_q_slots), (self.args.k_order, self.args.n_k_slots) = (
+            (o.data_ptr(), o.numel()) for o in self.orders)
+        key = (self.args.dtype, B, H, Lq, Lk, D, kv.max_cnt)
+        self.bytes = _WORKSPACE_BYTES.get(key)
+        if self.bytes is None:
+            n = ctypes.c_int64(0)
+            _lib.check(_lib.load().sa_block_sparse_bwd_workspace(self.args, ctypes.byref(n)),
+                       "sa_block_sparse_bwd_workspace")
+            self.bytes = _WORKSPACE_BYTES[key] = n.value
+
+
+def _forward(call: _lib.AttnTrain, q, k, v, kv: KVList, n_text_blocks: int):
     """(out, lse) of a call."""
     B, H, Lq, D = q.shape
     n_items = B * H * kv.nqb
@@ -131,36 +154,18 @@ def _forward(call, q, k, v, kv: KVList, n_text_blocks: int):
     return out, lse
 
 
-_WORKSPACE_BYTES = {}
-
-
-def _backward(call, dout, q, kv_nqb: int, kv_nkb: int, n_text_blocks: int, needs):
-    """(dq, dk, dv), None where not needed, of a call whose operands, out and lse are set."""
+def _backward(args: _lib.AttnTrain, call: _Call, dout, needs):
+    """[dq, dk, dv], None where not needed; args describes the call with its operands, out and lse."""
     dout = _rows16(dout)
-    _set(call, dout=dout)
-    B, H, Lk, D = call.B, call.H, call.Lk, call.D
-    grads = [torch.empty(B, H, L, D, dtype=q.dtype, device=q.device) if n else None
-             for n, L in zip(needs, (call.Lq, Lk, Lk))]
-    for name, t in zip(("dq", "dk", "dv"), grads):
-        if t is None:
-            setattr(call, name, None)
-        else:
-            _set(call, **{name: t})
-    key = (call.dtype, B, H, call.Lq, Lk, D, call.max_cnt)
-    n = _WORKSPACE_BYTES.get(key)
-    if n is None:
-        b = ctypes.c_int64(0)
-        _lib.check(_lib.load().sa_block_sparse_bwd_workspace(call, ctypes.byref(b)), "sa_block_sparse_bwd_workspace")
-        n = _WORKSPACE_BYTES[key] = b.value
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    call.workspace, call.workspace_bytes = ws.data_ptr(), n
-    order = work_order(B, H, kv_nqb, n_text_blocks, q.device)
-    call.q_order, call.n_q_slots = order.data_ptr(), order.numel()
-    if kv_nkb != kv_nqb:
-        order = work_order(B, H, kv_nkb, n_text_blocks, q.device)
-    call.k_order, call.n_k_slots = order.data_ptr(), order.numel()
-    with _lib.on(q.device):
-        rc = _lib.load().sa_block_sparse_bwd(call, _lib.stream_of(q))
+    device = dout.device
+    args.dout = dout.data_ptr()
+    args.strides[12:15] = dout.stride()[:3]
+    grads = [torch.empty(shape, dtype=dout.dtype, device=device) if n else None for n, shape in zip(needs, call.shapes)]
+    args.dq, args.dk, args.dv = (t.data_ptr() if t is not None else None for t in grads)
+    ws = torch.empty(call.bytes, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), call.bytes
+    with _lib.on(device):
+        rc = _lib.load().sa_block_sparse_bwd(args, _lib.stream_of(dout))
     _lib.check(rc, "sa_block_sparse_bwd")
     return grads
 
@@ -189,7 +194,7 @@ def block_sparse_attention_lse(q, k, v, kv: KVList, sm_scale: float, key_bias: O
     key_bias = _check_inputs(q, k, v, kv, key_bias)
     with torch.no_grad():
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        return _forward(_call(q, k, v, kv, float(sm_scale), key_bias), q, k, v, kv, n_text_blocks)
+        return _forward(_Call(q, k, v, kv, float(sm_scale), key_bias, n_text_blocks).args, q, k, v, kv, n_text_blocks)
 
 
 def block_sparse_attention_backward(dout, q, k, v, out, lse, kv: KVList, sm_scale: float,
@@ -207,36 +212,38 @@ def block_sparse_attention_backward(dout, q, k, v, out, lse, kv: KVList, sm_scal
         raise ValueError("lse must be block_sparse_attention_lse's")
     with torch.no_grad():
         q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
-        call = _call(q, k, v, kv, float(sm_scale), key_bias)
-        _set(call, out=out)
-        call.lse = lse.data_ptr()
-        return tuple(_backward(call, dout, q, kv.nqb, kv.nkb, n_text_blocks, needs))
+        call = _Call(q, k, v, kv, float(sm_scale), key_bias, n_text_blocks)
+        _set(call.args, out=out)
+        call.args.lse = lse.data_ptr()
+        return tuple(_backward(call.args, call, dout, needs))
 
 
 class _TrainAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv, sm_scale, key_bias, n_text_blocks):
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        call = _call(q, k, v, kv, sm_scale, key_bias)
-        out, lse = _forward(call, q, k, v, kv, n_text_blocks)
-        ctx.save_for_backward(q, k, v, out, lse, kv.idx, kv.cnt, key_bias)
-        ctx.call, ctx.blocks = call, (kv.nqb, kv.nkb, n_text_blocks)
+        call = ctx.call = _Call(q, k, v, kv, sm_scale, key_bias, n_text_blocks)
+        out, lse = _forward(call.args, q, k, v, kv, n_text_blocks)
+        saved = (q, k, v, out, lse, kv.idx, kv.cnt, key_bias)
+        ctx.save_for_backward(*saved)
+        ctx.places = [(t.data_ptr(), t.stride()) for t in saved if t is not None]
         return out
 
     @staticmethod
     def backward(ctx, dout):
         if torch.is_grad_enabled():
             raise RuntimeError("block-sparse attention is differentiable once (create_graph=True is not supported)")
-        q, k, v, out, lse, kv_idx, kv_cnt, key_bias = ctx.saved_tensors
-        # A copy of the forward pass's description: this may run twice, or in two threads, and hooks on
-        # saved tensors may have moved them.
-        call = _lib.AttnTrain.from_buffer_copy(ctx.call)
-        _set(call, q=q, k=k, v=v, out=out)
-        call.lse, call.kv_idx, call.kv_cnt = lse.data_ptr(), kv_idx.data_ptr(), kv_cnt.data_ptr()
-        if key_bias is not None:
-            call.key_bias = key_bias.data_ptr()
-            call.bias_strides[:] = key_bias.stride()[:2]
-        return (*_backward(call, dout, q, *ctx.blocks, ctx.needs_input_grad[:3]), None, None, None, None)
+        saved = ctx.saved_tensors
+        # A copy of the forward pass's description: this may run twice, or in two threads.
+        args = _lib.AttnTrain.from_buffer_copy(ctx.call.args)
+        if ctx.places != [(t.data_ptr(), t.stride()) for t in saved if t is not None]:
+            # Hooks on saved tensors have moved them.
+            q, k, v, out, lse, kv_idx, kv_cnt, key_bias = saved
+            q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
+            _set(args, q=q, k=k, v=v, out=out)
+            args.lse, args.kv_idx, args.kv_cnt = lse.data_ptr(), kv_idx.data_ptr(), kv_cnt.data_ptr()
+            _set_bias(args, key_bias)
+        return (*_backward(args, ctx.call, dout, ctx.needs_input_grad[:3]), None, None, None, None)
 
 
 class _NoKeys(torch.autograd.Function):
