@@ -23,6 +23,7 @@ has zero gradients. The mask, the lists and key_bias are not differentiated.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -34,22 +35,21 @@ from .._kv import KVList, kv_list_from_mask
 from .block_sparse_attn_kernel import (BLOCK, F32_TERMS_BLOCKS, cell_kv_list, f32_terms_workspace, shares_text_rows,
                                        split_parts, split_workspace_bytes, work_order)
 
-_TYPES = (torch.bfloat16, torch.float16, torch.float32)
-
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t with a contiguous last axis and 16-byte aligned rows (a copy where it has not)."""
-    per16 = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s < 0 or s % per16 for s in t.stride()[:-1]):
+    """t [B,H,L,D] with a contiguous last axis and 16-byte aligned rows (a copy where it has not)."""
+    sb, sh, sl, sd = t.stride()
+    if sd != 1 or (sb | sh | sl) * t.element_size() % 16 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _check_inputs(q, k, v, kv: KVList, key_bias):
-    _lib.require_gpu(q, k, v, key_bias, kv.idx, kv.cnt)
+    tensors = (q, k, v, kv.idx, kv.cnt) if key_bias is None else (q, k, v, kv.idx, kv.cnt, key_bias)
+    _lib.require_gpu(*tensors)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"q, k, v must be [B, H, L, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if q.dtype not in _TYPES or not q.dtype == k.dtype == v.dtype:
+    if q.dtype not in _lib.DTYPES or not q.dtype == k.dtype == v.dtype:
         raise TypeError(f"q, k, v must share one of bf16, fp16 and fp32, got {q.dtype}, {k.dtype}, {v.dtype}")
     B, H, Lq, D = q.shape
     Lk = k.shape[2]
@@ -57,10 +57,13 @@ def _check_inputs(q, k, v, kv: KVList, key_bias):
         raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
     if D not in (64, 128):
         raise NotImplementedError(f"head_dim {D} (64 or 128)")
-    if any(x is not None and x.device != q.device for x in (k, v, key_bias, kv.idx, kv.cnt)):
-        raise ValueError("q, k, v, the lists and key_bias must be on one device")
-    nqb, nkb = math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK)
-    if (kv.B, kv.H, kv.nqb, kv.nkb) != (B, H, nqb, nkb) or kv.rows != B * H * nqb:
+    device = q.device
+    for t in tensors:
+        if t.device != device:
+            raise ValueError("q, k, v, the lists and key_bias must be on one device")
+    nqb, nkb = (Lq + BLOCK - 1) // BLOCK, (Lk + BLOCK - 1) // BLOCK
+    if (kv.B, kv.H, kv.nqb, kv.nkb) != (B, H, nqb, nkb) or kv.cnt.numel() != B * H * nqb or kv.idx.dim() != 2 \
+            or kv.idx.shape[0] != B * H * nqb:
         raise ValueError(f"kv lists of {kv.B} x {kv.H} x {kv.nqb} x {kv.nkb} blocks, expected {B} x {H} x {nqb} x {nkb}")
     for t in (kv.idx, kv.cnt):
         if t.dtype != torch.int32 or not t.is_contiguous():
@@ -70,7 +73,8 @@ def _check_inputs(q, k, v, kv: KVList, key_bias):
             raise NotImplementedError("fp32 inputs: plain block lists only (no key_bias)")
         if key_bias.requires_grad:
             raise ValueError("key_bias is not differentiated; pass key_bias.detach()")
-        if key_bias.dtype != torch.float32 or key_bias.shape[-1] != Lk or key_bias.stride(-1) != 1:
+        if key_bias.dtype != torch.float32 or key_bias.dim() == 0 or key_bias.shape[-1] != Lk \
+                or (Lk > 1 and key_bias.stride(-1) != 1):
             raise ValueError("key_bias must be fp32 [B,H,Lk] with a contiguous key axis")
         key_bias = key_bias.expand(B, H, Lk)
     return key_bias
@@ -92,78 +96,84 @@ def _set_bias(call, key_bias):
         call.bias_strides[:] = key_bias.stride()[:2]
 
 
-_WORKSPACE_BYTES = {}
+class _Plan:
+    """What calls of one shape share: a description without pointers, launch variants, dispatch orders
+    and workspace sizes."""
 
-
-class _Call:
-    """What the backward pass needs of a call beside its tensors: the description of the call on checked,
-    aligned inputs (key_bias expanded), its dispatch orders and the size of its workspace."""
-
-    def __init__(self, q, k, v, kv: KVList, sm_scale: float, key_bias, n_text_blocks: int):
-        B, H, Lq, D = q.shape
-        Lk = k.shape[2]
-        self.args = _lib.AttnTrain(dtype=_lib.DTYPES[q.dtype], B=B, H=H, Lq=Lq, Lk=Lk, D=D, max_cnt=kv.max_cnt, parts=1,
-                                   kv_idx=kv.idx.data_ptr(), kv_cnt=kv.cnt.data_ptr(), sm_scale=sm_scale)
-        _set(self.args, q=q, k=k, v=v)
-        _set_bias(self.args, key_bias)
-        self.shapes = (B, H, Lq, D), (B, H, Lk, D), (B, H, Lk, D)  # of the gradients, contiguous
+    def __init__(self, dtype, device, q_shape, Lk, q_strides, k_strides, v_strides, max_cnt, row_blocks, biased, sm_scale,
+                 n_text_blocks):
+        B, H, Lq, D = q_shape
+        nqb, nkb = math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK)
+        n_items = B * H * nqb
+        args = self.args = _lib.AttnTrain(dtype=_lib.DTYPES[dtype], B=B, H=H, Lq=Lq, Lk=Lk, D=D, max_cnt=max_cnt, parts=1,
+                                          sm_scale=sm_scale)
+        self.out, self.lse = (B, H, Lq, D), (B, H, nqb * BLOCK)
+        self.grads = (B, H, Lq, D), (B, H, Lk, D), (B, H, Lk, D)
         sq, sk = (H * Lq * D, Lq * D, D), (H * Lk * D, Lk * D, D)
-        self.args.strides[15:24] = (*sq, *sk, *sk)
-        self.orders = [work_order(B, H, n, n_text_blocks, q.device) for n in (kv.nqb, kv.nkb)]
-        (self.args.q_order, self.args.n_q_slots), (self.args.k_order, self.args.n_k_slots) = (
-            (o.data_ptr(), o.numel()) for o in self.orders)
-        key = (self.args.dtype, B, H, Lq, Lk, D, kv.max_cnt)
-        self.bytes = _WORKSPACE_BYTES.get(key)
-        if self.bytes is None:
-            n = ctypes.c_int64(0)
-            _lib.check(_lib.load().sa_block_sparse_bwd_workspace(self.args, ctypes.byref(n)),
-                       "sa_block_sparse_bwd_workspace")
-            self.bytes = _WORKSPACE_BYTES[key] = n.value
-
-
-def _forward(call: _lib.AttnTrain, q, k, v, kv: KVList, n_text_blocks: int):
-    """(out, lse) of a call."""
-    B, H, Lq, D = q.shape
-    n_items = B * H * kv.nqb
-    out = torch.empty(B, H, Lq, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, kv.nqb * BLOCK, dtype=torch.float32, device=q.device)
-    # The launch variants of block_sparse_attention: key-range parts for few blocks over long lists,
-    # else a work order; fp32 on split operands where it takes them.
-    ws = None
-    if q.dtype == torch.float32:
-        if kv.nqb >= F32_TERMS_BLOCKS:
-            ws = f32_terms_workspace(B, H, k.shape[2], D, q.device)
-    elif not call.key_bias:
-        call.parts = split_parts(n_items, kv.max_cnt, D)
-        if call.parts > 1:
-            ws = torch.empty(split_workspace_bytes(n_items, D, call.parts), dtype=torch.uint8, device=q.device)
-    if call.parts == 1:
+        args.strides[:] = (*q_strides[:3], *k_strides[:3], *v_strides[:3], *sq, 0, 0, 0, *sq, *sk, *sk)
+        # The forward pass takes block_sparse_attention's launch variants: key-range parts for few blocks
+        # over long lists, else a work order; fp32 split operands where it takes them.
+        self.terms = dtype == torch.float32 and nqb >= F32_TERMS_BLOCKS
+        if dtype != torch.float32 and not biased:
+            args.parts = split_parts(n_items, max_cnt, D)
+        self.forward_bytes = split_workspace_bytes(n_items, D, args.parts) if args.parts > 1 else 0
         # Lists of unknown length count as short ones beside the text rows': [1, 15, 17776, 64] with a
         # fifth of the blocks 376 / 338 us without / with shared text rows, [1, 30, 4546, 64] 91 / 73 (were
         # they all long after all: [1, 15, 17776, 64] dense 1 185 / 1 364).
-        row_blocks = kv.row_blocks if kv.row_blocks is not None or kv.dense else 0.0
-        share_text = q.dtype != torch.float32 and shares_text_rows(n_items, kv.nkb, n_text_blocks, row_blocks, D)
-        order = work_order(B, H, kv.nqb, n_text_blocks, q.device, share_text)
-        call.fwd_order, call.n_fwd_slots = order.data_ptr(), order.numel()
-    call.workspace, call.workspace_bytes = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
-    _set(call, out=out)
-    call.lse = lse.data_ptr()
-    with _lib.on(q.device):
-        rc = _lib.load().sa_block_sparse_fwd_lse(call, _lib.stream_of(q))
+        share_text = dtype != torch.float32 and shares_text_rows(n_items, nkb, n_text_blocks, row_blocks, D)
+        self.orders = [work_order(B, H, nqb, n_text_blocks, device, share_text), work_order(B, H, nqb, n_text_blocks, device),
+                       work_order(B, H, nkb, n_text_blocks, device)]
+        for name, order in zip(("fwd", "q", "k"), self.orders):
+            setattr(args, name + "_order", order.data_ptr())
+            setattr(args, "n_" + name + "_slots", order.numel())
+        n = ctypes.c_int64(0)
+        _lib.check(_lib.load().sa_block_sparse_bwd_workspace(args, ctypes.byref(n)), "sa_block_sparse_bwd_workspace")
+        self.backward_bytes = n.value
+
+
+_plan = functools.lru_cache(maxsize=1024)(_Plan)
+
+
+def _describe(q, k, v, kv: KVList, sm_scale: float, key_bias, n_text_blocks: int):
+    """(plan, description) of a call on checked, aligned inputs; key_bias expanded."""
+    row_blocks = kv.row_blocks if kv.row_blocks is not None or kv.dense else 0.0
+    plan = _plan(q.dtype, q.device, q.shape, k.shape[2], q.stride(), k.stride(), v.stride(), kv.idx.shape[1], row_blocks,
+                 key_bias is not None, sm_scale, n_text_blocks)
+    args = _lib.AttnTrain.from_buffer_copy(plan.args)
+    args.q, args.k, args.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    args.kv_idx, args.kv_cnt = kv.idx.data_ptr(), kv.cnt.data_ptr()
+    _set_bias(args, key_bias)
+    return plan, args
+
+
+def _forward(plan: _Plan, args: _lib.AttnTrain, q):
+    """(out, lse) of a call, whose description then has them."""
+    device = q.device
+    out = torch.empty(plan.out, dtype=q.dtype, device=device)
+    lse = torch.empty(plan.lse, dtype=torch.float32, device=device)
+    ws = None
+    if plan.terms:
+        ws = f32_terms_workspace(args.B, args.H, args.Lk, args.D, device)
+    elif plan.forward_bytes:
+        ws = torch.empty(plan.forward_bytes, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
+    args.out, args.lse = out.data_ptr(), lse.data_ptr()
+    with _lib.on(device):
+        rc = _lib.load().sa_block_sparse_fwd_lse(args, _lib.stream_of(q))
     _lib.check(rc, "sa_block_sparse_fwd_lse")
     return out, lse
 
 
-def _backward(args: _lib.AttnTrain, call: _Call, dout, needs):
+def _backward(plan: _Plan, args: _lib.AttnTrain, dout, needs):
     """[dq, dk, dv], None where not needed; args describes the call with its operands, out and lse."""
     dout = _rows16(dout)
     device = dout.device
     args.dout = dout.data_ptr()
     args.strides[12:15] = dout.stride()[:3]
-    grads = [torch.empty(shape, dtype=dout.dtype, device=device) if n else None for n, shape in zip(needs, call.shapes)]
+    grads = [torch.empty(shape, dtype=dout.dtype, device=device) if n else None for n, shape in zip(needs, plan.grads)]
     args.dq, args.dk, args.dv = (t.data_ptr() if t is not None else None for t in grads)
-    ws = torch.empty(call.bytes, dtype=torch.uint8, device=device)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), call.bytes
+    ws = torch.empty(plan.backward_bytes, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), plan.backward_bytes
     with _lib.on(device):
         rc = _lib.load().sa_block_sparse_bwd(args, _lib.stream_of(dout))
     _lib.check(rc, "sa_block_sparse_bwd")
@@ -194,7 +204,7 @@ def block_sparse_attention_lse(q, k, v, kv: KVList, sm_scale: float, key_bias: O
     key_bias = _check_inputs(q, k, v, kv, key_bias)
     with torch.no_grad():
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        return _forward(_Call(q, k, v, kv, float(sm_scale), key_bias, n_text_blocks).args, q, k, v, kv, n_text_blocks)
+        return _forward(*_describe(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks)), q)
 
 
 def block_sparse_attention_backward(dout, q, k, v, out, lse, kv: KVList, sm_scale: float,
@@ -212,18 +222,18 @@ def block_sparse_attention_backward(dout, q, k, v, out, lse, kv: KVList, sm_scal
         raise ValueError("lse must be block_sparse_attention_lse's")
     with torch.no_grad():
         q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
-        call = _Call(q, k, v, kv, float(sm_scale), key_bias, n_text_blocks)
-        _set(call.args, out=out)
-        call.args.lse = lse.data_ptr()
-        return tuple(_backward(call.args, call, dout, needs))
+        plan, args = _describe(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
+        _set(args, out=out)
+        args.lse = lse.data_ptr()
+        return tuple(_backward(plan, args, dout, needs))
 
 
 class _TrainAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv, sm_scale, key_bias, n_text_blocks):
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        call = ctx.call = _Call(q, k, v, kv, sm_scale, key_bias, n_text_blocks)
-        out, lse = _forward(call.args, q, k, v, kv, n_text_blocks)
+        ctx.plan, ctx.args = _describe(q, k, v, kv, sm_scale, key_bias, n_text_blocks)
+        out, lse = _forward(ctx.plan, ctx.args, q)
         saved = (q, k, v, out, lse, kv.idx, kv.cnt, key_bias)
         ctx.save_for_backward(*saved)
         ctx.places = [(t.data_ptr(), t.stride()) for t in saved if t is not None]
@@ -235,7 +245,7 @@ class _TrainAttention(torch.autograd.Function):
             raise RuntimeError("block-sparse attention is differentiable once (create_graph=True is not supported)")
         saved = ctx.saved_tensors
         # A copy of the forward pass's description: this may run twice, or in two threads.
-        args = _lib.AttnTrain.from_buffer_copy(ctx.call.args)
+        args = _lib.AttnTrain.from_buffer_copy(ctx.args)
         if ctx.places != [(t.data_ptr(), t.stride()) for t in saved if t is not None]:
             # Hooks on saved tensors have moved them.
             q, k, v, out, lse, kv_idx, kv_cnt, key_bias = saved
@@ -243,7 +253,7 @@ class _TrainAttention(torch.autograd.Function):
             _set(args, q=q, k=k, v=v, out=out)
             args.lse, args.kv_idx, args.kv_cnt = lse.data_ptr(), kv_idx.data_ptr(), kv_cnt.data_ptr()
             _set_bias(args, key_bias)
-        return (*_backward(args, ctx.call, dout, ctx.needs_input_grad[:3]), None, None, None, None)
+        return (*_backward(ctx.plan, args, dout, ctx.needs_input_grad[:3]), None, None, None, None)
 
 
 class _NoKeys(torch.autograd.Function):
@@ -286,7 +296,7 @@ def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Option
     B, H, Lq, D = q.shape
     Lk = k.shape[2]
     if B * H * Lq == 0 or Lk == 0:
-        if q.dtype not in _TYPES or not q.dtype == k.dtype == v.dtype:
+        if q.dtype not in _lib.DTYPES or not q.dtype == k.dtype == v.dtype:
             raise TypeError(f"q, k, v must share one of bf16, fp16 and fp32, got {q.dtype}, {k.dtype}, {v.dtype}")
         if k.shape != (B, H, Lk, D) or v.shape != (B, H, Lk, D):
             raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
