@@ -16,6 +16,8 @@ __all__ = ["install_alias"]
 _SUBMODULES = (
     "utils",
     "utils.block_sparse_attn_kernel",
+    "utils.block_sparse_attn_grad",
+    "utils.rotary",
     "utils.merge_unmerge",
     "utils.mask_related",
     "utils.attn_pooling_kernel",

@@ -16,6 +16,11 @@ Differences from the reference, by design:
     preprocess_qkv, the first frame's inner block mask, their Kronecker fusion with dense text
     blocks, block-sparse attention and the inverse layout -- each a HIP kernel here (see
     utils/mask_related.py); it draws the same torch random numbers in the same order.
+
+Beyond the reference, `trainable=True` makes the output differentiable in q, k and v (the block mask
+is chosen from their values and not differentiated; utils/block_sparse_attn_grad.py), and `rotary`
+turns q and k by their positions first (`utils.rotary.VideoRotary`, or any callable of q and k that
+returns both); `forward_backup` takes neither.
 """
 from __future__ import annotations
 
@@ -25,6 +30,7 @@ import torch
 
 from ._kv import KVList, kv_list_from_mask
 from .block_masks import meanpool_topk_kv_list
+from .utils.block_sparse_attn_grad import block_sparse_attention_train
 from .utils.block_sparse_attn_kernel import block_sparse_attention
 from .workloads import COGVIDEOX_2B, Geometry, topk_count
 
@@ -38,13 +44,15 @@ def dense_kv_list(B: int, H: int, nqb: int, nkb: int, device) -> KVList:
 
 class BlockSparseAttention:
     def __init__(self, block_size: int = 64, keep_ratio: float = 0.2, geometry: Geometry = COGVIDEOX_2B,
-                 sm_scale: float = 1 / 8):
+                 sm_scale: float = 1 / 8, trainable: bool = False, rotary=None):
         if block_size != 64:
             raise NotImplementedError("the MI355X kernel uses 64-token blocks")
         self.block_size = block_size
         self.sm_scale = sm_scale
         self.keep_ratio = keep_ratio
         self.geometry = geometry
+        self.trainable = trainable
+        self.rotary = rotary
         self.last_kv = None  # kv lists of the last call (sparsity statistics)
 
     def n_text_blocks(self) -> int:
@@ -58,15 +66,22 @@ class BlockSparseAttention:
                                      block=self.block_size, with_fp16_keys=with_fp16_keys)
 
     def forward(self, q, k, v):
+        if self.rotary is not None:
+            q, k = self.rotary(q, k)
+        if self.trainable:
+            self.last_kv = kv = self.build_kv_list(q.detach(), k.detach())
+            return block_sparse_attention_train(q, k, v, kv, self.sm_scale, n_text_blocks=self.n_text_blocks())
         kv, k16 = self.build_kv_list(q, k, with_fp16_keys=True)
         self.last_kv = kv
         return block_sparse_attention(q, k, v, kv, self.sm_scale, n_text_blocks=self.n_text_blocks(), k16=k16)
 
     def forward_dense(self, q, k, v):
+        if self.rotary is not None:
+            q, k = self.rotary(q, k)
         B, H, L, _ = q.shape
         nb = math.ceil(L / self.block_size)
-        return block_sparse_attention(q, k, v, dense_kv_list(B, H, nb, math.ceil(k.shape[2] / 64), q.device),
-                                      self.sm_scale)
+        attend = block_sparse_attention_train if self.trainable else block_sparse_attention
+        return attend(q, k, v, dense_kv_list(B, H, nb, math.ceil(k.shape[2] / 64), q.device), self.sm_scale)
 
     def forward_backup(self, q, k, v, frame_draws=None, starts=None):
         """block_mask_attn.py:11-20: frame-level mask (generate_attention_mask_frame_scope),
@@ -75,6 +90,8 @@ class BlockSparseAttention:
         attention on the processed layout and reverse_process_out. `frame_draws` / `starts`
         replace the two torch.randint draws (CPU: 60 first-frame positions; GPU: the (B, 13)
         truncation offsets) when given."""
+        if self.trainable or self.rotary is not None:
+            raise NotImplementedError("forward_backup has no gradients and no rotary positions")
         from .utils.mask_related import (generate_attention_mask_frame_scope, get_block_mask, get_inner_frame_mask,
                                          preprocess_qkv, reverse_process_out)
 

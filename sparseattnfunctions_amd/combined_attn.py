@@ -25,6 +25,10 @@ the combined rule in the rearranged layout, as the reference's block-sparse head
 estimated there: block means of the permuted q and k for the global top-k, the local window
 between the original (t, h, w) of the permuted blocks' centre tokens, the blocks holding text
 (last in that layout) dense; the output is recovered to the natural order.
+
+Beyond the reference, `trainable=True` makes the output differentiable in q, k and v (in the natural
+order, without head routing; utils/block_sparse_attn_grad.py), and `rotary` turns q and k by their
+positions first (`utils.rotary.VideoRotary`, or any callable of q and k that returns both).
 """
 from __future__ import annotations
 
@@ -35,6 +39,7 @@ import torch
 from ._gather import gather_tokens
 from .block_mask_attn import dense_kv_list
 from .block_masks import local_window_bitmap, local_window_bitmap_perm, meanpool_topk_kv_list
+from .utils.block_sparse_attn_grad import block_sparse_attention_train
 from .utils.block_sparse_attn_kernel import block_sparse_attention
 from .workloads import COGVIDEOX_2B, Geometry, topk_count
 
@@ -79,7 +84,12 @@ def _perms(device):
 class CombinedAttn:
     def __init__(self, warmup_epoch: int = 5, geometry: Geometry = COGVIDEOX_2B, global_ratio: float = 0.10,
                  window=(1, 8, 8), layer_num: int = 42, timestep: int = 50, sm_scale: float = None,
-                 head_routing: bool = False, pattern_geometry=None, verbose: bool = False):
+                 head_routing: bool = False, pattern_geometry=None, verbose: bool = False, trainable: bool = False,
+                 rotary=None):
+        if trainable and head_routing:
+            raise NotImplementedError("head routing has no gradients")
+        self.trainable = trainable
+        self.rotary = rotary
         self.layer_num = layer_num
         self.timestep = timestep
         self.counter = 0
@@ -203,6 +213,10 @@ class CombinedAttn:
         return meanpool_topk_kv_list(qr, kr, topk_count(self.global_ratio, nb), 0, local_bitmap=local)
 
     def __call__(self, q, k, v, use_rearranger: bool = False):
+        if self.trainable and use_rearranger:
+            raise NotImplementedError("the rearranged layout has no gradients")
+        if self.rotary is not None:
+            q, k = self.rotary(q, k)
         if self.head_routing:
             return self._routed(q, k, v, use_rearranger)
         warm = self.ct // self.layer_num < self.warmup_epoch
@@ -222,9 +236,10 @@ class CombinedAttn:
         else:
             # bf16 scores: these lists (31-46 blocks of 278) earn less in the tile loop than the
             # fp16 copy of k costs the pooling pass
-            kv = self.build_kv_list(q, k)
+            kv = self.build_kv_list(q.detach(), k.detach())
         self.last_kv = kv
-        return block_sparse_attention(q, k, v, kv, self._scale(q), n_text_blocks=self.n_text_blocks())
+        attend = block_sparse_attention_train if self.trainable else block_sparse_attention
+        return attend(q, k, v, kv, self._scale(q), n_text_blocks=self.n_text_blocks())
 
     def sparsity(self) -> float:
         kv = self.last_kv

@@ -7,7 +7,8 @@ that step:
   * `rotary_table(positions, axes)`: the cosines and sines of a sequence's positions, made once per
     geometry (`sa_rotary_table`); `video_positions(geometry)` are those of a video;
   * `apply_rotary(q, k, table)`: q and k turned in one launch (`sa_rotary_apply`), differentiable;
-    `apply_rotary_(q, k, table)` does it in place.
+    `apply_rotary_(q, k, table)` does it in place;
+  * `VideoRotary(geometry)`: both for a video, as the processors take it.
 
 A head's first 2 * pairs values turn in pairs, (a, b) -> (a cos - b sin, b cos + a sin), computed in
 fp32 and rounded once; the others stay. Layouts: "interleaved" pairs values 2i and 2i + 1, "half"
@@ -127,6 +128,52 @@ def video_positions(geometry, device=None) -> torch.Tensor:
     t, h, w = torch.meshgrid(*(torch.arange(n, dtype=torch.int32, device=device)
                                for n in (geometry.T, geometry.Hp, geometry.Wp)), indexing="ij")
     return torch.stack((t.reshape(-1), h.reshape(-1), w.reshape(-1)))
+
+
+class VideoRotary:
+    """The rotary positions of a video's tokens, as a processor's `rotary`: `rotary(q, k)` is
+    `apply_rotary` with the table of `geometry` (a `workloads.Geometry`), its text tokens left alone.
+
+    `axes` are the values of a head that turn with t, h and w (`rotary_table`); `positions` ([3,
+    n_video]) replaces `video_positions`, e.g. for a grid rescaled to the trained one. The table of a
+    device is made by its first call, which waits for it, so that later calls may run on any stream; a call
+    captured into a graph needs one before."""
+
+    def __init__(self, geometry, axes: Sequence[int] = (16, 24, 24), theta: float = 10000.0,
+                 scaling: Optional[dict] = None, layout: str = "interleaved",
+                 positions: Optional[torch.Tensor] = None):
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
+        if len(axes) != 3:
+            raise ValueError(f"axes {tuple(axes)}: one number of values each for t, h and w")
+        _frequency_arrays(tuple(axes), float(theta), tuple(sorted(scaling.items())) if scaling is not None else None)
+        if positions is not None and tuple(positions.shape) != (3, geometry.n_video):
+            raise ValueError(f"positions of shape {tuple(positions.shape)}, expected (3, {geometry.n_video})")
+        self.geometry, self.axes, self.theta, self.scaling = geometry, tuple(axes), theta, scaling
+        self.layout, self.positions = layout, positions
+        self._tables = {}  # device -> (table, the stream it was made on)
+
+    def table(self, device) -> torch.Tensor:
+        device = torch.device(device)
+        if device.index is None:
+            device = torch.device(device.type, torch.cuda.current_device())
+        made = self._tables.get(device)
+        if made is None:
+            positions = self.positions
+            if positions is None:
+                positions = video_positions(self.geometry)
+            stream = torch.cuda.current_stream(device)
+            table = rotary_table(positions.to(device), self.axes, self.theta, self.scaling)
+            stream.synchronize()
+            made = self._tables[device] = (table, stream)
+        table, stream = made
+        here = torch.cuda.current_stream(device)
+        if here != stream:
+            table.record_stream(here)
+        return table
+
+    def __call__(self, q, k):
+        return apply_rotary(q, k, self.table(q.device), layout=self.layout, skip=self.geometry.text_len)
 
 
 def _check(q, k, table, layout, skip, rows):
