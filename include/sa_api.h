@@ -273,7 +273,8 @@ int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
  * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type.
  *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype and max_cnt): the query
  *             rows' statistics, the transposed lists, sums of lists split over workgroups.
- * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv.
+ * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv, sm_scale
+ * at least 1e-30.
  */
 int sa_block_sparse_bwd_workspace(const sa_attn_train* call, int64_t* bytes);
 int sa_block_sparse_bwd(const sa_attn_train* call, void* stream);

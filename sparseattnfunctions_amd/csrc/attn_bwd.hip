@@ -121,7 +121,7 @@ __device__ inline const __attribute__((address_space(4))) int32_t* bwd_list(cons
 // kParts: pairs per workgroup, each on its share of the item's list; their sums are added in LDS, in
 // order, at the end.
 template <bool kKeys, bool kBias, typename T, int kD, int kParts>
-__global__ __launch_bounds__(128 * kParts, kD == 64 && kParts < 4 ? 3 : 2) void bsa_bwd_kernel(BwdArgs a) {
+__global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel(BwdArgs a) {
   typedef Elem<T> E;
   typedef typename E::v8 v8;
   constexpr int kDS = kD / 16;      // 16-wide d steps of the first products
@@ -732,39 +732,38 @@ void launch_parts(const BwdArgs& a, hipStream_t s) {
 }
 
 // Pairs per item, by the number of items and the lists' width (how many entries they hold the host does
-// not know). One, two or four pairs, us of the query pass (the key pass is alike):
-//   head dim 64, dense lists of 40: 40 items 41 / 23 / 19, 160 43 / 24 / 21, 320 47 / 32 / 40, 1 280
-//     93 / 86 / 107, 1 920 141 / 132 / 166; of 10: 40 items 13.8 / 10.3 / 10.6, 640 20 / 20 / 28, 1 500
-//     33 / 36 / 55; lists of 5 of 40: 640 items 19 / 17 / 24, 1 920 32 / 33 / 59, 3 200 45 / 51 / 93;
-//     28 of 278: 278 items 51 / 30 / 34, 2 224 120 / 115 / 154;
-//   head dim 128, dense lists of 40: 40 items 60 / 38 / 36, 160 62 / 41 / 37, 320 82 / 59 / 73, 640 98 / 100 /
-//     112, 1 280 178 / 165 / 203, 1 920 239 / 245 / 299; of 10: 320 27 / 24 / 33, 640 34 / 37 / 50; 28 of
-//     278: 1 112 139 / 125 / 149, 2 224 225 / 232 / 275.
+// not know). One or two pairs, us of the query pass (the key pass is alike; four pairs, one workgroup per
+// CU: slower in every case but those that splits_of takes):
+//   head dim 64, dense lists of 40: 160 items 43 / 24, 320 47 / 32, 1 280 93 / 86, 1 920 141 / 132; of 10:
+//     40 items 13.8 / 10.3, 640 20 / 20, 1 500 33 / 36; lists of 5 of 40: 640 items 19 / 17, 1 920 32 / 33, 3 200
+//     45 / 51; 28 of 278: 278 items 51 / 30, 2 224 120 / 115;
+//   head dim 128, dense lists of 40: 160 items 62 / 41, 320 82 / 59, 640 98 / 100, 1 280 178 / 165, 1 920 239 /
+//     245; of 10: 320 27 / 24, 640 34 / 37; 28 of 278: 1 112 139 / 125, 2 224 225 / 232.
 // (Lists much longer than the others, of text blocks say, gain further by a second pair: [1, 15, 17776,
 // 64] with 4 of 278 blocks dense 449 / 431 us.)
 int pairs_per_item(int n_items, int max_cnt, int D) {
-  if (n_items <= 160 && max_cnt >= 32) return 4;
   if (D == 64) return n_items > 768 && max_cnt <= 16 ? 1 : 2;
   return n_items <= 512 || (n_items <= 1536 && max_cnt >= 32) ? 2 : 1;
 }
 
-// Splits of each item's list over workgroups, where the items leave most of the card idle and their
-// lists (of up to `width` entries) are long: at least 8 entries each, 2 in fp32, whose entries take 16 times
-// as long. Without / with, us of the query pass of 64 queries and the key pass of 64 keys against 17 776
-// of the other: one head 93 / 9 and 114 / 10, 30 heads 112 / 27 and 120 / 29; fp32, one head 594 / 36 and 1
-// 076 / 48; [1, 1, 2048, 64], 8 of 32 blocks, 10.3 / 7.0 and 10.9 / 8.0.
+// Splits of each item's list over workgroups of two pairs, where the items leave most of the card idle
+// and their lists (of up to `width` entries) are long: at least 8 entries each. Without / with, us of the
+// query pass of 64 queries and the key pass of 64 keys against 17 776 of the other: one head 93 / 9 and 114 / 10,
+// 30 heads 112 / 27 and 120 / 29; fp32, one head 594 / 36 and 1 076 / 48; [1, 1, 2048, 64], 8 of 32 blocks, 10.3 /
+// 7.0 and 10.9 / 8.0. The merge is 4 us more: two to five splits gain no more than that (160 items with dense
+// lists of 40: 24.2 / 21.2 and the merge), but in fp32, whose steps take 16 times as long.
 int splits_of(int64_t n_items, int width, int D, bool f32) {
-  if (width < (f32 ? 8 : 32)) return 1;
-  // workgroups of two pairs that the card holds at once
-  const int64_t slots = f32 ? (D == 64 ? 512 : 256) : (D == 64 ? 768 : 512);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({slots / n_items, width / (f32 ? 2 : 8), 32}));
+  if (width < (f32 ? 16 : 32)) return 1;
+  const int64_t slots = f32 ? (D == 64 ? 512 : 256) : (D == 64 ? 768 : 512);  // such workgroups on the card
+  const int64_t fit = slots / n_items;
+  if (fit < (f32 ? 4 : 6)) return 1;
+  return (int)std::min<int64_t>({fit, width / 8, 32});
 }
 
 template <bool kKeys, typename T, int kD>
 void launch_pass(const BwdArgs& a, int width, hipStream_t s) {
   const int parts = a.splits > 1 ? 2 : pairs_per_item(a.n_items, width, kD);
-  if (parts == 4) launch_parts<kKeys, T, kD, 4>(a, s);
-  else if (parts == 2) launch_parts<kKeys, T, kD, 2>(a, s);
+  if (parts == 2) launch_parts<kKeys, T, kD, 2>(a, s);
   else launch_parts<kKeys, T, kD, 1>(a, s);
   launch_merge<kKeys, T>(a, kD, s);
 }
@@ -839,6 +838,8 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   const int B = t->B, H = t->H, Lq = t->Lq, Lk = t->Lk, D = t->D;
   SA_REQUIRE(t->q && t->k && t->v && t->out && t->dout && t->lse && t->kv_idx && t->kv_cnt, "%s: null pointer", fn);
   SA_REQUIRE(std::isfinite(t->sm_scale) && t->sm_scale > 0.f, "%s: sm_scale must be finite and > 0", fn);
+  // (the key pass takes the rows' sums in units of the scores, lse / sm_scale)
+  if (t->sm_scale < 1e-30f) return sa::fail(SA_ERR_UNSUPPORTED, "%s: sm_scale %g below 1e-30", fn, t->sm_scale);
   const bool f32 = t->dtype == SA_DTYPE_F32;
   if (f32 && t->key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
   const int nqb = sa::cdiv(Lq, kBlk), nkb = sa::cdiv(Lk, kBlk);

@@ -44,7 +44,8 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _check_inputs(q, k, v, kv: KVList, key_bias):
+def _check_inputs(q, k, v, kv: KVList, key_bias, own_lists: bool = False):
+    """key_bias expanded; `own_lists`: the lists were made here for these shapes."""
     tensors = (q, k, v, kv.idx, kv.cnt) if key_bias is None else (q, k, v, kv.idx, kv.cnt, key_bias)
     _lib.require_gpu(*tensors)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -62,12 +63,14 @@ def _check_inputs(q, k, v, kv: KVList, key_bias):
         if t.device != device:
             raise ValueError("q, k, v, the lists and key_bias must be on one device")
     nqb, nkb = (Lq + BLOCK - 1) // BLOCK, (Lk + BLOCK - 1) // BLOCK
-    if (kv.B, kv.H, kv.nqb, kv.nkb) != (B, H, nqb, nkb) or kv.cnt.numel() != B * H * nqb or kv.idx.dim() != 2 \
+    if own_lists:
+        pass
+    elif (kv.B, kv.H, kv.nqb, kv.nkb) != (B, H, nqb, nkb) or kv.cnt.numel() != B * H * nqb or kv.idx.dim() != 2 \
             or kv.idx.shape[0] != B * H * nqb:
         raise ValueError(f"kv lists of {kv.B} x {kv.H} x {kv.nqb} x {kv.nkb} blocks, expected {B} x {H} x {nqb} x {nkb}")
-    for t in (kv.idx, kv.cnt):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError("kv lists must be contiguous int32 tensors")
+    elif kv.idx.dtype != torch.int32 or kv.cnt.dtype != torch.int32 or not kv.idx.is_contiguous() \
+            or not kv.cnt.is_contiguous():
+        raise ValueError("kv lists must be contiguous int32 tensors")
     if key_bias is not None:
         if q.dtype == torch.float32:
             raise NotImplementedError("fp32 inputs: plain block lists only (no key_bias)")
@@ -307,4 +310,5 @@ def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Option
         raise NotImplementedError(f"gradients of {BLOCK_M} x {BLOCK_N} blocks: blocks smaller than 64")
     else:
         kv, _ = cell_kv_list(block_sparse_mask, B, H, Lq, Lk, int(BLOCK_M), int(BLOCK_N))
-    return block_sparse_attention_train(q, k, v, kv, sm_scale, key_bias, n_text_blocks)
+    key_bias = _check_inputs(q, k, v, kv, key_bias, own_lists=True)
+    return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))

@@ -253,6 +253,10 @@ class _ApplyRotary(torch.autograd.Function):
     def backward(ctx, dq, dk):
         table, rows = ctx.saved_tensors
         layout, skip, inverse = ctx.args
+        if not ctx.needs_input_grad[0]:
+            dq = None
+        if not ctx.needs_input_grad[1]:
+            dk = None
         if dq is None and dk is None:
             return (None,) * 7
         # The transpose turns back; linear, so it is differentiable itself.
@@ -279,7 +283,8 @@ def apply_rotary(q, k, table, layout: str = "interleaved", skip: int = 0, rows: 
 def apply_rotary_(q, k, table, layout: str = "interleaved", skip: int = 0, rows: Optional[torch.Tensor] = None,
                   inverse: bool = False):
     """`apply_rotary` in place (values that do not turn are not touched); returns (q, k). Not for tensors
-    that autograd follows, nor for ones whose elements share memory."""
+    that autograd follows, nor for ones whose elements share memory, within one or between the two (views
+    of one fused tensor with values of their own may be turned)."""
     _check(q, k, table, layout, skip, rows)
     for x in (q, k):
         if x is None:

@@ -110,7 +110,8 @@ def test_c_argument_checks():
                 dict(workspace=16), dict(workspace_bytes=100), dict(q_order=256, n_q_slots=3), dict(k_order=256)):
         assert bwd(**bad) == _lib.SA_ERR_INVALID, bad
     for bad in (dict(D=96), dict(q=8), dict(dv=8), dict(stride=[0, 0, 65] * 8), dict(stride=[0, 0, 1 << 30] * 8),
-                dict(stride=[0, 0, -64] * 8), dict(dtype=2, key_bias=256), dict(max_cnt=65536, workspace_bytes=1 << 40)):
+                dict(stride=[0, 0, -64] * 8), dict(dtype=2, key_bias=256), dict(max_cnt=65536, workspace_bytes=1 << 40),
+                dict(sm_scale=1e-31)):
         assert bwd(**bad) == _lib.SA_ERR_UNSUPPORTED, bad
 
     def lse(**changed):
