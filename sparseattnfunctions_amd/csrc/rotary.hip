@@ -71,43 +71,21 @@ struct RotArgs {
   int group;            // heads per workgroup (of q's and k's together)
 };
 
-template <typename T>
-struct Vec8;  // eight values of a head as floats
-template <>
-struct Vec8<float> {
-  static __device__ inline void load(const void* p, float (&v)[8]) {
-    const float4 a = static_cast<const float4*>(p)[0], b = static_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  }
-  static __device__ inline void store(void* p, const float (&v)[8]) {
-    static_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    static_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  }
-};
-template <typename T>
-struct Vec8 {
-  typedef T t8 __attribute__((ext_vector_type(8)));
-  static __device__ inline void load(const void* p, float (&v)[8]) {
-    const t8 a = *static_cast<const t8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
-  }
-  static __device__ inline void store(void* p, const float (&v)[8]) {
-    t8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (T)v[i];  // round to nearest even
-    *static_cast<t8*>(p) = a;
-  }
+// N consecutive values of a head, moved together (16 bytes at most at a time).
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Chunk {
+  T v[N];
 };
 
-// A thread turns one unit of one token in every head of its group: interleaved, eight consecutive
-// values (four pairs); halves, eight values of each half (eight pairs). Units past the turned part
-// copy eight values. Loads of kUnroll heads are in flight together.
-template <typename T, bool kHalf>
+// A thread turns one unit of one token in every head of its group. Interleaved: V consecutive values
+// (V / 2 pairs, those past the last one left alone). Halves: V values of each half (V pairs); units past
+// the turned part copy 2 V values, in the same two accesses, so that the lanes of a wave stay together.
+// Loads of kUnroll heads are in flight together.
+template <typename T, bool kHalf, int V>
 __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
   constexpr int kUnroll = 4;
-  constexpr int kPairs = kHalf ? 8 : 4;
+  constexpr int kPairs = kHalf ? V : V / 2;
+  constexpr int kChunks = kHalf ? 2 : 1;
   const int unit = threadIdx.x % a.units;
   const int rest = threadIdx.x / a.units;
   const int slot = rest / a.tokens;
@@ -116,59 +94,62 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
   const int t = (blockIdx.x - b * token_groups) * a.tokens + (rest - slot * a.tokens);
   if (slot >= a.slots || t >= a.L) return;
   const int row = a.rows ? a.rows[b * a.rows_sb + t] : t - a.skip;
-  const int turned = kHalf ? a.pairs / 8 : a.pairs / 4;  // units that turn
+  const int turned = (a.pairs + kPairs - 1) / kPairs;  // units that turn (halves: whole ones)
   const bool turn = unit < turned && (unsigned)row < (unsigned)a.n_rows;
   if (!turn && !a.copy) return;
   float c[kPairs], s[kPairs];
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) c[i] = 1.f, s[i] = 0.f;
   if (turn) {
-    const float4* p = reinterpret_cast<const float4*>(a.table + (int64_t)row * a.pairs + kPairs * unit);
+    const float2* p = a.table + (int64_t)row * a.pairs + kPairs * unit;
 #pragma unroll
-    for (int i = 0; i < kPairs; i += 2) {
-      const float4 x = p[i >> 1];
-      c[i] = x.x; s[i] = x.y * a.sign;
-      c[i + 1] = x.z; s[i + 1] = x.w * a.sign;
+    for (int i = 0; i < kPairs; ++i) {
+      const bool ok = kHalf || kPairs * unit + i < a.pairs;
+      const float2 x = ok ? p[i] : make_float2(1.f, 0.f);
+      c[i] = x.x;
+      s[i] = x.y * a.sign;
     }
   }
-  // Halves: a unit has two chunks where it lies in the turned part, else one.
-  const bool two = kHalf && unit < turned;
-  const int at0 = kHalf ? (unit < turned ? 8 * unit : 2 * a.pairs + 8 * (unit - turned)) : 8 * unit;
-  const int at1 = a.pairs + 8 * unit;
   const int n_heads = a.heads[0] + a.heads[1];
   const int end = min(n_heads, (int)(blockIdx.y + 1) * a.group);
+  auto from = [&](int h) {
+    const int w = h >= a.heads[0];
+    return static_cast<const T*>(w ? a.x[1] : a.x[0]) + b * (w ? a.xs[1][0] : a.xs[0][0]) +
+           (h - (w ? a.heads[0] : 0)) * (w ? a.xs[1][1] : a.xs[0][1]) + t * (w ? a.xs[1][2] : a.xs[0][2]);
+  };
+  auto to = [&](int h) {
+    const int w = h >= a.heads[0];
+    return static_cast<T*>(w ? a.y[1] : a.y[0]) + b * (w ? a.ys[1][0] : a.ys[0][0]) +
+           (h - (w ? a.heads[0] : 0)) * (w ? a.ys[1][1] : a.ys[0][1]) + t * (w ? a.ys[1][2] : a.ys[0][2]);
+  };
+  const int at0 = kHalf && unit >= turned ? 2 * a.pairs + 2 * V * (unit - turned) : V * unit;
+  const int at1 = kHalf && unit < turned ? a.pairs + V * unit : at0 + V;
   for (int h0 = blockIdx.y * a.group + slot; h0 < end; h0 += kUnroll * a.slots) {
-    float x[kUnroll][8], y[kHalf ? kUnroll : 1][8];
+    Chunk<T, V> x[kUnroll][kChunks];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int h = h0 + u * a.slots;
-      if (h < end) {
-        const int w = h >= a.heads[0];
-        const T* p = static_cast<const T*>(w ? a.x[1] : a.x[0]) + b * (w ? a.xs[1][0] : a.xs[0][0]) +
-                     (h - (w ? a.heads[0] : 0)) * (w ? a.xs[1][1] : a.xs[0][1]) + t * (w ? a.xs[1][2] : a.xs[0][2]);
-        Vec8<T>::load(p + at0, x[u]);
-        if (two) Vec8<T>::load(p + at1, y[kHalf ? u : 0]);
+      if (h0 + u * a.slots < end) {
+        const T* p = from(h0 + u * a.slots);
+        x[u][0] = *reinterpret_cast<const Chunk<T, V>*>(p + at0);
+        if constexpr (kHalf) x[u][1] = *reinterpret_cast<const Chunk<T, V>*>(p + at1);
       }
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int h = h0 + u * a.slots;
-      if (h < end) {
-        const int w = h >= a.heads[0];
-        T* p = static_cast<T*>(w ? a.y[1] : a.y[0]) + b * (w ? a.ys[1][0] : a.ys[0][0]) +
-               (h - (w ? a.heads[0] : 0)) * (w ? a.ys[1][1] : a.ys[0][1]) + t * (w ? a.ys[1][2] : a.ys[0][2]);
-        if (turn) {  // (a token without a position keeps its values, infinities among them)
+      if (h0 + u * a.slots < end) {
+        if (turn) {  // (a token without a position keeps its bits, as do values past the last pair)
 #pragma unroll
           for (int i = 0; i < kPairs; ++i) {
-            float& xa = kHalf ? x[u][i] : x[u][2 * (i & 3)];
-            float& xb = kHalf ? y[kHalf ? u : 0][i] : x[u][2 * (i & 3) + 1];
-            const float va = xa, vb = xb;
-            xa = fmaf(va, c[i], -(vb * s[i]));
-            xb = fmaf(vb, c[i], va * s[i]);
+            T& xa = kHalf ? x[u][0].v[i] : x[u][0].v[2 * i & (V - 1)];
+            T& xb = kHalf ? x[u][kChunks - 1].v[i] : x[u][0].v[(2 * i + 1) & (V - 1)];
+            const float va = (float)xa, vb = (float)xb;
+            if (kHalf || kPairs * unit + i < a.pairs) {
+              xa = (T)fmaf(va, c[i], -(vb * s[i]));
+              xb = (T)fmaf(vb, c[i], va * s[i]);
+            }
           }
         }
-        Vec8<T>::store(p + at0, x[u]);
-        if (two) Vec8<T>::store(p + at1, y[kHalf ? u : 0]);
+        T* p = to(h0 + u * a.slots);
+        *reinterpret_cast<Chunk<T, V>*>(p + at0) = x[u][0];
+        if constexpr (kHalf) *reinterpret_cast<Chunk<T, V>*>(p + at1) = x[u][1];
       }
     }
   }
@@ -205,10 +186,27 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(RotArgs a) {
   }
 }
 
+// Values that a thread moves together: 8, or in halves of fewer multiples 4 or 2 (whole units have to fill
+// the half and the rest of the head, and the rows have to be aligned to them); 1 for anything else.
+int width_of(const RotArgs& a, bool half, int size) {
+  int64_t strides = a.D;
+  uint64_t ptrs = 0;
+  for (int w = 0; w < (a.heads[1] ? 2 : 1); ++w) {
+    for (int i = 0; i < 3; ++i) strides |= a.xs[w][i] | a.ys[w][i];
+    ptrs |= reinterpret_cast<uintptr_t>(a.x[w]) | reinterpret_cast<uintptr_t>(a.y[w]);
+  }
+  for (int v = 8; v >= (half ? 2 : 8); v /= 2) {
+    if (half && (a.pairs % v || (a.D - 2 * a.pairs) % (2 * v))) continue;
+    if (strides % v == 0 && ptrs % std::min(16, v * size) == 0) return v;
+  }
+  return 1;
+}
+
 template <typename T>
-int launch_rotary(RotArgs a, bool half, bool wide, hipStream_t s, const char* fn) {
+int launch_rotary(RotArgs a, bool half, hipStream_t s, const char* fn) {
+  const int v = width_of(a, half, sizeof(T));
   // units per token, then as many tokens (a power of two up to the length) and head slots as fit 256 threads
-  a.units = !wide ? a.D - a.pairs : half ? a.pairs / 8 + (a.D - 2 * a.pairs) / 8 : a.D / 8;
+  a.units = v == 1 ? a.D - a.pairs : half ? a.D / (2 * v) : a.D / 8;
   const int room = 256 / a.units;
   a.tokens = 1;
   while (2 * a.tokens <= room && a.tokens < a.L) a.tokens *= 2;
@@ -220,12 +218,15 @@ int launch_rotary(RotArgs a, bool half, bool wide, hipStream_t s, const char* fn
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(n_heads, 4096 / wgs));
   a.group = std::max((int)((n_heads + want - 1) / want), std::min(n_heads, a.slots));
   const dim3 grid((unsigned)wgs, (unsigned)((n_heads + a.group - 1) / a.group)), blk(256);
-  if (wide) {
-    if (half) hipLaunchKernelGGL((rotary_kernel<T, true>), grid, blk, 0, s, a);
-    else hipLaunchKernelGGL((rotary_kernel<T, false>), grid, blk, 0, s, a);
-  } else {
+  if (v == 1) {
     if (half) hipLaunchKernelGGL((rotary_any_kernel<T, true>), grid, blk, 0, s, a);
     else hipLaunchKernelGGL((rotary_any_kernel<T, false>), grid, blk, 0, s, a);
+  } else if (!half) {
+    hipLaunchKernelGGL((rotary_kernel<T, false, 8>), grid, blk, 0, s, a);
+  } else {
+    if (v == 8) hipLaunchKernelGGL((rotary_kernel<T, true, 8>), grid, blk, 0, s, a);
+    else if (v == 4) hipLaunchKernelGGL((rotary_kernel<T, true, 4>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, true, 2>), grid, blk, 0, s, a);
   }
   return sa::check_launch(fn);
 }
@@ -293,17 +294,11 @@ extern "C" int sa_rotary_apply(int dtype, const void* q, void* q_out, const void
   a.x[1] = k; a.y[1] = k_out;
   a.heads[0] = H;
   a.heads[1] = k ? Hk : 0;
-  const int size = dtype == SA_DTYPE_F32 ? 4 : 2;
-  bool wide = D % 8 == 0 && pairs % (halves ? 8 : 4) == 0 && reinterpret_cast<uintptr_t>(table) % 16 == 0;
-  for (int w = 0; w < (k ? 2 : 1); ++w)
+  for (int w = 0; w < 2; ++w)
     for (int i = 0; i < 3; ++i) {
-      a.xs[w][i] = strides[6 * w + i];
-      a.ys[w][i] = strides[6 * w + 3 + i];
-      wide = wide && a.xs[w][i] * size % 16 == 0 && a.ys[w][i] * size % 16 == 0;
+      a.xs[w][i] = k || w == 0 ? strides[6 * w + i] : 0;
+      a.ys[w][i] = k || w == 0 ? strides[6 * w + 3 + i] : 0;
     }
-  if (!k)
-    for (int i = 0; i < 3; ++i) a.xs[1][i] = a.ys[1][i] = 0;
-  for (const void* p : {q, (const void*)q_out, k, (const void*)k_out}) wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
   a.B = B; a.L = L; a.D = D;
   a.table = reinterpret_cast<const float2*>(table);
   a.n_rows = n_rows;
@@ -315,7 +310,7 @@ extern "C" int sa_rotary_apply(int dtype, const void* q, void* q_out, const void
   // Each thread reads its values before it writes them, so that out may be the input itself.
   a.copy = !(q == q_out && (!k || k == k_out));
   hipStream_t s = sa::as_stream(stream);
-  if (dtype == SA_DTYPE_F32) return launch_rotary<float>(a, halves != 0, wide, s, fn);
-  if (dtype == SA_DTYPE_F16) return launch_rotary<_Float16>(a, halves != 0, wide, s, fn);
-  return launch_rotary<__bf16>(a, halves != 0, wide, s, fn);
+  if (dtype == SA_DTYPE_F32) return launch_rotary<float>(a, halves != 0, s, fn);
+  if (dtype == SA_DTYPE_F16) return launch_rotary<_Float16>(a, halves != 0, s, fn);
+  return launch_rotary<__bf16>(a, halves != 0, s, fn);
 }

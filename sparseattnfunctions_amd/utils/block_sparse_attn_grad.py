@@ -12,8 +12,8 @@ does as well. Training code calls this module instead:
   * `block_sparse_attention_lse` and `block_sparse_attention_backward`: its two halves without
     autograd, e.g. for a step captured into a HIP graph.
 
-The forward pass is the kernel of `block_sparse_attention` with bf16 (fp16, fp32) scores and also
-stores each row's log2-sum-exp2; the backward pass recomputes the probabilities from it, block by
+The forward pass is the kernel of `block_sparse_attention` with bf16 (fp16) scores, or fp32 on split
+operands, and also stores each row's log2-sum-exp2; the backward pass recomputes the probabilities from it, block by
 block, and keeps nothing of the size of the attention map (`sa_block_sparse_bwd`). Gradients of a
 16-bit call round P and dS to its type, sums are fp32 in a fixed order, so that a step repeats bit for
 bit. In fp16, dS has the range of the type: scale the loss as usual. A query row without a key (an
@@ -32,7 +32,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._kv import KVList, kv_list_from_mask
-from .block_sparse_attn_kernel import (BLOCK, F32_TERMS_BLOCKS, cell_kv_list, f32_terms_workspace, shares_text_rows,
+from .block_sparse_attn_kernel import (BLOCK, cell_kv_list, f32_terms_workspace, shares_text_rows,
                                        split_parts, split_workspace_bytes, work_order)
 
 
@@ -115,8 +115,9 @@ class _Plan:
         sq, sk = (H * Lq * D, Lq * D, D), (H * Lk * D, Lk * D, D)
         args.strides[:] = (*q_strides[:3], *k_strides[:3], *v_strides[:3], *sq, 0, 0, 0, *sq, *sk, *sk)
         # The forward pass takes block_sparse_attention's launch variants: key-range parts for few blocks
-        # over long lists, else a work order; fp32 split operands where it takes them.
-        self.terms = dtype == torch.float32 and nqb >= F32_TERMS_BLOCKS
+        # over long lists, else a work order. fp32 takes split operands for few query blocks too: 30 heads of one
+        # block over 1, 4, 8 and 63 blocks 16.6 / 17.6, 46 / 18, 87 / 25 and 697 / 102 us without / with.
+        self.terms = dtype == torch.float32
         if dtype != torch.float32 and not biased:
             args.parts = split_parts(n_items, max_cnt, D)
         self.forward_bytes = split_workspace_bytes(n_items, D, args.parts) if args.parts > 1 else 0

@@ -54,7 +54,8 @@ CASES = [
     (2, 30, 30, 45, 64, 32, 45),
     (1, 12, 3, 257, 128, 96, 7),
     (3, 5, 1, 33, 96, 96, 0),
-    (2, 2, 2, 70, 64, 20, 3),  # pairs that no wide access holds
+    (2, 2, 2, 70, 64, 20, 3),  # pairs of which narrower accesses hold whole ones
+    (2, 3, 2, 37, 64, 24, 5),
     (1, 4, 2, 19, 80, 2, 0),
     (1, 2, 2, 9, 7, 6, 1),
     (1, 1, 2, 5, 256, 256, 0),
