@@ -4,9 +4,10 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin), and with -sin for the gradient (the transpose)
 //
 // The table kernel forms the angles in 64 bits, as turns, so that far positions keep their fraction,
-// and takes the quarter turn off before the 32-bit sine and cosine. The rotation is bound by memory:
-// each value is read and written once, and a thread keeps its pairs' cosines and sines while it goes
-// through the heads.
+// and takes the quarter turn off before the 32-bit sine and cosine: 1 350 tokens of 32 pairs take 2 us,
+// 45 104 of 64 pairs 7 (3.3 TB/s of table written; the 64-bit product and rounding are hidden behind it).
+// The rotation is bound by memory: each value is read and written once, and a thread keeps its pairs'
+// cosines and sines while it goes through the heads.
 #include <math.h>
 
 #include <algorithm>
@@ -77,15 +78,23 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Chunk {
   T v[N];
 };
 
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
+
 // A thread turns one unit of one token in every head of its group. Interleaved: V consecutive values
 // (V / 2 pairs, those past the last one left alone). Halves: V values of each half (V pairs); units past
 // the turned part copy 2 V values, in the same two accesses, so that the lanes of a wave stay together.
 // Loads of kUnroll heads are in flight together.
+//
+// kLines: each store of a wave fills whole lines (interleaved 16-bit values), so that they need not wait
+// in a cache for the rest: they are streamed out. [2, 30, 17776, 64] queries and keys in bf16 take 91 us so
+// (6.0 TB/s), 108 with ordinary stores; halves (106 us, streamed 110) and fp32
+// (30 us, streamed 33), whose lines are put together from two stores, keep the ordinary ones.
 template <typename T, bool kHalf, int V>
 __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
   constexpr int kUnroll = 4;
   constexpr int kPairs = kHalf ? V : V / 2;
   constexpr int kChunks = kHalf ? 2 : 1;
+  constexpr bool kLines = !kHalf && sizeof(T) == 2;
   const int unit = threadIdx.x % a.units;
   const int rest = threadIdx.x / a.units;
   const int slot = rest / a.tokens;
@@ -148,8 +157,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
           }
         }
         T* p = to(h0 + u * a.slots);
-        *reinterpret_cast<Chunk<T, V>*>(p + at0) = x[u][0];
-        if constexpr (kHalf) *reinterpret_cast<Chunk<T, V>*>(p + at1) = x[u][1];
+        if constexpr (kLines) {
+          __builtin_nontemporal_store(__builtin_bit_cast(Words, x[u][0]), reinterpret_cast<Words*>(p + at0));
+        } else {
+          *reinterpret_cast<Chunk<T, V>*>(p + at0) = x[u][0];
+          if constexpr (kHalf) *reinterpret_cast<Chunk<T, V>*>(p + at1) = x[u][1];
+        }
       }
     }
   }
@@ -214,9 +227,12 @@ int launch_rotary(RotArgs a, bool half, hipStream_t s, const char* fn) {
   const int n_heads = a.heads[0] + a.heads[1];
   const int64_t wgs = (int64_t)a.B * ((a.L + a.tokens - 1) / a.tokens);
   SA_REQUIRE(wgs < (1LL << 31), "%s: grid too large", fn);
-  // A group of heads shares the table's values; groups as large as leave some 4 096 workgroups.
+  // A group of heads shares the table's values; groups as large as leave some 4 096 workgroups (8 192: 92 -> 90 us at
+  // [2, 30, 17776, 64], but 9.3 -> 11.6 at 1 576 tokens), of at most 16 heads a slot (2 x 48 heads of 45 104 tokens: 222 us
+  // in groups of 48, 206 in groups of 16).
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(n_heads, 4096 / wgs));
-  a.group = std::max((int)((n_heads + want - 1) / want), std::min(n_heads, a.slots));
+  a.group = std::min((int)((n_heads + want - 1) / want), 16 * a.slots);
+  a.group = std::max(a.group, std::min(n_heads, a.slots));
   const dim3 grid((unsigned)wgs, (unsigned)((n_heads + a.group - 1) / a.group)), blk(256);
   if (v == 1) {
     if (half) hipLaunchKernelGGL((rotary_any_kernel<T, true>), grid, blk, 0, s, a);
