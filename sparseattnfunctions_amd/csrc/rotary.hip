@@ -3,9 +3,11 @@
 //   angle[token][pair] = position[axis of pair][token] * frequency[pair]
 //   (a, b) -> (a cos - b sin, b cos + a sin), and with -sin for the gradient (the transpose)
 //
-// The table kernel forms the angles in 64 bits, as turns, so that far positions keep their fraction,
-// and takes the quarter turn off before the 32-bit sine and cosine: 1 350 tokens of 32 pairs take 2 us,
-// 45 104 of 64 pairs 7 (3.3 TB/s of table written; the 64-bit product and rounding are hidden behind it).
+// The table kernel forms the angles in 64 bits, as turns, so that far positions keep their fraction, and
+// takes the quarter turn off before the 32-bit sine and cosine. It is bound by arithmetic until the table
+// outgrows the caches: 45 104 tokens of 64 pairs take 8.3 us (2.8 TB/s written; 10.1 with sincospif, 11.6
+// with one token a thread as well), 1 350 of 32 pairs 2.4, which an empty launch takes too.
+//
 // The rotation is bound by memory: each value is read and written once, and a thread keeps its pairs'
 // cosines and sines while it goes through the heads.
 #include <math.h>
@@ -20,37 +22,45 @@ namespace {
 
 constexpr int kMaxAxes = 4;
 constexpr int kMaxPairs = 128;
+constexpr double kTurn = 6.283185307179586476925287;
 
 struct TableArgs {
   const void* positions;
   int64_t stride_axis, stride_token;
-  int64_t n;  // tokens * pairs
-  int pairs, n_axes;
+  int64_t L;
+  int pairs;
+  int tokens, steps;  // of a workgroup: tokens at once, and how often
   int axis_end[kMaxAxes];  // pairs of the axes up to this one
   float factor[kMaxAxes];  // of the axis's cosines and sines
   double turns[kMaxPairs];  // turns per position
   float2* table;
 };
 
+// A thread keeps its pair and takes `steps` tokens, so that the axis and the frequency are found once.
 template <typename P>
 __global__ __launch_bounds__(256) void rotary_table_kernel(TableArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.n) return;
-  const int64_t token = i / a.pairs;
-  const int pair = (int)(i - token * a.pairs);
+  const int slot = threadIdx.x / (unsigned)a.pairs;
+  const int pair = threadIdx.x - slot * a.pairs;
+  if (slot >= a.tokens) return;
   int axis = 0;
   while (pair >= a.axis_end[axis]) ++axis;  // (axis_end of the last axis is the number of pairs)
-  const double pos = (double)static_cast<const P*>(a.positions)[axis * a.stride_axis + token * a.stride_token];
-  const double t = pos * a.turns[pair];
-  const double quarter = rint(4.0 * t);
-  const float f = (float)(t - 0.25 * quarter);  // |f| <= 1/8 turn
-  float s, c;
-  sincospif(2.f * f, &s, &c);
-  // quarter mod 4 (an infinite or NaN position gives NaN either way)
-  const int q = (int)(quarter - 4.0 * floor(0.25 * quarter));
-  const float sn = (q & 1) ? c : s, cs = (q & 1) ? s : c;
+  const double turns = a.turns[pair];
   const float m = a.factor[axis];
-  a.table[i] = make_float2((q == 1 || q == 2) ? -cs * m : cs * m, (q & 2) ? -sn * m : sn * m);
+  const P* positions = static_cast<const P*>(a.positions) + axis * a.stride_axis;
+  int64_t token = (int64_t)blockIdx.x * a.tokens * a.steps + slot;
+  for (int i = 0; i < a.steps && token < a.L; ++i, token += a.tokens) {
+    const double t = (double)positions[token * a.stride_token] * turns;
+    const double r = t - rint(t);  // exact
+    const double quarter = rint(4.0 * r);
+    const float y = (float)((r - 0.25 * quarter) * kTurn);  // |y| <= pi / 4
+    const float z = y * y;
+    // Their power series, up to y^9 and y^10 (what is left out is below 2e-9 of the value).
+    const float s = fmaf(y * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), y);
+    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
+    const int q = (int)quarter & 3;  // (an infinite or NaN position gives NaN either way)
+    const float sn = (q & 1) ? c : s, cs = (q & 1) ? s : c;
+    a.table[token * a.pairs + pair] = make_float2((q == 1 || q == 2) ? -cs * m : cs * m, (q & 2) ? -sn * m : sn * m);
+  }
 }
 
 // ---- rotation -----------------------------------------------------------------------------------
@@ -262,7 +272,6 @@ extern "C" int sa_rotary_table(const void* positions, int position_type, const i
   a.stride_axis = strides[0];
   a.stride_token = strides[1];
   a.pairs = 0;
-  a.n_axes = n_axes;
   for (int i = 0; i < n_axes; ++i) {
     SA_REQUIRE(axis_pairs[i] > 0 && axis_pairs[i] <= kMaxPairs - a.pairs, "%s: axes of more than %d pairs", fn, kMaxPairs);
     a.pairs += axis_pairs[i];
@@ -272,11 +281,15 @@ extern "C" int sa_rotary_table(const void* positions, int position_type, const i
   }
   for (int i = 0; i < a.pairs; ++i) {
     SA_REQUIRE(std::isfinite(frequencies[i]), "%s: frequency %d is not finite", fn, i);
-    a.turns[i] = frequencies[i] / 6.283185307179586476925287;
+    a.turns[i] = frequencies[i] / kTurn;
   }
-  a.n = L * a.pairs;
+  a.L = L;
   a.table = reinterpret_cast<float2*>(table);
-  const int64_t wgs = (a.n + 255) / 256;
+  a.tokens = 256 / a.pairs;
+  // As many steps as leave some 1 024 workgroups (45 104 tokens of 64 pairs: 12.8 us in one, 10.1 in four and more; 1 350
+  // of 32: 2.4 and 3.2).
+  a.steps = (int)std::min<int64_t>(8, std::max<int64_t>(1, L / ((int64_t)a.tokens * 1024)));
+  const int64_t wgs = (L + (int64_t)a.tokens * a.steps - 1) / ((int64_t)a.tokens * a.steps);
   SA_REQUIRE(wgs < (1LL << 31), "%s: grid too large", fn);
   const dim3 grid((unsigned)wgs), blk(256);
   hipStream_t s = sa::as_stream(stream);
