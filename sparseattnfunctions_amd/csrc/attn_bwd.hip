@@ -72,9 +72,10 @@ struct BwdArgs {
   // [bh][2 * query blocks][2][32]: per 32 query rows their -lse / scale_log2, then their -delta. Written
   // by the query pass, read by the key pass.
   float* stats;
-  // More than one split: a workgroup computes its split's share of the item's steps and
-  // stores its sums to partial[item][split][result][64][kD]; bwd_merge_kernel adds them in order.
-  int splits;
+  // More than one split: an item of those behind the first `whole` dispatch slots of an XCD (whole < 0: every
+  // item) is computed by `splits` workgroups, each on its share of the item's steps, which store their sums
+  // to partial[place][split][result][64][kD]; bwd_merge_kernel adds them in order.
+  int splits, whole, tail;  // tail: slots of an XCD behind the whole ones
   float* partial;
 };
 
@@ -87,19 +88,31 @@ __device__ inline float2 unpack2(uint32_t w) {
   return make_float2((float)h[0], (float)h[1]);
 }
 
-// Item of a workgroup: the four slots of dispatch group w (placed on XCD w % 8 by the work order) go to
-// the workgroups 32 (w / 8) + 8 i + w % 8, i = 0 .. 3, which the dispatcher places on the same XCD.
-// With splits there are no idle workgroups, which would leave CUs out of turn ([1, 1, 64 x 17776, 64] in
-// fp32 ran on a quarter of 32 CUs): item and split count up.
-__device__ inline int bwd_item(const BwdArgs& a, int x, int& split) {
-  split = 0;
-  if (a.splits > 1) {
-    split = x % a.splits;
-    return x / a.splits;
-  }
-  const int slot = 4 * (8 * (x >> 5) + (x & 7)) + ((x >> 3) & 3);
+// Item of slot `seq` of XCD `xcd` (the work order's slots come in groups of four, group w on XCD w % 8).
+__device__ inline int slot_item(const BwdArgs& a, int xcd, int seq) {
+  const int slot = 4 * (8 * (seq >> 2) + xcd) + (seq & 3);
   if (slot >= a.n_slots) return -1;
   return a.order ? order_item(a.order, slot) : slot;
+}
+
+// Item of a workgroup (-1: none), its split, and the place of its sums (-1: not split). The dispatcher deals
+// workgroups out to the XCDs in turn. Where every item is split there are no idle workgroups, which would
+// leave CUs out of turn ([1, 1, 64 x 17776, 64] in fp32 ran on a quarter of 32 CUs): item and split count up.
+__device__ inline int bwd_item(const BwdArgs& a, int x, int& split, int& place) {
+  split = 0;
+  place = -1;
+  if (a.splits > 1 && a.whole < 0) {
+    split = x % a.splits;
+    return place = x / a.splits;
+  }
+  int seq = x >> 3;
+  if (a.splits > 1 && seq >= a.whole) {
+    const int t = (seq - a.whole) / a.splits;
+    split = seq - a.whole - t * a.splits;
+    place = (x & 7) * a.tail + t;
+    seq = a.whole + t;
+  }
+  return slot_item(a, x & 7, seq);
 }
 
 // The item's list: entries list[0 .. n).
@@ -142,8 +155,8 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = wave >> 1, w = wave & 1;
   const int col = lane & 31, hh = lane >> 5;
-  int split;
-  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x, split));
+  int split, place;
+  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x, split, place));
   if (item < 0 || item >= a.n_items) return;  // (the whole workgroup)
   const int bh = item / a.n_own;
   const int blk = item - bh * a.n_own;
@@ -202,7 +215,8 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   const uint32_t stat_bytes = kKeys ? (uint32_t)a.n_st * 512 : (uint32_t)a.L_st * 4;
 
   // The split's share of the 2 cnt steps, of it the part's.
-  const int per_split = (2 * cnt + a.splits - 1) / a.splits;
+  const int splits = place < 0 ? 1 : a.splits;
+  const int per_split = (2 * cnt + splits - 1) / splits;
   const int n_steps = min(2 * cnt, per_split * (split + 1));
   const int per_part = (per_split + kParts - 1) / kParts;
   const int beg = split * per_split + part * per_part;
@@ -434,8 +448,8 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
           s.z += y.z;
           s.w += y.w;
         }
-        if (a.splits > 1)
-          *reinterpret_cast<float4*>(a.partial + ((((int64_t)item * a.splits + split) * kAcc + x) * kBlk + r) * kD +
+        if (place >= 0)
+          *reinterpret_cast<float4*>(a.partial + ((((int64_t)place * a.splits + split) * kAcc + x) * kBlk + r) * kD +
                                      4 * ch) = s;
         else if (g && blk * kBlk + r < a.L_own)
           *reinterpret_cast<uint2*>(g + b * sb + h * sh + (int64_t)(blk * kBlk + r) * sl + 4 * ch) =
@@ -476,8 +490,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = wave >> 1, w = wave & 1;
   const int col = lane & 31, hh = lane >> 5;
-  int split;
-  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x, split));
+  int split, place;
+  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x, split, place));
   if (item < 0 || item >= a.n_items) return;  // (the whole workgroup)
   const int bh = item / a.n_own;
   const int blk = item - bh * a.n_own;
@@ -523,7 +537,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   const float* stat_src = a.stats + (int64_t)bh * a.n_st * 128;
   const uint32_t stat_bytes = (uint32_t)a.n_st * 512;
 
-  const int per_split = (2 * cnt + a.splits - 1) / a.splits;
+  const int splits = place < 0 ? 1 : a.splits;
+  const int per_split = (2 * cnt + splits - 1) / splits;
   const int n_steps = min(2 * cnt, per_split * (split + 1));
   const int per_part = (per_split + kParts - 1) / kParts;
   const int beg = split * per_split + part * per_part;
@@ -669,8 +684,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
       const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tile1) + at);
       const float4 s = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
       const int row = blk * kBlk + r;
-      if (a.splits > 1)
-        *reinterpret_cast<float4*>(a.partial + ((((int64_t)item * a.splits + split) * kAcc + x) * kBlk + r) * kD +
+      if (place >= 0)
+        *reinterpret_cast<float4*>(a.partial + ((((int64_t)place * a.splits + split) * kAcc + x) * kBlk + r) * kD +
                                    4 * ch) = s;
       else if (g && row < a.L_own)
         *reinterpret_cast<float4*>(g + b * sb + h * sh + (int64_t)row * sl + 4 * ch) =
@@ -679,11 +694,13 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   }
 }
 
-// Gradients from the splits' sums, in order: one workgroup per item and result.
+// Gradients from the splits' sums, in order: one workgroup per split item and result.
 template <bool kKeys, typename T>
 __global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
   constexpr int kAcc = kKeys ? 2 : 1;
-  const int item = blockIdx.x, x = blockIdx.y;
+  const int place = blockIdx.x, x = blockIdx.y;
+  const int item = a.whole < 0 ? place : slot_item(a, place / a.tail, a.whole + place % a.tail);
+  if (item < 0 || item >= a.n_items) return;
   const int bh = item / a.n_own;
   const int blk = item - bh * a.n_own;
   const int b = bh / a.H;
@@ -694,7 +711,7 @@ __global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
   const int64_t sl = x == 0 ? a.ga_sl : a.gb_sl;
   const float f = x == 0 ? a.sm_scale : 1.f;
   const int64_t n = (int64_t)kBlk * D;
-  const float* from = a.partial + ((int64_t)item * a.splits * kAcc + x) * n;
+  const float* from = a.partial + ((int64_t)place * a.splits * kAcc + x) * n;
   for (int t = threadIdx.x; t < kBlk * D / 4; t += 256) {
     const int r = t / (D / 4), d = 4 * (t % (D / 4));
     if (blk * kBlk + r >= a.L_own) break;
@@ -717,11 +734,16 @@ __global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
 template <bool kKeys, typename T>
 void launch_merge(const BwdArgs& a, int D, hipStream_t s) {
   if (a.splits > 1)
-    hipLaunchKernelGGL((bwd_merge_kernel<kKeys, T>), dim3((unsigned)a.n_items, kKeys ? 2 : 1), dim3(256), 0, s, a, D);
+    hipLaunchKernelGGL((bwd_merge_kernel<kKeys, T>), dim3((unsigned)(a.whole < 0 ? a.n_items : 8 * a.tail), kKeys ? 2 : 1),
+                       dim3(256), 0, s, a, D);
 }
 
+// Slots of an XCD.
+int xcd_slots(int64_t n_slots) { return (int)(((n_slots + 3) / 4 + 7) / 8 * 4); }
+
 unsigned workgroups(const BwdArgs& a) {
-  return a.splits > 1 ? (unsigned)a.n_items * a.splits : (unsigned)(((a.n_slots + 3) / 4 + 7) / 8 * 32);
+  if (a.splits > 1 && a.whole < 0) return (unsigned)a.n_items * a.splits;
+  return a.splits > 1 ? 8u * (a.whole + a.tail * a.splits) : 8u * xcd_slots(a.n_slots);
 }
 
 template <bool kKeys, typename T, int kD, int kParts>
@@ -760,9 +782,39 @@ int splits_of(int64_t n_items, int width, int D, bool f32) {
   return (int)std::min<int64_t>({fit, width / 8, 32});
 }
 
+// How the items of a pass are dealt out.
+struct Deal {
+  int parts;                // pairs of waves per workgroup
+  int splits, whole, tail;  // as in BwdArgs
+  int64_t places() const { return splits == 1 ? 0 : whole < 0 ? tail : 8 * (int64_t)tail; }  // items that are split
+};
+
+// fp32: the items behind the last full round of an XCD's workgroups are split, by three where lists may be long.
+// Whole / split, us of the query and key pass with the merge: [1, 30, 2560, 64] half the blocks 383 / 349 and 488 /
+// 463, 0.15 of them 151 / 147 and 214 / 210; [1, 12, 2100, 64], less than a round, 159 / 140 and 211 / 190; [1, 10,
+// 3500, 128] 492 / 418 and 638 / 564; of 24 blocks or fewer by two 88 / 86 and 129 / 123 (by three 93, 129); at worst
+// [1, 20, 3333, 128] with a tenth of the blocks 265 / 278 and 403 / 393. 16-bit steps are too short for it: dense
+// lists of 40 gain 171 / 163 and 229 / 227 (by two 159 and 222), the same lists with a fifth of the blocks lose 54 / 61
+// and 87 / 94, and the host does not know which they are.
+Deal deal(int64_t n_items, int width, int D, bool f32) {
+  Deal d = {2, splits_of(n_items, width, D, f32), -1, (int)n_items};
+  if (d.splits > 1) return d;
+  if (!f32) {
+    d.parts = pairs_per_item((int)n_items, width, D);
+    return d;
+  }
+  const int slots = xcd_slots(n_items);
+  const int left = slots % (D == 64 ? 64 : 32);  // (two workgroups, or one, per CU)
+  if (left > 0 && width >= 16) {
+    d.splits = width >= 32 ? 3 : 2;
+    d.whole = slots - left;
+    d.tail = left;
+  }
+  return d;
+}
+
 template <bool kKeys, typename T, int kD>
-void launch_pass(const BwdArgs& a, int width, hipStream_t s) {
-  const int parts = a.splits > 1 ? 2 : pairs_per_item(a.n_items, width, kD);
+void launch_pass(const BwdArgs& a, int parts, hipStream_t s) {
   if (parts == 2) launch_parts<kKeys, T, kD, 2>(a, s);
   else launch_parts<kKeys, T, kD, 1>(a, s);
   launch_merge<kKeys, T>(a, kD, s);
@@ -777,11 +829,15 @@ void launch_pass_f32(const BwdArgs& a, int D, hipStream_t s) {
 }
 
 template <bool kKeys>
-void launch_pass_any(const BwdArgs& a, int dtype, int D, int width, hipStream_t s) {
+void launch_pass_any(BwdArgs& a, int dtype, int D, const Deal& d, hipStream_t s) {
+  // (a caller's order may have other slots than a plain one)
+  a.splits = d.splits > 1 && d.whole >= 0 && xcd_slots(a.n_slots) != d.whole + d.tail ? 1 : d.splits;
+  a.whole = d.whole;
+  a.tail = d.tail;
   if (dtype == SA_DTYPE_F32) return launch_pass_f32<kKeys>(a, D, s);
   if (dtype == SA_DTYPE_F16)
-    return D == 64 ? launch_pass<kKeys, _Float16, 64>(a, width, s) : launch_pass<kKeys, _Float16, 128>(a, width, s);
-  return D == 64 ? launch_pass<kKeys, __bf16, 64>(a, width, s) : launch_pass<kKeys, __bf16, 128>(a, width, s);
+    return D == 64 ? launch_pass<kKeys, _Float16, 64>(a, d.parts, s) : launch_pass<kKeys, _Float16, 128>(a, d.parts, s);
+  return D == 64 ? launch_pass<kKeys, __bf16, 64>(a, d.parts, s) : launch_pass<kKeys, __bf16, 128>(a, d.parts, s);
 }
 
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -790,7 +846,7 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // pass at a time).
 struct Layout {
   int64_t q_beg, q_idx, partial, bytes;
-  int q_splits, k_splits;
+  Deal q, k;
 };
 
 Layout layout(const sa_attn_train& t) {
@@ -801,11 +857,10 @@ Layout layout(const sa_attn_train& t) {
   l.q_idx = l.q_beg + align256(BH * (nkb + 1) * (int64_t)sizeof(int32_t));
   l.partial = l.q_idx + align256(BH * nqb * t.max_cnt * (int64_t)sizeof(int32_t));
   // (a list is no longer than the other side has blocks, but for repeated entries)
-  l.q_splits = splits_of(BH * nqb, std::min<int64_t>(t.max_cnt, nkb), t.D, f32);
-  l.k_splits = splits_of(BH * nkb, (int)nqb, t.D, f32);
+  l.q = deal(BH * nqb, (int)std::min<int64_t>(t.max_cnt, nkb), t.D, f32);
+  l.k = deal(BH * nkb, (int)nqb, t.D, f32);
   const int64_t tile = (int64_t)kBlk * t.D * sizeof(float);
-  const int64_t q = l.q_splits > 1 ? BH * nqb * l.q_splits * tile : 0, k = l.k_splits > 1 ? BH * nkb * l.k_splits * 2 * tile : 0;
-  l.bytes = l.partial + std::max(q, k);
+  l.bytes = l.partial + std::max(l.q.places() * l.q.splits * tile, l.k.places() * l.k.splits * 2 * tile);
   return l;
 }
 
@@ -859,7 +914,7 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   for (int i = 0; i < 4; ++i)
     if (strides[3 * at[i] + 2] < 0 || (rows[i] + kBlk) * strides[3 * at[i] + 2] * size + 2 * D > INT_MAX)
       return sa::fail(SA_ERR_UNSUPPORTED, "%s: rows of one head span more than 2 GiB", fn);
-  const Layout l = layout(*t);
+  Layout l = layout(*t);
   SA_REQUIRE(t->workspace && reinterpret_cast<uintptr_t>(t->workspace) % 256 == 0,
              "%s: workspace null or not 256-byte aligned", fn);
   SA_REQUIRE(t->workspace_bytes >= l.bytes, "%s: workspace of %lld bytes < %lld", fn, (long long)t->workspace_bytes,
@@ -900,8 +955,8 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   a.order = t->q_order;
   a.n_slots = (int)(t->q_order ? t->n_q_slots : (a.n_items + 3) / 4 * 4);
   a.idx = t->kv_idx; a.cnt = t->kv_cnt;
-  a.splits = t->dq ? l.q_splits : 1;
-  launch_pass_any<false>(a, t->dtype, D, std::min(t->max_cnt, nkb), s);
+  if (!t->dq) l.q.splits = 1;
+  launch_pass_any<false>(a, t->dtype, D, l.q, s);
   if (int rc = sa::check_launch(fn)) return rc;
   if (!t->dk && !t->dv) return sa::ok();
 
@@ -916,7 +971,6 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   a.order = t->k_order;
   a.n_slots = (int)(t->k_order ? t->n_k_slots : (a.n_items + 3) / 4 * 4);
   a.idx = q_idx; a.cnt = q_beg;
-  a.splits = l.k_splits;
-  launch_pass_any<true>(a, t->dtype, D, nqb, s);
+  launch_pass_any<true>(a, t->dtype, D, l.k, s);
   return sa::check_launch(fn);
 }

@@ -94,6 +94,23 @@ def test_forward_keeps_the_bits_of_block_sparse_triton_fn(dev, dtype):
         assert torch.equal(block_sparse_train_fn(q, k, v, mask, 0.1), want)
 
 
+# The blocks behind the last full round of workgroups are split: by two in short lists, by three in long ones,
+# all of them where there is less than a round.
+@pytest.mark.parametrize("H,L,D,text", [(9, 1100, 64, 0), (17, 2100, 64, 2), (9, 2100, 128, 0)])
+def test_fp32_remainders(dev, H, L, D, text):
+    case(f"fp32 remainders H={H} L={L} D={D}")
+    Lk = L - 20
+    (q, k, v, do), g = _inputs(17, FP32, 1, H, L, Lk, D)
+    mask = _mask(g, 1, H, L, Lk, 0.3, 0.1)
+    mask[:, :, :text] = True
+    mask[..., :text] = True
+    fn = lambda *x: block_sparse_train_fn(*x, mask.to(dev), 0.125, n_text_blocks=text)
+    got = _grads(fn, *(t.to(dev) for t in (q, k, v, do)))
+    # (as in test_gradients, sums of up to 2 100 terms)
+    check(got, reference(q, k, v, do, mask, 0.125), norm=64 * 2.0 ** -24)
+    assert all(torch.equal(a, b) for a, b in zip(got, _grads(fn, *(t.to(dev) for t in (q, k, v, do)))))
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_text_blocks(dev, D):
     # The hint of long first rows changes the schedule (shared rows in the forward pass) and no value.
