@@ -255,6 +255,7 @@ typedef struct sa_attn_train {
   void* workspace;          /* of the call that is made, 256-byte aligned */
   int64_t workspace_bytes;
   float sm_scale;
+  int32_t n_text_blocks;    /* so many first blocks of each head, which the orders put first, have long lists (0: none) */
 } sa_attn_train;
 
 /*
@@ -271,7 +272,7 @@ int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
  * lse), dS = P * (dout v^T - rowsum(dout * out)), dq = sm_scale dS k, dk = sm_scale dS^T q, dv = P^T
  * dout. Rows and keys in no list get zeros; a block that a row lists twice counts twice. Sums are fp32 in a
  * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type.
- *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype and max_cnt): the query
+ *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype, max_cnt and n_text_blocks): the query
  *             rows' statistics, the transposed lists, sums of lists split over workgroups.
  * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv, sm_scale
  * at least 1e-30.

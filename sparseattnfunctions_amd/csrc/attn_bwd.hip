@@ -72,10 +72,10 @@ struct BwdArgs {
   // [bh][2 * query blocks][2][32]: per 32 query rows their -lse / scale_log2, then their -delta. Written
   // by the query pass, read by the key pass.
   float* stats;
-  // More than one split: an item of those behind the first `whole` dispatch slots of an XCD (whole < 0: every
-  // item) is computed by `splits` workgroups, each on its share of the item's steps, which store their sums
-  // to partial[place][split][result][64][kD]; bwd_merge_kernel adds them in order.
-  int splits, whole, tail;  // tail: slots of an XCD behind the whole ones
+  // More than one split: the items of an XCD's dispatch slots first .. first + n_split - 1 (first < 0: every
+  // item, n_split of them) are computed by `splits` workgroups each, on shares of the item's steps, which store
+  // their sums to partial[place][split][result][64][kD]; bwd_merge_kernel adds them in order.
+  int splits, first, n_split;
   float* partial;
 };
 
@@ -101,16 +101,20 @@ __device__ inline int slot_item(const BwdArgs& a, int xcd, int seq) {
 __device__ inline int bwd_item(const BwdArgs& a, int x, int& split, int& place) {
   split = 0;
   place = -1;
-  if (a.splits > 1 && a.whole < 0) {
+  if (a.splits > 1 && a.first < 0) {
     split = x % a.splits;
     return place = x / a.splits;
   }
   int seq = x >> 3;
-  if (a.splits > 1 && seq >= a.whole) {
-    const int t = (seq - a.whole) / a.splits;
-    split = seq - a.whole - t * a.splits;
-    place = (x & 7) * a.tail + t;
-    seq = a.whole + t;
+  if (a.splits > 1 && seq >= a.first) {
+    const int t = (seq - a.first) / a.splits;
+    if (t < a.n_split) {
+      split = seq - a.first - t * a.splits;
+      place = (x & 7) * a.n_split + t;
+      seq = a.first + t;
+    } else {
+      seq -= a.n_split * (a.splits - 1);
+    }
   }
   return slot_item(a, x & 7, seq);
 }
@@ -699,7 +703,7 @@ template <bool kKeys, typename T>
 __global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
   constexpr int kAcc = kKeys ? 2 : 1;
   const int place = blockIdx.x, x = blockIdx.y;
-  const int item = a.whole < 0 ? place : slot_item(a, place / a.tail, a.whole + place % a.tail);
+  const int item = a.first < 0 ? place : slot_item(a, place / a.n_split, a.first + place % a.n_split);
   if (item < 0 || item >= a.n_items) return;
   const int bh = item / a.n_own;
   const int blk = item - bh * a.n_own;
@@ -734,7 +738,7 @@ __global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
 template <bool kKeys, typename T>
 void launch_merge(const BwdArgs& a, int D, hipStream_t s) {
   if (a.splits > 1)
-    hipLaunchKernelGGL((bwd_merge_kernel<kKeys, T>), dim3((unsigned)(a.whole < 0 ? a.n_items : 8 * a.tail), kKeys ? 2 : 1),
+    hipLaunchKernelGGL((bwd_merge_kernel<kKeys, T>), dim3((unsigned)(a.first < 0 ? a.n_items : 8 * a.n_split), kKeys ? 2 : 1),
                        dim3(256), 0, s, a, D);
 }
 
@@ -742,8 +746,8 @@ void launch_merge(const BwdArgs& a, int D, hipStream_t s) {
 int xcd_slots(int64_t n_slots) { return (int)(((n_slots + 3) / 4 + 7) / 8 * 4); }
 
 unsigned workgroups(const BwdArgs& a) {
-  if (a.splits > 1 && a.whole < 0) return (unsigned)a.n_items * a.splits;
-  return a.splits > 1 ? 8u * (a.whole + a.tail * a.splits) : 8u * xcd_slots(a.n_slots);
+  if (a.splits > 1 && a.first < 0) return (unsigned)a.n_items * a.splits;
+  return 8u * (xcd_slots(a.n_slots) + (a.splits - 1) * a.n_split);
 }
 
 template <bool kKeys, typename T, int kD, int kParts>
@@ -782,11 +786,19 @@ int splits_of(int64_t n_items, int width, int D, bool f32) {
   return (int)std::min<int64_t>({fit, width / 8, 32});
 }
 
+// The most text items of an XCD (its items are a contiguous eighth, the first n_text of each n_own text).
+int text_slots(int64_t n_items, int n_own, int n_text) {
+  auto before = [&](int64_t it) { return it / n_own * n_text + std::min<int64_t>(it % n_own, n_text); };
+  int64_t most = 0;
+  for (int x = 0; x < 8; ++x) most = std::max(most, before(n_items * (x + 1) / 8) - before(n_items * x / 8));
+  return (int)most;
+}
+
 // How the items of a pass are dealt out.
 struct Deal {
-  int parts;                // pairs of waves per workgroup
-  int splits, whole, tail;  // as in BwdArgs
-  int64_t places() const { return splits == 1 ? 0 : whole < 0 ? tail : 8 * (int64_t)tail; }  // items that are split
+  int parts;                   // pairs of waves per workgroup
+  int splits, first, n_split;  // as in BwdArgs
+  int64_t places() const { return splits == 1 ? 0 : first < 0 ? n_split : 8 * (int64_t)n_split; }  // items that are split
 };
 
 // fp32: the items behind the last full round of an XCD's workgroups are split, by three where lists may be long.
@@ -796,20 +808,25 @@ struct Deal {
 // [1, 20, 3333, 128] with a tenth of the blocks 265 / 278 and 403 / 393. 16-bit steps are too short for it: dense
 // lists of 40 gain 171 / 163 and 229 / 227 (by two 159 and 222), the same lists with a fifth of the blocks lose 54 / 61
 // and 87 / 94, and the host does not know which they are.
-Deal deal(int64_t n_items, int width, int D, bool f32) {
+//
+// 16 bits: text items, several times as long as the others, are split by two where they outlast them: up to one
+// round of workgroups over lists of 40 and more, two rounds over 96. Whole / split, us of the query pass, texts of 4
+// blocks: [2, 12, 1350 x 5626, 64] with 0.3 of the blocks 59 / 53, [1, 8, 3000, 64] 0.2 of them 31 / 26, [1, 10, 8000, 64]
+// 0.1 of them 78 / 59 (more splits: 51, 26, 63 and slower); past those lines [1, 5, 1500, 64] 18 / 20, [1, 24, 4546,
+// 64] 89 / 95, [1, 20, 3000, 64] dense 80 / 90, [1, 30, 8000, 64] 136 / 147.
+Deal deal(int64_t n_items, int n_own, int n_text, int width, int D, bool f32) {
   Deal d = {2, splits_of(n_items, width, D, f32), -1, (int)n_items};
   if (d.splits > 1) return d;
-  if (!f32) {
-    d.parts = pairs_per_item((int)n_items, width, D);
+  const int slots = xcd_slots(n_items);
+  if (f32) {
+    const int left = slots % (D == 64 ? 64 : 32);  // (two workgroups, or one, per CU)
+    if (left > 0 && width >= 16) d = {2, width >= 32 ? 3 : 2, slots - left, left};
     return d;
   }
-  const int slots = xcd_slots(n_items);
-  const int left = slots % (D == 64 ? 64 : 32);  // (two workgroups, or one, per CU)
-  if (left > 0 && width >= 16) {
-    d.splits = width >= 32 ? 3 : 2;
-    d.whole = slots - left;
-    d.tail = left;
-  }
+  d.parts = pairs_per_item((int)n_items, width, D);
+  const int room = 32 * (D == 64 ? 3 : 2);  // of workgroups of two pairs
+  if (n_text > 0 && d.parts == 2 && (slots <= room ? width >= 40 : slots <= 2 * room && width >= 96))
+    d = {2, 2, 0, text_slots(n_items, n_own, n_text)};
   return d;
 }
 
@@ -830,10 +847,10 @@ void launch_pass_f32(const BwdArgs& a, int D, hipStream_t s) {
 
 template <bool kKeys>
 void launch_pass_any(BwdArgs& a, int dtype, int D, const Deal& d, hipStream_t s) {
-  // (a caller's order may have other slots than a plain one)
-  a.splits = d.splits > 1 && d.whole >= 0 && xcd_slots(a.n_slots) != d.whole + d.tail ? 1 : d.splits;
-  a.whole = d.whole;
-  a.tail = d.tail;
+  // (a caller's order may have fewer slots than a plain one)
+  a.splits = d.first >= 0 && d.first + d.n_split > xcd_slots(a.n_slots) ? 1 : d.splits;
+  a.first = d.first;
+  a.n_split = d.n_split;
   if (dtype == SA_DTYPE_F32) return launch_pass_f32<kKeys>(a, D, s);
   if (dtype == SA_DTYPE_F16)
     return D == 64 ? launch_pass<kKeys, _Float16, 64>(a, d.parts, s) : launch_pass<kKeys, _Float16, 128>(a, d.parts, s);
@@ -857,8 +874,8 @@ Layout layout(const sa_attn_train& t) {
   l.q_idx = l.q_beg + align256(BH * (nkb + 1) * (int64_t)sizeof(int32_t));
   l.partial = l.q_idx + align256(BH * nqb * t.max_cnt * (int64_t)sizeof(int32_t));
   // (a list is no longer than the other side has blocks, but for repeated entries)
-  l.q = deal(BH * nqb, (int)std::min<int64_t>(t.max_cnt, nkb), t.D, f32);
-  l.k = deal(BH * nkb, (int)nqb, t.D, f32);
+  l.q = deal(BH * nqb, (int)nqb, t.n_text_blocks, (int)std::min<int64_t>(t.max_cnt, nkb), t.D, f32);
+  l.k = deal(BH * nkb, (int)nkb, t.n_text_blocks, (int)nqb, t.D, f32);
   const int64_t tile = (int64_t)kBlk * t.D * sizeof(float);
   l.bytes = l.partial + std::max(l.q.places() * l.q.splits * tile, l.k.places() * l.k.splits * 2 * tile);
   return l;

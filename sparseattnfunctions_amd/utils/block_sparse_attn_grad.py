@@ -109,7 +109,7 @@ class _Plan:
         nqb, nkb = math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK)
         n_items = B * H * nqb
         args = self.args = _lib.AttnTrain(dtype=_lib.DTYPES[dtype], B=B, H=H, Lq=Lq, Lk=Lk, D=D, max_cnt=max_cnt, parts=1,
-                                          sm_scale=sm_scale)
+                                          sm_scale=sm_scale, n_text_blocks=n_text_blocks)
         self.out, self.lse = (B, H, Lq, D), (B, H, nqb * BLOCK)
         self.grads = (B, H, Lq, D), (B, H, Lk, D), (B, H, Lk, D)
         sq, sk = (H * Lq * D, Lq * D, D), (H * Lk * D, Lk * D, D)

@@ -111,6 +111,25 @@ def test_fp32_remainders(dev, H, L, D, text):
     assert all(torch.equal(a, b) for a, b in zip(got, _grads(fn, *(t.to(dev) for t in (q, k, v, do)))))
 
 
+# Text blocks whose long lists are split: of the query pass, of the key pass (and more text blocks than a head has
+# blocks), of both, unlike many of them on each XCD.
+@pytest.mark.parametrize("H,Lq,Lk,D,text,bias", [(12, 330, 2700, 64, 4, True), (24, 2700, 200, 128, 9, False),
+                                                 (3, 6200, 6150, 64, 1, False)])
+def test_split_text_blocks(dev, H, Lq, Lk, D, text, bias):
+    case(f"split text blocks H={H} {Lq} x {Lk} D={D}")
+    (q, k, v, do), g = _inputs(18, BF16, 2 if bias else 1, H, Lq, Lk, D)
+    B = q.shape[0]
+    mask = _mask(g, B, H, Lq, Lk, 0.2, 0.1)
+    mask[:, :, :text] = True
+    mask[..., :text] = True
+    b = _rand(g, B, 1, Lk) if bias else None
+    fn = lambda *x: block_sparse_train_fn(*x, mask.to(dev), 0.125, n_text_blocks=text,
+                                          key_bias=b.to(dev) if bias else None)
+    got = _grads(fn, *(t.to(dev) for t in (q, k, v, do)))
+    check(got, reference(q, k, v, do, mask, 0.125, bias=b), norm=1.5 * unit(BF16))
+    assert all(torch.equal(x, y) for x, y in zip(got, _grads(fn, *(t.to(dev) for t in (q, k, v, do)))))
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_text_blocks(dev, D):
     # The hint of long first rows changes the schedule (shared rows in the forward pass) and no value.
