@@ -24,6 +24,13 @@
 // with row reads for the first and transposed reads for the second from the same LDS rows. For dk and
 // dv the streamed rows' -lse / scale and -delta start the accumulators of S and dP, so that an element
 // costs two products, an exp2 and its share of two roundings.
+//
+// Bound: the issue of MFMA and VALU, as in the forward pass. [2, 30, 2560, 64] bf16 with every block: query pass
+// 177 us (850 TFLOP/s of its three products), key pass 229 us (880 of its four); there the matrix cores work 51 % of
+// the cycles at 1.85 GHz under the power limit, the VALU 42 %, LDS 40 % without bank conflicts, and 85 % of the CU
+// time has a workgroup. [1, 15, 8229, 128] fp16 with 0.35 of the blocks: 327 and 418 us (835, 870), the
+// matrix cores 49 %, CUs 79 %: lists of unlike lengths over two rounds. Of four parts, wave priorities over
+// the two product phases, and splits of the last round nothing was faster (see deal).
 #include <math.h>
 
 #include <algorithm>
@@ -467,7 +474,8 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
 // products. Steps, stages and parts are those of bsa_bwd_kernel. The contraction over d gives k slot hh of
 // step s the value d = hh * kD / 2 + s, so that a lane reads half a row in 16-byte chunks; that over the
 // streamed rows takes row 8 (e / 4) + 4 hh + e % 4 at step e, where P and dS lie, and reads 32
-// consecutive values of it per lane half.
+// consecutive values of it per lane half. Bound by the matrix cores: [1, 30, 2560, 64] with half the blocks 349
+// us (query pass) and 463 (key pass with its lists), 110 TFLOP/s of the 154 that a large fp32 product reaches.
 
 __device__ inline sa_f32x16 mfma32x2(float x, float y, sa_f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x2f32(x, y, c, 0, 0, 0);
@@ -698,7 +706,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   }
 }
 
-// Gradients from the splits' sums, in order: one workgroup per split item and result.
+// Gradients from the splits' sums, in order: D / 16 workgroups per split item and result, four values a thread.
 template <bool kKeys, typename T>
 __global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
   constexpr int kAcc = kKeys ? 2 : 1;
@@ -716,29 +724,29 @@ __global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
   const float f = x == 0 ? a.sm_scale : 1.f;
   const int64_t n = (int64_t)kBlk * D;
   const float* from = a.partial + ((int64_t)place * a.splits * kAcc + x) * n;
-  for (int t = threadIdx.x; t < kBlk * D / 4; t += 256) {
-    const int r = t / (D / 4), d = 4 * (t % (D / 4));
-    if (blk * kBlk + r >= a.L_own) break;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < a.splits; ++p) {
-      const float4 y = *reinterpret_cast<const float4*>(from + (int64_t)p * kAcc * n + 4 * t);
-      s.x += y.x;
-      s.y += y.y;
-      s.z += y.z;
-      s.w += y.w;
-    }
-    T* o = g + (int64_t)(blk * kBlk + r) * sl + d;
-    if constexpr (std::is_same<T, float>::value)
-      *reinterpret_cast<float4*>(o) = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
-    else
-      *reinterpret_cast<uint2*>(o) = make_uint2(Elem<T>::pack(s.x * f, s.y * f), Elem<T>::pack(s.z * f, s.w * f));
+  const int t = blockIdx.z * 256 + threadIdx.x;
+  const int r = t / (D / 4), d = 4 * (t % (D / 4));
+  if (blk * kBlk + r >= a.L_own) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int p = 0; p < a.splits; ++p) {
+    const float4 y = *reinterpret_cast<const float4*>(from + (int64_t)p * kAcc * n + 4 * t);
+    s.x += y.x;
+    s.y += y.y;
+    s.z += y.z;
+    s.w += y.w;
   }
+  T* o = g + (int64_t)(blk * kBlk + r) * sl + d;
+  if constexpr (std::is_same<T, float>::value)
+    *reinterpret_cast<float4*>(o) = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+  else
+    *reinterpret_cast<uint2*>(o) = make_uint2(Elem<T>::pack(s.x * f, s.y * f), Elem<T>::pack(s.z * f, s.w * f));
 }
 
 template <bool kKeys, typename T>
 void launch_merge(const BwdArgs& a, int D, hipStream_t s) {
   if (a.splits > 1)
-    hipLaunchKernelGGL((bwd_merge_kernel<kKeys, T>), dim3((unsigned)(a.first < 0 ? a.n_items : 8 * a.n_split), kKeys ? 2 : 1),
+    hipLaunchKernelGGL((bwd_merge_kernel<kKeys, T>), dim3((unsigned)(a.first < 0 ? a.n_items : 8 * a.n_split), kKeys ? 2 : 1, D / 16),
                        dim3(256), 0, s, a, D);
 }
 
@@ -776,7 +784,7 @@ int pairs_per_item(int n_items, int max_cnt, int D) {
 // and their lists (of up to `width` entries) are long: at least 8 entries each. Without / with, us of the
 // query pass of 64 queries and the key pass of 64 keys against 17 776 of the other: one head 93 / 9 and 114 / 10,
 // 30 heads 112 / 27 and 120 / 29; fp32, one head 594 / 36 and 1 076 / 48; [1, 1, 2048, 64], 8 of 32 blocks, 10.3 /
-// 7.0 and 10.9 / 8.0. The merge is 4 us more: two to five splits gain no more than that (160 items with dense
+// 7.0 and 10.9 / 8.0. The merge is 4 to 5 us more: two to five splits gain no more than that (160 items with dense
 // lists of 40: 24.2 / 21.2 and the merge), but in fp32, whose steps take 16 times as long.
 int splits_of(int64_t n_items, int width, int D, bool f32) {
   if (width < (f32 ? 16 : 32)) return 1;

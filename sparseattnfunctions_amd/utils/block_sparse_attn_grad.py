@@ -13,12 +13,16 @@ does as well. Training code calls this module instead:
     autograd, e.g. for a step captured into a HIP graph.
 
 The forward pass is the kernel of `block_sparse_attention` with bf16 (fp16) scores, or fp32 on split
-operands, and also stores each row's log2-sum-exp2; the backward pass recomputes the probabilities from it, block by
-block, and keeps nothing of the size of the attention map (`sa_block_sparse_bwd`). Gradients of a
-16-bit call round P and dS to its type, sums are fp32 in a fixed order, so that a step repeats bit for
-bit. In fp16, dS has the range of the type: scale the loss as usual. A query row without a key (an
-empty list, or keys all biased to -inf) has a zero output and zero gradients; a key block in no list
-has zero gradients. The mask, the lists and key_bias are not differentiated.
+operands, and also stores each row's log2-sum-exp2; the backward pass recomputes the probabilities
+from it, block by block, and keeps nothing of the size of the attention map (`sa_block_sparse_bwd`).
+Gradients of a 16-bit call round P and dS to its type, sums are fp32 in a fixed order, so that a step
+repeats bit for bit. In fp16, dS has the range of the type: scale the loss as usual. A query row
+without a key (an empty list, or keys all biased to -inf) has a zero output and zero gradients; a key
+block in no list has zero gradients. The mask, the lists and key_bias are not differentiated.
+
+A key_bias below -2.35e38 (the type's lowest value among them) counts as -inf, and keys that it masks
+still enter the products: their k and v have to be finite, as with any additive mask. Keys in blocks
+that no row lists, and memory behind the last row, are not read into any sum.
 """
 from __future__ import annotations
 
@@ -281,8 +285,12 @@ def block_sparse_attention_train(q, k, v, kv: KVList, sm_scale: float, key_bias:
     q [B,H,Lq,D], k/v [B,H,Lk,D] on the GPU, bf16, fp16 or fp32 (one type), D = 64 or 128, any strides
     (tensors whose rows are not 16-byte aligned are copied); key_bias fp32 [B,H,Lk] or None, not
     differentiated, not with fp32. `n_text_blocks` only affects scheduling: so many first block rows
-    and columns are listed by every other block, beside shorter lists. The lists (and key_bias) must stay as they are until
-    the backward pass has run."""
+    and columns are listed by every other block, beside shorter lists. The lists (and key_bias) must
+    stay as they are until the backward pass has run.
+
+    A call captured into a HIP graph needs an eager one of its shapes before it (which makes the
+    dispatch orders), and leaves that no eager graph holds: autograd ties a leaf's gradient to the
+    stream of the leaf's first use, and its backward pass outside the capture would end the process."""
     key_bias = _check_inputs(q, k, v, kv, key_bias)
     return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
 
