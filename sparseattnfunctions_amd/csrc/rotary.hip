@@ -96,9 +96,10 @@ typedef uint32_t Words __attribute__((ext_vector_type(4)));
 // Loads of kUnroll heads are in flight together.
 //
 // kLines: each store of a wave fills whole lines (interleaved 16-bit values), so that they need not wait
-// in a cache for the rest: they are streamed out. [2, 30, 17776, 64] queries and keys in bf16 take 91 us so
-// (6.0 TB/s), 108 with ordinary stores; halves (106 us, streamed 110) and fp32
-// (30 us, streamed 33), whose lines are put together from two stores, keep the ordinary ones.
+// in a cache for the rest: they are streamed out. [2, 30, 17776, 64] queries and keys in bf16 take 98 us so
+// (5.6 TB/s, other tensors each time; 91 the same ones), 105 (108) with ordinary stores; halves (107 us, streamed
+// 109) and fp32 halves ([1, 15 + 5, 8229, 128] 42 us, 4.1 TB/s, streamed 42 to 48), whose lines are put together
+// from two stores, keep the ordinary ones.
 template <typename T, bool kHalf, int V>
 __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
   constexpr int kUnroll = 4;
