@@ -45,6 +45,7 @@ namespace {
 
 constexpr int kBlk = 64;   // rows per block of either side
 constexpr int kStep = 32;  // streamed rows per step, own rows per wave
+constexpr int kMostLast = 128;
 
 struct BwdArgs {
   const void* own_a;  // k or q
@@ -83,6 +84,9 @@ struct BwdArgs {
   // item, n_split of them) are computed by `splits` workgroups each, on shares of the item's steps, which store
   // their sums to partial[place][split][result][64][kD]; bwd_merge_kernel adds them in order.
   int splits, first, n_split;
+  // The items of an XCD's last n_last slots (at most kMostLast; not beside splits) run longest list first; lists
+  // below 2^length_bits - 1 entries are told apart.
+  int n_last, length_bits;
   float* partial;
 };
 
@@ -95,6 +99,9 @@ __device__ inline float2 unpack2(uint32_t w) {
   return make_float2((float)h[0], (float)h[1]);
 }
 
+// Slots of an XCD.
+__host__ __device__ inline int xcd_slots(int64_t n_slots) { return (int)(((n_slots + 3) / 4 + 7) / 8 * 4); }
+
 // Item of slot `seq` of XCD `xcd` (the work order's slots come in groups of four, group w on XCD w % 8).
 __device__ inline int slot_item(const BwdArgs& a, int xcd, int seq) {
   const int slot = 4 * (8 * (seq >> 2) + xcd) + (seq & 3);
@@ -102,9 +109,51 @@ __device__ inline int slot_item(const BwdArgs& a, int xcd, int seq) {
   return a.order ? order_item(a.order, slot) : slot;
 }
 
+// Entries of an item's list.
+template <bool kKeys>
+__device__ inline int list_length(const BwdArgs& a, int item) {
+  if (!kKeys) return min(max(a.cnt[item], 0), a.max_cnt);
+  const int bh = item / a.n_own;
+  const int32_t* beg = a.cnt + item + bh;  // bh * (n_own + 1) + block
+  return beg[1] - beg[0];
+}
+
+// The item with the t-th longest list (from 0) of the XCD's last slots, the same in every lane: the largest key that
+// t + 1 of them reach, bit by bit. Keys are unlike, equal lists in order of their slots.
+template <bool kKeys>
+__device__ inline int longest_item(const BwdArgs& a, int xcd, int from, int t) {
+  constexpr int kPer = kMostLast / 64;
+  const int lane = threadIdx.x & 63;
+  int item[kPer];
+  uint32_t key[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = lane + 64 * i;
+    item[i] = at < a.n_last ? slot_item(a, xcd, from + at) : -1;
+    const bool ok = item[i] >= 0 && item[i] < a.n_items;
+    const int n = ok ? min(1 + list_length<kKeys>(a, item[i]), (1 << a.length_bits) - 1) : 0;
+    key[i] = at < a.n_last ? (uint32_t)(n * kMostLast + kMostLast - 1 - at) : 0;
+  }
+  uint32_t found = 0;
+  for (uint32_t bit = (uint32_t)kMostLast << a.length_bits >> 1; bit; bit >>= 1) {
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) reach += __popcll(__ballot(key[i] >= (found | bit)));
+    if (reach > t) found |= bit;
+  }
+  int r = -1;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint64_t m = __ballot(key[i] == found && lane + 64 * i < a.n_last);
+    if (m) r = __builtin_amdgcn_readlane(item[i], __ffsll((unsigned long long)m) - 1);
+  }
+  return r;
+}
+
 // Item of a workgroup (-1: none), its split, and the place of its sums (-1: not split). The dispatcher deals
 // workgroups out to the XCDs in turn. Where every item is split there are no idle workgroups, which would
 // leave CUs out of turn ([1, 1, 64 x 17776, 64] in fp32 ran on a quarter of 32 CUs): item and split count up.
+template <bool kKeys, bool kSorted>
 __device__ inline int bwd_item(const BwdArgs& a, int x, int& split, int& place) {
   split = 0;
   place = -1;
@@ -122,6 +171,10 @@ __device__ inline int bwd_item(const BwdArgs& a, int x, int& split, int& place) 
     } else {
       seq -= a.n_split * (a.splits - 1);
     }
+  }
+  if constexpr (kSorted) {
+    const int from = xcd_slots(a.n_slots) - a.n_last;
+    if (seq >= from) return longest_item<kKeys>(a, x & 7, from, seq - from);
   }
   return slot_item(a, x & 7, seq);
 }
@@ -167,7 +220,7 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   const int part = wave >> 1, w = wave & 1;
   const int col = lane & 31, hh = lane >> 5;
   int split, place;
-  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x, split, place));
+  const int item = __builtin_amdgcn_readfirstlane(bwd_item<kKeys, true>(a, blockIdx.x, split, place));
   if (item < 0 || item >= a.n_items) return;  // (the whole workgroup)
   const int bh = item / a.n_own;
   const int blk = item - bh * a.n_own;
@@ -503,7 +556,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   const int part = wave >> 1, w = wave & 1;
   const int col = lane & 31, hh = lane >> 5;
   int split, place;
-  const int item = __builtin_amdgcn_readfirstlane(bwd_item(a, blockIdx.x, split, place));
+  const int item = __builtin_amdgcn_readfirstlane(bwd_item<kKeys, false>(a, blockIdx.x, split, place));
   if (item < 0 || item >= a.n_items) return;  // (the whole workgroup)
   const int bh = item / a.n_own;
   const int blk = item - bh * a.n_own;
@@ -750,9 +803,6 @@ void launch_merge(const BwdArgs& a, int D, hipStream_t s) {
                        dim3(256), 0, s, a, D);
 }
 
-// Slots of an XCD.
-int xcd_slots(int64_t n_slots) { return (int)(((n_slots + 3) / 4 + 7) / 8 * 4); }
-
 unsigned workgroups(const BwdArgs& a) {
   if (a.splits > 1 && a.first < 0) return (unsigned)a.n_items * a.splits;
   return 8u * (xcd_slots(a.n_slots) + (a.splits - 1) * a.n_split);
@@ -806,6 +856,7 @@ int text_slots(int64_t n_items, int n_own, int n_text) {
 struct Deal {
   int parts;                   // pairs of waves per workgroup
   int splits, first, n_split;  // as in BwdArgs
+  int n_last, length_bits;
   int64_t places() const { return splits == 1 ? 0 : first < 0 ? n_split : 8 * (int64_t)n_split; }  // items that are split
 };
 
@@ -822,19 +873,30 @@ struct Deal {
 // blocks: [2, 12, 1350 x 5626, 64] with 0.3 of the blocks 59 / 53, [1, 8, 3000, 64] 0.2 of them 31 / 26, [1, 10, 8000, 64]
 // 0.1 of them 78 / 59 (more splits: 51, 26, 63 and slower); past those lines [1, 5, 1500, 64] 18 / 20, [1, 24, 4546,
 // 64] 89 / 95, [1, 20, 3000, 64] dense 80 / 90, [1, 30, 8000, 64] 136 / 147.
+//
+// 16 bits, more than one round: the last round's items, which run together in any order, start with the longest lists
+// (other orders of all items part neighbours that share keys). Order of the items / longest first, us of both
+// passes, random lists: [1, 15, 8229, 128] 0.35 of the blocks 315 / 280 and 411 / 385, [2, 15, 4096, 128] 0.3 of them 139 /
+// 126 and 200 / 185, [1, 15, 17776, 64] 0.2 of them 377 / 359 and 511 / 504, [1, 8, 8192, 64] 0.3 of them 80 / 72 and 117 /
+// 108; equal or short lists pay one to two us for it: [2, 30, 2560, 64] a fifth of 40 blocks 53 / 54 and 86 / 88.
 Deal deal(int64_t n_items, int n_own, int n_text, int width, int D, bool f32) {
-  Deal d = {2, splits_of(n_items, width, D, f32), -1, (int)n_items};
+  Deal d = {2, splits_of(n_items, width, D, f32), -1, (int)n_items, 0, 1};
   if (d.splits > 1) return d;
   const int slots = xcd_slots(n_items);
   if (f32) {
     const int left = slots % (D == 64 ? 64 : 32);  // (two workgroups, or one, per CU)
-    if (left > 0 && width >= 16) d = {2, width >= 32 ? 3 : 2, slots - left, left};
+    if (left > 0 && width >= 16) d = {2, width >= 32 ? 3 : 2, slots - left, left, 0, 1};
     return d;
   }
   d.parts = pairs_per_item((int)n_items, width, D);
   const int room = 32 * (D == 64 ? 3 : 2);  // of workgroups of two pairs
   if (n_text > 0 && d.parts == 2 && (slots <= room ? width >= 40 : slots <= 2 * room && width >= 96))
-    d = {2, 2, 0, text_slots(n_items, n_own, n_text)};
+    return {2, 2, 0, text_slots(n_items, n_own, n_text), 0, 1};
+  const int round = room * 2 / d.parts;
+  if (slots > round && round <= kMostLast && width >= (D == 64 ? 64 : 32)) {
+    d.n_last = round;
+    while (d.length_bits < 22 && (1 << d.length_bits) < width + 3) ++d.length_bits;
+  }
   return d;
 }
 
@@ -859,6 +921,8 @@ void launch_pass_any(BwdArgs& a, int dtype, int D, const Deal& d, hipStream_t s)
   a.splits = d.first >= 0 && d.first + d.n_split > xcd_slots(a.n_slots) ? 1 : d.splits;
   a.first = d.first;
   a.n_split = d.n_split;
+  a.n_last = a.splits == 1 ? std::min(d.n_last, xcd_slots(a.n_slots)) : 0;
+  a.length_bits = d.length_bits;
   if (dtype == SA_DTYPE_F32) return launch_pass_f32<kKeys>(a, D, s);
   if (dtype == SA_DTYPE_F16)
     return D == 64 ? launch_pass<kKeys, _Float16, 64>(a, d.parts, s) : launch_pass<kKeys, _Float16, 128>(a, d.parts, s);

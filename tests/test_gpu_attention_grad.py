@@ -111,6 +111,24 @@ def test_fp32_remainders(dev, H, L, D, text):
     assert all(torch.equal(a, b) for a, b in zip(got, _grads(fn, *(t.to(dev) for t in (q, k, v, do)))))
 
 
+# Launches of more than a round, whose last items run longest list first: the bits of launches of some heads
+# each, which take the order of the items.
+@pytest.mark.parametrize("dtype,H,group,L,D", [(BF16, 12, 6, 4170, 64), (FP16, 33, 11, 2090, 128)])
+def test_last_round_by_length(dev, dtype, H, group, L, D):
+    case(f"last round H={H} L={L} D={D}")
+    (q, k, v, do), g = _inputs(19, dtype, 1, H, L, L, D)
+    mask = _mask(g, 1, H, L, L, 0.1, 0.2)
+    mask &= torch.rand(1, H, *mask.shape[2:], generator=g) < torch.rand(1, H, mask.shape[2], 1, generator=g)
+    q, k, v, do, mask = (t.to(dev) for t in (q, k, v, do, mask))
+    got = _grads(lambda *x: block_sparse_train_fn(*x, mask, 0.125), q, k, v, do)
+    for h in range(0, H, group):
+        some = slice(h, h + group)
+        want = _grads(lambda *x: block_sparse_train_fn(*x, mask[:, some], 0.125), *(t[:, some] for t in (q, k, v, do)))
+        assert all(torch.equal(x[:, some], y) for x, y in zip(got[1:], want[1:]))
+    check([x[:, :1] for x in got], reference(*(t[:, :1].cpu() for t in (q, k, v, do, mask)), 0.125),
+          norm=1.5 * unit(dtype))
+
+
 # Text blocks whose long lists are split: of the query pass, of the key pass (and more text blocks than a head has
 # blocks), of both, unlike many of them on each XCD.
 @pytest.mark.parametrize("H,Lq,Lk,D,text,bias", [(12, 330, 2700, 64, 4, True), (24, 2700, 200, 128, 9, False),
