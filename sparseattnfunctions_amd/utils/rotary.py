@@ -22,6 +22,7 @@ import math
 from typing import Optional, Sequence, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -226,6 +227,12 @@ def _launch(q, q_out, k, k_out, table, layout, skip, rows, inverse):
 
 def _turned(q, k, table, layout, skip, rows, inverse):
     """New tensors of q's and k's (either may be None) memory layouts."""
+    if q is not None and k is not None and q.stride(-1) == k.stride(-1) == 1 and q.numel() and k.numel() \
+            and table.shape[0]:
+        q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+        if q_out.stride(-1) == k_out.stride(-1) == 1:
+            _launch(q, q_out, k, k_out, table, layout, skip, rows, inverse)
+            return q_out, k_out
     xs = [x if x.stride(-1) == 1 else x.contiguous() for x in (q, k) if x is not None]
     outs = [torch.empty_like(x) for x in xs]
     outs = [o if o.stride(-1) == 1 else torch.empty(o.shape, dtype=o.dtype, device=o.device) for o in outs]
@@ -277,7 +284,16 @@ def apply_rotary(q, k, table, layout: str = "interleaved", skip: int = 0, rows: 
     padding. `inverse` turns back."""
     _check(q, k, table, layout, skip, rows)
     rows = rows if rows is None or rows.stride(-1) == 1 else rows.contiguous()
-    return _ApplyRotary.apply(q, k, table, layout, int(skip), rows, bool(inverse))
+    if _followed(q) or _followed(k):
+        return _ApplyRotary.apply(q, k, table, layout, int(skip), rows, bool(inverse))
+    return _turned(q, k, table, layout, int(skip), rows, bool(inverse))
+
+
+def _followed(x) -> bool:
+    """Whether autograd has to know of an operation on x (entering it costs a call of one token 4 us of 17).
+    Forward-mode tangents are left to autograd, which refuses them."""
+    return x is not None and (x.requires_grad and torch.is_grad_enabled()
+                              or forward_ad.unpack_dual(x).tangent is not None)
 
 
 def apply_rotary_(q, k, table, layout: str = "interleaved", skip: int = 0, rows: Optional[torch.Tensor] = None,

@@ -251,6 +251,26 @@ def test_second_derivatives_and_partial_gradients(dev):
     assert torch.equal(gk, only)
 
 
+def test_with_and_without_autograd(dev):
+    # The same values with gradients, without, and where they are off; forward-mode tangents are refused.
+    case("rotary without autograd")
+    table = rotary_table(torch.arange(20, device=dev), 64)
+    q, k = torch.randn(2, 1, 3, 20, 64, device=dev)
+    want = apply_rotary(q, k, table)
+    assert not want[0].requires_grad and not want[1].requires_grad
+    for grads in ((True, False), (False, True)):
+        x, y = (t.clone().requires_grad_(g) for t, g in zip((q, k), grads))
+        got = apply_rotary(x, y, table)
+        assert got[0].requires_grad and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        with torch.no_grad():
+            got = apply_rotary(x, y, table)
+        assert not got[0].requires_grad and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(k, torch.ones_like(k))
+        with pytest.raises(RuntimeError):
+            apply_rotary(q, dual, table)
+
+
 def test_no_tokens_or_heads(dev):
     case("rotary empty")
     table = rotary_table(torch.arange(4, device=dev), 64)
