@@ -523,34 +523,60 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   }
 }
 
-// ---- fp32: the same passes on v_mfma_f32_32x32x2_f32, which takes 16 times as long as the 16-bit
-// products. Steps, stages and parts are those of bsa_bwd_kernel. The contraction over d gives k slot hh of
-// step s the value d = hh * kD / 2 + s, so that a lane reads half a row in 16-byte chunks; that over the
-// streamed rows takes row 8 (e / 4) + 4 hh + e % 4 at step e, where P and dS lie, and reads 32
-// consecutive values of it per lane half. Bound by the matrix cores: [1, 30, 2560, 64] with half the blocks 349
-// us (query pass) and 463 (key pass with its lists), 110 TFLOP/s of the 154 that a large fp32 product reaches.
+// ---- fp32: the same passes on the bf16 matrix core, whose rate is 16 times the fp32 one's: every operand is
+// split exactly into three bf16 terms (x = hi + mid + lo, 8 significand bits each) and each product takes the six
+// term products down to 2^-18 of the largest (the dropped ones are below 2^-26), smallest first, in fp32 sums.
+// Streamed rows are loaded a step ahead into registers, split once per pair of waves and stored to LDS as three
+// 16-bit tiles of bsa_bwd_kernel's layout, whose row and transposed reads serve both products; P and dS are split
+// where they come out. One stage and two barriers per step (a step's products take 2 304 cycles and more at head
+// dim 64).
+//
+// Bound: the matrix core, beside the splits (11 VALU operations a pair of values) and exp2. [1, 30, 2560, 64] with
+// half the blocks: query pass 256 us, key pass with its lists 325 (150 and 160 TFLOP/s of fp32 products, six times
+// that in bf16 ones; on the fp32 matrix instructions 365 and 459); [1, 10, 3500, 128] with 0.4 of them 289 and 390
+// (410 and 555). Values have to be finite; those below about 1e-33, as of gradients of a loss scaled down so far, lose
+// their low terms.
 
-__device__ inline sa_f32x16 mfma32x2(float x, float y, sa_f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x2f32(x, y, c, 0, 0, 0);
+// The six term products of A and B onto c.
+__device__ inline sa_f32x16 mfma_terms(const sa_u32x4v (&A)[3], const sa_bf16x8 (&B)[3], sa_f32x16 c) {
+  c = mfma32(as_bf16x8(A[0]), B[2], c);
+  c = mfma32(as_bf16x8(A[2]), B[0], c);
+  c = mfma32(as_bf16x8(A[1]), B[1], c);
+  c = mfma32(as_bf16x8(A[0]), B[1], c);
+  c = mfma32(as_bf16x8(A[1]), B[0], c);
+  return mfma32(as_bf16x8(A[0]), B[0], c);
 }
 
-// Chunk c (16 bytes) of LDS row r lies at chunk c ^ swz_f32(r) of its 256 bytes. Sixteen rows at one
-// chunk take every bank once (row reads), as do 32 values of a row and of the row four below it
-// (column reads).
-__device__ inline int swz_f32(int r) { return (r & 3) | ((r >> 1) & 4) | ((r << 1) & 8); }
+// Eight fp32 values (two 16-byte loads) as operand terms.
+__device__ inline void split8(sa_u32x4v x, sa_u32x4v y, sa_u32x4v (&t)[3]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const sa_u32x4v& z = i < 2 ? x : y;
+    uint32_t hi, mid, lo;
+    split3(__uint_as_float(z[2 * (i & 1)]), __uint_as_float(z[2 * (i & 1) + 1]), hi, mid, lo);
+    t[0][i] = hi;
+    t[1][i] = mid;
+    t[2][i] = lo;
+  }
+}
 
 template <bool kKeys, int kD>
 __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdArgs a) {
   constexpr int kParts = 2;
-  constexpr int kHD = kD / 2;
+  constexpr int kDS = kD / 16;
   constexpr int kDC = kD / 32;
+  constexpr int kHalves = kD / 64;
   constexpr int kAcc = kKeys ? 2 : 1;
-  constexpr int kRow = kD * 4;             // bytes of a row
-  constexpr int kMat = kStep * kRow;       // a step's rows of one matrix
-  constexpr int kCopies = kMat / 1024;     // 1 KB each
-  constexpr int kLanes = kRow / 16;        // lanes per row of a copy
-  __shared__ __attribute__((aligned(1024))) uint8_t tile0[kParts * 2 * kMat], tile1[kParts * 2 * kMat];
-  __shared__ __attribute__((aligned(256))) float stat0[kParts * 64], stat1[kParts * 64];
+  constexpr int kRowTile = kStep * 128;       // one half of a step's rows of one term
+  constexpr int kTerm = kHalves * kRowTile;   // a step's rows of one term
+  constexpr int kMat = 3 * kTerm;             // of one matrix
+  constexpr int kLanes = kD / 8;              // lanes per row of a copy, 8 values each
+  constexpr int kPasses = kStep * kLanes / 64;
+  __shared__ __attribute__((aligned(1024))) uint8_t tile_lds[kParts * 2 * kMat];
+  __shared__ __attribute__((aligned(256))) float stat[kParts * 64];
+  // The key pass at two waves per SIMD has no registers for its own v's low terms (spilled: 348 us for the 325 above).
+  constexpr bool kLowInLds = kKeys && kD == 64;
+  __shared__ sa_u32x4v low[kLowInLds ? 2 * kParts : 1][kLowInLds ? kDS : 1][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int part = wave >> 1, w = wave & 1;
@@ -566,24 +592,34 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   const auto list = bwd_list<kKeys>(a, item, bh, blk, cnt);
   const int own_row = blk * kBlk + kStep * w + col;
   const int own_clamped = min(own_row, a.L_own - 1);  // rows past L_own are never stored
-  const float* oa = static_cast<const float*>(a.own_a) + b * a.oa_sb + h * a.oa_sh + (int64_t)own_clamped * a.oa_sl;
-  const float* ob = static_cast<const float*>(a.own_b) + b * a.ob_sb + h * a.ob_sh + (int64_t)own_clamped * a.ob_sl;
-  float fa[kHD], fb[kHD];
-#pragma unroll
-  for (int s = 0; s < kHD; s += 4) {
-    const float4 x = *reinterpret_cast<const float4*>(oa + hh * kHD + s);
-    const float4 y = *reinterpret_cast<const float4*>(ob + hh * kHD + s);
-    fa[s] = x.x; fa[s + 1] = x.y; fa[s + 2] = x.z; fa[s + 3] = x.w;
-    fb[s] = y.x; fb[s + 1] = y.y; fb[s + 2] = y.z; fb[s + 3] = y.w;
-  }
+  const float* oa = static_cast<const float*>(a.own_a) + b * a.oa_sb + h * a.oa_sh + (int64_t)own_clamped * a.oa_sl + 8 * hh;
+  const float* ob = static_cast<const float*>(a.own_b) + b * a.ob_sb + h * a.ob_sh + (int64_t)own_clamped * a.ob_sl + 8 * hh;
+  const float* op = kKeys ? nullptr : static_cast<const float*>(a.out) + b * a.o_sb + h * a.o_sh + (int64_t)own_clamped * a.o_sl + 8 * hh;
+  sa_bf16x8 fa[kDS][3], fb[kDS][3];
   float lse = 0.f, delta = 0.f;
-  if constexpr (!kKeys) {
-    const float* op = static_cast<const float*>(a.out) + b * a.o_sb + h * a.o_sh + (int64_t)own_clamped * a.o_sl;
 #pragma unroll
-    for (int s = 0; s < kHD; s += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(op + hh * kHD + s);
-      delta = fmaf(x.x, fb[s], fmaf(x.y, fb[s + 1], fmaf(x.z, fb[s + 2], fmaf(x.w, fb[s + 3], delta))));
+  for (int s = 0; s < kDS; ++s) {
+    sa_u32x4v x[2], y[2], t[3];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[i] = *reinterpret_cast<const sa_u32x4v*>(oa + 16 * s + 4 * i);
+      y[i] = *reinterpret_cast<const sa_u32x4v*>(ob + 16 * s + 4 * i);
+      if constexpr (!kKeys) {
+        const float4 o = *reinterpret_cast<const float4*>(op + 16 * s + 4 * i);
+        delta = fmaf(o.x, __uint_as_float(y[i][0]), fmaf(o.y, __uint_as_float(y[i][1]),
+                fmaf(o.z, __uint_as_float(y[i][2]), fmaf(o.w, __uint_as_float(y[i][3]), delta))));
+      }
     }
+    split8(x[0], x[1], t);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) fa[s][i] = as_bf16x8(t[i]);
+    split8(y[0], y[1], t);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (!kLowInLds || i < 2) fb[s][i] = as_bf16x8(t[i]);
+    if constexpr (kLowInLds) low[wave][s][lane] = t[2];  // (read by this lane alone)
+  }
+  if constexpr (!kKeys) {
     delta = xhalf_sum(delta);
     lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col];
     if (part == 0 && split == 0) {
@@ -598,9 +634,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   const float* st = w == 0 ? static_cast<const float*>(a.st_a) + b * a.sa_sb + h * a.sa_sh
                            : static_cast<const float*>(a.st_b) + b * a.sb_sb + h * a.sb_sh;
   const uint32_t row_bytes = (uint32_t)(w == 0 ? a.sa_sl : a.sb_sl) * 4;
-  const uint32_t st_bytes = (uint32_t)(a.L_st - 1) * row_bytes + kRow;
+  const uint32_t st_bytes = (uint32_t)(a.L_st - 1) * row_bytes + 4 * kD;
   const float* stat_src = a.stats + (int64_t)bh * a.n_st * 128;
-  const uint32_t stat_bytes = (uint32_t)a.n_st * 512;
 
   const int splits = place < 0 ? 1 : a.splits;
   const int per_split = (2 * cnt + splits - 1) / splits;
@@ -609,118 +644,149 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   const int beg = split * per_split + part * per_part;
   auto block_of = [&](int i) -> int {  // the streamed block of the part's i-th step, -1: none
     const int s = beg + i;
-    return i < per_part && s < n_steps ? list[s >> 1] : -1;
+    const int rb = i < per_part && s < n_steps ? list[s >> 1] : -1;
+    return (unsigned)rb < (unsigned)a.n_st ? rb : -1;
   };
-  auto issue = [&](int rb, int i, lds_u8* tile, lds_u8* stat) __attribute__((always_inline)) {
-    if ((unsigned)rb >= (unsigned)a.n_st) return;
+  // Rows of the part's i-th step: wave 0 st_a's (and the statistics), wave 1 st_b's. The descriptor begins at the
+  // step's rows and ends with the head's, so that rows past the last one read as zero.
+  const int r_lane = lane / kLanes, c_lane = lane % kLanes;
+  sa_u32x4v pre[kPasses][2];
+  float pre_stat = 0.f;
+  auto fetch = [&](int rb, int i) __attribute__((always_inline)) {
+    if (rb < 0) return;
     const uint32_t row0 = __builtin_amdgcn_readfirstlane(rb * kBlk + kStep * ((beg + i) & 1));
     const uint32_t off = min(row0 * row_bytes, st_bytes);
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(st) + off), (short)0, (int)(st_bytes - off), 0x00020000);
-    lds_u8* dst = tile + (part * 2 + w) * kMat;
 #pragma unroll
-    for (int j = 0; j < kCopies; ++j) {
-      const int r = j * (64 / kLanes) + lane / kLanes, c = lane % kLanes;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_u8*)(dst + 1024 * j), 16, r * row_bytes + 16 * (c ^ swz_f32(r)),
-                                               0, 0, 0);
+    for (int j = 0; j < kPasses; ++j) {
+      const uint32_t at = (j * (64 / kLanes) + r_lane) * row_bytes + 32 * c_lane;
+      pre[j][0] = __builtin_bit_cast(sa_u32x4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+      pre[j][1] = __builtin_bit_cast(sa_u32x4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16, 0, 0));
     }
-    if (kKeys && w == 0) {
-      const uint32_t soff = min(row0 * 8, stat_bytes);
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(stat_src) + soff), (short)0, (int)(stat_bytes - soff),
-          0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u8*)(stat + part * 256), 4, 4 * lane, 0, 0, 0);
-    }
+    if (kKeys && w == 0) pre_stat = stat_src[2 * row0 + lane];
   };
+  lds_u8* const tile = (lds_u8*)tile_lds + part * 2 * kMat;
+  auto stage = [&](int rb) __attribute__((always_inline)) {
+    if (rb < 0) return;
+#pragma unroll
+    for (int j = 0; j < kPasses; ++j) {
+      const int r = j * (64 / kLanes) + r_lane;
+      sa_u32x4v t[3];
+      split8(pre[j][0], pre[j][1], t);
+      lds_u8* q = tile + w * kMat + (c_lane >> 3) * kRowTile + 128 * r + 16 * ((c_lane & 7) ^ swz(r));
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<__attribute__((address_space(3))) sa_u32x4v*>(q + i * kTerm) = t[i];
+    }
+    if (kKeys && w == 0) stat[part * 64 + lane] = pre_stat;
+  };
+
+  // Lane constants of the reads (as in bsa_bwd_kernel).
+  int ro[4], to[2][2];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) ro[s] = 128 * col + 16 * ((2 * s + hh) ^ swz(col));
+  {
+    const int i = lane & 15, hq = lane >> 5, dg = (lane >> 4) & 1;
+#pragma unroll
+    for (int dc = 0; dc < 2; ++dc)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = 8 * t + 4 * hq + (i >> 2);
+        const int chunk = 4 * dc + 2 * dg + ((i & 3) >> 1);
+        to[dc][t] = 128 * r + 16 * (chunk ^ swz(r)) + 8 * (i & 1);
+      }
+  }
 
   sa_f32x16 acc[kAcc][kDC];
 #pragma unroll
   for (int x = 0; x < kAcc; ++x)
 #pragma unroll
     for (int dc = 0; dc < kDC; ++dc) acc[x][dc] = sa_f32x16{};
-  const int at_row = part * 2 * kMat + col * kRow, row_swz = swz_f32(col);
-  const int at_col = part * 2 * kMat + 4 * hh * kRow + 4 * (col & 3);
 
-  auto compute = [&](int cur, int i, const lds_u8* tile, const float* stat) __attribute__((always_inline)) {
+  auto compute = [&](int cur, int i) __attribute__((always_inline)) {
     const int row0 = cur * kBlk + kStep * ((beg + i) & 1);
-    if ((unsigned)cur >= (unsigned)a.n_st || row0 >= a.L_st) return;
-    typedef __attribute__((address_space(3))) const float lds_f;
+    if (cur < 0 || row0 >= a.L_st) return;
     sa_f32x16 S = {}, dP = {};
-    float nl[16];
+    const float* st_ = stat + part * 64 + 4 * hh;
     if constexpr (kKeys) {
-      const float* x = stat + part * 64 + 4 * hh;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        nl[e] = x[8 * (e >> 2) + (e & 3)];
-        dP[e] = x[32 + 8 * (e >> 2) + (e & 3)];
-      }
+      for (int e = 0; e < 16; ++e) dP[e] = st_[32 + 8 * (e >> 2) + (e & 3)];
     }
-    // (each group of reads is issued before the products of the group before it)
-    sa_u32x4v x[2], y[2];
-    auto rows = [&](int s) __attribute__((always_inline)) {
-      const lds_u8* q = tile + at_row + 16 * ((hh * (kHD / 4) + s / 4) ^ row_swz);
-      x[(s >> 2) & 1] = lds_read_b128(q);
-      y[(s >> 2) & 1] = lds_read_b128(q + kMat);
+    // Operands of st_a and st_b in turn, each requested before the products of the one before it.
+    sa_u32x4v x[2][3];
+    auto rows = [&](int g) __attribute__((always_inline)) {
+      const int s = g >> 1;
+#pragma unroll
+      for (int t = 0; t < 3; ++t)
+        x[g & 1][t] = lds_read_b128(tile + ro[s & 3] + (s >> 2) * kRowTile + t * kTerm + (g & 1) * kMat);
     };
     rows(0);
 #pragma unroll
-    for (int s = 0; s < kHD; s += 4) {
+    for (int g = 0; g < 2 * kDS; ++g) {
       __builtin_amdgcn_sched_barrier(0);
-      if (s + 4 < kHD) rows(s + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        S = mfma32x2(__uint_as_float(x[(s >> 2) & 1][j]), fa[s + j], S);
-        dP = mfma32x2(__uint_as_float(y[(s >> 2) & 1][j]), fb[s + j], dP);
+      if (g + 1 < 2 * kDS) rows(g + 1);
+      if (g & 1) {
+        if constexpr (kLowInLds) {
+          const sa_bf16x8 B[3] = {fb[g >> 1][0], fb[g >> 1][1], as_bf16x8(low[wave][g >> 1][lane])};
+          dP = mfma_terms(x[1], B, dP);
+        } else {
+          dP = mfma_terms(x[1], fb[g >> 1], dP);
+        }
+      } else {
+        S = mfma_terms(x[0], fa[g >> 1], S);
       }
     }
-    float cols[2][kAcc][kDC];
-    auto columns = [&](int e) __attribute__((always_inline)) {
-      const int r = 8 * (e >> 2) + (e & 3);  // + 4 hh
-#pragma unroll
-      for (int dc = 0; dc < kDC; ++dc) {
-        const lds_u8* q = tile + at_col + r * kRow + 16 * ((8 * dc + (col >> 2)) ^ (swz_f32(r) | (hh << 3)));
-#pragma unroll
-        for (int z = 0; z < kAcc; ++z) cols[e & 1][z][dc] = *reinterpret_cast<lds_f*>(q + z * kMat);
-      }
-    };
-    columns(0);
+    // Elements e: streamed row 8 (e / 4) + 4 hh + e % 4 of the step, own row col.
     float p[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) p[e] = exp2f(fmaf(S[e], a.scale_log2, kKeys ? nl[e] : -lse));
+    for (int e = 0; e < 16; ++e) p[e] = exp2f(fmaf(S[e], a.scale_log2, kKeys ? st_[8 * (e >> 2) + (e & 3)] : -lse));
     if (!kKeys && row0 + kStep > a.L_st) {  // keys past the last one (the statistics see to queries)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (row0 + 8 * (e >> 2) + 4 * hh + (e & 3) >= a.L_st) p[e] = 0.f;
     }
+    // st_b^T P, then st_a^T dS, 16 streamed rows (u) at a time.
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      __builtin_amdgcn_sched_barrier(0);
-      if (e < 15) columns(e + 1);
-      const float ds = kKeys ? p[e] * dP[e] : p[e] * (dP[e] - delta);
+    for (int z = kAcc - 1; z >= 0; --z)
 #pragma unroll
-      for (int dc = 0; dc < kDC; ++dc)
+      for (int u = 0; u < 2; ++u) {
+        sa_u32x4v t[3];
 #pragma unroll
-        for (int z = 0; z < kAcc; ++z) acc[z][dc] = mfma32x2(cols[e & 1][z][dc], z == 0 ? ds : p[e], acc[z][dc]);
-    }
+        for (int j = 0; j < 4; ++j) {
+          const int e = 8 * u + 2 * j;
+          const float v0 = z ? p[e] : p[e] * (kKeys ? dP[e] : dP[e] - delta);
+          const float v1 = z ? p[e + 1] : p[e + 1] * (kKeys ? dP[e + 1] : dP[e + 1] - delta);
+          uint32_t hi, mid, lo;
+          split3(v0, v1, hi, mid, lo);
+          t[0][j] = hi;
+          t[1][j] = mid;
+          t[2][j] = lo;
+        }
+        const sa_bf16x8 B[3] = {as_bf16x8(t[0]), as_bf16x8(t[1]), as_bf16x8(t[2])};
+#pragma unroll
+        for (int dc = 0; dc < kDC; ++dc) {
+          sa_u32x4v A[3];
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            const lds_u8* q = tile + z * kMat + i * kTerm + (dc >> 1) * kRowTile + 2048 * u;
+            const uint2 lo = lds_read_tr16(q + to[dc & 1][0]), hi = lds_read_tr16(q + to[dc & 1][1]);
+            A[i] = sa_u32x4v{lo.x, lo.y, hi.x, hi.y};
+          }
+          acc[z][dc] = mfma_terms(A, B, acc[z][dc]);
+        }
+      }
   };
 
-  lds_u8* const t0 = (lds_u8*)tile0;
-  lds_u8* const t1 = (lds_u8*)tile1;
   int rb = block_of(0);
-  issue(rb, 0, t0, (lds_u8*)stat0);
-  int rb_next = block_of(1);
-  for (int i = 0; i < per_part; i += 2) {  // (as in bsa_bwd_kernel)
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    wg_barrier();
-    issue(rb_next, i + 1, t1, (lds_u8*)stat1);
-    compute(rb, i, t0, stat0);
-    if (i + 1 >= per_part) break;
-    rb = block_of(i + 2);
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    wg_barrier();
-    issue(rb, i + 2, t0, (lds_u8*)stat0);
-    compute(rb_next, i + 1, t1, stat1);
-    rb_next = block_of(i + 3);
+  fetch(rb, 0);
+  for (int i = 0; i < per_part; ++i) {
+    __syncthreads();  // everyone is done with the step before
+    stage(rb);
+    __syncthreads();
+    const int rb_next = block_of(i + 1);
+    fetch(rb_next, i + 1);
+    compute(rb, i);
+    rb = rb_next;
   }
 
   // ---- Results: the parts' sums are added in LDS, in order.
@@ -730,9 +796,10 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
     float* g = static_cast<float*>(x == 0 ? a.grad_a : a.grad_b);
     const int64_t sb = x == 0 ? a.ga_sb : a.gb_sb, sh = x == 0 ? a.ga_sh : a.gb_sh, sl = x == 0 ? a.ga_sl : a.gb_sl;
     const float f = x == 0 ? a.sm_scale : 1.f;
-    static_assert(kBlk * kD * 4 <= kParts * 2 * kMat, "the sums of a part fit a stage");
+    constexpr int kSums = kBlk * kD;
+    static_assert(kParts * kSums * 4 <= kParts * 2 * kMat, "the sums fit the tiles");
     __syncthreads();
-    float* mine = reinterpret_cast<float*>(part ? tile1 : tile0) + (kStep * w + col) * kD;
+    float* mine = reinterpret_cast<float*>(tile_lds) + part * kSums + (kStep * w + col) * kD;
 #pragma unroll
     for (int dc = 0; dc < kDC; ++dc)
 #pragma unroll
@@ -745,8 +812,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
     for (int t = threadIdx.x; t < kBlk * kCh; t += 256) {
       const int r = t / kCh, ch = t % kCh;
       const int at = r * kD + 4 * (ch ^ (r & 31 & (kCh - 1)));
-      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tile0) + at);
-      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tile1) + at);
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tile_lds) + at);
+      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(tile_lds) + kSums + at);
       const float4 s = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
       const int row = blk * kBlk + r;
       if (place >= 0)
@@ -833,9 +900,9 @@ int pairs_per_item(int n_items, int max_cnt, int D) {
 // Splits of each item's list over workgroups of two pairs, where the items leave most of the card idle
 // and their lists (of up to `width` entries) are long: at least 8 entries each. Without / with, us of the
 // query pass of 64 queries and the key pass of 64 keys against 17 776 of the other: one head 93 / 9 and 114 / 10,
-// 30 heads 112 / 27 and 120 / 29; fp32, one head 594 / 36 and 1 076 / 48; [1, 1, 2048, 64], 8 of 32 blocks, 10.3 /
-// 7.0 and 10.9 / 8.0. The merge is 4 to 5 us more: two to five splits gain no more than that (160 items with dense
-// lists of 40: 24.2 / 21.2 and the merge), but in fp32, whose steps take 16 times as long.
+// 30 heads 112 / 27 and 120 / 29; [1, 1, 2048, 64], 8 of 32 blocks, 10.3 / 7.0 and 10.9 / 8.0; fp32 [1, 4, 2000, 64], 0.3 of
+// 32 blocks, in three or four 32.8 / 29.2 and 55.7 / 49.8. The merge is 4 to 5 us more: two to five splits gain no more than that (160 items with dense
+// lists of 40: 24.2 / 21.2 and the merge), but in fp32, whose steps take six times as long.
 int splits_of(int64_t n_items, int width, int D, bool f32) {
   if (width < (f32 ? 16 : 32)) return 1;
   const int64_t slots = f32 ? (D == 64 ? 512 : 256) : (D == 64 ? 768 : 512);  // such workgroups on the card
@@ -861,12 +928,11 @@ struct Deal {
 };
 
 // fp32: the items behind the last full round of an XCD's workgroups are split, by three where lists may be long.
-// Whole / split, us of the query and key pass with the merge: [1, 30, 2560, 64] half the blocks 383 / 349 and 488 /
-// 463, 0.15 of them 151 / 147 and 214 / 210; [1, 12, 2100, 64], less than a round, 159 / 140 and 211 / 190; [1, 10,
-// 3500, 128] 492 / 418 and 638 / 564; of 24 blocks or fewer by two 88 / 86 and 129 / 123 (by three 93, 129); at worst
-// [1, 20, 3333, 128] with a tenth of the blocks 265 / 278 and 403 / 393. 16-bit steps are too short for it: dense
-// lists of 40 gain 171 / 163 and 229 / 227 (by two 159 and 222), the same lists with a fifth of the blocks lose 54 / 61
-// and 87 / 94, and the host does not know which they are.
+// Whole / split, us of the query and key pass with the merge: [1, 30, 2560, 64] half the blocks 262 / 256 and 353 /
+// 330, 0.15 of them 104 / 103 and 153 / 153; [1, 12, 2100, 64], less than a round, 106 / 95 and 142 / 139; [1, 10,
+// 3500, 128] 340 / 289 and 447 / 390, [1, 3, 1700, 128] 80 / 51 and 125 / 81; at worst, by two, [2, 10, 1500, 64] 60 / 60
+// and 86 / 92. 16-bit steps are too short for it: dense lists of 40 gain 171 / 163 and 229 / 227 (by two 159 and 222),
+// the same lists with a fifth of the blocks lose 54 / 61 and 87 / 94, and the host does not know which they are.
 //
 // 16 bits: text items, several times as long as the others, are split by two where they outlast them: up to one
 // round of workgroups over lists of 40 and more, two rounds over 96. Whole / split, us of the query pass, texts of 4

@@ -29,6 +29,15 @@ __device__ inline uint32_t cvt_pk_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, r);
 }
 
+// The three bf16 terms of x0 and x1, packed: each remainder is exact in fp32, and the last one
+// has at most 8 significand bits, so hi + mid + lo = x (above bf16's subnormals).
+__device__ inline void split3(float x0, float x1, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  hi = cvt_pk_bf16(x0, x1);
+  const float a0 = x0 - __uint_as_float(hi << 16), a1 = x1 - __uint_as_float(hi & 0xffff0000u);
+  mid = cvt_pk_bf16(a0, a1);
+  lo = cvt_pk_bf16(a0 - __uint_as_float(mid << 16), a1 - __uint_as_float(mid & 0xffff0000u));
+}
+
 __device__ inline float dot2_bf16_ones(uint32_t pair, float acc) {
   const sa_bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(sa_bf16x2, pair), ones, acc, false);

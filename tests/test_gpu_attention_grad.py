@@ -129,6 +129,21 @@ def test_last_round_by_length(dev, dtype, H, group, L, D):
           norm=1.5 * unit(dtype))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp32_small_and_large_gradients(dev, D):
+    # Powers of two come out of every product: 2^-60 and 2^60 times the gradient give as much of the results, but for
+    # terms 2^-60 of the others.
+    case(f"fp32 gradients far from one D={D}")
+    (q, k, v, do), g = _inputs(20, FP32, 1, 2, 200, 150, D)
+    mask = _mask(g, 1, 2, 200, 150, 0.6).to(dev)
+    q, k, v, do = (t.to(dev) for t in (q, k, v, do))
+    want = _grads(lambda *x: block_sparse_train_fn(*x, mask, 0.125), q, k, v, do)[1:]
+    for f in (2.0 ** -60, 2.0 ** 60):
+        got = _grads(lambda *x: block_sparse_train_fn(*x, mask, 0.125), q, k, v, do * f)[1:]
+        for x, y in zip(got, want):
+            assert torch.allclose(x / f, y, rtol=2.0 ** -22, atol=2.0 ** -22 * y.abs().max().item())
+
+
 # Text blocks whose long lists are split: of the query pass, of the key pass (and more text blocks than a head has
 # blocks), of both, unlike many of them on each XCD.
 @pytest.mark.parametrize("H,Lq,Lk,D,text,bias", [(12, 330, 2700, 64, 4, True), (24, 2700, 200, 128, 9, False),
