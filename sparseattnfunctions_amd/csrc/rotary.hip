@@ -95,17 +95,19 @@ typedef uint32_t Words __attribute__((ext_vector_type(4)));
 // the turned part copy 2 V values, in the same two accesses, so that the lanes of a wave stay together.
 // Loads of kUnroll heads are in flight together.
 //
-// kLines: each store of a wave fills whole lines (interleaved 16-bit values), so that they need not wait
-// in a cache for the rest: they are streamed out. [2, 30, 17776, 64] queries and keys in bf16 take 98 us so
-// (5.6 TB/s, other tensors each time; 91 the same ones), 105 (108) with ordinary stores; halves (107 us, streamed
-// 109) and fp32 halves ([1, 15 + 5, 8229, 128] 42 us, 4.1 TB/s, streamed 42 to 48), whose lines are put together
-// from two stores, keep the ordinary ones.
-template <typename T, bool kHalf, int V>
+// V values are 16 bytes, or fewer where the halves are no multiples of that (fp32 in 32 bytes, two accesses that leave
+// every second 16 to each other: [1, 15 + 5, 8229, 128], 96 of 128 values, halves 42 us, in 16 bytes 35).
+//
+// kStream (a template argument: the choice beside the stores costs 4 %): a run of such stores fills whole lines (128
+// bytes: the row, or its half), so that they need not wait in a cache for the rest and are streamed out. Other tensors
+// each time, ordinary / streamed, us: bf16 interleaved [2, 30 + 30, 17776, 64] 105 / 98 (5.6 TB/s), fp16 halves [1, 16 +
+// 4, 20000, 128] 48 / 41, fp32 [2, 24 + 8, 8000, 64] interleaved 50 / 47 and halves 51 / 47 (5.6 TB/s); halves of 64
+// bytes, [2, 30 + 30, 17776, 64] in bf16, 107 / 109.
+template <typename T, bool kHalf, int V, bool kStream>
 __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
   constexpr int kUnroll = 4;
   constexpr int kPairs = kHalf ? V : V / 2;
   constexpr int kChunks = kHalf ? 2 : 1;
-  constexpr bool kLines = !kHalf && sizeof(T) == 2;
   const int unit = threadIdx.x % a.units;
   const int rest = threadIdx.x / a.units;
   const int slot = rest / a.tokens;
@@ -168,8 +170,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotArgs a) {
           }
         }
         T* p = to(h0 + u * a.slots);
-        if constexpr (kLines) {
+        if constexpr (kStream) {
           __builtin_nontemporal_store(__builtin_bit_cast(Words, x[u][0]), reinterpret_cast<Words*>(p + at0));
+          if constexpr (kHalf)
+            __builtin_nontemporal_store(__builtin_bit_cast(Words, x[u][kChunks - 1]), reinterpret_cast<Words*>(p + at1));
         } else {
           *reinterpret_cast<Chunk<T, V>*>(p + at0) = x[u][0];
           if constexpr (kHalf) *reinterpret_cast<Chunk<T, V>*>(p + at1) = x[u][1];
@@ -210,8 +214,8 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(RotArgs a) {
   }
 }
 
-// Values that a thread moves together: 8, or in halves of fewer multiples 4 or 2 (whole units have to fill
-// the half and the rest of the head, and the rows have to be aligned to them); 1 for anything else.
+// Values that a thread moves together: 16 bytes, or fewer in halves that are no multiples of them (whole units have
+// to fill the half and the rest of the head, and the rows have to be aligned to them); 1 for anything else.
 int width_of(const RotArgs& a, bool half, int size) {
   int64_t strides = a.D;
   uint64_t ptrs = 0;
@@ -219,7 +223,7 @@ int width_of(const RotArgs& a, bool half, int size) {
     for (int i = 0; i < 3; ++i) strides |= a.xs[w][i] | a.ys[w][i];
     ptrs |= reinterpret_cast<uintptr_t>(a.x[w]) | reinterpret_cast<uintptr_t>(a.y[w]);
   }
-  for (int v = 8; v >= (half ? 2 : 8); v /= 2) {
+  for (int v = 16 / size; v >= (half ? 2 : 16 / size); v /= 2) {
     if (half && (a.pairs % v || (a.D - 2 * a.pairs) % (2 * v))) continue;
     if (strides % v == 0 && ptrs % std::min(16, v * size) == 0) return v;
   }
@@ -228,9 +232,11 @@ int width_of(const RotArgs& a, bool half, int size) {
 
 template <typename T>
 int launch_rotary(RotArgs a, bool half, hipStream_t s, const char* fn) {
+  constexpr int kWide = 16 / sizeof(T);
   const int v = width_of(a, half, sizeof(T));
+  const bool stream = (half ? a.pairs : a.D) * sizeof(T) >= 128;
   // units per token, then as many tokens (a power of two up to the length) and head slots as fit 256 threads
-  a.units = v == 1 ? a.D - a.pairs : half ? a.D / (2 * v) : a.D / 8;
+  a.units = v == 1 ? a.D - a.pairs : half ? a.D / (2 * v) : a.D / v;
   const int room = 256 / a.units;
   a.tokens = 1;
   while (2 * a.tokens <= room && a.tokens < a.L) a.tokens *= 2;
@@ -249,11 +255,15 @@ int launch_rotary(RotArgs a, bool half, hipStream_t s, const char* fn) {
     if (half) hipLaunchKernelGGL((rotary_any_kernel<T, true>), grid, blk, 0, s, a);
     else hipLaunchKernelGGL((rotary_any_kernel<T, false>), grid, blk, 0, s, a);
   } else if (!half) {
-    hipLaunchKernelGGL((rotary_kernel<T, false, 8>), grid, blk, 0, s, a);
+    if (stream) hipLaunchKernelGGL((rotary_kernel<T, false, kWide, true>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, false, kWide, false>), grid, blk, 0, s, a);
+  } else if (v == kWide) {
+    if (stream) hipLaunchKernelGGL((rotary_kernel<T, true, kWide, true>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, true, kWide, false>), grid, blk, 0, s, a);
+  } else if (v == 4) {
+    if constexpr (kWide > 4) hipLaunchKernelGGL((rotary_kernel<T, true, 4, false>), grid, blk, 0, s, a);
   } else {
-    if (v == 8) hipLaunchKernelGGL((rotary_kernel<T, true, 8>), grid, blk, 0, s, a);
-    else if (v == 4) hipLaunchKernelGGL((rotary_kernel<T, true, 4>), grid, blk, 0, s, a);
-    else hipLaunchKernelGGL((rotary_kernel<T, true, 2>), grid, blk, 0, s, a);
+    hipLaunchKernelGGL((rotary_kernel<T, true, 2, false>), grid, blk, 0, s, a);
   }
   return sa::check_launch(fn);
 }
