@@ -243,7 +243,7 @@ typedef struct sa_attn_train {
   void *dq, *dk, *dv;  /* each nullable: not computed */
   int64_t strides[24]; /* {b, h, l} in elements of q, k, v, out, dout, dq, dk, dv */
   float* lse;          /* [B*H][64*ceil(Lq/64)]; forward: written; backward: read */
-  const int32_t *kv_idx, *kv_cnt;
+  int32_t *kv_idx, *kv_cnt; /* read; written by a forward call with a mask */
   const float* key_bias; /* nullable; not with fp32 */
   int64_t bias_strides[2];
   const int32_t* fwd_order; /* nullable dispatch order of the forward pass (not read with parts > 1), */
@@ -256,6 +256,8 @@ typedef struct sa_attn_train {
   int64_t workspace_bytes;
   float sm_scale;
   int32_t n_text_blocks;    /* so many first blocks of each head, which the orders put first, have long lists (0: none) */
+  const uint8_t* mask;      /* forward, nullable: kv_idx and kv_cnt are made from it first, as by sa_mask_to_kv_list */
+  int64_t mask_strides[4];  /* with max_cnt entries a row: {b, h, q block, k block} in bytes */
 } sa_attn_train;
 
 /*

@@ -1848,6 +1848,12 @@ extern "C" int sa_block_sparse_fwd_lse(const sa_attn_train* t, void* stream) {
              t->dtype);
   SA_REQUIRE(t->lse, "%s: null lse", fn);
   SA_REQUIRE(t->parts >= 1, "%s: parts=%d must be >= 1", fn, t->parts);
+  if (t->mask) {
+    SA_REQUIRE(t->Lq > 0 && t->Lk > 0, "%s: bad shape Lq=%d Lk=%d", fn, t->Lq, t->Lk);
+    if (int rc = sa_mask_to_kv_list(t->mask, t->mask_strides, t->B, t->H, (int)sa::cdiv(t->Lq, kBlock),
+                                    (int)sa::cdiv(t->Lk, kBlock), t->kv_idx, t->max_cnt, t->kv_cnt, stream))
+      return rc;
+  }
   const int64_t* st = t->strides;
   if (t->dtype == SA_DTYPE_F32) {
     if (t->key_bias || t->parts != 1) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias or key-range parts", fn);

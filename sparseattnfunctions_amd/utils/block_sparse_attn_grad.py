@@ -35,7 +35,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .._kv import KVList, kv_list_from_mask
+from .._kv import KVList
 from .block_sparse_attn_kernel import (BLOCK, cell_kv_list, f32_terms_workspace, shares_text_rows,
                                        split_parts, split_workspace_bytes, work_order)
 
@@ -48,9 +48,28 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _check_inputs(q, k, v, kv: KVList, key_bias, own_lists: bool = False):
-    """key_bias expanded; `own_lists`: the lists were made here for these shapes."""
-    tensors = (q, k, v, kv.idx, kv.cnt) if key_bias is None else (q, k, v, kv.idx, kv.cnt, key_bias)
+class _MaskLists:
+    """The lists of a 64 x 64 block mask, which the forward call makes: one buffer, the counts behind
+    the entries."""
+
+    def __init__(self, mask, B, H, nqb, nkb):
+        if mask.shape[2] < nqb or mask.shape[3] < nkb:
+            raise ValueError(f"block mask {tuple(mask.shape)} smaller than the block grid ({nqb}, {nkb})")
+        if mask.dtype != torch.bool:
+            mask = mask != 0
+        if mask.shape[:2] != (B, H):
+            mask = mask.expand(B, H, -1, -1)
+        self.mask, self.nkb = mask, nkb
+        self.idx = torch.empty(B * H * nqb * (nkb + 1), dtype=torch.int32, device=mask.device)
+        self.cnt = None
+
+
+def _check_inputs(q, k, v, kv, key_bias):
+    """key_bias expanded. kv: a caller's lists, or ones for these shapes (_MaskLists)."""
+    own_lists = type(kv) is _MaskLists
+    tensors = (q, k, v, kv.idx, kv.idx if own_lists else kv.cnt)
+    if key_bias is not None:
+        tensors += (key_bias,)
     _lib.require_gpu(*tensors)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"q, k, v must be [B, H, L, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -95,6 +114,16 @@ def _set(call, **tensors):
         setattr(call, name, t.data_ptr())
         i = 3 * _OPERANDS.index(name)
         call.strides[i:i + 3] = t.stride()[:3]
+
+
+def _set_lists(call, idx, cnt):
+    """cnt None: a _MaskLists' buffer."""
+    call.kv_idx = at = idx.data_ptr()
+    if cnt is None:
+        rows = call.B * call.H * ((call.Lq + BLOCK - 1) // BLOCK)
+        call.kv_cnt = at + 4 * rows * call.max_cnt
+    else:
+        call.kv_cnt = cnt.data_ptr()
 
 
 def _set_bias(call, key_bias):
@@ -142,14 +171,21 @@ class _Plan:
 _plan = functools.lru_cache(maxsize=1024)(_Plan)
 
 
-def _describe(q, k, v, kv: KVList, sm_scale: float, key_bias, n_text_blocks: int):
+def _describe(q, k, v, kv, sm_scale: float, key_bias, n_text_blocks: int):
     """(plan, description) of a call on checked, aligned inputs; key_bias expanded."""
-    row_blocks = kv.row_blocks if kv.row_blocks is not None or kv.dense else 0.0
-    plan = _plan(q.dtype, q.device, q.shape, k.shape[2], q.stride(), k.stride(), v.stride(), kv.idx.shape[1], row_blocks,
+    masked = type(kv) is _MaskLists
+    if masked:
+        max_cnt, row_blocks = kv.nkb, 0.0
+    else:
+        max_cnt, row_blocks = kv.idx.shape[1], kv.row_blocks if kv.row_blocks is not None or kv.dense else 0.0
+    plan = _plan(q.dtype, q.device, q.shape, k.shape[2], q.stride(), k.stride(), v.stride(), max_cnt, row_blocks,
                  key_bias is not None, sm_scale, n_text_blocks)
     args = _lib.AttnTrain.from_buffer_copy(plan.args)
     args.q, args.k, args.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    args.kv_idx, args.kv_cnt = kv.idx.data_ptr(), kv.cnt.data_ptr()
+    _set_lists(args, kv.idx, kv.cnt)
+    if masked:
+        args.mask = kv.mask.data_ptr()
+        args.mask_strides[:] = kv.mask.stride()
     _set_bias(args, key_bias)
     return plan, args
 
@@ -242,6 +278,7 @@ class _TrainAttention(torch.autograd.Function):
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
         ctx.plan, ctx.args = _describe(q, k, v, kv, sm_scale, key_bias, n_text_blocks)
         out, lse = _forward(ctx.plan, ctx.args, q)
+        ctx.args.mask = None  # (read by the forward call alone)
         saved = (q, k, v, out, lse, kv.idx, kv.cnt, key_bias)
         ctx.save_for_backward(*saved)
         ctx.places = [(t.data_ptr(), t.stride()) for t in saved if t is not None]
@@ -259,7 +296,8 @@ class _TrainAttention(torch.autograd.Function):
             q, k, v, out, lse, kv_idx, kv_cnt, key_bias = saved
             q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
             _set(args, q=q, k=k, v=v, out=out)
-            args.lse, args.kv_idx, args.kv_cnt = lse.data_ptr(), kv_idx.data_ptr(), kv_cnt.data_ptr()
+            args.lse = lse.data_ptr()
+            _set_lists(args, kv_idx, kv_cnt)
             _set_bias(args, key_bias)
         return (*_backward(ctx.plan, args, dout, ctx.needs_input_grad[:3]), None, None, None, None)
 
@@ -314,10 +352,10 @@ def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Option
             raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
         return _NoKeys.apply(q, k, v)
     if BLOCK_M == BLOCK and BLOCK_N == BLOCK:
-        kv = kv_list_from_mask(block_sparse_mask, B, H, math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK))
+        kv = _MaskLists(block_sparse_mask, B, H, math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK))
     elif min(BLOCK_M, BLOCK_N) < BLOCK:
         raise NotImplementedError(f"gradients of {BLOCK_M} x {BLOCK_N} blocks: blocks smaller than 64")
     else:
         kv, _ = cell_kv_list(block_sparse_mask, B, H, Lq, Lk, int(BLOCK_M), int(BLOCK_N))
-    key_bias = _check_inputs(q, k, v, kv, key_bias, own_lists=True)
+    key_bias = _check_inputs(q, k, v, kv, key_bias)
     return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
