@@ -273,7 +273,8 @@ int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
  * dq, dk, dv for the gradient dout of out, the probabilities recomputed from lse: P = exp2(score -
  * lse), dS = P * (dout v^T - rowsum(dout * out)), dq = sm_scale dS k, dk = sm_scale dS^T q, dv = P^T
  * dout. Rows and keys in no list get zeros; a block that a row lists twice counts twice. Sums are fp32 in a
- * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type.
+ * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type; fp32 takes its operands in
+ * three bf16 terms (finite ones; those below about 1e-33 lose their low terms).
  *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype, max_cnt and n_text_blocks): the query
  *             rows' statistics, the transposed lists, sums of lists split over workgroups.
  * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv, sm_scale
@@ -312,7 +313,7 @@ int sa_rotary_table(const void* positions, int position_type, const int64_t stri
  * a sin), computed in fp32 and rounded once; the other values are copied. For q [B,H,L,D] and, unless
  * NULL, k [B,Hk,L,D] in one launch. out may be x itself; otherwise they must not overlap.
  *   strides   4 triples {b, h, l} in elements: q, q_out, k, k_out; the D axis is contiguous. D up to
- *             256; 16-byte aligned rows and multiples of 8 pairs (4 interleaved) take wide accesses.
+ *             256; aligned rows, and halves, of whole 16 bytes take wide accesses.
  *   table     [n_rows][pairs][2].
  *   rows      nullable int32 [B or 1][L]: table row of token t of sequence b at rows[b *
  *             rows_batch_stride + t]; a token whose entry lies outside [0, n_rows) is copied.

@@ -913,6 +913,7 @@ int splits_of(int64_t n_items, int width, int D, bool f32) {
 
 // The most text items of an XCD (its items are a contiguous eighth, the first n_text of each n_own text).
 int text_slots(int64_t n_items, int n_own, int n_text) {
+  n_text = std::min(n_text, n_own);
   auto before = [&](int64_t it) { return it / n_own * n_text + std::min<int64_t>(it % n_own, n_text); };
   int64_t most = 0;
   for (int x = 0; x < 8; ++x) most = std::max(most, before(n_items * (x + 1) / 8) - before(n_items * x / 8));

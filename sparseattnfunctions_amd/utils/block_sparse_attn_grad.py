@@ -15,10 +15,12 @@ does as well. Training code calls this module instead:
 The forward pass is the kernel of `block_sparse_attention` with bf16 (fp16) scores, or fp32 on split
 operands, and also stores each row's log2-sum-exp2; the backward pass recomputes the probabilities
 from it, block by block, and keeps nothing of the size of the attention map (`sa_block_sparse_bwd`).
-Gradients of a 16-bit call round P and dS to its type, sums are fp32 in a fixed order, so that a step
-repeats bit for bit. In fp16, dS has the range of the type: scale the loss as usual. A query row
-without a key (an empty list, or keys all biased to -inf) has a zero output and zero gradients; a key
-block in no list has zero gradients. The mask, the lists and key_bias are not differentiated.
+Gradients of a 16-bit call round P and dS to its type, those of an fp32 call take finite operands as
+three exact bf16 terms (values below about 1e-33 lose their low ones); sums are fp32 in a fixed order,
+so that a step repeats bit for bit. In fp16, dS has the range of the type: scale the loss as usual. A
+query row without a key (an empty list, or keys all biased to -inf) has a zero output and zero
+gradients; a key block in no list has zero gradients. The mask, the lists and key_bias are not
+differentiated.
 
 A key_bias below -2.35e38 (the type's lowest value among them) counts as -inf, and keys that it masks
 still enter the products: their k and v have to be finite, as with any additive mask. Keys in blocks
