@@ -353,6 +353,21 @@ def test_larger_blocks(dev, block_m, block_n):
     check(got, reference(q, k, v, do, None, 0.125, allowed=allowed))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+def test_offsets_past_32_bits(dev, dtype):
+    # Batches 2^31 values apart.
+    case(f"far batches {dtype}")
+    (q, k, v, do), g = _inputs(21, dtype, 2, 2, 100, 100, 64)
+    mask = _mask(g, 2, 2, 100, 100, 0.7).to(dev)
+    tensors = [t.to(dev) for t in (q, k, v, do)]
+    fn = lambda *x: block_sparse_train_fn(*x, mask, 0.125)
+    want = _grads(fn, *tensors)
+    n = 2 * 100 * 64
+    base = torch.empty(2 ** 31 + 4 * n, dtype=dtype, device=dev)
+    far = [base.as_strided((2, 2, 100, 64), (2 ** 31, 6400, 64, 1), i * n).copy_(t) for i, t in enumerate(tensors)]
+    assert all(torch.equal(x, y) for x, y in zip(_grads(fn, *far), want))
+
+
 def test_differences(dev):
     # <grad, step> against the loss on both sides of it: fp32, steps of 2^-9, whose third-order term and
     # rounding (2^-24 of the loss's terms over the step) are below 1e-3 of the change.

@@ -271,6 +271,21 @@ def test_with_and_without_autograd(dev):
             apply_rotary(q, dual, table)
 
 
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_offsets_past_32_bits(dev, layout):
+    # Batches 2^31 values apart, in wide accesses and one by one (20 turned values in halves); in place too.
+    case(f"rotary far batches {layout}")
+    base = torch.empty(2 ** 31 + 2 * 3840, dtype=torch.bfloat16, device=dev)
+    for dims in (64, 20):
+        table = rotary_table(torch.arange(20, device=dev), dims)
+        q, k = torch.randn(2, 2, 3, 20, 64, device=dev).bfloat16()
+        want = apply_rotary(q, k, table, layout=layout)
+        far = [base.as_strided((2, 3, 20, 64), (2 ** 31, 1280, 64, 1), i * 3840).copy_(t) for i, t in enumerate((q, k))]
+        assert all(torch.equal(x, y) for x, y in zip(apply_rotary(*far, table, layout=layout), want))
+        apply_rotary_(*far, table, layout=layout)
+        assert all(torch.equal(x, y) for x, y in zip(far, want))
+
+
 def test_no_tokens_or_heads(dev):
     case("rotary empty")
     table = rotary_table(torch.arange(4, device=dev), 64)
