@@ -532,7 +532,7 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
 // dim 64).
 //
 // Bound: the matrix core, beside the splits (11 VALU operations a pair of values) and exp2. [1, 30, 2560, 64] with
-// half the blocks: query pass 256 us, key pass with its lists 325 (150 and 160 TFLOP/s of fp32 products, six times
+// half the blocks: query pass 255 us, key pass with its lists 325 (150 and 160 TFLOP/s of fp32 products, six times
 // that in bf16 ones; on the fp32 matrix instructions 365 and 459); [1, 10, 3500, 128] with 0.4 of them 289 and 390
 // (410 and 555). Values have to be finite; those below about 1e-33, as of gradients of a loss scaled down so far, lose
 // their low terms.
@@ -708,10 +708,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
     if (cur < 0 || row0 >= a.L_st) return;
     sa_f32x16 S = {}, dP = {};
     const float* st_ = stat + part * 64 + 4 * hh;
-    if constexpr (kKeys) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) dP[e] = st_[32 + 8 * (e >> 2) + (e & 3)];
-    }
+    for (int e = 0; e < 16; ++e) dP[e] = kKeys ? st_[32 + 8 * (e >> 2) + (e & 3)] : -delta;
     // Operands of st_a and st_b in turn, each requested before the products of the one before it.
     sa_u32x4v x[2][3];
     auto rows = [&](int g) __attribute__((always_inline)) {
@@ -739,7 +737,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
     // Elements e: streamed row 8 (e / 4) + 4 hh + e % 4 of the step, own row col.
     float p[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) p[e] = exp2f(fmaf(S[e], a.scale_log2, kKeys ? st_[8 * (e >> 2) + (e & 3)] : -lse));
+    for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(S[e], a.scale_log2, kKeys ? st_[8 * (e >> 2) + (e & 3)] : -lse));
     if (!kKeys && row0 + kStep > a.L_st) {  // keys past the last one (the statistics see to queries)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -754,8 +752,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int e = 8 * u + 2 * j;
-          const float v0 = z ? p[e] : p[e] * (kKeys ? dP[e] : dP[e] - delta);
-          const float v1 = z ? p[e + 1] : p[e + 1] * (kKeys ? dP[e + 1] : dP[e + 1] - delta);
+          const float v0 = z ? p[e] : p[e] * dP[e];
+          const float v1 = z ? p[e + 1] : p[e + 1] * dP[e + 1];
           uint32_t hi, mid, lo;
           split3(v0, v1, hi, mid, lo);
           t[0][j] = hi;
