@@ -27,10 +27,10 @@
 //
 // Bound: the issue of MFMA and VALU, as in the forward pass. [2, 30, 2560, 64] bf16 with every block: query pass
 // 177 us (850 TFLOP/s of its three products), key pass 229 us (880 of its four); there the matrix cores work 51 % of
-// the cycles at 1.85 GHz under the power limit, the VALU 42 %, LDS 40 % without bank conflicts, and 85 % of the CU
-// time has a workgroup. [1, 15, 8229, 128] fp16 with 0.35 of the blocks: 327 and 418 us (835, 870), the
-// matrix cores 49 %, CUs 79 %: lists of unlike lengths over two rounds. Of four parts, wave priorities over
-// the two product phases, and splits of the last round nothing was faster (see deal).
+// the cycles at 1.85 GHz under the power limit, the VALU 43 %, LDS 40 % without bank conflicts, and 85 % of the CU
+// time has a workgroup. [1, 15, 8229, 128] fp16 with 0.35 of the blocks: 309 and 392 us (885, 930), the matrix cores 55
+// %, CUs 87 %; with every block 1 050. Of four parts, wave priorities over the two product phases, and splits of the last
+// round nothing was faster (see deal).
 #include <math.h>
 
 #include <algorithm>
@@ -532,10 +532,10 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
 // dim 64).
 //
 // Bound: the matrix core, beside the splits (11 VALU operations a pair of values) and exp2. [1, 30, 2560, 64] with
-// half the blocks: query pass 255 us, key pass with its lists 325 (150 and 160 TFLOP/s of fp32 products, six times
-// that in bf16 ones; on the fp32 matrix instructions 365 and 459); [1, 10, 3500, 128] with 0.4 of them 289 and 390
-// (410 and 555). Values have to be finite; those below about 1e-33, as of gradients of a loss scaled down so far, lose
-// their low terms.
+// half the blocks: query pass 236 us, key pass 297 (162 and 171 TFLOP/s of fp32 products, six times that in bf16 ones, the
+// matrix cores 45 and 48 % of the cycles); with merges and lists 250 and 320, on the fp32 matrix instructions 365 and
+// 459. [1, 10, 3500, 128] with 0.4 of them 288 and 388 (410 and 555). Values have to be finite; those below about
+// 1e-33, as of gradients of a loss scaled down so far, lose their low terms.
 
 // The six term products of A and B onto c.
 __device__ inline sa_f32x16 mfma_terms(const sa_u32x4v (&A)[3], const sa_bf16x8 (&B)[3], sa_f32x16 c) {
