@@ -1,6 +1,8 @@
-"""Rotary frequencies and what `sa_rotary_*` and `sa_block_sparse_bwd` refuse, without a GPU."""
+"""The training calls' struct, rotary frequencies and what `sa_rotary_*` and `sa_block_sparse_bwd` refuse, without a GPU."""
 import ctypes
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -119,7 +121,8 @@ def test_c_argument_checks():
 
     assert lib.sa_block_sparse_fwd_lse(None, None) == _lib.SA_ERR_INVALID
     for bad in (dict(dtype=7), dict(lse=None), dict(parts=0), dict(parts=2, workspace=None), dict(out=None), dict(sm_scale=-1.0),
-                dict(dtype=2, workspace_bytes=10), dict(Lk=0)):
+                dict(dtype=2, workspace_bytes=10), dict(Lk=0), dict(mask=256, Lq=0), dict(mask=256, kv_idx=None),
+                dict(mask=256, kv_cnt=None), dict(mask=256, Lk=64 * 100, max_cnt=99)):
         assert lse(**bad) == _lib.SA_ERR_INVALID, bad
     for bad in (dict(dtype=2, key_bias=256), dict(dtype=2, parts=2), dict(key_bias=256, parts=2), dict(D=80),
                 dict(stride=[0, 0, 66] * 8)):
@@ -132,3 +135,17 @@ def test_c_argument_checks():
         assert transpose(**bad) == _lib.SA_ERR_INVALID, bad
     for bad in (dict(cnt=65536), dict(nqb=1 << 20, cnt=1 << 12)):
         assert transpose(**bad) == _lib.SA_ERR_UNSUPPORTED, bad
+
+
+def test_struct_layout(tmp_path):
+    # The binding's fields lie where the header's do.
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    names = [f[0] for f in _lib.AttnTrain._fields_]
+    prints = "".join(f'printf("%zu\\n", offsetof(sa_attn_train, {n}));' for n in names)
+    source = tmp_path / "layout.c"
+    source.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "sa_api.h"\n'
+                      f'int main() {{ {prints} printf("%zu\\n", sizeof(sa_attn_train)); return 0; }}\n')
+    subprocess.run(["gcc", f"-I{include}", str(source), "-o", str(tmp_path / "layout")], check=True)
+    out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout
+    want = [getattr(_lib.AttnTrain, n).offset for n in names] + [ctypes.sizeof(_lib.AttnTrain)]
+    assert [int(x) for x in out.split()] == want
