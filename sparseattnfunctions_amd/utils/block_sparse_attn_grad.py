@@ -51,8 +51,8 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
 
 class _MaskLists:
-    """The lists of a 64 x 64 block mask, which the forward call makes: one buffer, the counts behind
-    the entries."""
+    """The lists of a 64 x 64 block mask, which the forward call makes, and room for the rows'
+    log2-sum-exp2: one buffer of entries, counts, sums."""
 
     def __init__(self, mask, B, H, nqb, nkb):
         if mask.shape[2] < nqb or mask.shape[3] < nkb:
@@ -62,17 +62,23 @@ class _MaskLists:
         if mask.shape[:2] != (B, H):
             mask = mask.expand(B, H, -1, -1)
         self.mask, self.nkb = mask, nkb
-        self.idx = torch.empty(B * H * nqb * (nkb + 1), dtype=torch.int32, device=mask.device)
+        self.idx = mask.new_empty(B * H * nqb * (nkb + 1 + BLOCK), dtype=torch.int32)
         self.cnt = None
 
 
 def _check_inputs(q, k, v, kv, key_bias):
     """key_bias expanded. kv: a caller's lists, or ones for these shapes (_MaskLists)."""
     own_lists = type(kv) is _MaskLists
-    tensors = (q, k, v, kv.idx, kv.idx if own_lists else kv.cnt)
+    tensors = (k, v, kv.idx) if own_lists else (k, v, kv.idx, kv.cnt)
     if key_bias is not None:
         tensors += (key_bias,)
-    _lib.require_gpu(*tensors)
+    device = q.device
+    if device.type != "cuda":
+        _lib.require_gpu(q)
+    for t in tensors:
+        if t.device != device:
+            _lib.require_gpu(*tensors)
+            raise ValueError("q, k, v, the lists and key_bias must be on one device")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"q, k, v must be [B, H, L, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q.dtype not in _lib.DTYPES or not q.dtype == k.dtype == v.dtype:
@@ -83,10 +89,6 @@ def _check_inputs(q, k, v, kv, key_bias):
         raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
     if D not in (64, 128):
         raise NotImplementedError(f"head_dim {D} (64 or 128)")
-    device = q.device
-    for t in tensors:
-        if t.device != device:
-            raise ValueError("q, k, v, the lists and key_bias must be on one device")
     nqb, nkb = (Lq + BLOCK - 1) // BLOCK, (Lk + BLOCK - 1) // BLOCK
     if own_lists:
         pass
@@ -118,14 +120,16 @@ def _set(call, **tensors):
         call.strides[i:i + 3] = t.stride()[:3]
 
 
-def _set_lists(call, idx, cnt):
-    """cnt None: a _MaskLists' buffer."""
+def _set_lists(call, plan, idx, cnt, lse=None):
+    """cnt None: a _MaskLists' buffer, which has the lse too."""
     call.kv_idx = at = idx.data_ptr()
     if cnt is None:
-        rows = call.B * call.H * ((call.Lq + BLOCK - 1) // BLOCK)
-        call.kv_cnt = at + 4 * rows * call.max_cnt
+        call.kv_cnt = at = at + 4 * plan.rows * call.max_cnt
+        call.lse = at + 4 * plan.rows
     else:
         call.kv_cnt = cnt.data_ptr()
+        if lse is not None:
+            call.lse = lse.data_ptr()
 
 
 def _set_bias(call, key_bias):
@@ -145,10 +149,12 @@ class _Plan:
         n_items = B * H * nqb
         args = self.args = _lib.AttnTrain(dtype=_lib.DTYPES[dtype], B=B, H=H, Lq=Lq, Lk=Lk, D=D, max_cnt=max_cnt, parts=1,
                                           sm_scale=sm_scale, n_text_blocks=n_text_blocks)
-        self.out, self.lse = (B, H, Lq, D), (B, H, nqb * BLOCK)
+        self.out, self.lse, self.rows = (B, H, Lq, D), (B, H, nqb * BLOCK), n_items
         self.grads = (B, H, Lq, D), (B, H, Lk, D), (B, H, Lk, D)
         sq, sk = (H * Lq * D, Lq * D, D), (H * Lk * D, Lk * D, D)
-        args.strides[:] = (*q_strides[:3], *k_strides[:3], *v_strides[:3], *sq, 0, 0, 0, *sq, *sk, *sk)
+        self.square = Lq == Lk  # dk and dv are like dout
+        self.plain_q = tuple(q_strides) == (*sq, 1)
+        args.strides[:] = (*q_strides[:3], *k_strides[:3], *v_strides[:3], *sq, *sq, *sq, *sk, *sk)
         # The forward pass takes block_sparse_attention's launch variants: key-range parts for few blocks
         # over long lists, else a work order. fp32 takes split operands for few query blocks too: 30 heads of one
         # block over 1, 4, 8 and 63 blocks 16.6 / 17.6, 46 / 18, 87 / 25 and 697 / 102 us without / with.
@@ -184,7 +190,7 @@ def _describe(q, k, v, kv, sm_scale: float, key_bias, n_text_blocks: int):
                  key_bias is not None, sm_scale, n_text_blocks)
     args = _lib.AttnTrain.from_buffer_copy(plan.args)
     args.q, args.k, args.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    _set_lists(args, kv.idx, kv.cnt)
+    _set_lists(args, plan, kv.idx, kv.cnt)
     if masked:
         args.mask = kv.mask.data_ptr()
         args.mask_strides[:] = kv.mask.stride()
@@ -193,17 +199,21 @@ def _describe(q, k, v, kv, sm_scale: float, key_bias, n_text_blocks: int):
 
 
 def _forward(plan: _Plan, args: _lib.AttnTrain, q):
-    """(out, lse) of a call, whose description then has them."""
+    """(out, lse) of a call, whose description then has them; lse None where it has room for it."""
     device = q.device
-    out = torch.empty(plan.out, dtype=q.dtype, device=device)
-    lse = torch.empty(plan.lse, dtype=torch.float32, device=device)
+    # (empty_like is the cheaper call: 1.1 us on the host, empty 2.1)
+    out = torch.empty_like(q) if plan.plain_q else torch.empty(plan.out, dtype=q.dtype, device=device)
+    lse = None
+    if not args.lse:
+        lse = torch.empty(plan.lse, dtype=torch.float32, device=device)
+        args.lse = lse.data_ptr()
     ws = None
     if plan.terms:
         ws = f32_terms_workspace(args.B, args.H, args.Lk, args.D, device)
     elif plan.forward_bytes:
         ws = torch.empty(plan.forward_bytes, dtype=torch.uint8, device=device)
     args.workspace, args.workspace_bytes = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
-    args.out, args.lse = out.data_ptr(), lse.data_ptr()
+    args.out = out.data_ptr()
     with _lib.on(device):
         rc = _lib.load().sa_block_sparse_fwd_lse(args, _lib.stream_of(q))
     _lib.check(rc, "sa_block_sparse_fwd_lse")
@@ -211,19 +221,30 @@ def _forward(plan: _Plan, args: _lib.AttnTrain, q):
 
 
 def _backward(plan: _Plan, args: _lib.AttnTrain, dout, needs):
-    """[dq, dk, dv], None where not needed; args describes the call with its operands, out and lse."""
-    dout = _rows16(dout)
-    device = dout.device
+    """(dq, dk, dv), None where not needed; args describes the call with its operands, out and lse."""
+    plain = dout.is_contiguous() and dout.data_ptr() % 16 == 0
+    if not plain:
+        dout = _rows16(dout)
+        args.strides[12:15] = dout.stride()[:3]
     args.dout = dout.data_ptr()
-    args.strides[12:15] = dout.stride()[:3]
-    grads = [torch.empty(shape, dtype=dout.dtype, device=device) if n else None for n, shape in zip(needs, plan.grads)]
-    args.dq, args.dk, args.dv = (t.data_ptr() if t is not None else None for t in grads)
-    ws = torch.empty(plan.backward_bytes, dtype=torch.uint8, device=device)
+    device = dout.device
+    dq = dk = dv = None
+    if needs[0]:
+        dq = torch.empty_like(dout) if plain else dout.new_empty(plan.grads[0])
+        args.dq = dq.data_ptr()
+    plain = plain and plan.square
+    if needs[1]:
+        dk = torch.empty_like(dout) if plain else dout.new_empty(plan.grads[1])
+        args.dk = dk.data_ptr()
+    if needs[2]:
+        dv = torch.empty_like(dout) if plain else dout.new_empty(plan.grads[2])
+        args.dv = dv.data_ptr()
+    ws = dout.new_empty(plan.backward_bytes, dtype=torch.uint8)
     args.workspace, args.workspace_bytes = ws.data_ptr(), plan.backward_bytes
     with _lib.on(device):
         rc = _lib.load().sa_block_sparse_bwd(args, _lib.stream_of(dout))
     _lib.check(rc, "sa_block_sparse_bwd")
-    return grads
+    return dq, dk, dv
 
 
 def transpose_kv_list(kv: KVList) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -271,7 +292,16 @@ def block_sparse_attention_backward(dout, q, k, v, out, lse, kv: KVList, sm_scal
         plan, args = _describe(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
         _set(args, out=out)
         args.lse = lse.data_ptr()
-        return tuple(_backward(plan, args, dout, needs))
+        return _backward(plan, args, dout, needs)
+
+
+def _places(q, k, v, out, kv_idx, kv_cnt, lse, key_bias):
+    """Where a call's saved tensors lie (lists and sums are contiguous)."""
+    at = (q.data_ptr(), q.stride(), k.data_ptr(), k.stride(), v.data_ptr(), v.stride(), out.data_ptr(), out.stride(),
+          kv_idx.data_ptr())
+    if kv_cnt is not None:
+        at += (kv_cnt.data_ptr(), lse.data_ptr())
+    return at if key_bias is None else at + (key_bias.data_ptr(), key_bias.stride())
 
 
 class _TrainAttention(torch.autograd.Function):
@@ -281,9 +311,8 @@ class _TrainAttention(torch.autograd.Function):
         ctx.plan, ctx.args = _describe(q, k, v, kv, sm_scale, key_bias, n_text_blocks)
         out, lse = _forward(ctx.plan, ctx.args, q)
         ctx.args.mask = None  # (read by the forward call alone)
-        saved = (q, k, v, out, lse, kv.idx, kv.cnt, key_bias)
-        ctx.save_for_backward(*saved)
-        ctx.places = [(t.data_ptr(), t.stride()) for t in saved if t is not None]
+        ctx.save_for_backward(q, k, v, out, kv.idx, kv.cnt, lse, key_bias)
+        ctx.places = _places(q, k, v, out, kv.idx, kv.cnt, lse, key_bias)
         return out
 
     @staticmethod
@@ -293,15 +322,14 @@ class _TrainAttention(torch.autograd.Function):
         saved = ctx.saved_tensors
         # A copy of the forward pass's description: this may run twice, or in two threads.
         args = _lib.AttnTrain.from_buffer_copy(ctx.args)
-        if ctx.places != [(t.data_ptr(), t.stride()) for t in saved if t is not None]:
+        if ctx.places != _places(*saved):
             # Hooks on saved tensors have moved them.
-            q, k, v, out, lse, kv_idx, kv_cnt, key_bias = saved
+            q, k, v, out, kv_idx, kv_cnt, lse, key_bias = saved
             q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
             _set(args, q=q, k=k, v=v, out=out)
-            args.lse = lse.data_ptr()
-            _set_lists(args, kv_idx, kv_cnt)
+            _set_lists(args, ctx.plan, kv_idx, kv_cnt, lse)
             _set_bias(args, key_bias)
-        return (*_backward(ctx.plan, args, dout, ctx.needs_input_grad[:3]), None, None, None, None)
+        return (*_backward(ctx.plan, args, dout, ctx.needs_input_grad), None, None, None, None)
 
 
 class _NoKeys(torch.autograd.Function):
@@ -342,12 +370,12 @@ def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Option
     differentiable in q, k and v. BLOCK_M and BLOCK_N are powers of two from 64 to 1024, as of
     `sparse_attention_factory`; smaller blocks have no gradients (NotImplementedError). See
     `block_sparse_attention_train`."""
-    _lib.require_gpu(q, k, v, block_sparse_mask)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4 or block_sparse_mask.dim() != 4:
         raise ValueError("q, k, v and the block mask must be 4-D")
     B, H, Lq, D = q.shape
     Lk = k.shape[2]
     if B * H * Lq == 0 or Lk == 0:
+        _lib.require_gpu(q, k, v, block_sparse_mask)
         if q.dtype not in _lib.DTYPES or not q.dtype == k.dtype == v.dtype:
             raise TypeError(f"q, k, v must share one of bf16, fp16 and fp32, got {q.dtype}, {k.dtype}, {v.dtype}")
         if k.shape != (B, H, Lk, D) or v.shape != (B, H, Lk, D):
@@ -358,6 +386,7 @@ def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Option
     elif min(BLOCK_M, BLOCK_N) < BLOCK:
         raise NotImplementedError(f"gradients of {BLOCK_M} x {BLOCK_N} blocks: blocks smaller than 64")
     else:
+        _lib.require_gpu(q, k, v, block_sparse_mask)
         kv, _ = cell_kv_list(block_sparse_mask, B, H, Lq, Lk, int(BLOCK_M), int(BLOCK_N))
     key_bias = _check_inputs(q, k, v, kv, key_bias)
     return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
