@@ -178,15 +178,18 @@ class VideoRotary:
 
 
 def _check(q, k, table, layout, skip, rows):
-    xs = [x for x in (q, k) if x is not None]
-    _lib.require_gpu(table, rows, *xs)
+    device, dtype = q.device, q.dtype
+    if device.type != "cuda" or table.device != device or (k is not None and k.device != device) \
+            or (rows is not None and rows.device != device):
+        _lib.require_gpu(table, rows, q, k)
+        raise ValueError("q, k, table and rows must be on one device")
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
-    for x in xs:
-        if x.dim() != 4:
-            raise ValueError(f"q and k must be [B, H, L, D], got {tuple(x.shape)}")
-        if x.dtype not in _lib.DTYPES or x.dtype != q.dtype:
-            raise TypeError(f"q and k must share one of bf16, fp16 and fp32, got {', '.join(str(y.dtype) for y in xs)}")
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError(f"q and k must be [B, H, L, D], got {', '.join(str(tuple(x.shape)) for x in (q, k) if x is not None)}")
+    if dtype not in _lib.DTYPES or (k is not None and k.dtype != dtype):
+        raise TypeError("q and k must share one of bf16, fp16 and fp32, got "
+                        + ", ".join(str(x.dtype) for x in (q, k) if x is not None))
     B, _, L, D = q.shape
     if k is not None and (k.shape[0], *k.shape[2:]) != (B, L, D):
         raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)}")
@@ -194,8 +197,6 @@ def _check(q, k, table, layout, skip, rows):
         raise ValueError("table must be a contiguous fp32 [rows, pairs, 2] tensor (rotary_table)")
     if table.requires_grad:
         raise ValueError("table is not differentiated; pass table.detach()")
-    if any(x is not None and x.device != q.device for x in (k, table, rows)):
-        raise ValueError("q, k, table and rows must be on one device")
     if not 0 < 2 * table.shape[1] <= D or D > 2 * MAX_PAIRS:
         raise ValueError(f"a table of {table.shape[1]} pairs for head dim {D} (at most {2 * MAX_PAIRS})")
     if not 0 <= skip <= L:
@@ -214,11 +215,13 @@ def _launch(q, q_out, k, k_out, table, layout, skip, rows, inverse):
     B, H, L, D = q.shape
     if B * H * L == 0 or table.shape[0] == 0 or (k is not None and k.shape[1] == 0):
         raise ValueError(f"nothing to turn: q{tuple(q.shape)}, a table of {table.shape[0]} rows")
-    strides = [*q.stride()[:3], *q_out.stride()[:3]]
-    strides += [*k.stride()[:3], *k_out.stride()[:3]] if k is not None else [0] * 6
+    if k is not None:
+        strides = _lib.i64(*q.stride()[:3], *q_out.stride()[:3], *k.stride()[:3], *k_out.stride()[:3])
+    else:
+        strides = _lib.i64(*q.stride()[:3], *q_out.stride()[:3], 0, 0, 0, 0, 0, 0)
     with _lib.on(q.device):
         rc = _lib.load().sa_rotary_apply(
-            _lib.DTYPES[q.dtype], q.data_ptr(), q_out.data_ptr(), _lib.ptr(k), _lib.ptr(k_out), _lib.i64(*strides), B, H,
+            _lib.DTYPES[q.dtype], q.data_ptr(), q_out.data_ptr(), _lib.ptr(k), _lib.ptr(k_out), strides, B, H,
             k.shape[1] if k is not None else 0, L, D, table.data_ptr(), table.shape[0], table.shape[1], _lib.ptr(rows),
             rows.stride(0) if rows is not None and rows.dim() == 2 else 0, int(skip), int(layout == "half"),
             int(inverse), _lib.stream_of(q))
