@@ -258,6 +258,9 @@ typedef struct sa_attn_train {
   int32_t n_text_blocks;    /* so many first blocks of each head, which the orders put first, have long lists (0: none) */
   const uint8_t* mask;      /* forward, nullable: kv_idx and kv_cnt are made from it first, as by sa_mask_to_kv_list */
   int64_t mask_strides[4];  /* with max_cnt entries a row: {b, h, q block, k block} in bytes */
+  int32_t *q_idx, *q_cnt;   /* nullable: [B*H*ceil(Lk/64)][ceil(Lq/64)] and their counts, the query blocks that list each */
+                            /* key block: written by a forward call with a mask, read by a backward call for dk and dv, */
+                            /* which else makes them itself */
 } sa_attn_train;
 
 /*
@@ -275,10 +278,10 @@ int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
  * dout. Rows and keys in no list get zeros; a block that a row lists twice counts twice. Sums are fp32 in a
  * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type; fp32 takes its operands in
  * three bf16 terms (finite ones; those below about 1e-33 lose their low terms).
- *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype, max_cnt and n_text_blocks): the query
- *             rows' statistics, the transposed lists, sums of lists split over workgroups.
- * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv, sm_scale
- * at least 1e-30.
+ *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype, max_cnt, n_text_blocks and whether there
+ *             is a q_idx): the query rows' statistics, the transposed lists, sums of lists split over workgroups.
+ * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv and no q_idx,
+ * sm_scale at least 1e-30.
  */
 int sa_block_sparse_bwd_workspace(const sa_attn_train* call, int64_t* bytes);
 int sa_block_sparse_bwd(const sa_attn_train* call, void* stream);

@@ -66,11 +66,11 @@ struct BwdArgs {
   int n_items;                      // B * H * n_own
   const int32_t* order;             // dispatch slot -> item, -1 = idle; may be null
   int n_slots;
-  // Query pass: item's entries idx[item * max_cnt ..], cnt[item] of them (clamped). Key pass: entries
-  // idx[bh * n_st * max_cnt + beg[bh * (n_own + 1) + block] ..] up to the next block's.
+  // Item's entries idx[item * max_cnt ..], cnt[item] of them (clamped). Key pass over transposed lists (packed):
+  // entries idx[bh * n_st * max_cnt + cnt[bh * (n_own + 1) + block] ..] up to the next block's.
   const int32_t* idx;
   const int32_t* cnt;
-  int max_cnt;
+  int max_cnt, packed;
   const float* bias;  // [b * bias_sb + h * bias_sh + key]
   int64_t bias_sb, bias_sh;
   float sm_scale;
@@ -112,7 +112,7 @@ __device__ inline int slot_item(const BwdArgs& a, int xcd, int seq) {
 // Entries of an item's list.
 template <bool kKeys>
 __device__ inline int list_length(const BwdArgs& a, int item) {
-  if (!kKeys) return min(max(a.cnt[item], 0), a.max_cnt);
+  if (!kKeys || !a.packed) return min(max(a.cnt[item], 0), a.max_cnt);
   const int bh = item / a.n_own;
   const int32_t* beg = a.cnt + item + bh;  // bh * (n_own + 1) + block
   return beg[1] - beg[0];
@@ -184,7 +184,7 @@ template <bool kKeys>
 __device__ inline const __attribute__((address_space(4))) int32_t* bwd_list(const BwdArgs& a, int item, int bh,
                                                                               int blk, int& n) {
   const int32_t* p;
-  if (kKeys) {
+  if (kKeys && a.packed) {
     const int32_t* beg = a.cnt + (int64_t)bh * (a.n_own + 1) + blk;
     p = a.idx + (int64_t)bh * a.n_st * a.max_cnt + beg[0];
     n = beg[1] - beg[0];
@@ -1008,8 +1008,8 @@ Layout layout(const sa_attn_train& t) {
   const bool f32 = t.dtype == SA_DTYPE_F32;
   Layout l;
   l.q_beg = align256(BH * nqb * 128 * (int64_t)sizeof(float));
-  l.q_idx = l.q_beg + align256(BH * (nkb + 1) * (int64_t)sizeof(int32_t));
-  l.partial = l.q_idx + align256(BH * nqb * t.max_cnt * (int64_t)sizeof(int32_t));
+  l.q_idx = l.q_beg + (t.q_idx ? 0 : align256(BH * (nkb + 1) * (int64_t)sizeof(int32_t)));
+  l.partial = l.q_idx + (t.q_idx ? 0 : align256(BH * nqb * t.max_cnt * (int64_t)sizeof(int32_t)));
   // (a list is no longer than the other side has blocks, but for repeated entries)
   l.q = deal(BH * nqb, (int)nqb, t.n_text_blocks, (int)std::min<int64_t>(t.max_cnt, nkb), t.D, f32);
   l.k = deal(BH * nkb, (int)nkb, t.n_text_blocks, (int)nqb, t.D, f32);
@@ -1045,7 +1045,8 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   const char* fn = "sa_block_sparse_bwd";
   if (int rc = check_train(t, fn)) return rc;
   const int B = t->B, H = t->H, Lq = t->Lq, Lk = t->Lk, D = t->D;
-  SA_REQUIRE(t->q && t->k && t->v && t->out && t->dout && t->lse && t->kv_idx && t->kv_cnt, "%s: null pointer", fn);
+  SA_REQUIRE(t->q && t->k && t->v && t->out && t->dout && t->lse && t->kv_idx && t->kv_cnt && !t->q_idx == !t->q_cnt,
+             "%s: null pointer", fn);
   SA_REQUIRE(std::isfinite(t->sm_scale) && t->sm_scale > 0.f, "%s: sm_scale must be finite and > 0", fn);
   // (the key pass takes the rows' sums in units of the scores, lse / sm_scale)
   if (t->sm_scale < 1e-30f) return sa::fail(SA_ERR_UNSUPPORTED, "%s: sm_scale %g below 1e-30", fn, t->sm_scale);
@@ -1080,12 +1081,13 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   int32_t* q_beg = reinterpret_cast<int32_t*>(ws + l.q_beg);
   int32_t* q_idx = reinterpret_cast<int32_t*>(ws + l.q_idx);
   hipStream_t s = sa::as_stream(stream);
-  if (t->dk || t->dv) {
+  if ((t->dk || t->dv) && !t->q_idx) {
     if (int rc = sa_kv_list_transpose(t->kv_idx, t->kv_cnt, B * H, nqb, nkb, t->max_cnt, q_beg, q_idx, stream)) return rc;
   }
   BwdArgs a;
   a.H = H;
   a.max_cnt = t->max_cnt;
+  a.packed = 0;
   a.bias = t->key_bias;
   a.bias_sb = t->key_bias ? t->bias_strides[0] : 0;
   a.bias_sh = t->key_bias ? t->bias_strides[1] : 0;
@@ -1124,7 +1126,10 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   a.n_items = B * H * nkb;
   a.order = t->k_order;
   a.n_slots = (int)(t->k_order ? t->n_k_slots : (a.n_items + 3) / 4 * 4);
-  a.idx = q_idx; a.cnt = q_beg;
+  a.idx = t->q_idx ? t->q_idx : q_idx;
+  a.cnt = t->q_idx ? t->q_cnt : q_beg;
+  a.packed = !t->q_idx;
+  if (t->q_idx) a.max_cnt = nqb;
   launch_pass_any<true>(a, t->dtype, D, l.k, s);
   return sa::check_launch(fn);
 }

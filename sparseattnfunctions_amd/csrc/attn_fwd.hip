@@ -1850,8 +1850,8 @@ extern "C" int sa_block_sparse_fwd_lse(const sa_attn_train* t, void* stream) {
   SA_REQUIRE(t->parts >= 1, "%s: parts=%d must be >= 1", fn, t->parts);
   if (t->mask) {
     SA_REQUIRE(t->Lq > 0 && t->Lk > 0, "%s: bad shape Lq=%d Lk=%d", fn, t->Lq, t->Lk);
-    if (int rc = sa_mask_to_kv_list(t->mask, t->mask_strides, t->B, t->H, (int)sa::cdiv(t->Lq, kBlock),
-                                    (int)sa::cdiv(t->Lk, kBlock), t->kv_idx, t->max_cnt, t->kv_cnt, stream))
+    if (int rc = sa::mask_lists(t->mask, t->mask_strides, t->B, t->H, (int)sa::cdiv(t->Lq, kBlock),
+                                (int)sa::cdiv(t->Lk, kBlock), t->kv_idx, t->max_cnt, t->kv_cnt, t->q_idx, t->q_cnt, stream, fn))
       return rc;
   }
   const int64_t* st = t->strides;

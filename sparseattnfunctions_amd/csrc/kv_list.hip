@@ -7,7 +7,28 @@
 
 namespace {
 
-// One wave per list row: ballot-compact the set entries of mask row (b, h, m).
+// A list row by one wave: ballot-compact the set entries of mask row (b, h, m).
+__device__ inline void mask_row(const uint8_t* mask, int64_t s0, int64_t s1, int64_t s2, int64_t s3, int H, int n_rows,
+                                int n_cols, int64_t row, int32_t* idx, int max_cnt, int32_t* cnt) {
+  const int lane = threadIdx.x & 63;
+  const int64_t bh = row / n_rows;
+  const int m = (int)(row - bh * n_rows);
+  const int64_t b = bh / H;
+  const int64_t h = bh - b * H;
+  const uint8_t* base = mask + b * s0 + h * s1 + (int64_t)m * s2;
+  int32_t* out = idx + row * max_cnt;
+  int total = 0;
+  for (int n0 = 0; n0 < n_cols; n0 += 64) {
+    const int n = n0 + lane;
+    const bool on = n < n_cols && base[(int64_t)n * s3] != 0;
+    const uint64_t bal = __ballot(on);
+    const int pre = __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0));
+    if (on) out[total + pre] = n;
+    total += __popcll(bal);
+  }
+  if (lane == 0) cnt[row] = total;
+}
+
 __global__ __launch_bounds__(256) void mask_to_list_kernel(const uint8_t* __restrict__ mask, int64_t s0,
                                                           int64_t s1, int64_t s2, int64_t s3, int H,
                                                           int nqb, int nkb, int64_t rows,
@@ -15,23 +36,19 @@ __global__ __launch_bounds__(256) void mask_to_list_kernel(const uint8_t* __rest
                                                           int32_t* __restrict__ kv_cnt) {
   const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 6;
   if (row >= rows) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t bh = row / nqb;
-  const int m = (int)(row - bh * nqb);
-  const int64_t b = bh / H;
-  const int64_t h = bh - b * H;
-  const uint8_t* base = mask + b * s0 + h * s1 + (int64_t)m * s2;
-  int32_t* out = kv_idx + row * max_cnt;
-  int total = 0;
-  for (int n0 = 0; n0 < nkb; n0 += 64) {
-    const int n = n0 + lane;
-    const bool on = n < nkb && base[(int64_t)n * s3] != 0;
-    const uint64_t bal = __ballot(on);
-    const int pre = __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0));
-    if (on) out[total + pre] = n;
-    total += __popcll(bal);
-  }
-  if (lane == 0) kv_cnt[row] = total;
+  mask_row(mask, s0, s1, s2, s3, H, nqb, nkb, row, kv_idx, max_cnt, kv_cnt);
+}
+
+// The lists of the rows and, behind them, those of the columns. Of both sides of [1, 15, 278, 278], a fifth set, 8 us;
+// the columns' from the rows' lists (transpose_lists_kernel) 25.
+__global__ __launch_bounds__(256) void mask_to_lists_kernel(const uint8_t* __restrict__ mask, int64_t s0, int64_t s1,
+                                                            int64_t s2, int64_t s3, int H, int nqb, int nkb,
+                                                            int64_t rows, int64_t cols, int32_t* __restrict__ kv_idx,
+                                                            int max_cnt, int32_t* __restrict__ kv_cnt,
+                                                            int32_t* __restrict__ q_idx, int32_t* __restrict__ q_cnt) {
+  const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 6;
+  if (row < rows) mask_row(mask, s0, s1, s2, s3, H, nqb, nkb, row, kv_idx, max_cnt, kv_cnt);
+  else if (row < rows + cols) mask_row(mask, s0, s1, s3, s2, H, nkb, nqb, row - rows, q_idx, nqb, q_cnt);
 }
 
 // Block masks of other block shapes (BLOCK_M x BLOCK_N, powers of two): one wave per 64-row
@@ -240,6 +257,23 @@ extern "C" int sa_mask_cells_to_kv_list(const uint8_t* mask, const int64_t mask_
   hipLaunchKernelGGL(mask_cells_to_list_kernel, dim3((unsigned)blocks), dim3(256), 0, sa::as_stream(stream), a);
   return sa::check_launch(fn);
 }
+
+namespace sa {
+int mask_lists(const uint8_t* mask, const int64_t mask_strides[4], int B, int H, int nqb, int nkb, int32_t* kv_idx,
+               int max_cnt, int32_t* kv_cnt, int32_t* q_idx, int32_t* q_cnt, void* stream, const char* fn) {
+  SA_REQUIRE(mask && kv_idx && kv_cnt && !q_idx == !q_cnt, "%s: null pointer", fn);
+  if (!q_idx) return sa_mask_to_kv_list(mask, mask_strides, B, H, nqb, nkb, kv_idx, max_cnt, kv_cnt, stream);
+  SA_REQUIRE(B > 0 && H > 0 && nqb > 0 && nkb > 0, "%s: bad shape B=%d H=%d nqb=%d nkb=%d", fn, B, H, nqb, nkb);
+  SA_REQUIRE(max_cnt >= nkb, "%s: max_cnt=%d < nkb=%d", fn, max_cnt, nkb);
+  const int64_t rows = (int64_t)B * H * nqb, cols = (int64_t)B * H * nkb;
+  const int64_t blocks = (rows + cols + 3) / 4;
+  SA_REQUIRE(blocks < (1LL << 31), "%s: too many rows", fn);
+  hipLaunchKernelGGL(mask_to_lists_kernel, dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), mask,
+                     mask_strides[0], mask_strides[1], mask_strides[2], mask_strides[3], H, nqb, nkb, rows, cols, kv_idx,
+                     max_cnt, kv_cnt, q_idx, q_cnt);
+  return check_launch(fn);
+}
+}  // namespace sa
 
 extern "C" int sa_mask_to_kv_list(const uint8_t* mask, const int64_t mask_strides[4], int B, int H,
                                   int nqb, int nkb, int32_t* kv_idx, int max_cnt, int32_t* kv_cnt,

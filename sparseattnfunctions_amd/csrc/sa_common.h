@@ -67,6 +67,9 @@ int attn_f32_lse(const float* q, const int64_t q_strides[3], const float* k, con
                  int Lq, int Lk, int D, const int32_t* kv_idx, const int32_t* kv_cnt, int max_cnt, float sm_scale,
                  const int32_t* work_order, int64_t n_slots, void* workspace, int64_t workspace_bytes, float* lse,
                  void* stream, const char* fn);
+// sa_mask_to_kv_list and, where q_idx is given, the lists of the columns (kv_list.hip).
+int mask_lists(const uint8_t* mask, const int64_t mask_strides[4], int B, int H, int nqb, int nkb, int32_t* kv_idx,
+               int max_cnt, int32_t* kv_cnt, int32_t* q_idx, int32_t* q_cnt, void* stream, const char* fn);
 // Bytes of the split-operand workspace of the fp32 attention (attn_f32.hip).
 int64_t attn_f32_terms_bytes(int B, int Hk, int Lk, int D);
 

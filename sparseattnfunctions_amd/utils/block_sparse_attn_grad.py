@@ -52,17 +52,19 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
 class _MaskLists:
     """The lists of a 64 x 64 block mask, which the forward call makes, and room for the rows'
-    log2-sum-exp2: one buffer of entries, counts, sums."""
+    log2-sum-exp2: one buffer of entries, counts, sums and, with `keys`, the key blocks' entries and
+    counts for the backward pass."""
 
-    def __init__(self, mask, B, H, nqb, nkb):
+    def __init__(self, mask, B, H, nqb, nkb, keys):
         if mask.shape[2] < nqb or mask.shape[3] < nkb:
             raise ValueError(f"block mask {tuple(mask.shape)} smaller than the block grid ({nqb}, {nkb})")
         if mask.dtype != torch.bool:
             mask = mask != 0
         if mask.shape[:2] != (B, H):
             mask = mask.expand(B, H, -1, -1)
-        self.mask, self.nkb = mask, nkb
-        self.idx = mask.new_empty(B * H * nqb * (nkb + 1 + BLOCK), dtype=torch.int32)
+        self.mask, self.nkb, self.keys = mask, nkb, keys
+        n = nqb * (nkb + 1 + BLOCK) + (nkb * (nqb + 1) if keys else 0)
+        self.idx = mask.new_empty(B * H * n, dtype=torch.int32)
         self.cnt = None
 
 
@@ -125,7 +127,10 @@ def _set_lists(call, plan, idx, cnt, lse=None):
     call.kv_idx = at = idx.data_ptr()
     if cnt is None:
         call.kv_cnt = at = at + 4 * plan.rows * call.max_cnt
-        call.lse = at + 4 * plan.rows
+        call.lse = at = at + 4 * plan.rows
+        if plan.keys:
+            call.q_idx = at = at + 4 * BLOCK * plan.rows
+            call.q_cnt = at + 4 * plan.rows * call.max_cnt
     else:
         call.kv_cnt = cnt.data_ptr()
         if lse is not None:
@@ -143,8 +148,9 @@ class _Plan:
     and workspace sizes."""
 
     def __init__(self, dtype, device, q_shape, Lk, q_strides, k_strides, v_strides, max_cnt, row_blocks, biased, sm_scale,
-                 n_text_blocks):
+                 n_text_blocks, keys):
         B, H, Lq, D = q_shape
+        self.keys = keys  # with key blocks' lists (_MaskLists)
         nqb, nkb = math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK)
         n_items = B * H * nqb
         args = self.args = _lib.AttnTrain(dtype=_lib.DTYPES[dtype], B=B, H=H, Lq=Lq, Lk=Lk, D=D, max_cnt=max_cnt, parts=1,
@@ -172,7 +178,9 @@ class _Plan:
             setattr(args, name + "_order", order.data_ptr())
             setattr(args, "n_" + name + "_slots", order.numel())
         n = ctypes.c_int64(0)
+        args.q_idx = 1 if keys else None  # (whether there is one is all that this reads)
         _lib.check(_lib.load().sa_block_sparse_bwd_workspace(args, ctypes.byref(n)), "sa_block_sparse_bwd_workspace")
+        args.q_idx = None
         self.backward_bytes = n.value
 
 
@@ -187,7 +195,7 @@ def _describe(q, k, v, kv, sm_scale: float, key_bias, n_text_blocks: int):
     else:
         max_cnt, row_blocks = kv.idx.shape[1], kv.row_blocks if kv.row_blocks is not None or kv.dense else 0.0
     plan = _plan(q.dtype, q.device, q.shape, k.shape[2], q.stride(), k.stride(), v.stride(), max_cnt, row_blocks,
-                 key_bias is not None, sm_scale, n_text_blocks)
+                 key_bias is not None, sm_scale, n_text_blocks, masked and kv.keys)
     args = _lib.AttnTrain.from_buffer_copy(plan.args)
     args.q, args.k, args.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     _set_lists(args, plan, kv.idx, kv.cnt)
@@ -382,7 +390,8 @@ def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Option
             raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
         return _NoKeys.apply(q, k, v)
     if BLOCK_M == BLOCK and BLOCK_N == BLOCK:
-        kv = _MaskLists(block_sparse_mask, B, H, math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK))
+        keys = torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)
+        kv = _MaskLists(block_sparse_mask, B, H, math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK), keys)
     elif min(BLOCK_M, BLOCK_N) < BLOCK:
         raise NotImplementedError(f"gradients of {BLOCK_M} x {BLOCK_N} blocks: blocks smaller than 64")
     else:

@@ -97,6 +97,7 @@ def test_c_argument_checks():
 
     assert need(B=2, H=30, Lq=640, Lk=650, max_cnt=11) == 0  # statistics, list beginnings and entries
     assert n.value == 60 * 10 * 128 * 4 + (60 * 12 * 4 + 255) // 256 * 256 + (60 * 10 * 11 * 4 + 255) // 256 * 256
+    assert need(B=2, H=30, Lq=640, Lk=650, max_cnt=11, q_idx=256) == 0 and n.value == 60 * 10 * 128 * 4
     for bad in (dict(B=0), dict(H=0), dict(Lq=0), dict(Lk=0), dict(max_cnt=0), dict(dtype=5), dict(H=1 << 27)):
         assert need(**bad) == _lib.SA_ERR_INVALID, bad
     assert need(D=32) == _lib.SA_ERR_UNSUPPORTED
@@ -109,7 +110,8 @@ def test_c_argument_checks():
     assert lib.sa_block_sparse_bwd(None, None) == _lib.SA_ERR_INVALID
     for bad in (dict(dtype=-1), *(dict([(x, None)]) for x in ("q", "k", "v", "out", "dout", "lse", "kv_idx", "kv_cnt")),
                 dict(Lq=0), dict(max_cnt=0), dict(sm_scale=0.0), dict(sm_scale=math.nan), dict(workspace=None),
-                dict(workspace=16), dict(workspace_bytes=100), dict(q_order=256, n_q_slots=3), dict(k_order=256)):
+                dict(workspace=16), dict(workspace_bytes=100), dict(q_order=256, n_q_slots=3), dict(k_order=256),
+                dict(q_idx=256), dict(q_cnt=256)):
         assert bwd(**bad) == _lib.SA_ERR_INVALID, bad
     for bad in (dict(D=96), dict(q=8), dict(dv=8), dict(stride=[0, 0, 65] * 8), dict(stride=[0, 0, 1 << 30] * 8),
                 dict(stride=[0, 0, -64] * 8), dict(dtype=2, key_bias=256), dict(max_cnt=65536, workspace_bytes=1 << 40),
@@ -122,7 +124,7 @@ def test_c_argument_checks():
     assert lib.sa_block_sparse_fwd_lse(None, None) == _lib.SA_ERR_INVALID
     for bad in (dict(dtype=7), dict(lse=None), dict(parts=0), dict(parts=2, workspace=None), dict(out=None), dict(sm_scale=-1.0),
                 dict(dtype=2, workspace_bytes=10), dict(Lk=0), dict(mask=256, Lq=0), dict(mask=256, kv_idx=None),
-                dict(mask=256, kv_cnt=None), dict(mask=256, Lk=64 * 100, max_cnt=99)):
+                dict(mask=256, kv_cnt=None), dict(mask=256, Lk=64 * 100, max_cnt=99), dict(mask=256, q_idx=256)):
         assert lse(**bad) == _lib.SA_ERR_INVALID, bad
     for bad in (dict(dtype=2, key_bias=256), dict(dtype=2, parts=2), dict(key_bias=256, parts=2), dict(D=80),
                 dict(stride=[0, 0, 66] * 8)):
