@@ -261,12 +261,15 @@ typedef struct sa_attn_train {
   int32_t *q_idx, *q_cnt;   /* nullable: [B*H*ceil(Lk/64)][ceil(Lq/64)] and their counts, the query blocks that list each */
                             /* key block: written by a forward call with a mask, read by a backward call for dk and dv, */
                             /* which else makes them itself */
+  float* row_max;           /* with key_bias, else not read: like lse, the offset of each row that lse is relative to */
 } sa_attn_train;
 
 /*
  * sa_block_sparse_fwd (bf16), sa_block_sparse_fwd_f16 or the fp32 attention, same contract and output
  * bits, that also stores each row's log2-sum-exp2 of its scores times log2(e): +inf for rows without a
- * key (empty lists, keys all biased to -inf) and past Lq. Reads neither dout nor the gradients.
+ * key (empty lists, keys all biased to -inf) and past Lq. With key_bias it is that of the scores less row_max,
+ * a score of the row or close to one (0 without a key): beside a bias of 1e9, say, one fp32 number has no bits
+ * left for the sum. Reads neither dout nor the gradients.
  *   workspace 16-bit: sa_attn_split_workspace bytes with parts > 1, else unused. fp32: NULL
  *             (sa_block_sparse_fwd_f32) or as for sa_block_sparse_fwd_f32_terms.
  */
@@ -279,7 +282,8 @@ int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
  * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type; fp32 takes its operands in
  * three bf16 terms (finite ones; those below about 1e-33 lose their low terms).
  *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype, max_cnt, n_text_blocks and whether there
- *             is a q_idx): the query rows' statistics, the transposed lists, sums of lists split over workgroups.
+ *             is a q_idx and a key_bias): the query rows' statistics, the transposed lists, sums of lists split over
+ *             workgroups.
  * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv and no q_idx,
  * sm_scale at least 1e-30.
  */

@@ -37,7 +37,7 @@ class AttnTrain(ctypes.Structure):
                    ("q_order", _P), ("n_q_slots", ctypes.c_int64), ("k_order", _P), ("n_k_slots", ctypes.c_int64),
                    ("workspace", _P), ("workspace_bytes", ctypes.c_int64), ("sm_scale", _F),
                    ("n_text_blocks", ctypes.c_int32), ("mask", _P), ("mask_strides", ctypes.c_int64 * 4),
-                   ("q_idx", _P), ("q_cnt", _P)])
+                   ("q_idx", _P), ("q_cnt", _P), ("row_max", _P)])
 
 
 # name -> (restype, argtypes); must match include/sa_api.h.

@@ -3,7 +3,7 @@
 //
 // With S = q k^T, lse the rows' log2-sum-exp2 that the forward pass stored, do the gradient of out
 // and everything restricted to the listed 64 x 64 blocks:
-//   P     = exp2(S * sm_scale * log2(e) [+ bias * log2(e)] - lse)
+//   P     = exp2(S * sm_scale * log2(e) [+ bias * log2(e) - offset] - lse)
 //   delta = rowsum(do * out),  dP = do v^T,  dS = P * (dP - delta)
 //   dq = sm_scale dS k,  dk = sm_scale dS^T q,  dv = P^T do
 // Two passes, each over the lists of one side: one per query block for dq (and delta), one per key
@@ -24,6 +24,13 @@
 // with row reads for the first and transposed reads for the second from the same LDS rows. For dk and
 // dv the streamed rows' -lse / scale and -delta start the accumulators of S and dP, so that an element
 // costs two products, an exp2 and its share of two roundings.
+//
+// With a key bias a row's offset and its lse, relative to it, come apart: where a row's keys all have a bias of -1e9,
+// say, one number for both has no bits for the sum. 32 rows with an offset past kFarOffset among them round a score as the
+// forward pass does, the bias times log2(e) and then the sum, and take off the offset and the lse one after the
+// other, so that they have the forward pass's probabilities; the others take off both at once (off by 2^-14 of a
+// probability at most). Two operations of the VALU more an element: the passes of [2, 12, 1350 x 5626, 64] with 0.3 of
+// the blocks take 49 and 62 us, all rows done so 57 and 69.
 //
 // Bound: the issue of MFMA and VALU, as in the forward pass. [2, 30, 2560, 64] bf16 with every block: query pass
 // 177 us (850 TFLOP/s of its three products), key pass 229 us (880 of its four); there the matrix cores work 51 % of
@@ -46,6 +53,7 @@ namespace {
 constexpr int kBlk = 64;   // rows per block of either side
 constexpr int kStep = 32;  // streamed rows per step, own rows per wave
 constexpr int kMostLast = 128;
+constexpr float kFarOffset = 64.f;  // (in log2 units)
 
 struct BwdArgs {
   const void* own_a;  // k or q
@@ -77,8 +85,10 @@ struct BwdArgs {
   float scale_log2;     // sm_scale * log2(e)
   float inv_scale_log2;
   const float* lse;     // query pass: [bh][64 * query blocks]
-  // [bh][2 * query blocks][2][32]: per 32 query rows their -lse / scale_log2, then their -delta. Written
-  // by the query pass, read by the key pass.
+  const float* row_max; // with a bias, alike: the rows' offsets
+  // [bh][2 * query blocks][2][32]: per 32 query rows their -lse / scale_log2, then their -delta. With a bias
+  // [..][4][32], then their offset and lse, which rows use whose first is NaN (all 32 or none). Written by the query
+  // pass, read by the key pass.
   float* stats;
   // More than one split: the items of an XCD's dispatch slots first .. first + n_split - 1 (first < 0: every
   // item, n_split of them) are computed by `splits` workgroups each, on shares of the item's steps, which store
@@ -207,13 +217,15 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   constexpr int kRowTile = kStep * 128;          // one half of a step's rows
   constexpr int kMat = kHalves * kRowTile;       // a step's rows of one matrix
   constexpr bool kStats = kKeys || kBias;
+  constexpr int kRowStats = kBias ? 128 : 64;               // statistics of 32 query rows
+  constexpr int kStatTile = kKeys ? kRowStats : 64;         // of a step, or its biases
   constexpr int kAcc = kKeys ? 2 : 1;
   constexpr int kRead = !kKeys && !kBias ? 4 : kKeys && kD == 128 ? 1 : 2;
   constexpr bool kEarly = !kKeys || kD == 64;  // registers for the first transposed reads before the exponentials
   // The two stages are separate objects, so that the compiler's waits tell reads of one from the
   // copies into the other.
   __shared__ __attribute__((aligned(1024))) uint8_t tile0[kParts * 2 * kMat], tile1[kParts * 2 * kMat];
-  __shared__ __attribute__((aligned(256))) float stat0[kParts * 64], stat1[kParts * 64];
+  __shared__ __attribute__((aligned(256))) float stat0[kParts * kStatTile], stat1[kParts * kStatTile];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -240,7 +252,8 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
     fb[s] = __builtin_bit_cast(v8, *reinterpret_cast<const uint4*>(ob + (int64_t)own_clamped * a.ob_sl + 16 * s + 8 * hh));
   }
 
-  float lse = 0.f, delta = 0.f;
+  float lse = 0.f, offset = 0.f, delta = 0.f;
+  bool far = false;  // query pass with a bias: the wave's rows take off offset and lse one after the other
   if constexpr (!kKeys) {
     const uint16_t* op = static_cast<const uint16_t*>(a.out) + b * a.o_sb + h * a.o_sh + (int64_t)own_clamped * a.o_sl;
 #pragma unroll
@@ -254,11 +267,19 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
       }
     }
     delta = xhalf_sum(delta);
-    lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col];
+    const int64_t at = ((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col;
+    lse = a.lse[at];
+    if constexpr (kBias) {
+      offset = a.row_max[at];
+      far = __ballot(fabsf(offset) > kFarOffset) != 0;
+      if (!far) lse += offset;
+    }
     if (part == 0 && split == 0) {
       const bool row_ok = own_row < a.L_own;
+      float* st = a.stats + (((int64_t)bh * a.n_own + blk) * 2 + w) * kRowStats;
       const float v = hh == 0 ? -lse * a.inv_scale_log2 : -delta;
-      a.stats[(((int64_t)bh * a.n_own + blk) * 2 + w) * 64 + lane] = row_ok ? v : hh == 0 ? -INFINITY : 0.f;
+      st[lane] = kBias && far && hh == 0 ? NAN : row_ok ? v : hh == 0 ? -INFINITY : 0.f;
+      if constexpr (kBias) st[64 + lane] = hh == 0 ? (far ? offset : 0.f) : lse;
     }
     if (!a.grad_a) return;  // only the statistics are wanted
   }
@@ -275,8 +296,8 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
 #pragma unroll
   for (int j = 0; j < 2; ++j)
     goff[j] = (8 * j + (lane >> 3)) * row_bytes + 16 * ((lane & 7) ^ swz(8 * j + (lane >> 3)));
-  const float* stat_src = kKeys ? a.stats + (int64_t)bh * a.n_st * 128 : bias;
-  const uint32_t stat_bytes = kKeys ? (uint32_t)a.n_st * 512 : (uint32_t)a.L_st * 4;
+  const float* stat_src = kKeys ? a.stats + (int64_t)bh * a.n_st * 2 * kRowStats : bias;
+  const uint32_t stat_bytes = kKeys ? (uint32_t)a.n_st * 8 * kRowStats : (uint32_t)a.L_st * 4;
 
   // The split's share of the 2 cnt steps, of it the part's.
   const int splits = place < 0 ? 1 : a.splits;
@@ -287,6 +308,14 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   auto block_of = [&](int i) -> int {  // the streamed block of the part's i-th step, -1: none
     const int s = beg + i;
     return i < per_part && s < n_steps ? list[s >> 1] : -1;
+  };
+  // Whether the rows of the part's i-th step take off offset and lse one after the other (a scalar load).
+  auto far_of = [&](int rb, int i) __attribute__((always_inline)) -> bool {
+    if constexpr (!kKeys || !kBias) return far;
+    if ((unsigned)rb >= (unsigned)a.n_st) return false;
+    const auto* st = (const __attribute__((address_space(4))) float*)stat_src;
+    const float first = st[((int64_t)2 * rb + ((beg + i) & 1)) * kRowStats];
+    return first != first;
   };
   // Copies of the part's i-th step. The descriptors begin at the step's rows and end with the head's, so
   // that rows past the last one read as zero and the lane offsets never change.
@@ -309,11 +338,13 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
       }
     }
     if (kStats && w == 0) {
-      const uint32_t soff = min(kKeys ? row0 * 8 : row0 * 4, stat_bytes);
+      const uint32_t soff = min(kKeys ? row0 * (kRowStats / 8) : row0 * 4, stat_bytes);
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(stat_src) + soff), (short)0, (int)(stat_bytes - soff),
           0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_u8*)(stat + part * 256), 4, 4 * lane, 0, 0, 0);
+      lds_u8* to = stat + part * 4 * kStatTile;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, to, 4, 4 * lane, 0, 0, 0);
+      if constexpr (kStatTile > 64) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, to, 4, 4 * lane, 0, 256, 0);
     }
   };
 
@@ -342,10 +373,10 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
 #pragma unroll
   for (int e = 0; e < 16; ++e) less_delta[e] = -delta;
 
-  auto compute = [&](int cur, int i, const lds_u8* tile, const float* stat) __attribute__((always_inline)) {
+  auto compute = [&](int cur, int i, bool far_step, const lds_u8* tile, const float* stat) __attribute__((always_inline)) {
     if ((unsigned)cur >= (unsigned)a.n_st) return;
-    const float* st_ = stat + part * 64 + 4 * hh;
-    auto stats = [&](int at) __attribute__((always_inline)) {  // 16 of the step's 32 statistics or biases
+    const float* st_ = stat + part * kStatTile + 4 * hh;
+    auto stats = [&](int at) __attribute__((always_inline)) {  // 16 of 32 of the step's statistics or biases
       sa_f32x16 r;
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
@@ -356,9 +387,10 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
     };
     sa_f32x16 S = {}, dP = less_delta;
     if constexpr (kKeys) {
-      S = stats(0);
+      if (!kBias || !far_step) S = stats(0);
       dP = stats(32);
     }
+    float scale = a.scale_log2, add = kKeys ? own_bias : -lse;  // (with a bias)
     // Row operands in groups of kRead 16-column steps: a group's reads are issued while the products of
     // the group before run, each of which waits for its own two.
     sa_u32x4v x[kDS], y[kDS];
@@ -402,10 +434,31 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
     // Elements e: streamed row 8 (e / 4) + 4 hh + e % 4 of the step, own row col.
     uint32_t Pp[8], Sp[8];
     if constexpr (kKeys) {
+      if constexpr (kBias) {
+        if (far_step) {  // S becomes the exponent
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {  // four rows' offsets, and sums, at a time, read no earlier (the registers)
+            __builtin_amdgcn_sched_barrier(0);
+            const float4 off = *reinterpret_cast<const float4*>(st_ + 64 + 2 * e);
+            S[e] = fmaf(S[e], scale, add) - off.x;
+            S[e + 1] = fmaf(S[e + 1], scale, add) - off.y;
+            S[e + 2] = fmaf(S[e + 2], scale, add) - off.z;
+            S[e + 3] = fmaf(S[e + 3], scale, add) - off.w;
+            __builtin_amdgcn_sched_barrier(0);
+            const float4 sum = *reinterpret_cast<const float4*>(st_ + 96 + 2 * e);
+            S[e] -= sum.x;
+            S[e + 1] -= sum.y;
+            S[e + 2] -= sum.z;
+            S[e + 3] -= sum.w;
+          }
+          scale = 1.f;
+          add = 0.f;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        const float p0 = fast_exp2(kBias ? fmaf(S[e], a.scale_log2, own_bias) : S[e] * a.scale_log2);
-        const float p1 = fast_exp2(kBias ? fmaf(S[e + 1], a.scale_log2, own_bias) : S[e + 1] * a.scale_log2);
+        const float p0 = fast_exp2(kBias ? fmaf(S[e], scale, add) : S[e] * a.scale_log2);
+        const float p1 = fast_exp2(kBias ? fmaf(S[e + 1], scale, add) : S[e + 1] * a.scale_log2);
         Pp[e >> 1] = E::pack(p0, p1);
         Sp[e >> 1] = E::pack(p0 * dP[e], p1 * dP[e + 1]);
       }
@@ -418,10 +471,22 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
         for (int e = 0; e < 16; ++e)
           if (row0 + 8 * (e >> 2) + 4 * hh + (e & 3) >= a.L_st) S[e] = -INFINITY;
       }
+      if constexpr (kBias) {
+        if (far_step) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            S[e] = fmaf(S[e], scale, kb2[e] * kLog2e) - offset - lse;
+            kb2[e] = 0.f;
+          }
+          scale = 1.f;
+          add = 0.f;
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        const float p0 = fast_exp2(fmaf(S[e], a.scale_log2, kBias ? fmaf(kb2[e], kLog2e, -lse) : -lse));
-        const float p1 = fast_exp2(fmaf(S[e + 1], a.scale_log2, kBias ? fmaf(kb2[e + 1], kLog2e, -lse) : -lse));
+        const float p0 = fast_exp2(kBias ? fmaf(S[e], scale, fmaf(kb2[e], kLog2e, add)) : fmaf(S[e], a.scale_log2, -lse));
+        const float p1 = fast_exp2(kBias ? fmaf(S[e + 1], scale, fmaf(kb2[e + 1], kLog2e, add))
+                                         : fmaf(S[e + 1], a.scale_log2, -lse));
         Sp[e >> 1] = E::pack(p0 * dP[e], p1 * dP[e + 1]);
       }
     }
@@ -447,6 +512,7 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   lds_u8* const t1 = (lds_u8*)tile1;
   int rb = block_of(0);
   issue(rb, 0, t0, (lds_u8*)stat0);
+  bool far0 = far_of(rb, 0), far1;
   int rb_next = block_of(1);
   for (int i = 0; i < per_part; i += 2) {
     // This wave's copies of step i have landed, then everyone's; every wave is done with step i - 1,
@@ -454,13 +520,15 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     wg_barrier();
     issue(rb_next, i + 1, t1, (lds_u8*)stat1);
-    compute(rb, i, t0, stat0);
+    far1 = far_of(rb_next, i + 1);
+    compute(rb, i, far0, t0, stat0);
     if (i + 1 >= per_part) break;
     rb = block_of(i + 2);
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     wg_barrier();
     issue(rb, i + 2, t0, (lds_u8*)stat0);
-    compute(rb_next, i + 1, t1, stat1);
+    far0 = far_of(rb, i + 2);
+    compute(rb_next, i + 1, far1, t1, stat1);
     rb_next = block_of(i + 3);
   }
 
@@ -1007,7 +1075,7 @@ Layout layout(const sa_attn_train& t) {
   const int64_t BH = (int64_t)t.B * t.H, nqb = sa::cdiv(t.Lq, kBlk), nkb = sa::cdiv(t.Lk, kBlk);
   const bool f32 = t.dtype == SA_DTYPE_F32;
   Layout l;
-  l.q_beg = align256(BH * nqb * 128 * (int64_t)sizeof(float));
+  l.q_beg = align256(BH * nqb * (t.key_bias ? 256 : 128) * (int64_t)sizeof(float));
   l.q_idx = l.q_beg + (t.q_idx ? 0 : align256(BH * (nkb + 1) * (int64_t)sizeof(int32_t)));
   l.partial = l.q_idx + (t.q_idx ? 0 : align256(BH * nqb * t.max_cnt * (int64_t)sizeof(int32_t)));
   // (a list is no longer than the other side has blocks, but for repeated entries)
@@ -1052,6 +1120,7 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   if (t->sm_scale < 1e-30f) return sa::fail(SA_ERR_UNSUPPORTED, "%s: sm_scale %g below 1e-30", fn, t->sm_scale);
   const bool f32 = t->dtype == SA_DTYPE_F32;
   if (f32 && t->key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
+  SA_REQUIRE(!t->key_bias || t->row_max, "%s: key_bias without row_max", fn);
   const int nqb = sa::cdiv(Lq, kBlk), nkb = sa::cdiv(Lk, kBlk);
   const int per16 = f32 ? 4 : 8, size = f32 ? 4 : 2;
   const void* ptrs[8] = {t->q, t->k, t->v, t->out, t->dout, t->dq, t->dk, t->dv};
@@ -1095,6 +1164,7 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   a.scale_log2 = t->sm_scale * kLog2e;
   a.inv_scale_log2 = 1.f / a.scale_log2;
   a.lse = t->lse;
+  a.row_max = t->row_max;
   a.stats = reinterpret_cast<float*>(ws);
   a.partial = reinterpret_cast<float*>(ws + l.partial);
   a.out = t->out;

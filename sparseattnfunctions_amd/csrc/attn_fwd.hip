@@ -108,7 +108,8 @@ struct FwdArgs {
   float* pool_r;
   int pool_ncol;
   int pool_lpad;
-  float* pool_lse;  // null: not stored. Without pooling: stored as the backward pass wants it (train_lse)
+  float* pool_lse;  // null: not stored. Without pooling: stored as the backward pass wants it (store_train_lse)
+  float* row_max;   // with a key bias: the offset that the stored log2-sum-exp2 is relative to
   // Fused pooled map (pool_po non-null; pooled block size = kPool): after its item the wave
   // forms the Po rows of its own query rows, Po[i][c] = max over the rows r of query block i
   // of exp2(R[c][r] - lse[r]), each Po row then divided by its sum. Po rows and columns are
@@ -135,10 +136,15 @@ __device__ inline int range_item(const FwdArgs& a, int slot) {
   return kDown ? hi - 1 - i : lo + i;
 }
 
-// log2-sum-exp2 of a row for the backward pass: +inf for a row without a key (its recomputed
-// probabilities are then 0), as for rows past Lq, which the padded array has.
-__device__ inline float train_lse(float m, float l, bool row_ok) {
-  return row_ok && l != 0.f ? (m == -INFINITY ? 0.f : m) + log2f(l) : INFINITY;
+// Stores the log2-sum-exp2 of row `at` of the padded array for the backward pass: +inf for a row without a key (its
+// recomputed probabilities are then 0), as for rows past Lq. With a key bias the offset m and the sum's logarithm stay
+// apart, since the bias may be so large that their sum rounds the latter away.
+template <bool kBias>
+__device__ inline void store_train_lse(const FwdArgs& a, int64_t at, float m, float l, bool row_ok) {
+  const bool any = row_ok && l != 0.f;
+  const float offset = any && m != -INFINITY ? m : 0.f;
+  a.pool_lse[at] = any ? (kBias ? log2f(l) : offset + log2f(l)) : INFINITY;
+  if constexpr (kBias) a.row_max[at] = offset;
 }
 
 // T: bf16 or fp16 operands (and output). kD: head dim 64 or 128. A 128-dim row is staged as
@@ -830,7 +836,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs 
       const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
       int row = qb * kBlock + r;
       bool store = row < a.Lq;
-      if (kPool == 0 && a.pool_lse && ch == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(M, lsum, store);
+      if (kPool == 0 && a.pool_lse && ch == 0) store_train_lse<kBias>(a, (int64_t)bh * a.pool_lpad + row, M, lsum, store);
       if (store && a.o_rows) {
         row = a.o_rows[row];
         store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -887,7 +893,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs 
     }
     int row = qb * kBlock + 32 * g + col;
     bool store = row < a.Lq;
-    if (kPool == 0 && a.pool_lse && g == hh) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(m[g], l_tot, store);
+    if (kPool == 0 && a.pool_lse && g == hh)
+      store_train_lse<kBias>(a, (int64_t)bh * a.pool_lpad + row, m[g], l_tot, store);
     if (store && a.o_rows) {  // remapped layout: query i goes to out row o_rows[i]
       row = a.o_rows[row];
       store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -1320,7 +1327,7 @@ __global__ __launch_bounds__(128, 2) void bsa_fwd_pair_kernel(FwdArgs a) {
   const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
   int row = qb * kBlock + 32 * g + col;
   bool store = row < a.Lq;
-  if (a.pool_lse && hh == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(m, l_tot, store);
+  if (a.pool_lse && hh == 0) store_train_lse<false>(a, (int64_t)bh * a.pool_lpad + row, m, l_tot, store);
   if (store && a.o_rows) {  // remapped layout: query i goes to out row o_rows[i]
     row = a.o_rows[row];
     store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -1456,7 +1463,7 @@ __global__ __launch_bounds__(256) void split_merge_kernel(FwdArgs a) {
   }
   const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
   int row = qb * kBlock + r;
-  if (a.pool_lse && d0 == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(mx, lsum, row < a.Lq);
+  if (a.pool_lse && d0 == 0) store_train_lse<false>(a, (int64_t)bh * a.pool_lpad + row, mx, lsum, row < a.Lq);
   if (row >= a.Lq) return;
   if (a.o_rows) {
     row = a.o_rows[row];
@@ -1635,7 +1642,7 @@ int launch_fwd(const uint16_t* q, const int64_t q_strides[3], const uint16_t* k,
                const char* fn, int kv_rep = 1, int pool_cols = 0, float* pool_r = nullptr,
                float* pool_lse = nullptr, const PoolOut* pool_out = nullptr, bool fp16 = false,
                bool v32 = false, int parts = 1, void* split_ws = nullptr, int64_t split_ws_bytes = 0,
-               const uint16_t* k16 = nullptr, const uint32_t* k16_norm2 = nullptr) {
+               const uint16_t* k16 = nullptr, const uint32_t* k16_norm2 = nullptr, float* row_max = nullptr) {
   SA_REQUIRE(q && k && v && out && q_strides && k_strides && v_strides && out_strides && kv_idx && kv_cnt,
              "%s: null pointer", fn);
   SA_REQUIRE(B > 0 && H > 0 && Lq > 0 && Lk > 0, "%s: bad shape B=%d H=%d Lq=%d Lk=%d", fn, B, H, Lq, Lk);
@@ -1712,6 +1719,7 @@ int launch_fwd(const uint16_t* q, const int64_t q_strides[3], const uint16_t* k,
   a.pool_ncol = pool_cols ? nkb * (kBlock / pool_cols) : 0;
   a.pool_lpad = nqb * kBlock;
   a.pool_lse = pool_lse;
+  a.row_max = row_max;
   a.pool_po = pool_out ? pool_out->po : nullptr;
   a.po_sb = pool_out ? pool_out->sb : 0;
   a.po_sh = pool_out ? pool_out->sh : 0;
@@ -1848,6 +1856,10 @@ extern "C" int sa_block_sparse_fwd_lse(const sa_attn_train* t, void* stream) {
              t->dtype);
   SA_REQUIRE(t->lse, "%s: null lse", fn);
   SA_REQUIRE(t->parts >= 1, "%s: parts=%d must be >= 1", fn, t->parts);
+  if ((t->dtype == SA_DTYPE_F32 || t->key_bias) && t->parts != 1)
+    return sa::fail(SA_ERR_UNSUPPORTED, "%s: key-range parts with fp32 or key_bias", fn);
+  if (t->dtype == SA_DTYPE_F32 && t->key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
+  SA_REQUIRE(!t->key_bias || t->row_max, "%s: key_bias without row_max", fn);
   if (t->mask) {
     SA_REQUIRE(t->Lq > 0 && t->Lk > 0, "%s: bad shape Lq=%d Lk=%d", fn, t->Lq, t->Lk);
     if (int rc = sa::mask_lists(t->mask, t->mask_strides, t->B, t->H, (int)sa::cdiv(t->Lq, kBlock),
@@ -1856,7 +1868,6 @@ extern "C" int sa_block_sparse_fwd_lse(const sa_attn_train* t, void* stream) {
   }
   const int64_t* st = t->strides;
   if (t->dtype == SA_DTYPE_F32) {
-    if (t->key_bias || t->parts != 1) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias or key-range parts", fn);
     return sa::attn_f32_lse(static_cast<const float*>(t->q), st, static_cast<const float*>(t->k), st + 3,
                             static_cast<const float*>(t->v), st + 6, static_cast<float*>(t->out), st + 9, t->B, t->H,
                             t->Lq, t->Lk, t->D, t->kv_idx, t->kv_cnt, t->max_cnt, t->sm_scale, t->fwd_order,
@@ -1867,7 +1878,7 @@ extern "C" int sa_block_sparse_fwd_lse(const sa_attn_train* t, void* stream) {
                     t->Lq, t->Lk, t->D, t->kv_idx, t->kv_cnt, t->max_cnt, false, nullptr, nullptr, t->key_bias,
                     t->bias_strides, t->sm_scale, t->fwd_order, t->n_fwd_slots, nullptr, 0, nullptr, 0, stream, fn, 1, 0,
                     nullptr, t->lse, nullptr, t->dtype == SA_DTYPE_F16, false, t->parts, t->workspace,
-                    t->workspace_bytes);
+                    t->workspace_bytes, nullptr, nullptr, t->row_max);
 }
 
 namespace {

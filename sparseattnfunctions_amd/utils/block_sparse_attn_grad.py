@@ -22,9 +22,11 @@ query row without a key (an empty list, or keys all biased to -inf) has a zero o
 gradients; a key block in no list has zero gradients. The mask, the lists and key_bias are not
 differentiated.
 
-A key_bias below -2.35e38 (the type's lowest value among them) counts as -inf, and keys that it masks
-still enter the products: their k and v have to be finite, as with any additive mask. Keys in blocks
-that no row lists, and memory behind the last row, are not read into any sum.
+A key_bias is added to the scores in fp32, in both passes alike, so that one as large as 1e9 leaves a
+row that lists nothing else few of its scores' bits. One below -2.35e38 (the type's lowest value among
+them) counts as -inf, and keys that it masks still enter the products: their k and v have to be finite,
+as with any additive mask. Keys in blocks that no row lists, and memory behind the last row, are not
+read into any sum.
 """
 from __future__ import annotations
 
@@ -52,10 +54,10 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
 class _MaskLists:
     """The lists of a 64 x 64 block mask, which the forward call makes, and room for the rows'
-    log2-sum-exp2: one buffer of entries, counts, sums and, with `keys`, the key blocks' entries and
-    counts for the backward pass."""
+    log2-sum-exp2: one buffer of entries, counts, sums (with `biased` and the rows' offsets) and, with `keys`, the
+    key blocks' entries and counts for the backward pass."""
 
-    def __init__(self, mask, B, H, nqb, nkb, keys):
+    def __init__(self, mask, B, H, nqb, nkb, keys, biased):
         if mask.shape[2] < nqb or mask.shape[3] < nkb:
             raise ValueError(f"block mask {tuple(mask.shape)} smaller than the block grid ({nqb}, {nkb})")
         if mask.dtype != torch.bool:
@@ -63,7 +65,7 @@ class _MaskLists:
         if mask.shape[:2] != (B, H):
             mask = mask.expand(B, H, -1, -1)
         self.mask, self.nkb, self.keys = mask, nkb, keys
-        n = nqb * (nkb + 1 + BLOCK) + (nkb * (nqb + 1) if keys else 0)
+        n = nqb * (nkb + 1 + (2 if biased else 1) * BLOCK) + (nkb * (nqb + 1) if keys else 0)
         self.idx = mask.new_empty(B * H * n, dtype=torch.int32)
         self.cnt = None
 
@@ -123,18 +125,28 @@ def _set(call, **tensors):
 
 
 def _set_lists(call, plan, idx, cnt, lse=None):
-    """cnt None: a _MaskLists' buffer, which has the lse too."""
+    """cnt None: a _MaskLists' buffer, which has the lse too. lse with a bias: [2, ...], the sums and the offsets."""
     call.kv_idx = at = idx.data_ptr()
     if cnt is None:
         call.kv_cnt = at = at + 4 * plan.rows * call.max_cnt
         call.lse = at = at + 4 * plan.rows
+        at += 4 * BLOCK * plan.rows
+        if plan.biased:
+            call.row_max = at
+            at += 4 * BLOCK * plan.rows
         if plan.keys:
-            call.q_idx = at = at + 4 * BLOCK * plan.rows
+            call.q_idx = at
             call.q_cnt = at + 4 * plan.rows * call.max_cnt
     else:
         call.kv_cnt = cnt.data_ptr()
         if lse is not None:
-            call.lse = lse.data_ptr()
+            _set_lse(call, plan, lse)
+
+
+def _set_lse(call, plan, lse):
+    call.lse = at = lse.data_ptr()
+    if plan.biased:
+        call.row_max = at + 4 * BLOCK * plan.rows
 
 
 def _set_bias(call, key_bias):
@@ -150,12 +162,13 @@ class _Plan:
     def __init__(self, dtype, device, q_shape, Lk, q_strides, k_strides, v_strides, max_cnt, row_blocks, biased, sm_scale,
                  n_text_blocks, keys):
         B, H, Lq, D = q_shape
-        self.keys = keys  # with key blocks' lists (_MaskLists)
+        self.keys, self.biased = keys, biased  # keys: with key blocks' lists (_MaskLists)
         nqb, nkb = math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK)
         n_items = B * H * nqb
         args = self.args = _lib.AttnTrain(dtype=_lib.DTYPES[dtype], B=B, H=H, Lq=Lq, Lk=Lk, D=D, max_cnt=max_cnt, parts=1,
                                           sm_scale=sm_scale, n_text_blocks=n_text_blocks)
-        self.out, self.lse, self.rows = (B, H, Lq, D), (B, H, nqb * BLOCK), n_items
+        self.out, self.rows = (B, H, Lq, D), n_items
+        self.lse = (2, B, H, nqb * BLOCK) if biased else (B, H, nqb * BLOCK)
         self.grads = (B, H, Lq, D), (B, H, Lk, D), (B, H, Lk, D)
         sq, sk = (H * Lq * D, Lq * D, D), (H * Lk * D, Lk * D, D)
         self.square = Lq == Lk  # dk and dv are like dout
@@ -178,9 +191,10 @@ class _Plan:
             setattr(args, name + "_order", order.data_ptr())
             setattr(args, "n_" + name + "_slots", order.numel())
         n = ctypes.c_int64(0)
-        args.q_idx = 1 if keys else None  # (whether there is one is all that this reads)
+        # (whether there are any is all that this reads)
+        args.q_idx, args.key_bias = 1 if keys else None, 1 if biased else None
         _lib.check(_lib.load().sa_block_sparse_bwd_workspace(args, ctypes.byref(n)), "sa_block_sparse_bwd_workspace")
-        args.q_idx = None
+        args.q_idx = args.key_bias = None
         self.backward_bytes = n.value
 
 
@@ -214,7 +228,7 @@ def _forward(plan: _Plan, args: _lib.AttnTrain, q):
     lse = None
     if not args.lse:
         lse = torch.empty(plan.lse, dtype=torch.float32, device=device)
-        args.lse = lse.data_ptr()
+        _set_lse(args, plan, lse)
     ws = None
     if plan.terms:
         ws = f32_terms_workspace(args.B, args.H, args.Lk, args.D, device)
@@ -274,7 +288,9 @@ def block_sparse_attention_lse(q, k, v, kv: KVList, sm_scale: float, key_bias: O
                                n_text_blocks: int = 0):
     """(out, lse): `block_sparse_attention` (q [B,H,Lq,D], k/v [B,H,Lk,D], bf16, fp16 or fp32, D 64 or
     128; key_bias fp32 [B,H,Lk], not with fp32) and the rows' log2-sum-exp2, fp32
-    [B, H, 64 * ceil(Lq / 64)], +inf for rows without a key and past Lq. No autograd.
+    [B, H, 64 * ceil(Lq / 64)], +inf for rows without a key and past Lq. With key_bias [2, B, H, ...]: the
+    log2-sum-exp2 of the scores less an offset of each row, and that offset; their sum is the whole, rounded to
+    the bias's magnitude. No autograd.
     `n_text_blocks` only affects scheduling, as there."""
     key_bias = _check_inputs(q, k, v, kv, key_bias)
     with torch.no_grad():
@@ -292,14 +308,16 @@ def block_sparse_attention_backward(dout, q, k, v, out, lse, kv: KVList, sm_scal
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
             raise ValueError(f"{name} must be like q: {tuple(q.shape)} {q.dtype}, got {tuple(t.shape)} {t.dtype}")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], q.shape[1], kv.nqb * BLOCK) \
-            or not lse.is_contiguous() or lse.device != q.device:
+    shape = (q.shape[0], q.shape[1], kv.nqb * BLOCK)
+    if key_bias is not None:
+        shape = (2, *shape)
+    if lse.dtype != torch.float32 or tuple(lse.shape) != shape or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError("lse must be block_sparse_attention_lse's")
     with torch.no_grad():
         q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
         plan, args = _describe(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
         _set(args, out=out)
-        args.lse = lse.data_ptr()
+        _set_lse(args, plan, lse)
         return _backward(plan, args, dout, needs)
 
 
@@ -391,7 +409,7 @@ def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Option
         return _NoKeys.apply(q, k, v)
     if BLOCK_M == BLOCK and BLOCK_N == BLOCK:
         keys = torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)
-        kv = _MaskLists(block_sparse_mask, B, H, math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK), keys)
+        kv = _MaskLists(block_sparse_mask, B, H, math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK), keys, key_bias is not None)
     elif min(BLOCK_M, BLOCK_N) < BLOCK:
         raise NotImplementedError(f"gradients of {BLOCK_M} x {BLOCK_N} blocks: blocks smaller than 64")
     else:

@@ -151,3 +151,25 @@ def test_struct_layout(tmp_path):
     out = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout
     want = [getattr(_lib.AttnTrain, n).offset for n in names] + [ctypes.sizeof(_lib.AttnTrain)]
     assert [int(x) for x in out.split()] == want
+
+
+def test_biased_calls_need_the_rows_offsets():
+    lib = _lib.load()
+
+    def call(**changed):
+        a = dict(dtype=0, B=1, H=1, Lq=128, Lk=128, D=64, max_cnt=2, parts=1, sm_scale=0.125, workspace=256,
+                 workspace_bytes=1 << 20)
+        a.update((x, 256) for x in ("q", "k", "v", "out", "dout", "dq", "dk", "dv", "lse", "kv_idx", "kv_cnt", "key_bias"))
+        t = _lib.AttnTrain(**{**a, **changed})
+        t.strides[:] = [0, 0, 64] * 8
+        return t
+
+    assert lib.sa_block_sparse_fwd_lse(call(), None) == _lib.SA_ERR_INVALID
+    assert lib.sa_block_sparse_bwd(call(), None) == _lib.SA_ERR_INVALID
+    # with a bias the rows' statistics take twice the room
+    sizes = []
+    for bias in (None, 256):
+        n = ctypes.c_int64(0)
+        assert lib.sa_block_sparse_bwd_workspace(call(key_bias=bias, q_idx=256), ctypes.byref(n)) == 0
+        sizes.append(n.value)
+    assert sizes == [2 * 128 * 4, 2 * 256 * 4]
