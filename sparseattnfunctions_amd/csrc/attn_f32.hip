@@ -64,7 +64,7 @@ struct F32Args {
   // log2-sum-exp2 to pool_lse[bh * pool_lpad + row].
   float* pool_r;
   int pool_ncol;
-  float* pool_lse;  // (without pooling nullable, stored as the backward pass wants it: train_lse)
+  float* pool_lse;  // (without pooling: of a training call, train_lse)
   int pool_lpad;
   // bsa_fwd_f32_terms_kernel: the split operands and the per-key-block flags (f32_terms_kernel).
   const uint8_t* planes;
@@ -250,7 +250,7 @@ __device__ __forceinline__ void f32_rows(const F32Args& a, int bh, int qb, int r
 }
 
 // Epilogue of one wave: out = acc / l; an empty list writes 0. Pooling: the row's log2-sum-exp2.
-template <int kD, int kPool, int kJ>
+template <int kD, int kPool, int kJ, bool kLse>
 __device__ __forceinline__ void f32_store(const F32Args& a, int bh, int qb, int row0, int lane,
                                           const sa_f32x4 (&acc)[kD / 16][kJ], const float (&m)[kJ],
                                           const float (&l)[kJ]) {
@@ -265,7 +265,7 @@ __device__ __forceinline__ void f32_store(const F32Args& a, int bh, int qb, int 
     const int row = qb * kBlk + row0 + 16 * j + r;
     if constexpr (kPool != 0) {
       if (g == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = (m[j] == -INFINITY ? 0.f : m[j]) + log2f(l_tot);
-    } else if (a.pool_lse && g == 0) {
+    } else if (kLse && g == 0) {
       a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(m[j], l_tot, row < a.Lq);
     }
     if (row < a.Lq) {
@@ -284,7 +284,8 @@ constexpr uint32_t kTermMax = 0x5d800000u;  // 2^60
 constexpr uint32_t kTermMin = 0x17800000u;  // 2^-80: 2^18 products that lose 2^-126 lose 2^-28 of a value
 constexpr uint32_t kTermSkip = 0xffffffffu;  // no |x| has these bits
 
-template <int kD, int kPool>
+// kLse: a training call's form, which stores the rows' log2-sum-exp2 without pooling.
+template <int kD, int kPool, bool kLse = false>
 __global__ __launch_bounds__(64 * kWavesF32, kD == 64 ? 2 : 1) void bsa_fwd_f32_kernel(F32Args a) {
   static_assert(kD == 64 || kD == 128, "head dim 64 or 128");
   static_assert(kPool == 0 || kPool == 32 || kPool == 64, "pooling columns of 32 or 64 keys");
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(64 * kWavesF32, kD == 64 ? 2 : 1) void bsa_fwd_f32_
   sa_f32x4 acc[kD / 16][4];
   float m[4], l[4];
   f32_rows<kD, kPool, 4>(a, bh, qb, 0, 0, 1, lane, acc, m, l);
-  f32_store<kD, kPool, 4>(a, bh, qb, 0, lane, acc, m, l);
+  f32_store<kD, kPool, 4, kLse>(a, bh, qb, 0, lane, acc, m, l);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -502,7 +503,7 @@ __device__ inline float half_sum(float x) {
 // load each operand for half the MFMAs, 64 bytes per cycle and CU, the vector cache's rate), and
 // [1, 2, 2048, 64] with a quarter of the blocks 153 -> 37 us. Error against a 64-bit softmax 9.6e-7
 // where the fp32 MFMA's was 1.1e-6 (2-norm, relative).
-template <int kD, int kPool, int kKW>
+template <int kD, int kPool, int kKW, bool kLse = false>
 __global__ __launch_bounds__(256, 2) void bsa_fwd_f32_terms_kernel(F32Args a) {
   static_assert(kD == 64 || kD == 128, "head dim 64 or 128");
   static_assert(kPool == 0 || kPool == 32 || kPool == 64, "pooling columns of 32 or 64 keys");
@@ -597,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void bsa_fwd_f32_terms_kernel(F32Args a) {
       float m[kJ], l[kJ];
       f32_rows<kD, kPool, kJ>(a, bh, qb, row0 + r0, it0, kKW, lane, acc, m, l);
       if constexpr (kKW == 1) {
-        f32_store<kD, kPool, kJ>(a, bh, qb, row0 + r0, lane, acc, m, l);
+        f32_store<kD, kPool, kJ, kLse>(a, bh, qb, row0 + r0, lane, acc, m, l);
       } else {
         const int r = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -796,7 +797,7 @@ __global__ __launch_bounds__(256, 2) void bsa_fwd_f32_terms_kernel(F32Args a) {
         const int row = qb * kBlk + row0 + lrow;
         if constexpr (kPool != 0) {
           if (hh == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = (m[g] == -INFINITY ? 0.f : m[g]) + log2f(l_tot);
-        } else if (a.pool_lse && hh == 0) {
+        } else if (kLse && hh == 0) {
           a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(m[g], l_tot, row < a.Lq);
         }
         if (row < a.Lq) {
@@ -850,7 +851,7 @@ __global__ __launch_bounds__(256, 2) void bsa_fwd_f32_terms_kernel(F32Args a) {
       const int row = qb * kBlk + row0 + lrow;
       if constexpr (kPool != 0) {
         if (ch == 0) a.pool_lse[(int64_t)bh * a.pool_lpad + row] = (M == -INFINITY ? 0.f : M) + log2f(L);
-      } else if (a.pool_lse && ch == 0) {
+      } else if (kLse && ch == 0) {
         a.pool_lse[(int64_t)bh * a.pool_lpad + row] = train_lse(M, L, row < a.Lq);
       }
       if (row < a.Lq) {
@@ -867,7 +868,7 @@ namespace {
 
 int64_t terms_blocks(int B, int Hk, int Lk) { return (int64_t)B * Hk * sa::cdiv(Lk, kBlk); }
 
-template <int kD, int kPool>
+template <int kD, int kPool, bool kLse = false>
 void launch_terms_pool(const F32Args& a, hipStream_t s) {
   // Up to three rounds of the card's 2 048 waves, four waves share each unit (64 query rows, 32
   // at head dim 128); measured, one wave against four per unit: 64 units 78 / 43 us, 504 154 / 84,
@@ -879,8 +880,8 @@ void launch_terms_pool(const F32Args& a, hipStream_t s) {
   const bool shared = (int64_t)a.n_items * kHalvesQ <= kSharedUnits;
   const int64_t wgs = shared ? 4 * kHalvesQ : kHalvesQ;  // workgroups per dispatch group
   const dim3 grid((unsigned)((groups + 7) / 8 * 8 * wgs)), blk(256);
-  if (shared) hipLaunchKernelGGL((bsa_fwd_f32_terms_kernel<kD, kPool, 4>), grid, blk, 0, s, a);
-  else hipLaunchKernelGGL((bsa_fwd_f32_terms_kernel<kD, kPool, 1>), grid, blk, 0, s, a);
+  if (shared) hipLaunchKernelGGL((bsa_fwd_f32_terms_kernel<kD, kPool, 4, kLse>), grid, blk, 0, s, a);
+  else hipLaunchKernelGGL((bsa_fwd_f32_terms_kernel<kD, kPool, 1, kLse>), grid, blk, 0, s, a);
 }
 
 // Heads with few tiles are not worth splitting k and v (12 D bytes per key). At head dim 64:
@@ -927,11 +928,13 @@ int launch_terms(F32Args& a, int B, void* ws, int pool_cols, void* stream, const
   a.flags = reinterpret_cast<const uint4*>(t.flags);
   if (pool_cols == 32) launch_terms_pool<kD, 32>(a, s);
   else if (pool_cols == 64) launch_terms_pool<kD, 64>(a, s);
+  else if (a.pool_lse) launch_terms_pool<kD, 0, true>(a, s);
   else launch_terms_pool<kD, 0>(a, s);
   if (a.plain_after) {
     if (int rc = sa::check_launch(fn)) return rc;
     const dim3 grid((unsigned)(a.n_slots / kWavesF32)), blk(64 * kWavesF32);
-    hipLaunchKernelGGL((bsa_fwd_f32_kernel<kD, 0>), grid, blk, 0, s, a);
+    if (a.pool_lse) hipLaunchKernelGGL((bsa_fwd_f32_kernel<kD, 0, true>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((bsa_fwd_f32_kernel<kD, 0>), grid, blk, 0, s, a);
   }
   return sa::check_launch(fn);
 }
@@ -1007,10 +1010,12 @@ int launch_f32(const float* q, const int64_t q_strides[3], const float* k, const
   if (D == 64) {
     if (pool_cols == 32) hipLaunchKernelGGL((bsa_fwd_f32_kernel<64, 32>), grid, blk, 0, s, a);
     else if (pool_cols == 64) hipLaunchKernelGGL((bsa_fwd_f32_kernel<64, 64>), grid, blk, 0, s, a);
+    else if (pool_lse) hipLaunchKernelGGL((bsa_fwd_f32_kernel<64, 0, true>), grid, blk, 0, s, a);
     else hipLaunchKernelGGL((bsa_fwd_f32_kernel<64, 0>), grid, blk, 0, s, a);
   } else {
     if (pool_cols == 32) hipLaunchKernelGGL((bsa_fwd_f32_kernel<128, 32>), grid, blk, 0, s, a);
     else if (pool_cols == 64) hipLaunchKernelGGL((bsa_fwd_f32_kernel<128, 64>), grid, blk, 0, s, a);
+    else if (pool_lse) hipLaunchKernelGGL((bsa_fwd_f32_kernel<128, 0, true>), grid, blk, 0, s, a);
     else hipLaunchKernelGGL((bsa_fwd_f32_kernel<128, 0>), grid, blk, 0, s, a);
   }
   return sa::check_launch(fn);

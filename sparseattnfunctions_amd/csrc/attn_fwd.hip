@@ -108,8 +108,7 @@ struct FwdArgs {
   float* pool_r;
   int pool_ncol;
   int pool_lpad;
-  float* pool_lse;  // null: not stored. Without pooling: stored as the backward pass wants it (store_train_lse)
-  float* row_max;   // with a key bias: the offset that the stored log2-sum-exp2 is relative to
+  float* pool_lse;  // null: not stored. Without pooling: of a training call (store_train_lse)
   // Fused pooled map (pool_po non-null; pooled block size = kPool): after its item the wave
   // forms the Po rows of its own query rows, Po[i][c] = max over the rows r of query block i
   // of exp2(R[c][r] - lse[r]), each Po row then divided by its sum. Po rows and columns are
@@ -123,6 +122,7 @@ struct FwdArgs {
   // bound passes computes S = K16 (fp16(q * scale_log2))^T, already in the exp2 domain.
   const uint16_t* k16;
   const uint32_t* k16_norm2;
+  float* row_max;  // a training call's with a key bias: the offsets that the stored log2-sum-exp2 are relative to
 };
 
 // Item of a dispatch slot in ranges: as sa_attn_work_order places them, each XCD (group w of four
@@ -161,9 +161,12 @@ __device__ inline void store_train_lse(const FwdArgs& a, int64_t at, float m, fl
 // the groups of a work order that hold one item four times (sa_attn_work_order_long): a text row
 // over nkb blocks is a serial chain of 1.2 us per block, the whole launch where the other rows are
 // short or few ([1, 6, 17776, 64] with a fifth of the blocks 348 -> 171 us, [1, 24, 2944, 64] 81 -> 58).
+// kLse: a training call's form, which stores the rows' log2-sum-exp2. (A run-time test in every form cost those that
+// never store it up to 68 bytes of scratch.)
 template <bool kBias, bool kMask, int kPool, typename T = __bf16, int kD = 64, int kDV = kD, bool kK16 = false,
-          bool kShare = false>
+          bool kShare = false, bool kLse = false>
 __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs a) {
+  static_assert(!kLse || (!kMask && kPool == 0 && !kK16 && kDV == kD), "training: plain or key-bias lists");
   static_assert(!kK16 || (!kMask && kPool == 0 && std::is_same<T, __bf16>::value && kD == 64 && kDV == 64),
                 "fp16 scores: plain or key-bias bf16 lists at head dim 64");
   // With fp16 scores the key bias arrives multiplied by log2(e) (the entry point's scaled copy).
@@ -836,7 +839,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs 
       const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
       int row = qb * kBlock + r;
       bool store = row < a.Lq;
-      if (kPool == 0 && a.pool_lse && ch == 0) store_train_lse<kBias>(a, (int64_t)bh * a.pool_lpad + row, M, lsum, store);
+      if (kLse && ch == 0) store_train_lse<kBias>(a, (int64_t)bh * a.pool_lpad + row, M, lsum, store);
       if (store && a.o_rows) {
         row = a.o_rows[row];
         store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -893,8 +896,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs 
     }
     int row = qb * kBlock + 32 * g + col;
     bool store = row < a.Lq;
-    if (kPool == 0 && a.pool_lse && g == hh)
-      store_train_lse<kBias>(a, (int64_t)bh * a.pool_lpad + row, m[g], l_tot, store);
+    if (kLse && g == hh) store_train_lse<kBias>(a, (int64_t)bh * a.pool_lpad + row, m[g], l_tot, store);
     if (store && a.o_rows) {  // remapped layout: query i goes to out row o_rows[i]
       row = a.o_rows[row];
       store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -992,7 +994,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_fwd_kernel(FwdArgs 
 // Slots: the four slots of dispatch group w (the work order's unit, placed on XCD w % 8)
 // go to the workgroups x = 32 (w / 8) + 8 i + w % 8, i = 0..3, which the dispatcher places
 // on the same XCD.
-template <typename T, bool kK16 = false>
+template <typename T, bool kK16 = false, bool kLse = false>
 __global__ __launch_bounds__(128, 2) void bsa_fwd_pair_kernel(FwdArgs a) {
   static_assert(!kK16 || std::is_same<T, __bf16>::value, "fp16 scores take bf16 inputs");
   typedef Elem<T> E;
@@ -1327,7 +1329,7 @@ __global__ __launch_bounds__(128, 2) void bsa_fwd_pair_kernel(FwdArgs a) {
   const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
   int row = qb * kBlock + 32 * g + col;
   bool store = row < a.Lq;
-  if (a.pool_lse && hh == 0) store_train_lse<false>(a, (int64_t)bh * a.pool_lpad + row, m, l_tot, store);
+  if (kLse && hh == 0) store_train_lse<false>(a, (int64_t)bh * a.pool_lpad + row, m, l_tot, store);
   if (store && a.o_rows) {  // remapped layout: query i goes to out row o_rows[i]
     row = a.o_rows[row];
     store = (unsigned)row < (unsigned)a.o_dst_rows;
@@ -1556,13 +1558,13 @@ bool xcd_ranges_pay(int BH, int64_t n_items, int D, int max_cnt, int pool_cols, 
   return pool_cols == 32 || (from < n_slots / kWaves && max_cnt >= share_min((int)n_slots, from));
 }
 
-template <bool kBias, bool kMask, typename T, int kDV, bool kK16, int kPool = 0>
+template <bool kBias, bool kMask, typename T, int kDV, bool kK16, int kPool = 0, bool kLse = false>
 void launch_shared(FwdArgs a, int from, hipStream_t s) {
   a.shared_from = from;
   a.share_min = share_min(a.n_slots, from);  // (pooling lists are dense: their width has decided)
   const int64_t left = a.n_slots / kWaves - from;
   const dim3 g((unsigned)(from + (left + 7) / 8 * 32)), blk(64 * kWaves);
-  hipLaunchKernelGGL((bsa_fwd_kernel<kBias, kMask, kPool, T, 64, kDV, kK16, true>), g, blk, 0, s, a);
+  hipLaunchKernelGGL((bsa_fwd_kernel<kBias, kMask, kPool, T, 64, kDV, kK16, true, kLse>), g, blk, 0, s, a);
 }
 
 // One kernel variant per (tile masks, key bias, pooling columns): the caller has rejected
@@ -1570,6 +1572,8 @@ void launch_shared(FwdArgs a, int from, hipStream_t s) {
 template <typename T, int kD>
 void launch_variant(const FwdArgs& a, dim3 g, dim3 blk, hipStream_t s, bool mask, bool bias, int pool_cols,
                     bool v32 = false) {
+  // A training call (plain or key-bias lists); of one in key-range parts split_merge_kernel has the row sums.
+  const bool lse = a.pool_lse && pool_cols == 0 && a.n_parts == 1;
   if constexpr (kD == 64) {
     // (A sharing pooling kernel runs in ranges, for which n_slots has to hold whole ones.)
     const bool may_share = a.n_parts == 1 && (!pool_cols || (!mask && a.xcd_ranges));
@@ -1588,6 +1592,9 @@ void launch_variant(const FwdArgs& a, dim3 g, dim3 blk, hipStream_t s, bool mask
                       : launch_shared<false, false, T, 32, false>(a, from, s);
       }
       if (mask) return launch_shared<false, true, T, 64, false>(a, from, s);
+      if (lse)
+        return bias ? launch_shared<true, false, T, 64, false, 0, true>(a, from, s)
+                    : launch_shared<false, false, T, 64, false, 0, true>(a, from, s);
       return bias ? launch_shared<true, false, T, 64, false>(a, from, s)
                   : launch_shared<false, false, T, 64, false>(a, from, s);
     }
@@ -1616,7 +1623,8 @@ void launch_variant(const FwdArgs& a, dim3 g, dim3 blk, hipStream_t s, bool mask
           return;
         }
       }
-      hipLaunchKernelGGL((bsa_fwd_pair_kernel<T>), pg, dim3(128), 0, s, a);
+      if (lse) hipLaunchKernelGGL((bsa_fwd_pair_kernel<T, false, true>), pg, dim3(128), 0, s, a);
+      else hipLaunchKernelGGL((bsa_fwd_pair_kernel<T>), pg, dim3(128), 0, s, a);
       return;
     }
   }
@@ -1625,8 +1633,15 @@ void launch_variant(const FwdArgs& a, dim3 g, dim3 blk, hipStream_t s, bool mask
     else if (pool_cols == 64) hipLaunchKernelGGL((bsa_fwd_kernel<false, true, 64, T, kD>), g, blk, 0, s, a);
     else hipLaunchKernelGGL((bsa_fwd_kernel<false, true, 0, T, kD>), g, blk, 0, s, a);
   } else if (bias) {
-    hipLaunchKernelGGL((bsa_fwd_kernel<true, false, 0, T, kD>), g, blk, 0, s, a);
+    if (lse) hipLaunchKernelGGL((bsa_fwd_kernel<true, false, 0, T, kD, kD, false, false, true>), g, blk, 0, s, a);
+    else hipLaunchKernelGGL((bsa_fwd_kernel<true, false, 0, T, kD>), g, blk, 0, s, a);
   } else {
+    if constexpr (kD == 64) {  // (at 128 such a training call runs pairs)
+      if (lse) {
+        hipLaunchKernelGGL((bsa_fwd_kernel<false, false, 0, T, kD, kD, false, false, true>), g, blk, 0, s, a);
+        return;
+      }
+    }
     if (pool_cols == 32) hipLaunchKernelGGL((bsa_fwd_kernel<false, false, 32, T, kD>), g, blk, 0, s, a);
     else if (pool_cols == 64) hipLaunchKernelGGL((bsa_fwd_kernel<false, false, 64, T, kD>), g, blk, 0, s, a);
     else hipLaunchKernelGGL((bsa_fwd_kernel<false, false, 0, T, kD>), g, blk, 0, s, a);
