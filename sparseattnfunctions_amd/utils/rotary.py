@@ -164,7 +164,8 @@ class VideoRotary:
             if positions is None:
                 positions = video_positions(self.geometry)
             stream = torch.cuda.current_stream(device)
-            table = rotary_table(positions.to(device), self.axes, self.theta, self.scaling)
+            with torch.inference_mode(False):  # (an inference tensor could not be saved for a later backward pass)
+                table = rotary_table(positions.to(device), self.axes, self.theta, self.scaling)
             stream.synchronize()
             made = self._tables[device] = (table, stream)
         table, stream = made

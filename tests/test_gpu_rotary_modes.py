@@ -1,0 +1,40 @@
+"""Rotary positions across autograd's modes."""
+import pytest
+import torch
+
+from conftest import case
+from sparseattnfunctions_amd.block_mask_attn import BlockSparseAttention
+from sparseattnfunctions_amd.utils.rotary import VideoRotary, video_positions
+from sparseattnfunctions_amd.workloads import Geometry
+
+pytestmark = pytest.mark.gpu
+
+GEOM = Geometry(text_len=70, T=2, Hp=6, Wp=10)
+
+
+def _qkv(dev, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(1, 2, GEOM.L, 64, generator=g).bfloat16().to(dev) for _ in range(4)]
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_table_made_in_inference_mode_serves_training(dev, given):
+    # A validation pass before the first step: the cached table must not be an inference tensor.
+    case(f"table made in inference mode, positions given: {given}")
+    q, k, v, do = _qkv(dev)
+    positions = None
+    if given:
+        with torch.inference_mode():
+            positions = video_positions(GEOM, device=dev)
+    rotary = VideoRotary(GEOM, positions=positions)
+    proc = BlockSparseAttention(64, keep_ratio=0.6, geometry=GEOM, trainable=True, rotary=rotary)
+    with torch.inference_mode():
+        seen = proc(q, k, v)
+    assert not rotary.table(dev).is_inference()
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = proc(*leaves)
+    grads = torch.autograd.grad(out, leaves, do)
+    assert torch.equal(out, seen)
+    fresh = BlockSparseAttention(64, keep_ratio=0.6, geometry=GEOM, trainable=True, rotary=VideoRotary(GEOM))
+    want = torch.autograd.grad(fresh(*leaves), leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
