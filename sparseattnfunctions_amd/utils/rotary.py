@@ -175,7 +175,8 @@ class VideoRotary:
         return table
 
     def __call__(self, q, k):
-        return apply_rotary(q, k, self.table(q.device), layout=self.layout, skip=self.geometry.text_len)
+        q_out, k_out = apply_rotary(q, k, self.table(q.device), layout=self.layout, skip=self.geometry.text_len)
+        return (q_out.detach() if q_out.requires_grad and not q.requires_grad else q_out), k_out
 
 
 def _check(q, k, table, layout, skip, rows):
@@ -258,7 +259,10 @@ class _ApplyRotary(torch.autograd.Function):
         ctx.save_for_backward(table, rows)
         ctx.args = layout, skip, inverse
         ctx.set_materialize_grads(False)
-        return _turned(q, k, table, layout, skip, rows, inverse)
+        out = _turned(q, k, table, layout, skip, rows, inverse)
+        if k is not None and not ctx.needs_input_grad[1]:
+            ctx.mark_non_differentiable(out[1])
+        return out
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -285,7 +289,8 @@ def apply_rotary(q, k, table, layout: str = "interleaved", skip: int = 0, rows: 
     at most D. Token t takes table row t - skip, and the first `skip` tokens (text) stay as they are;
     or, with `rows` (int32 [L], or [B, L] for sequences at places of their own), row rows[t], and a
     token whose entry lies outside the table stays as it is: permuted layouts, single new tokens,
-    padding. `inverse` turns back."""
+    padding. `inverse` turns back. Where autograd follows q and not k, it does not follow the turned k either;
+    the other way round the turned q counts as followed (detach it, and nobody computes its gradient)."""
     _check(q, k, table, layout, skip, rows)
     rows = rows if rows is None or rows.stride(-1) == 1 else rows.contiguous()
     if _followed(q) or _followed(k):

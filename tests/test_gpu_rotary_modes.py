@@ -4,7 +4,7 @@ import torch
 
 from conftest import case
 from sparseattnfunctions_amd.block_mask_attn import BlockSparseAttention
-from sparseattnfunctions_amd.utils.rotary import VideoRotary, video_positions
+from sparseattnfunctions_amd.utils.rotary import VideoRotary, apply_rotary, video_positions
 from sparseattnfunctions_amd.workloads import Geometry
 
 pytestmark = pytest.mark.gpu
@@ -38,3 +38,28 @@ def test_table_made_in_inference_mode_serves_training(dev, given):
     fresh = BlockSparseAttention(64, keep_ratio=0.6, geometry=GEOM, trainable=True, rotary=VideoRotary(GEOM))
     want = torch.autograd.grad(fresh(*leaves), leaves, do)
     assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+@pytest.mark.parametrize("trained", ["q", "k"])
+def test_a_frozen_side_has_no_gradient(dev, trained):
+    # Only q or only k is followed: the turned other one is not, so that the attention behind it computes no gradient of it.
+    case(f"only {trained} followed")
+    q, k, v, do = _qkv(dev, 1)
+    rotary = VideoRotary(GEOM)
+    want = rotary(q, k)
+    leaf = (q if trained == "q" else k).requires_grad_()
+    turned = rotary(q, k)
+    assert [t.requires_grad for t in turned] == [trained == "q", trained == "k"]
+    assert all(torch.equal(a, b) for a, b in zip(turned, want))
+    if trained == "q":
+        assert not apply_rotary(q, k, rotary.table(dev), skip=GEOM.text_len)[1].requires_grad
+    proc = BlockSparseAttention(64, keep_ratio=0.6, geometry=GEOM, trainable=True, rotary=rotary)
+    out = proc(q, k, v)
+    wanted = [f is not None for f, _ in out.grad_fn.next_functions[:3]]
+    assert wanted == [trained == "q", trained == "k", False]
+    (only,) = torch.autograd.grad(out, leaf, do)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    both = torch.autograd.grad(proc(*leaves), leaves, do)
+    assert torch.equal(only, both[0 if trained == "q" else 1])
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in rotary(q, k))
