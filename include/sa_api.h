@@ -285,8 +285,11 @@ int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
  *             is a q_idx and a key_bias): the query rows' statistics, the transposed lists, sums of lists split over
  *             workgroups.
  * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv and no q_idx,
- * sm_scale at least 1e-30.
+ * sm_scale at least 1e-30. sa_block_sparse_bwd_check says whether a call is within these limits before its forward
+ * pass: SA_ERR_UNSUPPORTED, or SA_OK. It reads the sizes, dtype, strides, max_cnt and sm_scale, and whether there is
+ * a key_bias, q_idx, dk and dv.
  */
+int sa_block_sparse_bwd_check(const sa_attn_train* call);
 int sa_block_sparse_bwd_workspace(const sa_attn_train* call, int64_t* bytes);
 int sa_block_sparse_bwd(const sa_attn_train* call, void* stream);
 

@@ -79,6 +79,7 @@ _PROTOTYPES = {
     "sa_block_sparse_fwd_lse": (_I, [ctypes.POINTER(AttnTrain), _P]),
     "sa_kv_list_transpose": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
     "sa_block_sparse_bwd_workspace": (_I, [ctypes.POINTER(AttnTrain), _I64P]),
+    "sa_block_sparse_bwd_check": (_I, [ctypes.POINTER(AttnTrain)]),
     "sa_block_sparse_bwd": (_I, [ctypes.POINTER(AttnTrain), _P]),
     "sa_rotary_table": (_I, [_P, _I, _I64P, ctypes.c_int64, _I, _P, _P, _P, _P, _P]),
     "sa_rotary_apply": (

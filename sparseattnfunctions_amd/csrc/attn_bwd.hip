@@ -1099,7 +1099,35 @@ int check_train(const sa_attn_train* t, const char* fn) {
   return SA_OK;
 }
 
+// What the passes cannot take, of a call whose sizes are right.
+int check_limits(const sa_attn_train* t, const char* fn) {
+  SA_REQUIRE(std::isfinite(t->sm_scale) && t->sm_scale > 0.f, "%s: sm_scale must be finite and > 0", fn);
+  // (the key pass takes the rows' sums in units of the scores, lse / sm_scale)
+  if (t->sm_scale < 1e-30f) return sa::fail(SA_ERR_UNSUPPORTED, "%s: sm_scale %g below 1e-30", fn, t->sm_scale);
+  if (t->dtype == SA_DTYPE_F32 && t->key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
+  // Streamed rows are copied through 32-bit buffer offsets relative to each head's first row.
+  const int size = t->dtype == SA_DTYPE_F32 ? 4 : 2;
+  const int64_t rows[4] = {t->Lq, t->Lk, t->Lk, t->Lq};
+  const int at[4] = {0, 1, 2, 4};
+  for (int i = 0; i < 4; ++i) {
+    const int64_t stride = t->strides[3 * at[i] + 2];
+    if (stride < 0 || stride > INT_MAX || (rows[i] + kBlk) * stride * size + 2 * t->D > INT_MAX)
+      return sa::fail(SA_ERR_UNSUPPORTED, "%s: rows of one head span more than 2 GiB", fn);
+  }
+  // (sa_kv_list_transpose's)
+  if ((t->dk || t->dv) && !t->q_idx && (t->max_cnt > 65535 || sa::cdiv(t->Lq, kBlk) * (int64_t)t->max_cnt >= (1LL << 31)))
+    return sa::fail(SA_ERR_UNSUPPORTED, "%s: lists of %d entries", fn, t->max_cnt);
+  return SA_OK;
+}
+
 }  // namespace
+
+extern "C" int sa_block_sparse_bwd_check(const sa_attn_train* t) {
+  const char* fn = "sa_block_sparse_bwd_check";
+  if (int rc = check_train(t, fn)) return rc;
+  if (int rc = check_limits(t, fn)) return rc;
+  return sa::ok();
+}
 
 extern "C" int sa_block_sparse_bwd_workspace(const sa_attn_train* t, int64_t* bytes) {
   const char* fn = "sa_block_sparse_bwd_workspace";
@@ -1115,14 +1143,11 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   const int B = t->B, H = t->H, Lq = t->Lq, Lk = t->Lk, D = t->D;
   SA_REQUIRE(t->q && t->k && t->v && t->out && t->dout && t->lse && t->kv_idx && t->kv_cnt && !t->q_idx == !t->q_cnt,
              "%s: null pointer", fn);
-  SA_REQUIRE(std::isfinite(t->sm_scale) && t->sm_scale > 0.f, "%s: sm_scale must be finite and > 0", fn);
-  // (the key pass takes the rows' sums in units of the scores, lse / sm_scale)
-  if (t->sm_scale < 1e-30f) return sa::fail(SA_ERR_UNSUPPORTED, "%s: sm_scale %g below 1e-30", fn, t->sm_scale);
+  if (int rc = check_limits(t, fn)) return rc;
   const bool f32 = t->dtype == SA_DTYPE_F32;
-  if (f32 && t->key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
   SA_REQUIRE(!t->key_bias || t->row_max, "%s: key_bias without row_max", fn);
   const int nqb = sa::cdiv(Lq, kBlk), nkb = sa::cdiv(Lk, kBlk);
-  const int per16 = f32 ? 4 : 8, size = f32 ? 4 : 2;
+  const int per16 = f32 ? 4 : 8;
   const void* ptrs[8] = {t->q, t->k, t->v, t->out, t->dout, t->dq, t->dk, t->dv};
   const int64_t* strides = t->strides;
   for (int i = 0; i < 8; ++i) {
@@ -1132,12 +1157,6 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
       if (ptrs[i] && strides[3 * i + j] % per16 != 0)
         return sa::fail(SA_ERR_UNSUPPORTED, "%s: strides must be multiples of %d elements", fn, per16);
   }
-  // Streamed rows are copied through 32-bit buffer offsets relative to each head's first row.
-  const int64_t rows[4] = {Lq, Lk, Lk, Lq};
-  const int at[4] = {0, 1, 2, 4};
-  for (int i = 0; i < 4; ++i)
-    if (strides[3 * at[i] + 2] < 0 || (rows[i] + kBlk) * strides[3 * at[i] + 2] * size + 2 * D > INT_MAX)
-      return sa::fail(SA_ERR_UNSUPPORTED, "%s: rows of one head span more than 2 GiB", fn);
   Layout l = layout(*t);
   SA_REQUIRE(t->workspace && reinterpret_cast<uintptr_t>(t->workspace) % 256 == 0,
              "%s: workspace null or not 256-byte aligned", fn);

@@ -196,6 +196,19 @@ class _Plan:
         _lib.check(_lib.load().sa_block_sparse_bwd_workspace(args, ctypes.byref(n)), "sa_block_sparse_bwd_workspace")
         args.q_idx = args.key_bias = None
         self.backward_bytes = n.value
+        # Why the backward pass refuses such calls, without and with dk or dv: nobody is to learn it there.
+        self.refusals = []
+        args.q_idx, args.key_bias = 1 if keys else None, 1 if biased else None
+        for wanted in (None, 1):
+            args.dk = wanted
+            rc = _lib.load().sa_block_sparse_bwd_check(args)
+            self.refusals.append(_lib.load().sa_last_error().decode() if rc == _lib.SA_ERR_UNSUPPORTED else None)
+        args.q_idx = args.key_bias = args.dk = None
+
+    def check_backward(self, needs):
+        refusal = self.refusals[bool(needs[1] or needs[2])]
+        if any(needs[:3]) and refusal is not None:
+            raise NotImplementedError(refusal)
 
 
 _plan = functools.lru_cache(maxsize=1024)(_Plan)
@@ -247,6 +260,8 @@ def _backward(plan: _Plan, args: _lib.AttnTrain, dout, needs):
     plain = dout.is_contiguous() and dout.data_ptr() % 16 == 0
     if not plain:
         dout = _rows16(dout)
+        if (dout.shape[2] + BLOCK) * dout.stride(2) * dout.element_size() >= 1 << 30:  # (rows far apart: 32-bit offsets)
+            dout = dout.contiguous()
         args.strides[12:15] = dout.stride()[:3]
     args.dout = dout.data_ptr()
     device = dout.device
@@ -332,9 +347,11 @@ def _places(q, k, v, out, kv_idx, kv_cnt, lse, key_bias):
 
 class _TrainAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, kv, sm_scale, key_bias, n_text_blocks):
+    def forward(ctx, q, k, v, kv, sm_scale, key_bias, n_text_blocks, followed):
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
         ctx.plan, ctx.args = _describe(q, k, v, kv, sm_scale, key_bias, n_text_blocks)
+        if followed:
+            ctx.plan.check_backward(ctx.needs_input_grad)
         out, lse = _forward(ctx.plan, ctx.args, q)
         ctx.args.mask = None  # (read by the forward call alone)
         ctx.save_for_backward(q, k, v, out, kv.idx, kv.cnt, lse, key_bias)
@@ -355,7 +372,7 @@ class _TrainAttention(torch.autograd.Function):
             _set(args, q=q, k=k, v=v, out=out)
             _set_lists(args, ctx.plan, kv_idx, kv_cnt, lse)
             _set_bias(args, key_bias)
-        return (*_backward(ctx.plan, args, dout, ctx.needs_input_grad), None, None, None, None)
+        return (*_backward(ctx.plan, args, dout, ctx.needs_input_grad), None, None, None, None, None)
 
 
 class _NoKeys(torch.autograd.Function):
@@ -386,7 +403,7 @@ def block_sparse_attention_train(q, k, v, kv: KVList, sm_scale: float, key_bias:
     dispatch orders), and leaves that no eager graph holds: autograd ties a leaf's gradient to the
     stream of the leaf's first use, and its backward pass outside the capture would end the process."""
     key_bias = _check_inputs(q, k, v, kv, key_bias)
-    return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
+    return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks), torch.is_grad_enabled())
 
 
 def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Optional[torch.Tensor] = None,
@@ -416,4 +433,4 @@ def block_sparse_train_fn(q, k, v, block_sparse_mask, sm_scale, key_bias: Option
         _lib.require_gpu(q, k, v, block_sparse_mask)
         kv, _ = cell_kv_list(block_sparse_mask, B, H, Lq, Lk, int(BLOCK_M), int(BLOCK_N))
     key_bias = _check_inputs(q, k, v, kv, key_bias)
-    return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks))
+    return _TrainAttention.apply(q, k, v, kv, float(sm_scale), key_bias, int(n_text_blocks), torch.is_grad_enabled())

@@ -173,3 +173,19 @@ def test_biased_calls_need_the_rows_offsets():
         assert lib.sa_block_sparse_bwd_workspace(call(key_bias=bias, q_idx=256), ctypes.byref(n)) == 0
         sizes.append(n.value)
     assert sizes == [2 * 128 * 4, 2 * 256 * 4]
+
+
+def test_backward_limits_are_known_before_the_forward_pass():
+    lib = _lib.load()
+
+    def check(stride=64, **changed):
+        t = _lib.AttnTrain(**{**dict(dtype=0, B=1, H=1, Lq=40, Lk=40, D=64, max_cnt=2, sm_scale=0.125), **changed})
+        t.strides[:] = [0, 0, stride] * 8
+        return lib.sa_block_sparse_bwd_check(t)
+
+    assert check() == check(sm_scale=1e-30, dk=256, dv=256) == check(max_cnt=65536) == 0
+    assert check(max_cnt=65536, dk=256, q_idx=256) == 0
+    for bad in (dict(sm_scale=1e-31), dict(dtype=2, key_bias=256), dict(stride=1 << 24), dict(stride=-64), dict(D=96),
+                dict(stride=1 << 62), dict(max_cnt=65536, dk=256), dict(max_cnt=65536, dv=256)):
+        assert check(**bad) == _lib.SA_ERR_UNSUPPORTED, bad
+    assert check(Lq=0) == check(sm_scale=0.0) == check(sm_scale=math.nan) == lib.sa_block_sparse_bwd_check(None) == _lib.SA_ERR_INVALID
