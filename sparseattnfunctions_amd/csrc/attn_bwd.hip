@@ -53,6 +53,12 @@ namespace {
 constexpr int kBlk = 64;   // rows per block of either side
 constexpr int kStep = 32;  // streamed rows per step, own rows per wave
 constexpr int kMostLast = 128;
+// fp16 holds normal numbers from 2^-14, which the probabilities of an even row fall short of over more than 16 384 keys:
+// where lists may be that long, P is rounded to the type with this factor, which dv loses at the end, so that they are
+// normal down to 2^-26. (dS has the loss's scale.) A product an element: the key pass of [1, 15, 8229, 128] with 0.35 of
+// the blocks takes 374 us without and 389 with.
+constexpr float kPScale = 4096.f;
+constexpr int64_t kPNormalKeys = 16384;
 constexpr float kFarOffset = 64.f;  // (in log2 units)
 
 struct BwdArgs {
@@ -84,6 +90,7 @@ struct BwdArgs {
   float sm_scale;
   float scale_log2;     // sm_scale * log2(e)
   float inv_scale_log2;
+  float dv_scale;       // 1 / the factor of P (kPScale or 1)
   const float* lse;     // query pass: [bh][64 * query blocks]
   const float* row_max; // with a bias, alike: the rows' offsets
   // [bh][2 * query blocks][2][32]: per 32 query rows their -lse / scale_log2, then their -delta. With a bias
@@ -206,8 +213,8 @@ __device__ inline const __attribute__((address_space(4))) int32_t* bwd_list(cons
 }
 
 // kParts: pairs per workgroup, each on its share of the item's list; their sums are added in LDS, in
-// order, at the end.
-template <bool kKeys, bool kBias, typename T, int kD, int kParts>
+// order, at the end. kScaleP: P has the factor kPScale.
+template <bool kKeys, bool kBias, typename T, int kD, int kParts, bool kScaleP = false>
 __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel(BwdArgs a) {
   typedef Elem<T> E;
   typedef typename E::v8 v8;
@@ -459,7 +466,7 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
       for (int e = 0; e < 16; e += 2) {
         const float p0 = fast_exp2(kBias ? fmaf(S[e], scale, add) : S[e] * a.scale_log2);
         const float p1 = fast_exp2(kBias ? fmaf(S[e + 1], scale, add) : S[e + 1] * a.scale_log2);
-        Pp[e >> 1] = E::pack(p0, p1);
+        Pp[e >> 1] = kScaleP ? E::pack(p0 * kPScale, p1 * kPScale) : E::pack(p0, p1);
         Sp[e >> 1] = E::pack(p0 * dP[e], p1 * dP[e + 1]);
       }
     } else {
@@ -537,7 +544,7 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   for (int x = 0; x < kAcc; ++x) {
     uint16_t* g = static_cast<uint16_t*>(x == 0 ? a.grad_a : a.grad_b);
     const int64_t sb = x == 0 ? a.ga_sb : a.gb_sb, sh = x == 0 ? a.ga_sh : a.gb_sh, sl = x == 0 ? a.ga_sl : a.gb_sl;
-    const float f = x == 0 ? a.sm_scale : 1.f;
+    const float f = x == 0 ? a.sm_scale : kScaleP ? a.dv_scale : 1.f;
     if constexpr (kParts == 1) {
       if (g && own_row < a.L_own) {
         uint16_t* p = g + b * sb + h * sh + (int64_t)own_row * sl + 4 * hh;
@@ -907,7 +914,7 @@ __global__ __launch_bounds__(256) void bwd_merge_kernel(BwdArgs a, int D) {
   if (!g) return;
   g += b * (x == 0 ? a.ga_sb : a.gb_sb) + h * (x == 0 ? a.ga_sh : a.gb_sh);
   const int64_t sl = x == 0 ? a.ga_sl : a.gb_sl;
-  const float f = x == 0 ? a.sm_scale : 1.f;
+  const float f = x == 0 ? a.sm_scale : a.dv_scale;
   const int64_t n = (int64_t)kBlk * D;
   const float* from = a.partial + ((int64_t)place * a.splits * kAcc + x) * n;
   const int t = blockIdx.z * 256 + threadIdx.x;
@@ -944,6 +951,13 @@ unsigned workgroups(const BwdArgs& a) {
 template <bool kKeys, typename T, int kD, int kParts>
 void launch_parts(const BwdArgs& a, hipStream_t s) {
   const dim3 grid(workgroups(a)), blk(128 * kParts);
+  if constexpr (kKeys && std::is_same<T, _Float16>::value) {
+    if (a.dv_scale != 1.f) {
+      if (a.bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, kParts, true>), grid, blk, 0, s, a);
+      else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, kParts, true>), grid, blk, 0, s, a);
+      return;
+    }
+  }
   if (a.bias) hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, true, T, kD, kParts>), grid, blk, 0, s, a);
   else hipLaunchKernelGGL((bsa_bwd_kernel<kKeys, false, T, kD, kParts>), grid, blk, 0, s, a);
 }
@@ -1182,6 +1196,8 @@ extern "C" int sa_block_sparse_bwd(const sa_attn_train* t, void* stream) {
   a.sm_scale = t->sm_scale;
   a.scale_log2 = t->sm_scale * kLog2e;
   a.inv_scale_log2 = 1.f / a.scale_log2;
+  // (a block listed more than once counts as often)
+  a.dv_scale = t->dtype == SA_DTYPE_F16 && (int64_t)t->max_cnt * kBlk > kPNormalKeys ? 1.f / kPScale : 1.f;
   a.lse = t->lse;
   a.row_max = t->row_max;
   a.stats = reinterpret_cast<float*>(ws);
