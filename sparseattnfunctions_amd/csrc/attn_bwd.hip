@@ -522,16 +522,16 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
   bool far0 = far_of(rb, 0), far1;
   int rb_next = block_of(1);
   for (int i = 0; i < per_part; i += 2) {
-    // This wave's copies of step i have landed, then everyone's; every wave is done with step i - 1,
-    // whose stage the copies of step i + 1 overwrite.
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    // This wave's copies of step i have landed, then everyone's; every wave is done with step i - 1 (its reads of LDS have
+    // returned), whose stage the copies of step i + 1 overwrite.
+    __builtin_amdgcn_s_waitcnt(kWaitVmLgkm0);
     wg_barrier();
     issue(rb_next, i + 1, t1, (lds_u8*)stat1);
     far1 = far_of(rb_next, i + 1);
     compute(rb, i, far0, t0, stat0);
     if (i + 1 >= per_part) break;
     rb = block_of(i + 2);
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    __builtin_amdgcn_s_waitcnt(kWaitVmLgkm0);
     wg_barrier();
     issue(rb, i + 2, t0, (lds_u8*)stat0);
     far0 = far_of(rb, i + 2);

@@ -171,6 +171,7 @@ __device__ __forceinline__ void lgkm_wait_pair(int n, sa_u32x2v& a, sa_u32x2v& b
 // s_waitcnt encodings (gfx9): vmcnt in bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8.
 constexpr int waitcnt_vm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0F70; }
 constexpr int kWaitLgkm0 = 0xC07F;
+constexpr int kWaitVmLgkm0 = 0x0070;
 
 // Workgroup barrier with no memory fence: the waits before it are explicit (a fence would
 // also wait for the copies in flight). The clobber keeps the compiler from moving LDS
