@@ -70,6 +70,15 @@ class _MaskLists:
         self.cnt = None
 
 
+def _check_lists(kv, B, H, nqb, nkb):
+    if (kv.B, kv.H, kv.nqb, kv.nkb) != (B, H, nqb, nkb) or kv.cnt.numel() != B * H * nqb or kv.idx.dim() != 2 \
+            or kv.idx.shape[0] != B * H * nqb:
+        raise ValueError(f"kv lists of {kv.B} x {kv.H} x {kv.nqb} x {kv.nkb} blocks, expected {B} x {H} x {nqb} x {nkb}")
+    if kv.idx.dtype != torch.int32 or kv.cnt.dtype != torch.int32 or not kv.idx.is_contiguous() \
+            or not kv.cnt.is_contiguous():
+        raise ValueError("kv lists must be contiguous int32 tensors")
+
+
 def _check_inputs(q, k, v, kv, key_bias):
     """key_bias expanded. kv: a caller's lists, or ones for these shapes (_MaskLists)."""
     own_lists = type(kv) is _MaskLists
@@ -94,14 +103,8 @@ def _check_inputs(q, k, v, kv, key_bias):
     if D not in (64, 128):
         raise NotImplementedError(f"head_dim {D} (64 or 128)")
     nqb, nkb = (Lq + BLOCK - 1) // BLOCK, (Lk + BLOCK - 1) // BLOCK
-    if own_lists:
-        pass
-    elif (kv.B, kv.H, kv.nqb, kv.nkb) != (B, H, nqb, nkb) or kv.cnt.numel() != B * H * nqb or kv.idx.dim() != 2 \
-            or kv.idx.shape[0] != B * H * nqb:
-        raise ValueError(f"kv lists of {kv.B} x {kv.H} x {kv.nqb} x {kv.nkb} blocks, expected {B} x {H} x {nqb} x {nkb}")
-    elif kv.idx.dtype != torch.int32 or kv.cnt.dtype != torch.int32 or not kv.idx.is_contiguous() \
-            or not kv.cnt.is_contiguous():
-        raise ValueError("kv lists must be contiguous int32 tensors")
+    if not own_lists:
+        _check_lists(kv, B, H, nqb, nkb)
     if key_bias is not None:
         if q.dtype == torch.float32:
             raise NotImplementedError("fp32 inputs: plain block lists only (no key_bias)")
@@ -289,6 +292,9 @@ def transpose_kv_list(kv: KVList) -> Tuple[torch.Tensor, torch.Tensor]:
     key block, ascending (`sa_kv_list_transpose`); key block j of a head has entries
     q_idx[q_beg[j]:q_beg[j + 1]] of the head's row. The backward pass makes its own."""
     _lib.require_gpu(kv.idx, kv.cnt)
+    if kv.cnt.device != kv.idx.device:
+        raise ValueError("the lists must be on one device")
+    _check_lists(kv, kv.B, kv.H, kv.nqb, kv.nkb)
     BH = kv.B * kv.H
     beg = torch.empty(BH, kv.nkb + 1, dtype=torch.int32, device=kv.idx.device)
     idx = torch.empty(BH, kv.nqb * kv.max_cnt, dtype=torch.int32, device=kv.idx.device)

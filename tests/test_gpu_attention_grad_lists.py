@@ -2,6 +2,7 @@
 special ways: last round by length, split text blocks, split remainders, split lists. Their key side is transposed by the
 backward call; a mask's both sides are made by the forward call. Both lists are ascending, so all results agree bit for
 bit."""
+import dataclasses
 import math
 
 import pytest
@@ -11,7 +12,8 @@ from conftest import case
 from grad_reference import check, reference, unit
 from sparseattnfunctions_amd._kv import kv_list_from_mask
 from sparseattnfunctions_amd.utils.block_sparse_attn_grad import (
-    block_sparse_attention_backward, block_sparse_attention_lse, block_sparse_attention_train, block_sparse_train_fn)
+    block_sparse_attention_backward, block_sparse_attention_lse, block_sparse_attention_train, block_sparse_train_fn,
+    transpose_kv_list)
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +67,14 @@ def test_lists_and_masks_agree(dev, name):
     some = slice(H - 2, H)
     check([x[:, some] for x in got], reference(*(t[:, some] for t in (q, k, v, do, mask)), 0.125, bias=bias),
           norm=1.5 * unit(dtype) if dtype != FP32 else 64 * 2.0 ** -24)
+
+
+def test_transposing_refuses_lists_of_other_sizes(dev):
+    # (the kernel would read past them)
+    case("transposed lists, refusals")
+    kv = kv_list_from_mask(torch.ones(1, 2, 3, 4, dtype=torch.bool, device=dev), 1, 2, 3, 4)
+    assert transpose_kv_list(kv)[0].tolist() == [[0, 3, 6, 9, 12]] * 2
+    for bad in (dict(idx=kv.idx.long()), dict(cnt=kv.cnt.long()), dict(cnt=kv.cnt[:5]), dict(idx=kv.idx[:4]), dict(H=3),
+                dict(nqb=4), dict(idx=kv.idx.flatten()), dict(idx=kv.idx[:, ::2]), dict(cnt=kv.cnt.cpu())):
+        with pytest.raises(ValueError):
+            transpose_kv_list(dataclasses.replace(kv, **bad))
