@@ -322,6 +322,7 @@ extern "C" int sa_rotary_apply(int dtype, const void* q, void* q_out, const void
   SA_REQUIRE(!k == !k_out, "%s: k without its output", fn);
   SA_REQUIRE(B > 0 && H > 0 && (!k || Hk > 0) && L > 0 && D > 0, "%s: bad shape B=%d H=%d Hk=%d L=%d D=%d", fn, B, H, Hk,
              L, D);
+  SA_REQUIRE(L <= INT_MAX - 255, "%s: L=%d", fn, L);  // (rounded up to a workgroup's tokens)
   SA_REQUIRE(D <= 2 * kMaxPairs, "%s: head dim %d (at most %d)", fn, D, 2 * kMaxPairs);
   SA_REQUIRE(n_rows > 0 && pairs > 0 && 2 * pairs <= D, "%s: a table of %d rows of %d pairs for head dim %d", fn, n_rows,
              pairs, D);

@@ -165,6 +165,9 @@ class _Plan:
     def __init__(self, dtype, device, q_shape, Lk, q_strides, k_strides, v_strides, max_cnt, row_blocks, biased, sm_scale,
                  n_text_blocks, keys):
         B, H, Lq, D = q_shape
+        if max(B, H, Lq, Lk, max_cnt) >= 2 ** 31 - BLOCK:
+            raise ValueError(f"B={B} H={H} Lq={Lq} Lk={Lk}: sizes of 32 bits")
+        n_text_blocks = min(n_text_blocks, max(Lq, Lk))  # (no head has more)
         self.keys, self.biased = keys, biased  # keys: with key blocks' lists (_MaskLists)
         nqb, nkb = math.ceil(Lq / BLOCK), math.ceil(Lk / BLOCK)
         n_items = B * H * nqb

@@ -28,6 +28,7 @@ from .. import _lib
 
 LAYOUTS = ("interleaved", "half")
 MAX_PAIRS = 128
+MAX_SIZE = 2 ** 31 - 256  # of a dimension (`sa_rotary_apply` takes 32-bit ones)
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 _SCALINGS = {"linear": {"factor"}, "ntk": {"factor"},
              "yarn": {"factor", "original_length", "beta_fast", "beta_slow"}}
@@ -195,6 +196,9 @@ def _check(q, k, table, layout, skip, rows):
     B, _, L, D = q.shape
     if k is not None and (k.shape[0], *k.shape[2:]) != (B, L, D):
         raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)}")
+    if q.numel() > MAX_SIZE < max(q.shape) or (k is not None and k.numel() > MAX_SIZE < max(k.shape)) \
+            or (table.dim() and table.shape[0] > MAX_SIZE):
+        raise ValueError(f"q, k and table may have at most {MAX_SIZE} tokens and rows")
     if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous():
         raise ValueError("table must be a contiguous fp32 [rows, pairs, 2] tensor (rotary_table)")
     if table.requires_grad:

@@ -5,7 +5,8 @@ import torch
 from conftest import case
 from sparseattnfunctions_amd._kv import KVList
 from sparseattnfunctions_amd.block_mask_attn import dense_kv_list
-from sparseattnfunctions_amd.utils.block_sparse_attn_grad import block_sparse_attention_train, block_sparse_train_fn
+from sparseattnfunctions_amd.utils.block_sparse_attn_grad import (_plan, block_sparse_attention_train,
+                                                                  block_sparse_train_fn)
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,17 @@ def test_far_rows(dev):
     grads = [torch.autograd.grad(block_sparse_attention_train(*leaves, kv, 0.125), leaves, do)
              for do in (far.clone(memory_format=torch.contiguous_format), far)]
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_sizes_past_32_bits(dev):
+    # A length cut to 32 bits would attend to 64 of the keys. (The lists' own checks come first, so the plan of such a call
+    # is asked for directly.) More text blocks than a head has blocks mean all of them.
+    case("sizes past 32 bits")
+    plain = (64 * 64, 64 * 64, 64, 1)
+    for shape, Lk in (((1, 1, 64, 64), 2 ** 32 + 64), ((1, 1, 2 ** 32 + 64, 64), 64), ((2 ** 32 + 1, 1, 64, 64), 64)):
+        with pytest.raises(ValueError, match="32 bits"):
+            _plan(BF16, dev, torch.Size(shape), Lk, plain, plain, plain, 1, 0.0, False, 0.125, 0, False)
+    leaves = _leaves(dev)
+    mask = torch.ones(1, 1, 1, 1, dtype=torch.bool, device=dev)
+    want = block_sparse_train_fn(*leaves, mask, 0.125, n_text_blocks=1)
+    assert torch.equal(block_sparse_train_fn(*leaves, mask, 0.125, n_text_blocks=2 ** 40), want)

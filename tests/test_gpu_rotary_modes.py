@@ -63,3 +63,18 @@ def test_a_frozen_side_has_no_gradient(dev, trained):
     assert torch.equal(only, both[0 if trained == "q" else 1])
     with torch.no_grad():
         assert not any(t.requires_grad for t in rotary(q, k))
+
+
+def test_sizes_past_32_bits_are_refused(dev):
+    # Expanded tensors take no memory; a length cut to 32 bits would turn four tokens.
+    case("rotary sizes past 32 bits")
+    n = 2 ** 32 + 4
+    q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device=dev)
+    table = torch.zeros(4, 32, 2, device=dev)
+    rows = torch.zeros(1, dtype=torch.int32, device=dev)
+    for far in (q.expand(1, 1, n, 64), q.expand(n, 1, 1, 64), q.expand(1, n, 1, 64)):
+        for a, b in ((far, None), (q, far) if far.shape[1] == n else (far, far)):
+            with pytest.raises(ValueError, match="at most"):
+                apply_rotary(a, b, table, rows=rows.expand(a.shape[2]))
+    with pytest.raises(ValueError, match="at most"):
+        apply_rotary(q, None, table[:1].expand(n, 32, 2))

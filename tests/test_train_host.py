@@ -189,3 +189,13 @@ def test_backward_limits_are_known_before_the_forward_pass():
                 dict(stride=1 << 62), dict(max_cnt=65536, dk=256), dict(max_cnt=65536, dv=256)):
         assert check(**bad) == _lib.SA_ERR_UNSUPPORTED, bad
     assert check(Lq=0) == check(sm_scale=0.0) == check(sm_scale=math.nan) == lib.sa_block_sparse_bwd_check(None) == _lib.SA_ERR_INVALID
+
+
+def test_lengths_of_more_than_32_bits():
+    # (a length behind which rounding up to a workgroup's tokens would pass 32 bits; the checks come before any launch)
+    lib = _lib.load()
+    p = ctypes.c_void_p(256)
+    st = _lib.i64(*range(0, 120, 10))
+    for L in (2 ** 31 - 1, 2 ** 31 - 255):
+        rc = lib.sa_rotary_apply(0, p, p, None, None, st, 1, 1, 0, L, 64, p, 8, 32, p, 0, 0, 0, 0, None)
+        assert rc == _lib.SA_ERR_INVALID
