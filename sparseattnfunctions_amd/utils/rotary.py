@@ -106,6 +106,8 @@ def rotary_table(positions: torch.Tensor, axes: Union[int, Sequence[int]], theta
     _lib.require_gpu(positions)
     if positions.dtype not in _POSITION_TYPES:
         raise TypeError(f"positions must be int32, int64, fp32 or fp64, got {positions.dtype}")
+    if positions.requires_grad:
+        raise ValueError("positions are not differentiated; pass positions.detach()")
     if positions.dim() == 1:
         positions = positions[None]
     if positions.dim() != 2 or positions.shape[0] != len(axes):

@@ -4,7 +4,7 @@ import torch
 
 from conftest import case
 from sparseattnfunctions_amd.block_mask_attn import BlockSparseAttention
-from sparseattnfunctions_amd.utils.rotary import VideoRotary, apply_rotary, video_positions
+from sparseattnfunctions_amd.utils.rotary import VideoRotary, apply_rotary, rotary_table, video_positions
 from sparseattnfunctions_amd.workloads import Geometry
 
 pytestmark = pytest.mark.gpu
@@ -78,3 +78,14 @@ def test_sizes_past_32_bits_are_refused(dev):
                 apply_rotary(a, b, table, rows=rows.expand(a.shape[2]))
     with pytest.raises(ValueError, match="at most"):
         apply_rotary(q, None, table[:1].expand(n, 32, 2))
+
+
+def test_positions_are_not_differentiated(dev):
+    # A gradient that would silently be lost is refused, as one of the table is.
+    case("positions that require gradients")
+    positions = torch.arange(5.0, device=dev, requires_grad=True)
+    with pytest.raises(ValueError, match="detach"):
+        rotary_table(positions, 64)
+    with pytest.raises(ValueError, match="detach"):
+        VideoRotary(GEOM, positions=video_positions(GEOM).float().requires_grad_()).table(dev)
+    assert torch.equal(rotary_table(positions.detach(), 64), rotary_table(torch.arange(5, device=dev), 64))
