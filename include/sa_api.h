@@ -284,7 +284,7 @@ int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
  *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype, max_cnt, n_text_blocks and whether there
  *             is a q_idx and a key_bias): the query rows' statistics, the transposed lists, sums of lists split over
  *             workgroups.
- * Rows of one head of q, k, v and dout span less than 2 GiB. max_cnt at most 65535 with dk or dv and no q_idx,
+ * At most 2^27 rows a head, which span less than 2 GiB in each of q, k, v and dout. max_cnt at most 65535 with dk or dv and no q_idx,
  * sm_scale at least 1e-30. sa_block_sparse_bwd_check says whether a call is within these limits before its forward
  * pass: SA_ERR_UNSUPPORTED, or SA_OK. It reads the sizes, dtype, strides, max_cnt and sm_scale, and whether there is
  * a key_bias, q_idx, dk and dv.

@@ -1119,7 +1119,9 @@ int check_limits(const sa_attn_train* t, const char* fn) {
   // (the key pass takes the rows' sums in units of the scores, lse / sm_scale)
   if (t->sm_scale < 1e-30f) return sa::fail(SA_ERR_UNSUPPORTED, "%s: sm_scale %g below 1e-30", fn, t->sm_scale);
   if (t->dtype == SA_DTYPE_F32 && t->key_bias) return sa::fail(SA_ERR_UNSUPPORTED, "%s: fp32 with key_bias", fn);
-  // Streamed rows are copied through 32-bit buffer offsets relative to each head's first row.
+  // Streamed rows are copied through 32-bit buffer offsets relative to each head's first row, and so are the statistics
+  // (up to 16 bytes a row; rows may be expanded ones, which take no room).
+  if (t->Lq > 1 << 27 || t->Lk > 1 << 27) return sa::fail(SA_ERR_UNSUPPORTED, "%s: more than 2^27 rows", fn);
   const int size = t->dtype == SA_DTYPE_F32 ? 4 : 2;
   const int64_t rows[4] = {t->Lq, t->Lk, t->Lk, t->Lq};
   const int at[4] = {0, 1, 2, 4};

@@ -184,9 +184,9 @@ def test_backward_limits_are_known_before_the_forward_pass():
         return lib.sa_block_sparse_bwd_check(t)
 
     assert check() == check(sm_scale=1e-30, dk=256, dv=256) == check(max_cnt=65536) == 0
-    assert check(max_cnt=65536, dk=256, q_idx=256) == 0
+    assert check(max_cnt=65536, dk=256, q_idx=256) == check(stride=0, Lq=1 << 27) == 0
     for bad in (dict(sm_scale=1e-31), dict(dtype=2, key_bias=256), dict(stride=1 << 24), dict(stride=-64), dict(D=96),
-                dict(stride=1 << 62), dict(max_cnt=65536, dk=256), dict(max_cnt=65536, dv=256)):
+                dict(stride=1 << 62), dict(stride=0, Lq=(1 << 27) + 1), dict(stride=0, Lk=(1 << 27) + 1), dict(max_cnt=65536, dk=256), dict(max_cnt=65536, dv=256)):
         assert check(**bad) == _lib.SA_ERR_UNSUPPORTED, bad
     assert check(Lq=0) == check(sm_scale=0.0) == check(sm_scale=math.nan) == lib.sa_block_sparse_bwd_check(None) == _lib.SA_ERR_INVALID
 
