@@ -8,11 +8,12 @@ import pytest
 import torch
 
 from conftest import case
-from grad_reference import check, unit
+from grad_reference import check, reference, unit
 from oracle.attention import expand_block_mask
 from sparseattnfunctions_amd._kv import kv_list_from_mask
 from sparseattnfunctions_amd.utils.block_sparse_attn_grad import (block_sparse_attention_backward,
-                                                                  block_sparse_attention_lse, block_sparse_train_fn)
+                                                                  block_sparse_attention_lse,
+                                                                  block_sparse_attention_train, block_sparse_train_fn)
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +108,46 @@ def test_probabilities_sum_to_one(dev):
         dv = block_sparse_attention_backward(torch.ones_like(out), *x, out, lse, kv, 0.125, key_bias=bias.to(dev))[2]
         off = dv.double().sum(2) / 200 - 1
         assert off.abs().max() <= 2 * 2.0 ** -8, (value, off.abs().max().item())
+
+
+def test_bias_of_each_head_and_of_all(dev):
+    # A bias with values of its own for every head, in a tensor with odd strides, and one for all heads.
+    case("bias per head")
+    g = torch.Generator().manual_seed(8)
+    B, H, Lq, Lk = 2, 3, 150, 200
+    q, k, v, do = (torch.randn(B, H, L, 64, generator=g).bfloat16() for L in (Lq, Lk, Lk, Lq))
+    mask = torch.rand(B, H, 3, 4, generator=g) < 0.7
+    mask[..., 0] = True
+    wide = torch.randn(H, B, Lk + 3, generator=g)
+    for bias in (wide[..., 1:Lk + 1].transpose(0, 1), wide[0, 0, :Lk]):
+        leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+        b = wide.to(dev)[..., 1:Lk + 1].transpose(0, 1) if bias.dim() == 3 else bias.to(dev)
+        out = block_sparse_train_fn(*leaves, mask.to(dev), 0.125, key_bias=b)
+        got = (out, *torch.autograd.grad(out, leaves, do.to(dev)))
+        check(got, reference(q, k, v, do, mask, 0.125, bias=bias.expand(B, H, Lk)), norm=1.5 * unit(BF16))
+
+
+@pytest.mark.parametrize("lists", ["mask", "lists"])
+def test_saved_tensors_of_a_biased_call_may_move(dev, lists):
+    case(f"saved tensor hooks with a bias, {lists}")
+    inputs, mask, bias = _inputs(BF16, 2, 3, 200, 330, 64, -1e9)
+    x, mask, bias = [t.to(dev) for t in inputs], mask.to(dev), bias.to(dev)
+    kv = kv_list_from_mask(mask, 2, 3, 4, 6)
+
+    def grads():
+        # (q in rows of 72 values, which come back from the host in rows of 64)
+        wide = torch.zeros(2, 3, 200, 72, dtype=BF16, device=dev)
+        wide[..., :64] = x[0]
+        leaves = [wide[..., :64].requires_grad_(), *(t.detach().requires_grad_() for t in x[1:3])]
+        if lists == "mask":
+            out = block_sparse_train_fn(*leaves, mask, 0.125, key_bias=bias)
+        else:
+            out = block_sparse_attention_train(*leaves, kv, 0.125, key_bias=bias)
+        return out, lambda: torch.autograd.grad(out, leaves, x[3])
+
+    want = grads()[1]()
+    with torch.autograd.graph.save_on_cpu():
+        out, back = grads()
+        got = back()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    check((out, *got), _reference(*inputs, mask.cpu(), 0.125, bias.cpu()))
