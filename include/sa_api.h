@@ -279,8 +279,9 @@ int sa_block_sparse_fwd_lse(const sa_attn_train* call, void* stream);
  * dq, dk, dv for the gradient dout of out, the probabilities recomputed from lse: P = exp2(score -
  * lse), dS = P * (dout v^T - rowsum(dout * out)), dq = sm_scale dS k, dk = sm_scale dS^T q, dv = P^T
  * dout. Rows and keys in no list get zeros; a block that a row lists twice counts twice. Sums are fp32 in a
- * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type; fp32 takes its operands in
- * three bf16 terms (finite ones; those below about 1e-33 lose their low terms).
+ * fixed order: results repeat bit for bit. 16-bit types round P and dS to the type (fp16 P with a factor of 4096 where
+ * max_cnt is above 256); fp32 takes its operands in three bf16 terms (ones below 3.39e38 in size, from where bf16 rounds
+ * to infinity; those below about 1e-33 lose their low terms).
  *   workspace sa_block_sparse_bwd_workspace bytes (which reads the sizes, dtype, max_cnt, n_text_blocks and whether there
  *             is a q_idx and a key_bias): the query rows' statistics, the transposed lists, sums of lists split over
  *             workgroups.

@@ -609,8 +609,8 @@ __global__ __launch_bounds__(128 * kParts, kD == 64 ? 3 : 2) void bsa_bwd_kernel
 // Bound: the matrix core, beside the splits (11 VALU operations a pair of values) and exp2. [1, 30, 2560, 64] with
 // half the blocks: query pass 236 us, key pass 297 (162 and 171 TFLOP/s of fp32 products, six times that in bf16 ones, the
 // matrix cores 45 and 48 % of the cycles); with merges and lists 250 and 320, on the fp32 matrix instructions 365 and
-// 459. [1, 10, 3500, 128] with 0.4 of them 288 and 388 (410 and 555). Values have to be finite; those below about
-// 1e-33, as of gradients of a loss scaled down so far, lose their low terms.
+// 459. [1, 10, 3500, 128] with 0.4 of them 288 and 388 (410 and 555). Values have to be below 3.39e38, from where
+// bf16 rounds to infinity; those below about 1e-33, as of gradients of a loss scaled down so far, lose their low terms.
 
 // The six term products of A and B onto c.
 __device__ inline sa_f32x16 mfma_terms(const sa_u32x4v (&A)[3], const sa_bf16x8 (&B)[3], sa_f32x16 c) {
@@ -649,7 +649,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 2 : 1) void bsa_bwd_f32_kernel(BwdA
   constexpr int kPasses = kStep * kLanes / 64;
   __shared__ __attribute__((aligned(1024))) uint8_t tile_lds[kParts * 2 * kMat];
   __shared__ __attribute__((aligned(256))) float stat[kParts * 64];
-  // The key pass at two waves per SIMD has no registers for its own v's low terms (spilled: 348 us for the 325 above).
+  // The key pass at two waves per SIMD has no registers for its own v's low terms: with them, [1, 30, 2560, 64] took 348
+  // us (key pass, lists and merge), without 325. Four registers are still spilled.
   constexpr bool kLowInLds = kKeys && kD == 64;
   __shared__ sa_u32x4v low[kLowInLds ? 2 * kParts : 1][kLowInLds ? kDS : 1][64];
   const int lane = threadIdx.x & 63;

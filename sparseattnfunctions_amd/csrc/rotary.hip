@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void rotary_table_kernel(TableArgs a) {
     const double quarter = rint(4.0 * r);
     const float y = (float)((r - 0.25 * quarter) * kTurn);  // |y| <= pi / 4
     const float z = y * y;
-    // Their power series, up to y^9 and y^10 (what is left out is below 2e-9 of the value).
+    // Their power series, up to y^9 and y^10 (what is left out is below 2.5e-9 of the value).
     const float s = fmaf(y * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), y);
     const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
     const int q = (int)quarter & 3;  // (an infinite or NaN position gives NaN either way)

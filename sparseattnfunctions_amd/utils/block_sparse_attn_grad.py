@@ -15,12 +15,20 @@ does as well. Training code calls this module instead:
 The forward pass is the kernel of `block_sparse_attention` with bf16 (fp16) scores, or fp32 on split
 operands, and also stores each row's log2-sum-exp2; the backward pass recomputes the probabilities
 from it, block by block, and keeps nothing of the size of the attention map (`sa_block_sparse_bwd`).
-Gradients of a 16-bit call round P and dS to its type, those of an fp32 call take finite operands as
-three exact bf16 terms (values below about 1e-33 lose their low ones); sums are fp32 in a fixed order,
-so that a step repeats bit for bit. In fp16, dS has the range of the type: scale the loss as usual. A
-query row without a key (an empty list, or keys all biased to -inf) has a zero output and zero
-gradients; a key block in no list has zero gradients. The mask, the lists and key_bias are not
-differentiated.
+Between the two a call holds q, k, v and out, a float per row and its lists: a mask's lists of both
+sides are full width, eight bytes for each pair of blocks (191 MB at [1, 48, 45104, 64], whose q has
+277 MB), a caller's are the caller's own and their key side is made in the backward call.
+
+Gradients of a 16-bit call round P and dS to its type, those of an fp32 call take operands below 3.39e38
+in size (from there on bf16 rounds to infinity) as three exact bf16 terms (values below about 1e-33 lose
+their low ones); sums are fp32 in a fixed order, so that a step repeats bit for bit. In fp16, dS has the
+range of the type: scale the loss as usual; P, which that does not help, takes a factor of 4096 of its
+own where lists may hold more than 16 384 keys.
+
+The attention is differentiable once, and `create_graph=True` is refused as a whole: take the gradient of
+a penalty on another part of the graph with `torch.autograd.grad` of that part. A query row without a key
+(an empty list, or keys all biased to -inf) has a zero output and zero gradients; a key block in no list
+has zero gradients. The mask, the lists and key_bias are not differentiated.
 
 A key_bias is added to the scores in fp32, in both passes alike, so that one as large as 1e9 leaves a
 row that lists nothing else few of its scores' bits. One below -2.35e38 (the type's lowest value among

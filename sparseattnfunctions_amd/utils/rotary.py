@@ -47,6 +47,10 @@ def rotary_frequencies(dims: int, theta: float = 10000.0, scaling: Optional[dict
                                         keep their frequency, those with fewer than beta_slow are
                                         divided by s, linearly in the turns between; cosines and
                                         sines times 0.1 ln(s) + 1.
+
+    This is YaRN's ramp as its paper writes it. Checkpoints are also trained with one that is linear in the pair's
+    index between the two limits, whose frequencies differ by up to a factor of two in the middle: not this
+    function's.
     """
     if dims <= 0 or dims % 2:
         raise ValueError(f"an axis has an even number of values, got {dims}")
