@@ -161,6 +161,9 @@ class VideoRotary:
         self.layout, self.positions = layout, positions
         self._tables = {}  # device -> (table, the stream it was made on)
 
+    def __getstate__(self):  # a copy makes its own tables (streams can neither be copied nor pickled)
+        return {**self.__dict__, "_tables": {}}
+
     def table(self, device) -> torch.Tensor:
         device = torch.device(device)
         if device.index is None:

@@ -1,4 +1,7 @@
 """Rotary positions across autograd's modes."""
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -89,3 +92,15 @@ def test_positions_are_not_differentiated(dev):
     with pytest.raises(ValueError, match="detach"):
         VideoRotary(GEOM, positions=video_positions(GEOM).float().requires_grad_()).table(dev)
     assert torch.equal(rotary_table(positions.detach(), 64), rotary_table(torch.arange(5, device=dev), 64))
+
+
+def test_processors_can_be_copied_and_pickled(dev):
+    # An averaged copy of a model copies its processors, tables made or not; the copy makes its own.
+    case("copied processors")
+    q, k, v, _ = _qkv(dev)
+    proc = BlockSparseAttention(64, keep_ratio=0.6, geometry=GEOM, trainable=True, rotary=VideoRotary(GEOM))
+    want = proc(q, k, v)
+    for copied in (copy.deepcopy(proc), pickle.loads(pickle.dumps(proc.rotary))):
+        got = copied(q, k, v) if isinstance(copied, BlockSparseAttention) else copied(q, k)
+        ref = (want,) if isinstance(copied, BlockSparseAttention) else proc.rotary(q, k)
+        assert all(torch.equal(a, b) for a, b in zip((got,) if torch.is_tensor(got) else got, ref))
