@@ -306,6 +306,66 @@ int sa_kv_list_transpose(const int32_t* kv_idx, const int32_t* kv_cnt, int BH, i
                          int32_t* q_beg, int32_t* q_idx, void* stream);
 
 /*
+ * Attention whose scores follow a rule besides the dot product, and its gradients. Beyond the reference, whose scores
+ * are plain ones under a block mask. Query head h reads the keys of key head h / (H / Hk); with d = i + q_start - j
+ *   s = sm_scale q.k;  cap c > 0: s = c tanh(s / c);  slopes: s -= slopes[h] |d|;
+ *   table: s += table[buckets[clamp(d, -radius, radius) + radius]][h]
+ * Row i sees key j where ranges[b][j][0] <= i < ranges[b][j][1] and mask[b][h][i / 64][j / 64] (either may be NULL: all).
+ */
+typedef struct sa_attn_scored {
+  int32_t dtype;       /* SA_DTYPE_*: of q .. dv */
+  int32_t B, H, Hk, Lq, Lk, D;
+  int32_t q_start;     /* position of query row 0, where key 0 has 0 */
+  const void *q, *k, *v;
+  void* out;           /* forward: written; backward: read */
+  const void* dout;    /* gradient of out */
+  void *dq, *dk, *dv;  /* each nullable: not computed */
+  int64_t strides[24]; /* {b, h, l} in elements of q, k, v, out, dout, dq, dk, dv */
+  float* lse;          /* [B*H][64*ceil(Lq/64)]; forward: written; backward: read */
+  const int32_t* ranges;   /* nullable [B][Lk][2], 8-byte aligned */
+  int64_t ranges_stride;   /* keys from one sequence to the next (0: one for all) */
+  const uint8_t* mask;     /* nullable block mask; read by the forward call alone */
+  int64_t mask_strides[4]; /* {b, h, q block, k block} in bytes */
+  float sm_scale, cap;
+  const float* slopes;     /* nullable [H] */
+  const void* table;       /* nullable [n_buckets][H] */
+  const int32_t* buckets;  /* [2*radius+1]; entries outside [0, n_buckets) are taken as the nearest one */
+  int32_t table_dtype, n_buckets, radius;
+  int32_t key_lists;       /* whether the plan has the lists of the key blocks, which dk and dv need */
+  void* dtable;            /* nullable [n_buckets][H] of the table's type: sum of dS over each bucket's pairs */
+  void* plan;              /* lists and biases, written by the forward call and read by the backward call */
+  int64_t plan_bytes;
+  void* workspace;         /* of the backward call */
+  int64_t workspace_bytes;
+} sa_attn_scored;
+
+/* Bytes of a call's plan and of its backward call's workspace (both 256-byte aligned). Reads the sizes, dtype,
+ * key_lists, radius, and whether there are ranges, a mask, a table and a dtable. */
+int sa_attn_scored_sizes(const sa_attn_scored* call, int64_t* plan_bytes, int64_t* workspace_bytes);
+
+/*
+ * out and each row's log2-sum-exp2: +inf, and a row of zeros, for a row that sees no key. bf16, fp16 (P rounded to the
+ * type) or fp32, D = 64 or 128. Keys and values of listed blocks have to be finite, also where a row does not see them.
+ * At most 2^27 rows, and less than 2 GiB from a head's first row to its last. Reads neither dout nor the gradients.
+ */
+int sa_attn_scored_fwd(const sa_attn_scored* call, void* stream);
+
+/* dq, dk, dv (summed over the query heads of a key head) and dtable, the probabilities recomputed from lse. Sums are fp32
+ * in a fixed order: results repeat bit for bit. 16-bit types round P (fp16: times 4096) and dC to the type. */
+int sa_attn_scored_bwd(const sa_attn_scored* call, void* stream);
+
+/*
+ * ranges [B][L][2] of sequences in which n documents of lengths[b][0 .. n) lie one after the other from token 0 (cut off at
+ * L; tokens behind the last one are seen by no row). A document's first prefix[b][i] tokens are seen by all its rows.
+ * Of the others, with causal, a row sees those of its own frame (groups of `frame` tokens behind the prefix; 1: itself)
+ * and of the ones before, else all; with window > 0 those less than `window` tokens away (before it, and, not causal, behind it;
+ * with frames, behind it to the end of its own).
+ *   prefix nullable. n at most 8192, B 65535, L 2^30. frame > 1 only with causal.
+ */
+int sa_row_ranges(const int32_t* lengths, const int32_t* prefix, int B, int n, int L, int causal, int frame, int window,
+                  int32_t* ranges, void* stream);
+
+/*
  * Rotary positions (the host model's part of the attention call: its processors receive q and k that
  * it has turned, SildingTileAttention.py:100-105 give the token order).
  *

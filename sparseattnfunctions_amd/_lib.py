@@ -40,6 +40,18 @@ class AttnTrain(ctypes.Structure):
                    ("q_idx", _P), ("q_cnt", _P), ("row_max", _P)])
 
 
+class AttnScored(ctypes.Structure):
+    """sa_attn_scored of include/sa_api.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "B", "H", "Hk", "Lq", "Lk", "D", "q_start")]
+                + [(n, _P) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")]
+                + [("strides", ctypes.c_int64 * 24), ("lse", _P), ("ranges", _P), ("ranges_stride", ctypes.c_int64),
+                   ("mask", _P), ("mask_strides", ctypes.c_int64 * 4), ("sm_scale", _F), ("cap", _F), ("slopes", _P),
+                   ("table", _P), ("buckets", _P)]
+                + [(n, ctypes.c_int32) for n in ("table_dtype", "n_buckets", "radius", "key_lists")]
+                + [("dtable", _P), ("plan", _P), ("plan_bytes", ctypes.c_int64), ("workspace", _P),
+                   ("workspace_bytes", ctypes.c_int64)])
+
+
 # name -> (restype, argtypes); must match include/sa_api.h.
 _PROTOTYPES = {
     "sa_abi_version": (_I, []),
@@ -81,6 +93,10 @@ _PROTOTYPES = {
     "sa_block_sparse_bwd_workspace": (_I, [ctypes.POINTER(AttnTrain), _I64P]),
     "sa_block_sparse_bwd_check": (_I, [ctypes.POINTER(AttnTrain)]),
     "sa_block_sparse_bwd": (_I, [ctypes.POINTER(AttnTrain), _P]),
+    "sa_attn_scored_sizes": (_I, [ctypes.POINTER(AttnScored), _I64P, _I64P]),
+    "sa_attn_scored_fwd": (_I, [ctypes.POINTER(AttnScored), _P]),
+    "sa_attn_scored_bwd": (_I, [ctypes.POINTER(AttnScored), _P]),
+    "sa_row_ranges": (_I, [_P, _P, _I, _I, _I, _I, _I, _I, _P, _P]),
     "sa_rotary_table": (_I, [_P, _I, _I64P, ctypes.c_int64, _I, _P, _P, _P, _P, _P]),
     "sa_rotary_apply": (
         _I,

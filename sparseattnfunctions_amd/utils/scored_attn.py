@@ -1,0 +1,370 @@
+"""Attention whose scores follow a rule besides the dot product, differentiable, on MI355X: scores
+capped by a tanh, less a slope times the distance, plus a learned bias by buckets of the distance, over
+documents, prefixes, causal rows and frames, windows and blocks of a mask. Beyond the reference, whose
+attention takes a block mask (special_attentions/utils/block_sparse_attn_kernel.py:211-265).
+
+  * `scored_attention(q, k, v, sm_scale, ...)`: the call, differentiable in q, k, v and the bias table;
+  * `scored_attention_forward` and `scored_attention_backward`: its two halves without autograd, e.g. for
+    a step captured into a HIP graph;
+  * `row_ranges`: which rows see each key, from the lengths of the documents that a sequence packs;
+  * `distance_buckets`: the buckets of a learned bias.
+
+With d = i + q_start - j the distance of query row i from key j of query head h, whose keys are those of
+key head h // (H // Hk), the score is
+
+  s = sm_scale q.k;  cap: s = cap tanh(s / cap);  slopes: s -= slopes[h] |d|;
+  table: s += table[buckets[clamp(d, -R, R) + R], h], 2 R + 1 = len(buckets)
+
+and row i sees key j where ranges[b, j, 0] <= i < ranges[b, j, 1] and block_mask[b, h, i // 64, j // 64].
+A row that sees no key has a zero output and zero gradients, a key that no row sees zero gradients.
+
+The backward pass recomputes the probabilities block by block (`sa_attn_scored_bwd`); between the two a
+call holds q, k, v, out, a float per row and its lists of blocks (eight bytes for each pair of 64-token
+blocks of a sequence, with a block mask of a head). Blocks of which no pair is seen are not read. Gradients
+of a 16-bit call round P and dS to its type; sums are fp32 in a fixed order, so that a step repeats bit
+for bit. In fp16, dS has the range of the type: scale the loss as usual.
+
+Keys and values of blocks that hold a visible pair enter the products whole: they have to be finite, also
+where a mask hides them, as do the slopes and the table. The calls are differentiable once; ranges, the
+mask and the slopes are not differentiated.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from .. import _lib
+from .block_sparse_attn_grad import _rows16
+from .block_sparse_attn_kernel import BLOCK
+
+MOST_RADIUS = 1024  # distances that a bias tells apart
+
+
+def distance_buckets(n_buckets: int, radius: int, bidirectional: bool = True, device="cuda") -> torch.Tensor:
+    """Buckets int32 [2 radius + 1] of the distances -radius .. radius (i - j: positive for keys before the
+    row) for `scored_attention`'s table; distances past the radius share the last one's.
+
+    Of the buckets of a side (all of them unless bidirectional; then keys behind the row have bucket 0)
+    the first half hold one distance each, the others grow in proportion to it, up to the radius."""
+    n_buckets, radius = int(n_buckets), int(radius)
+    if not 0 <= radius <= MOST_RADIUS:
+        raise ValueError(f"radius {radius} (0 to {MOST_RADIUS})")
+    if n_buckets < 1:
+        raise ValueError(f"n_buckets {n_buckets}")
+    side = (n_buckets - 1) // 2 if bidirectional else n_buckets - 1
+    exact = max(1, side // 2)
+    places = []
+    for d in range(-radius, radius + 1):
+        a = abs(d) if bidirectional else max(d, 0)
+        if a > exact:
+            a = exact + int((side - exact) * math.log(a / exact) / math.log(radius / exact)) + 1
+        a = min(side, a)
+        places.append(a if d >= 0 or not bidirectional or a == 0 else side + a)
+    return torch.tensor(places, dtype=torch.int32, device=device)
+
+
+def row_ranges(lengths: torch.Tensor, L: int, causal: bool = True, prefix: Optional[torch.Tensor] = None, frame: int = 1,
+               window: int = 0) -> torch.Tensor:
+    """ranges int32 [B, L, 2] of B sequences that pack documents of `lengths` (integers [B, n], or [n] for
+    one sequence) one after the other from token 0, made on the GPU (`sa_row_ranges`). Rows see the keys of
+    their own document; tokens behind the last document are seen by no row, and see none.
+
+    Of a document, its first prefix[b, i] tokens (none by default) are seen by all its rows. Of the others
+    a causal row sees itself and those before it, with `frame` > 1 those of its own and earlier groups of
+    `frame` tokens, counted from behind the prefix; a row that is not causal sees all. With a window a key
+    outside the prefix is seen by no row that lies `window` tokens or more behind it (or, not causal,
+    before it)."""
+    tensors = (lengths,) if prefix is None else (lengths, prefix)
+    _lib.require_gpu(*tensors)
+    if lengths.dim() == 1:
+        lengths = lengths[None]
+    if lengths.dim() != 2 or lengths.shape[1] == 0 or lengths.is_floating_point():
+        raise ValueError(f"lengths must be integers [B, n], got {lengths.dtype} {tuple(lengths.shape)}")
+    B, n = lengths.shape
+    if prefix is not None:
+        if prefix.is_floating_point() or prefix.device != lengths.device:
+            raise ValueError("prefix must be integers on the device of lengths")
+        prefix = prefix.expand(B, n).to(torch.int32).contiguous()
+    L, frame, window = int(L), int(frame), int(window)
+    if L < 0:
+        raise ValueError(f"L={L}")
+    if max(L, frame, window) >= 2 ** 31:
+        raise ValueError(f"L={L} frame={frame} window={window}: sizes of 32 bits")
+    out = torch.empty(B, L, 2, dtype=torch.int32, device=lengths.device)
+    if out.numel() == 0:
+        return out
+    if lengths.dtype == torch.int64:  # (a longer one is cut off at L anyway)
+        lengths = lengths.clamp(0, L)
+    lengths = lengths.to(torch.int32).contiguous()
+    with _lib.on(out.device):
+        rc = _lib.load().sa_row_ranges(lengths.data_ptr(), _lib.ptr(prefix), B, n, L, int(bool(causal)), frame, window,
+                                       out.data_ptr(), _lib.stream_of(out))
+    _lib.check(rc, "sa_row_ranges")
+    return out
+
+
+def check_rule(q, H: int, cap, slopes, table, buckets):
+    """The checked parameters of a score rule: (cap, slopes, table, buckets, radius)."""
+    if cap is not None and not (cap > 0 and math.isfinite(cap)):
+        raise ValueError(f"cap {cap} must be positive and finite")
+    if slopes is not None:
+        if slopes.requires_grad:
+            raise ValueError("slopes are not differentiated; pass slopes.detach()")
+        if slopes.dtype != torch.float32 or slopes.shape != (H,):
+            raise ValueError(f"slopes must be fp32 [{H}], got {slopes.dtype} {tuple(slopes.shape)}")
+        slopes = slopes.contiguous()
+    if (table is None) != (buckets is None):
+        raise ValueError("a table needs buckets, and buckets a table")
+    radius = 0
+    if table is not None:
+        if table.dtype not in _lib.DTYPES:
+            raise TypeError(f"table must be bf16, fp16 or fp32, got {table.dtype}")
+        if table.dim() != 2 or table.shape[1] != H or table.shape[0] == 0:
+            raise ValueError(f"table must be [buckets, {H}], got {tuple(table.shape)}")
+        if buckets.dtype != torch.int32 or buckets.dim() != 1 or buckets.numel() % 2 == 0:
+            raise ValueError("buckets must be int32 [2 radius + 1]")
+        radius = buckets.numel() // 2
+        if radius > MOST_RADIUS:
+            raise NotImplementedError(f"distances up to {radius} told apart (at most {MOST_RADIUS})")
+        table, buckets = table.contiguous(), buckets.contiguous()
+    for t in (slopes, table, buckets):
+        if t is not None and t.device != q.device:
+            _lib.require_gpu(t)
+            raise ValueError("q, k, v and the rule's tensors must be on one device")
+    return 0.0 if cap is None else float(cap), slopes, table, buckets, radius
+
+
+def check_heads(q, k, v):
+    """(B, H, Hk, Lq, Lk, D) of q [B,H,Lq,D] and k, v [B,Hk,Lk,D]."""
+    _lib.require_gpu(q, k, v)
+    if not q.device == k.device == v.device:
+        raise ValueError("q, k and v must be on one device")
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q, k, v must be [B, H, L, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in _lib.DTYPES or not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"q, k, v must share one of bf16, fp16 and fp32, got {q.dtype}, {k.dtype}, {v.dtype}")
+    B, H, Lq, D = q.shape
+    Hk, Lk = k.shape[1:3]
+    if k.shape != (B, Hk, Lk, D) or v.shape != k.shape:
+        raise ValueError(f"shape mismatch q{tuple(q.shape)} k{tuple(k.shape)} v{tuple(v.shape)}")
+    if (H % Hk if Hk else H) != 0:
+        raise ValueError(f"{H} query heads over {Hk} key heads")
+    if D not in (64, 128):
+        raise NotImplementedError(f"head_dim {D} (64 or 128)")
+    return B, H, Hk, Lq, Lk, D
+
+
+class ScoredState:
+    """What `scored_attention_forward` keeps for `scored_attention_backward`: the tensors and the call's
+    description."""
+
+    __slots__ = ("tensors", "numbers")
+
+    NAMES = ("q", "k", "v", "out", "lse", "plan", "ranges", "slopes", "table", "buckets")
+
+    def __init__(self, tensors, numbers):
+        self.tensors, self.numbers = tensors, numbers
+
+
+_PLACES = {name: 3 * i for i, name in enumerate(("q", "k", "v", "out", "dout", "dq", "dk", "dv"))}
+
+
+def _set(call, **tensors):
+    for name, t in tensors.items():
+        setattr(call, name, t.data_ptr())
+        at = _PLACES[name]
+        call.strides[at:at + 3] = t.stride()[:3]
+
+
+def _describe(q, k, v, slopes, table, buckets, ranges, numbers):
+    """A call's description; numbers: (sm_scale, cap, q_start, key_lists, masked)."""
+    sm_scale, cap, q_start, key_lists, masked = numbers
+    B, H, Lq, D = q.shape
+    call = _lib.AttnScored(dtype=_lib.DTYPES[q.dtype], B=B, H=H, Hk=k.shape[1], Lq=Lq, Lk=k.shape[2], D=D, q_start=q_start,
+                           sm_scale=sm_scale, cap=cap, key_lists=key_lists)
+    _set(call, q=q, k=k, v=v)
+    if slopes is not None:
+        call.slopes = slopes.data_ptr()
+    if table is not None:
+        call.table, call.buckets = table.data_ptr(), buckets.data_ptr()
+        call.table_dtype, call.n_buckets, call.radius = _lib.DTYPES[table.dtype], table.shape[0], buckets.numel() // 2
+    if ranges is not None:
+        call.ranges, call.ranges_stride = ranges.data_ptr(), ranges.stride(0) // 2
+    if masked:  # (the backward call reads its lists)
+        call.mask = 1
+    return call
+
+
+def _sizes(call):
+    plan, work = ctypes.c_int64(0), ctypes.c_int64(0)
+    _lib.check(_lib.load().sa_attn_scored_sizes(call, ctypes.byref(plan), ctypes.byref(work)), "sa_attn_scored_sizes")
+    return plan.value, work.value
+
+
+def _check_ranges(ranges, q, B, Lk):
+    if ranges is None:
+        return None
+    if ranges.device != q.device:
+        _lib.require_gpu(ranges)
+        raise ValueError("q, k, v and ranges must be on one device")
+    if ranges.dtype != torch.int32 or ranges.dim() not in (2, 3) or ranges.shape[-2:] != (Lk, 2) \
+            or (ranges.dim() == 3 and ranges.shape[0] not in (1, B)):
+        raise ValueError(f"ranges must be int32 [{B}, {Lk}, 2], got {ranges.dtype} {tuple(ranges.shape)}")
+    if ranges.dim() == 2:
+        ranges = ranges[None]
+    if ranges.stride(2) != 1 or (ranges.stride(1) != 2 and Lk > 1) or ranges.stride(0) % 2 or ranges.data_ptr() % 8:
+        ranges = ranges.clone(memory_format=torch.contiguous_format)
+    return ranges.expand(B, -1, -1)
+
+
+def _check_mask(mask, q, B, H, nqb, nkb):
+    if mask is None:
+        return None
+    if mask.device != q.device:
+        _lib.require_gpu(mask)
+        raise ValueError("q, k, v and the block mask must be on one device")
+    if mask.dim() != 4:
+        raise ValueError(f"block mask must be 4-D [B,H,nqb,nkb], got {tuple(mask.shape)}")
+    if mask.shape[2] < nqb or mask.shape[3] < nkb:
+        raise ValueError(f"block mask {tuple(mask.shape)} smaller than the block grid ({nqb}, {nkb})")
+    if mask.dtype != torch.bool:
+        mask = mask != 0
+    return mask.expand(B, H, -1, -1)
+
+
+def _check(q, k, v, cap, slopes, table, buckets, ranges, block_mask, q_start):
+    B, H, Hk, Lq, Lk, D = check_heads(q, k, v)
+    cap, slopes, table, buckets, _ = check_rule(q, H, cap, slopes, table, buckets)
+    if not -2 ** 29 < q_start < 2 ** 29:
+        raise ValueError(f"q_start {q_start}")
+    ranges = _check_ranges(ranges, q, B, Lk)
+    block_mask = _check_mask(block_mask, q, B, H, -(-Lq // BLOCK), -(-Lk // BLOCK))
+    return cap, slopes, table, buckets, ranges, block_mask
+
+
+def _forward(q, k, v, sm_scale, cap, slopes, table, buckets, ranges, mask, q_start, key_lists):
+    """(out, state) on checked arguments."""
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    numbers = (sm_scale, cap, q_start, key_lists, mask is not None)
+    call = _describe(q, k, v, slopes, table, buckets, ranges, numbers)
+    if mask is not None:
+        call.mask = mask.data_ptr()
+        call.mask_strides[:] = mask.stride()
+    B, H, Lq, D = q.shape
+    out = torch.empty((B, H, Lq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, -(-Lq // BLOCK) * BLOCK), dtype=torch.float32, device=q.device)
+    plan_bytes = _sizes(call)[0]
+    plan = torch.empty(plan_bytes, dtype=torch.uint8, device=q.device)
+    _set(call, out=out)
+    call.lse, call.plan, call.plan_bytes = lse.data_ptr(), plan.data_ptr(), plan_bytes
+    with _lib.on(q.device):
+        rc = _lib.load().sa_attn_scored_fwd(call, _lib.stream_of(q))
+    _lib.check(rc, "sa_attn_scored_fwd")
+    return out, ScoredState((q, k, v, out, lse, plan, ranges, slopes, table, buckets), numbers)
+
+
+def _backward(dout, state, needs):
+    """(dq, dk, dv, dtable), None where not needed."""
+    q, k, v, out, lse, plan, ranges, slopes, table, buckets = state.tensors
+    q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
+    dout = _rows16(dout)
+    if (dout.shape[2] + BLOCK) * dout.stride(2) * dout.element_size() >= 1 << 30:  # (rows far apart: 32-bit offsets)
+        dout = dout.contiguous()
+    call = _describe(q, k, v, slopes, table, buckets, ranges, state.numbers)
+    _set(call, out=out, dout=dout)
+    call.lse, call.plan, call.plan_bytes = lse.data_ptr(), plan.data_ptr(), plan.numel()
+    grads = [None] * 4
+    for i, (name, like) in enumerate((("dq", q), ("dk", k), ("dv", v))):
+        if needs[i]:
+            grads[i] = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+            _set(call, **{name: grads[i]})
+    if needs[3]:
+        grads[3] = torch.empty_like(table)
+        call.dtable = grads[3].data_ptr()
+    n = _sizes(call)[1]
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    call.workspace, call.workspace_bytes = ws.data_ptr(), n
+    with _lib.on(q.device):
+        rc = _lib.load().sa_attn_scored_bwd(call, _lib.stream_of(q))
+    _lib.check(rc, "sa_attn_scored_bwd")
+    return tuple(grads)
+
+
+def scored_attention_forward(q, k, v, sm_scale: float, *, cap: Optional[float] = None, slopes=None, table=None, buckets=None,
+                             ranges=None, block_mask=None, q_start: int = 0):
+    """(out, state): `scored_attention` without autograd, and what `scored_attention_backward` needs of it."""
+    checked = _check(q, k, v, cap, slopes, table, buckets, ranges, block_mask, int(q_start))
+    if q.numel() == 0 or k.numel() == 0:
+        raise ValueError(f"no query or no key: q{tuple(q.shape)} k{tuple(k.shape)}")
+    with torch.no_grad():
+        return _forward(q, k, v, float(sm_scale), *checked, int(q_start), True)
+
+
+def scored_attention_backward(dout, state: ScoredState, needs=(True, True, True, True)):
+    """(dq, dk, dv, dtable) for the gradient dout of `scored_attention_forward`'s out, whose tensors must be as
+    they were; None where `needs` is false, and for dtable without a table."""
+    q, table = state.tensors[0], state.tensors[8]
+    _lib.require_gpu(dout)
+    if dout.shape != q.shape or dout.dtype != q.dtype or dout.device != q.device:
+        raise ValueError(f"dout must be like q: {tuple(q.shape)} {q.dtype}, got {tuple(dout.shape)} {dout.dtype}")
+    with torch.no_grad():
+        return _backward(dout, state, (*needs[:3], needs[3] and table is not None))
+
+
+class _ScoredAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, sm_scale, cap, slopes, buckets, ranges, mask, q_start, followed):
+        out, state = _forward(q, k, v, sm_scale, cap, slopes, table, buckets, ranges, mask, q_start, followed)
+        ctx.numbers = state.numbers
+        ctx.save_for_backward(*state.tensors)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        if torch.is_grad_enabled():
+            raise RuntimeError("scored attention is differentiable once (create_graph=True is not supported)")
+        needs = ctx.needs_input_grad
+        dq, dk, dv, dtable = _backward(dout, ScoredState(ctx.saved_tensors, ctx.numbers), needs[:4])
+        return (dq, dk, dv, dtable) + (None,) * 8
+
+
+class _Nothing(torch.autograd.Function):
+    """The output where there is no query or no key: zeros, with zero gradients."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table):
+        ctx.save_for_backward(q, k, v, table)
+        return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+
+    @staticmethod
+    def backward(ctx, dout):
+        return tuple(None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors)
+
+
+def scored_attention(q, k, v, sm_scale: float, *, cap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
+                     table: Optional[torch.Tensor] = None, buckets: Optional[torch.Tensor] = None,
+                     ranges: Optional[torch.Tensor] = None, block_mask: Optional[torch.Tensor] = None,
+                     q_start: int = 0) -> torch.Tensor:
+    """softmax attention under the score rule of this module, differentiable (once) in q, k, v and table.
+
+    q [B,H,Lq,D], k and v [B,Hk,Lk,D] (H a multiple of Hk) on the GPU, bf16, fp16 or fp32 (one type), D = 64
+    or 128, any strides (tensors whose rows are not 16-byte aligned are copied). cap: a number; slopes: fp32
+    [H]; table: [n, H] of any of the three types, with buckets int32 [2 R + 1] (R up to 1024; entries outside
+    [0, n) count as the nearest one); ranges: int32 [B or 1, Lk, 2] (`row_ranges`, or a caller's own);
+    block_mask: bool or integer [B or 1, H or 1, >= ceil(Lq / 64), >= ceil(Lk / 64)]; q_start: the position of
+    row 0 where key 0 has position 0, for the distances alone (ranges count rows from 0).
+
+    The tensors must stay as they are until the backward pass has run. A call captured into a HIP graph needs
+    leaves that no eager graph holds (autograd ties a leaf's gradient to the stream of its first use)."""
+    cap, slopes, table, buckets, ranges, block_mask = _check(q, k, v, cap, slopes, table, buckets, ranges, block_mask,
+                                                             int(q_start))
+    if not (sm_scale > 0 and math.isfinite(sm_scale)):
+        raise ValueError(f"sm_scale {sm_scale} must be positive and finite")
+    if q.numel() == 0 or k.numel() == 0:
+        return _Nothing.apply(q, k, v, table)
+    followed = torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)
+    return _ScoredAttention.apply(q, k, v, table, float(sm_scale), cap, slopes, buckets, ranges, block_mask, int(q_start),
+                                  followed)
