@@ -355,6 +355,38 @@ int sa_attn_scored_fwd(const sa_attn_scored* call, void* stream);
 int sa_attn_scored_bwd(const sa_attn_scored* call, void* stream);
 
 /*
+ * Attention of Ln new tokens of each sequence over its cached keys and values, with sa_attn_scored's rule of scores, and over
+ * a prefix of Lp tokens that all sequences begin with, whose keys and values are held (and read) once.
+ * Sequence b has lengths[b] cached tokens (clamped to [0, L]), the last Ln of them the new ones; new token i is its
+ * token t = lengths[b] - Ln + i, at distance d = t - j from its key j and Lp + t - j from the prefix's. It sees keys at
+ * d >= 0, with window > 0 at d < window; where t < 0 none, and its output is zeros. Cached rows from lengths[b] on are not used,
+ * whatever they hold.
+ */
+typedef struct sa_attn_cached {
+  int32_t dtype;       /* SA_DTYPE_*: of q, out and the keys and values */
+  int32_t B, H, Hk, Ln, L, Lp, D;
+  int32_t window, table_dtype, n_buckets, radius;
+  const void* q;       /* [B][H][Ln][D] */
+  void* out;
+  const void *k, *v;   /* [B][Hk][L][D] */
+  const void *prefix_k, *prefix_v; /* [Hk][Lp][D]; not read with Lp 0 */
+  int64_t strides[18]; /* {b, h, l} in elements of q, out, k, v, prefix_k, prefix_v (b not read for the prefix) */
+  const int32_t* lengths;  /* [B] */
+  const float* slopes;     /* slopes, table and buckets as in sa_attn_scored */
+  const void* table;
+  const int32_t* buckets;
+  float sm_scale, cap;
+  void* workspace;         /* sa_attn_cached_workspace bytes, 256-byte aligned: sums of keys that are split over workgroups */
+  int64_t workspace_bytes;
+} sa_attn_cached;
+
+/* Reads the sizes. */
+int sa_attn_cached_workspace(const sa_attn_cached* call, int64_t* bytes);
+
+/* bf16, fp16 or fp32, D = 64 or 128, at most 2^29 keys. Results repeat bit for bit. */
+int sa_attn_cached_fwd(const sa_attn_cached* call, void* stream);
+
+/*
  * ranges [B][L][2] of sequences in which n documents of lengths[b][0 .. n) lie one after the other from token 0 (cut off at
  * L; tokens behind the last one are seen by no row). A document's first prefix[b][i] tokens are seen by all its rows.
  * Of the others, with causal, a row sees those of its own frame (groups of `frame` tokens behind the prefix; 1: itself)

@@ -19,6 +19,7 @@ _SUBMODULES = (
     "utils.block_sparse_attn_grad",
     "utils.rotary",
     "utils.scored_attn",
+    "utils.cached_attn",
     "utils.merge_unmerge",
     "utils.mask_related",
     "utils.attn_pooling_kernel",

@@ -52,6 +52,15 @@ class AttnScored(ctypes.Structure):
                    ("workspace_bytes", ctypes.c_int64)])
 
 
+class AttnCached(ctypes.Structure):
+    """sa_attn_cached of include/sa_api.h."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "B", "H", "Hk", "Ln", "L", "Lp", "D", "window", "table_dtype",
+                                               "n_buckets", "radius")]
+                + [(n, _P) for n in ("q", "out", "k", "v", "prefix_k", "prefix_v")] + [("strides", ctypes.c_int64 * 18)]
+                + [(n, _P) for n in ("lengths", "slopes", "table", "buckets")]
+                + [("sm_scale", _F), ("cap", _F), ("workspace", _P), ("workspace_bytes", ctypes.c_int64)])
+
+
 # name -> (restype, argtypes); must match include/sa_api.h.
 _PROTOTYPES = {
     "sa_abi_version": (_I, []),
@@ -96,6 +105,8 @@ _PROTOTYPES = {
     "sa_attn_scored_sizes": (_I, [ctypes.POINTER(AttnScored), _I64P, _I64P]),
     "sa_attn_scored_fwd": (_I, [ctypes.POINTER(AttnScored), _P]),
     "sa_attn_scored_bwd": (_I, [ctypes.POINTER(AttnScored), _P]),
+    "sa_attn_cached_workspace": (_I, [ctypes.POINTER(AttnCached), _I64P]),
+    "sa_attn_cached_fwd": (_I, [ctypes.POINTER(AttnCached), _P]),
     "sa_row_ranges": (_I, [_P, _P, _I, _I, _I, _I, _I, _I, _P, _P]),
     "sa_rotary_table": (_I, [_P, _I, _I64P, ctypes.c_int64, _I, _P, _P, _P, _P, _P]),
     "sa_rotary_apply": (

@@ -1,0 +1,456 @@
+// Attention of a few new tokens of each sequence over its cached keys and values, and over a prefix that all sequences
+// share, with the score rule of attn_scored.hip.
+//
+// Sequence b has lengths[b] cached tokens, of which the last Ln are the new ones; behind the Lp tokens of the shared prefix.
+// New token i is the sequence's own token t = lengths[b] - Ln + i, at distance d = t - j from own key j and d = Lp + t - j
+// from prefix key j; it sees keys at 0 <= d (< window, if there is one), and none where t < 0.
+//
+// A call reads every cached key and value once, and that is its bound (one new token: 2 operations a byte in 16 bits, against
+// the card's 300), so the work is dealt out by keys: a sequence's and key head's rows (its query heads' new tokens) share one
+// read of the keys as the columns of a 32-wide matrix product, and the keys are split over workgroups and their waves.
+// The prefix's keys are read once for the rows of all sequences, 32 rows a workgroup. Each wave copies its steps of 32
+// keys into LDS stages of its own, with no barrier between steps; a workgroup's waves join their sums in LDS, and
+// cached_merge_kernel joins the workgroups', in order: results do not depend on the order in which they run.
+#include <math.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "attn_score.h"
+
+namespace {
+
+struct Cache {
+  const void *k, *v;
+  int64_t k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;  // elements
+};
+
+struct CachedArgs {
+  const void* q;
+  void* out;
+  int64_t q_sb, q_sh, q_sl, o_sb, o_sh, o_sl;
+  Cache own, prefix;
+  const int32_t* lengths;
+  int B, H, Hk, rep, Ln, L, Lp, window;
+  int tiles, splits;                // 32-row tiles of a sequence's rows of a key head, and workgroups that share their keys
+  int prefix_tiles, prefix_splits;  // of all sequences' rows of a key head, and alike for the prefix
+  int own_groups;                   // B * Hk * tiles * splits workgroups, and behind them the prefix's
+  float scale_log2, cap_in, cap_log2;
+  const float* slopes;
+  const void* table;
+  const int32_t* buckets;
+  int table_dtype, n_buckets, radius;
+  float *sums, *parts;  // [workgroup][32] {offset, sum}, and [workgroup][32][kD]; null: the output is written
+};
+
+template <typename T, int kD>
+struct CachedShape {
+  static constexpr int kRow = kD * (int)sizeof(T);
+  static constexpr int kMat = kStep * kRow;  // a step's keys or values
+  // Waves of a workgroup: two stages of 2 kMat bytes each.
+  static constexpr int kWaves = kRow <= 256 ? 4 : 2;
+};
+
+template <bool kCap, typename T, int kD>
+__global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kernel(CachedArgs a) {
+  constexpr int kSize = sizeof(T), kRow = CachedShape<T, kD>::kRow, kMat = CachedShape<T, kD>::kMat;
+  constexpr int kWaves = CachedShape<T, kD>::kWaves;
+  constexpr int kDS = kRow / 32, kDC = kD / 32, kPieces = kRow / 128;
+  __shared__ __attribute__((aligned(1024))) uint8_t tile0[kWaves * 2 * kMat], tile1[kWaves * 2 * kMat];
+  __shared__ float joined[kWaves][2][kStep];
+
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, hh = lane >> 5;
+  const bool shared = (int)blockIdx.x >= a.own_groups;
+  int x = shared ? blockIdx.x - a.own_groups : blockIdx.x;
+  const int splits = shared ? a.prefix_splits : a.splits, tiles = shared ? a.prefix_tiles : a.tiles;
+  const int split = x % splits;
+  x /= splits;
+  const int tile = x % tiles;
+  x /= tiles;
+  const int hk = shared ? x : x % a.Hk, b0 = shared ? 0 : x / a.Hk;
+
+  // The lane's row: of sequence b, query head h, new token i.
+  const int per = a.rep * a.Ln, n_rows = shared ? a.B * per : per;
+  const int row = tile * kStep + col;
+  const int r = min(row, n_rows - 1);  // (rows past the last one are computed like it and not stored)
+  const int b = shared ? r / per : b0, in = shared ? r - b * per : r;
+  const int h = hk * a.rep + in / a.Ln, i = in % a.Ln;
+  const int t = min(max(a.lengths[b], 0), a.L) - a.Ln + i;
+  const int place = shared ? a.Lp + t : t;  // d = place - key
+  sa_u32x4v fa[kDS];
+  {
+    const uint8_t* p = static_cast<const uint8_t*>(a.q) + (b * a.q_sb + h * a.q_sh + i * a.q_sl) * kSize + 16 * hh;
+#pragma unroll
+    for (int s = 0; s < kDS; ++s) fa[s] = *reinterpret_cast<const sa_u32x4v*>(p + 32 * s);
+  }
+  const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+  auto bias_at = [&](int d) {
+    const int n = min(max(a.buckets[min(max(d, -a.radius), a.radius) + a.radius], 0), a.n_buckets - 1);
+    return load_as_float(a.table, a.table_dtype, (int64_t)n * a.H + h) * kLog2e;
+  };
+  const float past = a.table ? bias_at(a.radius) : 0.f;
+
+  // Nearest and furthest row of the tile, and whether one sees nothing.
+  int near = t >= 0 ? place : INT_MAX, far = t >= 0 ? place : -1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    near = min(near, __shfl_xor(near, o));
+    far = max(far, __shfl_xor(far, o));
+  }
+  near = __builtin_amdgcn_readfirstlane(near);
+  far = __builtin_amdgcn_readfirstlane(far);
+  const bool blind = __ballot(t < 0) != 0;
+  // The tile's keys, whole steps of them from the first that a row sees, and the split's and wave's share.
+  const int end = shared ? a.Lp : __builtin_amdgcn_readfirstlane(min(max(a.lengths[b0], 0), a.L));
+  int first = 0;
+  if (a.window && near != INT_MAX) first = max(0, min(near - a.window + 1, end)) / kStep;
+  const int n_steps = far < 0 ? 0 : (end + kStep - 1) / kStep - first;
+  const int per_split = (n_steps + splits - 1) / splits;
+  const int last = min(n_steps, per_split * (split + 1));
+  const int begin = split * per_split + w;  // steps begin, begin + kWaves, ..
+
+  const Cache& c = shared ? a.prefix : a.own;
+  const uint8_t* kp = static_cast<const uint8_t*>(c.k) + (b0 * c.k_sb + hk * c.k_sh) * kSize;
+  const uint8_t* vp = static_cast<const uint8_t*>(c.v) + (b0 * c.v_sb + hk * c.v_sh) * kSize;
+  // Copies of a step's keys and values: rows past the last cached one read as zero whatever is there.
+  auto issue = [&](int step, lds_u8* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int64_t row_bytes = (m == 0 ? c.k_sl : c.v_sl) * kSize;
+#pragma unroll
+      for (int r16 = 0; r16 < 2; ++r16) {
+        const int row0 = (first + step) * kStep + 16 * r16;
+        const int64_t left = row0 < end ? (end - 1 - row0) * row_bytes + 128 : 0;
+        const int size = __builtin_amdgcn_readfirstlane((int)min(left, (int64_t)INT_MAX));
+        const uint8_t* from = (m == 0 ? kp : vp) + row0 * row_bytes;
+#pragma unroll
+        for (int hf = 0; hf < kPieces; ++hf) {
+          const __amdgpu_buffer_rsrc_t rsrc =
+              __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from + 128 * hf), (short)0, size, 0x00020000);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int lr = 8 * j + (lane >> 3);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rsrc, (lds_u8*)(to + (w * 2 + m) * kMat + hf * kStep * 128 + 2048 * r16 + 1024 * j), 16,
+                lr * (int)row_bytes + 16 * ((lane & 7) ^ swz(lr)), 0, 0, 0);
+          }
+        }
+      }
+    }
+  };
+
+  const TileReads<T, kD> reads(lane);
+  sa_f32x16 acc[kDC];
+#pragma unroll
+  for (int dc = 0; dc < kDC; ++dc) acc[dc] = sa_f32x16{};
+  float m = -INFINITY, l = 0.f;
+
+  auto compute = [&](int step, const lds_u8* from) __attribute__((always_inline)) {
+    const lds_u8* mat = from + w * 2 * kMat;
+    const int row0 = (first + step) * kStep;
+    sa_f32x16 S = {};
+#pragma unroll
+    for (int s = 0; s < kDS; ++s) S = mfma_chunk<T>(lds_read_b128(reads.row(mat, s)), fa[s], S);
+    float sc = a.scale_log2;
+    if constexpr (kCap) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float none;
+        S[e] = bend<T, false>(S[e] * a.cap_in, none) * a.cap_log2;
+      }
+      sc = 1.f;
+    }
+    const int base = place - row0 - 4 * hh;  // d = base - c_e
+    if (a.slopes) {
+      const float f = slope * (float)base;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) S[e] = fmaf(S[e], sc, -fabsf(fmaf(slope, -(float)(8 * (e >> 2) + (e & 3)), f)));
+      sc = 1.f;
+    }
+    if (a.table) {
+      if (near - row0 - 31 >= a.radius) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[e] = fmaf(S[e], sc, past);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[e] = fmaf(S[e], sc, bias_at(base - (8 * (e >> 2) + (e & 3))));
+      }
+      sc = 1.f;
+    }
+    if (blind || row0 + 31 > near || row0 + 31 >= end || (a.window && far - row0 >= a.window)) {
+      const unsigned most = a.window ? a.window : 0x80000000u;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int k = 8 * (e >> 2) + (e & 3);
+        if (t < 0 || (unsigned)(base - k) >= most || row0 + 4 * hh + k >= end) S[e] = -INFINITY;
+      }
+    }
+    float top = S[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) top = fmaxf(top, S[e]);
+    top = xhalf_max(top) * sc;
+    if (__ballot(top > m + kSlack)) {
+      const float next_m = fmaxf(m, top);
+      const float f = next_m == m ? 1.f : fast_exp2(m - next_m);
+      m = next_m;
+      l *= f;
+#pragma unroll
+      for (int dc = 0; dc < kDC; ++dc)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dc][e] *= f;
+    }
+    const float off = m == -INFINITY ? 0.f : m;
+    Weights<T> P;
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) P.set(e, fast_exp2(fmaf(S[e], sc, -off)), fast_exp2(fmaf(S[e + 1], sc, -off)));
+    l = P.sum(l);
+    reads.product(mat + kMat, P, acc);
+  };
+
+  // The copies of a wave's next step run while it computes; the stage that they overwrite has been read.
+  lds_u8* const t0 = (lds_u8*)tile0;
+  lds_u8* const t1 = (lds_u8*)tile1;
+  if (begin < last) issue(begin, t0);
+  for (int s = begin; s < last; s += 2 * kWaves) {
+    __builtin_amdgcn_s_waitcnt(kWaitVmLgkm0);
+    if (s + kWaves < last) issue(s + kWaves, t1);
+    compute(s, t0);
+    if (s + kWaves >= last) break;
+    __builtin_amdgcn_s_waitcnt(kWaitVmLgkm0);
+    if (s + 2 * kWaves < last) issue(s + 2 * kWaves, t0);
+    compute(s + kWaves, t1);
+  }
+
+  // ---- The waves' sums: [wave][32 rows][kD] over the stages, 16-byte chunks swizzled by the row.
+  l = xhalf_sum(l);
+  if (hh == 0) {
+    joined[w][0][col] = m;
+    joined[w][1][col] = l;
+  }
+  __syncthreads();  // (every wave is done with its stages, too)
+  constexpr int kCh = kD / 4;
+  float* mine = reinterpret_cast<float*>(tile0) + w * kStep * kD;
+  static_assert(kWaves * kStep * kD * 4 <= kWaves * 2 * kMat, "the sums fit a stage");
+#pragma unroll
+  for (int dc = 0; dc < kDC; ++dc)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+      *reinterpret_cast<float4*>(mine + col * kD + 4 * ((8 * dc + 2 * q4 + hh) ^ (col & (kCh - 1)))) =
+          make_float4(acc[dc][4 * q4], acc[dc][4 * q4 + 1], acc[dc][4 * q4 + 2], acc[dc][4 * q4 + 3]);
+  __syncthreads();
+  const int group = blockIdx.x;
+  for (int at = threadIdx.x; at < kStep * kCh; at += 64 * kWaves) {
+    const int rr = at / kCh, ch = at % kCh;
+    if (tile * kStep + rr >= n_rows) break;
+    float top = joined[0][0][rr];
+#pragma unroll
+    for (int v = 1; v < kWaves; ++v) top = fmaxf(top, joined[v][0][rr]);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float mv = joined[v][0][rr], f = mv == top ? 1.f : fast_exp2(mv - top);
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(tile0) + (v * kStep + rr) * kD +
+                                                        4 * (ch ^ (rr & (kCh - 1))));
+      s.x = fmaf(y.x, f, s.x);
+      s.y = fmaf(y.y, f, s.y);
+      s.z = fmaf(y.z, f, s.z);
+      s.w = fmaf(y.w, f, s.w);
+      sum = fmaf(joined[v][1][rr], f, sum);
+    }
+    if (a.parts) {
+      *reinterpret_cast<float4*>(a.parts + ((int64_t)group * kStep + rr) * kD + 4 * ch) = s;
+      if (ch == 0) *reinterpret_cast<float2*>(a.sums + ((int64_t)group * kStep + rr) * 2) = make_float2(top, sum);
+      continue;
+    }
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    const int in_ = tile * kStep + rr;  // (no prefix: a row of sequence b0)
+    uint8_t* p = static_cast<uint8_t*>(a.out) +
+                 (b0 * a.o_sb + (hk * a.rep + in_ / a.Ln) * a.o_sh + (in_ % a.Ln) * a.o_sl + 4 * ch) * kSize;
+    if constexpr (std::is_same<T, float>::value)
+      *reinterpret_cast<float4*>(p) = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
+    else
+      *reinterpret_cast<uint2*>(p) = make_uint2(Elem<T>::pack(s.x * f, s.y * f), Elem<T>::pack(s.z * f, s.w * f));
+  }
+}
+
+// out = the workgroups' sums of each row, those of its own keys and then those of the prefix: kD / 4 lanes a row.
+template <typename T, int kD>
+__global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs a) {
+  constexpr int kCh = kD / 4;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kCh;
+  if (at >= (int64_t)a.B * a.H * a.Ln) return;
+  const int ch = threadIdx.x % kCh;
+  const int i = (int)(at % a.Ln), h = (int)(at / a.Ln % a.H), b = (int)(at / a.Ln / a.H);
+  const int hk = h / a.rep, in = (h - hk * a.rep) * a.Ln + i, all = b * a.rep * a.Ln + in;
+  // Place of the s-th sums of the row, in units of rows.
+  const int n = a.splits + (a.Lp ? a.prefix_splits : 0);
+  auto place = [&](int s) {
+    if (s < a.splits) {
+      const int64_t g = ((int64_t)(b * a.Hk + hk) * a.tiles + in / kStep) * a.splits + s;
+      return g * kStep + in % kStep;
+    }
+    const int64_t g = a.own_groups + ((int64_t)hk * a.prefix_tiles + all / kStep) * a.prefix_splits + s - a.splits;
+    return g * kStep + all % kStep;
+  };
+  float top = -INFINITY;
+  for (int s = 0; s < n; ++s) top = fmaxf(top, a.sums[2 * place(s)]);
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const int64_t p = place(s);
+    const float2 x = *reinterpret_cast<const float2*>(a.sums + 2 * p);
+    const float f = x.x == top ? 1.f : fast_exp2(x.x - top);
+    const float4 y = *reinterpret_cast<const float4*>(a.parts + p * kD + 4 * ch);
+    r.x = fmaf(y.x, f, r.x);
+    r.y = fmaf(y.y, f, r.y);
+    r.z = fmaf(y.z, f, r.z);
+    r.w = fmaf(y.w, f, r.w);
+    sum = fmaf(x.y, f, sum);
+  }
+  const float f = sum == 0.f ? 0.f : 1.f / sum;
+  uint8_t* p = static_cast<uint8_t*>(a.out) + (b * a.o_sb + h * a.o_sh + i * a.o_sl + 4 * ch) * (int64_t)sizeof(T);
+  if constexpr (std::is_same<T, float>::value)
+    *reinterpret_cast<float4*>(p) = make_float4(r.x * f, r.y * f, r.z * f, r.w * f);
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(Elem<T>::pack(r.x * f, r.y * f), Elem<T>::pack(r.z * f, r.w * f));
+}
+
+// ---- Host side.
+
+constexpr int kTarget = 512;      // workgroups that a call aims at: two on each of the 256 CUs
+constexpr int kLeastSteps = 8;    // of a workgroup, before the keys are split further
+
+struct CachedPlan {
+  int tiles, splits, prefix_tiles, prefix_splits;
+  int64_t own_groups, groups, sums, bytes;
+};
+
+int plan_cached(const sa_attn_cached& t, const char* fn, CachedPlan& p) {
+  const int64_t per = (int64_t)(t.H / t.Hk) * t.Ln;
+  const int64_t tiles = (per + kStep - 1) / kStep, prefix_tiles = t.Lp ? (t.B * per + kStep - 1) / kStep : 0;
+  const int64_t items = t.B * t.Hk * tiles, prefix_items = t.Hk * prefix_tiles;
+  if (t.B * per >= 1LL << 30 || items + prefix_items >= 1LL << 22)
+    return sa::fail(SA_ERR_UNSUPPORTED, "%s: too many rows", fn);
+  // Splits in proportion to the keys, so that workgroups have alike many of them, about kTarget in all.
+  const int64_t steps = (t.L + kStep - 1) / kStep, prefix_steps = t.Lp ? (t.Lp + kStep - 1) / kStep : 0;
+  const int64_t all = items * steps + prefix_items * prefix_steps;
+  const int64_t each = std::max<int64_t>(kLeastSteps, (all + kTarget - 1) / kTarget);
+  p.tiles = (int)tiles;
+  p.prefix_tiles = (int)prefix_tiles;
+  p.splits = (int)std::max<int64_t>(1, (steps + each - 1) / each);
+  p.prefix_splits = t.Lp ? (int)std::max<int64_t>(1, (prefix_steps + each - 1) / each) : 0;
+  p.own_groups = items * p.splits;
+  p.groups = p.own_groups + prefix_items * p.prefix_splits;
+  const bool merged = p.splits > 1 || t.Lp;
+  p.sums = (p.groups * kStep * 8 + 255) / 256 * 256;
+  p.bytes = merged ? p.sums + p.groups * kStep * t.D * 4 : 0;
+  return SA_OK;
+}
+
+int check_cached(const sa_attn_cached* t, const char* fn) {
+  SA_REQUIRE(t, "%s: null call", fn);
+  SA_REQUIRE(t->dtype >= SA_DTYPE_BF16 && t->dtype <= SA_DTYPE_F32, "%s: dtype %d", fn, t->dtype);
+  SA_REQUIRE(t->B > 0 && t->H > 0 && t->Hk > 0 && t->Ln > 0 && t->L > 0 && t->Lp >= 0,
+             "%s: bad shape B=%d H=%d Hk=%d Ln=%d L=%d Lp=%d", fn, t->B, t->H, t->Hk, t->Ln, t->L, t->Lp);
+  SA_REQUIRE(t->H % t->Hk == 0, "%s: %d query heads over %d key heads", fn, t->H, t->Hk);
+  SA_REQUIRE(t->window >= 0, "%s: window %d", fn, t->window);
+  if (t->D != 64 && t->D != 128) return sa::fail(SA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", fn, t->D);
+  if (t->L > 1 << 29 || t->Lp > 1 << 29) return sa::fail(SA_ERR_UNSUPPORTED, "%s: more than 2^29 keys", fn);
+  SA_REQUIRE(t->sm_scale > 0.f && std::isfinite(t->sm_scale), "%s: sm_scale must be positive and finite", fn);
+  SA_REQUIRE(t->cap >= 0.f && std::isfinite(t->cap), "%s: cap must be positive and finite, or 0 for none", fn);
+  SA_REQUIRE(!t->cap || (t->cap > 1e-30f && std::isfinite(t->sm_scale / t->cap * 3.f) && t->sm_scale / t->cap > 0.f),
+             "%s: sm_scale / cap out of range", fn);
+  if (t->table) {
+    SA_REQUIRE(t->buckets && t->n_buckets > 0, "%s: table without buckets", fn);
+    SA_REQUIRE(t->table_dtype >= SA_DTYPE_BF16 && t->table_dtype <= SA_DTYPE_F32, "%s: table dtype %d", fn, t->table_dtype);
+    if (t->radius < 0 || t->radius > kMostRadius)
+      return sa::fail(SA_ERR_UNSUPPORTED, "%s: distances up to %d told apart (at most %d)", fn, t->radius, kMostRadius);
+  }
+  return SA_OK;
+}
+
+template <bool kCap, typename T, int kD>
+void launch_cached(const CachedArgs& a, const CachedPlan& p, hipStream_t s) {
+  hipLaunchKernelGGL((cached_kernel<kCap, T, kD>), dim3((unsigned)p.groups), dim3(64 * CachedShape<T, kD>::kWaves), 0, s, a);
+  if (!p.bytes) return;
+  const int64_t threads = (int64_t)a.B * a.H * a.Ln * (kD / 4);
+  hipLaunchKernelGGL((cached_merge_kernel<T, kD>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a);
+}
+
+template <typename T>
+void launch_type(const CachedArgs& a, const CachedPlan& p, int D, bool cap, hipStream_t s) {
+  if (D == 64 && cap) launch_cached<true, T, 64>(a, p, s);
+  else if (D == 64) launch_cached<false, T, 64>(a, p, s);
+  else if (cap) launch_cached<true, T, 128>(a, p, s);
+  else launch_cached<false, T, 128>(a, p, s);
+}
+
+}  // namespace
+
+extern "C" int sa_attn_cached_workspace(const sa_attn_cached* t, int64_t* bytes) {
+  const char* fn = "sa_attn_cached_workspace";
+  SA_REQUIRE(bytes, "%s: null bytes", fn);
+  if (int rc = check_cached(t, fn)) return rc;
+  CachedPlan p;
+  if (int rc = plan_cached(*t, fn, p)) return rc;
+  *bytes = p.bytes;
+  return sa::ok();
+}
+
+extern "C" int sa_attn_cached_fwd(const sa_attn_cached* t, void* stream) {
+  const char* fn = "sa_attn_cached_fwd";
+  if (int rc = check_cached(t, fn)) return rc;
+  SA_REQUIRE(t->q && t->k && t->v && t->out && t->lengths && (!t->Lp || (t->prefix_k && t->prefix_v)), "%s: null pointer", fn);
+  CachedPlan p;
+  if (int rc = plan_cached(*t, fn, p)) return rc;
+  const int size = t->dtype == SA_DTYPE_F32 ? 4 : 2, per16 = 16 / size;
+  const void* ptrs[6] = {t->q, t->out, t->k, t->v, t->prefix_k, t->prefix_v};
+  for (int i = 0; i < (t->Lp ? 6 : 4); ++i) {
+    if (reinterpret_cast<uintptr_t>(ptrs[i]) % 16 != 0)
+      return sa::fail(SA_ERR_UNSUPPORTED, "%s: tensor base not 16-byte aligned", fn);
+    for (int j = 0; j < 3; ++j)
+      if (t->strides[3 * i + j] % per16 != 0)
+        return sa::fail(SA_ERR_UNSUPPORTED, "%s: strides must be multiples of %d elements", fn, per16);
+    // (a step's rows are reached through 32-bit offsets)
+    if (t->strides[3 * i + 2] < 0 || t->strides[3 * i + 2] > 1 << 24)
+      return sa::fail(SA_ERR_UNSUPPORTED, "%s: rows more than 2^24 elements apart", fn);
+  }
+  SA_REQUIRE(!p.bytes || (t->workspace && reinterpret_cast<uintptr_t>(t->workspace) % 256 == 0),
+             "%s: workspace null or not 256-byte aligned", fn);
+  SA_REQUIRE(t->workspace_bytes >= p.bytes, "%s: workspace of %lld bytes < %lld", fn, (long long)t->workspace_bytes,
+             (long long)p.bytes);
+  CachedArgs a{};
+  const int64_t* st = t->strides;
+  a.q = t->q; a.q_sb = st[0]; a.q_sh = st[1]; a.q_sl = st[2];
+  a.out = t->out; a.o_sb = st[3]; a.o_sh = st[4]; a.o_sl = st[5];
+  a.own = Cache{t->k, t->v, st[6], st[7], st[8], st[9], st[10], st[11]};
+  a.prefix = Cache{t->prefix_k, t->prefix_v, st[12], st[13], st[14], st[15], st[16], st[17]};
+  a.lengths = t->lengths;
+  a.B = t->B; a.H = t->H; a.Hk = t->Hk; a.rep = t->H / t->Hk;
+  a.Ln = t->Ln; a.L = t->L; a.Lp = t->Lp; a.window = t->window;
+  a.tiles = p.tiles; a.splits = p.splits;
+  a.prefix_tiles = p.prefix_tiles; a.prefix_splits = p.prefix_splits;
+  a.own_groups = (int)p.own_groups;
+  a.scale_log2 = t->sm_scale * kLog2e;
+  if (t->cap > 0) {
+    a.cap_in = t->sm_scale / t->cap * (t->dtype == SA_DTYPE_F32 ? 1.f : 2.f * kLog2e);
+    a.cap_log2 = t->cap * kLog2e;
+  }
+  a.slopes = t->slopes;
+  a.table = t->table; a.buckets = t->buckets;
+  a.table_dtype = t->table_dtype; a.n_buckets = t->n_buckets; a.radius = t->radius;
+  if (p.bytes) {
+    a.sums = static_cast<float*>(t->workspace);
+    a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(t->workspace) + p.sums);
+  }
+  hipStream_t s = sa::as_stream(stream);
+  if (t->dtype == SA_DTYPE_BF16) launch_type<__bf16>(a, p, t->D, t->cap > 0, s);
+  else if (t->dtype == SA_DTYPE_F16) launch_type<_Float16>(a, p, t->D, t->cap > 0, s);
+  else launch_type<float>(a, p, t->D, t->cap > 0, s);
+  return sa::check_launch(fn);
+}
