@@ -331,21 +331,25 @@ typedef struct sa_attn_scored {
   const void* table;       /* nullable [n_buckets][H] */
   const int32_t* buckets;  /* [2*radius+1]; entries outside [0, n_buckets) are taken as the nearest one */
   int32_t table_dtype, n_buckets, radius;
-  int32_t key_lists;       /* whether the plan has the lists of the key blocks, which dk and dv need */
+  int32_t follow;          /* SA_SCORED_*: gradients that the backward call is to give besides dq */
   void* dtable;            /* nullable [n_buckets][H] of the table's type: sum of dS over each bucket's pairs */
-  void* plan;              /* lists and biases, written by the forward call and read by the backward call */
+  void* plan;              /* lists, biases and units of work, written by the forward call and read by the backward call */
   int64_t plan_bytes;
-  void* workspace;         /* of the backward call */
+  void* workspace;         /* of the call that is made */
   int64_t workspace_bytes;
+  void* out_lo;            /* 16-bit types, nullable, laid out like out: what its rounding leaves. Forward: written; */
+                           /* backward: read, so that rowsum(do * out) has the bits that dS = P (dP - rowsum) needs */
 } sa_attn_scored;
+#define SA_SCORED_KEYS 1  /* dk, dv */
+#define SA_SCORED_TABLE 2 /* dtable */
 
-/* Bytes of a call's plan and of its backward call's workspace (both 256-byte aligned). Reads the sizes, dtype,
- * key_lists, radius, and whether there are ranges, a mask, a table and a dtable. */
-int sa_attn_scored_sizes(const sa_attn_scored* call, int64_t* plan_bytes, int64_t* workspace_bytes);
+/* Bytes of a call's plan, and of the forward and the backward call's workspaces (all 256-byte aligned). Reads the sizes,
+ * dtype, q_start, follow, radius, and whether there are ranges, a mask and a table. */
+int sa_attn_scored_sizes(const sa_attn_scored* call, int64_t bytes[3]);
 
 /*
- * out and each row's log2-sum-exp2: +inf, and a row of zeros, for a row that sees no key. bf16, fp16 (P rounded to the
- * type) or fp32, D = 64 or 128. Keys and values of listed blocks have to be finite, also where a row does not see them.
+ * out and each row's log2-sum-exp2: +inf, and a row of zeros, for a row that sees no key. bf16 and fp16 (P as two terms
+ * of the type) or fp32, D = 64 or 128. Keys and values of listed blocks have to be finite, also where a row does not see them.
  * At most 2^27 rows, and less than 2 GiB from a head's first row to its last. Reads neither dout nor the gradients.
  */
 int sa_attn_scored_fwd(const sa_attn_scored* call, void* stream);

@@ -47,9 +47,9 @@ class AttnScored(ctypes.Structure):
                 + [("strides", ctypes.c_int64 * 24), ("lse", _P), ("ranges", _P), ("ranges_stride", ctypes.c_int64),
                    ("mask", _P), ("mask_strides", ctypes.c_int64 * 4), ("sm_scale", _F), ("cap", _F), ("slopes", _P),
                    ("table", _P), ("buckets", _P)]
-                + [(n, ctypes.c_int32) for n in ("table_dtype", "n_buckets", "radius", "key_lists")]
+                + [(n, ctypes.c_int32) for n in ("table_dtype", "n_buckets", "radius", "follow")]
                 + [("dtable", _P), ("plan", _P), ("plan_bytes", ctypes.c_int64), ("workspace", _P),
-                   ("workspace_bytes", ctypes.c_int64)])
+                   ("workspace_bytes", ctypes.c_int64), ("out_lo", _P)])
 
 
 class AttnCached(ctypes.Structure):
@@ -102,7 +102,7 @@ _PROTOTYPES = {
     "sa_block_sparse_bwd_workspace": (_I, [ctypes.POINTER(AttnTrain), _I64P]),
     "sa_block_sparse_bwd_check": (_I, [ctypes.POINTER(AttnTrain)]),
     "sa_block_sparse_bwd": (_I, [ctypes.POINTER(AttnTrain), _P]),
-    "sa_attn_scored_sizes": (_I, [ctypes.POINTER(AttnScored), _I64P, _I64P]),
+    "sa_attn_scored_sizes": (_I, [ctypes.POINTER(AttnScored), _I64P]),
     "sa_attn_scored_fwd": (_I, [ctypes.POINTER(AttnScored), _P]),
     "sa_attn_scored_bwd": (_I, [ctypes.POINTER(AttnScored), _P]),
     "sa_attn_cached_workspace": (_I, [ctypes.POINTER(AttnCached), _I64P]),

@@ -41,6 +41,7 @@ from .block_sparse_attn_grad import _rows16
 from .block_sparse_attn_kernel import BLOCK
 
 MOST_RADIUS = 1024  # distances that a bias tells apart
+_KEYS, _TABLE = 1, 2  # SA_SCORED_KEYS, SA_SCORED_TABLE
 
 
 def distance_buckets(n_buckets: int, radius: int, bidirectional: bool = True, device="cuda") -> torch.Tensor:
@@ -163,7 +164,7 @@ class ScoredState:
 
     __slots__ = ("tensors", "numbers")
 
-    NAMES = ("q", "k", "v", "out", "lse", "plan", "ranges", "slopes", "table", "buckets")
+    NAMES = ("q", "k", "v", "out", "out_lo", "lse", "plan", "ranges", "slopes", "table", "buckets")
 
     def __init__(self, tensors, numbers):
         self.tensors, self.numbers = tensors, numbers
@@ -180,11 +181,11 @@ def _set(call, **tensors):
 
 
 def _describe(q, k, v, slopes, table, buckets, ranges, numbers):
-    """A call's description; numbers: (sm_scale, cap, q_start, key_lists, masked)."""
-    sm_scale, cap, q_start, key_lists, masked = numbers
+    """A call's description; numbers: (sm_scale, cap, q_start, follow, masked)."""
+    sm_scale, cap, q_start, follow, masked = numbers
     B, H, Lq, D = q.shape
     call = _lib.AttnScored(dtype=_lib.DTYPES[q.dtype], B=B, H=H, Hk=k.shape[1], Lq=Lq, Lk=k.shape[2], D=D, q_start=q_start,
-                           sm_scale=sm_scale, cap=cap, key_lists=key_lists)
+                           sm_scale=sm_scale, cap=cap, follow=follow)
     _set(call, q=q, k=k, v=v)
     if slopes is not None:
         call.slopes = slopes.data_ptr()
@@ -199,9 +200,10 @@ def _describe(q, k, v, slopes, table, buckets, ranges, numbers):
 
 
 def _sizes(call):
-    plan, work = ctypes.c_int64(0), ctypes.c_int64(0)
-    _lib.check(_lib.load().sa_attn_scored_sizes(call, ctypes.byref(plan), ctypes.byref(work)), "sa_attn_scored_sizes")
-    return plan.value, work.value
+    """Bytes of the plan and of the two calls' workspaces."""
+    n = (ctypes.c_int64 * 3)()
+    _lib.check(_lib.load().sa_attn_scored_sizes(call, n), "sa_attn_scored_sizes")
+    return n
 
 
 def _check_ranges(ranges, q, B, Lk):
@@ -245,36 +247,47 @@ def _check(q, k, v, cap, slopes, table, buckets, ranges, block_mask, q_start):
     return cap, slopes, table, buckets, ranges, block_mask
 
 
-def _forward(q, k, v, sm_scale, cap, slopes, table, buckets, ranges, mask, q_start, key_lists):
-    """(out, state) on checked arguments."""
+def _forward(q, k, v, sm_scale, cap, slopes, table, buckets, ranges, mask, q_start, follow):
+    """(out, state) on checked arguments. follow: _KEYS and _TABLE, or None: no gradient."""
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    numbers = (sm_scale, cap, q_start, key_lists, mask is not None)
+    numbers = (sm_scale, cap, q_start, follow or 0, mask is not None)
     call = _describe(q, k, v, slopes, table, buckets, ranges, numbers)
     if mask is not None:
         call.mask = mask.data_ptr()
         call.mask_strides[:] = mask.stride()
     B, H, Lq, D = q.shape
     out = torch.empty((B, H, Lq, D), dtype=q.dtype, device=q.device)
+    out_lo = None
+    if follow is not None and q.dtype != torch.float32:
+        out_lo = torch.empty_like(out)
+        call.out_lo = out_lo.data_ptr()
     lse = torch.empty((B, H, -(-Lq // BLOCK) * BLOCK), dtype=torch.float32, device=q.device)
-    plan_bytes = _sizes(call)[0]
+    plan_bytes, n, _ = _sizes(call)
     plan = torch.empty(plan_bytes, dtype=torch.uint8, device=q.device)
     _set(call, out=out)
     call.lse, call.plan, call.plan_bytes = lse.data_ptr(), plan.data_ptr(), plan_bytes
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        call.workspace, call.workspace_bytes = ws.data_ptr(), n
     with _lib.on(q.device):
         rc = _lib.load().sa_attn_scored_fwd(call, _lib.stream_of(q))
     _lib.check(rc, "sa_attn_scored_fwd")
-    return out, ScoredState((q, k, v, out, lse, plan, ranges, slopes, table, buckets), numbers)
+    return out, ScoredState((q, k, v, out, out_lo, lse, plan, ranges, slopes, table, buckets), numbers)
 
 
 def _backward(dout, state, needs):
     """(dq, dk, dv, dtable), None where not needed."""
-    q, k, v, out, lse, plan, ranges, slopes, table, buckets = state.tensors
+    q, k, v, out, out_lo, lse, plan, ranges, slopes, table, buckets = state.tensors
     q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
     dout = _rows16(dout)
     if (dout.shape[2] + BLOCK) * dout.stride(2) * dout.element_size() >= 1 << 30:  # (rows far apart: 32-bit offsets)
         dout = dout.contiguous()
     call = _describe(q, k, v, slopes, table, buckets, ranges, state.numbers)
     _set(call, out=out, dout=dout)
+    if out_lo is not None:
+        if out_lo.stride() != out.stride():  # (hooks on saved tensors have moved one of them)
+            out_lo = torch.empty_strided(out.shape, out.stride(), dtype=out.dtype, device=out.device).copy_(out_lo)
+        call.out_lo = out_lo.data_ptr()
     call.lse, call.plan, call.plan_bytes = lse.data_ptr(), plan.data_ptr(), plan.numel()
     grads = [None] * 4
     for i, (name, like) in enumerate((("dq", q), ("dk", k), ("dv", v))):
@@ -284,7 +297,7 @@ def _backward(dout, state, needs):
     if needs[3]:
         grads[3] = torch.empty_like(table)
         call.dtable = grads[3].data_ptr()
-    n = _sizes(call)[1]
+    n = _sizes(call)[2]
     ws = torch.empty(n, dtype=torch.uint8, device=q.device)
     call.workspace, call.workspace_bytes = ws.data_ptr(), n
     with _lib.on(q.device):
@@ -300,13 +313,13 @@ def scored_attention_forward(q, k, v, sm_scale: float, *, cap: Optional[float] =
     if q.numel() == 0 or k.numel() == 0:
         raise ValueError(f"no query or no key: q{tuple(q.shape)} k{tuple(k.shape)}")
     with torch.no_grad():
-        return _forward(q, k, v, float(sm_scale), *checked, int(q_start), True)
+        return _forward(q, k, v, float(sm_scale), *checked, int(q_start), _KEYS | (0 if table is None else _TABLE))
 
 
 def scored_attention_backward(dout, state: ScoredState, needs=(True, True, True, True)):
     """(dq, dk, dv, dtable) for the gradient dout of `scored_attention_forward`'s out, whose tensors must be as
     they were; None where `needs` is false, and for dtable without a table."""
-    q, table = state.tensors[0], state.tensors[8]
+    q, table = state.tensors[0], state.tensors[9]
     _lib.require_gpu(dout)
     if dout.shape != q.shape or dout.dtype != q.dtype or dout.device != q.device:
         raise ValueError(f"dout must be like q: {tuple(q.shape)} {q.dtype}, got {tuple(dout.shape)} {dout.dtype}")
@@ -316,8 +329,8 @@ def scored_attention_backward(dout, state: ScoredState, needs=(True, True, True,
 
 class _ScoredAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, sm_scale, cap, slopes, buckets, ranges, mask, q_start, followed):
-        out, state = _forward(q, k, v, sm_scale, cap, slopes, table, buckets, ranges, mask, q_start, followed)
+    def forward(ctx, q, k, v, table, sm_scale, cap, slopes, buckets, ranges, mask, q_start, follow):
+        out, state = _forward(q, k, v, sm_scale, cap, slopes, table, buckets, ranges, mask, q_start, follow)
         ctx.numbers = state.numbers
         ctx.save_for_backward(*state.tensors)
         return out
@@ -365,6 +378,10 @@ def scored_attention(q, k, v, sm_scale: float, *, cap: Optional[float] = None, s
         raise ValueError(f"sm_scale {sm_scale} must be positive and finite")
     if q.numel() == 0 or k.numel() == 0:
         return _Nothing.apply(q, k, v, table)
-    followed = torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)
+    follow = None
+    if torch.is_grad_enabled():
+        of_keys, of_table = k.requires_grad or v.requires_grad, table is not None and table.requires_grad
+        if q.requires_grad or of_keys or of_table:
+            follow = (_KEYS if of_keys else 0) | (_TABLE if of_table else 0)
     return _ScoredAttention.apply(q, k, v, table, float(sm_scale), cap, slopes, buckets, ranges, block_mask, int(q_start),
-                                  followed)
+                                  follow)
