@@ -76,6 +76,23 @@ struct Weights<float> {
   }
 };
 
+// Two weights as two terms of the type each, exact to its bits twice over. bf16: the upper halves of the floats, so that
+// they are picked out of the registers, and the rest rounded.
+template <typename T>
+__device__ __forceinline__ void set_two_terms(Weights<T>& hi, Weights<T>& lo, int e, float a, float b) {
+  if constexpr (std::is_same<T, float>::value) {
+    hi.set(e, a, b);
+  } else if constexpr (std::is_same<T, __bf16>::value) {
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    hi.w[e >> 1] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+    lo.set(e, a - __uint_as_float(x & 0xffff0000u), b - __uint_as_float(y & 0xffff0000u));
+  } else {
+    hi.set(e, a, b);
+    const float2 p = unpack2<T>(hi.w[e >> 1]);
+    lo.set(e, a - p.x, b - p.y);
+  }
+}
+
 // tanh(y) and 1 - tanh(y)^2 from two exponentials' accuracy to the type's. 16-bit types: 1 - 2 / (exp2(y') + 1), whose
 // error is absolute, 2^-23; y' = 2 log2(e) y is the argument. fp32: below 0.6 the odd polynomial through tanh(y) / y at
 // Chebyshev nodes (relative error 7e-8), because a small score would otherwise lose its bits.
@@ -138,6 +155,32 @@ struct TileReads {
     }
   }
   __device__ inline const lds_u8* row(const lds_u8* mat, int c) const { return mat + ro[c & 3] + (c >> 2) * kPiece; }
+  // 16-bit types: 64 columns transposed, and to += those columns' rows^T W.
+  struct Columns {
+    sa_u32x4v x[2][2];  // [16 streamed rows][32 columns]
+  };
+  __device__ __forceinline__ Columns columns(const lds_u8* mat, int hf) const {
+    Columns r;
+    if constexpr (!kF32) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int dc = 0; dc < 2; ++dc) {
+          const lds_u8* p = mat + hf * kPiece + 2048 * u;
+          const uint2 r0 = lds_read_tr16(p + tr[2 * dc]), r1 = lds_read_tr16(p + tr[2 * dc + 1]);
+          r.x[u][dc] = sa_u32x4v{r0.x, r0.y, r1.x, r1.y};
+        }
+    }
+    return r;
+  }
+  __device__ __forceinline__ void product(const Columns& c, int hf, const Weights<T>& W, sa_f32x16 (&to)[kD / 32]) const {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int dc = 0; dc < 2; ++dc)
+        to[2 * hf + dc] = mfma_chunk<T>(c.x[u][dc], sa_u32x4v{W.w[4 * u], W.w[4 * u + 1], W.w[4 * u + 2], W.w[4 * u + 3]},
+                                        to[2 * hf + dc]);
+  }
   __device__ __forceinline__ void product(const lds_u8* mat, const Weights<T>& W, sa_f32x16 (&to)[kD / 32]) const {
     if constexpr (kF32) {
 #pragma unroll
@@ -150,17 +193,7 @@ struct TileReads {
         }
     } else {
 #pragma unroll
-      for (int hf = 0; hf < kD / 64; ++hf)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int dc = 0; dc < 2; ++dc) {
-            const lds_u8* p = mat + hf * kPiece + 2048 * u;
-            const uint2 r0 = lds_read_tr16(p + tr[2 * dc]), r1 = lds_read_tr16(p + tr[2 * dc + 1]);
-            to[2 * hf + dc] = mfma_chunk<T>(sa_u32x4v{r0.x, r0.y, r1.x, r1.y},
-                                            sa_u32x4v{W.w[4 * u], W.w[4 * u + 1], W.w[4 * u + 2], W.w[4 * u + 3]},
-                                            to[2 * hf + dc]);
-          }
+      for (int hf = 0; hf < kD / 64; ++hf) product(columns(mat, hf), hf, W, to);
     }
   }
 };
