@@ -412,6 +412,11 @@ __global__ __launch_bounds__(256) void row_ranges_kernel(RangeArgs a) {
 
 constexpr int kDirect = 32;
 
+// Where both sides have few blocks and there is no block mask, a call walks over all of them, cut ones all.
+bool has_lists(const sa_attn_scored& t) {
+  return t.mask || (t.ranges && std::max(t.Lq, t.Lk) > 4 * kBlk);
+}
+
 struct SidePlan {  // how a side's items are dealt out; byte offsets into a call's plan buffer
   bool scheduled, sorted;
   int slots, least, max_units, cap, split_cap, unit_cost, split_cost, merge_cost, part_cost;
@@ -460,7 +465,7 @@ struct Buffer {
 Plan plan_of(const sa_attn_scored& t) {
   Plan p;
   const int64_t nqb = sa::cdiv(t.Lq, kBlk), nkb = sa::cdiv(t.Lk, kBlk);
-  const int64_t lists = t.ranges || t.mask ? (int64_t)t.B * (t.mask ? t.H : 1) : 0;
+  const int64_t lists = has_lists(t) ? (int64_t)t.B * (t.mask ? t.H : 1) : 0;
   const bool keys = t.follow & SA_SCORED_KEYS;
   Buffer buf;
   p.bounds = buf.take(t.ranges && nkb > kDirect ? t.B * nkb * 16 : 0);
@@ -606,7 +611,7 @@ void own_queries(ScoredArgs& a, const sa_attn_scored& t, const Plan& p) {
   a.own_a = side_of(t, t.q, 0);
   a.st_a = side_of(t, t.k, 1);
   a.st_b = side_of(t, t.v, 2);
-  if (t.ranges || t.mask) {
+  if (has_lists(t)) {
     a.idx = reinterpret_cast<const int32_t*>(plan + p.kv_idx);
     a.cnt = reinterpret_cast<const int32_t*>(plan + p.kv_cnt);
   }
@@ -666,9 +671,9 @@ extern "C" int sa_attn_scored_fwd(const sa_attn_scored* t, void* stream) {
   hipStream_t s = sa::as_stream(stream);
   uint8_t* plan = static_cast<uint8_t*>(t->plan);
   const int nqb = sa::cdiv(t->Lq, kBlk), nkb = sa::cdiv(t->Lk, kBlk);
-  const bool lists = t->ranges || t->mask, keys = t->follow & SA_SCORED_KEYS;
+  const bool lists = has_lists(*t), keys = t->follow & SA_SCORED_KEYS;
   // Bounds of few key blocks are taken from the ranges where they are needed.
-  const int4* bounds = t->ranges && nkb > kDirect ? reinterpret_cast<const int4*>(plan + p.bounds) : nullptr;
+  const int4* bounds = t->ranges && lists && nkb > kDirect ? reinterpret_cast<const int4*>(plan + p.bounds) : nullptr;
   if (bounds) {
     const int64_t n = (int64_t)t->B * nkb;
     hipLaunchKernelGGL(scored_bounds_kernel, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s,
@@ -741,7 +746,7 @@ extern "C" int sa_attn_scored_bwd(const sa_attn_scored* t, void* stream) {
   if (int rc = check_scored(t, fn)) return rc;
   SA_REQUIRE(t->q && t->k && t->v && t->out && t->dout && t->lse, "%s: null pointer", fn);
   if (int rc = check_operands(t, fn, 0, 8)) return rc;
-  const bool lists = t->ranges || t->mask, keys = t->dk || t->dv;
+  const bool lists = has_lists(*t), keys = t->dk || t->dv;
   SA_REQUIRE((!keys || (t->follow & SA_SCORED_KEYS)) && (!t->dtable || (t->follow & SA_SCORED_TABLE)),
              "%s: gradients that the plan does not follow", fn);
   const Plan p = plan_of(*t);

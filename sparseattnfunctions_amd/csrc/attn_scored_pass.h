@@ -46,7 +46,7 @@ struct ScoredArgs {
   int H, rep;             // query heads, and how many share a key head
   int L_own, L_st, n_own, n_st, q_start;
   // Lists of the own blocks: entries (block << 1 | cut) idx[row * width ..], cnt[row] of them, row = ((b or, per_head,
-  // b * H + query head) * n_own + block); idx null: every block.
+  // b * H + query head) * n_own + block); idx null: every block, all cut if there are ranges.
   const int32_t *idx, *cnt;
   int per_head;
   const int2* ranges;  // [b * ranges_sb + key] = {from, until}; may be null
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
     }
     Step s = {-1, 0, half, g, slope_h * kLog2e, past, before};
     if (pos < cnt && left > 0) {
-      const int e = a.idx ? ahead : 2 * pos + (kBlk * (pos + 1) > a.L_st);
+      const int e = a.idx ? ahead : 2 * pos + (a.ranges || kBlk * (pos + 1) > a.L_st);
       s.block = e >> 1;
       s.cut = e & 1;
       // (the second half of a block that ends before it is left out)

@@ -31,6 +31,7 @@ mask and the slopes are not differentiated.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -67,6 +68,16 @@ def distance_buckets(n_buckets: int, radius: int, bidirectional: bool = True, de
     return torch.tensor(places, dtype=torch.int32, device=device)
 
 
+_INTEGERS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
+def _int32(t, most):
+    """t as contiguous int32 (64-bit numbers no larger than `most`, above which they all mean the same)."""
+    if t.dtype != torch.int32:
+        t = (t.clamp(-1, most) if t.dtype == torch.int64 else t).to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def row_ranges(lengths: torch.Tensor, L: int, causal: bool = True, prefix: Optional[torch.Tensor] = None, frame: int = 1,
                window: int = 0) -> torch.Tensor:
     """ranges int32 [B, L, 2] of B sequences that pack documents of `lengths` (integers [B, n], or [n] for
@@ -78,31 +89,33 @@ def row_ranges(lengths: torch.Tensor, L: int, causal: bool = True, prefix: Optio
     `frame` tokens, counted from behind the prefix; a row that is not causal sees all. With a window a key
     outside the prefix is seen by no row that lies `window` tokens or more behind it (or, not causal,
     before it)."""
-    tensors = (lengths,) if prefix is None else (lengths, prefix)
-    _lib.require_gpu(*tensors)
+    device = lengths.device
+    if device.type != "cuda":
+        _lib.require_gpu(lengths)
     if lengths.dim() == 1:
         lengths = lengths[None]
-    if lengths.dim() != 2 or lengths.shape[1] == 0 or lengths.is_floating_point():
+    if lengths.dim() != 2 or lengths.shape[1] == 0 or lengths.dtype not in _INTEGERS:
         raise ValueError(f"lengths must be integers [B, n], got {lengths.dtype} {tuple(lengths.shape)}")
     B, n = lengths.shape
-    if prefix is not None:
-        if prefix.is_floating_point() or prefix.device != lengths.device:
-            raise ValueError("prefix must be integers on the device of lengths")
-        prefix = prefix.expand(B, n).to(torch.int32).contiguous()
     L, frame, window = int(L), int(frame), int(window)
     if L < 0:
         raise ValueError(f"L={L}")
     if max(L, frame, window) >= 2 ** 31:
         raise ValueError(f"L={L} frame={frame} window={window}: sizes of 32 bits")
-    out = torch.empty(B, L, 2, dtype=torch.int32, device=lengths.device)
-    if out.numel() == 0:
+    if prefix is not None:
+        if prefix.device != device:
+            _lib.require_gpu(prefix)
+            raise ValueError("lengths and prefix must be on one device")
+        if prefix.dtype not in _INTEGERS:
+            raise ValueError(f"prefix must be integers, got {prefix.dtype}")
+        prefix = _int32(prefix if prefix.shape == (B, n) else prefix.expand(B, n), L)
+    lengths = _int32(lengths, L)
+    out = torch.empty((B, L, 2), dtype=torch.int32, device=device)
+    if B == 0 or L == 0:
         return out
-    if lengths.dtype == torch.int64:  # (a longer one is cut off at L anyway)
-        lengths = lengths.clamp(0, L)
-    lengths = lengths.to(torch.int32).contiguous()
-    with _lib.on(out.device):
-        rc = _lib.load().sa_row_ranges(lengths.data_ptr(), _lib.ptr(prefix), B, n, L, int(bool(causal)), frame, window,
-                                       out.data_ptr(), _lib.stream_of(out))
+    with _lib.on(device):
+        rc = _lib.load().sa_row_ranges(lengths.data_ptr(), None if prefix is None else prefix.data_ptr(), B, n, L,
+                                       1 if causal else 0, frame, window, out.data_ptr(), _lib.stream_of(out))
     _lib.check(rc, "sa_row_ranges")
     return out
 
@@ -131,8 +144,9 @@ def check_rule(q, H: int, cap, slopes, table, buckets):
         if radius > MOST_RADIUS:
             raise NotImplementedError(f"distances up to {radius} told apart (at most {MOST_RADIUS})")
         table, buckets = table.contiguous(), buckets.contiguous()
+    device = q.device
     for t in (slopes, table, buckets):
-        if t is not None and t.device != q.device:
+        if t is not None and t.device != device:
             _lib.require_gpu(t)
             raise ValueError("q, k, v and the rule's tensors must be on one device")
     return 0.0 if cap is None else float(cap), slopes, table, buckets, radius
@@ -140,8 +154,9 @@ def check_rule(q, H: int, cap, slopes, table, buckets):
 
 def check_heads(q, k, v):
     """(B, H, Hk, Lq, Lk, D) of q [B,H,Lq,D] and k, v [B,Hk,Lk,D]."""
-    _lib.require_gpu(q, k, v)
-    if not q.device == k.device == v.device:
+    device = q.device
+    if device.type != "cuda" or k.device != device or v.device != device:
+        _lib.require_gpu(q, k, v)
         raise ValueError("q, k and v must be on one device")
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"q, k, v must be [B, H, L, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -159,51 +174,66 @@ def check_heads(q, k, v):
 
 
 class ScoredState:
-    """What `scored_attention_forward` keeps for `scored_attention_backward`: the tensors and the call's
-    description."""
+    """What `scored_attention_forward` keeps for `scored_attention_backward`: q, k, v, out, one buffer (the
+    plan, the rows' log2-sum-exp2 and what out's rounding leaves), ranges, slopes, table and buckets, and the
+    call's description."""
 
-    __slots__ = ("tensors", "numbers")
+    __slots__ = ("tensors", "call", "args")
 
-    NAMES = ("q", "k", "v", "out", "out_lo", "lse", "plan", "ranges", "slopes", "table", "buckets")
-
-    def __init__(self, tensors, numbers):
-        self.tensors, self.numbers = tensors, numbers
-
-
-_PLACES = {name: 3 * i for i, name in enumerate(("q", "k", "v", "out", "dout", "dq", "dk", "dv"))}
+    def __init__(self, tensors, call, args):
+        self.tensors, self.call, self.args = tensors, call, args
 
 
-def _set(call, **tensors):
-    for name, t in tensors.items():
-        setattr(call, name, t.data_ptr())
-        at = _PLACES[name]
-        call.strides[at:at + 3] = t.stride()[:3]
+_ORDER = ("q", "k", "v", "out", "dout", "dq", "dk", "dv")  # of AttnScored.strides
 
 
-def _describe(q, k, v, slopes, table, buckets, ranges, numbers):
-    """A call's description; numbers: (sm_scale, cap, q_start, follow, masked)."""
-    sm_scale, cap, q_start, follow, masked = numbers
-    B, H, Lq, D = q.shape
-    call = _lib.AttnScored(dtype=_lib.DTYPES[q.dtype], B=B, H=H, Hk=k.shape[1], Lq=Lq, Lk=k.shape[2], D=D, q_start=q_start,
-                           sm_scale=sm_scale, cap=cap, follow=follow)
-    _set(call, q=q, k=k, v=v)
-    if slopes is not None:
-        call.slopes = slopes.data_ptr()
-    if table is not None:
-        call.table, call.buckets = table.data_ptr(), buckets.data_ptr()
-        call.table_dtype, call.n_buckets, call.radius = _lib.DTYPES[table.dtype], table.shape[0], buckets.numel() // 2
+class _Call:
+    """What calls of one shape share: a description without pointers, and the sizes of their buffers."""
+
+    def __init__(self, dtype, q_shape, k_shape, strides, sm_scale, cap, q_start, slopes, table, ranges, mask, follow):
+        (B, H, Lq, D), (_, Hk, Lk, _) = q_shape, k_shape
+        args = self.args = _lib.AttnScored(dtype=_lib.DTYPES[dtype], B=B, H=H, Hk=Hk, Lq=Lq, Lk=Lk, D=D, q_start=q_start,
+                                           sm_scale=sm_scale, cap=cap, follow=follow or 0)
+        self.strides = strides  # of q, k and v; the others' are contiguous, dout's are set where they are not
+        of_q, of_k = (H * Lq * D, Lq * D, D), (Hk * Lk * D, Lk * D, D)
+        args.strides[:] = (*(x for t in strides for x in t[:3]), *of_q, *of_q, *of_q, *of_k, *of_k)
+        if slopes:
+            args.slopes = 1  # (the sizes depend on what there is; the pointers follow)
+        if table is not None:
+            args.table = args.buckets = 1
+            args.table_dtype, args.n_buckets, args.radius = _lib.DTYPES[table[0]], table[1], table[2]
+        if ranges is not None:
+            args.ranges, args.ranges_stride = 1, ranges
+        if mask is not None:
+            args.mask = 1
+            args.mask_strides[:] = mask
+        n = (ctypes.c_int64 * 3)()
+        _lib.check(_lib.load().sa_attn_scored_sizes(args, n), "sa_attn_scored_sizes")
+        args.plan_bytes, self.fwd_bytes, self.bwd_bytes = n[0], n[1], n[2]
+        self.out, self.grads = (B, H, Lq, D), ((B, H, Lq, D), (B, Hk, Lk, D), (B, Hk, Lk, D))
+        self.contiguous = (*of_q, 1)
+        # The buffer: the plan (a multiple of 256 bytes), the sums, the rest of out.
+        self.lse_at = n[0]
+        rows = B * H * (-(-Lq // BLOCK)) * BLOCK
+        self.lo_at = self.lse_at + 4 * rows if follow is not None and dtype != torch.float32 else None
+        self.buffer_bytes = self.lse_at + 4 * rows + (0 if self.lo_at is None else 2 * B * H * Lq * D)
+
+
+_call = functools.lru_cache(maxsize=1024)(_Call)
+
+
+def _point(call, args, q, k, v, out, buffer, ranges, slopes, table, buckets):
+    args.q, args.k, args.v, args.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    args.plan = at = buffer.data_ptr()
+    args.lse = at + call.lse_at
+    if call.lo_at is not None:
+        args.out_lo = at + call.lo_at
     if ranges is not None:
-        call.ranges, call.ranges_stride = ranges.data_ptr(), ranges.stride(0) // 2
-    if masked:  # (the backward call reads its lists)
-        call.mask = 1
-    return call
-
-
-def _sizes(call):
-    """Bytes of the plan and of the two calls' workspaces."""
-    n = (ctypes.c_int64 * 3)()
-    _lib.check(_lib.load().sa_attn_scored_sizes(call, n), "sa_attn_scored_sizes")
-    return n
+        args.ranges = ranges.data_ptr()
+    if slopes is not None:
+        args.slopes = slopes.data_ptr()
+    if table is not None:
+        args.table, args.buckets = table.data_ptr(), buckets.data_ptr()
 
 
 def _check_ranges(ranges, q, B, Lk):
@@ -250,60 +280,60 @@ def _check(q, k, v, cap, slopes, table, buckets, ranges, block_mask, q_start):
 def _forward(q, k, v, sm_scale, cap, slopes, table, buckets, ranges, mask, q_start, follow):
     """(out, state) on checked arguments. follow: _KEYS and _TABLE, or None: no gradient."""
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    numbers = (sm_scale, cap, q_start, follow or 0, mask is not None)
-    call = _describe(q, k, v, slopes, table, buckets, ranges, numbers)
+    device = q.device
+    call = _call(q.dtype, q.shape, k.shape, (q.stride(), k.stride(), v.stride()), sm_scale, cap, q_start, slopes is not None,
+                 None if table is None else (table.dtype, table.shape[0], buckets.numel() // 2),
+                 None if ranges is None else ranges.stride(0) // 2, None if mask is None else mask.stride(), follow)
+    out = torch.empty(call.out, dtype=q.dtype, device=device)
+    buffer = torch.empty(call.buffer_bytes, dtype=torch.uint8, device=device)
+    args = _lib.AttnScored.from_buffer_copy(call.args)
+    _point(call, args, q, k, v, out, buffer, ranges, slopes, table, buckets)
     if mask is not None:
-        call.mask = mask.data_ptr()
-        call.mask_strides[:] = mask.stride()
-    B, H, Lq, D = q.shape
-    out = torch.empty((B, H, Lq, D), dtype=q.dtype, device=q.device)
-    out_lo = None
-    if follow is not None and q.dtype != torch.float32:
-        out_lo = torch.empty_like(out)
-        call.out_lo = out_lo.data_ptr()
-    lse = torch.empty((B, H, -(-Lq // BLOCK) * BLOCK), dtype=torch.float32, device=q.device)
-    plan_bytes, n, _ = _sizes(call)
-    plan = torch.empty(plan_bytes, dtype=torch.uint8, device=q.device)
-    _set(call, out=out)
-    call.lse, call.plan, call.plan_bytes = lse.data_ptr(), plan.data_ptr(), plan_bytes
-    if n:
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-        call.workspace, call.workspace_bytes = ws.data_ptr(), n
-    with _lib.on(q.device):
-        rc = _lib.load().sa_attn_scored_fwd(call, _lib.stream_of(q))
-    _lib.check(rc, "sa_attn_scored_fwd")
-    return out, ScoredState((q, k, v, out, out_lo, lse, plan, ranges, slopes, table, buckets), numbers)
+        args.mask = mask.data_ptr()
+    if call.fwd_bytes:
+        ws = torch.empty(call.fwd_bytes, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), call.fwd_bytes
+    with _lib.on(device):
+        rc = _lib.load().sa_attn_scored_fwd(args, _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "sa_attn_scored_fwd")
+    return out, ScoredState((q, k, v, out, buffer, ranges, slopes, table, buckets), call, args)
 
 
 def _backward(dout, state, needs):
     """(dq, dk, dv, dtable), None where not needed."""
-    q, k, v, out, out_lo, lse, plan, ranges, slopes, table, buckets = state.tensors
-    q, k, v, out = _rows16(q), _rows16(k), _rows16(v), _rows16(out)
-    dout = _rows16(dout)
-    if (dout.shape[2] + BLOCK) * dout.stride(2) * dout.element_size() >= 1 << 30:  # (rows far apart: 32-bit offsets)
-        dout = dout.contiguous()
-    call = _describe(q, k, v, slopes, table, buckets, ranges, state.numbers)
-    _set(call, out=out, dout=dout)
-    if out_lo is not None:
-        if out_lo.stride() != out.stride():  # (hooks on saved tensors have moved one of them)
-            out_lo = torch.empty_strided(out.shape, out.stride(), dtype=out.dtype, device=out.device).copy_(out_lo)
-        call.out_lo = out_lo.data_ptr()
-    call.lse, call.plan, call.plan_bytes = lse.data_ptr(), plan.data_ptr(), plan.numel()
+    q, k, v, out, buffer, ranges, slopes, table, buckets = state.tensors
+    call = state.call
+    args = _lib.AttnScored.from_buffer_copy(state.args)  # (this may run twice, or in two threads)
+    if (q.stride(), k.stride(), v.stride()) != call.strides or out.stride() != call.contiguous \
+            or not all(t.data_ptr() % 16 == 0 for t in (q, k, v, out)):  # (hooks on saved tensors have moved them)
+        q, k, v, out = _rows16(q), _rows16(k), _rows16(v), out.contiguous()
+        args.strides[:9] = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+    if table is not None and not table.is_contiguous():
+        table = table.contiguous()
+    _point(call, args, q, k, v, out, buffer, ranges, slopes, table, buckets)
+    if dout.stride() != call.contiguous or dout.data_ptr() % 16:
+        dout = _rows16(dout)
+        if (dout.shape[2] + BLOCK) * dout.stride(2) * dout.element_size() >= 1 << 30:  # (rows far apart: 32-bit offsets)
+            dout = dout.contiguous()
+        args.strides[12:15] = dout.stride()[:3]
+    args.dout = dout.data_ptr()
+    device, dtype = q.device, q.dtype
     grads = [None] * 4
-    for i, (name, like) in enumerate((("dq", q), ("dk", k), ("dv", v))):
+    for i, name in enumerate(("dq", "dk", "dv")):
         if needs[i]:
-            grads[i] = torch.empty(like.shape, dtype=like.dtype, device=like.device)
-            _set(call, **{name: grads[i]})
+            grads[i] = g = torch.empty(call.grads[i], dtype=dtype, device=device)
+            setattr(args, name, g.data_ptr())
     if needs[3]:
         grads[3] = torch.empty_like(table)
-        call.dtable = grads[3].data_ptr()
-    n = _sizes(call)[2]
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    call.workspace, call.workspace_bytes = ws.data_ptr(), n
-    with _lib.on(q.device):
-        rc = _lib.load().sa_attn_scored_bwd(call, _lib.stream_of(q))
-    _lib.check(rc, "sa_attn_scored_bwd")
-    return tuple(grads)
+        args.dtable = grads[3].data_ptr()
+    ws = torch.empty(call.bwd_bytes, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), call.bwd_bytes
+    with _lib.on(device):
+        rc = _lib.load().sa_attn_scored_bwd(args, _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "sa_attn_scored_bwd")
+    return grads
 
 
 def scored_attention_forward(q, k, v, sm_scale: float, *, cap: Optional[float] = None, slopes=None, table=None, buckets=None,
@@ -319,19 +349,19 @@ def scored_attention_forward(q, k, v, sm_scale: float, *, cap: Optional[float] =
 def scored_attention_backward(dout, state: ScoredState, needs=(True, True, True, True)):
     """(dq, dk, dv, dtable) for the gradient dout of `scored_attention_forward`'s out, whose tensors must be as
     they were; None where `needs` is false, and for dtable without a table."""
-    q, table = state.tensors[0], state.tensors[9]
+    q, table = state.tensors[0], state.tensors[7]
     _lib.require_gpu(dout)
     if dout.shape != q.shape or dout.dtype != q.dtype or dout.device != q.device:
         raise ValueError(f"dout must be like q: {tuple(q.shape)} {q.dtype}, got {tuple(dout.shape)} {dout.dtype}")
     with torch.no_grad():
-        return _backward(dout, state, (*needs[:3], needs[3] and table is not None))
+        return tuple(_backward(dout, state, (*needs[:3], needs[3] and table is not None)))
 
 
 class _ScoredAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, sm_scale, cap, slopes, buckets, ranges, mask, q_start, follow):
         out, state = _forward(q, k, v, sm_scale, cap, slopes, table, buckets, ranges, mask, q_start, follow)
-        ctx.numbers = state.numbers
+        ctx.call, ctx.args = state.call, state.args
         ctx.save_for_backward(*state.tensors)
         return out
 
@@ -339,9 +369,8 @@ class _ScoredAttention(torch.autograd.Function):
     def backward(ctx, dout):
         if torch.is_grad_enabled():
             raise RuntimeError("scored attention is differentiable once (create_graph=True is not supported)")
-        needs = ctx.needs_input_grad
-        dq, dk, dv, dtable = _backward(dout, ScoredState(ctx.saved_tensors, ctx.numbers), needs[:4])
-        return (dq, dk, dv, dtable) + (None,) * 8
+        grads = _backward(dout, ScoredState(ctx.saved_tensors, ctx.call, ctx.args), ctx.needs_input_grad)
+        return (*grads, None, None, None, None, None, None, None, None)
 
 
 class _Nothing(torch.autograd.Function):
