@@ -52,11 +52,18 @@ struct CachedShape {
   static constexpr int kWaves = kRow <= 256 ? 4 : 2;
 };
 
+template <typename T>
+__device__ __forceinline__ void store_four(uint8_t* row, int at, float x, float y, float z, float w) {
+  if constexpr (std::is_same<T, float>::value) *reinterpret_cast<float4*>(row + 4 * at) = make_float4(x, y, z, w);
+  else *reinterpret_cast<uint2*>(row + 2 * at) = make_uint2(Elem<T>::pack(x, y), Elem<T>::pack(z, w));
+}
+
+// kPieces: a piece of the row of all steps (parts is not null); else an item.
 template <bool kCap, typename T, int kD>
 __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kernel(CachedArgs a) {
   constexpr int kSize = sizeof(T), kRow = CachedShape<T, kD>::kRow, kMat = CachedShape<T, kD>::kMat;
   constexpr int kWaves = CachedShape<T, kD>::kWaves;
-  constexpr int kDS = kRow / 32, kDC = kD / 32, kPieces = kRow / 128;
+  constexpr int kDS = kRow / 32, kDC = kD / 32, kParts = kRow / 128;
   __shared__ __attribute__((aligned(1024))) uint8_t tile0[kWaves * 2 * kMat], tile1[kWaves * 2 * kMat];
   __shared__ float joined[kWaves][2][kStep];
 
@@ -86,12 +93,12 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 #pragma unroll
     for (int s = 0; s < kDS; ++s) fa[s] = *reinterpret_cast<const sa_u32x4v*>(p + 32 * s);
   }
-  const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+  float slope = a.slopes ? a.slopes[h] * kLog2e : 0.f;
   auto bias_at = [&](int d) {
     const int n = min(max(a.buckets[min(max(d, -a.radius), a.radius) + a.radius], 0), a.n_buckets - 1);
     return load_as_float(a.table, a.table_dtype, (int64_t)n * a.H + h) * kLog2e;
   };
-  const float past = a.table ? bias_at(a.radius) : 0.f;
+  float past = a.table ? bias_at(a.radius) : 0.f;
 
   // Nearest and furthest row of the tile, and whether one sees nothing.
   int near = t >= 0 ? place : INT_MAX, far = t >= 0 ? place : -1;
@@ -115,7 +122,8 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
   const Cache& c = shared ? a.prefix : a.own;
   const uint8_t* kp = static_cast<const uint8_t*>(c.k) + (b0 * c.k_sb + hk * c.k_sh) * kSize;
   const uint8_t* vp = static_cast<const uint8_t*>(c.v) + (b0 * c.v_sb + hk * c.v_sh) * kSize;
-  // Copies of a step's keys and values: rows past the last cached one read as zero whatever is there.
+  // Copies of a step's keys and values: rows past the last cached one, and steps past the wave's last, read as zero whatever is
+  // there.
   auto issue = [&](int step, lds_u8* to) __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -123,11 +131,11 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 #pragma unroll
       for (int r16 = 0; r16 < 2; ++r16) {
         const int row0 = (first + step) * kStep + 16 * r16;
-        const int64_t left = row0 < end ? (end - 1 - row0) * row_bytes + 128 : 0;
+        const int64_t left = step < last && row0 < end ? (end - 1 - row0) * row_bytes + 128 : 0;
         const int size = __builtin_amdgcn_readfirstlane((int)min(left, (int64_t)INT_MAX));
         const uint8_t* from = (m == 0 ? kp : vp) + row0 * row_bytes;
 #pragma unroll
-        for (int hf = 0; hf < kPieces; ++hf) {
+        for (int hf = 0; hf < kParts; ++hf) {
           const __amdgpu_buffer_rsrc_t rsrc =
               __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from + 128 * hf), (short)0, size, 0x00020000);
 #pragma unroll
@@ -152,8 +160,15 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
     const lds_u8* mat = from + w * 2 * kMat;
     const int row0 = (first + step) * kStep;
     sa_f32x16 S = {};
+    sa_u32x4v x[kDS];
 #pragma unroll
-    for (int s = 0; s < kDS; ++s) S = mfma_chunk<T>(lds_read_b128(reads.row(mat, s)), fa[s], S);
+    for (int s = 0; s < kDS; ++s) x[s] = lds_read_b128(reads.row(mat, s));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < kDS; ++s) S = mfma_chunk<T>(x[s], fa[s], S);
+    // (the first values are requested before the exponentials)
+    typename TileReads<T, kD>::Columns values = reads.columns(mat + kMat, 0);
+    __builtin_amdgcn_sched_barrier(0);
     float sc = a.scale_log2;
     if constexpr (kCap) {
 #pragma unroll
@@ -207,22 +222,38 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 #pragma unroll
     for (int e = 0; e < 16; e += 2) P.set(e, fast_exp2(fmaf(S[e], sc, -off)), fast_exp2(fmaf(S[e + 1], sc, -off)));
     l = P.sum(l);
-    reads.product(mat + kMat, P, acc);
+    if constexpr (std::is_same<T, float>::value) {
+      reads.product(mat + kMat, P, acc);
+    } else {
+#pragma unroll
+      for (int hf = 0; hf < kD / 64; ++hf) {
+        const auto now = values;
+        if (hf + 1 < kD / 64) values = reads.columns(mat + kMat, hf + 1);
+        reads.product(now, hf, P, acc);
+      }
+    }
   };
 
-  // The copies of a wave's next step run while it computes; the stage that they overwrite has been read.
+  // Both stages' copies are in flight but for the time in which one is computed on: a stage that has been read takes the step
+  // after next at once. What the row needs has landed before the first copy is on its way, and there are copies for every
+  // stage, past the last step empty ones: the compiler would else wait for all copies in every step.
   lds_u8* const t0 = (lds_u8*)tile0;
   lds_u8* const t1 = (lds_u8*)tile1;
-  if (begin < last) issue(begin, t0);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+#pragma unroll
+  for (int s = 0; s < kDS; ++s) asm volatile("" : "+v"(fa[s]));
+  asm volatile("" : "+v"(slope), "+v"(past));
+  issue(begin, t0);
+  issue(begin + kWaves, t1);
   for (int s = begin; s < last; s += 2 * kWaves) {
-    __builtin_amdgcn_s_waitcnt(kWaitVmLgkm0);
-    if (s + kWaves < last) issue(s + kWaves, t1);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(8 * kParts));
     compute(s, t0);
-    if (s + kWaves >= last) break;
-    __builtin_amdgcn_s_waitcnt(kWaitVmLgkm0);
-    if (s + 2 * kWaves < last) issue(s + 2 * kWaves, t0);
-    compute(s + kWaves, t1);
+    issue(s + 2 * kWaves, t0);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(8 * kParts));
+    if (s + kWaves < last) compute(s + kWaves, t1);
+    issue(s + 3 * kWaves, t1);
   }
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
 
   // ---- The waves' sums: [wave][32 rows][kD] over the stages, 16-byte chunks swizzled by the row.
   l = xhalf_sum(l);
@@ -269,61 +300,61 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
     const float f = sum == 0.f ? 0.f : 1.f / sum;
     const int in_ = tile * kStep + rr;  // (no prefix: a row of sequence b0)
     uint8_t* p = static_cast<uint8_t*>(a.out) +
-                 (b0 * a.o_sb + (hk * a.rep + in_ / a.Ln) * a.o_sh + (in_ % a.Ln) * a.o_sl + 4 * ch) * kSize;
-    if constexpr (std::is_same<T, float>::value)
-      *reinterpret_cast<float4*>(p) = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
-    else
-      *reinterpret_cast<uint2*>(p) = make_uint2(Elem<T>::pack(s.x * f, s.y * f), Elem<T>::pack(s.z * f, s.w * f));
+                 (b0 * a.o_sb + (hk * a.rep + in_ / a.Ln) * a.o_sh + (in_ % a.Ln) * a.o_sl) * kSize;
+    store_four<T>(p, 4 * ch, s.x * f, s.y * f, s.z * f, s.w * f);
   }
 }
 
-// out = the workgroups' sums of each row, those of its own keys and then those of the prefix: kD / 4 lanes a row.
+// out = the workgroups' sums of each row, those of its own keys and then those of the prefix: a wave per row, whose groups of
+// kD / 4 lanes take turns at them. A row without any is zeros.
 template <typename T, int kD>
 __global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs a) {
-  constexpr int kCh = kD / 4;
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kCh;
-  if (at >= (int64_t)a.B * a.H * a.Ln) return;
-  const int ch = threadIdx.x % kCh;
+  constexpr int kCh = kD / 4, kGroups = 64 / kCh;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= (int64_t)a.B * a.H * a.Ln) return;  // (the whole wave)
+  const int lane = threadIdx.x & 63, ch = lane % kCh, turn = lane / kCh;
   const int i = (int)(at % a.Ln), h = (int)(at / a.Ln % a.H), b = (int)(at / a.Ln / a.H);
   const int hk = h / a.rep, in = (h - hk * a.rep) * a.Ln + i, all = b * a.rep * a.Ln + in;
   // Place of the s-th sums of the row, in units of rows.
   const int n = a.splits + (a.Lp ? a.prefix_splits : 0);
-  auto place = [&](int s) {
-    if (s < a.splits) {
-      const int64_t g = ((int64_t)(b * a.Hk + hk) * a.tiles + in / kStep) * a.splits + s;
-      return g * kStep + in % kStep;
-    }
-    const int64_t g = a.own_groups + ((int64_t)hk * a.prefix_tiles + all / kStep) * a.prefix_splits + s - a.splits;
-    return g * kStep + all % kStep;
-  };
+  const int64_t own = ((int64_t)(b * a.Hk + hk) * a.tiles + in / kStep) * a.splits;
+  const int64_t shared = a.own_groups + ((int64_t)hk * a.prefix_tiles + all / kStep) * a.prefix_splits - a.splits;
+  auto place = [&](int s) { return s < a.splits ? (own + s) * kStep + in % kStep : (shared + s) * kStep + all % kStep; };
   float top = -INFINITY;
-  for (int s = 0; s < n; ++s) top = fmaxf(top, a.sums[2 * place(s)]);
-  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
+  for (int s = lane; s < n; s += 64) top = fmaxf(top, a.sums[2 * place(s)]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  float r[5] = {};  // the chunk, and the sum
 #pragma unroll 4
-  for (int s = 0; s < n; ++s) {
+  for (int s = turn; s < n; s += kGroups) {
     const int64_t p = place(s);
     const float2 x = *reinterpret_cast<const float2*>(a.sums + 2 * p);
     const float f = x.x == top ? 1.f : fast_exp2(x.x - top);
     const float4 y = *reinterpret_cast<const float4*>(a.parts + p * kD + 4 * ch);
-    r.x = fmaf(y.x, f, r.x);
-    r.y = fmaf(y.y, f, r.y);
-    r.z = fmaf(y.z, f, r.z);
-    r.w = fmaf(y.w, f, r.w);
-    sum = fmaf(x.y, f, sum);
+    r[0] = fmaf(y.x, f, r[0]);
+    r[1] = fmaf(y.y, f, r[1]);
+    r[2] = fmaf(y.z, f, r[2]);
+    r[3] = fmaf(y.w, f, r[3]);
+    r[4] = fmaf(x.y, f, r[4]);
   }
-  const float f = sum == 0.f ? 0.f : 1.f / sum;
-  uint8_t* p = static_cast<uint8_t*>(a.out) + (b * a.o_sb + h * a.o_sh + i * a.o_sl + 4 * ch) * (int64_t)sizeof(T);
-  if constexpr (std::is_same<T, float>::value)
-    *reinterpret_cast<float4*>(p) = make_float4(r.x * f, r.y * f, r.z * f, r.w * f);
-  else
-    *reinterpret_cast<uint2*>(p) = make_uint2(Elem<T>::pack(r.x * f, r.y * f), Elem<T>::pack(r.z * f, r.w * f));
+#pragma unroll
+  for (int o = kCh; o < 64; o <<= 1)
+#pragma unroll
+    for (int x = 0; x < 5; ++x) r[x] += __shfl_xor(r[x], o);
+  if (turn > 0) return;
+  const float f = r[4] == 0.f ? 0.f : 1.f / r[4];
+  store_four<T>(static_cast<uint8_t*>(a.out) + (b * a.o_sb + h * a.o_sh + i * a.o_sl) * (int64_t)sizeof(T), 4 * ch, r[0] * f,
+                r[1] * f, r[2] * f, r[3] * f);
 }
 
 // ---- Host side.
 
-constexpr int kTarget = 512;      // workgroups that a call aims at: two on each of the 256 CUs
-constexpr int kLeastSteps = 8;    // of a workgroup, before the keys are split further
+constexpr int kLeastSteps = 8;   // of a workgroup, before the keys are split further
+constexpr int kWholeSteps = 32;  // up to so many, and without a prefix, a workgroup takes all: 8.9 us in one launch, not 6.9 + 3.9
+// Workgroups that a call aims at, by the bytes of a row: twice as many as the 256 CUs' LDS holds at once, so that one's first
+// copies and its join run beside another's steps. 32 sequences of up to 1350 own keys behind 17776 shared ones, D 64: 58 us, of
+// as many as it holds 71, of four times as many 63; 4 sequences of up to 45104 keys, D 128: 117 us, of four times as many 125.
+inline int target_groups(int row) { return 512 * (row <= 128 ? 2 : 1); }
 
 struct CachedPlan {
   int tiles, splits, prefix_tiles, prefix_splits;
@@ -336,13 +367,14 @@ int plan_cached(const sa_attn_cached& t, const char* fn, CachedPlan& p) {
   const int64_t items = t.B * t.Hk * tiles, prefix_items = t.Hk * prefix_tiles;
   if (t.B * per >= 1LL << 30 || items + prefix_items >= 1LL << 22)
     return sa::fail(SA_ERR_UNSUPPORTED, "%s: too many rows", fn);
-  // Splits in proportion to the keys, so that workgroups have alike many of them, about kTarget in all.
+  // Splits in proportion to the keys, so that workgroups have alike many of them, about `target` in all.
+  const int target = target_groups(t.D * (t.dtype == SA_DTYPE_F32 ? 4 : 2));
   const int64_t steps = (t.L + kStep - 1) / kStep, prefix_steps = t.Lp ? (t.Lp + kStep - 1) / kStep : 0;
   const int64_t all = items * steps + prefix_items * prefix_steps;
-  const int64_t each = std::max<int64_t>(kLeastSteps, (all + kTarget - 1) / kTarget);
+  const int64_t each = std::max<int64_t>(kLeastSteps, (all + target - 1) / target);
   p.tiles = (int)tiles;
   p.prefix_tiles = (int)prefix_tiles;
-  p.splits = (int)std::max<int64_t>(1, (steps + each - 1) / each);
+  p.splits = !t.Lp && steps <= kWholeSteps ? 1 : (int)std::max<int64_t>(1, (steps + each - 1) / each);
   p.prefix_splits = t.Lp ? (int)std::max<int64_t>(1, (prefix_steps + each - 1) / each) : 0;
   p.own_groups = items * p.splits;
   p.groups = p.own_groups + prefix_items * p.prefix_splits;
@@ -378,8 +410,8 @@ template <bool kCap, typename T, int kD>
 void launch_cached(const CachedArgs& a, const CachedPlan& p, hipStream_t s) {
   hipLaunchKernelGGL((cached_kernel<kCap, T, kD>), dim3((unsigned)p.groups), dim3(64 * CachedShape<T, kD>::kWaves), 0, s, a);
   if (!p.bytes) return;
-  const int64_t threads = (int64_t)a.B * a.H * a.Ln * (kD / 4);
-  hipLaunchKernelGGL((cached_merge_kernel<T, kD>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a);
+  const int64_t rows = (int64_t)a.B * a.H * a.Ln;
+  hipLaunchKernelGGL((cached_merge_kernel<T, kD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
 }
 
 template <typename T>
