@@ -349,8 +349,8 @@ int sa_attn_scored_sizes(const sa_attn_scored* call, int64_t bytes[3]);
 
 /*
  * out and each row's log2-sum-exp2: +inf, and a row of zeros, for a row that sees no key. bf16 and fp16 (P as two terms
- * of the type) or fp32, D = 64 or 128. Keys and values of listed blocks have to be finite, also where a row does not see them.
- * At most 2^27 rows, and less than 2 GiB from a head's first row to its last. Reads neither dout nor the gradients.
+ * of the type) or fp32, D = 64 or 128. Rows, keys and values of 64 x 64 blocks that hold a pair that is seen (without a mask and
+ * up to 256 rows and keys, of all) have to be finite, also where they are not seen (the backward call's dout, too). Fewer than 2^20 heads and 2^24 blocks of rows or keys, and less than 2 GiB from a head's first row to its last. Reads neither dout nor the gradients.
  */
 int sa_attn_scored_fwd(const sa_attn_scored* call, void* stream);
 
@@ -387,7 +387,8 @@ typedef struct sa_attn_cached {
 /* Reads the sizes. */
 int sa_attn_cached_workspace(const sa_attn_cached* call, int64_t* bytes);
 
-/* bf16, fp16 or fp32, D = 64 or 128, at most 2^29 keys. Results repeat bit for bit. */
+/* bf16, fp16 or fp32, D = 64 or 128, at most 2^29 keys, rows (of the caches, too) at most 2^24 elements apart, and fewer than
+ * 2^20 tiles of 32 rows. Results repeat bit for bit. */
 int sa_attn_cached_fwd(const sa_attn_cached* call, void* stream);
 
 /*

@@ -180,9 +180,8 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
     }
     const int base = place - row0 - 4 * hh;  // d = base - c_e
     if (a.slopes) {
-      const float f = slope * (float)base;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) S[e] = fmaf(S[e], sc, -fabsf(fmaf(slope, -(float)(8 * (e >> 2) + (e & 3)), f)));
+      for (int e = 0; e < 16; ++e) S[e] = fmaf(S[e], sc, -slope * fabsf((float)(base - (8 * (e >> 2) + (e & 3)))));
       sc = 1.f;
     }
     if (a.table) {
@@ -365,7 +364,7 @@ int plan_cached(const sa_attn_cached& t, const char* fn, CachedPlan& p) {
   const int64_t per = (int64_t)(t.H / t.Hk) * t.Ln;
   const int64_t tiles = (per + kStep - 1) / kStep, prefix_tiles = t.Lp ? (t.B * per + kStep - 1) / kStep : 0;
   const int64_t items = t.B * t.Hk * tiles, prefix_items = t.Hk * prefix_tiles;
-  if (t.B * per >= 1LL << 30 || items + prefix_items >= 1LL << 22)
+  if (t.B * per >= 1LL << 30 || items + prefix_items >= 1LL << 20)
     return sa::fail(SA_ERR_UNSUPPORTED, "%s: too many rows", fn);
   // Splits in proportion to the keys, so that workgroups have alike many of them, about `target` in all.
   const int target = target_groups(t.D * (t.dtype == SA_DTYPE_F32 ? 4 : 2));

@@ -521,8 +521,8 @@ int check_scored(const sa_attn_scored* t, const char* fn) {
              "%s: sm_scale / cap out of range", fn);
   if (t->Lq > 1 << 27 || t->Lk > 1 << 27) return sa::fail(SA_ERR_UNSUPPORTED, "%s: more than 2^27 rows", fn);
   SA_REQUIRE(t->q_start > -(1 << 29) && t->q_start < 1 << 29, "%s: q_start %d", fn, t->q_start);
-  if ((int64_t)t->B * t->H * std::max(sa::cdiv(t->Lq, kBlk), sa::cdiv(t->Lk, kBlk)) >= 1LL << 30)
-    return sa::fail(SA_ERR_UNSUPPORTED, "%s: more than 2^30 blocks", fn);
+  if ((int64_t)t->B * t->H * std::max(sa::cdiv(t->Lq, kBlk), sa::cdiv(t->Lk, kBlk)) >= 1LL << 24 || t->H >= 1 << 20)
+    return sa::fail(SA_ERR_UNSUPPORTED, "%s: 2^24 blocks or 2^20 heads, or more", fn);  // (grids of fewer than 2^32 threads)
   if (t->table) {
     SA_REQUIRE(t->buckets && t->n_buckets > 0, "%s: table without buckets", fn);
     SA_REQUIRE(t->table_dtype >= SA_DTYPE_BF16 && t->table_dtype <= SA_DTYPE_F32, "%s: table dtype %d", fn, t->table_dtype);

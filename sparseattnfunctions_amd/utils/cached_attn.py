@@ -15,6 +15,7 @@ shapes alone, so that a captured call serves sequences as they grow.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -26,13 +27,14 @@ from .scored_attn import check_heads, check_rule
 
 def _check_rows(name, t):
     size = t.element_size()
-    if t.stride(-1) != 1 or any(s * size % 16 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+    if t.stride(-1) != 1 or any(n > 1 and s * size % 16 for n, s in zip(t.shape, t.stride()[:-1])) or t.data_ptr() % 16:
         raise ValueError(f"{name} must have a contiguous last axis and 16-byte aligned rows (strides {tuple(t.stride())})")
 
 
 def _set(call, at, t):
-    """Strides {b, h, l} of [B, H, L, D], or of [H, L, D] (b unused)."""
-    call.strides[at:at + 3] = t.stride()[:3] if t.dim() == 4 else (0, *t.stride()[:2])
+    """Strides {b, h, l} of [B, H, L, D], or of [H, L, D] (b unused); 0 where there is one."""
+    strides = [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
+    call.strides[at:at + 3] = strides[:3] if t.dim() == 4 else (0, *strides[:2])
 
 
 @torch.no_grad()
@@ -56,6 +58,8 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
         raise ValueError("q, k, v and lengths must be on one device")
     if lengths.dtype != torch.int32 or lengths.shape != (B,):
         raise ValueError(f"lengths must be int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
+    if not (sm_scale > 0 and math.isfinite(sm_scale)):
+        raise ValueError(f"sm_scale {sm_scale} must be positive and finite")
     window = int(window)
     if not 0 <= window < 2 ** 31:
         raise ValueError(f"window {window}")

@@ -24,8 +24,10 @@ blocks of a sequence, with a block mask of a head). Blocks of which no pair is s
 of a 16-bit call round P and dS to its type; sums are fp32 in a fixed order, so that a step repeats bit
 for bit. In fp16, dS has the range of the type: scale the loss as usual.
 
-Keys and values of blocks that hold a visible pair enter the products whole: they have to be finite, also
-where a mask hides them, as do the slopes and the table. The calls are differentiable once; ranges, the
+Rows (of q and, in the backward pass, of the output's gradient), keys and values of 64 x 64 blocks that hold
+a visible pair (without a mask and up to 256 rows and keys, all of them) enter the products whole: they have
+to be finite, also where a mask hides them, as do the slopes and the table; but a table's value of -inf, or
+below -2.3e38 (the lowest of bf16 and fp32), hides its pairs. The calls are differentiable once; ranges, the
 mask and the slopes are not differentiated.
 """
 from __future__ import annotations
@@ -108,7 +110,11 @@ def row_ranges(lengths: torch.Tensor, L: int, causal: bool = True, prefix: Optio
             raise ValueError("lengths and prefix must be on one device")
         if prefix.dtype not in _INTEGERS:
             raise ValueError(f"prefix must be integers, got {prefix.dtype}")
-        prefix = _int32(prefix if prefix.shape == (B, n) else prefix.expand(B, n), L)
+        if prefix.shape != (B, n):
+            if prefix.dim() > 2 or any(x not in (1, y) for x, y in zip(prefix.shape[::-1], (n, B))):
+                raise ValueError(f"prefix must be [{B}, {n}], or of one sequence or number, got {tuple(prefix.shape)}")
+            prefix = prefix.expand(B, n)
+        prefix = _int32(prefix, L)
     lengths = _int32(lengths, L)
     out = torch.empty((B, L, 2), dtype=torch.int32, device=device)
     if B == 0 or L == 0:
@@ -260,6 +266,8 @@ def _check_mask(mask, q, B, H, nqb, nkb):
         raise ValueError("q, k, v and the block mask must be on one device")
     if mask.dim() != 4:
         raise ValueError(f"block mask must be 4-D [B,H,nqb,nkb], got {tuple(mask.shape)}")
+    if mask.shape[0] not in (1, B) or mask.shape[1] not in (1, H):
+        raise ValueError(f"block mask {tuple(mask.shape)} of other sequences or heads than ({B}, {H})")
     if mask.shape[2] < nqb or mask.shape[3] < nkb:
         raise ValueError(f"block mask {tuple(mask.shape)} smaller than the block grid ({nqb}, {nkb})")
     if mask.dtype != torch.bool:
@@ -340,6 +348,8 @@ def scored_attention_forward(q, k, v, sm_scale: float, *, cap: Optional[float] =
                              ranges=None, block_mask=None, q_start: int = 0):
     """(out, state): `scored_attention` without autograd, and what `scored_attention_backward` needs of it."""
     checked = _check(q, k, v, cap, slopes, table, buckets, ranges, block_mask, int(q_start))
+    if not (sm_scale > 0 and math.isfinite(sm_scale)):
+        raise ValueError(f"sm_scale {sm_scale} must be positive and finite")
     if q.numel() == 0 or k.numel() == 0:
         raise ValueError(f"no query or no key: q{tuple(q.shape)} k{tuple(k.shape)}")
     with torch.no_grad():
