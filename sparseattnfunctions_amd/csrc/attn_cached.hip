@@ -36,6 +36,7 @@ struct CachedArgs {
   int tiles, splits;                // 32-row tiles of a sequence's rows of a key head, and workgroups that share their keys
   int prefix_tiles, prefix_splits;  // of all sequences' rows of a key head, and alike for the prefix
   int own_groups;                   // B * Hk * tiles * splits workgroups, and behind them the prefix's
+  int lead;                         // steps of the prefix that each sequence takes before its own; then prefix_splits is 0
   float scale_log2, cap_in, cap_log2;
   const float* slopes;
   const void* table;
@@ -59,7 +60,8 @@ __device__ __forceinline__ void store_four(uint8_t* row, int at, float x, float 
 }
 
 // kPieces: a piece of the row of all steps (parts is not null); else an item.
-template <bool kCap, typename T, int kD>
+// kLead: a sequence's steps begin with those of the prefix.
+template <bool kLead, bool kCap, typename T, int kD>
 __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kernel(CachedArgs a) {
   constexpr int kSize = sizeof(T), kRow = CachedShape<T, kD>::kRow, kMat = CachedShape<T, kD>::kMat;
   constexpr int kWaves = CachedShape<T, kD>::kWaves;
@@ -70,7 +72,7 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hh = lane >> 5;
-  const bool shared = (int)blockIdx.x >= a.own_groups;
+  const bool shared = !kLead && (int)blockIdx.x >= a.own_groups;
   int x = shared ? blockIdx.x - a.own_groups : blockIdx.x;
   const int splits = shared ? a.prefix_splits : a.splits, tiles = shared ? a.prefix_tiles : a.tiles;
   const int split = x % splits;
@@ -110,30 +112,37 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
   near = __builtin_amdgcn_readfirstlane(near);
   far = __builtin_amdgcn_readfirstlane(far);
   const bool blind = __ballot(t < 0) != 0;
-  // The tile's keys, whole steps of them from the first that a row sees, and the split's and wave's share.
+  // The tile's keys, whole steps of them from the first that a row sees, and the split's and wave's share. Steps of a leading
+  // prefix hold keys -Lp .. -1.
   const int end = shared ? a.Lp : __builtin_amdgcn_readfirstlane(min(max(a.lengths[b0], 0), a.L));
+  const int lead = kLead ? a.lead : 0;
   int first = 0;
-  if (a.window && near != INT_MAX) first = max(0, min(near - a.window + 1, end)) / kStep;
-  const int n_steps = far < 0 ? 0 : (end + kStep - 1) / kStep - first;
+  if (a.window && near != INT_MAX) {
+    const int key = near - a.window + 1;
+    first = key >= 0 || !lead ? lead + max(0, min(key, end)) / kStep : max(0, key + a.Lp) / kStep;
+  }
+  const int n_steps = far < 0 ? 0 : lead + (end + kStep - 1) / kStep - first;
   const int per_split = (n_steps + splits - 1) / splits;
   const int last = min(n_steps, per_split * (split + 1));
   const int begin = split * per_split + w;  // steps begin, begin + kWaves, ..
 
-  const Cache& c = shared ? a.prefix : a.own;
-  const uint8_t* kp = static_cast<const uint8_t*>(c.k) + (b0 * c.k_sb + hk * c.k_sh) * kSize;
-  const uint8_t* vp = static_cast<const uint8_t*>(c.v) + (b0 * c.v_sb + hk * c.v_sh) * kSize;
+  auto at = [&](const void* p, int64_t sb, int64_t sh) { return static_cast<const uint8_t*>(p) + (b0 * sb + hk * sh) * kSize; };
   // Copies of a step's keys and values: rows past the last cached one, and steps past the wave's last, read as zero whatever is
   // there.
   auto issue = [&](int step, lds_u8* to) __attribute__((always_inline)) {
+    const bool ahead = kLead && first + step < lead;
+    const Cache& c = shared || ahead ? a.prefix : a.own;
+    const int rows = ahead ? a.Lp : end;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const int64_t row_bytes = (m == 0 ? c.k_sl : c.v_sl) * kSize;
+      const uint8_t* base = m == 0 ? at(c.k, ahead ? 0 : c.k_sb, c.k_sh) : at(c.v, ahead ? 0 : c.v_sb, c.v_sh);
 #pragma unroll
       for (int r16 = 0; r16 < 2; ++r16) {
-        const int row0 = (first + step) * kStep + 16 * r16;
-        const int64_t left = step < last && row0 < end ? (end - 1 - row0) * row_bytes + 128 : 0;
+        const int row0 = (first + step - (ahead ? 0 : lead)) * kStep + 16 * r16;
+        const int64_t left = step < last && row0 < rows ? (rows - 1 - row0) * row_bytes + 128 : 0;
         const int size = __builtin_amdgcn_readfirstlane((int)min(left, (int64_t)INT_MAX));
-        const uint8_t* from = (m == 0 ? kp : vp) + row0 * row_bytes;
+        const uint8_t* from = base + row0 * row_bytes;
 #pragma unroll
         for (int hf = 0; hf < kParts; ++hf) {
           const __amdgpu_buffer_rsrc_t rsrc =
@@ -158,7 +167,8 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 
   auto compute = [&](int step, const lds_u8* from) __attribute__((always_inline)) {
     const lds_u8* mat = from + w * 2 * kMat;
-    const int row0 = (first + step) * kStep;
+    const bool ahead = kLead && first + step < lead;
+    const int row0 = (first + step - (ahead ? 0 : lead)) * kStep - (ahead ? a.Lp : 0), limit = ahead ? 0 : end;
     sa_f32x16 S = {};
     sa_u32x4v x[kDS];
 #pragma unroll
@@ -194,12 +204,12 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
       }
       sc = 1.f;
     }
-    if (blind || row0 + 31 > near || row0 + 31 >= end || (a.window && far - row0 >= a.window)) {
+    if (blind || row0 + 31 > near || row0 + 31 >= limit || (a.window && far - row0 >= a.window)) {
       const unsigned most = a.window ? a.window : 0x80000000u;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int k = 8 * (e >> 2) + (e & 3);
-        if (t < 0 || (unsigned)(base - k) >= most || row0 + 4 * hh + k >= end) S[e] = -INFINITY;
+        if (t < 0 || (unsigned)(base - k) >= most || row0 + 4 * hh + k >= limit) S[e] = -INFINITY;
       }
     }
     float top = S[0];
@@ -297,7 +307,7 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
       continue;
     }
     const float f = sum == 0.f ? 0.f : 1.f / sum;
-    const int in_ = tile * kStep + rr;  // (no prefix: a row of sequence b0)
+    const int in_ = tile * kStep + rr;  // (a row of sequence b0)
     uint8_t* p = static_cast<uint8_t*>(a.out) +
                  (b0 * a.o_sb + (hk * a.rep + in_ / a.Ln) * a.o_sh + (in_ % a.Ln) * a.o_sl) * kSize;
     store_four<T>(p, 4 * ch, s.x * f, s.y * f, s.z * f, s.w * f);
@@ -315,7 +325,7 @@ __global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs a) {
   const int i = (int)(at % a.Ln), h = (int)(at / a.Ln % a.H), b = (int)(at / a.Ln / a.H);
   const int hk = h / a.rep, in = (h - hk * a.rep) * a.Ln + i, all = b * a.rep * a.Ln + in;
   // Place of the s-th sums of the row, in units of rows.
-  const int n = a.splits + (a.Lp ? a.prefix_splits : 0);
+  const int n = a.splits + a.prefix_splits;
   const int64_t own = ((int64_t)(b * a.Hk + hk) * a.tiles + in / kStep) * a.splits;
   const int64_t shared = a.own_groups + ((int64_t)hk * a.prefix_tiles + all / kStep) * a.prefix_splits - a.splits;
   auto place = [&](int s) { return s < a.splits ? (own + s) * kStep + in % kStep : (shared + s) * kStep + all % kStep; };
@@ -349,14 +359,14 @@ __global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs a) {
 // ---- Host side.
 
 constexpr int kLeastSteps = 8;   // of a workgroup, before the keys are split further
-constexpr int kWholeSteps = 32;  // up to so many, and without a prefix, a workgroup takes all: 8.9 us in one launch, not 6.9 + 3.9
+constexpr int kWholeSteps = 32;  // up to so many a workgroup takes them all: 526 keys 8.9 us in one launch, not 6.9 + 3.9 in two
 // Workgroups that a call aims at, by the bytes of a row: twice as many as the 256 CUs' LDS holds at once, so that one's first
 // copies and its join run beside another's steps. 32 sequences of up to 1350 own keys behind 17776 shared ones, D 64: 58 us, of
 // as many as it holds 71, of four times as many 63; 4 sequences of up to 45104 keys, D 128: 117 us, of four times as many 125.
 inline int target_groups(int row) { return 512 * (row <= 128 ? 2 : 1); }
 
 struct CachedPlan {
-  int tiles, splits, prefix_tiles, prefix_splits;
+  int tiles, splits, prefix_tiles, prefix_splits, lead;
   int64_t own_groups, groups, sums, bytes;
 };
 
@@ -372,12 +382,17 @@ int plan_cached(const sa_attn_cached& t, const char* fn, CachedPlan& p) {
   const int64_t all = items * steps + prefix_items * prefix_steps;
   const int64_t each = std::max<int64_t>(kLeastSteps, (all + target - 1) / target);
   p.tiles = (int)tiles;
-  p.prefix_tiles = (int)prefix_tiles;
-  p.splits = !t.Lp && steps <= kWholeSteps ? 1 : (int)std::max<int64_t>(1, (steps + each - 1) / each);
-  p.prefix_splits = t.Lp ? (int)std::max<int64_t>(1, (prefix_steps + each - 1) / each) : 0;
+  // A short prefix is read by each sequence for itself, ahead of its own keys, where the card holds all workgroups at once: the
+  // prefix comes out of the L2 then, and there are no sums to join (4 answers of up to 77 tokens to a caption of 226: 15 us in
+  // two launches, 11 in one).
+  const bool whole = steps + prefix_steps <= kWholeSteps && (!t.Lp || items <= target / 2);
+  p.lead = whole ? (int)prefix_steps : 0;
+  p.prefix_tiles = whole ? 0 : (int)prefix_tiles;
+  p.splits = whole ? 1 : (int)std::max<int64_t>(1, (steps + each - 1) / each);
+  p.prefix_splits = whole || !t.Lp ? 0 : (int)std::max<int64_t>(1, (prefix_steps + each - 1) / each);
   p.own_groups = items * p.splits;
-  p.groups = p.own_groups + prefix_items * p.prefix_splits;
-  const bool merged = p.splits > 1 || t.Lp;
+  p.groups = p.own_groups + (int64_t)t.Hk * p.prefix_tiles * p.prefix_splits;
+  const bool merged = p.splits > 1 || p.prefix_splits > 0;
   p.sums = (p.groups * kStep * 8 + 255) / 256 * 256;
   p.bytes = merged ? p.sums + p.groups * kStep * t.D * 4 : 0;
   return SA_OK;
@@ -407,7 +422,9 @@ int check_cached(const sa_attn_cached* t, const char* fn) {
 
 template <bool kCap, typename T, int kD>
 void launch_cached(const CachedArgs& a, const CachedPlan& p, hipStream_t s) {
-  hipLaunchKernelGGL((cached_kernel<kCap, T, kD>), dim3((unsigned)p.groups), dim3(64 * CachedShape<T, kD>::kWaves), 0, s, a);
+  const dim3 grid((unsigned)p.groups), group(64 * CachedShape<T, kD>::kWaves);
+  if (p.lead) hipLaunchKernelGGL((cached_kernel<true, kCap, T, kD>), grid, group, 0, s, a);
+  else hipLaunchKernelGGL((cached_kernel<false, kCap, T, kD>), grid, group, 0, s, a);
   if (!p.bytes) return;
   const int64_t rows = (int64_t)a.B * a.H * a.Ln;
   hipLaunchKernelGGL((cached_merge_kernel<T, kD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
@@ -466,7 +483,7 @@ extern "C" int sa_attn_cached_fwd(const sa_attn_cached* t, void* stream) {
   a.Ln = t->Ln; a.L = t->L; a.Lp = t->Lp; a.window = t->window;
   a.tiles = p.tiles; a.splits = p.splits;
   a.prefix_tiles = p.prefix_tiles; a.prefix_splits = p.prefix_splits;
-  a.own_groups = (int)p.own_groups;
+  a.own_groups = (int)p.own_groups; a.lead = p.lead;
   a.scale_log2 = t->sm_scale * kLog2e;
   if (t->cap > 0) {
     a.cap_in = t->sm_scale / t->cap * (t->dtype == SA_DTYPE_F32 ? 1.f : 2.f * kLog2e);

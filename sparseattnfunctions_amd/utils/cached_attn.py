@@ -15,6 +15,7 @@ shapes alone, so that a captured call serves sequences as they grow.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -25,19 +26,51 @@ from .block_sparse_attn_grad import _rows16
 from .scored_attn import check_heads, check_rule
 
 
-def _check_rows(name, t):
-    size = t.element_size()
-    if t.stride(-1) != 1 or any(n > 1 and s * size % 16 for n, s in zip(t.shape, t.stride()[:-1])) or t.data_ptr() % 16:
-        raise ValueError(f"{name} must have a contiguous last axis and 16-byte aligned rows (strides {tuple(t.stride())})")
+class _Call:
+    """What calls of one shape share: a description without pointers, and the bytes of its workspace."""
+
+    def __init__(self, dtype, q_shape, k_shape, strides, prefix_shape, sm_scale, cap, window, slopes, table):
+        (B, H, Ln, D), (_, Hk, L, _) = q_shape, k_shape
+        if not (sm_scale > 0 and math.isfinite(sm_scale)):
+            raise ValueError(f"sm_scale {sm_scale} must be positive and finite")
+        if not 0 <= window < 2 ** 31:
+            raise ValueError(f"window {window}")
+        size = dtype.itemsize
+        q, k, v, pk, pv = strides
+        for name, shape, s in (("k", k_shape, k), ("v", k_shape, v), ("the prefix's k", prefix_shape, pk),
+                               ("the prefix's v", prefix_shape, pv)):
+            if s is not None and (s[-1] != 1 or any(n > 1 and x * size % 16 for n, x in zip(shape, s[:-1]))):
+                raise ValueError(f"{name} must have a contiguous last axis and 16-byte aligned rows (strides {s})")
+        self.nothing = 0 in q_shape or L == 0
+        if self.nothing:
+            return
+        Lp = 0 if prefix_shape is None else prefix_shape[1]
+        args = self.args = _lib.AttnCached(dtype=_lib.DTYPES[dtype], B=B, H=H, Hk=Hk, Ln=Ln, L=L, Lp=Lp, D=D, window=window,
+                                           sm_scale=sm_scale, cap=cap)
+        # {b, h, l}, 0 where there is one
+        k, v, pk, pv = ([x if n > 1 else 0 for n, x in zip(shape, s)] if s is not None else None
+                        for shape, s in ((k_shape, k), (k_shape, v), (prefix_shape, pk), (prefix_shape, pv)))
+        args.strides[:12] = (*q[:3], H * Ln * D, Ln * D, D, *k[:3], *v[:3])
+        if Lp:
+            args.strides[12:] = (0, *pk[:2], 0, *pv[:2])
+        if slopes:
+            args.slopes = 1
+        if table is not None:
+            args.table = args.buckets = 1
+            args.table_dtype, args.n_buckets, args.radius = _lib.DTYPES[table[0]], table[1], table[2]
+        n = ctypes.c_int64(0)
+        _lib.check(_lib.load().sa_attn_cached_workspace(args, ctypes.byref(n)), "sa_attn_cached_workspace")
+        self.bytes = n.value
 
 
-def _set(call, at, t):
-    """Strides {b, h, l} of [B, H, L, D], or of [H, L, D] (b unused); 0 where there is one."""
-    strides = [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
-    call.strides[at:at + 3] = strides[:3] if t.dim() == 4 else (0, *strides[:2])
+_call = functools.lru_cache(maxsize=1024)(_Call)
 
 
-@torch.no_grad()
+def _aligned(name, t):
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name} must have 16-byte aligned rows")
+
+
 def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, sm_scale: float, *,
                      cap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
                      table: Optional[torch.Tensor] = None, buckets: Optional[torch.Tensor] = None, window: int = 0,
@@ -58,14 +91,7 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
         raise ValueError("q, k, v and lengths must be on one device")
     if lengths.dtype != torch.int32 or lengths.shape != (B,):
         raise ValueError(f"lengths must be int32 [{B}], got {lengths.dtype} {tuple(lengths.shape)}")
-    if not (sm_scale > 0 and math.isfinite(sm_scale)):
-        raise ValueError(f"sm_scale {sm_scale} must be positive and finite")
-    window = int(window)
-    if not 0 <= window < 2 ** 31:
-        raise ValueError(f"window {window}")
-    _check_rows("k", k)
-    _check_rows("v", v)
-    Lp = 0
+    pk = pv = None
     if prefix is not None:
         pk, pv = (t[0] if t.dim() == 4 and t.shape[0] == 1 else t for t in prefix)
         for t in (pk, pv):
@@ -76,37 +102,37 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
                 raise TypeError(f"the prefix must be {q.dtype}, got {t.dtype}")
             if t.dim() != 3 or t.shape != pk.shape or t.shape[0] != Hk or t.shape[2] != D:
                 raise ValueError(f"the prefix must be two [{Hk}, Lp, {D}], got {tuple(pk.shape)} and {tuple(pv.shape)}")
-        Lp = pk.shape[1]
-    out = torch.empty((B, H, Ln, D), dtype=q.dtype, device=q.device)
-    if out.numel() == 0:
-        return out
-    if L == 0:  # no sequence has a token
-        return out.zero_()
+        if pk.shape[1]:
+            _aligned("the prefix's k", pk)
+            _aligned("the prefix's v", pv)
+        else:
+            pk = pv = None
+    _aligned("k", k)
+    _aligned("v", v)
     q = _rows16(q)
-    call = _lib.AttnCached(dtype=_lib.DTYPES[q.dtype], B=B, H=H, Hk=Hk, Ln=Ln, L=L, Lp=Lp, D=D, window=window, radius=radius,
-                           sm_scale=sm_scale, cap=cap)
-    call.q, call.out, call.k, call.v = q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr()
-    for i, t in enumerate((q, out, k, v)):
-        _set(call, 3 * i, t)
-    if Lp:
-        _check_rows("the prefix's k", pk)
-        _check_rows("the prefix's v", pv)
-        call.prefix_k, call.prefix_v = pk.data_ptr(), pv.data_ptr()
-        _set(call, 12, pk)
-        _set(call, 15, pv)
-    lengths = lengths.contiguous()
-    call.lengths = lengths.data_ptr()
+    call = _call(q.dtype, q.shape, k.shape, (q.stride(), k.stride(), v.stride(), None if pk is None else pk.stride(),
+                                             None if pv is None else pv.stride()),
+                 None if pk is None else pk.shape, float(sm_scale), cap, int(window), slopes is not None,
+                 None if table is None else (table.dtype, table.shape[0], radius))
+    out = torch.empty((B, H, Ln, D), dtype=q.dtype, device=q.device)
+    if call.nothing:  # no sequence has a token
+        return out.zero_()
+    args = _lib.AttnCached.from_buffer_copy(call.args)
+    args.q, args.out, args.k, args.v = q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr()
+    if pk is not None:
+        args.prefix_k, args.prefix_v = pk.data_ptr(), pv.data_ptr()
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    args.lengths = lengths.data_ptr()
     if slopes is not None:
-        call.slopes = slopes.data_ptr()
+        args.slopes = slopes.data_ptr()
     if table is not None:
-        call.table, call.buckets = table.data_ptr(), buckets.data_ptr()
-        call.table_dtype, call.n_buckets = _lib.DTYPES[table.dtype], table.shape[0]
-    n = ctypes.c_int64(0)
-    _lib.check(_lib.load().sa_attn_cached_workspace(call, ctypes.byref(n)), "sa_attn_cached_workspace")
-    if n.value:
-        ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-        call.workspace, call.workspace_bytes = ws.data_ptr(), n.value
+        args.table, args.buckets = table.data_ptr(), buckets.data_ptr()
+    if call.bytes:
+        ws = torch.empty(call.bytes, dtype=torch.uint8, device=q.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), call.bytes
     with _lib.on(q.device):
-        rc = _lib.load().sa_attn_cached_fwd(call, _lib.stream_of(q))
-    _lib.check(rc, "sa_attn_cached_fwd")
+        rc = _lib.load().sa_attn_cached_fwd(args, _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "sa_attn_cached_fwd")
     return out

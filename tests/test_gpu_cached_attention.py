@@ -48,6 +48,8 @@ CASES = {
     "prefix_one": (dict(B=2, H=2, Hk=2, Ln=1, L=8), [1, 8], dict(Lp=1)),
     "prefix": (dict(B=5, H=6, Hk=2, Ln=3, L=77, D=128), [0, 2, 3, 77, 50], dict(Lp=226, kind="cap slopes")),
     "prefix_long": (dict(B=40, H=2, Hk=2, Ln=1, L=30), [i % 31 for i in range(40)], dict(Lp=5000, kind="table")),
+    "prefix_of_many": (dict(B=60, H=10, Hk=10, Ln=1, L=40), [i % 41 for i in range(60)], dict(Lp=90, kind="slopes")),
+    "prefix_of_long": (dict(B=2, H=4, Hk=2, Ln=20, L=1500), [1500, 7], dict(Lp=700, window=900, kind="cap")),
     "prefix_window": (dict(B=4, H=3, Hk=3, Ln=2, L=600), [0, 1, 100, 600], dict(Lp=300, window=150, kind="table cap")),
 }
 

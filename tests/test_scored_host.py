@@ -143,8 +143,11 @@ def test_cached_workspace():
     assert n.value == 0  # up to 1024 keys without a prefix: nothing is split
     _lib.check(lib.sa_attn_cached_workspace(cached(Lp=0, L=1025), ctypes.byref(n)), "workspace")
     assert n.value > 0
-    _lib.check(lib.sa_attn_cached_workspace(cached(Lp=1, L=1), ctypes.byref(n)), "workspace")
-    assert n.value > 0
+    _lib.check(lib.sa_attn_cached_workspace(cached(Lp=500, L=500), ctypes.byref(n)), "workspace")
+    assert n.value == 0  # nor with a short one, for as few sequences
+    for over in (dict(Lp=1000, L=500), dict(Lp=50, L=50, B=1000)):
+        _lib.check(lib.sa_attn_cached_workspace(cached(**over), ctypes.byref(n)), "workspace")
+        assert n.value > 0
     assert lib.sa_attn_cached_workspace(cached(), None) == INVALID
 
 
