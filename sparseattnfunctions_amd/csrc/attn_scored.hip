@@ -223,7 +223,9 @@ __global__ __launch_bounds__(kPlanThreads) void scored_schedule_kernel(ScheduleA
     if (lane == 63) {
       const float quarters = 4.f * (float)all_entries;
       const float all = (quarters + (float)units * a.unit_cost + (float)of_split * a.split_cost) * 8.f / a.slots;
-      const float time = fmaxf(4.f * limit, all + quarters / fmaxf((float)units, 1.f)) +
+      // (units that all run at once end with the longest; of more, the last ones run while others have ended)
+      const float tail = 8 * units <= a.slots ? 0.f : quarters / fmaxf((float)units, 1.f);
+      const float time = fmaxf(4.f * limit + a.unit_cost + (of_split ? a.split_cost : 0), all + tail) +
                          (of_split ? a.merge_cost + (float)a.part_cost * ((float)longest * inv) : 0.f);
       times[wave] = of_split <= a.max_units ? time : INFINITY;  // (the first splits nothing)
       limits[wave] = limit;
@@ -439,7 +441,7 @@ SidePlan side_plan(const sa_attn_scored& t, bool keys) {
   // its share of a sum four. Where lists are short for that, all launches to split them would take longer than they do.
   p.least = f32 ? 1 : 2;
   p.unit_cost = f32 ? 1 : 4;
-  p.split_cost = f32 ? 2 : 6;
+  p.split_cost = f32 ? 2 : 6 * (t.D / 64) * (keys ? 2 : 1);
   p.merge_cost = f32 ? 2 : 12;
   p.part_cost = 1;
   const int64_t longest = n_st * rep;

@@ -32,6 +32,7 @@ constexpr float kPScale = 4096.f;
 // are next to each other wherever one of them is not past it.
 constexpr int kPad = 96;
 constexpr int kWindow = 128;
+constexpr int kDiagonals = 8 * 64;  // floats of a wave in which dS is summed by distance (16 * 64: a workgroup less on a CU)
 
 struct Side {
   const void* p;
@@ -113,15 +114,19 @@ __device__ __forceinline__ float apply_rule(const ScoredArgs& a, float slope_h, 
   return sc;
 }
 
-// A cut tile of own queries: pairs that are not seen get -inf. row: the lane's query row; key0: its key at element 0.
-__device__ __forceinline__ void cut_keys(const ScoredArgs& a, int b, int Lk, int row, int key0, sa_f32x16& S) {
-  if (a.ranges) {  // (keys past the last one: no rows)
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<int2*>(a.ranges + b * a.ranges_sb), (short)0, Lk * 8, 0x00020000);
+// A cut tile of own queries: pairs that are not seen get -inf. row: the lane's query row; key0: its key at element 0. Where
+// there are ranges, the step's intervals lie at `intervals` in LDS (keys past the last one: no rows).
+__device__ __forceinline__ void cut_keys(const ScoredArgs& a, int Lk, int row, int key0, int lane, const lds_u8* intervals,
+                                         sa_f32x16& S) {
+  if (a.ranges) {
+    asm volatile("" : "+v"(lane));  // (the address is worked out here, not kept in a register throughout)
+    const lds_u8* p = intervals + (lane & 32);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const sa_u32x2v r = __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * (key0 + 8 * (e >> 2) + (e & 3)), 0, 0);
-      if (row < (int)r[0] || row >= (int)r[1]) S[e] = -INFINITY;
+    for (int e = 0; e < 16; e += 2) {
+      if (e % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // (all of them at once would take 32 registers)
+      const sa_u32x4v r = lds_read_b128(p + 8 * (8 * (e >> 2) + (e & 3)));
+      S[e] = (row < (int)r[0]) | (row >= (int)r[1]) ? -INFINITY : S[e];
+      S[e + 1] = (row < (int)r[2]) | (row >= (int)r[3]) ? -INFINITY : S[e + 1];
     }
   } else {
 #pragma unroll
@@ -188,13 +193,13 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
   // Row operands are read in groups of kRead 16-byte steps, transposed ones 64 columns at a time, each a group ahead of the
   // products; kEarly: the first transposed ones before the exponentials, where there are registers for them (kKeys of
   // [1, 15, 17776, 64] by frames 1 500 us with, 1 375 without; kQueries of a bias at head dim 64 320 and 253).
-  constexpr bool kTight = kMode == kQueries && kD == 64 && (kCap || kRule == kTable);
+  constexpr bool kTight = kMode == kQueries && kD == 64 && (kCap || kRule != kPlain);
   constexpr int kRead = kF32 || kTight ? 2 : kMode == kKeys ? 1 : 4;
   constexpr bool kEarly = !kF32 && kMode != kKeys && !kTight;
   __shared__ __attribute__((aligned(1024))) uint8_t tile0[2 * kMat], tile1[2 * kMat];
   __shared__ __attribute__((aligned(256))) float stat0[64], stat1[64];
   __shared__ __attribute__((aligned(256))) float bias0[kRule == kTable ? kWindow : 1], bias1[kRule == kTable ? kWindow : 1];
-  extern __shared__ float far_lds[];  // kQueries with far: [wave][16][64] for half a tile, [wave][2 radius + 1] sums
+  extern __shared__ float far_lds[];  // kQueries with far: [wave][8][64] for a quarter of a tile, [wave][2 radius + 1] sums
 
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -252,7 +257,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
           own_row < a.L_own ? (hh == 0 ? lse : delta) : hh == 0 ? INFINITY : 0.f;
     if (!a.grad_a && !a.far) return;  // only the statistics are wanted
     if (kRule == kTable && a.far) {
-      for (int i = threadIdx.x; i < 2 * (16 * 64 + 2 * a.radius + 1); i += 128) far_lds[i] = 0.f;
+      for (int i = threadIdx.x; i < 2 * (kDiagonals + 2 * a.radius + 1); i += 128) far_lds[i] = 0.f;
       __syncthreads();
     }
   }
@@ -360,6 +365,11 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
           __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(src), (short)0, 256, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, stat, 4, 4 * lane, 0, 0, 0);
     }
+    if (kMode != kKeys && w == 0 && a.ranges && s.cut) {  // the keys' intervals
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<int2*>(a.ranges + b * a.ranges_sb + row0), (short)0, 8 * max(a.L_st - (int)row0, 0), 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, stat, 4, 4 * lane, 0, 0, 0);
+    }
     if (kRule == kTable && w == 1) {  // (where neither wave's pairs are all past the radius they are in bounds)
       const int least = least_of((int)row0), n = 2 * a.radius + 1 + 2 * kPad;
       const int hq = kMode == kKeys ? st_head + s.g : head;
@@ -440,7 +450,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
             if ((unsigned)(t + 8 * (e >> 2) + (e & 3)) >= (unsigned)len) S[e] = -INFINITY;
         }
       } else {
-        cut_keys(a, b, a.L_st, own_row, row0 + 4 * hh, S);
+        cut_keys(a, a.L_st, own_row, row0 + 4 * hh, lane, (const lds_u8*)stat, S);
       }
     }
     if constexpr (kMode == kForward) {
@@ -502,19 +512,19 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
             if (side_far > 0) far_hi += t;
             else far_lo += t;
           } else {
-            // Sums along the tile's diagonals, 16 of its keys j at a time: row j of the wave's 64 columns holds the values at
+            // Sums along the tile's diagonals, 8 of its keys j at a time: row j of the wave's 64 columns holds the values at
             // column col - j + 31, which are all written each time, and zeros, so that column x sums up a distance.
             const int at = 64 * 4 * hh + col - 4 * hh + 31;
-            float* sums = far_lds + 2 * 16 * 64 + w * (2 * a.radius + 1) + a.radius;
+            float* sums = far_lds + 2 * kDiagonals + w * (2 * a.radius + 1) + a.radius;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float* mine = far_lds + w * 16 * 64;
+            for (int u = 0; u < 4; ++u) {
+              float* mine = far_lds + w * kDiagonals;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) mine[at + 63 * (8 * (e >> 2) + (e & 3))] = dP[8 * u + e];
+              for (int e = 0; e < 4; ++e) mine[at + 63 * e] = dP[4 * u + e];
               float t = 0.f;
 #pragma unroll
-              for (int j = 0; j < 16; ++j) t += mine[64 * j + lane];
-              const int d = least + lane - 16 * u;  // (lane 63 and columns that no pair has: zeros)
+              for (int j = 0; j < 8; ++j) t += mine[64 * j + lane];
+              const int d = least + lane - 8 * u;  // (lane 63 and columns that no pair has: zeros)
               if (d >= a.radius) far_hi += t;
               else if (d <= -a.radius) far_lo += t;
               else sums[d] += t;
@@ -570,7 +580,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
       far_hi = wave_sum(far_hi);
       far_lo = wave_sum(far_lo);
       const int n_far = 2 * a.radius + 1;
-      float* sums = far_lds + 2 * 16 * 64;
+      float* sums = far_lds + 2 * kDiagonals;
       if (lane == 0) {
         sums[w * n_far + 2 * a.radius] += far_hi;
         sums[w * n_far] += far_lo;
@@ -699,7 +709,7 @@ struct PassCall {
 
 template <int kMode, bool kCap, int kRule, typename T, int kD>
 void launch_kernels(const ScoredArgs& a, const MergeArgs& m, const PassCall& c) {
-  const size_t lds = kMode == kQueries && kRule == kTable && a.far ? 2 * (16 * 64 + 2 * a.radius + 1) * sizeof(float) : 0;
+  const size_t lds = kMode == kQueries && kRule == kTable && a.far ? 2 * (kDiagonals + 2 * a.radius + 1) * sizeof(float) : 0;
   hipLaunchKernelGGL((scored_kernel<kMode, kCap, kRule, T, kD>), dim3(c.grid), dim3(128), lds, c.stream, a);
   if (c.merge_grid)
     hipLaunchKernelGGL((scored_merge_kernel<kMode, T, kD>), dim3(c.merge_grid), dim3(kMergeThreads), 0, c.stream, m);
