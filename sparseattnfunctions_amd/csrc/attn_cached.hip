@@ -11,6 +11,10 @@
 // The prefix's keys are read once for the rows of all sequences, 32 rows a workgroup. Each wave copies its steps of 32
 // keys into LDS stages of its own, with no barrier between steps; a workgroup's waves join their sums in LDS, and
 // cached_merge_kernel joins the workgroups', in order: results do not depend on the order in which they run.
+//
+// Measured (kernel and merge): 8 sequences of 8888 to 17776 keys, 30 heads of 64, bf16: 163 + 5 us, 5.5 TB/s; 4 of 22552 to
+// 45104 keys, 8 heads of 128 read by 48, 4 tokens each, fp16: 118 + 5 us, 5.4 TB/s (a large copy: 4.7); one of 263 to 526 keys,
+// 30 heads of 64: 9.0 us in one launch, of which the first loads from HBM and cold code are most.
 #include <math.h>
 
 #include <algorithm>
