@@ -188,7 +188,7 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         float none;
-        S[e] = bend<T, false>(S[e] * a.cap_in, none) * a.cap_log2;
+        S[e] = bend<T, false>(S[e] * a.cap_in, a.cap_log2, none);
       }
       sc = 1.f;
     }

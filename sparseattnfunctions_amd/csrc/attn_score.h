@@ -96,11 +96,11 @@ __device__ __forceinline__ void set_two_terms(Weights<T>& hi, Weights<T>& lo, in
   }
 }
 
-// tanh(y) and 1 - tanh(y)^2 from two exponentials' accuracy to the type's. 16-bit types: 1 - 2 / (exp2(y') + 1), whose
-// error is absolute, 2^-23; y' = 2 log2(e) y is the argument. fp32: below 0.6 the odd polynomial through tanh(y) / y at
+// cap tanh(y) and 1 - tanh(y)^2, from an exponential's accuracy to the type's. 16-bit types: cap - 2 cap / (exp2(y') + 1), whose
+// error is absolute, 2^-23 cap; y' = 2 log2(e) y is the argument. fp32: below 0.6 the odd polynomial through tanh(y) / y at
 // Chebyshev nodes (relative error 7e-8), because a small score would otherwise lose its bits.
 template <typename T, bool kSlope>
-__device__ inline float bend(float y, float& slope) {
+__device__ inline float bend(float y, float cap, float& slope) {
   if constexpr (std::is_same<T, float>::value) {
     const float z = y * y;
     float p = 2.3734868e-3f;
@@ -112,11 +112,11 @@ __device__ inline float bend(float y, float& slope) {
     const float r = __builtin_amdgcn_rcpf(fast_exp2(y * (2.f * kLog2e)) + 1.f);
     const float t = fabsf(y) < 0.6f ? fmaf(y * z, p, y) : fmaf(r, -2.f, 1.f);
     if constexpr (kSlope) slope = fabsf(y) < 0.6f ? fmaf(-t, t, 1.f) : 4.f * fmaf(-r, r, r);
-    return t;
+    return t * cap;
   } else {
     const float r = __builtin_amdgcn_rcpf(fast_exp2(y) + 1.f);
     if constexpr (kSlope) slope = 4.f * fmaf(-r, r, r);
-    return fmaf(r, -2.f, 1.f);
+    return fmaf(r, -2.f * cap, cap);
   }
 }
 

@@ -92,7 +92,7 @@ __device__ __forceinline__ float apply_rule(const ScoredArgs& a, float slope_h, 
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       float t = 0.f;
-      S[e] = bend<T, kSlope>(S[e] * a.cap_in, t) * a.cap_log2;
+      S[e] = bend<T, kSlope>(S[e] * a.cap_in, a.cap_log2, t);
       if constexpr (kSlope) slope[e] = t;
     }
     sc = 1.f;
