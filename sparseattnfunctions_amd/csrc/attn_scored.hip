@@ -603,6 +603,7 @@ ScoredArgs common_args(const sa_attn_scored& t) {
   if (t.cap > 0) {
     a.cap_in = t.sm_scale / t.cap * (t.dtype == SA_DTYPE_F32 ? 1.f : 2.f * kLog2e);
     a.cap_log2 = t.cap * kLog2e;
+    a.cap_out = 1.f / a.cap_log2;
   }
   a.slopes = t.slopes;
   a.radius = t.table ? t.radius : 0;

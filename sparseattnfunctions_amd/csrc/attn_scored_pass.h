@@ -62,7 +62,7 @@ struct ScoredArgs {
   const int2* ranges;  // [b * ranges_sb + key] = {from, until}; may be null
   int64_t ranges_sb;
   float sm_scale, scale_log2;
-  float cap_in, cap_log2;  // 2 log2(e) sm_scale / cap (fp32: sm_scale / cap), cap log2(e)
+  float cap_in, cap_log2, cap_out;  // 2 log2(e) sm_scale / cap (fp32: sm_scale / cap), cap log2(e), 1 / cap_log2
   const float* slopes;     // [H]; may be null
   const float* ebias;      // [H][2 radius + 1 + 2 kPad] biases of distances -radius - kPad .., times log2(e); may be null
   int radius;
@@ -448,7 +448,10 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
     const int least = kMode == kKeys ? row0 + a.q_start - first - 31 : first + a.q_start - row0 - 31;
     int side_far;
     const int own = kStep * w + col;
-    const float sc = apply_rule<kMode == kKeys ? 1 : -1, kCap, kRule, kMode != kForward, T>(
+    // With nothing but a cap the key pass takes its derivative from the score where that is used up: 16 registers less, which
+    // were spilled (428 us at head dim 128, 401 so; the query pass has them, and takes 2 % longer so).
+    constexpr bool kFromScore = kMode == kKeys && kCap && kRule == kPlain && !kF32;
+    const float sc = apply_rule<kMode == kKeys ? 1 : -1, kCap, kRule, kMode != kForward && !kFromScore, T>(
         a, s.slope, s.past, s.before, base, least, bias + (kMode == kKeys ? 4 * hh + 63 - own : own + 4 - 4 * hh), S, slope,
         side_far);
     if (s.cut) {
@@ -511,7 +514,13 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
           P.set(e + 2, p[2] * f, p[3] * f);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) dP[e + i] *= p[i];
+        for (int i = 0; i < 4; ++i) {
+          dP[e + i] *= p[i];
+          if constexpr (kFromScore) {  // (clamped: pairs that are not seen have -inf, and P 0)
+            const float t = S[e + i] * a.cap_out;
+            dP[e + i] *= __builtin_amdgcn_fmed3f(fmaf(-t, t, 1.f), 0.f, 1.f);
+          }
+        }
       }
       if constexpr (kMode == kQueries && kRule == kTable) {
         if (a.far) {
@@ -544,7 +553,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
       }
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        if constexpr (kCap) dC.set(e, dP[e] * slope[e], dP[e + 1] * slope[e + 1]);
+        if constexpr (kCap && !kFromScore) dC.set(e, dP[e] * slope[e], dP[e + 1] * slope[e + 1]);
         else dC.set(e, dP[e], dP[e + 1]);
       }
       if constexpr (kF32) {
