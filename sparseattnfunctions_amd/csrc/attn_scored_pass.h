@@ -15,7 +15,7 @@
 // rounding or two: at [1, 15, 17776, 64] by frames of 1350 the matrix units are busy for 50, 58 and 57 % of the
 // three passes' cycles and vector instructions issue in 77, 52 and 51 %, at 1.5 GHz; LDS has no bank conflicts.
 // Measured, us of forward, query and key pass (TFLOP/s of the products done): 1130, 975, 1320 (865, 1000, 990) there;
-// [1, 16, 4096, 128] fp16, every pair, 229, 229, 335 (900, 900, 820), with a cap 350, 335, 515 (its tanh is an exp2, a
+// [1, 16, 4096, 128] fp16, every pair, 229, 229, 335 (900, 900, 820), with a cap 278, 300, 401 (its tanh is an exp2, a
 // reciprocal and three more an element); [2, 30, 2560, 64] with a bias 225, 240, 258 (670, 630, 780).
 // Tiles of 32 own rows a wave: 64 would halve the LDS reads, which are not the bound, for twice the registers.
 #pragma once

@@ -44,6 +44,7 @@ CASES = {
     "split_short": (dict(B=4, H=2, Hk=2, Ln=2, L=2500), [0, 1, 64, 2500], dict()),
     "window_one": (dict(B=2, H=2, Hk=2, Ln=3, L=90), [90, 2], dict(window=1)),
     "window": (dict(B=3, H=4, Hk=2, Ln=4, L=2000, D=128), [2000, 40, 3], dict(window=37, kind="table")),
+    "longer_than_the_cache": (dict(B=2, H=2, Hk=1, Ln=9, L=4), [4, 2], dict(Lp=40, window=7)),
     "many": (dict(B=70, H=2, Hk=1, Ln=1, L=20), list(range(-25, 45)), dict(kind="slopes")),
     "prefix_one": (dict(B=2, H=2, Hk=2, Ln=1, L=8), [1, 8], dict(Lp=1)),
     "prefix": (dict(B=5, H=6, Hk=2, Ln=3, L=77, D=128), [0, 2, 3, 77, 50], dict(Lp=226, kind="cap slopes")),

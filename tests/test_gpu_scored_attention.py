@@ -383,6 +383,24 @@ def test_other_stream(dev):
         assert torch.equal(a, b)
 
 
+def test_two_steps_at_once(dev):
+    case("two streams")
+    calls = [make(n, BF16, dev) for n in ("split_keys", "causal_table")]
+    want = [results(*x, 0.25, opts) for x, opts in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for s, (x, opts), to in zip(streams, calls, got):
+            with torch.cuda.stream(s):
+                to.append(results(*[t.detach().requires_grad_() for t in x[:3]], x[3], 0.25,
+                                  dict(opts, table=opts["table"].detach().requires_grad_())))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, w))
+
+
 @pytest.mark.parametrize("name", ["documents", "split_keys", "mask_and_ranges"])
 def test_captured_step(dev, name):
     case(f"captured {name}")
