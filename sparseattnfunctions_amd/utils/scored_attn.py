@@ -251,11 +251,15 @@ def _check_ranges(ranges, q, B, Lk):
     if ranges.dtype != torch.int32 or ranges.dim() not in (2, 3) or ranges.shape[-2:] != (Lk, 2) \
             or (ranges.dim() == 3 and ranges.shape[0] not in (1, B)):
         raise ValueError(f"ranges must be int32 [{B}, {Lk}, 2], got {ranges.dtype} {tuple(ranges.shape)}")
-    if ranges.dim() == 2:
-        ranges = ranges[None]
-    if ranges.stride(2) != 1 or (ranges.stride(1) != 2 and Lk > 1) or ranges.stride(0) % 2 or ranges.data_ptr() % 8:
+    return _pairs(ranges if ranges.dim() == 3 else ranges[None]).expand(B, -1, -1)
+
+
+def _pairs(ranges):
+    """ranges [b, Lk, 2] as the kernels read them: a sequence's pairs one after the other, 8-byte aligned."""
+    sb, sl, s1 = ranges.stride()
+    if s1 != 1 or (sl != 2 and ranges.shape[1] > 1) or sb % 2 or ranges.data_ptr() % 8:
         ranges = ranges.clone(memory_format=torch.contiguous_format)
-    return ranges.expand(B, -1, -1)
+    return ranges
 
 
 def _check_mask(mask, q, B, H, nqb, nkb):
@@ -317,8 +321,13 @@ def _backward(dout, state, needs):
             or not all(t.data_ptr() % 16 == 0 for t in (q, k, v, out)):  # (hooks on saved tensors have moved them)
         q, k, v, out = _rows16(q), _rows16(k), _rows16(v), out.contiguous()
         args.strides[:9] = (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
-    if table is not None and not table.is_contiguous():
-        table = table.contiguous()
+    if slopes is not None:
+        slopes = slopes.contiguous()
+    if table is not None:
+        table, buckets = table.contiguous(), buckets.contiguous()
+    if ranges is not None:
+        ranges = _pairs(ranges)
+        args.ranges_stride = ranges.stride(0) // 2
     _point(call, args, q, k, v, out, buffer, ranges, slopes, table, buckets)
     if dout.stride() != call.contiguous or dout.data_ptr() % 16:
         dout = _rows16(dout)
