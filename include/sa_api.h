@@ -326,7 +326,7 @@ typedef struct sa_attn_scored {
   int64_t ranges_stride;   /* keys from one sequence to the next (0: one for all) */
   const uint8_t* mask;     /* nullable block mask; read by the forward call alone */
   int64_t mask_strides[4]; /* {b, h, q block, k block} in bytes */
-  float sm_scale, cap;
+  float sm_scale, cap;     /* cap 0: none; else above 1e-30 and below 1e30, and sm_scale / cap a normal number */
   const float* slopes;     /* nullable [H] */
   const void* table;       /* nullable [n_buckets][H] */
   const int32_t* buckets;  /* [2*radius+1]; entries outside [0, n_buckets) are taken as the nearest one */

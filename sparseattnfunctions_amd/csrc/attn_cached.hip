@@ -41,7 +41,8 @@ struct CachedArgs {
   int prefix_tiles, prefix_splits;  // of all sequences' rows of a key head, and alike for the prefix
   int own_groups;                   // B * Hk * tiles * splits workgroups, and behind them the prefix's
   int lead;                         // steps of the prefix that each sequence takes before its own; then prefix_splits is 0
-  float scale_log2, cap_in, cap_log2;
+  float scale_log2;
+  Cap cap;
   const float* slopes;
   const void* table;
   const int32_t* buckets;
@@ -185,11 +186,9 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
     __builtin_amdgcn_sched_barrier(0);
     float sc = a.scale_log2;
     if constexpr (kCap) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float none;
-        S[e] = bend<T, false>(S[e] * a.cap_in, a.cap_log2, none);
-      }
+      sa_f32x16 none;
+      if (std::is_same<T, float>::value || a.cap.fine) bend_all<true, false>(a.cap.in, a.cap.log2, S, none);
+      else bend_all<false, false>(a.cap.in, a.cap.log2, S, none);
       sc = 1.f;
     }
     const int base = place - row0 - 4 * hh;  // d = base - c_e
@@ -413,8 +412,7 @@ int check_cached(const sa_attn_cached* t, const char* fn) {
   if (t->L > 1 << 29 || t->Lp > 1 << 29) return sa::fail(SA_ERR_UNSUPPORTED, "%s: more than 2^29 keys", fn);
   SA_REQUIRE(t->sm_scale > 0.f && std::isfinite(t->sm_scale), "%s: sm_scale must be positive and finite", fn);
   SA_REQUIRE(t->cap >= 0.f && std::isfinite(t->cap), "%s: cap must be positive and finite, or 0 for none", fn);
-  SA_REQUIRE(!t->cap || (t->cap > 1e-30f && std::isfinite(t->sm_scale / t->cap * 3.f) && t->sm_scale / t->cap > 0.f),
-             "%s: sm_scale / cap out of range", fn);
+  SA_REQUIRE(cap_in_range(t->sm_scale, t->cap), "%s: cap or sm_scale / cap out of range", fn);
   if (t->table) {
     SA_REQUIRE(t->buckets && t->n_buckets > 0, "%s: table without buckets", fn);
     SA_REQUIRE(t->table_dtype >= SA_DTYPE_BF16 && t->table_dtype <= SA_DTYPE_F32, "%s: table dtype %d", fn, t->table_dtype);
@@ -489,10 +487,7 @@ extern "C" int sa_attn_cached_fwd(const sa_attn_cached* t, void* stream) {
   a.prefix_tiles = p.prefix_tiles; a.prefix_splits = p.prefix_splits;
   a.own_groups = (int)p.own_groups; a.lead = p.lead;
   a.scale_log2 = t->sm_scale * kLog2e;
-  if (t->cap > 0) {
-    a.cap_in = t->sm_scale / t->cap * (t->dtype == SA_DTYPE_F32 ? 1.f : 2.f * kLog2e);
-    a.cap_log2 = t->cap * kLog2e;
-  }
+  a.cap = cap_of(t->sm_scale, t->cap, t->dtype);
   a.slopes = t->slopes;
   a.table = t->table; a.buckets = t->buckets;
   a.table_dtype = t->table_dtype; a.n_buckets = t->n_buckets; a.radius = t->radius;

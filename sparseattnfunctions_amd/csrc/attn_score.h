@@ -2,6 +2,7 @@
 // 32 bits, the cap, and the products of a step of 32 streamed rows with an own row per MFMA column.
 #pragma once
 
+#include <cfloat>
 #include <type_traits>
 
 #include "attn_tile.h"
@@ -96,12 +97,14 @@ __device__ __forceinline__ void set_two_terms(Weights<T>& hi, Weights<T>& lo, in
   }
 }
 
-// cap tanh(y) and 1 - tanh(y)^2, from an exponential's accuracy to the type's. 16-bit types: cap - 2 cap / (exp2(y') + 1), whose
-// error is absolute, 2^-23 cap; y' = 2 log2(e) y is the argument. fp32: below 0.6 the odd polynomial through tanh(y) / y at
-// Chebyshev nodes (relative error 7e-8), because a small score would otherwise lose its bits.
-template <typename T, bool kSlope>
+// cap tanh(y) and 1 - tanh(y)^2, in one of two ways. Fine: below 0.6 the odd polynomial through tanh(y) / y at Chebyshev nodes
+// (relative error 7e-8), because a small score would otherwise lose its bits. Else cap - 2 cap / (exp2(y') + 1), whose error is
+// absolute, 2e-7 cap; y' = 2 log2(e) y is the argument. fp32 calls are fine, 16-bit ones where the cap is above kFineCap, whose
+// 2e-7 is a tenth of fp16's rounding of P (at a cap of 1e4 scores were off by 0.002, at 1e7 by 1.7).
+constexpr float kFineCap = 256.f;
+template <bool kFine, bool kSlope>
 __device__ inline float bend(float y, float cap, float& slope) {
-  if constexpr (std::is_same<T, float>::value) {
+  if constexpr (kFine) {
     const float z = y * y;
     float p = 2.3734868e-3f;
     p = fmaf(p, z, -8.4125260e-3f);
@@ -118,6 +121,35 @@ __device__ inline float bend(float y, float cap, float& slope) {
     if constexpr (kSlope) slope = 4.f * fmaf(-r, r, r);
     return fmaf(r, -2.f * cap, cap);
   }
+}
+
+// The capped products of a tile.
+template <bool kFine, bool kSlope>
+__device__ __forceinline__ void bend_all(float cap_in, float cap, sa_f32x16& S, sa_f32x16& slope) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float t = 0.f;
+    S[e] = bend<kFine, kSlope>(S[e] * cap_in, cap, t);
+    if constexpr (kSlope) slope[e] = t;
+  }
+}
+
+// A call's cap as the kernels have it: the products' factor, the cap times log2(e), and the way.
+struct Cap {
+  float in, log2;
+  int fine;
+};
+inline Cap cap_of(float sm_scale, float cap, int dtype) {
+  Cap c{};
+  if (!(cap > 0)) return c;
+  c.fine = dtype == SA_DTYPE_F32 || cap > kFineCap;
+  c.in = sm_scale / cap * (c.fine ? 1.f : 2.f * kLog2e);
+  c.log2 = cap * kLog2e;
+  return c;
+}
+// Caps and scales whose quotient is a normal number, with room for its factors.
+inline bool cap_in_range(float sm_scale, float cap) {
+  return !cap || (cap > 1e-30f && cap < 1e30f && sm_scale / cap * 3.f <= FLT_MAX && sm_scale / cap >= FLT_MIN);
 }
 
 __device__ inline float load_as_float(const void* p, int dtype, int64_t i) {

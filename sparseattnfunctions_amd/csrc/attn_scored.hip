@@ -527,8 +527,7 @@ int check_scored(const sa_attn_scored* t, const char* fn) {
   if (t->D != 64 && t->D != 128) return sa::fail(SA_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", fn, t->D);
   SA_REQUIRE(t->sm_scale > 0.f && std::isfinite(t->sm_scale), "%s: sm_scale must be positive and finite", fn);
   SA_REQUIRE(t->cap >= 0.f && std::isfinite(t->cap), "%s: cap must be positive and finite, or 0 for none", fn);
-  SA_REQUIRE(!t->cap || (t->cap > 1e-30f && std::isfinite(t->sm_scale / t->cap * 3.f) && t->sm_scale / t->cap > 0.f),
-             "%s: sm_scale / cap out of range", fn);
+  SA_REQUIRE(cap_in_range(t->sm_scale, t->cap), "%s: cap or sm_scale / cap out of range", fn);
   if (t->Lq > 1 << 27 || t->Lk > 1 << 27) return sa::fail(SA_ERR_UNSUPPORTED, "%s: more than 2^27 rows", fn);
   SA_REQUIRE(t->q_start > -(1 << 29) && t->q_start < 1 << 29, "%s: q_start %d", fn, t->q_start);
   if ((int64_t)t->B * t->H * std::max(sa::cdiv(t->Lq, kBlk), sa::cdiv(t->Lk, kBlk)) >= 1LL << 24 || t->H >= 1 << 20)
@@ -579,7 +578,8 @@ void launch_pass(int mode, ScoredArgs a, const sa_attn_scored& t, const SidePlan
     m.gb_sb = a.gb_sb; m.gb_sh = a.gb_sh; m.gb_sl = a.gb_sl;
     m.sm_scale = a.sm_scale; m.lse = a.lse; m.far = a.far; m.n_far = 2 * a.radius + 1;
   }
-  PassCall c = {mode, t.D, t.cap > 0, 8u * (unsigned)(p.scheduled ? p.cap : xcd_items(a.BH_own, a.n_own)), 0, s};
+  const int cap = !(t.cap > 0) ? kNoCap : cap_of(t.sm_scale, t.cap, t.dtype).fine ? kFineTanh : kTanh;
+  PassCall c = {mode, t.D, cap, 8u * (unsigned)(p.scheduled ? p.cap : xcd_items(a.BH_own, a.n_own)), 0, s};
   // (the statistics alone are written by every item's first unit)
   if (p.scheduled && (a.grad_a || a.grad_b || a.far)) c.merge_grid = 8u * (unsigned)p.split_cap;
   if (t.dtype == SA_DTYPE_BF16) launch_pass_bf16(a, m, c);
@@ -601,9 +601,10 @@ ScoredArgs common_args(const sa_attn_scored& t) {
   a.sm_scale = t.sm_scale;
   a.scale_log2 = t.sm_scale * kLog2e;
   if (t.cap > 0) {
-    a.cap_in = t.sm_scale / t.cap * (t.dtype == SA_DTYPE_F32 ? 1.f : 2.f * kLog2e);
-    a.cap_log2 = t.cap * kLog2e;
-    a.cap_out = 1.f / a.cap_log2;
+    const Cap c = cap_of(t.sm_scale, t.cap, t.dtype);
+    a.cap_in = c.in;
+    a.cap_log2 = c.log2;
+    a.cap_out = 1.f / c.log2;
   }
   a.slopes = t.slopes;
   a.radius = t.table ? t.radius : 0;

@@ -33,6 +33,9 @@ constexpr int kBlk = 64;
 constexpr int kCus = 256;
 enum { kForward = 0, kQueries = 1, kKeys = 2 };
 enum { kPlain = 0, kSlopes = 1, kTable = 2 };  // kTable: with or without slopes
+// How scores are capped (bend). A choice of kernels: with both ways in one, registers that fit are spilled (query pass with
+// slopes at head dim 64 20 bytes a lane, 36 so).
+enum { kNoCap = 0, kTanh = 1, kFineTanh = 2 };
 // fp16 holds normal numbers from 2^-14, which the probabilities of an even row fall short of over more than 16 384
 // keys: P is rounded to the type with this factor (one product an element), which dv loses at the end.
 constexpr float kPScale = 4096.f;
@@ -62,7 +65,7 @@ struct ScoredArgs {
   const int2* ranges;  // [b * ranges_sb + key] = {from, until}; may be null
   int64_t ranges_sb;
   float sm_scale, scale_log2;
-  float cap_in, cap_log2, cap_out;  // 2 log2(e) sm_scale / cap (fp32: sm_scale / cap), cap log2(e), 1 / cap_log2
+  float cap_in, cap_log2, cap_out;  // 2 log2(e) sm_scale / cap (fine: sm_scale / cap), cap log2(e), 1 / cap_log2
   const float* slopes;     // [H]; may be null
   const float* ebias;      // [H][2 radius + 1 + 2 kPad] biases of distances -radius - kPad .., times log2(e); may be null
   int radius;
@@ -84,17 +87,12 @@ struct ScoredArgs {
 // 0, from which element e is kSign (8 (e / 4) + e % 4) away. least .. least + 62: the wave's distances. window: where the
 // lane's biases lie in LDS, from element 0 (kSign > 0) or element 15 (kSign < 0) on. kSlope: slope becomes the cap's
 // derivative. side: whether all pairs of the wave are past the radius, 1 above, -1 below, 0 not all.
-template <int kSign, bool kCap, int kRule, bool kSlope, typename T>
+template <int kSign, int kCap, int kRule, bool kSlope, typename T>
 __device__ __forceinline__ float apply_rule(const ScoredArgs& a, float slope_h, float past, float before, int base, int least,
                                             const float* window, sa_f32x16& S, sa_f32x16& slope, int& side) {
   float sc = a.scale_log2;
   if constexpr (kCap) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float t = 0.f;
-      S[e] = bend<T, kSlope>(S[e] * a.cap_in, a.cap_log2, t);
-      if constexpr (kSlope) slope[e] = t;
-    }
+    bend_all<kCap == kFineTanh || std::is_same<T, float>::value, kSlope>(a.cap_in, a.cap_log2, S, slope);
     sc = 1.f;
   }
   if (kRule == kSlopes || (kRule == kTable && a.slopes)) {
@@ -190,7 +188,7 @@ constexpr int waves_per_simd() {
   return std::is_same<T, float>::value ? (kD == 64 ? 2 : 1) : kD == 64 ? 3 : 2;
 }
 
-template <int kMode, bool kCap, int kRule, typename T, int kD>
+template <int kMode, int kCap, int kRule, typename T, int kD>
 __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(ScoredArgs a) {
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int kSize = kF32 ? 4 : 2;
@@ -722,12 +720,12 @@ __global__ __launch_bounds__(kMergeThreads) void scored_merge_kernel(MergeArgs a
 // ---- Launches of a pass. Each element type's kernels are compiled by themselves (attn_scored_*.hip).
 struct PassCall {
   int mode, D;
-  bool cap;
+  int cap;  // kNoCap, kTanh or kFineTanh
   unsigned grid, merge_grid;  // merge_grid 0: no item is split
   hipStream_t stream;
 };
 
-template <int kMode, bool kCap, int kRule, typename T, int kD>
+template <int kMode, int kCap, int kRule, typename T, int kD>
 void launch_kernels(const ScoredArgs& a, const MergeArgs& m, const PassCall& c) {
   const size_t lds = kMode == kQueries && kRule == kTable && a.far ? 2 * (kDiagonals + 2 * a.radius + 1) * sizeof(float) : 0;
   hipLaunchKernelGGL((scored_kernel<kMode, kCap, kRule, T, kD>), dim3(c.grid), dim3(128), lds, c.stream, a);
@@ -739,7 +737,7 @@ template <typename T>
 void launch_pass_of(const ScoredArgs& a, const MergeArgs& m, const PassCall& c) {
   auto dim = [&](auto mode, auto cap, auto rule) {
     constexpr int kMode = decltype(mode)::value, kRule = decltype(rule)::value;
-    constexpr bool kCap = decltype(cap)::value;
+    constexpr int kCap = decltype(cap)::value;
     if (c.D == 64) launch_kernels<kMode, kCap, kRule, T, 64>(a, m, c);
     else launch_kernels<kMode, kCap, kRule, T, 128>(a, m, c);
   };
@@ -749,8 +747,10 @@ void launch_pass_of(const ScoredArgs& a, const MergeArgs& m, const PassCall& c) 
     else dim(mode, cap, std::integral_constant<int, kPlain>());
   };
   auto cap = [&](auto mode) {
-    if (c.cap) rule(mode, std::true_type());
-    else rule(mode, std::false_type());
+    if (c.cap == kNoCap) return rule(mode, std::integral_constant<int, kNoCap>());
+    if constexpr (!std::is_same<T, float>::value)
+      if (c.cap == kTanh) return rule(mode, std::integral_constant<int, kTanh>());
+    rule(mode, std::integral_constant<int, kFineTanh>());
   };
   if (c.mode == kForward) cap(std::integral_constant<int, kForward>());
   else if (c.mode == kQueries) cap(std::integral_constant<int, kQueries>());

@@ -4,7 +4,8 @@ import torch
 
 import scored_reference as ref
 from conftest import case
-from sparseattnfunctions_amd.utils.scored_attn import row_ranges, scored_attention
+from sparseattnfunctions_amd.utils.cached_attn import cached_attention
+from sparseattnfunctions_amd.utils.scored_attn import distance_buckets, row_ranges, scored_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +30,54 @@ def test_moved_ranges(dev, cut):
         got = [out, *torch.autograd.grad(out, (q, k, v), do)]
     for n, x in zip(NAMES, got):
         ref.check(n, x, want[n])
+
+
+def fine_cap(monkeypatch):
+    """The reference's scores with an error that does not grow with the cap: tanh below 0.6 comes from a polynomial, off by 7e-8
+    of the value and a handful of roundings, above it from 1 - 2 r, off by 2 (|y'| + 4) r 2^-24 <= 2^-22: less than 2^-20 of
+    the score in all."""
+    plain = ref.scores
+
+    def scores(q, k, scale, far, cap=None, slopes=None, table=None, buckets=None):
+        s, c, _, e_c, place = plain(q, k, scale, far, cap, slopes, table, buckets)
+        e = plain(q, k, scale, far, None, slopes, table, buckets)[2]
+        product = scale * (q @ k.transpose(-1, -2))
+        return s, c, e + 2.0 ** -20 * product.abs(), e_c, place
+
+    monkeypatch.setattr(ref, "scores", scores)
+
+
+@pytest.mark.parametrize("cap", [257.0, 1e3, 1e4, 1e5, 1e7, 1e20])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=str)
+@pytest.mark.parametrize("kind", ["plain", "slopes", "table"])
+def test_large_caps(dev, monkeypatch, cap, dtype, kind):
+    case(f"cap {cap} {dtype} {kind}")
+    fine_cap(monkeypatch)
+    H, D = 2, 128 if kind == "slopes" else 64
+    q, k, v, do = ref.inputs(13, 1, H, 1, 150, 330, D, dtype, dev)
+    opts = dict(cap=cap, q_start=180)
+    wanted = [q, k, v]
+    if kind == "slopes":
+        opts["slopes"] = torch.tensor([0.02, -0.01], device=dev)
+    if kind == "table":
+        opts["buckets"] = distance_buckets(32, 128, device=dev)
+        opts["table"] = torch.randn(32, H, generator=torch.Generator().manual_seed(1)).to(dev)
+        wanted.append(opts["table"])
+    for t in wanted:
+        t.requires_grad_()
+    ranges = row_ranges(torch.tensor([330], device=dev), 330)
+    want = ref.train(q, k, v, do, 0.3, ranges=ranges, **opts)
+    out = scored_attention(q, k, v, 0.3, ranges=ranges, **opts)
+    for n, x in zip(NAMES, (out, *torch.autograd.grad(out, wanted, do))):
+        ref.check(n, x, want[n])
+
+
+@pytest.mark.parametrize("cap", [257.0, 1e4, 1e7, 1e20])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=str)
+def test_large_caps_over_caches(dev, monkeypatch, cap, dtype):
+    case(f"cap {cap} over caches {dtype}")
+    fine_cap(monkeypatch)
+    q, k, v, _ = ref.inputs(14, 2, 4, 2, 3, 1500, 64, dtype, dev)
+    q = q[:, :, :3]
+    n = torch.tensor([1500, 40], dtype=torch.int32, device=dev)
+    ref.check("out", cached_attention(q, k, v, n, 0.3, cap=cap), ref.serve(q, k, v, n, 0.3, cap=cap))
