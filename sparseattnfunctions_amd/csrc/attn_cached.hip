@@ -219,8 +219,8 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, S[e]);
     top = xhalf_max(top) * sc;
-    if (__ballot(top > m + kSlack)) {
-      const float next_m = fmaxf(m, top);
+    if (__ballot(top > m + kAbove<T>)) {
+      const float next_m = fmaxf(m, top - kBelow<T>);
       const float f = next_m == m ? 1.f : fast_exp2(m - next_m);
       m = next_m;
       l *= f;

@@ -12,8 +12,13 @@ namespace {
 
 constexpr int kStep = 32;          // streamed rows per step, own rows per wave
 constexpr int kMostRadius = 1024;  // distances that a bias tells apart
-// A row's offset follows its maximum when that has grown by more than this (log2 units): P stays below 2^8.
-constexpr float kSlack = 8.f;
+// A row's offset (log2 units) is left where it is until its maximum lies more than kAbove over it; then it is put kBelow under
+// that. P stays below 2^kAbove. fp16 has no number under 2^-25 but zero: with the offset at the maximum itself, 45104 keys of
+// 2^-25.5 behind a strong one lost 1e-3 of the row; this way what is below 2^-36 of the maximum is lost.
+template <typename T>
+constexpr float kAbove = std::is_same<T, _Float16>::value ? 15.f : 8.f;
+template <typename T>
+constexpr float kBelow = std::is_same<T, _Float16>::value ? 11.f : 0.f;
 
 template <typename T>
 __device__ inline float2 unpack2(uint32_t w) {

@@ -469,8 +469,8 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, S[e]);
       top = xhalf_max(top) * sc;
-      if (__ballot(top > m + kSlack)) {
-        const float next_m = fmaxf(m, top);
+      if (__ballot(top > m + kAbove<T>)) {
+        const float next_m = fmaxf(m, top - kBelow<T>);
         const float f = next_m == m ? 1.f : fast_exp2(m - next_m);
         m = next_m;
         l *= f;

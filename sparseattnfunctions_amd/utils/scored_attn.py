@@ -413,10 +413,10 @@ def scored_attention(q, k, v, sm_scale: float, *, cap: Optional[float] = None, s
 
     q [B,H,Lq,D], k and v [B,Hk,Lk,D] (H a multiple of Hk) on the GPU, bf16, fp16 or fp32 (one type), D = 64
     or 128, any strides (tensors whose rows are not 16-byte aligned are copied). cap: a number between 1e-30 and
-    1e30, however large beside the scores; slopes: fp32 [H]; table: [n, H] of any of the three types, with buckets int32 [2 R + 1] (R up to 1024; entries outside
-    [0, n) count as the nearest one); ranges: int32 [B or 1, Lk, 2] (`row_ranges`, or a caller's own);
-    block_mask: bool or integer [B or 1, H or 1, >= ceil(Lq / 64), >= ceil(Lk / 64)]; q_start: the position of
-    row 0 where key 0 has position 0, for the distances alone (ranges count rows from 0).
+    1e30; slopes: fp32 [H]; table: [n, H] of any of the three types, with buckets int32 [2 R + 1] (R up to 1024;
+    entries outside [0, n) count as the nearest one); ranges: int32 [B or 1, Lk, 2] (`row_ranges`, or a caller's
+    own); block_mask: bool or integer [B or 1, H or 1, >= ceil(Lq / 64), >= ceil(Lk / 64)]; q_start: the position
+    of row 0 where key 0 has position 0, for the distances alone (ranges count rows from 0).
 
     The tensors must stay as they are until the backward pass has run. A call captured into a HIP graph needs
     leaves that no eager graph holds (autograd ties a leaf's gradient to the stream of its first use)."""

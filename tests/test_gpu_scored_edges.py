@@ -1,4 +1,6 @@
 """Attention with score rules on the GPU at the ends of what its arguments allow, against 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -81,3 +83,29 @@ def test_large_caps_over_caches(dev, monkeypatch, cap, dtype):
     q = q[:, :, :3]
     n = torch.tensor([1500, 40], dtype=torch.int32, device=dev)
     ref.check("out", cached_attention(q, k, v, n, 0.3, cap=cap), ref.serve(q, k, v, n, 0.3, cap=cap))
+
+
+@pytest.mark.parametrize("n", [300, 17776, 45104])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("dtype", [FP16, BF16], ids=str)
+def test_many_weak_keys(dev, dtype, first, n):
+    """A key that stands out, its value 0, and n of 2^-25.5 of its weight, their values 1."""
+    case(f"{n} weak keys {dtype}, the strong one first: {first}")
+    k = torch.zeros(1, 1, n + 1, 64, dtype=dtype, device=dev)
+    v = torch.ones(1, 1, n + 1, 64, dtype=dtype, device=dev)
+    at = 0 if first else n
+    k[:, :, at, 0] = 16.0
+    v[:, :, at] = 0
+    q = torch.zeros(1, 1, 1, 64, dtype=dtype, device=dev)
+    q[..., 0] = 1.0
+    scale = 25.5 * math.log(2.0) / 16
+    weak = n * 2.0 ** -25.5
+    want = weak / (1 + weak)
+    # P rounded to the type (fp16: also to steps of 2^-24, 2^-11 under the row's maximum) for all weak keys alike, out
+    # rounded, the scores' 25.5 in fp32, and sums of n
+    u = torch.finfo(dtype).eps / 2
+    bound = want * (2 * u + 2.0 ** -18 + n * 2.0 ** -24) + (n * 2.0 ** -36 if dtype == FP16 else 0.0)
+    assert bound < 0.02 * want
+    lengths = torch.tensor([n + 1], dtype=torch.int32, device=dev)
+    for out in (cached_attention(q, k, v, lengths, scale), scored_attention(q, k, v, scale)):
+        assert (out.double() - want).abs().max().item() <= bound
