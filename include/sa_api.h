@@ -363,8 +363,8 @@ int sa_attn_scored_bwd(const sa_attn_scored* call, void* stream);
  * a prefix of Lp tokens that all sequences begin with, whose keys and values are held (and read) once.
  * Sequence b has lengths[b] cached tokens (clamped to [0, L]), the last Ln of them the new ones; new token i is its
  * token t = lengths[b] - Ln + i, at distance d = t - j from its key j and Lp + t - j from the prefix's. It sees keys at
- * d >= 0, with window > 0 at d < window; where t < 0 none, and its output is zeros. Cached rows from lengths[b] on are not used,
- * whatever they hold.
+ * d >= 0, with window > 0 at d < window; where t < 0 none, and its output is zeros. Cached rows that no new token of the
+ * sequence sees, from lengths[b] on or before the window, are not used, whatever they hold (nor prefix rows that none at all sees).
  */
 typedef struct sa_attn_cached {
   int32_t dtype;       /* SA_DTYPE_*: of q, out and the keys and values */

@@ -117,16 +117,22 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
   near = __builtin_amdgcn_readfirstlane(near);
   far = __builtin_amdgcn_readfirstlane(far);
   const bool blind = __ballot(t < 0) != 0;
-  // The tile's keys, whole steps of them from the first that a row sees, and the split's and wave's share. Steps of a leading
-  // prefix hold keys -Lp .. -1.
+  // The tile's keys: of a leading prefix those from p0 on, `lead` steps of them (keys -Lp + p0 .. -1), and then those from k0 on.
+  // Both begin with the first key that a row sees: rows of the cache before a window may hold anything, and P = 0 times that
+  // need not be 0.
   const int end = shared ? a.Lp : __builtin_amdgcn_readfirstlane(min(max(a.lengths[b0], 0), a.L));
-  const int lead = kLead ? a.lead : 0;
-  int first = 0;
+  int p0 = 0, k0 = 0, lead = kLead ? a.lead : 0;
   if (a.window && near != INT_MAX) {
     const int key = near - a.window + 1;
-    first = key >= 0 || !lead ? lead + max(0, min(key, end)) / kStep : max(0, key + a.Lp) / kStep;
+    if (kLead && key < 0) {
+      p0 = max(0, key + a.Lp);
+      lead = (a.Lp - p0 + kStep - 1) / kStep;
+    } else {
+      lead = 0;
+      k0 = max(0, min(key, end));
+    }
   }
-  const int n_steps = far < 0 ? 0 : lead + (end + kStep - 1) / kStep - first;
+  const int n_steps = far < 0 ? 0 : lead + (end - k0 + kStep - 1) / kStep;
   const int per_split = (n_steps + splits - 1) / splits;
   const int last = min(n_steps, per_split * (split + 1));
   const int begin = split * per_split + w;  // steps begin, begin + kWaves, ..
@@ -135,16 +141,16 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
   // Copies of a step's keys and values: rows past the last cached one, and steps past the wave's last, read as zero whatever is
   // there.
   auto issue = [&](int step, lds_u8* to) __attribute__((always_inline)) {
-    const bool ahead = kLead && first + step < lead;
+    const bool ahead = kLead && step < lead;
     const Cache& c = shared || ahead ? a.prefix : a.own;
-    const int rows = ahead ? a.Lp : end;
+    const int rows = ahead ? a.Lp : end, first = ahead ? p0 + step * kStep : k0 + (step - lead) * kStep;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const int64_t row_bytes = (m == 0 ? c.k_sl : c.v_sl) * kSize;
       const uint8_t* base = m == 0 ? at(c.k, ahead ? 0 : c.k_sb, c.k_sh) : at(c.v, ahead ? 0 : c.v_sb, c.v_sh);
 #pragma unroll
       for (int r16 = 0; r16 < 2; ++r16) {
-        const int row0 = (first + step - (ahead ? 0 : lead)) * kStep + 16 * r16;
+        const int row0 = first + 16 * r16;
         const int64_t left = step < last && row0 < rows ? (rows - 1 - row0) * row_bytes + 128 : 0;
         const int size = __builtin_amdgcn_readfirstlane((int)min(left, (int64_t)INT_MAX));
         const uint8_t* from = base + row0 * row_bytes;
@@ -172,8 +178,8 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 
   auto compute = [&](int step, const lds_u8* from) __attribute__((always_inline)) {
     const lds_u8* mat = from + w * 2 * kMat;
-    const bool ahead = kLead && first + step < lead;
-    const int row0 = (first + step - (ahead ? 0 : lead)) * kStep - (ahead ? a.Lp : 0), limit = ahead ? 0 : end;
+    const bool ahead = kLead && step < lead;
+    const int row0 = ahead ? p0 + step * kStep - a.Lp : k0 + (step - lead) * kStep, limit = ahead ? 0 : end;
     sa_f32x16 S = {};
     sa_u32x4v x[kDS];
 #pragma unroll

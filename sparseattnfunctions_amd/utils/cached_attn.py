@@ -80,8 +80,8 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
     D = 64 or 128. No autograd.
 
     prefix: (k, v) of the shared prefix, each [Hk,Lp,D] or [1,Hk,Lp,D]. The caches and the prefix may have
-    any strides with a contiguous last axis and 16-byte aligned rows; they are not copied. Cached rows from
-    lengths[b] on are not used, whatever they hold. A new token before its sequence's first (lengths[b] <
+    any strides with a contiguous last axis and 16-byte aligned rows; they are not copied. Cached rows that no
+    new token sees, from lengths[b] on or before a window, are not used, whatever they hold. A new token before its sequence's first (lengths[b] <
     Ln) sees nothing: zeros. cap, slopes, table and buckets as in `scored_attention`; window: see above
     (0: none)."""
     B, H, Hk, Ln, L, D = check_heads(q, k, v)

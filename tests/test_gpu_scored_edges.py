@@ -109,3 +109,24 @@ def test_many_weak_keys(dev, dtype, first, n):
     lengths = torch.tensor([n + 1], dtype=torch.int32, device=dev)
     for out in (cached_attention(q, k, v, lengths, scale), scored_attention(q, k, v, scale)):
         assert (out.double() - want).abs().max().item() <= bound
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=str)
+@pytest.mark.parametrize("L, Ln, Lp, window", [(400, 1, 0, 37), (400, 3, 0, 1), (2600, 2, 0, 700), (5000, 4, 0, 100), (60, 2, 100, 90),
+                                               (60, 1, 100, 20), (60, 1, 300, 250), (90, 1, 3000, 2900), (90, 3, 3000, 30)])
+def test_what_a_window_has_left_behind(dev, dtype, L, Ln, Lp, window):
+    case(f"rows before a window: {L} {Ln} {Lp} {window} {dtype}")
+    B, H, Hk = 3, 4, 2
+    g = torch.Generator().manual_seed(15)
+    q, k, v = (torch.randn(B, h, n, 64, generator=g).to(dtype).to(dev) for h, n in ((H, Ln), (Hk, L), (Hk, L)))
+    prefix = tuple(torch.randn(Hk, Lp, 64, generator=g).to(dtype).to(dev) for _ in range(2)) if Lp else None
+    n = torch.tensor([L, L // 2 + 5, Ln], dtype=torch.int32, device=dev)
+    want = ref.serve(q, k, v, n, 0.3, window=window, prefix=prefix)
+    first = n - Ln - window + 1  # of each sequence's own keys; of the prefix the first that any sequence sees
+    at = torch.arange(L, device=dev)
+    unseen = ((at < first[:, None]) | (at >= n[:, None]))[:, None, :, None]
+    k, v = k.masked_fill(unseen, float("nan")), v.masked_fill(unseen, float("inf"))
+    if Lp:
+        unseen = (torch.arange(Lp, device=dev) < first.min() + Lp)[:, None]
+        prefix = (prefix[0].masked_fill(unseen, float("-inf")), prefix[1].masked_fill(unseen, float("nan")))
+    ref.check("out", cached_attention(q, k, v, n, 0.3, window=window, prefix=prefix), want)
