@@ -71,19 +71,39 @@ def _aligned(name, t):
         raise ValueError(f"{name} must have 16-byte aligned rows")
 
 
+class _NotDifferentiable(torch.autograd.Function):
+    """The output of a call on tensors that autograd follows."""
+
+    @staticmethod
+    def forward(ctx, out, *tensors):
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise NotImplementedError("cached_attention has no backward pass; train with scored_attention")
+
+
 def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, sm_scale: float, *,
                      cap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
                      table: Optional[torch.Tensor] = None, buckets: Optional[torch.Tensor] = None, window: int = 0,
                      prefix: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
     """out [B,H,Ln,D] of the new tokens q [B,H,Ln,D] over the caches k and v [B,Hk,L,D] (H a multiple of Hk)
     with lengths int32 [B] (counted with the new tokens, clamped to [0, L]); bf16, fp16 or fp32 (one type),
-    D = 64 or 128. No autograd.
+    D = 64 or 128. Not differentiable: the backward pass of an output whose inputs autograd follows raises.
 
     prefix: (k, v) of the shared prefix, each [Hk,Lp,D] or [1,Hk,Lp,D]. The caches and the prefix may have
     any strides with a contiguous last axis and 16-byte aligned rows; they are not copied. Cached rows that no
     new token sees, from lengths[b] on or before a window, are not used, whatever they hold. A new token before its sequence's first (lengths[b] <
     Ln) sees nothing: zeros. cap, slopes, table and buckets as in `scored_attention`; window: see above
     (0: none)."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or slopes is not None and slopes.requires_grad or table is not None and table.requires_grad
+                                    or prefix is not None and any(t.requires_grad for t in prefix)):
+        with torch.no_grad():
+            out = cached_attention(q, k, v, lengths, sm_scale, cap=cap, slopes=slopes, table=table, buckets=buckets,
+                                   window=window, prefix=prefix)
+        tensors = (q, k, v, slopes, table, *(prefix or ()))
+        return _NotDifferentiable.apply(out, *(t for t in tensors if t is not None))
     B, H, Hk, Ln, L, D = check_heads(q, k, v)
     cap, slopes, table, buckets, radius = check_rule(q, H, cap, None if slopes is None else slopes.detach(), table, buckets)
     if lengths.device != q.device:

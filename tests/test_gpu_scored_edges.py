@@ -130,3 +130,27 @@ def test_what_a_window_has_left_behind(dev, dtype, L, Ln, Lp, window):
         unseen = (torch.arange(Lp, device=dev) < first.min() + Lp)[:, None]
         prefix = (prefix[0].masked_fill(unseen, float("-inf")), prefix[1].masked_fill(unseen, float("nan")))
     ref.check("out", cached_attention(q, k, v, n, 0.3, window=window, prefix=prefix), want)
+
+
+def test_caches_are_not_differentiated(dev):
+    case("a call over caches on tensors that autograd follows")
+    q, k, v, _ = ref.inputs(16, 2, 2, 2, 1, 30, 64, BF16, dev)
+    p = tuple(t[0].clone() for t in (k, v))
+    n = torch.tensor([30, 4], dtype=torch.int32, device=dev)
+    slopes, table = torch.ones(2, device=dev), torch.ones(3, 2, device=dev)
+    buckets = distance_buckets(3, 1, device=dev)
+
+    def call():
+        return cached_attention(q, k, v, n, 0.3, slopes=slopes, table=table, buckets=buckets, prefix=p)
+
+    want = call()
+    assert not want.requires_grad
+    for t in (q, k, v, slopes, table, *p):
+        t.requires_grad_()
+        out = call()
+        assert torch.equal(out, want) and out.requires_grad
+        with pytest.raises(NotImplementedError):
+            out.sum().backward()
+        with torch.no_grad():
+            assert not call().requires_grad
+        t.requires_grad_(False)
