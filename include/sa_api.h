@@ -344,11 +344,12 @@ typedef struct sa_attn_scored {
 #define SA_SCORED_TABLE 2 /* dtable */
 
 /* Bytes of a call's plan, and of the forward and the backward call's workspaces (all 256-byte aligned). Reads the sizes,
- * dtype, q_start, follow, radius, and whether there are ranges, a mask and a table. */
+ * dtype, q_start, follow, radius, and whether there are ranges, a mask, slopes and a table. */
 int sa_attn_scored_sizes(const sa_attn_scored* call, int64_t bytes[3]);
 
 /*
- * out and each row's log2-sum-exp2: +inf, and a row of zeros, for a row that sees no key. bf16 and fp16 (P as two terms
+ * out and each row's log2-sum-exp2 (with slopes of the distances from the row's position or, where no key lies there, from the
+ * nearest key's): +inf, and a row of zeros, for a row that sees no key. bf16 and fp16 (P as two terms
  * of the type) or fp32, D = 64 or 128. Rows, keys and values of 64 x 64 blocks that hold a pair that is seen (without a mask and
  * up to 256 rows and keys, of all) have to be finite, also where they are not seen (the backward call's dout, too). Fewer than 2^20 heads and 2^24 blocks of rows or keys, and less than 2 GiB from a head's first row to its last. Reads neither dout nor the gradients.
  */

@@ -198,11 +198,6 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
       sc = 1.f;
     }
     const int base = place - row0 - 4 * hh;  // d = base - c_e
-    if (a.slopes) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) S[e] = fmaf(S[e], sc, -slope * fabsf((float)(base - (8 * (e >> 2) + (e & 3)))));
-      sc = 1.f;
-    }
     if (a.table) {
       if (near - row0 - 31 >= a.radius) {
 #pragma unroll
@@ -211,6 +206,16 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 #pragma unroll
         for (int e = 0; e < 16; ++e) S[e] = fmaf(S[e], sc, bias_at(base - (8 * (e >> 2) + (e & 3))));
       }
+      sc = 1.f;
+    }
+    // Slopes: S becomes S - slope |d| - ref, with ref the row's offset, or what the step's middle key loses where that is less. It
+    // goes in before S does: of two large numbers that cancel no bits are lost.
+    float ref = 0.f;
+    if (a.slopes) {
+      ref = fmaxf(m, -slope * fabsf((float)(place - row0 - kStep / 2)));
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        S[e] = fmaf(S[e], sc, fmaf(-slope, fabsf((float)(base - (8 * (e >> 2) + (e & 3)))), -ref));
       sc = 1.f;
     }
     if (blind || row0 + 31 > near || row0 + 31 >= limit || (a.window && far - row0 >= a.window)) {
@@ -224,7 +229,7 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
     float top = S[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, S[e]);
-    top = xhalf_max(top) * sc;
+    top = xhalf_max(top) * sc + ref;
     if (__ballot(top > m + kAbove<T>)) {
       const float next_m = fmaxf(m, top - kBelow<T>);
       const float f = next_m == m ? 1.f : fast_exp2(m - next_m);
@@ -235,7 +240,7 @@ __global__ __launch_bounds__((64 * CachedShape<T, kD>::kWaves)) void cached_kern
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[dc][e] *= f;
     }
-    const float off = m == -INFINITY ? 0.f : m;
+    const float off = m == -INFINITY ? 0.f : m - ref;
     Weights<T> P;
 #pragma unroll
     for (int e = 0; e < 16; e += 2) P.set(e, fast_exp2(fmaf(S[e], sc, -off)), fast_exp2(fmaf(S[e + 1], sc, -off)));

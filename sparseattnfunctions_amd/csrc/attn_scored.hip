@@ -432,7 +432,7 @@ struct SidePlan {  // how a side's items are dealt out; byte offsets into a call
   int64_t units, n_units, splits, n_splits;
 };
 struct Plan {
-  int64_t bounds, ebias, kv_idx, kv_cnt, q_idx, q_cnt, bytes;
+  int64_t bounds, ebias, offsets, kv_idx, kv_cnt, q_idx, q_cnt, bytes;
   SidePlan side[2];  // queries, keys
 };
 
@@ -480,6 +480,7 @@ Plan plan_of(const sa_attn_scored& t) {
   Buffer buf;
   p.bounds = buf.take(t.ranges && nkb > kDirect ? t.B * nkb * 16 : 0);
   p.ebias = buf.take(t.table ? (int64_t)t.H * (2 * t.radius + 1 + 2 * kPad) * 4 : 0);
+  p.offsets = buf.take(t.slopes ? (int64_t)t.B * t.H * nqb * kBlk * 8 : 0);
   p.kv_idx = buf.take(lists * nqb * nkb * 4);
   p.kv_cnt = buf.take(lists * nqb * 4);
   p.q_idx = buf.take(keys ? lists * nqb * nkb * 4 : 0);
@@ -507,7 +508,7 @@ Work work_of(const sa_attn_scored& t, const Plan& p) {
   w.fwd_parts = fwd.take(q_places * sums);
   w.fwd_sums = fwd.take(q_places * kBlk * 8);
   w.fwd_bytes = fwd.at;
-  w.stats = bwd.take(rows * 512);
+  w.stats = bwd.take(rows * (t.slopes ? 1024 : 512));
   const bool table = t.follow & SA_SCORED_TABLE;
   const int64_t n_far = 4 * (2 * t.radius + 1);
   w.far = bwd.take(table ? rows * n_far : 0);
@@ -576,7 +577,7 @@ void launch_pass(int mode, ScoredArgs a, const sa_attn_scored& t, const SidePlan
     m.grad_a = a.grad_a; m.grad_b = a.grad_b; m.out_lo = a.out_lo;
     m.ga_sb = a.ga_sb; m.ga_sh = a.ga_sh; m.ga_sl = a.ga_sl;
     m.gb_sb = a.gb_sb; m.gb_sh = a.gb_sh; m.gb_sl = a.gb_sl;
-    m.sm_scale = a.sm_scale; m.lse = a.lse; m.far = a.far; m.n_far = 2 * a.radius + 1;
+    m.sm_scale = a.sm_scale; m.lse = a.lse; m.offsets = a.offsets; m.far = a.far; m.n_far = 2 * a.radius + 1;
   }
   const int cap = !(t.cap > 0) ? kNoCap : cap_of(t.sm_scale, t.cap, t.dtype).fine ? kFineTanh : kTanh;
   PassCall c = {mode, t.D, cap, 8u * (unsigned)(p.scheduled ? p.cap : xcd_items(a.BH_own, a.n_own)), 0, s};
@@ -591,7 +592,7 @@ Side side_of(const sa_attn_scored& t, const void* p, int i) {
   return Side{p, t.strides[3 * i], t.strides[3 * i + 1], t.strides[3 * i + 2]};
 }
 
-ScoredArgs common_args(const sa_attn_scored& t) {
+ScoredArgs common_args(const sa_attn_scored& t, const Plan& p) {
   ScoredArgs a{};
   a.H = t.H;
   a.rep = t.H / t.Hk;
@@ -610,6 +611,7 @@ ScoredArgs common_args(const sa_attn_scored& t) {
   a.radius = t.table ? t.radius : 0;
   a.per_head = t.mask != nullptr;
   a.lse = t.lse;
+  if (t.slopes) a.offsets = reinterpret_cast<float2*>(static_cast<uint8_t*>(t.plan) + p.offsets);
   a.out_lo = t.dtype == SA_DTYPE_F32 ? nullptr : t.out_lo;
   return a;
 }
@@ -742,7 +744,7 @@ extern "C" int sa_attn_scored_fwd(const sa_attn_scored* t, void* stream) {
     hipLaunchKernelGGL(scored_schedule_kernel, dim3(8 * n_sides), dim3(kPlanThreads), 0, s, g);
     if (int rc = sa::check_launch(fn)) return rc;
   }
-  ScoredArgs a = common_args(*t);
+  ScoredArgs a = common_args(*t, p);
   own_queries(a, *t, p);
   a.grad_a = t->out;
   a.ga_sb = t->strides[9]; a.ga_sh = t->strides[10]; a.ga_sl = t->strides[11];
@@ -767,7 +769,7 @@ extern "C" int sa_attn_scored_bwd(const sa_attn_scored* t, void* stream) {
   hipStream_t s = sa::as_stream(stream);
   uint8_t* ws = static_cast<uint8_t*>(t->workspace);
   const uint8_t* plan = static_cast<const uint8_t*>(t->plan);
-  ScoredArgs a = common_args(*t);
+  ScoredArgs a = common_args(*t, p);
   own_queries(a, *t, p);
   a.own_b = side_of(*t, t->dout, 4);
   a.out = side_of(*t, t->out, 3);

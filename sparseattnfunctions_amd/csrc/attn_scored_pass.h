@@ -32,7 +32,7 @@ namespace sa_scored {
 constexpr int kBlk = 64;
 constexpr int kCus = 256;
 enum { kForward = 0, kQueries = 1, kKeys = 2 };
-enum { kPlain = 0, kSlopes = 1, kTable = 2 };  // kTable: with or without slopes
+enum { kPlain = 0, kSlopes = 1, kTable = 2 };  // (both: 3)
 // How scores are capped (bend). A choice of kernels: with both ways in one, registers that fit are spilled (query pass with
 // slopes at head dim 64 20 bytes a lane, 36 so).
 enum { kNoCap = 0, kTanh = 1, kFineTanh = 2 };
@@ -70,7 +70,10 @@ struct ScoredArgs {
   const float* ebias;      // [H][2 radius + 1 + 2 kPad] biases of distances -radius - kPad .., times log2(e); may be null
   int radius;
   float* lse;              // [b * H + h][64 n]
-  float* stats;            // [b * H + h][2 n][2][32]: of 32 query rows their lse, then their delta
+  float2* offsets;         // with slopes: {offset, log2-sum-exp2 relative to it} of each row, laid out like lse; else null
+  // [b * H + h][2 n][2][32]: of 32 query rows their lse, then their delta. With slopes [4][32]: the relative one, delta, the
+  // offset, the position p.
+  float* stats;
   void* out_lo;            // what out's rounding left out, laid out like it; may be null
   // Units of work of each XCD, {item = (b * heads_own + head) * n_own + block, first entry, behind the last, place of the
   // sums}: units[xcd * unit_cap ..], n_units[xcd] of them (scored_schedule_kernel). Null: items as own_block has them.
@@ -83,27 +86,20 @@ struct ScoredArgs {
   float* part_far;   // and [place]
 };
 
-// The rule on a tile's products S: S times what is returned is the score times log2(e). base: the lane's distance at element
-// 0, from which element e is kSign (8 (e / 4) + e % 4) away. least .. least + 62: the wave's distances. window: where the
-// lane's biases lie in LDS, from element 0 (kSign > 0) or element 15 (kSign < 0) on. kSlope: slope becomes the cap's
-// derivative. side: whether all pairs of the wave are past the radius, 1 above, -1 below, 0 not all.
+// The rule on a tile's products S, but for the slopes: S times what is returned is the score times log2(e). least .. least + 62:
+// the wave's distances. window: where the lane's biases lie in LDS, from element 0 (kSign > 0) or element 15 (kSign < 0) on; element
+// e is kSign (8 (e / 4) + e % 4) away from element 0. kSlope: slope becomes the cap's derivative. side: whether all pairs of the
+// wave are past the radius, 1 above, -1 below, 0 not all.
 template <int kSign, int kCap, int kRule, bool kSlope, typename T>
-__device__ __forceinline__ float apply_rule(const ScoredArgs& a, float slope_h, float past, float before, int base, int least,
-                                            const float* window, sa_f32x16& S, sa_f32x16& slope, int& side) {
+__device__ __forceinline__ float apply_rule(const ScoredArgs& a, float past, float before, int least, const float* window,
+                                            sa_f32x16& S, sa_f32x16& slope, int& side) {
   float sc = a.scale_log2;
   if constexpr (kCap) {
     bend_all<kCap == kFineTanh || std::is_same<T, float>::value, kSlope>(a.cap_in, a.cap_log2, S, slope);
     sc = 1.f;
   }
-  if (kRule == kSlopes || (kRule == kTable && a.slopes)) {
-    // (slopes of either sign: |d| is an addition of its own, which takes 2 us of 207)
-    const float d0 = (float)base;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) S[e] = fmaf(S[e], sc, -slope_h * fabsf(d0 + (float)(kSign * (8 * (e >> 2) + (e & 3)))));
-    sc = 1.f;
-  }
   side = 0;
-  if constexpr (kRule == kTable) {
+  if constexpr (kRule & kTable) {
     side = least >= a.radius ? 1 : least + 62 <= -a.radius ? -1 : 0;
     if (side) {
       const float c = side > 0 ? past : before;
@@ -177,6 +173,13 @@ __device__ __forceinline__ void store_result(uint8_t* row, uint8_t* lo, int at, 
   }
 }
 
+// A row's log2-sum-exp2 (none: it sees no key), of sum l relative to offset m.
+__device__ __forceinline__ void store_sums(float* lse, float2* offsets, int64_t at, bool none, float m, float l) {
+  const float log = none ? INFINITY : __builtin_amdgcn_logf(l), off = none ? 0.f : m;
+  lse[at] = off + log;
+  if (offsets) offsets[at] = make_float2(off, log);
+}
+
 __device__ inline float wave_sum(float x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
@@ -188,8 +191,17 @@ constexpr int waves_per_simd() {
   return std::is_same<T, float>::value ? (kD == 64 ? 2 : 1) : kD == 64 ? 3 : 2;
 }
 
+// The forward pass with a bias would fit four waves a SIMD (125 registers), and is held to the three that a call's plan counts
+// with: [2, 30, 2560, 64] 219 us, 237 with four.
+template <int kMode, int kRule, typename T, int kD>
+constexpr int most_waves() {
+  return kMode == kForward && (kRule & kTable) ? waves_per_simd<T, kD>() : 8;
+}
+
 template <int kMode, int kCap, int kRule, typename T, int kD>
-__global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(ScoredArgs a) {
+__global__ __launch_bounds__(128)
+__attribute__((amdgpu_waves_per_eu((waves_per_simd<T, kD>()), (most_waves<kMode, kRule, T, kD>()))))
+void scored_kernel(ScoredArgs a) {
   constexpr bool kF32 = std::is_same<T, float>::value;
   constexpr int kSize = kF32 ? 4 : 2;
   constexpr int kDS = kD * kSize / 32;      // steps of the first products
@@ -205,8 +217,11 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
   constexpr int kRead = kF32 || kTight ? 2 : kMode == kKeys ? 1 : 4;
   constexpr bool kEarly = !kF32 && kMode != kKeys && !kTight;
   __shared__ __attribute__((aligned(1024))) uint8_t tile0[2 * kMat], tile1[2 * kMat];
-  __shared__ __attribute__((aligned(256))) float stat0[64], stat1[64];
-  __shared__ __attribute__((aligned(256))) float bias0[kRule == kTable ? kWindow : 1], bias1[kRule == kTable ? kWindow : 1];
+  constexpr bool kSloped = kRule & kSlopes, kBiased = kRule & kTable;
+  constexpr int kRowStats = kSloped ? 128 : 64;  // of 32 query rows
+  constexpr int kStat = kMode == kKeys ? kRowStats : 64;
+  __shared__ __attribute__((aligned(256))) float stat0[kStat], stat1[kStat];
+  __shared__ __attribute__((aligned(256))) float bias0[kBiased ? kWindow : 1], bias1[kBiased ? kWindow : 1];
   extern __shared__ float far_lds[];  // kQueries with far: [wave][8][64] for a quarter of a tile, [wave][2 radius + 1] sums
 
   const int lane = threadIdx.x & 63;
@@ -248,7 +263,8 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
     }
   }
 
-  float lse = 0.f, delta = 0.f;
+  // kQueries: of the row its log2-sum-exp2, with slopes relative to its offset; rowsum(do out).
+  float lse = 0.f, row_off = 0.f, delta = 0.f;
   if constexpr (kMode == kQueries) {
     const int64_t at_row = (int64_t)own_clamped * a.out.sl * kSize + 16 * hh;
     const uint8_t* po = at(a.out, b, head) + at_row;
@@ -259,12 +275,21 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
       if (!kF32 && a.out_lo) delta = dot_chunk<T>(*reinterpret_cast<const sa_u32x4v*>(pl + 32 * s), fb[s], delta);
     }
     delta = xhalf_sum(delta);
-    lse = a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col];
-    if (first_entry == 0)
-      a.stats[(((int64_t)bh * a.n_own + blk) * 2 + w) * 64 + lane] =
-          own_row < a.L_own ? (hh == 0 ? lse : delta) : hh == 0 ? INFINITY : 0.f;
+    const int64_t row = ((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col;
+    if constexpr (kSloped) {
+      const float2 x = a.offsets[row];
+      row_off = x.x;
+      lse = x.y;
+    } else {
+      lse = a.lse[row];
+    }
+    if (first_entry == 0) {
+      float* to = a.stats + (((int64_t)bh * a.n_own + blk) * 2 + w) * kRowStats + lane;
+      to[0] = own_row < a.L_own ? (hh == 0 ? lse : delta) : hh == 0 ? INFINITY : 0.f;
+      if constexpr (kSloped) to[64] = hh == 0 ? row_off : (float)min(max(own_row + a.q_start, 0), a.L_st - 1);
+    }
     if (!a.grad_a && !a.far) return;  // only the statistics are wanted
-    if (kRule == kTable && a.far) {
+    if (kBiased && a.far) {
       for (int i = threadIdx.x; i < 2 * (kDiagonals + 2 * a.radius + 1); i += 128) far_lds[i] = 0.f;
       __syncthreads();
     }
@@ -291,8 +316,8 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
   float slope_h = 0.f, past = 0.f, before = 0.f;
   auto set_list = [&]() __attribute__((always_inline)) {  // (at entry 0)
     const int hq = kMode == kKeys ? st_head + g : head;
-    if (kRule == kSlopes || (kRule == kTable && a.slopes)) slope_h = *(ConstPtr)(a.slopes + hq);
-    if (kRule == kTable) {
+    if (kSloped) slope_h = *(ConstPtr)(a.slopes + hq);
+    if (kBiased) {
       const float* eb = a.ebias + (int64_t)hq * (2 * a.radius + 1 + 2 * kPad) + kPad;
       before = *(ConstPtr)eb;
       past = *(ConstPtr)(eb + 2 * a.radius);
@@ -368,17 +393,18 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
       }
     }
     if (kMode == kKeys && w == 0) {
-      const float* src = a.stats + ((int64_t)(b * a.H + st_head + s.g) * a.n_st * 2 + 2 * s.block + s.half) * 64;
+      const float* src = a.stats + ((int64_t)(b * a.H + st_head + s.g) * a.n_st * 2 + 2 * s.block + s.half) * kRowStats;
       const __amdgpu_buffer_rsrc_t rs =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(src), (short)0, 256, 0x00020000);
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(src), (short)0, 4 * kRowStats, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, stat, 4, 4 * lane, 0, 0, 0);
+      if (kSloped) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, stat, 4, 4 * lane, 0, 256, 0);
     }
     if (kMode != kKeys && w == 0 && a.ranges && s.cut) {  // the keys' intervals
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<int2*>(a.ranges + b * a.ranges_sb + row0), (short)0, 8 * max(a.L_st - (int)row0, 0), 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, stat, 4, 4 * lane, 0, 0, 0);
     }
-    if (kRule == kTable && w == 1) {  // (where neither wave's pairs are all past the radius they are in bounds)
+    if (kBiased && w == 1) {  // (where neither wave's pairs are all past the radius they are in bounds)
       const int least = least_of((int)row0), n = 2 * a.radius + 1 + 2 * kPad;
       const int hq = kMode == kKeys ? st_head + s.g : head;
       if (least < a.radius && least + 94 > -a.radius) {
@@ -442,16 +468,42 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
     }
     // Elements e: streamed row row0 + 4 hh + 8 (e / 4) + e % 4 of own row own_row.
     const int first = __builtin_amdgcn_readfirstlane(blk * kBlk + kStep * w);
-    const int base = kMode == kKeys ? row0 + 4 * hh + a.q_start - own_row : own_row + a.q_start - row0 - 4 * hh;
     const int least = kMode == kKeys ? row0 + a.q_start - first - 31 : first + a.q_start - row0 - 31;
     int side_far;
     const int own = kStep * w + col;
     // With nothing but a cap the key pass takes its derivative from the score where that is used up: 16 registers less, which
     // were spilled (428 us at head dim 128, 401 so; the query pass has them, and takes 2 % longer so).
     constexpr bool kFromScore = kMode == kKeys && kCap && kRule == kPlain && !kF32;
-    const float sc = apply_rule<kMode == kKeys ? 1 : -1, kCap, kRule, kMode != kForward && !kFromScore, T>(
-        a, s.slope, s.past, s.before, base, least, bias + (kMode == kKeys ? 4 * hh + 63 - own : own + 4 - 4 * hh), S, slope,
-        side_far);
+    float sc = apply_rule<kMode == kKeys ? 1 : -1, kCap, kRule, kMode != kForward && !kFromScore, T>(
+        a, s.past, s.before, least, bias + (kMode == kKeys ? 4 * hh + 63 - own : own + 4 - 4 * hh), S, slope, side_far);
+    // Slopes: with the query's position p taken as the nearest of the keys' positions (which leaves out what all of a row's
+    // distances have in common), S becomes S - slope |p - j| - ref. ref is close to what the row's nearer keys lose: the row's
+    // offset, or where the forward pass has yet to find one as large, what this step's middle key loses. It goes in before S does:
+    // of two large numbers that cancel no bits are lost (a row that sees nothing but keys 1e5 away: P off by 4e-3 of itself
+    // where it went in last). (Slopes of either sign: |d| is an addition of its own, which takes 2 us of 207.)
+    float ref = row_off;
+    if constexpr (kSloped) {
+      if constexpr (kMode == kKeys) {
+        const float* offs = stat + 64 + 4 * hh;
+        const float key = (float)own_row;
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const float4 y = *reinterpret_cast<const float4*>(offs + 8 * q4), z = *reinterpret_cast<const float4*>(offs + 32 + 8 * q4);
+          const float off[4] = {y.x, y.y, y.z, y.w}, p[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            S[4 * q4 + i] = fmaf(S[4 * q4 + i], sc, fmaf(-s.slope, fabsf(p[i] - key), -off[i]));
+        }
+      } else {
+        const int p = min(max(own_row + a.q_start, 0), a.L_st - 1) - row0;
+        const float d0 = (float)(p - 4 * hh);
+        if constexpr (kMode == kForward) ref = fmaxf(m, -s.slope * fabsf((float)(p - kStep / 2)));
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          S[e] = fmaf(S[e], sc, fmaf(-s.slope, fabsf(d0 - (float)(8 * (e >> 2) + (e & 3))), -ref));
+      }
+      sc = 1.f;
+    }
     if (s.cut) {
       if constexpr (kMode == kKeys) {
         if (a.ranges) {
@@ -469,6 +521,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, S[e]);
       top = xhalf_max(top) * sc;
+      if constexpr (kSloped) top += ref;
       if (__ballot(top > m + kAbove<T>)) {
         const float next_m = fmaxf(m, top - kBelow<T>);
         const float f = next_m == m ? 1.f : fast_exp2(m - next_m);
@@ -479,7 +532,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[0][dc][e] *= f;
       }
-      const float off = m == -INFINITY ? 0.f : m;
+      const float off = m == -INFINITY ? 0.f : kSloped ? m - ref : m;
       Weights<T> P, rest;
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
@@ -520,7 +573,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
           }
         }
       }
-      if constexpr (kMode == kQueries && kRule == kTable) {
+      if constexpr (kMode == kQueries && kBiased) {
         if (a.far) {
           if (side_far) {
             float t = 0.f;
@@ -592,7 +645,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
 
   // ---- Results: element 4 q4 + j of acc[x][dc] is d = 32 dc + 8 q4 + 4 hh + j of own row own_row.
   if constexpr (kMode == kForward) l = xhalf_sum(l);
-  if constexpr (kMode == kQueries && kRule == kTable) {
+  if constexpr (kMode == kQueries && kBiased) {
     if (a.far) {
       far_hi = wave_sum(far_hi);
       far_lo = wave_sum(far_lo);
@@ -629,8 +682,7 @@ __global__ __launch_bounds__(128, (waves_per_simd<T, kD>())) void scored_kernel(
   if constexpr (kMode == kForward) {
     f_a = l == 0.f ? 0.f : 1.f / l;
     if (hh == 0)
-      a.lse[((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col] =
-          own_row >= a.L_own || l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+      store_sums(a.lse, a.offsets, ((int64_t)bh * a.n_own + blk) * kBlk + kStep * w + col, own_row >= a.L_own || l == 0.f, m, l);
   }
 #pragma unroll
   for (int x = 0; x < kAcc; ++x) {
@@ -662,6 +714,7 @@ struct MergeArgs {
   int64_t ga_sb, ga_sh, ga_sl, gb_sb, gb_sh, gb_sl;
   float sm_scale;
   float *lse, *far;
+  float2* offsets;
 };
 
 constexpr int kMergeThreads = 1024;  // (a unit's sums are a load of each thread's: latency)
@@ -706,7 +759,7 @@ __global__ __launch_bounds__(kMergeThreads) void scored_merge_kernel(MergeArgs a
     if constexpr (kMode == kForward) {
       f = l == 0.f ? 0.f : 1.f / l;
       if (ch == 0)
-        a.lse[(int64_t)u.x * kBlk + r] = row >= a.L_own || l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
+        store_sums(a.lse, a.offsets, (int64_t)u.x * kBlk + r, row >= a.L_own || l == 0.f, top, l);
     }
     uint8_t* grad = static_cast<uint8_t*>(x == 0 ? a.grad_a : a.grad_b);
     if (!grad || row >= a.L_own) continue;
@@ -727,7 +780,7 @@ struct PassCall {
 
 template <int kMode, int kCap, int kRule, typename T, int kD>
 void launch_kernels(const ScoredArgs& a, const MergeArgs& m, const PassCall& c) {
-  const size_t lds = kMode == kQueries && kRule == kTable && a.far ? 2 * (kDiagonals + 2 * a.radius + 1) * sizeof(float) : 0;
+  const size_t lds = kMode == kQueries && (kRule & kTable) && a.far ? 2 * (kDiagonals + 2 * a.radius + 1) * sizeof(float) : 0;
   hipLaunchKernelGGL((scored_kernel<kMode, kCap, kRule, T, kD>), dim3(c.grid), dim3(128), lds, c.stream, a);
   if (c.merge_grid)
     hipLaunchKernelGGL((scored_merge_kernel<kMode, T, kD>), dim3(c.merge_grid), dim3(kMergeThreads), 0, c.stream, m);
@@ -742,7 +795,8 @@ void launch_pass_of(const ScoredArgs& a, const MergeArgs& m, const PassCall& c) 
     else launch_kernels<kMode, kCap, kRule, T, 128>(a, m, c);
   };
   auto rule = [&](auto mode, auto cap) {
-    if (a.ebias) dim(mode, cap, std::integral_constant<int, kTable>());
+    if (a.ebias && a.slopes) dim(mode, cap, std::integral_constant<int, kTable | kSlopes>());
+    else if (a.ebias) dim(mode, cap, std::integral_constant<int, kTable>());
     else if (a.slopes) dim(mode, cap, std::integral_constant<int, kSlopes>());
     else dim(mode, cap, std::integral_constant<int, kPlain>());
   };

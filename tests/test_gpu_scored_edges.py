@@ -154,3 +154,80 @@ def test_caches_are_not_differentiated(dev):
         with torch.no_grad():
             assert not call().requires_grad
         t.requires_grad_(False)
+
+
+def shifted(monkeypatch, shift):
+    """The reference with `shift` taken from each row's distances (which changes no probability) before the slopes: what the
+    errors are relative to."""
+    plain = ref.scores
+
+    def scores(q, k, scale, far, cap=None, slopes=None, table=None, buckets=None):
+        s, c, e, e_c, place = plain(q, k, scale, far, cap, None, table, buckets)
+        add = slopes.double().cpu()[:, None, None] * (far.abs() - shift).double()
+        return s - add, c, e + 2.0 ** -22 * (s.abs() + add.abs()), e_c, place
+
+    monkeypatch.setattr(ref, "scores", scores)
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=str)
+@pytest.mark.parametrize("kind", ["", "cap", "table"])
+@pytest.mark.parametrize("where", ["behind", "ahead", "far behind", "far ahead", "across", "first keys"])
+def test_slopes_of_distant_keys(dev, monkeypatch, where, kind, dtype):
+    case(f"rows that see distant keys: {where} {kind} {dtype}")
+    H, Lq, Lk, D, keys = 3, 70, 200, 64, 200
+    start = {"behind": 100_000, "ahead": -100_000, "far behind": 2 ** 29 - 100, "far ahead": 100 - 2 ** 29, "across": 165,
+             "first keys": 19_950}[where]
+    if where == "first keys":
+        Lq, Lk, D, keys = 40, 20_000, 128, 150
+    q, k, v, do = ref.inputs(17, 1, H, 1, Lq, Lk, D, dtype, dev)
+    slopes = torch.tensor([0.5, 0.02, -0.25], device=dev)
+    ranges = torch.zeros(Lk, 2, dtype=torch.int32, device=dev)
+    ranges[:keys, 1] = Lq
+    place = torch.arange(Lq)[:, None] + start
+    near, last = (place - place.clamp(0, keys - 1)).abs(), torch.maximum(place.abs(), (place - keys + 1).abs())
+    shifted(monkeypatch, torch.stack([near, near, last]))  # (the row's heaviest keys: with a negative slope the far ones)
+    opts = dict(slopes=slopes, ranges=ranges, q_start=start)
+    wanted = [q, k, v]
+    if kind == "cap":
+        opts["cap"] = 5.0
+    if kind == "table":
+        opts["buckets"] = distance_buckets(32, 128, device=dev)
+        opts["table"] = torch.randn(32, H, generator=torch.Generator().manual_seed(2)).to(dev)
+        wanted.append(opts["table"])
+    for t in wanted:
+        t.requires_grad_()
+    want = ref.train(q, k, v, do, 0.2, **opts)
+    out = scored_attention(q, k, v, 0.2, **opts)
+    for n, x in zip(NAMES, (out, *torch.autograd.grad(out, wanted, do))):
+        ref.check(n, x, want[n])
+
+
+def test_slopes_of_distant_keys_in_split_lists(dev, monkeypatch):
+    case("rows that see distant keys, a document's lists split")
+    H, L, start = 2, 2000, 300_000
+    q, k, v, do = ref.inputs(18, 1, H, 1, L, L, 64, FP32, dev)
+    slopes = torch.tensor([0.5, -0.01], device=dev)
+    place = torch.arange(L)[:, None] + start
+    shifted(monkeypatch, torch.stack([place - L + 1, place]))
+    for t in (q, k, v):
+        t.requires_grad_()
+    want = ref.train(q, k, v, do, 0.2, slopes=slopes, q_start=start)
+    out = scored_attention(q, k, v, 0.2, slopes=slopes, q_start=start)
+    for n, x in zip(NAMES, (out, *torch.autograd.grad(out, (q, k, v), do))):
+        ref.check(n, x, want[n])
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=str)
+@pytest.mark.parametrize("Lp", [0, 100, 12_000])
+def test_slopes_of_distant_keys_over_caches(dev, monkeypatch, Lp, dtype):
+    case(f"the first keys of a long cache weigh most, a prefix of {Lp}, {dtype}")
+    B, H, L = 2, 2, 20_000 if Lp == 0 else 500
+    g = torch.Generator().manual_seed(19)
+    q, k, v = (torch.randn(B, h, n, 64, generator=g).to(dtype).to(dev) for h, n in ((H, 2), (1, L), (1, L)))
+    prefix = tuple(torch.randn(1, Lp, 64, generator=g).to(dtype).to(dev) for _ in range(2)) if Lp else None
+    n = torch.tensor([L, L - 77], dtype=torch.int32, device=dev)
+    slopes = torch.tensor([-0.5, -0.25], device=dev)
+    shift = (Lp + n.cpu().long()[:, None] - 2 + torch.arange(2))[:, None, :, None]  # the distance of the first key
+    shifted(monkeypatch, shift)
+    ref.check("out", cached_attention(q, k, v, n, 0.2, slopes=slopes, prefix=prefix),
+              ref.serve(q, k, v, n, 0.2, slopes=slopes, prefix=prefix))
