@@ -27,7 +27,8 @@ using namespace sa_scored;
 // ---- What a call's passes read besides its operands.
 
 // {smallest from, largest until} of the keys of a block that have rows, {largest from, smallest until} of all (a key without
-// rows: 0). Key blocks whose bounds say that a query block sees none of them are left out.
+// rows: 0; -1 in the last place: there are rows between the first two that see none of the keys). Key blocks whose bounds say
+// that a query block sees none of them are left out.
 __device__ inline int4 key_bounds(int2 x) {
   x.x = max(x.x, 0);
   return x.y > x.x ? make_int4(x.x, x.y, x.x, x.y) : make_int4(INT_MAX, 0, INT_MAX, 0);
@@ -37,13 +38,35 @@ __device__ inline int4 join_bounds(int4 a, int4 b) {
 }
 __device__ inline int4 no_bounds() { return make_int4(INT_MAX, 0, 0, INT_MAX); }
 
-// Of the block that the wave's lanes have a key of each.
+// Of the block that the wave's lanes have a key of each. Its rows have no gap where each interval that ends before the last one
+// does ends within another, mostly the first of those that end last.
 __device__ inline int4 wave_bounds(const int2* ranges, int first, int Lk, int lane) {
   int4 r = first + lane < Lk ? key_bounds(ranges[first + lane]) : no_bounds();
+  const int from = r.x, until = r.y;  // (of a key without rows: none, 0)
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1)
     r = join_bounds(r, make_int4(__shfl_xor(r.x, o), __shfl_xor(r.y, o), __shfl_xor(r.z, o), __shfl_xor(r.w, o)));
+  const int last = __ffsll((unsigned long long)__ballot(until == r.y)) - 1;
+  const int from_last = __shfl(from, last);
+  bool open = until > 0 && until < r.y && from_last > until;
+  if (__ballot(open)) {
+    for (int i = 0; i < 64; ++i) {
+      const int a = __shfl(from, i), z = __shfl(until, i);  // (of all lanes: no short cut)
+      open &= a > until || z <= until;
+    }
+    if (__ballot(open)) r.w = -1;
+  }
   return r;
+}
+
+// Whether one of the rows r0 .. r1 - 1 sees one of a block's keys.
+__device__ inline bool some_seen(const int2* ranges, int first, int Lk, int r0, int r1) {
+  bool some = false;
+  for (int j = first; j < min(first + kBlk, Lk); ++j) {
+    const int4 x = key_bounds(ranges[j]);
+    some = some || (x.x < r1 && x.y > r0);
+  }
+  return some;
 }
 
 __global__ __launch_bounds__(256) void scored_bounds_kernel(const int2* ranges, int64_t ranges_sb, int64_t n, int Lk, int nkb,
@@ -104,14 +127,20 @@ __global__ __launch_bounds__(256) void scored_lists_kernel(ListArgs a) {
     bool any = n < n_st, whole = (kb + 1) * kBlk <= a.Lk;
     if (any && ranges) {
       const int r0 = qb * kBlk, r1 = min(r0 + kBlk, a.Lq);
+      bool some = false;
       if (bounds) {
         x = bounds[kb];
       } else if (!keys) {
         x = no_bounds();
 #pragma unroll 8
-        for (int j = kb * kBlk; j < min((kb + 1) * kBlk, a.Lk); ++j) x = join_bounds(x, key_bounds(ranges[j]));
+        for (int j = kb * kBlk; j < min((kb + 1) * kBlk, a.Lk); ++j) {
+          const int4 y = key_bounds(ranges[j]);
+          some = some || (y.x < r1 && y.y > r0);
+          x = join_bounds(x, y);
+        }
       }
-      any = x.x < r1 && x.y > r0;
+      any = !bounds && !keys ? some : x.x < r1 && x.y > r0;
+      if (any && x.w < 0) any = some_seen(ranges, kb * kBlk, a.Lk, r0, r1);
       whole = whole && x.z <= r0 && x.w >= r1;
     }
     if (any && mask) any = mask[(int64_t)qb * a.s2 + (int64_t)kb * a.s3] != 0;

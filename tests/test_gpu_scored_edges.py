@@ -231,3 +231,37 @@ def test_slopes_of_distant_keys_over_caches(dev, monkeypatch, Lp, dtype):
     shifted(monkeypatch, shift)
     ref.check("out", cached_attention(q, k, v, n, 0.2, slopes=slopes, prefix=prefix),
               ref.serve(q, k, v, n, 0.2, slopes=slopes, prefix=prefix))
+
+
+@pytest.mark.parametrize("L", [768, 4000])  # bounds of key blocks taken where they are needed, and once for all
+@pytest.mark.parametrize("kind", ["two", "three", "scattered"])
+def test_ranges_with_gaps(dev, kind, L):
+    """Keys of one block that rows far apart see, and rows between them that may hold anything."""
+    case(f"ranges with gaps {kind} {L}")
+    ranges = torch.zeros(L, 2, dtype=torch.int32)
+    at = torch.arange(L)
+    last = L // 64 * 64 - 64
+    ranges[at % 2 == 0, 1] = 50
+    ranges[at % 2 == 1] = torch.tensor([last, last + 40], dtype=torch.int32)
+    if kind == "three":  # a bridge between two of them, and a key without rows
+        ranges[at % 64 == 7] = torch.tensor([45, 64 * 5], dtype=torch.int32)
+        ranges[at % 64 == 8] = torch.tensor([9, 9], dtype=torch.int32)
+        ranges[at % 64 == 9] = torch.tensor([64 * 5, 64 * 6], dtype=torch.int32)
+    if kind == "scattered":
+        g = torch.Generator().manual_seed(3)
+        begin = torch.randint(0, L // 64, (L,), generator=g) * 64
+        ranges = torch.stack([begin, (begin + 3).clamp(max=L)], 1).int()
+        ranges[(at // 64 > 1) | (at % 31 > 0)] = 0
+    q, k, v, do = ref.inputs(20, 1, 2, 2, L, L, 64, FP32, dev)
+    want = ref.train(q, k, v, do, 0.2, ranges=ranges)
+    sees = torch.zeros(L // 64 + 2, dtype=torch.bool)  # blocks of rows
+    for a, z in ranges.unique(dim=0).tolist():
+        sees[a // 64:(z + 63) // 64 if z > a else 0] = True
+    assert 2 <= sees.sum() < L // 64 - 1
+    blind = (~sees[at // 64]).to(dev)
+    q, do = q.masked_fill(blind[:, None], float("nan")), do.masked_fill(blind[:, None], float("inf"))
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = scored_attention(q, k, v, 0.2, ranges=ranges.to(dev))
+    for n, x in zip(NAMES, (out, *torch.autograd.grad(out, (q, k, v), do))):
+        ref.check(n, x, want[n])
