@@ -387,7 +387,7 @@ struct CachedPlan {
 int plan_cached(const sa_attn_cached& t, const char* fn, CachedPlan& p) {
   const int64_t per = (int64_t)(t.H / t.Hk) * t.Ln;
   const int64_t tiles = (per + kStep - 1) / kStep, prefix_tiles = t.Lp ? (t.B * per + kStep - 1) / kStep : 0;
-  const int64_t items = t.B * t.Hk * tiles, prefix_items = t.Hk * prefix_tiles;
+  const int64_t items = (int64_t)t.B * t.Hk * tiles, prefix_items = t.Hk * prefix_tiles;
   if (t.B * per >= 1LL << 30 || items + prefix_items >= 1LL << 20)
     return sa::fail(SA_ERR_UNSUPPORTED, "%s: too many rows", fn);
   // Splits in proportion to the keys, so that workgroups have alike many of them, about `target` in all.

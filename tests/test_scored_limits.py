@@ -24,3 +24,12 @@ def test_caps_in_range(over):
     lib = _lib.load()
     assert lib.sa_attn_scored_sizes(scored(**over), (ctypes.c_int64 * 3)()) == 0
     assert lib.sa_attn_cached_workspace(cached(**over), ctypes.byref(ctypes.c_int64())) == 0
+
+
+@pytest.mark.parametrize("over", [dict(B=1 << 16, H=1 << 16, Hk=1 << 16, Ln=1), dict(B=1 << 15, H=1 << 17, Hk=1 << 17, Ln=1, Lp=0)],
+                         ids=str)
+def test_many_sequences_and_key_heads(over):
+    lib = _lib.load()
+    n = ctypes.c_int64()
+    assert lib.sa_attn_cached_workspace(cached(**over), ctypes.byref(n)) == _lib.SA_ERR_UNSUPPORTED
+    assert lib.sa_attn_cached_fwd(cached(**over), None) == _lib.SA_ERR_UNSUPPORTED
