@@ -431,5 +431,12 @@ def scored_attention(q, k, v, sm_scale: float, *, cap: Optional[float] = None, s
         of_keys, of_table = k.requires_grad or v.requires_grad, table is not None and table.requires_grad
         if q.requires_grad or of_keys or of_table:
             follow = (_KEYS if of_keys else 0) | (_TABLE if of_table else 0)
+            # (what a validation pass made in inference mode could not be saved)
+            if slopes is not None and slopes.is_inference():
+                slopes = slopes.clone()
+            if buckets is not None and buckets.is_inference():
+                buckets = buckets.clone()
+            if ranges is not None and ranges.is_inference():
+                ranges = ranges.clone()
     return _ScoredAttention.apply(q, k, v, table, float(sm_scale), cap, slopes, buckets, ranges, block_mask, int(q_start),
                                   follow)

@@ -265,3 +265,44 @@ def test_ranges_with_gaps(dev, kind, L):
     out = scored_attention(q, k, v, 0.2, ranges=ranges.to(dev))
     for n, x in zip(NAMES, (out, *torch.autograd.grad(out, (q, k, v), do))):
         ref.check(n, x, want[n])
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16], ids=str)
+def test_most_distances_at_the_larger_head_dim(dev, dtype):
+    case(f"1024 distances told apart on each side, head dim 128, {dtype}")
+    q, k, v, do = ref.inputs(21, 1, 2, 1, 400, 1300, 128, dtype, dev)
+    table = torch.randn(40, 2, generator=torch.Generator().manual_seed(4)).to(dev)
+    buckets = distance_buckets(40, 1024, device=dev)
+    for t in (q, k, v, table):
+        t.requires_grad_()
+    opts = dict(table=table, buckets=buckets, q_start=500, cap=20.0)
+    want = ref.train(q, k, v, do, 0.1, **opts)
+    out = scored_attention(q, k, v, 0.1, **opts)
+    for n, x in zip(NAMES, (out, *torch.autograd.grad(out, (q, k, v, table), do))):
+        ref.check(n, x, want[n])
+
+
+def test_inference_mode(dev):
+    case("calls in inference mode, and tensors made in it")
+    q, k, v, do = ref.inputs(22, 2, 2, 2, 300, 300, 64, BF16, dev)
+    lengths = torch.tensor([[200, 50], [300, 0]], device=dev)
+    n = torch.tensor([300, 7], dtype=torch.int32, device=dev)
+    table = torch.randn(9, 2, device=dev)
+    buckets = distance_buckets(9, 7, device=dev)
+    opts = dict(table=table, buckets=buckets)
+    want = scored_attention(q, k, v, 0.2, ranges=row_ranges(lengths, 300), **opts)
+    served = cached_attention(q[:, :, :2], k, v, n, 0.2, **opts)
+    table.requires_grad_()
+    with torch.inference_mode():
+        opts["buckets"] = distance_buckets(9, 7, device=dev)
+        ranges = row_ranges(lengths, 300)
+        assert torch.equal(scored_attention(q, k, v, 0.2, ranges=ranges, **opts), want)
+        assert torch.equal(cached_attention(q[:, :, :2], k, v, n, 0.2, **opts), served)
+    # and in training, what was made there
+    q.requires_grad_()
+    for made in (opts["buckets"], ranges):
+        assert made.is_inference()
+    grads = torch.autograd.grad(scored_attention(q, k, v, 0.2, ranges=ranges, **opts), (q, table), do)
+    opts["buckets"] = distance_buckets(9, 7, device=dev)
+    for a, b in zip(grads, torch.autograd.grad(scored_attention(q, k, v, 0.2, ranges=row_ranges(lengths, 300), **opts), (q, table), do)):
+        assert torch.equal(a, b)
