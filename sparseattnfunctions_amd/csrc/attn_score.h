@@ -105,8 +105,10 @@ __device__ __forceinline__ void set_two_terms(Weights<T>& hi, Weights<T>& lo, in
 // cap tanh(y) and 1 - tanh(y)^2, in one of two ways. Fine: below 0.6 the odd polynomial through tanh(y) / y at Chebyshev nodes
 // (relative error 7e-8), because a small score would otherwise lose its bits. Else cap - 2 cap / (exp2(y') + 1), whose error is
 // absolute, 2e-7 cap; y' = 2 log2(e) y is the argument. fp32 calls are fine, 16-bit ones where the cap is above kFineCap, whose
-// 2e-7 is a tenth of fp16's rounding of P (at a cap of 1e4 scores were off by 0.002, at 1e7 by 1.7).
-constexpr float kFineCap = 256.f;
+// 2e-7 is a tenth of fp16's rounding of P (at a cap of 1e4 scores were off by 0.002, at 1e7 by 1.7). The derivative 4 (r - r^2)
+// of r = 1 / (exp2(y') + 1) keeps its bits above 0; towards minus the cap, where r is close to 1, it is off by 2^-22.
+constexpr float kFineCap = 256.f, kLeastCap = 1e-12f;  // (below that fine, too: what the key pass hides pairs by counts in caps)
+__device__ inline float bend_r(float y) { return __builtin_amdgcn_rcpf(fast_exp2(y) + 1.f); }
 template <bool kFine, bool kSlope>
 __device__ inline float bend(float y, float cap, float& slope) {
   if constexpr (kFine) {
@@ -122,7 +124,7 @@ __device__ inline float bend(float y, float cap, float& slope) {
     if constexpr (kSlope) slope = fabsf(y) < 0.6f ? fmaf(-t, t, 1.f) : 4.f * fmaf(-r, r, r);
     return t * cap;
   } else {
-    const float r = __builtin_amdgcn_rcpf(fast_exp2(y) + 1.f);
+    const float r = bend_r(y);
     if constexpr (kSlope) slope = 4.f * fmaf(-r, r, r);
     return fmaf(r, -2.f * cap, cap);
   }
@@ -147,7 +149,7 @@ struct Cap {
 inline Cap cap_of(float sm_scale, float cap, int dtype) {
   Cap c{};
   if (!(cap > 0)) return c;
-  c.fine = dtype == SA_DTYPE_F32 || cap > kFineCap;
+  c.fine = dtype == SA_DTYPE_F32 || cap > kFineCap || cap < kLeastCap;
   c.in = sm_scale / cap * (c.fine ? 1.f : 2.f * kLog2e);
   c.log2 = cap * kLog2e;
   return c;

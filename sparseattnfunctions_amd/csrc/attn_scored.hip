@@ -634,7 +634,6 @@ ScoredArgs common_args(const sa_attn_scored& t, const Plan& p) {
     const Cap c = cap_of(t.sm_scale, t.cap, t.dtype);
     a.cap_in = c.in;
     a.cap_log2 = c.log2;
-    a.cap_out = 1.f / c.log2;
   }
   a.slopes = t.slopes;
   a.radius = t.table ? t.radius : 0;

@@ -65,7 +65,7 @@ struct ScoredArgs {
   const int2* ranges;  // [b * ranges_sb + key] = {from, until}; may be null
   int64_t ranges_sb;
   float sm_scale, scale_log2;
-  float cap_in, cap_log2, cap_out;  // 2 log2(e) sm_scale / cap (fine: sm_scale / cap), cap log2(e), 1 / cap_log2
+  float cap_in, cap_log2;  // 2 log2(e) sm_scale / cap (fine: sm_scale / cap), cap log2(e)
   const float* slopes;     // [H]; may be null
   const float* ebias;      // [H][2 radius + 1 + 2 kPad] biases of distances -radius - kPad .., times log2(e); may be null
   int radius;
@@ -471,11 +471,18 @@ void scored_kernel(ScoredArgs a) {
     const int least = kMode == kKeys ? row0 + a.q_start - first - 31 : first + a.q_start - row0 - 31;
     int side_far;
     const int own = kStep * w + col;
-    // With nothing but a cap the key pass takes its derivative from the score where that is used up: 16 registers less, which
-    // were spilled (428 us at head dim 128, 401 so; the query pass has them, and takes 2 % longer so).
-    constexpr bool kFromScore = kMode == kKeys && kCap && kRule == kPlain && !kF32;
-    float sc = apply_rule<kMode == kKeys ? 1 : -1, kCap, kRule, kMode != kForward && !kFromScore, T>(
-        a, s.past, s.before, least, bias + (kMode == kKeys ? 4 * hh + 63 - own : own + 4 - 4 * hh), S, slope, side_far);
+    // With nothing but a cap the key pass keeps the reciprocals r of bend in S: the score is cap - 2 cap r, its derivative 4 (r - r^2).
+    // That takes 16 registers less than both, which were spilled (428 us at head dim 128, 401 so).
+    constexpr bool kHoldsR = kMode == kKeys && kCap == kTanh && kRule == kPlain && !kF32;
+    constexpr float kHidden = kHoldsR ? 1e18f : -INFINITY;  // of pairs that are not seen (2e18 of the least cap, and P is 0)
+    float sc = 1.f;
+    if constexpr (kHoldsR) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) S[e] = bend_r(S[e] * a.cap_in);
+    } else {
+      sc = apply_rule<kMode == kKeys ? 1 : -1, kCap, kRule, kMode != kForward, T>(
+          a, s.past, s.before, least, bias + (kMode == kKeys ? 4 * hh + 63 - own : own + 4 - 4 * hh), S, slope, side_far);
+    }
     // Slopes: with the query's position p taken as the nearest of the keys' positions (which leaves out what all of a row's
     // distances have in common), S becomes S - slope |p - j| - ref. ref is close to what the row's nearer keys lose: the row's
     // offset, or where the forward pass has yet to find one as large, what this step's middle key loses. It goes in before S does:
@@ -510,7 +517,7 @@ void scored_kernel(ScoredArgs a) {
           const int t = row0 + 4 * hh - from;
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if ((unsigned)(t + 8 * (e >> 2) + (e & 3)) >= (unsigned)len) S[e] = -INFINITY;
+            if ((unsigned)(t + 8 * (e >> 2) + (e & 3)) >= (unsigned)len) S[e] = kHidden;
         }
       } else {
         cut_keys(a, a.L_st, own_row, row0 + 4 * hh, lane, (const lds_u8*)stat, S);
@@ -557,6 +564,10 @@ void scored_kernel(ScoredArgs a) {
       for (int e = 0; e < 16; e += 4) {
         float4 off = make_float4(lse, lse, lse, lse);
         if constexpr (kMode == kKeys) off = *reinterpret_cast<const float4*>(stat + 2 * e + 4 * hh);
+        if constexpr (kHoldsR) {
+          off.x -= a.cap_log2; off.y -= a.cap_log2; off.z -= a.cap_log2; off.w -= a.cap_log2;
+          sc = -2.f * a.cap_log2;
+        }
         const float p[4] = {fast_exp2(fmaf(S[e], sc, -off.x)), fast_exp2(fmaf(S[e + 1], sc, -off.y)),
                             fast_exp2(fmaf(S[e + 2], sc, -off.z)), fast_exp2(fmaf(S[e + 3], sc, -off.w))};
         if constexpr (kMode == kKeys) {
@@ -567,10 +578,7 @@ void scored_kernel(ScoredArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           dP[e + i] *= p[i];
-          if constexpr (kFromScore) {  // (clamped: pairs that are not seen have -inf, and P 0)
-            const float t = S[e + i] * a.cap_out;
-            dP[e + i] *= __builtin_amdgcn_fmed3f(fmaf(-t, t, 1.f), 0.f, 1.f);
-          }
+          if constexpr (kHoldsR) dP[e + i] *= 4.f * fmaf(-S[e + i], S[e + i], S[e + i]);
         }
       }
       if constexpr (kMode == kQueries && kBiased) {
@@ -604,7 +612,7 @@ void scored_kernel(ScoredArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        if constexpr (kCap && !kFromScore) dC.set(e, dP[e] * slope[e], dP[e + 1] * slope[e + 1]);
+        if constexpr (kCap && !kHoldsR) dC.set(e, dP[e] * slope[e], dP[e + 1] * slope[e + 1]);
         else dC.set(e, dP[e], dP[e + 1]);
       }
       if constexpr (kF32) {

@@ -306,3 +306,40 @@ def test_inference_mode(dev):
     opts["buckets"] = distance_buckets(9, 7, device=dev)
     for a, b in zip(grads, torch.autograd.grad(scored_attention(q, k, v, 0.2, ranges=row_ranges(lengths, 300), **opts), (q, table), do)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["", "slopes"])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=str)
+def test_gradients_of_saturated_caps(dev, monkeypatch, dtype, kind, D):
+    """Scores of six to eleven caps, all of one sign: what is left of the cap's derivative has its bits."""
+    case(f"saturated caps {dtype} {kind} {D}")
+    plain = ref.scores
+
+    def scores(q, k, scale, far, cap=None, slopes=None, table=None, buckets=None):
+        # r = 1 / (exp2(y') + 1), y' up to 32: the argument's rounding 2^-24 |y'| log(2), exp2's, the sum's and the reciprocal's
+        # 2^-22, and 4 (r - r^2) with it: 2^-19 of itself in all, besides twice the score's error over the cap
+        s, c, e, _, place = plain(q, k, scale, far, cap, slopes, table, buckets)
+        product = plain(q, k, scale, far, None, slopes, table, buckets)[2]
+        return s, c, e, c * (2.0 ** -19 + 2 * product / cap), place
+
+    monkeypatch.setattr(ref, "scores", scores)
+    q, k, v, do = ref.inputs(23, 1, 2, 1, 200, 330, D, dtype, dev)
+    q[..., 0], k[..., 0] = 8, 8  # scores of 43 +- 4 at a cap of 5
+    q[..., 1:] *= 0.7 * (64 / D) ** 0.5
+    k[..., 1:] *= 0.7
+    scale = 43.0 / 64
+    q[..., 1:] /= 8 * scale
+    do = do * 2.0 ** 12  # (fp16: dS of 1e-7 and less times this; with 2^14 some were infinite)
+    assert torch.isfinite(do).all()
+    s = scale * (q.double() @ k.double().transpose(2, 3).repeat_interleave(2, 1))
+    assert 30 < s.min() and s.max() < 55
+    opts = dict(cap=5.0, q_start=130, ranges=row_ranges(torch.tensor([330], device=dev), 330))
+    if kind == "slopes":
+        opts["slopes"] = torch.tensor([0.02, -0.01], device=dev)
+    for t in (q, k, v):
+        t.requires_grad_()
+    want = ref.train(q, k, v, do, scale, **opts)
+    out = scored_attention(q, k, v, scale, **opts)
+    for n, x in zip(NAMES, (out, *torch.autograd.grad(out, (q, k, v), do))):
+        ref.check(n, x, want[n])
