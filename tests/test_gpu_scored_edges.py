@@ -343,3 +343,19 @@ def test_gradients_of_saturated_caps(dev, monkeypatch, dtype, kind, D):
     out = scored_attention(q, k, v, scale, **opts)
     for n, x in zip(NAMES, (out, *torch.autograd.grad(out, (q, k, v), do))):
         ref.check(n, x, want[n])
+
+
+@pytest.mark.parametrize("cap", [1e-2, 2e-12, 1e-13, 1e-25])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=str)
+def test_small_caps(dev, dtype, cap):
+    case(f"cap {cap} {dtype}")
+    q, k, v, do = ref.inputs(24, 1, 2, 1, 150, 330, 64, dtype, dev)
+    opts = dict(cap=cap, ranges=row_ranges(torch.tensor([100, 180], device=dev), 330))
+    for t in (q, k, v):
+        t.requires_grad_()
+    want = ref.train(q, k, v, do, 0.3, **opts)
+    out = scored_attention(q, k, v, 0.3, **opts)
+    for n, x in zip(NAMES, (out, *torch.autograd.grad(out, (q, k, v), do))):
+        ref.check(n, x, want[n])
+    n = torch.tensor([330], dtype=torch.int32, device=dev)
+    ref.check("served", cached_attention(q.detach()[:, :, :3], k, v, n, 0.3, cap=cap), ref.serve(q[:, :, :3], k, v, n, 0.3, cap=cap))
