@@ -127,20 +127,16 @@ __global__ __launch_bounds__(256) void scored_lists_kernel(ListArgs a) {
     bool any = n < n_st, whole = (kb + 1) * kBlk <= a.Lk;
     if (any && ranges) {
       const int r0 = qb * kBlk, r1 = min(r0 + kBlk, a.Lq);
-      bool some = false;
       if (bounds) {
         x = bounds[kb];
       } else if (!keys) {
         x = no_bounds();
 #pragma unroll 8
-        for (int j = kb * kBlk; j < min((kb + 1) * kBlk, a.Lk); ++j) {
-          const int4 y = key_bounds(ranges[j]);
-          some = some || (y.x < r1 && y.y > r0);
-          x = join_bounds(x, y);
-        }
+        for (int j = kb * kBlk; j < min((kb + 1) * kBlk, a.Lk); ++j) x = join_bounds(x, key_bounds(ranges[j]));
       }
-      any = !bounds && !keys ? some : x.x < r1 && x.y > r0;
-      if (any && x.w < 0) any = some_seen(ranges, kb * kBlk, a.Lk, r0, r1);
+      any = x.x < r1 && x.y > r0;
+      // (intervals that all share a row have no gap; of the others the wave's or the call's bounds say so)
+      if (any && (x.w < 0 || (!bounds && !keys && x.z > x.w))) any = some_seen(ranges, kb * kBlk, a.Lk, r0, r1);
       whole = whole && x.z <= r0 && x.w >= r1;
     }
     if (any && mask) any = mask[(int64_t)qb * a.s2 + (int64_t)kb * a.s3] != 0;
