@@ -361,7 +361,8 @@ int sa_attn_scored_bwd(const sa_attn_scored* call, void* stream);
 
 /*
  * Attention of Ln new tokens of each sequence over its cached keys and values, with sa_attn_scored's rule of scores, and over
- * a prefix of Lp tokens that all sequences begin with, whose keys and values are held (and read) once.
+ * a prefix of Lp tokens that all sequences begin with, whose keys and values are held once. Keys are read once for each 32
+ * rows (new tokens of the query heads of a key head; of the prefix, those of all sequences).
  * Sequence b has lengths[b] cached tokens (clamped to [0, L]), the last Ln of them the new ones; new token i is its
  * token t = lengths[b] - Ln + i, at distance d = t - j from its key j and Lp + t - j from the prefix's. It sees keys at
  * d >= 0, with window > 0 at d < window; where t < 0 none, and its output is zeros. Cached rows that no new token of the

@@ -5,16 +5,18 @@
 // New token i is the sequence's own token t = lengths[b] - Ln + i, at distance d = t - j from own key j and d = Lp + t - j
 // from prefix key j; it sees keys at 0 <= d (< window, if there is one), and none where t < 0.
 //
-// A call reads every cached key and value once, and that is its bound (one new token: 2 operations a byte in 16 bits, against
-// the card's 300), so the work is dealt out by keys: a sequence's and key head's rows (its query heads' new tokens) share one
-// read of the keys as the columns of a 32-wide matrix product, and the keys are split over workgroups and their waves.
-// The prefix's keys are read once for the rows of all sequences, 32 rows a workgroup. Each wave copies its steps of 32
+// Reading the cached keys and values is a call's bound (one new token: 2 operations a byte in 16 bits, against the card's 300), so
+// the work is dealt out by keys: a sequence's and key head's rows (its query heads' new tokens) share a read of the keys, 32
+// rows as the columns of a matrix product, and the keys are split over workgroups and their waves. Every 32 rows read the keys
+// again, so that many new tokens (a chunk of a prompt) cost as many reads. The prefix's keys are read once for each 32 rows of
+// all sequences together; a short prefix by each sequence, ahead of its own keys. Each wave copies its steps of 32
 // keys into LDS stages of its own, with no barrier between steps; a workgroup's waves join their sums in LDS, and
 // cached_merge_kernel joins the workgroups', in order: results do not depend on the order in which they run.
 //
-// Measured (kernel and merge): 8 sequences of 8888 to 17776 keys, 30 heads of 64, bf16: 163 + 5 us, 5.5 TB/s; 4 of 22552 to
-// 45104 keys, 8 heads of 128 read by 48, 4 tokens each, fp16: 118 + 5 us, 5.4 TB/s (a large copy: 4.7); one of 263 to 526 keys,
-// 30 heads of 64: 9.0 us in one launch, of which the first loads from HBM and cold code are most.
+// Measured (kernel and merge): 8 sequences of 8888 to 17776 keys, 30 heads of 64, bf16: 162 to 169 + 5 us, 5.5 TB/s; 4 of 22552 to
+// 45104 keys, 8 heads of 128 read by 48, 4 tokens each, fp16: 118 to 124 + 5 us, 5.4 TB/s (a large copy: 4.7); one of 263 to 526
+// keys, 30 heads of 64: 9.0 us in one launch, of which the first loads from HBM and cold code are most. In fp32 at head dim 128 a
+// workgroup has two waves for the LDS of a CU (128 KB): half of its SIMDs work.
 #include <math.h>
 
 #include <algorithm>

@@ -12,11 +12,14 @@
 //
 // Bound: the matrix instructions and the vector ones beside them, at the clock that the power limit leaves. An element
 // of a tile takes 3 D (forward: 2 D, and D for P's second term), 3 D and 4 D products, and an exp2, a scaling, a sum, a
-// rounding or two: at [1, 15, 17776, 64] by frames of 1350 the matrix units are busy for 50, 58 and 57 % of the
-// three passes' cycles and vector instructions issue in 77, 52 and 51 %, at 1.5 GHz; LDS has no bank conflicts.
-// Measured, us of forward, query and key pass (TFLOP/s of the products done): 1130, 975, 1320 (865, 1000, 990) there;
-// [1, 16, 4096, 128] fp16, every pair, 229, 229, 335 (900, 900, 820), with a cap 278, 300, 401 (its tanh is an exp2, a
-// reciprocal and three more an element); [2, 30, 2560, 64] with a bias 225, 240, 258 (670, 630, 780).
+// rounding or two: at [1, 15, 17776, 64] by frames of 1350 the matrix units are busy for 51, 57 and 57 % of the
+// three passes' cycles and vector instructions issue in 77, 51 and 50 %, at 1.8 GHz; LDS has no bank conflicts. Shorter or
+// capped calls have neither unit busy (25 to 40 %, 30 to 58 %): with two or three waves a SIMD each step waits for its copies, a
+// barrier and the chains of its products. The query and key passes spill registers where there is a cap besides slopes or a
+// bias, the key pass at head dim 128 always (8 to 48 of them).
+// Measured, us of forward, query and key pass (TFLOP/s of the products done), of 50 passes without a pause: 1010, 930, 1225
+// (970, 1050, 1065) there; seven documents in a row of [1, 15 of 5 key heads, 8229, 128] fp16 with a cap 123, 132, 175 (its tanh is
+// an exp2, a reciprocal and three more an element); [2, 30, 2560, 64] with a bias 193, 205, 222 (780, 740, 910).
 // Tiles of 32 own rows a wave: 64 would halve the LDS reads, which are not the bound, for twice the registers.
 #pragma once
 

@@ -6,8 +6,9 @@ has no cache.
 Sequence b has lengths[b] cached tokens, the last Ln of them the new ones (their keys and values are
 written into the cache before the call); a shared prefix of Lp tokens lies before them. New token i is its
 sequence's token t = lengths[b] - Ln + i and sees the keys up to itself: the prefix's, at the distance
-d = Lp + t - j, and its own, at d = t - j; with a window those at d < window. Scores are those of
-`scored_attention` at these distances.
+d = Lp + t - j, and its own, at d = t - j; with a window those at d < window (of the prefix too, which a
+window of `row_ranges` leaves alone). Scores are those of `scored_attention` at these distances. The new
+tokens of one call are causal among themselves: there are no frames, nor a block mask.
 
 The lengths stay on the device: a call reads none of them on the host, and its launches depend on the
 shapes alone, so that a captured call serves sequences as they grow.
@@ -93,12 +94,13 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
 
     prefix: (k, v) of the shared prefix, each [Hk,Lp,D] or [1,Hk,Lp,D]. The caches and the prefix may have
     any strides with a contiguous last axis and 16-byte aligned rows; they are not copied. Cached rows that no
-    new token sees, from lengths[b] on or before a window, are not used, whatever they hold. A new token before its sequence's first (lengths[b] <
-    Ln) sees nothing: zeros. cap, slopes, table and buckets as in `scored_attention`; window: see above
-    (0: none)."""
+    new token sees, from lengths[b] on or before a window, are not used, whatever they hold. A new token before
+    its sequence's first (lengths[b] < Ln) sees nothing: zeros. cap, slopes, table and buckets as in
+    `scored_attention`; window: see above (0: none). The keys are read again for every 32 rows of a key head
+    (its query heads times Ln): it is a call for single tokens and a few."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or slopes is not None and slopes.requires_grad or table is not None and table.requires_grad
-                                    or prefix is not None and any(t.requires_grad for t in prefix)):
+                                    or prefix is not None and (prefix[0].requires_grad or prefix[1].requires_grad)):
         with torch.no_grad():
             out = cached_attention(q, k, v, lengths, sm_scale, cap=cap, slopes=slopes, table=table, buckets=buckets,
                                    window=window, prefix=prefix)

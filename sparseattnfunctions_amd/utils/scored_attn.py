@@ -19,7 +19,7 @@ and row i sees key j where ranges[b, j, 0] <= i < ranges[b, j, 1] and block_mask
 A row that sees no key has a zero output and zero gradients, a key that no row sees zero gradients.
 
 The backward pass recomputes the probabilities block by block (`sa_attn_scored_bwd`); between the two a
-call holds q, k, v, out, a float per row and its lists of blocks (eight bytes for each pair of 64-token
+call holds q, k, v, out, a float per row (three with slopes) and its lists of blocks (eight bytes for each pair of 64-token
 blocks of a sequence, with a block mask of a head). Blocks of which no pair is seen are not read. Gradients
 of a 16-bit call round P and dS to its type; sums are fp32 in a fixed order, so that a step repeats bit
 for bit. In fp16, dS has the range of the type: scale the loss as usual.
@@ -51,8 +51,9 @@ def distance_buckets(n_buckets: int, radius: int, bidirectional: bool = True, de
     """Buckets int32 [2 radius + 1] of the distances -radius .. radius (i - j: positive for keys before the
     row) for `scored_attention`'s table; distances past the radius share the last one's.
 
-    Of the buckets of a side (all of them unless bidirectional; then keys behind the row have bucket 0)
-    the first half hold one distance each, the others grow in proportion to it, up to the radius."""
+    Of the buckets of a side (unless bidirectional there is one, and keys behind the row have bucket 0)
+    the first half hold one distance each, the others grow in proportion to it, up to the radius. Bidirectional,
+    bucket 0 is distance 0 and each side has (n_buckets - 1) // 2: the last one of an even number is not used."""
     n_buckets, radius = int(n_buckets), int(radius)
     if not 0 <= radius <= MOST_RADIUS:
         raise ValueError(f"radius {radius} (0 to {MOST_RADIUS})")
