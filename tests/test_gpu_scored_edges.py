@@ -359,3 +359,36 @@ def test_small_caps(dev, dtype, cap):
         ref.check(n, x, want[n])
     n = torch.tensor([330], dtype=torch.int32, device=dev)
     ref.check("served", cached_attention(q.detach()[:, :, :3], k, v, n, 0.3, cap=cap), ref.serve(q[:, :, :3], k, v, n, 0.3, cap=cap))
+
+
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16], ids=str)
+@pytest.mark.parametrize("cap", [None, 5.0, 1e4])
+def test_a_bias_that_hides_beside_slopes(dev, dtype, cap):
+    case(f"a bias of -inf beside slopes, cap {cap}, {dtype}")
+    q, k, v, do = ref.inputs(25, 1, 2, 2, 300, 300, 64, dtype, dev)
+    slopes = torch.tensor([0.5, -0.02], device=dev)
+    for t in (q, k, v):
+        t.requires_grad_()
+    buckets = distance_buckets(5, 2, device=dev)  # -2 and less, -1, 0, 1, 2 and more: 4, 3, 0, 1, 2
+    table = torch.zeros(5, 2, device=dev)
+    hiding = table.clone()
+    hiding[3:] = float("-inf")  # keys behind the row
+    opts = dict(cap=cap, slopes=slopes, buckets=buckets)
+    want = ref.train(q, k, v, do, 0.2, table=table, ranges=row_ranges(torch.tensor([300], device=dev), 300), **opts)
+    hiding.requires_grad_()
+    out = scored_attention(q, k, v, 0.2, table=hiding, **opts)
+    for n, x in zip(NAMES, (out, *torch.autograd.grad(out, (q, k, v, hiding), do))):
+        ref.check(n, x, want[n])
+    # all keys: rows of zeros, and no gradients
+    nothing = torch.full_like(table, float("-inf")).requires_grad_()
+    out = scored_attention(q, k, v, 0.2, table=nothing, **opts)
+    assert not out.any()
+    for x in torch.autograd.grad(out, (q, k, v, nothing), do):
+        assert not x.any()
+    # over caches, keys two and more away
+    far = torch.zeros(5, 2, device=dev)
+    far[2] = float("-inf")
+    n = torch.tensor([300], dtype=torch.int32, device=dev)
+    want = ref.serve(q[:, :, :2], k, v, n, 0.2, cap=cap, slopes=slopes, window=2)
+    ref.check("served", cached_attention(q.detach()[:, :, :2], k.detach(), v.detach(), n, 0.2, table=far, **opts), want)
+    assert not cached_attention(q.detach()[:, :, :2], k.detach(), v.detach(), n, 0.2, table=nothing.detach(), **opts).any()
